@@ -2,7 +2,8 @@
 
 The library holds the C++ front end (IR, scheduler, rangeify, autograd),
 the gfx950 lowering/codegen and the HIP runtime behind the C-ABI declared in
-`include/`. Generated kernels are compiled at run time by hiprtc for gfx950.
+`include/`. Generated kernels are compiled at run time by hiprtc for gfx950,
+hand-written ones (`csrc/kernels/`) here.
 
 Usage: python -m ferrograd_amd.build  (or `build()` from __graft_entry__).
 """
@@ -20,7 +21,10 @@ OBJ = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libferrograd_amd.so")
 
 SOURCES = ["ir.cpp", "device.cpp", "schedule.cpp", "tensor.cpp", "gpu_lower.cpp", "hip_device.cpp",
-           "hip_runtime.cpp", "kernel_text.cpp", "hip_kernel.cpp", "dataset.cpp", "capi.cpp"]
+           "hip_runtime.cpp", "kernel_text.cpp", "hip_kernel.cpp", "dataset.cpp", "operators.cpp", "capi.cpp"]
+# Hand-written kernels (csrc/kernels/*.hip): device code objects, linked into
+# the library as data.
+KERNELS = ["attention", "dropout", "norm_rotate"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 CXXFLAGS = ["-O2", "-g0", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function",
@@ -28,6 +32,10 @@ CXXFLAGS = ["-O2", "-g0", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function"
             "-I" + os.path.join(ROOT, "include"), "-I" + CSRC]
 LDFLAGS = ["-shared", "-L/opt/rocm/lib", "-lhiprtc", "-lamdhip64", "-lhsa-runtime64", "-ldl",
            "-Wl,-rpath,/opt/rocm/lib"]
+
+
+KERNELFLAGS = ["-O3", "-std=c++17", "--offload-arch=gfx950", "--offload-device-only", "--no-gpu-bundle-output",
+               "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-I" + os.path.join(CSRC, "kernels")]
 
 
 def _run(cmd: list[str]) -> None:
@@ -61,8 +69,21 @@ def build(jobs: int = 8) -> str:
         _run([HIPCC, *CXXFLAGS, "-c", os.path.join(CSRC, src), "-o", obj])
         return obj
 
+    def compile_kernel(name: str) -> str:
+        """kernels/<name>.hip as an object file holding its gfx950 code object
+        between fg_image_<name> and fg_image_<name>_end."""
+        code, asm, obj = (os.path.join(OBJ, name + ext) for ext in (".hsaco", "_image.s", "_image.o"))
+        _run([HIPCC, *KERNELFLAGS, "-c", os.path.join(CSRC, "kernels", name + ".hip"), "-o", code])
+        with open(asm, "w") as f:
+            f.write(f'.section .rodata\n.global fg_image_{name}, fg_image_{name}_end\n.balign 4096\n'
+                    f'fg_image_{name}:\n.incbin "{code}"\nfg_image_{name}_end:\n.byte 0\n'
+                    '.section .note.GNU-stack,"",@progbits\n')
+        _run(["gcc", "-c", asm, "-o", obj])
+        return obj
+
     with ThreadPoolExecutor(max_workers=jobs) as ex:
-        objs = list(ex.map(compile_one, SOURCES))
+        images = ex.map(compile_kernel, KERNELS)
+        objs = list(ex.map(compile_one, SOURCES)) + list(images)
     tmp = LIB + ".tmp"
     _run([HIPCC, *objs, "-o", tmp, *LDFLAGS])
     os.replace(tmp, LIB)

@@ -8,6 +8,7 @@
 
 #include "gpu_lower.hpp"
 #include "kernel_text.hpp"
+#include "operators.hpp"
 #include "schedule.hpp"
 #include "tensor.hpp"
 
@@ -194,6 +195,27 @@ int fg_tensor_narrow(fg_tensor* t, int64_t dim, int64_t start, int64_t len, fg_t
     FG_CHECK(dim >= 0 && start >= 0 && len >= 0, "narrow: negative argument");
     *out = wrap(t->t.narrow(static_cast<size_t>(dim), static_cast<size_t>(start), static_cast<size_t>(len)));
   });
+}
+
+int fg_tensor_attention(fg_tensor* q, fg_tensor* k, fg_tensor* v, fg_tensor* lengths, int64_t batch, int64_t heads,
+                        int64_t kv_heads, int causal, double scale, fg_tensor** out) {
+  return guard([&] {
+    FG_CHECK(batch >= 1 && heads >= 1 && kv_heads >= 1, "attention: batch, heads and kv_heads must be at least 1");
+    *out = wrap(q->t.attention(k->t, v->t, lengths ? &lengths->t : nullptr, static_cast<size_t>(batch),
+                               static_cast<size_t>(heads), static_cast<size_t>(kv_heads), causal != 0, scale));
+  });
+}
+
+int fg_tensor_norm_rotate(fg_tensor* x, fg_tensor* weight, fg_tensor* positions, int64_t heads, double eps, double base,
+                          fg_tensor** out) {
+  return guard([&] {
+    FG_CHECK(heads >= 1, "norm_rotate: heads must be at least 1");
+    *out = wrap(x->t.norm_rotate(weight->t, positions->t, static_cast<size_t>(heads), eps, base));
+  });
+}
+
+int fg_tensor_dropout(fg_tensor* t, double p, uint64_t seed, uint64_t offset, fg_tensor** out) {
+  return guard([&] { *out = wrap(t->t.dropout(p, seed, offset)); });
 }
 
 int fg_tensor_log_softmax(fg_tensor* t, int64_t axis, fg_tensor** out) {
@@ -513,7 +535,21 @@ int fg_debug_plan(fg_tensor** roots, int n, int fuse, int render, char* buf, siz
           }
         }
         os << "]";
-        if (render) {
+        if (render && (it.kernel || it.storage_only)) {
+          // A hand-written kernel's call, or the storage of one of its outputs.
+          fg::RenderedKernel rk;
+          if (it.kernel) rk = fg::render_hip_call(it.kernel);
+          os << ", \"class\": \"" << (it.kernel ? rk.kind : "storage") << "\", \"workspace\": " << rk.workspace_bytes
+             << ", \"launches\": [";
+          for (size_t j = 0; j < rk.launches.size(); j++)
+            os << (j ? ", " : "") << "{\"name\": \"" << rk.launches[j].func << "\", \"grid\": " << rk.launches[j].grid[0]
+               << ", \"block\": " << rk.launches[j].block[0] << ", \"lds\": " << rk.launches[j].lds_bytes << "}";
+          os << "]";
+          is_block.push_back(false);
+          nargs.push_back(it.inputs.size() + 1);
+          binfo.emplace_back();
+          rks.push_back(std::move(rk));
+        } else if (render) {
           fg::UOp rangeified = fg::rangeify(it.sink);
           os << ", \"kernel\": \"" << json_escape(fg::kernel_to_text(rangeified)) << "\"";
           fg::UOp k = fg::with_all_params(fg::gpu_optimize(rangeified), it.sink);

@@ -61,6 +61,21 @@ struct LaunchSpec {
   unsigned lds_bytes = 0;
 };
 
+// One argument of a hand-written kernel's launches, in the order of its
+// signature: a parameter slot of the call (a buffer, or a scalar that changes
+// from call to call), a number fixed by the call's shapes, a null pointer (an
+// absent input), or the device's workspace.
+struct CallArg {
+  enum class Kind : uint8_t { Slot, I32, F32, Null, Workspace } kind = Kind::Null;
+  int32_t i = 0;  // the slot, or the number
+  float f = 0.f;
+  static CallArg slot(int32_t s) { CallArg a; a.kind = Kind::Slot; a.i = s; return a; }
+  static CallArg i32(int64_t v) { CallArg a; a.kind = Kind::I32; a.i = static_cast<int32_t>(v); return a; }
+  static CallArg f32(float v) { CallArg a; a.kind = Kind::F32; a.f = v; return a; }
+  static CallArg null() { return CallArg(); }
+  static CallArg workspace() { CallArg a; a.kind = Kind::Workspace; return a; }
+};
+
 // What a renderer hands to `Device::compile`: the source and everything the
 // launch needs that the reference's `compile(source, name, num_args)` lacks.
 struct RenderedKernel {
@@ -80,6 +95,16 @@ struct RenderedKernel {
   // launch (partial results between passes; nothing needs zeroing).
   std::vector<LaunchSpec> launches;
   size_t scratch_bytes = 0;
+  // Hand-written kernels (operators.hpp): `launches` name functions of a code
+  // object linked into the library (`image`), each called with `call_args`;
+  // nothing is rendered or compiled. `workspace_bytes` of the device's workspace hold
+  // what the launches of one call hand on to each other. `side_outputs`:
+  // parameter slots written besides out_slot.
+  std::vector<CallArg> call_args;
+  const void* image = nullptr;
+  size_t image_size = 0;
+  size_t workspace_bytes = 0;
+  std::vector<int> side_outputs;
   // Block kernels (one workgroup): the device function the kernel calls, its
   // parameter types in slot order, and its source, so a device can run a run
   // of them as one launch (render_block_batch).
@@ -149,6 +174,12 @@ class Device {
     return optimized;
   }
   virtual RenderedKernel render(const UOp& optimized, const std::string& name) = 0;
+  // The launches of a call of a hand-written kernel (an Op::Kernel over
+  // numbered parameters).
+  virtual RenderedKernel render_call(const UOp& call) {
+    (void)call;
+    fail("the device has no hand-written kernels");
+  }
   virtual std::shared_ptr<Program> compile(const RenderedKernel& rk, size_t num_args) = 0;
   virtual void execute(Program& p, std::vector<KernelArg>& args) = 0;
   // Run a recorded sequence of launches (a replayed realisation plan) in

@@ -1,6 +1,7 @@
 // The HIP device: implements the Device interface (src/device.rs:275-332) on
 // top of the C-ABI in include/ferrograd_hip.h, with the gfx950 lowering in
 // gpu_lower.cpp as its optimize/render stages.
+#include <algorithm>
 #include <cstdlib>
 #include <cstring>
 #include <map>
@@ -10,6 +11,7 @@
 #include "device.hpp"
 #include "hip_internal.hpp"
 #include "gpu_lower.hpp"
+#include "operators.hpp"
 #include "tensor.hpp"
 
 namespace fg {
@@ -137,8 +139,25 @@ class HipDevice : public Device {
     return render_hip_stable(optimized);
   }
 
+  RenderedKernel render_call(const UOp& call) override { return render_hip_call(call); }
+
   std::shared_ptr<Program> compile(const RenderedKernel& rk, size_t num_args) override {
     auto p = std::make_shared<HipProgram>();
+    if (!rk.call_args.empty()) {
+      // A hand-written kernel: functions of the library's own code object.
+      FG_CHECK(rk.params.size() == num_args, "the call has " + std::to_string(rk.params.size()) +
+                                                 " parameters but is launched with " + std::to_string(num_args));
+      for (const LaunchSpec& l : rk.launches) {
+        fg_prog* q = nullptr;
+        check(fg_hip_builtin_function(ctx(), rk.image, rk.image_size, l.func.c_str(),
+                                      static_cast<int>(rk.call_args.size()), &q),
+              "loading a built-in kernel failed");
+        p->passes.push_back(q);
+      }
+      p->num_args = num_args;
+      p->meta = rk;
+      return p;
+    }
     FG_CHECK(rk.params.size() == num_args || rk.params.empty(),
              "kernel declares " + std::to_string(rk.params.size()) + " parameters but is launched with " +
                  std::to_string(num_args));
@@ -173,6 +192,7 @@ class HipDevice : public Device {
   std::vector<fg_arg> marshal(HipProgram& p, std::vector<KernelArg>& args) {
     FG_CHECK(args.size() == p.num_args,
              "expected " + std::to_string(p.num_args) + " kernel args, got " + std::to_string(args.size()));
+    if (!p.meta.call_args.empty()) return marshal_call(p, args);
     std::vector<fg_arg> a(args.size());
     for (size_t i = 0; i < args.size(); i++) {
       std::memset(&a[i], 0, sizeof(fg_arg));
@@ -196,6 +216,55 @@ class HipDevice : public Device {
       a.push_back(s);
     }
     return a;
+  }
+
+  // The launch arguments of a hand-written kernel, in its signature's order.
+  std::vector<fg_arg> marshal_call(HipProgram& p, std::vector<KernelArg>& args) {
+    std::vector<fg_arg> a;
+    a.reserve(p.meta.call_args.size());
+    for (const CallArg& ca : p.meta.call_args) {
+      fg_arg x;
+      std::memset(&x, 0, sizeof(x));
+      switch (ca.kind) {
+        case CallArg::Kind::Slot: {
+          const KernelArg& k = args.at(static_cast<size_t>(ca.i));
+          if (k.kind == KernelArg::Kind::I32) {
+            x.kind = FG_ARG_I32;
+            x.v.i = k.i;
+            break;
+          }
+          FG_CHECK(k.kind == KernelArg::Kind::Buffer && k.buffer->device == DeviceId::Hip && k.buffer->realized,
+                   "HIP backend received unrealized or non-HIP buffer");
+          x.kind = FG_ARG_PTR;
+          x.v.p = k.buffer->storage;
+          break;
+        }
+        case CallArg::Kind::I32: x.kind = FG_ARG_I32; x.v.i = ca.i; break;
+        case CallArg::Kind::F32: x.kind = FG_ARG_F32; x.v.f = ca.f; break;
+        case CallArg::Kind::Null: x.kind = FG_ARG_PTR; break;
+        case CallArg::Kind::Workspace: x.kind = FG_ARG_PTR; x.v.p = workspace(p.meta.workspace_bytes); break;
+      }
+      a.push_back(x);
+    }
+    return a;
+  }
+
+  // One block of device memory that the calls of hand-written kernels share:
+  // what a call's launches hand on to each other. Every launch is ordered on
+  // the context's stream (or its own queue, which the stream waits for), so
+  // one call's launches are over before the next one's write it, and a block
+  // that is too small goes back to the allocator, which reuses it in stream
+  // order. A sequence's arguments are marshalled at every launch, so a
+  // recorded graph never keeps an old address.
+  void* workspace(size_t nbytes) {
+    if (nbytes > workspace_bytes_) {
+      if (workspace_) check(fg_hip_free(ctx(), workspace_), "fg_hip_free (workspace)");
+      workspace_ = nullptr;
+      workspace_bytes_ = 0;
+      check(fg_hip_alloc(ctx(), nbytes, 0, &workspace_), "fg_hip_alloc (workspace)");
+      workspace_bytes_ = nbytes;
+    }
+    return workspace_;
   }
 
   void execute(Program& prog, std::vector<KernelArg>& args) override {  // cpu.rs:328-380
@@ -656,7 +725,9 @@ class HipDevice : public Device {
       for (size_t j = 0; j < args[i].size(); j++) {
         if (args[i][j].kind != KernelArg::Kind::Buffer || !args[i][j].buffer->realized) continue;
         void* ptr = args[i][j].buffer->storage;
-        const bool out = j < m.params.size() && m.params[j].first == m.out_slot;
+        const bool out = j < m.params.size() &&
+                         (m.params[j].first == m.out_slot ||
+                          std::find(m.side_outputs.begin(), m.side_outputs.end(), m.params[j].first) != m.side_outputs.end());
         (out ? writes : reads)[i].insert(ptr);
         if (out) reads[i].insert(ptr);  // an in-place update also reads its destination
       }
@@ -811,6 +882,8 @@ class HipDevice : public Device {
   fg_ctx* ctx_ = nullptr;
   bool aql_on_ = false, aql_failed_ = false;
   size_t read_bytes_[FG_READ_SLOTS] = {};
+  void* workspace_ = nullptr;
+  size_t workspace_bytes_ = 0;
   std::shared_ptr<Program> readback_;
 };
 

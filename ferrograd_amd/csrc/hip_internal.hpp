@@ -7,6 +7,9 @@
 extern "C" {
 // Sets fg_hip_last_error() and returns `code`.
 int fg_hip_set_error(int code, const char* msg);
+// Function `func` of a code object in memory (the hand-written kernels, linked
+// into the library), loaded once per context and device.
+int fg_hip_builtin_function(fg_ctx* c, const void* image, size_t size, const char* func, int num_args, fg_prog** out);
 // The device ordinal a context was created on.
 int fg_hip_context_device(const fg_ctx* c);
 // fg_hip_launch without launch profiling: one hipModuleLaunchKernel, nothing

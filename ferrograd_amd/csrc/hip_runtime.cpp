@@ -184,6 +184,8 @@ struct fg_ctx {
   // loading the code object again.
   std::unordered_map<std::string, std::shared_ptr<ModuleRef>> loaded;
   std::deque<std::string> loaded_order;
+  // The hand-written kernels' code objects in use, by their image's address.
+  std::unordered_map<const void*, std::shared_ptr<ModuleRef>> builtin;
   hipEvent_t events[64] = {};
   // Caching allocator: exact-size free lists. Blocks are only reused by work
   // queued later on the same stream, so reuse needs no synchronisation.
@@ -423,6 +425,7 @@ int fg_hip_destroy(fg_ctx* c) {
   }
   (void)hipStreamSynchronize(c->stream);
   c->loaded.clear();  // modules no program holds are unloaded here
+  c->builtin.clear();
   fg_hip_trim(c);
   for (auto& ev : c->events) (void)hipEventDestroy(ev);
   (void)hipEventDestroy(c->staging_event);
@@ -775,6 +778,26 @@ int fg_hip_compile(fg_ctx* c, const char* source, const char* func, int num_args
     c->loaded_order.pop_front();
   }
   *out = p;
+  return FG_OK;
+}
+
+int fg_hip_builtin_function(fg_ctx* c, const void* image, size_t size, const char* func, int num_args, fg_prog** out) {
+  if (!c || !image || !func || !out) return set_err(FG_ERR_INVALID, "fg_hip_builtin_function: null argument");
+  std::shared_ptr<ModuleRef>& module = c->builtin[image];
+  if (!module) {
+    auto m = std::make_shared<ModuleRef>();
+    HIP_TRY(hipModuleLoadData(&m->module, image));
+    m->code.assign(static_cast<const char*>(image), static_cast<const char*>(image) + size);
+    module = m;
+  }
+  auto p = std::make_unique<fg_prog>();
+  p->num_args = num_args;
+  p->name = func;
+  p->module = module;
+  hipError_t e = hipModuleGetFunction(&p->func, p->module->module, func);
+  if (e != hipSuccess)
+    return set_err(FG_ERR_SYMBOL, std::string("symbol '") + func + "' not found: " + hipGetErrorString(e));
+  *out = p.release();
   return FG_OK;
 }
 

@@ -89,7 +89,7 @@ const char* op_name(Op op) {
       "Contiguous", "ReduceAxis", "ParamBuffer", "ParamScalar", "Range", "End", "Sink",
       "Index", "Load", "Store", "Vectorize", "Unroll", "Contract", "Const", "Neg", "Exp2",
       "Log2", "Sqrt", "Reciprocal", "Add", "Mul", "Max", "CmpLt", "Where", "Reduce", "After",
-      "DefineAcc", "Assign", "Gep"};
+      "DefineAcc", "Assign", "Gep", "Kernel", "KernelBuf", "KernelOut"};
   return names[static_cast<int>(op)];
 }
 
@@ -138,6 +138,12 @@ Arg Arg::lanes(const std::vector<std::pair<int64_t, int64_t>>& l) {
 Arg Arg::reduce(Op op, const std::vector<size_t>& ax) {
   Arg x; x.kind = Kind::Reduce; x.rop = op; x.v.assign(ax.begin(), ax.end()); return x;
 }
+Arg Arg::kernel(int64_t id, const Shape& out, const std::vector<int64_t>& params) {
+  Arg x; x.kind = Kind::Kernel; x.a = id; x.b = static_cast<int64_t>(out.size());
+  x.v.assign(out.begin(), out.end());
+  x.v.insert(x.v.end(), params.begin(), params.end());
+  return x;
+}
 
 bool Arg::operator==(const Arg& o) const {
   if (kind != o.kind) return false;
@@ -156,6 +162,7 @@ bool Arg::operator==(const Arg& o) const {
     case Kind::Buffer: return buf.get() == o.buf.get();
     case Kind::Bounds: case Kind::Shape: case Kind::Axes: case Kind::Lanes: return v == o.v;
     case Kind::Reduce: return rop == o.rop && v == o.v;
+    case Kind::Kernel: return a == o.a && b == o.b && v == o.v;
   }
   return false;
 }
@@ -180,6 +187,10 @@ size_t Arg::hash() const {
       break;
     }
     case Kind::Buffer: h = hmix(h, reinterpret_cast<size_t>(buf.get())); break;
+    case Kind::Kernel:
+      h = hmix(hmix(h, static_cast<size_t>(a)), static_cast<size_t>(b));
+      for (auto x : v) h = hmix(h, static_cast<size_t>(x));
+      break;
     case Kind::Reduce: h = hmix(h, static_cast<size_t>(rop)); [[fallthrough]];
     case Kind::Bounds: case Kind::Shape: case Kind::Axes: case Kind::Lanes:
       for (auto x : v) h = hmix(h, static_cast<size_t>(x));
@@ -209,6 +220,7 @@ std::string Arg::str() const {
     case Kind::Buffer: os << "buf#" << (buf ? buf->id : 0) << "[" << (buf ? buf->numel : 0) << "]"; break;
     case Kind::Bounds: case Kind::Shape: case Kind::Axes: case Kind::Lanes: vec(v); break;
     case Kind::Reduce: os << op_name(rop) << "("; vec(v); os << ")"; break;
+    case Kind::Kernel: os << a << "("; vec(v); os << ")"; break;
   }
   return os.str();
 }
@@ -455,6 +467,13 @@ bool UOp::compute_shape(Shape* out) const {
     case Op::Contiguous:
     case Op::After:
       return src(0).shape_opt(out);
+    case Op::Kernel:
+    case Op::KernelBuf:
+      if (a.kind != Arg::Kind::Kernel) return false;
+      *out = Shape(a.v.begin(), a.v.begin() + a.b);
+      return true;
+    case Op::KernelOut:
+      return !srcs().empty() && src(0).shape_opt(out);
     default:
       if (is_alu(op())) return src(0).shape_opt(out);
       return false;

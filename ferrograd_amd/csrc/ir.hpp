@@ -80,11 +80,17 @@ enum class Op : uint8_t {
   Device, DefineVar, Bind, Buffer, Shrink, Reshape, Permute, Expand, Contiguous,
   ReduceAxis, ParamBuffer, ParamScalar, Range, End, Sink, Index, Load, Store,
   Vectorize, Unroll, Contract, Const, Neg, Exp2, Log2, Sqrt, Reciprocal, Add, Mul,
-  Max, CmpLt, Where, Reduce, After, DefineAcc, Assign, Gep
+  Max, CmpLt, Where, Reduce, After, DefineAcc, Assign, Gep,
+  // Hand-written kernels (operators.hpp; no reference counterpart): one call
+  // with its arguments as sources, the storage of a further output of a call
+  // (a source of it), and that output once the call has run (sources: the
+  // storage, the call).
+  Kernel, KernelBuf, KernelOut
 };
 const char* op_name(Op op);
 bool is_alu(Op op);
 bool is_movement(Op op);
+inline bool is_kernel(Op op) { return op == Op::Kernel || op == Op::KernelBuf || op == Op::KernelOut; }
 
 enum class AxisKind : uint8_t { Loop, Global, Local, Reduce, GroupReduce, Upcast, Unroll, Thread };
 const char* axis_kind_name(AxisKind k);
@@ -99,15 +105,15 @@ using Buffer = std::shared_ptr<BufferInner>;
 struct Arg {
   enum class Kind : uint8_t {
     None, Device, Variable, Index, Range, ParamBuffer, ParamScalar, Float, Int, Bool,
-    Buffer, Bounds, Shape, Axes, Lanes, Reduce
+    Buffer, Bounds, Shape, Axes, Lanes, Reduce, Kernel
   };
   Kind kind = Kind::None;
-  int64_t a = 0;                 // Device id, Index tag, Range axis, slot, Int, Bool
-  int64_t b = 0;                 // Range kind, ParamBuffer numel, Variable min
+  int64_t a = 0;                 // Device id, Index tag, Range axis, slot, Int, Bool, Kernel id
+  int64_t b = 0;                 // Range kind, ParamBuffer numel, Variable min, Kernel output rank
   int64_t c = 0;                 // Variable max
   double f = 0.0;                // Float
   Op rop = Op::Add;              // Reduce op
-  std::vector<int64_t> v;        // Bounds/Shape/Axes/Lanes(flattened pairs)/Reduce axes
+  std::vector<int64_t> v;        // Bounds/Shape/Axes/Lanes(flattened pairs)/Reduce axes/Kernel output shape, then its parameters
   Buffer buf;                    // Buffer
   std::string name;              // Variable
 
@@ -126,6 +132,7 @@ struct Arg {
   static Arg axes(const std::vector<size_t>& ax);
   static Arg lanes(const std::vector<std::pair<int64_t, int64_t>>& l);
   static Arg reduce(Op op, const std::vector<size_t>& ax);
+  static Arg kernel(int64_t id, const Shape& out, const std::vector<int64_t>& params);
 
   AxisKind range_kind() const { return static_cast<AxisKind>(b); }
   std::vector<size_t> usizes() const { return std::vector<size_t>(v.begin(), v.end()); }

@@ -1,0 +1,355 @@
+// Graph nodes, gradients and launches of the hand-written kernels.
+#include "operators.hpp"
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+#include "tensor.hpp"
+
+// The kernels' code objects, compiled for gfx950 from kernels/*.hip when the
+// library is built.
+#define FG_IMAGE(name)                                     \
+  extern "C" const unsigned char fg_image_##name[];        \
+  extern "C" const unsigned char fg_image_##name##_end[];
+FG_IMAGE(dropout)
+FG_IMAGE(norm_rotate)
+FG_IMAGE(attention)
+
+namespace fg {
+
+namespace {
+
+void set_image(RenderedKernel& rk, const unsigned char* begin, const unsigned char* end) {
+  rk.image = begin;
+  rk.image_size = static_cast<size_t>(end - begin);
+}
+
+// The products of a fixed grid dimension: HIP takes 2^31 - 1 workgroups.
+unsigned grid_of(uint64_t n, const char* what) {
+  FG_CHECK(n >= 1 && n <= 0x7fffffffULL, std::string(what) + ": " + std::to_string(n) + " workgroups in one launch");
+  return static_cast<unsigned>(n);
+}
+
+int64_t to_bits(double f) {
+  int64_t b;
+  std::memcpy(&b, &f, 8);
+  return b;
+}
+
+double from_bits(int64_t b) {
+  double f;
+  std::memcpy(&f, &b, 8);
+  return f;
+}
+
+// A call's parameters (its Arg past the output's shape).
+std::vector<int64_t> params_of(const UOp& call) {
+  const Arg& a = call.arg();
+  return std::vector<int64_t>(a.v.begin() + a.b, a.v.end());
+}
+
+Shape shape_of(const UOp& call) {
+  const Arg& a = call.arg();
+  return Shape(a.v.begin(), a.v.begin() + a.b);
+}
+
+// A matrix a call reads: as it is, except that a literal or a value behind an
+// in-place store is copied first (both need a kernel that writes them out).
+UOp source(const UOp& u) {
+  UOp b = u;
+  while (b.op() == Op::Reshape) b = b.src(0);
+  return b.op() == Op::Const || b.op() == Op::After ? UOp::contiguous(u) : u;
+}
+
+// Whether every element of `u` is the literal 1.
+bool is_ones(UOp u) {
+  while (u.op() == Op::Reshape || u.op() == Op::Expand) u = u.src(0);
+  return u.op() == Op::Const && u.is_const_float(1.0);
+}
+
+// A gradient as a call reads it. `y.mul(g).sum(...)`, the way to seed a
+// gradient, arrives as g times an expanded 1: the same values without writing
+// the product out.
+UOp gradient_source(UOp g) {
+  while (g.op() == Op::Mul) {
+    if (is_ones(g.src(1))) g = g.src(0);
+    else if (is_ones(g.src(0))) g = g.src(1);
+    else break;
+  }
+  return source(g);
+}
+
+UOp word(uint64_t v, DeviceId d) { return UOp::const_int(static_cast<int32_t>(static_cast<uint32_t>(v)), DType::I32(), d); }
+
+UOp make_call(KernelId id, const Shape& out, const std::vector<UOp>& srcs, const std::vector<int64_t>& params) {
+  return UOp::make_new(Op::Kernel, DType::F32(), srcs, Arg::kernel(static_cast<int64_t>(id), out, params));
+}
+
+// The device check every operator makes once its arguments are in order.
+void need_hip(const Tensor& t, const char* what) {
+  FG_CHECK(t.device() == DeviceId::Hip, std::string(what) + ": the " + device_name(t.device()) +
+                                            " device has no kernel for it (only hip has)");
+}
+
+LaunchSpec launch(const std::string& func, uint64_t grid, unsigned block, const char* what, unsigned lds = 0) {
+  LaunchSpec l;
+  l.func = func;
+  l.grid[0] = grid_of(grid, what);
+  l.block[0] = block;
+  l.lds_bytes = lds;
+  return l;
+}
+
+// ── dropout ─────────────────────────────────────────────────────────────────
+// params: p's bits.
+
+RenderedKernel render_dropout(const UOp& call) {
+  const double p = from_bits(params_of(call)[0]);
+  const uint64_t n = numel(shape_of(call));
+  RenderedKernel rk;
+  rk.kind = "dropout";
+  set_image(rk, fg_image_dropout, fg_image_dropout_end);
+  const uint64_t threshold = static_cast<uint64_t>(p * 4294967296.0);
+  // 4 elements a thread (one block of four random words).
+  rk.launches = {launch("fg_dropout", (n + 1023) / 1024, 256, "dropout")};
+  rk.call_args = {CallArg::slot(0), CallArg::slot(1), CallArg::slot(2), CallArg::slot(3), CallArg::slot(4),
+                  CallArg::slot(5), CallArg::i32(static_cast<int32_t>(n & 0xffffffffu)),
+                  CallArg::i32(static_cast<int64_t>(n >> 32)), CallArg::i32(static_cast<int32_t>(threshold)),
+                  CallArg::f32(static_cast<float>(1.0 / (1.0 - p)))};
+  return rk;
+}
+
+// Output i (from 1 on) of a call with sources `srcs`: its storage, a source of
+// the call besides them.
+UOp output_storage(KernelId id, int64_t i, const Shape& shape, const std::vector<UOp>& srcs) {
+  return UOp::make_new(Op::KernelBuf, DType::F32(), srcs, Arg::kernel(static_cast<int64_t>(id), shape, {i}));
+}
+
+UOp output_of(const UOp& storage, const UOp& call) {
+  return UOp::make_new(Op::KernelOut, storage.dtype(), {storage, call}, Arg::none());
+}
+
+// ── norm_rotate ─────────────────────────────────────────────────────────────
+// params: tokens, heads, dim, bits of eps, bits of base. Sources: x, weight,
+// positions; of the gradient also g and dweight's storage.
+
+// A head in vectors of `vec` on `lanes` lanes, `turns` vectors of each half a
+// lane (kernels/norm_rotate.hip).
+struct RowSplit {
+  int vec, lanes, turns;
+  std::string suffix() const {
+    return "_" + std::to_string(vec) + "_" + std::to_string(lanes) + "_" + std::to_string(turns);
+  }
+};
+
+RowSplit row_split(int64_t dim) {
+  const int64_t half = dim / 2;
+  RowSplit r;
+  r.vec = half % 4 == 0 ? 4 : half % 2 == 0 ? 2 : 1;  // halves of a row start on a vector's alignment
+  const int64_t vectors = half / r.vec;
+  r.lanes = 8;
+  while (r.lanes < vectors && r.lanes < 64) r.lanes *= 2;
+  r.turns = 1;
+  while (r.lanes * r.turns < vectors) r.turns *= 2;
+  return r;
+}
+
+RenderedKernel render_norm_rotate(const UOp& call, bool grad) {
+  const std::vector<int64_t> p = params_of(call);
+  const int64_t tokens = p[0], heads = p[1], dim = p[2];
+  const double eps = from_bits(p[3]), log2_base = std::log2(from_bits(p[4]));
+  const RowSplit r = row_split(dim);
+  // Heads of a token that share its cosines: more while 16384 groups are left
+  // (every lane of the chip four waves deep at 16 lanes a group).
+  const int64_t heads_per = std::max<int64_t>(1, std::min<int64_t>({heads, 8, tokens * heads / 16384}));
+  const int64_t units = tokens * ((heads + heads_per - 1) / heads_per), per_block = 256 / r.lanes;
+  const int64_t blocks = std::min<int64_t>((units + per_block - 1) / per_block, grad ? 1024 : 4096);
+  RenderedKernel rk;
+  set_image(rk, fg_image_norm_rotate, fg_image_norm_rotate_end);
+  const float hi = static_cast<float>(log2_base);
+  const std::vector<CallArg> tail = {CallArg::i32(tokens), CallArg::i32(heads), CallArg::i32(dim), CallArg::i32(heads_per),
+                                     CallArg::f32(static_cast<float>(eps)), CallArg::f32(hi),
+                                     CallArg::f32(static_cast<float>(log2_base - hi))};
+  rk.call_args = {CallArg::slot(0), CallArg::slot(1), CallArg::slot(2), CallArg::slot(3)};
+  if (!grad) {
+    rk.kind = "norm_rotate";
+    rk.launches = {launch("fg_norm_rotate" + r.suffix(), static_cast<uint64_t>(blocks), 256, "norm_rotate")};
+  } else {
+    rk.kind = "norm_rotate_grad";
+    rk.launches = {launch("fg_norm_rotate_grad" + r.suffix(), static_cast<uint64_t>(blocks), 256, "norm_rotate"),
+                   launch("fg_norm_rotate_weight", static_cast<uint64_t>((dim + 63) / 64), 1024, "norm_rotate")};
+    rk.workspace_bytes = static_cast<size_t>(blocks * dim) * 4;
+    rk.side_outputs = {5};
+    for (CallArg a : {CallArg::slot(4), CallArg::slot(5), CallArg::workspace(), CallArg::i32(blocks)}) rk.call_args.push_back(a);
+  }
+  rk.call_args.insert(rk.call_args.end(), tail.begin(), tail.end());
+  return rk;
+}
+
+// ── attention ───────────────────────────────────────────────────────────────
+// params: batch, sq, sk, heads, kv_heads, dim, causal, whether there are
+// lengths, bits of scale. Sources: q, k, v, [lengths], the stats' storage; of
+// the gradient: q, k, v, y, g, stats, [lengths], dk's and dv's storage.
+
+RenderedKernel render_attention(const UOp& call, bool grad) {
+  const std::vector<int64_t> p = params_of(call);
+  const int64_t batch = p[0], sq = p[1], sk = p[2], heads = p[3], kv_heads = p[4];
+  const bool lengths = p[7] != 0;
+  RenderedKernel rk;
+  set_image(rk, fg_image_attention, fg_image_attention_end);
+  const uint64_t q_rows = static_cast<uint64_t>(batch * heads * sq), k_rows = static_cast<uint64_t>(batch * kv_heads * sk);
+  if (!grad) {
+    rk.kind = "attention";
+    rk.launches = {launch("fg_attention", (q_rows + 3) / 4, 256, "attention")};
+    rk.call_args = {CallArg::slot(0), CallArg::slot(1), CallArg::slot(2), CallArg::slot(3), CallArg::slot(lengths ? 5 : 4),
+                    lengths ? CallArg::slot(4) : CallArg::null()};
+    rk.side_outputs = {lengths ? 5 : 4};
+  } else {
+    rk.kind = "attention_grad";
+    rk.launches = {launch("fg_attention_dq", (q_rows + 3) / 4, 256, "attention"),
+                   launch("fg_attention_dkv", (k_rows + 3) / 4, 256, "attention")};
+    const int dk = lengths ? 8 : 7;
+    for (int i = 0; i < 7; i++) rk.call_args.push_back(CallArg::slot(i));
+    rk.call_args.push_back(CallArg::slot(dk));
+    rk.call_args.push_back(CallArg::slot(dk + 1));
+    rk.call_args.push_back(lengths ? CallArg::slot(7) : CallArg::null());
+    rk.side_outputs = {dk, dk + 1};
+  }
+  for (int i = 0; i < 7; i++) rk.call_args.push_back(CallArg::i32(p[static_cast<size_t>(i)]));
+  rk.call_args.push_back(CallArg::f32(static_cast<float>(from_bits(p[8]))));
+  return rk;
+}
+
+void check_matrix(const Tensor& t, const char* what) {
+  FG_CHECK(t.dtype() == DType::F32(), std::string(what) + " must be f32");
+  FG_CHECK(t.ndim() == 2, std::string(what) + " must be 2D (one row per token), got shape " + shape_str(t.shape()));
+  FG_CHECK(t.numel() > 0, std::string(what) + " is empty");
+}
+
+}  // namespace
+
+Tensor Tensor::norm_rotate(const Tensor& weight, const Tensor& positions, size_t heads, double eps, double base) const {
+  check_matrix(*this, "norm_rotate: the input");
+  FG_CHECK(device() == weight.device() && device() == positions.device(), "norm_rotate: all tensors must be on the same device");
+  const Shape s = shape();
+  FG_CHECK(heads >= 1 && s[1] % heads == 0,
+           "norm_rotate: " + std::to_string(s[1]) + " columns do not split into " + std::to_string(heads) + " heads");
+  const size_t dim = s[1] / heads;
+  FG_CHECK(dim % 2 == 0 && dim <= 512, "norm_rotate: the head size must be even and at most 512, got " + std::to_string(dim));
+  FG_CHECK(weight.dtype() == DType::F32() && weight.shape() == Shape{dim},
+           "norm_rotate: the weight must be f32 of shape " + shape_str(Shape{dim}) + ", got " + shape_str(weight.shape()));
+  FG_CHECK(positions.dtype() == DType::I32() && positions.shape() == Shape{s[0]},
+           "norm_rotate: the positions must be i32 of shape " + shape_str(Shape{s[0]}) + ", got " + shape_str(positions.shape()));
+  FG_CHECK(eps >= 0 && std::isfinite(eps), "norm_rotate: eps must be finite and not negative");
+  FG_CHECK(base > 0 && std::isfinite(base), "norm_rotate: base must be finite and positive");
+  FG_CHECK(s[0] * heads <= 0x7fffffffu, "norm_rotate: more than 2^31 - 1 heads of tokens");
+  need_hip(*this, "norm_rotate");
+  return from_uop(make_call(KernelId::NormRotate, s, {source(uop()), source(weight.uop()), source(positions.uop())},
+                            {static_cast<int64_t>(s[0]), static_cast<int64_t>(heads), static_cast<int64_t>(dim),
+                             to_bits(eps), to_bits(base)}),
+                  requires_grad() || weight.requires_grad());
+}
+
+Tensor Tensor::attention(const Tensor& k, const Tensor& v, const Tensor* lengths, size_t batch, size_t heads,
+                         size_t kv_heads, bool causal, double scale) const {
+  check_matrix(*this, "attention: q");
+  check_matrix(k, "attention: k");
+  check_matrix(v, "attention: v");
+  FG_CHECK(device() == k.device() && device() == v.device() && (!lengths || device() == lengths->device()),
+           "attention: all tensors must be on the same device");
+  const Shape qs = shape(), ks = k.shape();
+  FG_CHECK(batch >= 1 && qs[0] % batch == 0 && ks[0] % batch == 0,
+           "attention: " + std::to_string(qs[0]) + " query rows and " + std::to_string(ks[0]) +
+               " key rows do not split into a batch of " + std::to_string(batch));
+  FG_CHECK(heads >= 1 && kv_heads >= 1 && heads % kv_heads == 0,
+           "attention: " + std::to_string(heads) + " heads do not share " + std::to_string(kv_heads) + " key heads evenly");
+  FG_CHECK(qs[1] % heads == 0, "attention: " + std::to_string(qs[1]) + " columns do not split into " + std::to_string(heads) + " heads");
+  const size_t dim = qs[1] / heads;
+  FG_CHECK(dim <= 128, "attention: the head size must be at most 128, got " + std::to_string(dim));
+  FG_CHECK(ks[1] == kv_heads * dim, "attention: k must have " + std::to_string(kv_heads) + " heads of " + std::to_string(dim) +
+                                        ", got " + std::to_string(ks[1]) + " columns");
+  FG_CHECK(v.shape() == ks, "attention: v must have k's shape " + shape_str(ks) + ", got " + shape_str(v.shape()));
+  if (lengths)
+    FG_CHECK(lengths->dtype() == DType::I32() && lengths->shape() == Shape{batch},
+             "attention: the lengths must be i32 of shape " + shape_str(Shape{batch}) + ", got " + shape_str(lengths->shape()));
+  FG_CHECK(std::isfinite(scale) && std::isfinite(static_cast<float>(scale)), "attention: scale must be finite");
+  const size_t sq = qs[0] / batch, sk = ks[0] / batch;
+  FG_CHECK(sq <= (1u << 28) && sk <= (1u << 28), "attention: sequences of more than 2^28 tokens");
+  need_hip(*this, "attention");
+  const std::vector<int64_t> params = {static_cast<int64_t>(batch), static_cast<int64_t>(sq), static_cast<int64_t>(sk),
+                                       static_cast<int64_t>(heads), static_cast<int64_t>(kv_heads),
+                                       static_cast<int64_t>(dim), causal, lengths != nullptr, to_bits(scale)};
+  std::vector<UOp> srcs = {source(uop()), source(k.uop()), source(v.uop())};
+  if (lengths) srcs.push_back(source(lengths->uop()));
+  srcs.push_back(output_storage(KernelId::Attention, 1, Shape{2, batch * heads * sq}, srcs));
+  return from_uop(make_call(KernelId::Attention, qs, srcs, params), requires_grad() || k.requires_grad() || v.requires_grad());
+}
+
+Tensor Tensor::dropout(double p, uint64_t seed, uint64_t offset) const {
+  FG_CHECK(dtype() == DType::F32(), "dropout: the input must be f32");
+  FG_CHECK(p >= 0.0 && p < 1.0, "dropout: p must be in [0, 1), got " + std::to_string(p));
+  FG_CHECK(numel() > 0, "dropout: the input is empty");
+  need_hip(*this, "dropout");
+  if (p == 0.0) return *this;
+  const DeviceId d = device();
+  return from_uop(make_call(KernelId::Dropout, shape(), {source(uop()), word(seed, d), word(seed >> 32, d), word(offset, d),
+                                                         word(offset >> 32, d)},
+                            {to_bits(p)}),
+                  requires_grad());
+}
+
+std::vector<UOp> kernel_gradient(const UOp& call, const UOp& grad) {
+  switch (static_cast<KernelId>(call.arg().a)) {
+    case KernelId::NormRotate: {
+      std::vector<UOp> srcs = call.srcs();
+      srcs.push_back(gradient_source(grad));
+      UOp dw = output_storage(KernelId::NormRotateGrad, 1, call.src(1).shape(), srcs);
+      srcs.push_back(dw);
+      UOp dx = make_call(KernelId::NormRotateGrad, call.src(0).shape(), srcs, params_of(call));
+      return {dx, output_of(dw, dx), UOp()};
+    }
+    case KernelId::Attention: {
+      const std::vector<int64_t> params = params_of(call);
+      std::vector<UOp> srcs = {call.src(0), call.src(1), call.src(2), call, gradient_source(grad)};
+      srcs.push_back(output_of(call.srcs().back(), call));
+      if (params[7]) srcs.push_back(call.src(3));
+      UOp dk = output_storage(KernelId::AttentionGrad, 1, call.src(1).shape(), srcs);
+      UOp dv = output_storage(KernelId::AttentionGrad, 2, call.src(2).shape(), srcs);
+      srcs.push_back(dk);
+      srcs.push_back(dv);
+      UOp dq = make_call(KernelId::AttentionGrad, call.src(0).shape(), srcs, params);
+      std::vector<UOp> grads = {dq, output_of(dk, dq), output_of(dv, dq)};
+      grads.resize(call.srcs().size());
+      return grads;
+    }
+    case KernelId::NormRotateGrad:
+    case KernelId::AttentionGrad: break;  // no second gradients
+    case KernelId::Dropout: {
+      // The same words again: the mask is never stored.
+      std::vector<UOp> srcs = call.srcs();
+      srcs[0] = gradient_source(grad);
+      return {UOp::make_new(Op::Kernel, call.dtype(), srcs, call.arg())};
+    }
+  }
+  fail("gradient not implemented for this kernel");
+}
+
+RenderedKernel render_hip_call(const UOp& call) {
+  RenderedKernel rk;
+  switch (static_cast<KernelId>(call.arg().a)) {
+    case KernelId::Dropout: rk = render_dropout(call); break;
+    case KernelId::NormRotate: rk = render_norm_rotate(call, false); break;
+    case KernelId::NormRotateGrad: rk = render_norm_rotate(call, true); break;
+    case KernelId::Attention: rk = render_attention(call, false); break;
+    case KernelId::AttentionGrad: rk = render_attention(call, true); break;
+  }
+  rk.name = rk.launches.at(0).func;
+  rk.out_slot = 0;
+  rk.out_count = numel(shape_of(call));
+  rk.params.emplace_back(0, call.dtype());
+  for (size_t i = 0; i < call.srcs().size(); i++) rk.params.emplace_back(static_cast<int>(i) + 1, call.src(i).dtype());
+  return rk;
+}
+
+}  // namespace fg

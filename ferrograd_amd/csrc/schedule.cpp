@@ -537,6 +537,55 @@ ScheduleItem parameterize_store(const UOp& store, const ScheduleOptions& opt) {
   return item;
 }
 
+namespace {
+
+// The node a hand-written kernel's source reads, under reshapes (which leave
+// the elements' order alone).
+UOp under_reshapes(UOp u) {
+  while (u.op() == Op::Reshape) u = u.src(0);
+  return u;
+}
+
+// The nodes the calls of `order` read as whole buffers: whatever computes them
+// gets a kernel of its own.
+UOpSet kernel_sources(const std::vector<UOp>& order) {
+  UOpSet out;
+  for (auto& n : order) {
+    if (n.op() != Op::Kernel) continue;
+    for (auto& s : n.srcs()) {
+      UOp b = under_reshapes(s);
+      if (b.op() != Op::Buffer && b.op() != Op::Const && !is_kernel(b.op())) out.insert(b);
+    }
+  }
+  return out;
+}
+
+// A call whose sources are buffers (seen through reshapes) and integer
+// constants, as a schedule item: output in slot 0, the sources from slot 1 on.
+ScheduleItem parameterize_kernel(const UOp& call) {
+  ScheduleItem item;
+  std::vector<UOp> params;
+  for (auto& s : call.srcs()) {
+    UOp b = under_reshapes(s);
+    const int64_t slot = static_cast<int64_t>(params.size()) + 1;
+    if (b.op() == Op::Const) {
+      item.inputs.push_back(scalar_input(b.arg()));
+      params.push_back(UOp::param_scalar(slot, b.dtype(), call.device()));
+      continue;
+    }
+    FG_CHECK(b.op() == Op::Buffer && b.arg().buf, "a kernel's source must be materialised before it");
+    item.inputs.push_back(KernelArg::buf(b.arg().buf));
+    params.push_back(UOp::param_buffer(slot, b.dtype(), static_cast<int64_t>(b.arg().buf->numel), call.device()));
+  }
+  item.kernel = UOp::make_new(call.op(), call.dtype(), params, call.arg());
+  item.sink = UOp::sink({item.kernel});
+  item.out_shape = call.shape();
+  item.output_buffer = get_device(call.device()).reserve_buffer(call.dtype(), numel(item.out_shape));
+  return item;
+}
+
+}  // namespace
+
 // schedule.rs:64-126
 SchedulePlan schedule_many(const std::vector<UOp>& exprs, const ScheduleOptions& opt) {
   FG_CHECK(!exprs.empty(), "schedule_many requires at least one root");
@@ -559,15 +608,41 @@ SchedulePlan schedule_many(const std::vector<UOp>& exprs, const ScheduleOptions&
   // feed (fusing only), keyed by that node. Value-preserving: the kernel
   // applies the same elementwise ops to the same reduced values.
   UOpMap<UOp> deferred;
+  const UOpSet kernel_reads = kernel_sources(order);
   for (auto& node : order) {
+    if (is_kernel(node.op())) {
+      // Hand-written kernels run in phase 1 even where they are roots, so that
+      // every reader of theirs reads a buffer.
+      UOp call = substitute_materialized(node, plan.replacements);
+      if (node.op() == Op::KernelOut) {
+        plan.replacements[node] = call.src(0);
+        continue;
+      }
+      ScheduleItem item;
+      if (node.op() == Op::KernelBuf) {
+        item.out_shape = node.shape();
+        item.output_buffer = get_device(node.device()).reserve_buffer(node.dtype(), numel(item.out_shape));
+        item.sink = UOp::sink({UOp::param_buffer(0, node.dtype(), static_cast<int64_t>(numel(item.out_shape)), node.device())});
+        item.storage_only = true;
+      } else {
+        item = parameterize_kernel(call);
+      }
+      plan.replacements[node] = buffer_replacement(item);
+      plan.items.push_back(std::move(item));
+      continue;
+    }
     auto d = deferred.find(node);
     if (d != deferred.end()) {
       // The reduce stays fused only if this node gets a kernel of its own and
       // that kernel computes no other reduction.
-      bool own_kernel = roots.count(node) ||
+      bool own_kernel = roots.count(node) || kernel_reads.count(node) ||
                         should_materialize(node, roots, consumers, nested, opt, topo_idx, plan.replacements);
       if (!own_kernel || has_unmaterialized_reduce(node, plan.replacements, d->second)) materialize(d->second);
       deferred.erase(d);
+    }
+    if (kernel_reads.count(node)) {
+      materialize(node);
+      continue;
     }
     if (!should_materialize(node, roots, consumers, nested, opt, topo_idx, plan.replacements)) continue;
     if (opt.fuse && node.op() == Op::ReduceAxis && !is_held(node, opt)) {
@@ -636,6 +711,7 @@ SchedulePlan schedule_many(const std::vector<UOp>& exprs, const ScheduleOptions&
     }
   }
   for (auto& expr : exprs) {
+    if (plan.replacements.count(expr)) continue;  // a call, or read by one: it ran in phase 1
     UOp fin = substitute_materialized(expr, plan.replacements);
     UOp store, value;
     if (assignment_effect(fin, &store, &value)) {

@@ -13,6 +13,8 @@ struct ScheduleItem {
   std::vector<KernelArg> inputs;   // runtime inputs in slot order, excluding output slot 0
   Buffer output_buffer;            // null for in-place stores
   Shape out_shape;
+  UOp kernel;                      // the call, its sources numbered parameters (hand-written kernels)
+  bool storage_only = false;       // no launch: output_buffer is a further output of a later item's call
 };
 
 // schedule.rs:45-50

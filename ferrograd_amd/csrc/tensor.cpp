@@ -2,6 +2,8 @@
 // Follows src/tensor.rs, src/gradient.rs, src/nn.rs and src/optim.rs.
 #include "tensor.hpp"
 
+#include "operators.hpp"
+
 #include <chrono>
 #include <cmath>
 #include <cstdio>
@@ -423,6 +425,10 @@ static void assert_kernel_ready(const UOp& root) {
 static std::shared_ptr<Program> execute_item(const ScheduleItem& item) {
   const uint64_t start_ns = now_ns();
   Device& backend = get_device(item.sink.device());
+  if (item.storage_only) {  // a later item's call writes it
+    backend.realize_storage(*item.output_buffer, false);
+    return nullptr;
+  }
   int debug = debug_level();
   size_t num_args = item.output_buffer ? item.inputs.size() + 1 : item.inputs.size();
   auto& lc = lowering_cache(backend.id());
@@ -436,6 +442,14 @@ static std::shared_ptr<Program> execute_item(const ScheduleItem& item) {
       std::fprintf(stderr, "*** %s %4zu  (cached)         arg %2zu\n", backend.id() == DeviceId::Hip ? "HIP" : "CPU",
                    kid, num_args);
     }
+  } else if (item.kernel) {
+    RenderedKernel rk = backend.render_call(item.kernel);
+    program = backend.compile(rk, num_args);
+    realize_stats().programs_compiled++;
+    if (debug >= 1)
+      std::fprintf(stderr, "*** HIP %4zu  %-16s arg %2zu  [%s]\n", g_kernel_count++, rk.name.c_str(), num_args,
+                   rk.kind.c_str());
+    lc[item.sink] = program;
   } else {
     if (debug >= 3) std::fprintf(stderr, "━━━ rangeify [before] ━━━\n%s", item.sink.dump().c_str());
     UOp rangeified = rangeify(item.sink);
@@ -567,8 +581,10 @@ GraphKey graph_key(const std::vector<UOp>& roots, bool fuse, const std::vector<c
       for (size_t j = 0; j < srcs.size(); j++) {
         if (srcs[j].op() != Op::Const || srcs[j].dtype() != DType::I32()) continue;
         uint32_t sp = pos.get(srcs[j].get());
-        bool param = shrink && j >= 1 && j - 1 < n.arg().v.size() &&
-                     static_cast<size_t>(n.arg().v[j - 1]) != src_shape[j - 1];
+        // A hand-written kernel's integers (dropout's seed and offset) are
+        // arguments of its launch too.
+        bool param = (shrink && j >= 1 && j - 1 < n.arg().v.size() &&
+                      static_cast<size_t>(n.arg().v[j - 1]) != src_shape[j - 1]) || is_kernel(n.op());
         use[sp] |= param ? 1 : 2;
       }
     }
@@ -645,7 +661,7 @@ struct PlanArg {
 };
 
 struct PlanKernel {
-  std::shared_ptr<Program> program;
+  std::shared_ptr<Program> program;  // null: nothing runs, the output is storage for a later kernel's call
   bool has_output = false;
   DType out_dtype;
   size_t out_numel = 0;
@@ -787,16 +803,17 @@ void replay_plan(Device& backend, const GraphKey& k, const std::shared_ptr<Cache
   std::vector<int32_t> starts;
   for (uint32_t i : plan.written_leaves) k.leaves[i]->known_zero = false;
   std::vector<Buffer> outs(plan.kernels.size());
-  std::vector<Program*> progs(plan.kernels.size());
-  std::vector<std::vector<KernelArg>> seq_args(plan.kernels.size());
+  std::vector<Program*> progs;
+  std::vector<std::vector<KernelArg>> seq_args;
+  progs.reserve(plan.kernels.size());
+  seq_args.reserve(plan.kernels.size());
   int debug = debug_level();
   uint64_t l0 = now_ns();
   // Every output and lazily zeroed input gets storage first (zero fills are
   // queued on the stream ahead of the launches), then the whole sequence runs.
   for (size_t j = 0; j < plan.kernels.size(); j++) {
     const PlanKernel& pk = plan.kernels[j];
-    std::vector<KernelArg>& args = seq_args[j];
-    progs[j] = pk.program.get();
+    std::vector<KernelArg> args;
     if (pk.has_output) {
       Buffer out = backend.reserve_buffer(pk.out_dtype, pk.out_numel);
       // The same storage as last time when it is free again, so a device that
@@ -808,6 +825,7 @@ void replay_plan(Device& backend, const GraphKey& k, const std::shared_ptr<Cache
       outs[j] = out;
       args.push_back(KernelArg::buf(out));
     }
+    if (!pk.program) continue;
     for (auto& pa : pk.args) {
       if (pa.kind == PlanArg::Value) {
         args.push_back(pa.value);
@@ -832,6 +850,8 @@ void replay_plan(Device& backend, const GraphKey& k, const std::shared_ptr<Cache
       std::fprintf(stderr, "*** %s %4zu  (plan)           arg %2zu\n", backend.id() == DeviceId::Hip ? "HIP" : "CPU",
                    kid, args.size());
     }
+    progs.push_back(pk.program.get());
+    seq_args.push_back(std::move(args));
   }
   uint64_t l1 = now_ns();
   realize_stats().ns_lower += l1 - l0;
@@ -1018,33 +1038,38 @@ std::vector<uint64_t> capture_shape(const CapturedStep& cap) {
 void replay_step(Device& backend, CapturedStep& cap, int slot, int64_t start = 0) {
   const size_t n = cap.kernels.size();
   std::vector<Buffer> outs(n);
-  std::vector<Program*> progs(n);
-  std::vector<std::vector<KernelArg>> args(n);
+  std::vector<Program*> progs;
+  std::vector<std::vector<KernelArg>> args;
+  progs.reserve(n);
+  args.reserve(n);
   uint64_t l0 = now_ns();
   for (size_t j = 0; j < n; j++) {
     const CapturedStep::Kernel& k = cap.kernels[j];
-    progs[j] = k.prog;
+    std::vector<KernelArg> ka;
     if (k.has_output) {
       Buffer out = backend.reserve_buffer(k.out_dtype, k.out_numel);
       backend.realize_storage_at(*out, false, cap.last_storage[j]);
       cap.last_storage[j] = out->storage;
       out->known_zero = false;
       outs[j] = out;
-      args[j].push_back(KernelArg::buf(out));
+      ka.push_back(KernelArg::buf(out));
     }
+    if (!k.prog) continue;  // storage for a later kernel's call
     for (const CapturedStep::Arg& a : k.args) {
-      if (a.kind == CapturedStep::Arg::Value) args[j].push_back(a.value);
-      else if (a.kind == CapturedStep::Arg::StepStart) args[j].push_back(KernelArg::i32(static_cast<int32_t>(start)));
-      else if (a.kind == CapturedStep::Arg::Persistent) args[j].push_back(KernelArg::buf(a.buf));
-      else args[j].push_back(KernelArg::buf(outs[a.out]));
+      if (a.kind == CapturedStep::Arg::Value) ka.push_back(a.value);
+      else if (a.kind == CapturedStep::Arg::StepStart) ka.push_back(KernelArg::i32(static_cast<int32_t>(start)));
+      else if (a.kind == CapturedStep::Arg::Persistent) ka.push_back(KernelArg::buf(a.buf));
+      else ka.push_back(KernelArg::buf(outs[a.out]));
     }
+    progs.push_back(k.prog);
+    args.push_back(std::move(ka));
   }
   uint64_t l1 = now_ns();
   realize_stats().ns_lower += l1 - l0;
   backend.execute_sequence_read(progs, args, cap.device_state, outs[cap.result_kernel], slot);
   realize_stats().ns_launch += now_ns() - l1;
-  realize_stats().kernels_launched += n;
-  realize_stats().lowering_cache_hits += n;
+  realize_stats().kernels_launched += progs.size();
+  realize_stats().lowering_cache_hits += progs.size();
 }
 
 // Steps of the native loop queued ahead of the device: FG_STEPS_IN_FLIGHT,
@@ -1286,6 +1311,7 @@ std::vector<UOp> gradient_for_op(const UOp& node, const UOp& grad) {
       fail("unsupported reduce op gradient");
     }
     case Op::Buffer: case Op::Const: return {};
+    case Op::Kernel: return kernel_gradient(node, grad);
     default: fail(std::string("gradient not implemented for ") + op_name(node.op()));
   }
 }

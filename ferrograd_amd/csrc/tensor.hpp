@@ -73,6 +73,19 @@ class Tensor {
   Tensor cross_entropy(const Tensor& targets) const;
   Tensor matmul(const Tensor& other) const;
 
+  // Hand-written kernels (operators.hpp; no reference counterpart).
+  // Dropout: x / (1 - p) where the element's random word is at least p * 2^32,
+  // else 0; the words are a function of (seed, offset, element index) alone.
+  // RMS norm of each head (weight [dim]) and the rotation of its pairs
+  // (i, i + dim/2) by positions[row] * base^(-2i/dim); x is [tokens, heads * dim].
+  Tensor norm_rotate(const Tensor& weight, const Tensor& positions, size_t heads, double eps, double base) const;
+  // softmax(scale q k^T) v with *this = q [batch * sq, heads * dim] and k, v
+  // [batch * sk, kv_heads * dim]. Keys at or past lengths[b] (i32 [batch], or
+  // null) are hidden, with `causal` also those past i + sk - sq.
+  Tensor attention(const Tensor& k, const Tensor& v, const Tensor* lengths, size_t batch, size_t heads, size_t kv_heads,
+                   bool causal, double scale) const;
+  Tensor dropout(double p, uint64_t seed, uint64_t offset) const;
+
   // Realisation (tensor.rs:781-930).
   static void realize_many(const std::vector<Tensor>& tensors);
   Tensor realize() const;

@@ -61,6 +61,32 @@ int fg_tensor_movement(fg_tensor* t, int op, const int64_t* arg, int narg, fg_te
 int fg_tensor_narrow(fg_tensor* t, int64_t dim, int64_t start, int64_t len, fg_tensor** out);
 int fg_tensor_log_softmax(fg_tensor* t, int64_t axis, fg_tensor** out);
 
+/* softmax(scale q k^T) v per head: q [batch * sq, heads * dim], k and v
+ * [batch * sk, kv_heads * dim], f32, dim at most 128; query head h reads key
+ * head h / (heads / kv_heads). Query i of a sequence sees the keys j <
+ * lengths[b] (i32 [batch], clamped to [0, sk]; NULL: all) and, with `causal`,
+ * j <= i + sk - sq. One that sees none gives 0 and gradients of 0. What hidden
+ * keys past a length hold never matters; every other value must be finite.
+ * Gradients flow to q, k and v: the probabilities are computed again from the
+ * row's maximum and sum. HIP device only. No reference counterpart. */
+int fg_tensor_attention(fg_tensor* q, fg_tensor* k, fg_tensor* v, fg_tensor* lengths, int64_t batch, int64_t heads,
+                        int64_t kv_heads, int causal, double scale, fg_tensor** out);
+
+/* Per-head norm and position rotation of x [tokens, heads * dim], f32, dim even
+ * and at most 512: z = x * (mean(x^2) + eps)^(-1/2) * weight over each head
+ * (weight f32 [dim]), then the pair (z_i, z_{i + dim/2}) turned by
+ * positions[token] * base^(-2i/dim) (positions i32 [tokens]). Gradients flow to
+ * x and weight. HIP device only. No reference counterpart. */
+int fg_tensor_norm_rotate(fg_tensor* x, fg_tensor* weight, fg_tensor* positions, int64_t heads, double eps, double base,
+                          fg_tensor** out);
+
+/* Dropout of an f32 tensor, 0 <= p < 1: element e is kept and
+ * scaled by 1 / (1 - p) where word e % 4 of Philox4x32-10 of the counter
+ * (e / 4, offset) under the key `seed` is at least floor(p * 2^32), else it is
+ * 0. Nothing about the mask is stored: the gradient draws the words again. HIP
+ * device only. No reference counterpart. */
+int fg_tensor_dropout(fg_tensor* t, double p, uint64_t seed, uint64_t offset, fg_tensor** out);
+
 /* In-place graph updates (tensor.rs:399-440). */
 int fg_tensor_assign(fg_tensor* t, fg_tensor* value);
 int fg_tensor_replace(fg_tensor* t, fg_tensor* value);

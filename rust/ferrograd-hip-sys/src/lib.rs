@@ -206,6 +206,9 @@ extern "C" {
     pub fn fg_tensor_movement(t: *mut fg_tensor, op: i32, arg: *const i64, narg: i32,
                               out: *mut *mut fg_tensor) -> i32;
     pub fn fg_tensor_narrow(t: *mut fg_tensor, dim: i64, start: i64, len: i64, out: *mut *mut fg_tensor) -> i32;
+    pub fn fg_tensor_attention(q: *mut fg_tensor, k: *mut fg_tensor, v: *mut fg_tensor, lengths: *mut fg_tensor, batch: i64, heads: i64, kv_heads: i64, causal: i32, scale: f64, out: *mut *mut fg_tensor) -> i32;
+    pub fn fg_tensor_norm_rotate(x: *mut fg_tensor, weight: *mut fg_tensor, positions: *mut fg_tensor, heads: i64, eps: f64, base: f64, out: *mut *mut fg_tensor) -> i32;
+    pub fn fg_tensor_dropout(t: *mut fg_tensor, p: f64, seed: u64, offset: u64, out: *mut *mut fg_tensor) -> i32;
     pub fn fg_tensor_log_softmax(t: *mut fg_tensor, axis: i64, out: *mut *mut fg_tensor) -> i32;
     pub fn fg_tensor_assign(t: *mut fg_tensor, value: *mut fg_tensor) -> i32;
     pub fn fg_tensor_replace(t: *mut fg_tensor, value: *mut fg_tensor) -> i32;
