@@ -42,12 +42,453 @@ __device__ inline float dot(const float* a, const float* b, int d) {
   return t;
 }
 
+// ── products of cut operands ────────────────────────────────────────────────
+// A float32 product on the float16 matrix cores: each operand is scaled by a
+// power of two that brings its block's largest value below 2^15 and cut into
+// two float16 parts, 11 bits each, and a b = a1 b1 + a1 b2 + a2 b1 with sums in
+// float32; a2 b2, 2^-20 of the product at most, is left out. Three float16
+// products cost less than a fifth of one float32 product's matrix-core time.
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+
+// Rows of a block that shares a scale, and of a tile.
+constexpr int kBlock = 32;
+// The scale of a block of zeros.
+constexpr int kZeroExponent = 127;
+constexpr int kPart = 1024;  // bytes of one fragment: 64 lanes of 8 float16
+
+// The power of two that brings `top`, a block's largest magnitude, into
+// [2^14, 2^15). Not finite: 0, and what the block takes part in is not finite.
+__device__ inline int block_exponent(float top) {
+  if (top == 0.f) return kZeroExponent;
+  if (!(top < INFINITY)) return 0;
+  int e;
+  frexpf(top, &e);  // top = f 2^e with f in [1/2, 1)
+  return min(15 - e, kZeroExponent);
+}
+
+// Eight scaled numbers as two parts, both rounded to nearest.
+__device__ inline void cut(const float (&x)[8], half8* hi, half8* lo) {
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const _Float16 h = static_cast<_Float16>(x[i]);
+    (*hi)[i] = h;
+    (*lo)[i] = static_cast<_Float16>(x[i] - static_cast<float>(h));
+  }
+}
+
+// The larger of the two halves of a wave, in both.
+__device__ inline float halves_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ inline float halves_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ inline floatx16 mfma(half8 a, half8 b, floatx16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ inline floatx16 mfma3(half8 ah, half8 al, half8 bh, half8 bl, floatx16 c) {
+  c = mfma(al, bh, c);
+  c = mfma(ah, bl, c);
+  return mfma(ah, bh, c);
+}
+
+// Fragments. A 32x32x16 product takes of its operands' rows (or columns) n and
+// terms k, in lane l, n = l % 32 and k = 8 (l / 32) + 0..7, and gives in lane l
+// column l % 32 and rows result_row(r, l / 32), r < 16. Rows that a later
+// product sums over are taken in the order in which results hold them:
+// registers 8u .. 8u + 7 of the lane are its eight terms of step u.
+__device__ inline int result_row(int r, int half) { return 8 * (r / 4) + 4 * half + r % 4; }
+
+// A block of 32 rows as fragments of a product over its columns: for each 16
+// columns the first parts, then the second.
+template <int NB>
+constexpr int kRowBytes = NB * 2 * 2 * kPart;
+// ... of a product over its rows: for each 32 columns and each 16 rows (in the
+// order of results) the first parts, then the second.
+template <int NB>
+constexpr int kColBytes = NB * 2 * 2 * kPart;
+
+// One block, x[row][column] in LDS (rows of kStride floats), times 2^e.
+template <int NB>
+constexpr int kStride = NB * 32 + 4;
+
+template <int NB>
+__device__ inline void write_rows(const float* x, float scale, char* out) {
+  for (int g = threadIdx.x; g < NB * 2 * 64; g += 256) {
+    const int t = g / 64, lane = g % 64;
+    const float* p = x + (lane % 32) * kStride<NB> + 16 * t + 8 * (lane / 32);
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = p[i] * scale;
+    half8 hi, lo;
+    cut(v, &hi, &lo);
+    *reinterpret_cast<half8*>(out + t * 2 * kPart + lane * 16) = hi;
+    *reinterpret_cast<half8*>(out + t * 2 * kPart + kPart + lane * 16) = lo;
+  }
+}
+
+template <int NB>
+__device__ inline void write_cols(const float* x, float scale, char* out) {
+  for (int g = threadIdx.x; g < NB * 2 * 64; g += 256) {
+    const int t = g / 64, lane = g % 64;  // t = 2 * (32 columns) + (16 rows)
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      v[i] = x[result_row(8 * (t % 2) + i, lane / 32) * kStride<NB> + 32 * (t / 2) + lane % 32] * scale;
+    half8 hi, lo;
+    cut(v, &hi, &lo);
+    *reinterpret_cast<half8*>(out + t * 2 * kPart + lane * 16) = hi;
+    *reinterpret_cast<half8*>(out + t * 2 * kPart + kPart + lane * 16) = lo;
+  }
+}
+
+// The largest of the 256 threads' values, in all of them. `shared`: 4 floats.
+__device__ inline float block_max(float x, float* shared) {
+  x = wave_max(x);
+  if (threadIdx.x % 64 == 0) shared[threadIdx.x / 64] = x;
+  __syncthreads();
+  x = fmaxf(fmaxf(shared[0], shared[1]), fmaxf(shared[2], shared[3]));
+  return x;
+}
+
+// A block of up to 32 rows of `rows` rows of D numbers into LDS, the rest 0;
+// the largest magnitude among this thread's.
+template <int NB>
+__device__ inline float load_block(const float* src, size_t stride, int rows, int D, float* x) {
+  float top = 0.f;
+  for (int n = threadIdx.x; n < kBlock * NB * 8; n += 256) {
+    const int row = n / (NB * 8), c = n % (NB * 8) * 4;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (row < rows) {
+      const float* p = src + row * stride + c;
+      if (D % 4 == 0) {
+        if (c < D) v = *reinterpret_cast<const float4*>(p);
+      } else {
+        if (c < D) v.x = p[0];
+        if (c + 1 < D) v.y = p[1];
+        if (c + 2 < D) v.z = p[2];
+        if (c + 3 < D) v.w = p[3];
+      }
+    }
+    // NaN counts as infinite: fmaxf would drop it.
+    const float m = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+    top = v.x + v.y + v.z + v.w == v.x + v.y + v.z + v.w ? fmaxf(top, m) : INFINITY;
+    *reinterpret_cast<float4*>(x + row * kStride<NB> + c) = v;
+  }
+  return top;
+}
+
+// Where a call's launches keep what they hand on. Per batch and key head and
+// block of 32 keys: the tile [K rows | V columns], and the two exponents.
+struct ForwardSpace {
+  int blocks;  // of keys, per batch and head
+  char* tiles;
+  int* exponents;
+};
+
+template <int NB>
+__device__ inline ForwardSpace forward_space(char* ws, int B, int Sk, int Hk) {
+  ForwardSpace f;
+  f.blocks = (Sk + kBlock - 1) / kBlock;
+  f.tiles = ws;
+  f.exponents = reinterpret_cast<int*>(ws + static_cast<size_t>(B) * Hk * f.blocks * (kRowBytes<NB> + kColBytes<NB>));
+  return f;
+}
+
+// Keys and values cut once per call: one workgroup per block and matrix.
+// Every query tile of a head reads them, so the main loop only copies.
+template <int NB>
+__device__ inline void pack_keys(const float* k, const float* v, const int* lengths, char* ws, int B, int Sk, int Hk,
+                                 int D) {
+  __shared__ float x[kBlock * kStride<NB>];
+  __shared__ float tops[4];
+  const ForwardSpace f = forward_space<NB>(ws, B, Sk, Hk);
+  const bool values = blockIdx.x % 2;
+  const size_t block = blockIdx.x / 2;  // (b, hk, kb)
+  const int kb = block % f.blocks, hk = block / f.blocks % Hk, b = block / f.blocks / Hk;
+  const int keys = lengths ? min(max(lengths[b], 0), Sk) : Sk;
+  if (kb * kBlock >= keys) return;
+  const size_t at = (static_cast<size_t>(b) * Sk + kb * kBlock) * Hk * D + static_cast<size_t>(hk) * D;
+  const float top = block_max(
+      load_block<NB>((values ? v : k) + at, static_cast<size_t>(Hk) * D, min(kBlock, keys - kb * kBlock), D, x), tops);
+  const int e = block_exponent(top);
+  const float scale = ldexpf(1.f, e);
+  char* tile = f.tiles + block * (kRowBytes<NB> + kColBytes<NB>);
+  if (values) write_cols<NB>(x, scale, tile + kRowBytes<NB>);
+  else write_rows<NB>(x, scale, tile);
+  if (threadIdx.x == 0) f.exponents[2 * block + values] = e;
+}
+
+// Copies `bytes` (a multiple of 4 KiB), contiguous, into LDS without passing
+// registers: each wave 1 KiB at a time.
+__device__ inline void copy_tile(const char* from, char* to, int bytes) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+  for (int at = wave * kPart; at < bytes; at += 4 * kPart)
+    __builtin_amdgcn_global_load_lds(
+        (const __attribute__((address_space(1))) void*)(from + at + lane * 16),
+        (__attribute__((address_space(3))) void*)(to + at), 16, 0, 0);
+}
+
+// The copies are in LDS, and every wave is done with what it read.
+__device__ inline void tile_barrier() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+
+// Scales of accumulators. Sums over rows meet blocks of one exponent after
+// another, and accumulators hold their sums times 2^(ref): ref follows the
+// blocks where they differ by more than kSlack, and results are multiplied
+// up or down, exactly. It stays within 60 of the least exponent met (of the
+// largest values), which keeps the sums finite.
+constexpr int kSlack = 4;
+struct RunningScale {
+  int ref = 0, least = 0;
+  bool any = false;
+  // Takes block exponent e; returns the power of two that accumulators have
+  // to be multiplied by (0: none), and leaves in *behind how far the block's
+  // operand is above ref (what the other operand makes up for).
+  __device__ int take(int e, int* behind) {
+    int change = 0;
+    if (!any) {
+      any = true;
+      ref = least = e;
+    } else if (e < ref || e > ref + kSlack) {
+      least = min(least, e);
+      const int to = min(e, least + 60);
+      change = to - ref;
+      ref = to;
+    }
+    *behind = e - ref;
+    return change;
+  }
+};
+
+// Probabilities are kept below 2^kLazy of 1 (the row's maximum follows only
+// where it grew by more), and times 2^kProbShift, less than 2^15, when cut.
+constexpr float kLazy = 2.f;
+constexpr int kProbShift = 13;
+
+// p[0..7] as two parts, cut off (not rounded: one instruction for two
+// numbers), the second from what the first leaves.
+__device__ inline void cut_probs(const float* p, half8* hi, half8* lo) {
+  typedef __fp16 fp16x2 __attribute__((ext_vector_type(2)));
+  union {
+    fp16x2 two[4];
+    half8 all;
+  } h, l;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    h.two[i] = __builtin_amdgcn_cvt_pkrtz(p[2 * i], p[2 * i + 1]);
+    l.two[i] = __builtin_amdgcn_cvt_pkrtz(p[2 * i] - static_cast<float>(h.two[i][0]),
+                                          p[2 * i + 1] - static_cast<float>(h.two[i][1]));
+  }
+  *hi = h.all;
+  *lo = l.all;
+}
+
+// Row l % 32 of this wave's 32 rows as the fragments of a product over its
+// columns, times sign 2^e with an exponent of the row's own.
+template <int NB>
+__device__ inline int row_fragments(const float* row, bool live, int D, float sign, half8 (&hi)[NB * 2],
+                                    half8 (&lo)[NB * 2]) {
+  const int half = threadIdx.x % 64 / 32;
+  float v[NB * 2][8];
+  float top = 0.f;
+#pragma unroll
+  for (int t = 0; t < NB * 2; t++) {
+    const int c = 16 * t + 8 * half;
+    if (D % 4 == 0) {
+#pragma unroll
+      for (int i = 0; i < 8; i += 4) {
+        const float4 x = live && c + i < D ? *reinterpret_cast<const float4*>(row + c + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+        v[t][i] = x.x;
+        v[t][i + 1] = x.y;
+        v[t][i + 2] = x.z;
+        v[t][i + 3] = x.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[t][i] = live && c + i < D ? row[c + i] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) top = v[t][i] == v[t][i] ? fmaxf(top, fabsf(v[t][i])) : INFINITY;
+  }
+  const int e = block_exponent(halves_max(top));
+  const float scale = ldexpf(sign, e);
+#pragma unroll
+  for (int t = 0; t < NB * 2; t++) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[t][i] *= scale;
+    cut(v[t], &hi[t], &lo[t]);
+  }
+  return e;
+}
+
+// 16 result registers of a 32-column group of row `row`: columns 32 n +
+// result_row(r, half), times scale 2^e (the power last: alone it may be out of
+// range).
+__device__ inline void store_columns(float* row, int n, int half, int D, const floatx16& o, float scale, int e) {
+#pragma unroll
+  for (int g = 0; g < 4; g++) {
+    const int c = 32 * n + 8 * g + 4 * half;
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = ldexpf(o[4 * g + i] * scale, e);
+    if (D % 4 == 0) {
+      if (c < D) *reinterpret_cast<float4*>(row + c) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (c + i < D) row[c + i] = v[i];
+    }
+  }
+}
+
+// A workgroup: 128 queries of one head, 32 a wave; all keys, 32 at a time.
+// S^T = K Q^T, so that a lane holds 16 scores of one query: the row's maximum
+// and sum cost one exchange between the wave's halves, and the probabilities
+// are in registers what O^T += V^T P^T takes as its second operand.
+template <int NB>
+__device__ inline void forward_tiles(float* __restrict__ y, const float* __restrict__ q, float* __restrict__ stats,
+                                     const int* __restrict__ lengths, char* __restrict__ ws, int B, int Sq, int Sk,
+                                     int Hq, int Hk, int D, int causal, float scale) {
+  constexpr int kTile = kRowBytes<NB> + kColBytes<NB>;
+  __shared__ __attribute__((aligned(1024))) char lds[2][kTile];
+  const ForwardSpace f = forward_space<NB>(ws, B, Sk, Hk);
+  const int tiles = (Sq + 127) / 128;
+  // The last queries see the most keys: first.
+  const int qt = tiles - 1 - static_cast<int>(blockIdx.x % tiles), h = blockIdx.x / tiles % Hq, b = blockIdx.x / tiles / Hq;
+  const int hk = h / (Hq / Hk);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, half = lane / 32;
+  const int i = qt * 128 + wave * 32 + lane % 32;  // this lane's query
+  const bool live = i < Sq;
+  const int keys = lengths ? min(max(lengths[b], 0), Sk) : Sk;
+  // Keys that the last query of the workgroup, of the wave, and this lane's see.
+  auto seen_by = [&](int row) { return causal ? max(0, min(keys, row + Sk - Sq + 1)) : keys; };
+  const int block_end = (seen_by(min(Sq, qt * 128 + 128) - 1) + kBlock - 1) / kBlock;
+  const int wave_last = min(Sq, qt * 128 + wave * 32 + 32) - 1;
+  const int wave_end = wave_last >= qt * 128 + wave * 32 ? (seen_by(wave_last) + kBlock - 1) / kBlock : 0;
+  const int wave_full = seen_by(qt * 128 + wave * 32) / kBlock;  // blocks that every query of the wave sees whole
+  const int seen = live ? seen_by(i) : 0;
+
+  const size_t head = static_cast<size_t>(b) * Hk + hk;
+  const char* tile = f.tiles + head * f.blocks * kTile;
+  const int* exponents = f.exponents + 2 * head * f.blocks;
+  if (block_end > 0) copy_tile(tile, lds[0], kTile);
+
+  half8 qh[NB * 2], ql[NB * 2];
+  const int eq = row_fragments<NB>(q + (static_cast<size_t>(b) * Sq + min(i, Sq - 1)) * Hq * D + static_cast<size_t>(h) * D, live,
+                                   D, scale < 0.f ? -1.f : 1.f, qh, ql);
+  const float factor = fabsf(scale) * kLog2e;
+  float m = -INFINITY, l = 0.f;
+  floatx16 o[NB] = {};
+  RunningScale vs;
+  tile_barrier();
+  for (int kb = 0; kb < block_end; kb++) {
+    if (kb + 1 < block_end) copy_tile(tile + static_cast<size_t>(kb + 1) * kTile, lds[(kb + 1) % 2], kTile);
+    if (kb < wave_end) {
+      const char* t = lds[kb % 2] + lane * 16;
+      const int ek = exponents[2 * kb], ev = exponents[2 * kb + 1];
+      floatx16 s = {};
+#pragma unroll
+      for (int n = 0; n < NB * 2; n++)
+        s = mfma3(*reinterpret_cast<const half8*>(t + n * 2 * kPart), *reinterpret_cast<const half8*>(t + n * 2 * kPart + kPart),
+                  qh[n], ql[n], s);
+      float fac = ldexpf(factor, -(eq + ek));
+      if (kb >= wave_full) {
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[r] = kb * kBlock + result_row(r, half) < seen ? s[r] * fac : -INFINITY;
+        fac = 1.f;
+      }
+      float top = s[0];
+#pragma unroll
+      for (int r = 1; r < 16; r++) top = fmaxf(top, s[r]);
+      top = halves_max(top) * fac;
+      int behind;
+      const int change = vs.take(ev, &behind);
+      if (change != 0) {
+#pragma unroll
+        for (int n = 0; n < NB; n++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) o[n][r] = ldexpf(o[n][r], change);
+      }
+      if (__any(top > m + kLazy)) {
+        const float to = top > m + kLazy ? top : m;
+        const float old = to == -INFINITY ? 1.f : exp2f(m - to);
+        m = to;
+        l *= old;
+#pragma unroll
+        for (int n = 0; n < NB; n++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) o[n][r] *= old;
+      }
+      // p 2^(13 - behind): what the block's values are above ref goes off here.
+      const float base = static_cast<float>(kProbShift - behind) - (m == -INFINITY ? 0.f : m);
+      float sum = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], fac, base));
+        sum += s[r];
+      }
+      l += ldexpf(sum, behind - kProbShift);
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        float p[8];
+#pragma unroll
+        for (int r = 0; r < 8; r++) p[r] = s[8 * u + r];
+        half8 ph, pl;
+        cut_probs(p, &ph, &pl);
+        const char* vt = t + kRowBytes<NB> + u * 2 * kPart;
+#pragma unroll
+        for (int n = 0; n < NB; n++)
+          o[n] = mfma3(*reinterpret_cast<const half8*>(vt + n * 4 * kPart),
+                       *reinterpret_cast<const half8*>(vt + n * 4 * kPart + kPart), ph, pl, o[n]);
+      }
+    }
+    tile_barrier();
+  }
+  l = halves_sum(l);
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  if (!live) return;
+  float* row = y + (static_cast<size_t>(b) * Sq + i) * Hq * D + static_cast<size_t>(h) * D;
+#pragma unroll
+  for (int n = 0; n < NB; n++) store_columns(row, n, half, D, o[n], inv, -kProbShift - vs.ref);
+  if (half == 0) {
+    const size_t at = (static_cast<size_t>(b) * Hq + h) * Sq + i;
+    stats[at] = m == -INFINITY ? 0.f : m;
+    stats[static_cast<size_t>(B) * Hq * Sq + at] = inv;
+  }
+}
+
 }  // namespace
+
+#define FG_ATTENTION(NB)                                                                                              \
+  extern "C" __global__ void __launch_bounds__(256) fg_attention_pack_##NB(                                           \
+      float* y, const float* q, const float* k, const float* v, float* stats, const int* lengths, char* ws, int B,    \
+      int Sq, int Sk, int Hq, int Hk, int D, int causal, float scale) {                                               \
+    pack_keys<NB>(k, v, lengths, ws, B, Sk, Hk, D);                                                                   \
+  }                                                                                                                   \
+  extern "C" __global__ void __launch_bounds__(256, 2) fg_attention_tiles_##NB(                                       \
+      float* y, const float* q, const float* k, const float* v, float* stats, const int* lengths, char* ws, int B,    \
+      int Sq, int Sk, int Hq, int Hk, int D, int causal, float scale) {                                               \
+    forward_tiles<NB>(y, q, stats, lengths, ws, B, Sq, Sk, Hq, Hk, D, causal, scale);                                 \
+  }
+
+FG_ATTENTION(1)
+FG_ATTENTION(2)
+FG_ATTENTION(3)
+FG_ATTENTION(4)
 
 // One wave per query row.
 extern "C" __global__ void __launch_bounds__(256)
     fg_attention(float* __restrict__ y, const float* __restrict__ q, const float* __restrict__ k,
-                 const float* __restrict__ v, float* __restrict__ stats, const int* __restrict__ lengths, int B, int Sq,
+                 const float* __restrict__ v, float* __restrict__ stats, const int* __restrict__ lengths, char* ws, int B, int Sq,
                  int Sk, int Hq, int Hk, int D, int causal, float scale) {
   __shared__ float probs[4][64];
   const Shape s{B, Sq, Sk, Hq, Hk, D, causal};

@@ -199,11 +199,20 @@ RenderedKernel render_attention(const UOp& call, bool grad) {
   RenderedKernel rk;
   set_image(rk, fg_image_attention, fg_image_attention_end);
   const uint64_t q_rows = static_cast<uint64_t>(batch * heads * sq), k_rows = static_cast<uint64_t>(batch * kv_heads * sk);
+  const int64_t dim = p[5], nb = (dim + 31) / 32, k_blocks = (sk + 31) / 32;
   if (!grad) {
     rk.kind = "attention";
-    rk.launches = {launch("fg_attention", (q_rows + 3) / 4, 256, "attention")};
+    if (sq * (heads / kv_heads) < 8) {
+      rk.launches = {launch("fg_attention", (q_rows + 3) / 4, 256, "attention")};
+    } else {
+      const uint64_t blocks = static_cast<uint64_t>(batch * kv_heads * k_blocks);
+      rk.workspace_bytes = blocks * static_cast<uint64_t>(nb * 8192 + 8);
+      rk.launches = {launch("fg_attention_pack_" + std::to_string(nb), 2 * blocks, 256, "attention"),
+                     launch("fg_attention_tiles_" + std::to_string(nb),
+                            static_cast<uint64_t>(batch * heads * ((sq + 127) / 128)), 256, "attention")};
+    }
     rk.call_args = {CallArg::slot(0), CallArg::slot(1), CallArg::slot(2), CallArg::slot(3), CallArg::slot(lengths ? 5 : 4),
-                    lengths ? CallArg::slot(4) : CallArg::null()};
+                    lengths ? CallArg::slot(4) : CallArg::null(), CallArg::workspace()};
     rk.side_outputs = {lengths ? 5 : 4};
   } else {
     rk.kind = "attention_grad";
