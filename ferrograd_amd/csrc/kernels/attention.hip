@@ -293,9 +293,9 @@ __device__ inline void cut_probs(const float* p, half8* hi, half8* lo) {
 }
 
 // Row l % 32 of this wave's 32 rows as the fragments of a product over its
-// columns, times sign 2^e with an exponent of the row's own.
+// columns, times `times` and sign 2^e with an exponent of the row's own.
 template <int NB>
-__device__ inline int row_fragments(const float* row, bool live, int D, float sign, half8 (&hi)[NB * 2],
+__device__ inline int row_fragments(const float* row, bool live, int D, float sign, float times, half8 (&hi)[NB * 2],
                                     half8 (&lo)[NB * 2]) {
   const int half = threadIdx.x % 64 / 32;
   float v[NB * 2][8];
@@ -317,7 +317,10 @@ __device__ inline int row_fragments(const float* row, bool live, int D, float si
       for (int i = 0; i < 8; i++) v[t][i] = live && c + i < D ? row[c + i] : 0.f;
     }
 #pragma unroll
-    for (int i = 0; i < 8; i++) top = v[t][i] == v[t][i] ? fmaxf(top, fabsf(v[t][i])) : INFINITY;
+    for (int i = 0; i < 8; i++) {
+      v[t][i] *= times;
+      top = v[t][i] == v[t][i] ? fmaxf(top, fabsf(v[t][i])) : INFINITY;
+    }
   }
   const int e = block_exponent(halves_max(top));
   const float scale = ldexpf(sign, e);
@@ -384,7 +387,7 @@ __device__ inline void forward_tiles(float* __restrict__ y, const float* __restr
 
   half8 qh[NB * 2], ql[NB * 2];
   const int eq = row_fragments<NB>(q + (static_cast<size_t>(b) * Sq + min(i, Sq - 1)) * Hq * D + static_cast<size_t>(h) * D, live,
-                                   D, scale < 0.f ? -1.f : 1.f, qh, ql);
+                                   D, scale < 0.f ? -1.f : 1.f, 1.f, qh, ql);
   const float factor = fabsf(scale) * kLog2e;
   float m = -INFINITY, l = 0.f;
   floatx16 o[NB] = {};
@@ -466,6 +469,387 @@ __device__ inline void forward_tiles(float* __restrict__ y, const float* __restr
   }
 }
 
+// ── gradients ───────────────────────────────────────────────────────────────
+// With r_i = 1 / (row i's sum), p_ij = exp2(S_ij log2 e - m_i) (r_i p_ij is the
+// probability), g'_i = r_i g_i and delta_i = g'_i . y_i:
+//   dv_j = sum_i p_ij g'_i
+//   ds_ij = p_ij (g'_i . v_j - delta_i)
+//   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i
+// so that both p and ds are cut where their largest is, whatever the row's sum.
+// |g'_i . v_j - delta_i| is at most twice the largest |g'_i| (of the block)
+// times the largest |v_j| (of the head), and p less than 2^kLazy: ds times
+// 2^(kScoreShift - the norms' exponents) is less than 2^15.
+constexpr int kScoreShift = 12;  // 15, less kLazy and one for the twice
+
+// The gradients' workspace. Per batch and key head and block of 32 keys: the
+// tile [K rows | V rows | K columns], and the exponents of K, V and of V's
+// largest row norm; per batch and query head and block of 32 queries: the tile
+// [Q rows | G rows | Q columns | G columns | m | delta] (G = g'), and the
+// exponents of Q, G and of G's largest row norm; then dk and dv of each part.
+template <int NB>
+constexpr int kKeyTile = 2 * kRowBytes<NB> + kColBytes<NB>;
+template <int NB>
+constexpr int kQueryTile = 2 * kRowBytes<NB> + 2 * kColBytes<NB> + 256;
+
+struct GradSpace {
+  int k_blocks, q_blocks;
+  char *k_tiles, *q_tiles;
+  int *k_exponents, *q_exponents;
+  float* parts;
+};
+
+template <int NB>
+__device__ inline GradSpace grad_space(char* ws, const Shape& s) {
+  GradSpace g;
+  g.k_blocks = (s.sk + kBlock - 1) / kBlock;
+  g.q_blocks = (s.sq + kBlock - 1) / kBlock;
+  const size_t nk = static_cast<size_t>(s.b) * s.hk * g.k_blocks, nq = static_cast<size_t>(s.b) * s.hq * g.q_blocks;
+  g.k_tiles = ws;
+  g.q_tiles = ws + nk * kKeyTile<NB>;
+  g.k_exponents = reinterpret_cast<int*>(g.q_tiles + nq * kQueryTile<NB>);
+  g.q_exponents = g.k_exponents + 4 * nk;
+  g.parts = reinterpret_cast<float*>(g.q_exponents + 4 * nq);
+  return g;
+}
+
+// The power of two above a norm, from the largest sum of squares of a block's
+// numbers times 2^e.
+__device__ inline int norm_exponent(float squares, int e) {
+  if (!(squares > 0.f)) return -120;
+  if (!(squares < INFINITY)) return 0;
+  int k;
+  frexpf(squares, &k);
+  return max((k + 1) / 2 - e, -120);
+}
+
+// 2^a for any a, saturating.
+__device__ inline float power(int a) { return ldexpf(1.f, a); }
+
+// Keys, values, queries and gradients cut once per call, one workgroup per
+// block and matrix.
+template <int NB>
+__device__ inline void pack_grad(const float* __restrict__ q, const float* __restrict__ k, const float* __restrict__ v,
+                                 const float* __restrict__ y, const float* __restrict__ g,
+                                 const float* __restrict__ stats, const int* __restrict__ lengths,
+                                 char* __restrict__ ws, const Shape& s) {
+  __shared__ float x[kBlock * kStride<NB>];
+  __shared__ float tops[4];
+  const GradSpace f = grad_space<NB>(ws, s);
+  const size_t nk = static_cast<size_t>(s.b) * s.hk * f.k_blocks;
+  const bool second = blockIdx.x % 2;  // V, or G
+  size_t block = blockIdx.x / 2;
+  const bool of_keys = block < nk;
+  if (!of_keys) block -= nk;
+  const int blocks = of_keys ? f.k_blocks : f.q_blocks, heads = of_keys ? s.hk : s.hq, n = of_keys ? s.sk : s.sq;
+  const int at = block % blocks * kBlock, h = block / blocks % heads, b = block / blocks / heads;
+  const int rows = of_keys ? key_count(s, lengths, b) : n;
+  if (at >= rows) return;
+  const size_t stride = static_cast<size_t>(heads) * s.d;
+  const size_t first = (static_cast<size_t>(b) * n + at) * stride + static_cast<size_t>(h) * s.d;
+  const float* src = (of_keys ? (second ? v : k) : (second ? g : q)) + first;
+  float top = load_block<NB>(src, stride, min(kBlock, rows - at), s.d, x);
+  char* tile = of_keys ? f.k_tiles + block * kKeyTile<NB> : f.q_tiles + block * kQueryTile<NB>;
+  int* exponents = (of_keys ? f.k_exponents : f.q_exponents) + 4 * block;
+  const int row = threadIdx.x / 8, part = threadIdx.x % 8;  // eight threads a row, for its sums
+  if (!of_keys && second) {
+    // g' and delta; rows past the last query stay 0.
+    __syncthreads();
+    const size_t rows_all = static_cast<size_t>(s.b) * s.hq * s.sq;
+    const size_t stat = (static_cast<size_t>(b) * s.hq + h) * s.sq + at + row;
+    const bool live = at + row < s.sq;
+    const float inv = live ? stats[rows_all + stat] : 0.f;
+    float delta = 0.f;
+    top = 0.f;
+    for (int c = part; c < s.d; c += 8) {
+      const float gx = x[row * kStride<NB> + c] * inv;
+      x[row * kStride<NB> + c] = gx;
+      top = gx == gx ? fmaxf(top, fabsf(gx)) : INFINITY;
+      if (live) delta += gx * y[first + row * stride + c];
+    }
+    delta += __shfl_xor(delta, 1);
+    delta += __shfl_xor(delta, 2);
+    delta += __shfl_xor(delta, 4);
+    float* tail = reinterpret_cast<float*>(tile + kQueryTile<NB> - 256);
+    if (part == 0) {
+      tail[row] = live ? stats[stat] : 0.f;
+      tail[32 + row] = delta;
+    }
+  }
+  const int e = block_exponent(block_max(top, tops));
+  const float scale = power(e);
+  if (second) {
+    float squares = 0.f;
+    for (int c = part; c < s.d; c += 8) {
+      const float t = x[row * kStride<NB> + c] * scale;
+      squares += t * t;
+    }
+    squares += __shfl_xor(squares, 1);
+    squares += __shfl_xor(squares, 2);
+    squares += __shfl_xor(squares, 4);
+    __syncthreads();  // tops is read
+    squares = block_max(squares, tops);
+    if (threadIdx.x == 0) exponents[2] = norm_exponent(squares, e);
+  }
+  if (threadIdx.x == 0) exponents[second] = e;
+  write_rows<NB>(x, scale, tile + (second ? kRowBytes<NB> : 0));
+  if (of_keys && !second) write_cols<NB>(x, scale, tile + 2 * kRowBytes<NB>);
+  if (!of_keys) write_cols<NB>(x, scale, tile + 2 * kRowBytes<NB> + (second ? kColBytes<NB> : 0));
+}
+
+// The exponent above the norms of every value row of a head.
+__device__ inline int values_norm(const int* exponents, int blocks) {
+  int top = -120;
+  for (int n = threadIdx.x % 64; n < blocks; n += 64) top = max(top, exponents[4 * n + 2]);
+  for (int d = 32; d > 0; d /= 2) top = max(top, __shfl_xor(top, d));
+  return __builtin_amdgcn_readfirstlane(top);
+}
+
+__device__ inline int clamp_power(int a) { return min(max(a, -120), 120); }
+
+// dq. A workgroup: 128 queries of one head, 32 a wave, over all keys; scores
+// and their gradients transposed as in the forward pass.
+template <int NB>
+__device__ inline void query_grads(float* __restrict__ dq, const float* __restrict__ q, const float* __restrict__ g,
+                                   const float* __restrict__ stats, const int* __restrict__ lengths,
+                                   char* __restrict__ ws, const Shape& s, float scale) {
+  constexpr int kTile = kKeyTile<NB>;
+  __shared__ __attribute__((aligned(1024))) char lds[2][kTile];
+  const GradSpace f = grad_space<NB>(ws, s);
+  const int tiles = (s.sq + 127) / 128;
+  const int qt = tiles - 1 - static_cast<int>(blockIdx.x % tiles), h = blockIdx.x / tiles % s.hq, b = blockIdx.x / tiles / s.hq;
+  const int hk = h / (s.hq / s.hk);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, half = lane / 32;
+  const int first = qt * 128 + wave * 32, i = first + lane % 32;
+  const bool live = i < s.sq, wave_live = first < s.sq;
+  const int keys = key_count(s, lengths, b);
+  const int block_end = (visible(s, keys, min(s.sq, qt * 128 + 128) - 1) + kBlock - 1) / kBlock;
+  const int wave_end = wave_live ? (visible(s, keys, min(s.sq, first + 32) - 1) + kBlock - 1) / kBlock : 0;
+  const int wave_full = visible(s, keys, first) / kBlock;
+  const int seen = live ? visible(s, keys, i) : 0;
+
+  const size_t head = static_cast<size_t>(b) * s.hk + hk;
+  const char* tile = f.k_tiles + head * f.k_blocks * kTile;
+  const int* exponents = f.k_exponents + 4 * head * f.k_blocks;
+  if (block_end > 0) copy_tile(tile, lds[0], kTile);
+
+  const size_t at = (static_cast<size_t>(b) * s.sq + min(i, s.sq - 1)) * s.hq * s.d + static_cast<size_t>(h) * s.d;
+  const size_t stat = (static_cast<size_t>(b) * s.hq + h) * s.sq + min(i, s.sq - 1);
+  const size_t q_block = (static_cast<size_t>(b) * s.hq + h) * f.q_blocks + min(first / kBlock, f.q_blocks - 1);
+  const float inv = live ? stats[static_cast<size_t>(s.b) * s.hq * s.sq + stat] : 0.f;
+  const float m = live ? stats[stat] : 0.f;
+  const float delta = reinterpret_cast<const float*>(f.q_tiles + (q_block + 1) * kQueryTile<NB> - 256)[32 + lane % 32];
+  half8 qh[NB * 2], ql[NB * 2], gh[NB * 2], gl[NB * 2];
+  const int eq = row_fragments<NB>(q + at, live, s.d, scale < 0.f ? -1.f : 1.f, 1.f, qh, ql);
+  const int eg = row_fragments<NB>(g + at, live, s.d, 1.f, inv, gh, gl);
+  const int shift = clamp_power(kScoreShift - f.q_exponents[4 * q_block + 2] - values_norm(exponents, (keys + kBlock - 1) / kBlock));
+  const float factor = fabsf(scale) * kLog2e;
+  floatx16 o[NB] = {};
+  RunningScale ks;
+  tile_barrier();
+  for (int kb = 0; kb < block_end; kb++) {
+    if (kb + 1 < block_end) copy_tile(tile + static_cast<size_t>(kb + 1) * kTile, lds[(kb + 1) % 2], kTile);
+    if (kb < wave_end) {
+      const char* t = lds[kb % 2] + lane * 16;
+      const int ek = exponents[4 * kb], ev = exponents[4 * kb + 1];
+      floatx16 x = {}, dp = {};
+#pragma unroll
+      for (int n = 0; n < NB * 2; n++)
+        x = mfma3(*reinterpret_cast<const half8*>(t + n * 2 * kPart), *reinterpret_cast<const half8*>(t + n * 2 * kPart + kPart),
+                  qh[n], ql[n], x);
+#pragma unroll
+      for (int n = 0; n < NB * 2; n++)
+        dp = mfma3(*reinterpret_cast<const half8*>(t + kRowBytes<NB> + n * 2 * kPart),
+                   *reinterpret_cast<const half8*>(t + kRowBytes<NB> + n * 2 * kPart + kPart), gh[n], gl[n], dp);
+      int behind;
+      const int change = ks.take(ek, &behind);
+      if (change != 0) {
+#pragma unroll
+        for (int n = 0; n < NB; n++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) o[n][r] = ldexpf(o[n][r], change);
+      }
+      const float fac = ldexpf(factor, -(eq + ek));
+      const float of_dp = power(shift - behind - eg - ev), of_delta = delta * power(shift - behind);
+      const bool whole = kb < wave_full;
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(x[r], fac, -m));
+        dp[r] = p * fmaf(dp[r], of_dp, -of_delta);
+        if (!whole) dp[r] = kb * kBlock + result_row(r, half) < seen ? dp[r] : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        float d[8];
+#pragma unroll
+        for (int r = 0; r < 8; r++) d[r] = dp[8 * u + r];
+        half8 dh, dl;
+        cut_probs(d, &dh, &dl);
+        const char* kt = t + 2 * kRowBytes<NB> + u * 2 * kPart;
+#pragma unroll
+        for (int n = 0; n < NB; n++)
+          o[n] = mfma3(*reinterpret_cast<const half8*>(kt + n * 4 * kPart),
+                       *reinterpret_cast<const half8*>(kt + n * 4 * kPart + kPart), dh, dl, o[n]);
+      }
+    }
+    tile_barrier();
+  }
+  if (!live) return;
+#pragma unroll
+  for (int n = 0; n < NB; n++) store_columns(dq + at, n, half, s.d, o[n], scale, -shift - ks.ref);
+}
+
+// dk and dv. A workgroup: 128 keys of one key head, 32 a wave, over its part
+// of the query blocks that see any of them, head after head of those that read
+// the key head. Scores are not transposed here: a lane holds 16 queries of one
+// key, which is what dv^T += G^T P and dk^T += Q^T dS take.
+template <int NB>
+__device__ inline void key_grads(float* __restrict__ dk, float* __restrict__ dv, const float* __restrict__ k,
+                                 const float* __restrict__ v, const int* __restrict__ lengths, char* __restrict__ ws,
+                                 const Shape& s, float scale, int parts) {
+  constexpr int kTile = kQueryTile<NB>;
+  __shared__ __attribute__((aligned(1024))) char lds[2][kTile];
+  const GradSpace f = grad_space<NB>(ws, s);
+  // The first keys are seen by the most queries: first.
+  const unsigned inner = static_cast<unsigned>(s.b * s.hk) * parts;
+  const int kt = blockIdx.x / inner, part = blockIdx.x % inner % parts;
+  const int hk = blockIdx.x % inner / parts % s.hk, b = blockIdx.x % inner / parts / s.hk, group = s.hq / s.hk;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, half = lane / 32;
+  const int first = kt * 128 + wave * 32, j = first + lane % 32;
+  const int keys = key_count(s, lengths, b), offset = s.sk - s.sq;
+  const bool live = j < keys;
+  // Query blocks that see a key of the workgroup: those from q_first on.
+  const int q_first = s.causal ? max(0, kt * 128 - offset) / kBlock : 0;
+  const int per_head = kt * 128 < keys ? max(0, f.q_blocks - q_first) : 0, units = per_head * group;
+  const int begin = static_cast<int>(static_cast<long long>(units) * part / parts);
+  const int end = static_cast<int>(static_cast<long long>(units) * (part + 1) / parts);
+
+  const size_t q_head = (static_cast<size_t>(b) * s.hq + static_cast<size_t>(hk) * group) * f.q_blocks;
+  auto unit_block = [&](int u) { return q_head + static_cast<size_t>(u / per_head) * f.q_blocks + q_first + u % per_head; };
+  auto copy_unit = [&](int u, char* to) {
+    const char* from = f.q_tiles + unit_block(u) * kTile;
+    copy_tile(from, to, kTile - 256);
+    if (wave == 0 && lane < 16)
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + kTile - 256 + lane * 16),
+                                       (__attribute__((address_space(3))) void*)(to + kTile - 256), 16, 0, 0);
+  };
+  if (begin < end) copy_unit(begin, lds[0]);
+
+  const size_t at = (static_cast<size_t>(b) * s.sk + min(j, s.sk - 1)) * s.hk * s.d + static_cast<size_t>(hk) * s.d;
+  half8 kh[NB * 2], kl[NB * 2], vh[NB * 2], vl[NB * 2];
+  const int ek = row_fragments<NB>(k + at, live, s.d, scale < 0.f ? -1.f : 1.f, 1.f, kh, kl);
+  const int ev = row_fragments<NB>(v + at, live, s.d, 1.f, 1.f, vh, vl);
+  const int norm = values_norm(f.k_exponents + 4 * (static_cast<size_t>(b) * s.hk + hk) * f.k_blocks, (keys + kBlock - 1) / kBlock);
+  const float factor = fabsf(scale) * kLog2e;
+  floatx16 ok[NB] = {}, ov[NB] = {};
+  RunningScale qs, gs;
+  tile_barrier();
+  for (int u = begin; u < end; u++) {
+    const char* now = lds[(u - begin) % 2];
+    if (u + 1 < end) copy_unit(u + 1, lds[(u + 1 - begin) % 2]);
+    const int q0 = (q_first + u % per_head) * kBlock;
+    // Whether any of the block's queries sees any of the wave's keys.
+    if (first < keys && (!s.causal || first <= q0 + kBlock - 1 + offset)) {
+      const char* t = now + lane * 16;
+      const int* exponents = f.q_exponents + 4 * unit_block(u);
+      const int eq = exponents[0], eg = exponents[1], shift = clamp_power(kScoreShift - exponents[2] - norm);
+      floatx16 x = {}, dp = {};
+#pragma unroll
+      for (int n = 0; n < NB * 2; n++)
+        x = mfma3(*reinterpret_cast<const half8*>(t + n * 2 * kPart), *reinterpret_cast<const half8*>(t + n * 2 * kPart + kPart),
+                  kh[n], kl[n], x);
+#pragma unroll
+      for (int n = 0; n < NB * 2; n++)
+        dp = mfma3(*reinterpret_cast<const half8*>(t + kRowBytes<NB> + n * 2 * kPart),
+                   *reinterpret_cast<const half8*>(t + kRowBytes<NB> + n * 2 * kPart + kPart), vh[n], vl[n], dp);
+      int q_behind, g_behind;
+      const int q_change = qs.take(shift + eq, &q_behind), g_change = gs.take(eg, &g_behind);
+      if (q_change != 0) {
+#pragma unroll
+        for (int n = 0; n < NB; n++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) ok[n][r] = ldexpf(ok[n][r], q_change);
+      }
+      if (g_change != 0) {
+#pragma unroll
+        for (int n = 0; n < NB; n++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) ov[n][r] = ldexpf(ov[n][r], g_change);
+      }
+      const float fac = ldexpf(factor, -(eq + ek));
+      // p carries 2^up; what multiplies it into ds takes that off again.
+      const int up = kProbShift - g_behind, off = shift - q_behind - up;
+      const float of_dp = power(off - eg - ev), of_delta = power(off);
+      const bool whole = !s.causal || first + 31 <= q0 + offset;
+      const float* tail = reinterpret_cast<const float*>(now + kTile - 256);
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        const float4 mm = *reinterpret_cast<const float4*>(tail + 8 * c + 4 * half);
+        const float4 dd = *reinterpret_cast<const float4*>(tail + 32 + 8 * c + 4 * half);
+        const float m4[4] = {mm.x, mm.y, mm.z, mm.w}, d4[4] = {dd.x, dd.y, dd.z, dd.w};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int r = 4 * c + e;
+          float p = __builtin_amdgcn_exp2f(fmaf(x[r], fac, static_cast<float>(up) - m4[e]));
+          if (!whole) p = j <= q0 + result_row(r, half) + offset ? p : 0.f;
+          x[r] = p;
+          dp[r] = p * fmaf(dp[r], of_dp, -d4[e] * of_delta);
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < 2; w++) {
+        float p[8], d[8];
+#pragma unroll
+        for (int r = 0; r < 8; r++) {
+          p[r] = x[8 * w + r];
+          d[r] = dp[8 * w + r];
+        }
+        half8 ph, pl, dh, dl;
+        cut_probs(p, &ph, &pl);
+        cut_probs(d, &dh, &dl);
+        const char* qt = t + 2 * kRowBytes<NB> + w * 2 * kPart;
+        const char* gt = qt + kColBytes<NB>;
+#pragma unroll
+        for (int n = 0; n < NB; n++) {
+          ov[n] = mfma3(*reinterpret_cast<const half8*>(gt + n * 4 * kPart),
+                        *reinterpret_cast<const half8*>(gt + n * 4 * kPart + kPart), ph, pl, ov[n]);
+          ok[n] = mfma3(*reinterpret_cast<const half8*>(qt + n * 4 * kPart),
+                        *reinterpret_cast<const half8*>(qt + n * 4 * kPart + kPart), dh, dl, ok[n]);
+        }
+      }
+    }
+    tile_barrier();
+  }
+  if (j >= s.sk) return;
+  const size_t all = static_cast<size_t>(s.b) * s.sk * s.hk * s.d;
+  if (parts > 1) {
+    dk = f.parts + 2 * all * part;
+    dv = dk + all;
+  }
+  // Keys past the length take no gradient (their lanes' sums are not of it).
+  if (!live) {
+#pragma unroll
+    for (int n = 0; n < NB; n++) {
+      ok[n] = floatx16{};
+      ov[n] = floatx16{};
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < NB; n++) {
+    store_columns(dk + at, n, half, s.d, ok[n], scale, -qs.ref);
+    store_columns(dv + at, n, half, s.d, ov[n], 1.f, -kProbShift - gs.ref);
+  }
+}
+
+// dk and dv from their parts, in order.
+__device__ inline void sum_parts(float* __restrict__ dk, float* __restrict__ dv, const float* __restrict__ partial,
+                                 size_t n, int parts) {
+  for (size_t e = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x; e < 2 * n; e += static_cast<size_t>(gridDim.x) * 256) {
+    float t = 0.f;
+    for (int part = 0; part < parts; part++) t += partial[2 * n * part + e];
+    (e < n ? dk : dv - n)[e] = t;
+  }
+}
+
 }  // namespace
 
 #define FG_ATTENTION(NB)                                                                                              \
@@ -478,6 +862,31 @@ __device__ inline void forward_tiles(float* __restrict__ y, const float* __restr
       float* y, const float* q, const float* k, const float* v, float* stats, const int* lengths, char* ws, int B,    \
       int Sq, int Sk, int Hq, int Hk, int D, int causal, float scale) {                                               \
     forward_tiles<NB>(y, q, stats, lengths, ws, B, Sq, Sk, Hq, Hk, D, causal, scale);                                 \
+  }                                                                                                                   \
+  extern "C" __global__ void __launch_bounds__(256) fg_attention_grad_pack_##NB(                                      \
+      float* dq, const float* q, const float* k, const float* v, const float* y, const float* g, const float* stats,  \
+      float* dk, float* dv, const int* lengths, char* ws, int parts, int B, int Sq, int Sk, int Hq, int Hk, int D,    \
+      int causal, float scale) {                                                                                      \
+    pack_grad<NB>(q, k, v, y, g, stats, lengths, ws, Shape{B, Sq, Sk, Hq, Hk, D, causal});                            \
+  }                                                                                                                   \
+  extern "C" __global__ void __launch_bounds__(256, (NB) < 3 ? 2 : 1) fg_attention_grad_q_##NB(                       \
+      float* dq, const float* q, const float* k, const float* v, const float* y, const float* g, const float* stats,  \
+      float* dk, float* dv, const int* lengths, char* ws, int parts, int B, int Sq, int Sk, int Hq, int Hk, int D,    \
+      int causal, float scale) {                                                                                      \
+    query_grads<NB>(dq, q, g, stats, lengths, ws, Shape{B, Sq, Sk, Hq, Hk, D, causal}, scale);                        \
+  }                                                                                                                   \
+  extern "C" __global__ void __launch_bounds__(256, (NB) < 3 ? 2 : 1) fg_attention_grad_kv_##NB(                      \
+      float* dq, const float* q, const float* k, const float* v, const float* y, const float* g, const float* stats,  \
+      float* dk, float* dv, const int* lengths, char* ws, int parts, int B, int Sq, int Sk, int Hq, int Hk, int D,    \
+      int causal, float scale) {                                                                                      \
+    key_grads<NB>(dk, dv, k, v, lengths, ws, Shape{B, Sq, Sk, Hq, Hk, D, causal}, scale, parts);                      \
+  }                                                                                                                   \
+  extern "C" __global__ void __launch_bounds__(256) fg_attention_grad_sum_##NB(                                       \
+      float* dq, const float* q, const float* k, const float* v, const float* y, const float* g, const float* stats,  \
+      float* dk, float* dv, const int* lengths, char* ws, int parts, int B, int Sq, int Sk, int Hq, int Hk, int D,    \
+      int causal, float scale) {                                                                                      \
+    const GradSpace f = grad_space<NB>(ws, Shape{B, Sq, Sk, Hq, Hk, D, causal});                                      \
+    sum_parts(dk, dv, f.parts, static_cast<size_t>(B) * Sk * Hk * D, parts);                                          \
   }
 
 FG_ATTENTION(1)
@@ -529,97 +938,4 @@ extern "C" __global__ void __launch_bounds__(256)
     stats[row] = m == -INFINITY ? 0.f : m;
     stats[static_cast<size_t>(B) * Hq * Sq + row] = inv;
   }
-}
-
-// dq: one wave per query row.
-extern "C" __global__ void __launch_bounds__(256)
-    fg_attention_dq(float* __restrict__ dq, const float* __restrict__ q, const float* __restrict__ k,
-                    const float* __restrict__ v, const float* __restrict__ y, const float* __restrict__ g,
-                    const float* __restrict__ stats, float* __restrict__ dk, float* __restrict__ dv,
-                    const int* __restrict__ lengths, int B, int Sq, int Sk, int Hq, int Hk, int D, int causal,
-                    float scale) {
-  __shared__ float probs[4][64];
-  const Shape s{B, Sq, Sk, Hq, Hk, D, causal};
-  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-  const size_t rows = static_cast<size_t>(B) * Hq * Sq, row = static_cast<size_t>(blockIdx.x) * 4 + wave;
-  const bool live = row < rows;
-  const int i = live ? row % Sq : 0, h = live ? row / Sq % Hq : 0, b = live ? row / Sq / Hq : 0;
-  const int hk = h / (Hq / Hk);
-  const int seen = live ? visible(s, key_count(s, lengths, b), i) : 0;
-  const size_t at = (static_cast<size_t>(b) * Sq + i) * Hq * D + static_cast<size_t>(h) * D;
-  const float* kb = k + static_cast<size_t>(b) * Sk * Hk * D + static_cast<size_t>(hk) * D;
-  const float* vb = v + static_cast<size_t>(b) * Sk * Hk * D + static_cast<size_t>(hk) * D;
-  const size_t stride = static_cast<size_t>(Hk) * D;
-  const float m = live ? stats[row] : 0.f, inv = live ? stats[rows + row] : 0.f;
-  const float delta = dot(g + at, y + at, D);
-  float o[2] = {0.f, 0.f};
-  for (int j0 = 0; j0 < seen; j0 += 64) {
-    const int j = j0 + lane;
-    float ds = 0.f;
-    if (j < seen) {
-      const float p = exp2f(dot(q + at, kb + j * stride, D) * (scale * kLog2e) - m) * inv;
-      ds = p * (dot(g + at, vb + j * stride, D) - delta) * scale;
-    }
-    probs[wave][lane] = ds;
-    __builtin_amdgcn_wave_barrier();
-    for (int t = 0; t < 2; t++) {
-      const int d = lane + 64 * t;
-      if (d >= D) continue;
-      for (int n = 0; n < min(64, seen - j0); n++) o[t] += probs[wave][n] * kb[(j0 + n) * stride + d];
-    }
-    __builtin_amdgcn_wave_barrier();
-  }
-  if (!live) return;
-  for (int t = 0; t < 2; t++)
-    if (lane + 64 * t < D) dq[at + lane + 64 * t] = o[t];
-}
-
-// dk, dv: one wave per key row, over the queries of every head that reads it.
-extern "C" __global__ void __launch_bounds__(256)
-    fg_attention_dkv(float* __restrict__ dq, const float* __restrict__ q, const float* __restrict__ k,
-                     const float* __restrict__ v, const float* __restrict__ y, const float* __restrict__ g,
-                     const float* __restrict__ stats, float* __restrict__ dk, float* __restrict__ dv,
-                     const int* __restrict__ lengths, int B, int Sq, int Sk, int Hq, int Hk, int D, int causal,
-                     float scale) {
-  __shared__ float probs[4][64], grads[4][64];
-  const Shape s{B, Sq, Sk, Hq, Hk, D, causal};
-  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-  const size_t rows = static_cast<size_t>(B) * Hq * Sq, row = static_cast<size_t>(blockIdx.x) * 4 + wave;
-  if (row >= static_cast<size_t>(B) * Hk * Sk) return;
-  const int j = row % Sk, hk = row / Sk % Hk, b = row / Sk / Hk;
-  const int keys = key_count(s, lengths, b), group = Hq / Hk;
-  const size_t at = (static_cast<size_t>(b) * Sk + j) * Hk * D + static_cast<size_t>(hk) * D;
-  const size_t stride = static_cast<size_t>(Hq) * D;
-  float ok[2] = {0.f, 0.f}, ov[2] = {0.f, 0.f};
-  const int first = causal ? max(0, j - (Sk - Sq)) : 0;
-  for (int h = hk * group; h < (hk + 1) * group && j < keys; h++) {
-    const size_t base = static_cast<size_t>(b) * Sq * Hq * D + static_cast<size_t>(h) * D;
-    const float* st = stats + (static_cast<size_t>(b) * Hq + h) * Sq;
-    for (int i0 = first; i0 < Sq; i0 += 64) {
-      const int i = i0 + lane;
-      float p = 0.f, ds = 0.f;
-      if (i < Sq) {
-        const size_t qi = base + i * stride;
-        p = exp2f(dot(q + qi, k + at, D) * (scale * kLog2e) - st[i]) * st[rows + i];
-        ds = p * (dot(g + qi, v + at, D) - dot(g + qi, y + qi, D)) * scale;
-      }
-      probs[wave][lane] = p;
-      grads[wave][lane] = ds;
-      __builtin_amdgcn_wave_barrier();
-      for (int t = 0; t < 2; t++) {
-        const int d = lane + 64 * t;
-        if (d >= D) continue;
-        for (int n = 0; n < min(64, Sq - i0); n++) {
-          ov[t] += probs[wave][n] * g[base + (i0 + n) * stride + d];
-          ok[t] += grads[wave][n] * q[base + (i0 + n) * stride + d];
-        }
-      }
-      __builtin_amdgcn_wave_barrier();
-    }
-  }
-  for (int t = 0; t < 2; t++)
-    if (lane + 64 * t < D) {
-      dk[at + lane + 64 * t] = ok[t];
-      dv[at + lane + 64 * t] = ov[t];
-    }
 }

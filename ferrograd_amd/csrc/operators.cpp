@@ -198,7 +198,7 @@ RenderedKernel render_attention(const UOp& call, bool grad) {
   const bool lengths = p[7] != 0;
   RenderedKernel rk;
   set_image(rk, fg_image_attention, fg_image_attention_end);
-  const uint64_t q_rows = static_cast<uint64_t>(batch * heads * sq), k_rows = static_cast<uint64_t>(batch * kv_heads * sk);
+  const uint64_t q_rows = static_cast<uint64_t>(batch * heads * sq);
   const int64_t dim = p[5], nb = (dim + 31) / 32, k_blocks = (sk + 31) / 32;
   if (!grad) {
     rk.kind = "attention";
@@ -216,13 +216,28 @@ RenderedKernel render_attention(const UOp& call, bool grad) {
     rk.side_outputs = {lengths ? 5 : 4};
   } else {
     rk.kind = "attention_grad";
-    rk.launches = {launch("fg_attention_dq", (q_rows + 3) / 4, 256, "attention"),
-                   launch("fg_attention_dkv", (k_rows + 3) / 4, 256, "attention")};
+    const std::string nbs = "_" + std::to_string(nb);
+    const int64_t q_blocks = (sq + 31) / 32, group = heads / kv_heads;
+    const uint64_t nk = static_cast<uint64_t>(batch * kv_heads * k_blocks), nq = static_cast<uint64_t>(batch * heads * q_blocks);
+    // Workgroups of 128 keys, each key tile's queries in parts until there are
+    // 1024, of at least 4 query blocks.
+    const int64_t tiles = batch * kv_heads * ((sk + 127) / 128);
+    const int64_t parts = std::max<int64_t>(1, std::min((1024 + tiles - 1) / tiles, q_blocks * group / 4));
+    const uint64_t all = static_cast<uint64_t>(batch * sk * kv_heads * dim);
+    rk.workspace_bytes = nk * static_cast<uint64_t>(nb * 12288 + 16) + nq * static_cast<uint64_t>(nb * 16384 + 256 + 16) +
+                         (parts > 1 ? 8 * all * static_cast<uint64_t>(parts) : 0);
+    rk.launches = {launch("fg_attention_grad_pack" + nbs, 2 * (nk + nq), 256, "attention"),
+                   launch("fg_attention_grad_kv" + nbs, static_cast<uint64_t>(tiles * parts), 256, "attention"),
+                   launch("fg_attention_grad_q" + nbs, static_cast<uint64_t>(batch * heads * ((sq + 127) / 128)), 256, "attention")};
+    if (parts > 1)
+      rk.launches.push_back(launch("fg_attention_grad_sum" + nbs, std::min<uint64_t>((2 * all + 255) / 256, 8192), 256, "attention"));
     const int dk = lengths ? 8 : 7;
     for (int i = 0; i < 7; i++) rk.call_args.push_back(CallArg::slot(i));
     rk.call_args.push_back(CallArg::slot(dk));
     rk.call_args.push_back(CallArg::slot(dk + 1));
     rk.call_args.push_back(lengths ? CallArg::slot(7) : CallArg::null());
+    rk.call_args.push_back(CallArg::workspace());
+    rk.call_args.push_back(CallArg::i32(parts));
     rk.side_outputs = {dk, dk + 1};
   }
   for (int i = 0; i < 7; i++) rk.call_args.push_back(CallArg::i32(p[static_cast<size_t>(i)]));
