@@ -114,6 +114,10 @@ constexpr int kRowBytes = NB * 2 * 2 * kPart;
 template <int NB>
 constexpr int kColBytes = NB * 2 * 2 * kPart;
 
+// A tile ends with a page of numbers of its blocks: read from LDS like the
+// rest. (A load of one inside the loop would wait for the copies before it.)
+constexpr int kTail = kPart;
+
 // One block, x[row][column] in LDS (rows of kStride floats), times 2^e.
 template <int NB>
 constexpr int kStride = NB * 32 + 4;
@@ -157,25 +161,38 @@ __device__ inline float block_max(float x, float* shared) {
   return x;
 }
 
+// Columns c .. c + 3 of a row of D, 0 past its end. Every lane loads from the
+// row whatever it keeps: loads under conditions would wait for one another.
+__device__ inline float4 load4(const float* row, int c, int D) {
+  float4 v;
+  if (D % 4 == 0) {
+    v = *reinterpret_cast<const float4*>(row + (c < D ? c : 0));
+    if (c >= D) v = make_float4(0.f, 0.f, 0.f, 0.f);
+  } else {
+    v = make_float4(row[c < D ? c : 0], row[c + 1 < D ? c + 1 : 0], row[c + 2 < D ? c + 2 : 0], row[c + 3 < D ? c + 3 : 0]);
+    if (c >= D) v.x = 0.f;
+    if (c + 1 >= D) v.y = 0.f;
+    if (c + 2 >= D) v.z = 0.f;
+    if (c + 3 >= D) v.w = 0.f;
+  }
+  return v;
+}
+
 // A block of up to 32 rows of `rows` rows of D numbers into LDS, the rest 0;
 // the largest magnitude among this thread's.
 template <int NB>
 __device__ inline float load_block(const float* src, size_t stride, int rows, int D, float* x) {
   float top = 0.f;
-  for (int n = threadIdx.x; n < kBlock * NB * 8; n += 256) {
-    const int row = n / (NB * 8), c = n % (NB * 8) * 4;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (row < rows) {
-      const float* p = src + row * stride + c;
-      if (D % 4 == 0) {
-        if (c < D) v = *reinterpret_cast<const float4*>(p);
-      } else {
-        if (c < D) v.x = p[0];
-        if (c + 1 < D) v.y = p[1];
-        if (c + 2 < D) v.z = p[2];
-        if (c + 3 < D) v.w = p[3];
-      }
-    }
+  float4 loaded[NB];
+#pragma unroll
+  for (int n = 0; n < NB; n++) {
+    const int at = n * 256 + threadIdx.x;
+    loaded[n] = load4(src + min(at / (NB * 8), rows - 1) * stride, at % (NB * 8) * 4, D);
+  }
+#pragma unroll
+  for (int n = 0; n < NB; n++) {
+    const int at = n * 256 + threadIdx.x, row = at / (NB * 8), c = at % (NB * 8) * 4;
+    const float4 v = row < rows ? loaded[n] : make_float4(0.f, 0.f, 0.f, 0.f);
     // NaN counts as infinite: fmaxf would drop it.
     const float m = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
     top = v.x + v.y + v.z + v.w == v.x + v.y + v.z + v.w ? fmaxf(top, m) : INFINITY;
@@ -184,22 +201,10 @@ __device__ inline float load_block(const float* src, size_t stride, int rows, in
   return top;
 }
 
-// Where a call's launches keep what they hand on. Per batch and key head and
-// block of 32 keys: the tile [K rows | V columns], and the two exponents.
-struct ForwardSpace {
-  int blocks;  // of keys, per batch and head
-  char* tiles;
-  int* exponents;
-};
-
+// The forward pass's workspace: per batch and key head and block of 32 keys the
+// tile [K rows | V columns | exponents of K, V].
 template <int NB>
-__device__ inline ForwardSpace forward_space(char* ws, int B, int Sk, int Hk) {
-  ForwardSpace f;
-  f.blocks = (Sk + kBlock - 1) / kBlock;
-  f.tiles = ws;
-  f.exponents = reinterpret_cast<int*>(ws + static_cast<size_t>(B) * Hk * f.blocks * (kRowBytes<NB> + kColBytes<NB>));
-  return f;
-}
+constexpr int kForwardTile = kRowBytes<NB> + kColBytes<NB> + kTail;
 
 // Keys and values cut once per call: one workgroup per block and matrix.
 // Every query tile of a head reads them, so the main loop only copies.
@@ -208,10 +213,10 @@ __device__ inline void pack_keys(const float* k, const float* v, const int* leng
                                  int D) {
   __shared__ float x[kBlock * kStride<NB>];
   __shared__ float tops[4];
-  const ForwardSpace f = forward_space<NB>(ws, B, Sk, Hk);
+  const int blocks = (Sk + kBlock - 1) / kBlock;
   const bool values = blockIdx.x % 2;
   const size_t block = blockIdx.x / 2;  // (b, hk, kb)
-  const int kb = block % f.blocks, hk = block / f.blocks % Hk, b = block / f.blocks / Hk;
+  const int kb = block % blocks, hk = block / blocks % Hk, b = block / blocks / Hk;
   const int keys = lengths ? min(max(lengths[b], 0), Sk) : Sk;
   if (kb * kBlock >= keys) return;
   const size_t at = (static_cast<size_t>(b) * Sk + kb * kBlock) * Hk * D + static_cast<size_t>(hk) * D;
@@ -219,21 +224,25 @@ __device__ inline void pack_keys(const float* k, const float* v, const int* leng
       load_block<NB>((values ? v : k) + at, static_cast<size_t>(Hk) * D, min(kBlock, keys - kb * kBlock), D, x), tops);
   const int e = block_exponent(top);
   const float scale = ldexpf(1.f, e);
-  char* tile = f.tiles + block * (kRowBytes<NB> + kColBytes<NB>);
+  char* tile = ws + block * kForwardTile<NB>;
   if (values) write_cols<NB>(x, scale, tile + kRowBytes<NB>);
   else write_rows<NB>(x, scale, tile);
-  if (threadIdx.x == 0) f.exponents[2 * block + values] = e;
+  if (threadIdx.x == 0) reinterpret_cast<int*>(tile + kRowBytes<NB> + kColBytes<NB>)[values] = e;
 }
 
-// Copies `bytes` (a multiple of 4 KiB), contiguous, into LDS without passing
+// Copies `Bytes` (a multiple of 1 KiB), contiguous, into LDS without passing
 // registers: each wave 1 KiB at a time.
-__device__ inline void copy_tile(const char* from, char* to, int bytes) {
+template <int Bytes>
+__device__ inline void copy_tile(const char* from, char* to) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
-  for (int at = wave * kPart; at < bytes; at += 4 * kPart)
+#pragma unroll
+  for (int at = wave * kPart; at < Bytes; at += 4 * kPart)
     __builtin_amdgcn_global_load_lds(
         (const __attribute__((address_space(1))) void*)(from + at + lane * 16),
         (__attribute__((address_space(3))) void*)(to + at), 16, 0, 0);
 }
+
+__device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // The copies are in LDS, and every wave is done with what it read.
 __device__ inline void tile_barrier() {
@@ -292,7 +301,8 @@ __device__ inline void cut_probs(const float* p, half8* hi, half8* lo) {
   *lo = l.all;
 }
 
-// Row l % 32 of this wave's 32 rows as the fragments of a product over its
+// Row l % 32 of this wave's 32 rows (a row to load from, also where it is not
+// live and counts as 0) as the fragments of a product over its
 // columns, times `times` and sign 2^e with an exponent of the row's own.
 template <int NB>
 __device__ inline int row_fragments(const float* row, bool live, int D, float sign, float times, half8 (&hi)[NB * 2],
@@ -301,27 +311,22 @@ __device__ inline int row_fragments(const float* row, bool live, int D, float si
   float v[NB * 2][8];
   float top = 0.f;
 #pragma unroll
-  for (int t = 0; t < NB * 2; t++) {
-    const int c = 16 * t + 8 * half;
-    if (D % 4 == 0) {
+  for (int t = 0; t < NB * 2; t++)
 #pragma unroll
-      for (int i = 0; i < 8; i += 4) {
-        const float4 x = live && c + i < D ? *reinterpret_cast<const float4*>(row + c + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-        v[t][i] = x.x;
-        v[t][i + 1] = x.y;
-        v[t][i + 2] = x.z;
-        v[t][i + 3] = x.w;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; i++) v[t][i] = live && c + i < D ? row[c + i] : 0.f;
+    for (int i = 0; i < 8; i += 4) {
+      const float4 x = load4(row, 16 * t + 8 * half + i, D);
+      v[t][i] = x.x;
+      v[t][i + 1] = x.y;
+      v[t][i + 2] = x.z;
+      v[t][i + 3] = x.w;
     }
+#pragma unroll
+  for (int t = 0; t < NB * 2; t++)
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      v[t][i] *= times;
+      v[t][i] = live ? v[t][i] * times : 0.f;
       top = v[t][i] == v[t][i] ? fmaxf(top, fabsf(v[t][i])) : INFINITY;
     }
-  }
   const int e = block_exponent(halves_max(top));
   const float scale = ldexpf(sign, e);
 #pragma unroll
@@ -353,6 +358,20 @@ __device__ inline void store_columns(float* row, int n, int half, int D, const f
   }
 }
 
+// Which 128 queries, head and batch a workgroup takes. The last queries of
+// every head come first: with `causal` they see the most keys, and what is
+// left for the end is small. Workgroups go to the 8 chiplets in turn, so
+// where the heads allow it each chiplet gets heads next to each other, which
+// share keys in its cache.
+__device__ inline void query_tile(const Shape& s, int* qt, int* h, int* b) {
+  const unsigned heads = static_cast<unsigned>(s.b) * s.hq, tiles = (s.sq + 127) / 128;
+  unsigned head = blockIdx.x % heads;
+  if (heads % 8 == 0) head = head % 8 * (heads / 8) + head / 8;
+  *qt = tiles - 1 - blockIdx.x / heads;
+  *h = head % s.hq;
+  *b = head / s.hq;
+}
+
 // A workgroup: 128 queries of one head, 32 a wave; all keys, 32 at a time.
 // S^T = K Q^T, so that a lane holds 16 scores of one query: the row's maximum
 // and sum cost one exchange between the wave's halves, and the probabilities
@@ -361,12 +380,13 @@ template <int NB>
 __device__ inline void forward_tiles(float* __restrict__ y, const float* __restrict__ q, float* __restrict__ stats,
                                      const int* __restrict__ lengths, char* __restrict__ ws, int B, int Sq, int Sk,
                                      int Hq, int Hk, int D, int causal, float scale) {
-  constexpr int kTile = kRowBytes<NB> + kColBytes<NB>;
-  __shared__ __attribute__((aligned(1024))) char lds[2][kTile];
-  const ForwardSpace f = forward_space<NB>(ws, B, Sk, Hk);
-  const int tiles = (Sq + 127) / 128;
-  // The last queries see the most keys: first.
-  const int qt = tiles - 1 - static_cast<int>(blockIdx.x % tiles), h = blockIdx.x / tiles % Hq, b = blockIdx.x / tiles / Hq;
+  constexpr int kTile = kForwardTile<NB>;
+  // Two buffers of their own, and a loop written out twice: the compiler then
+  // knows that what a step reads is not what its copies write, and does not
+  // wait for them first.
+  __shared__ __attribute__((aligned(1024))) char even[kTile], odd[kTile];
+  int qt, h, b;
+  query_tile(Shape{B, Sq, Sk, Hq, Hk, D, causal}, &qt, &h, &b);
   const int hk = h / (Hq / Hk);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, half = lane / 32;
   const int i = qt * 128 + wave * 32 + lane % 32;  // this lane's query
@@ -381,9 +401,8 @@ __device__ inline void forward_tiles(float* __restrict__ y, const float* __restr
   const int seen = live ? seen_by(i) : 0;
 
   const size_t head = static_cast<size_t>(b) * Hk + hk;
-  const char* tile = f.tiles + head * f.blocks * kTile;
-  const int* exponents = f.exponents + 2 * head * f.blocks;
-  if (block_end > 0) copy_tile(tile, lds[0], kTile);
+  const char* tile = ws + head * ((Sk + kBlock - 1) / kBlock) * kTile;
+  if (block_end > 0) copy_tile<kTile>(tile, even);
 
   half8 qh[NB * 2], ql[NB * 2];
   const int eq = row_fragments<NB>(q + (static_cast<size_t>(b) * Sq + min(i, Sq - 1)) * Hq * D + static_cast<size_t>(h) * D, live,
@@ -393,11 +412,12 @@ __device__ inline void forward_tiles(float* __restrict__ y, const float* __restr
   floatx16 o[NB] = {};
   RunningScale vs;
   tile_barrier();
-  for (int kb = 0; kb < block_end; kb++) {
-    if (kb + 1 < block_end) copy_tile(tile + static_cast<size_t>(kb + 1) * kTile, lds[(kb + 1) % 2], kTile);
+  auto step = [&](const char* now, char* next, int kb) {
+    if (kb + 1 < block_end) copy_tile<kTile>(tile + static_cast<size_t>(kb + 1) * kTile, next);
     if (kb < wave_end) {
-      const char* t = lds[kb % 2] + lane * 16;
-      const int ek = exponents[2 * kb], ev = exponents[2 * kb + 1];
+      const char* t = now + lane * 16;
+      const int* tail = reinterpret_cast<const int*>(now + kTile - kTail);
+      const int ek = uniform(tail[0]), ev = uniform(tail[1]);
       floatx16 s = {};
 #pragma unroll
       for (int n = 0; n < NB * 2; n++)
@@ -455,6 +475,10 @@ __device__ inline void forward_tiles(float* __restrict__ y, const float* __restr
       }
     }
     tile_barrier();
+  };
+  for (int kb = 0; kb < block_end; kb += 2) {
+    step(even, odd, kb);
+    if (kb + 1 < block_end) step(odd, even, kb + 1);
   }
   l = halves_sum(l);
   const float inv = l > 0.f ? 1.f / l : 0.f;
@@ -482,19 +506,20 @@ __device__ inline void forward_tiles(float* __restrict__ y, const float* __restr
 constexpr int kScoreShift = 12;  // 15, less kLazy and one for the twice
 
 // The gradients' workspace. Per batch and key head and block of 32 keys: the
-// tile [K rows | V rows | K columns], and the exponents of K, V and of V's
-// largest row norm; per batch and query head and block of 32 queries: the tile
-// [Q rows | G rows | Q columns | G columns | m | delta] (G = g'), and the
-// exponents of Q, G and of G's largest row norm; then dk and dv of each part.
+// tile [K rows | V rows | K columns | exponents of K, V]; per batch and query
+// head and block of 32 queries: the tile [Q rows | G rows | Q columns | G
+// columns | m, delta of each row, exponents of Q, G and of G's largest row
+// norm] (G = g'); then the exponents of the key blocks' largest row norms of V;
+// then dk and dv of each part.
 template <int NB>
-constexpr int kKeyTile = 2 * kRowBytes<NB> + kColBytes<NB>;
+constexpr int kKeyTile = 2 * kRowBytes<NB> + kColBytes<NB> + kTail;
 template <int NB>
-constexpr int kQueryTile = 2 * kRowBytes<NB> + 2 * kColBytes<NB> + 256;
+constexpr int kQueryTile = 2 * kRowBytes<NB> + 2 * kColBytes<NB> + kTail;
 
 struct GradSpace {
   int k_blocks, q_blocks;
   char *k_tiles, *q_tiles;
-  int *k_exponents, *q_exponents;
+  int* norms;
   float* parts;
 };
 
@@ -506,9 +531,8 @@ __device__ inline GradSpace grad_space(char* ws, const Shape& s) {
   const size_t nk = static_cast<size_t>(s.b) * s.hk * g.k_blocks, nq = static_cast<size_t>(s.b) * s.hq * g.q_blocks;
   g.k_tiles = ws;
   g.q_tiles = ws + nk * kKeyTile<NB>;
-  g.k_exponents = reinterpret_cast<int*>(g.q_tiles + nq * kQueryTile<NB>);
-  g.q_exponents = g.k_exponents + 4 * nk;
-  g.parts = reinterpret_cast<float*>(g.q_exponents + 4 * nq);
+  g.norms = reinterpret_cast<int*>(g.q_tiles + nq * kQueryTile<NB>);
+  g.parts = reinterpret_cast<float*>(g.norms + (nk + 3) / 4 * 4);
   return g;
 }
 
@@ -549,7 +573,8 @@ __device__ inline void pack_grad(const float* __restrict__ q, const float* __res
   const float* src = (of_keys ? (second ? v : k) : (second ? g : q)) + first;
   float top = load_block<NB>(src, stride, min(kBlock, rows - at), s.d, x);
   char* tile = of_keys ? f.k_tiles + block * kKeyTile<NB> : f.q_tiles + block * kQueryTile<NB>;
-  int* exponents = (of_keys ? f.k_exponents : f.q_exponents) + 4 * block;
+  char* tail = tile + (of_keys ? kKeyTile<NB> : kQueryTile<NB>) - kTail;
+  int* exponents = reinterpret_cast<int*>(tail) + (of_keys ? 0 : 64);
   const int row = threadIdx.x / 8, part = threadIdx.x % 8;  // eight threads a row, for its sums
   if (!of_keys && second) {
     // g' and delta; rows past the last query stay 0.
@@ -569,10 +594,9 @@ __device__ inline void pack_grad(const float* __restrict__ q, const float* __res
     delta += __shfl_xor(delta, 1);
     delta += __shfl_xor(delta, 2);
     delta += __shfl_xor(delta, 4);
-    float* tail = reinterpret_cast<float*>(tile + kQueryTile<NB> - 256);
     if (part == 0) {
-      tail[row] = live ? stats[stat] : 0.f;
-      tail[32 + row] = delta;
+      reinterpret_cast<float*>(tail)[row] = live ? stats[stat] : 0.f;
+      reinterpret_cast<float*>(tail)[32 + row] = delta;
     }
   }
   const int e = block_exponent(block_max(top, tops));
@@ -588,7 +612,7 @@ __device__ inline void pack_grad(const float* __restrict__ q, const float* __res
     squares += __shfl_xor(squares, 4);
     __syncthreads();  // tops is read
     squares = block_max(squares, tops);
-    if (threadIdx.x == 0) exponents[2] = norm_exponent(squares, e);
+    if (threadIdx.x == 0) *(of_keys ? f.norms + block : exponents + 2) = norm_exponent(squares, e);
   }
   if (threadIdx.x == 0) exponents[second] = e;
   write_rows<NB>(x, scale, tile + (second ? kRowBytes<NB> : 0));
@@ -597,9 +621,9 @@ __device__ inline void pack_grad(const float* __restrict__ q, const float* __res
 }
 
 // The exponent above the norms of every value row of a head.
-__device__ inline int values_norm(const int* exponents, int blocks) {
+__device__ inline int values_norm(const int* norms, int blocks) {
   int top = -120;
-  for (int n = threadIdx.x % 64; n < blocks; n += 64) top = max(top, exponents[4 * n + 2]);
+  for (int n = threadIdx.x % 64; n < blocks; n += 64) top = max(top, norms[n]);
   for (int d = 32; d > 0; d /= 2) top = max(top, __shfl_xor(top, d));
   return __builtin_amdgcn_readfirstlane(top);
 }
@@ -613,10 +637,10 @@ __device__ inline void query_grads(float* __restrict__ dq, const float* __restri
                                    const float* __restrict__ stats, const int* __restrict__ lengths,
                                    char* __restrict__ ws, const Shape& s, float scale) {
   constexpr int kTile = kKeyTile<NB>;
-  __shared__ __attribute__((aligned(1024))) char lds[2][kTile];
+  __shared__ __attribute__((aligned(1024))) char even[kTile], odd[kTile];
   const GradSpace f = grad_space<NB>(ws, s);
-  const int tiles = (s.sq + 127) / 128;
-  const int qt = tiles - 1 - static_cast<int>(blockIdx.x % tiles), h = blockIdx.x / tiles % s.hq, b = blockIdx.x / tiles / s.hq;
+  int qt, h, b;
+  query_tile(s, &qt, &h, &b);
   const int hk = h / (s.hq / s.hk);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, half = lane / 32;
   const int first = qt * 128 + wave * 32, i = first + lane % 32;
@@ -629,28 +653,30 @@ __device__ inline void query_grads(float* __restrict__ dq, const float* __restri
 
   const size_t head = static_cast<size_t>(b) * s.hk + hk;
   const char* tile = f.k_tiles + head * f.k_blocks * kTile;
-  const int* exponents = f.k_exponents + 4 * head * f.k_blocks;
-  if (block_end > 0) copy_tile(tile, lds[0], kTile);
+  if (block_end > 0) copy_tile<kTile>(tile, even);
 
   const size_t at = (static_cast<size_t>(b) * s.sq + min(i, s.sq - 1)) * s.hq * s.d + static_cast<size_t>(h) * s.d;
   const size_t stat = (static_cast<size_t>(b) * s.hq + h) * s.sq + min(i, s.sq - 1);
   const size_t q_block = (static_cast<size_t>(b) * s.hq + h) * f.q_blocks + min(first / kBlock, f.q_blocks - 1);
   const float inv = live ? stats[static_cast<size_t>(s.b) * s.hq * s.sq + stat] : 0.f;
   const float m = live ? stats[stat] : 0.f;
-  const float delta = reinterpret_cast<const float*>(f.q_tiles + (q_block + 1) * kQueryTile<NB> - 256)[32 + lane % 32];
+  const char* q_tail = f.q_tiles + (q_block + 1) * kQueryTile<NB> - kTail;
+  const float delta = reinterpret_cast<const float*>(q_tail)[32 + lane % 32];
   half8 qh[NB * 2], ql[NB * 2], gh[NB * 2], gl[NB * 2];
   const int eq = row_fragments<NB>(q + at, live, s.d, scale < 0.f ? -1.f : 1.f, 1.f, qh, ql);
   const int eg = row_fragments<NB>(g + at, live, s.d, 1.f, inv, gh, gl);
-  const int shift = clamp_power(kScoreShift - f.q_exponents[4 * q_block + 2] - values_norm(exponents, (keys + kBlock - 1) / kBlock));
+  const int shift = uniform(clamp_power(kScoreShift - reinterpret_cast<const int*>(q_tail)[66] -
+                                        values_norm(f.norms + head * f.k_blocks, (keys + kBlock - 1) / kBlock)));
   const float factor = fabsf(scale) * kLog2e;
   floatx16 o[NB] = {};
   RunningScale ks;
   tile_barrier();
-  for (int kb = 0; kb < block_end; kb++) {
-    if (kb + 1 < block_end) copy_tile(tile + static_cast<size_t>(kb + 1) * kTile, lds[(kb + 1) % 2], kTile);
+  auto step = [&](const char* now, char* next, int kb) {
+    if (kb + 1 < block_end) copy_tile<kTile>(tile + static_cast<size_t>(kb + 1) * kTile, next);
     if (kb < wave_end) {
-      const char* t = lds[kb % 2] + lane * 16;
-      const int ek = exponents[4 * kb], ev = exponents[4 * kb + 1];
+      const char* t = now + lane * 16;
+      const int* tail = reinterpret_cast<const int*>(now + kTile - kTail);
+      const int ek = uniform(tail[0]), ev = uniform(tail[1]);
       floatx16 x = {}, dp = {};
 #pragma unroll
       for (int n = 0; n < NB * 2; n++)
@@ -692,6 +718,10 @@ __device__ inline void query_grads(float* __restrict__ dq, const float* __restri
       }
     }
     tile_barrier();
+  };
+  for (int kb = 0; kb < block_end; kb += 2) {
+    step(even, odd, kb);
+    if (kb + 1 < block_end) step(odd, even, kb + 1);
   }
   if (!live) return;
 #pragma unroll
@@ -707,7 +737,7 @@ __device__ inline void key_grads(float* __restrict__ dk, float* __restrict__ dv,
                                  const float* __restrict__ v, const int* __restrict__ lengths, char* __restrict__ ws,
                                  const Shape& s, float scale, int parts) {
   constexpr int kTile = kQueryTile<NB>;
-  __shared__ __attribute__((aligned(1024))) char lds[2][kTile];
+  __shared__ __attribute__((aligned(1024))) char even[kTile], odd[kTile];
   const GradSpace f = grad_space<NB>(ws, s);
   // The first keys are seen by the most queries: first.
   const unsigned inner = static_cast<unsigned>(s.b * s.hk) * parts;
@@ -725,33 +755,27 @@ __device__ inline void key_grads(float* __restrict__ dk, float* __restrict__ dv,
 
   const size_t q_head = (static_cast<size_t>(b) * s.hq + static_cast<size_t>(hk) * group) * f.q_blocks;
   auto unit_block = [&](int u) { return q_head + static_cast<size_t>(u / per_head) * f.q_blocks + q_first + u % per_head; };
-  auto copy_unit = [&](int u, char* to) {
-    const char* from = f.q_tiles + unit_block(u) * kTile;
-    copy_tile(from, to, kTile - 256);
-    if (wave == 0 && lane < 16)
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + kTile - 256 + lane * 16),
-                                       (__attribute__((address_space(3))) void*)(to + kTile - 256), 16, 0, 0);
-  };
-  if (begin < end) copy_unit(begin, lds[0]);
+  auto copy_unit = [&](int u, char* to) { copy_tile<kTile>(f.q_tiles + unit_block(u) * kTile, to); };
+  if (begin < end) copy_unit(begin, even);
 
   const size_t at = (static_cast<size_t>(b) * s.sk + min(j, s.sk - 1)) * s.hk * s.d + static_cast<size_t>(hk) * s.d;
   half8 kh[NB * 2], kl[NB * 2], vh[NB * 2], vl[NB * 2];
   const int ek = row_fragments<NB>(k + at, live, s.d, scale < 0.f ? -1.f : 1.f, 1.f, kh, kl);
   const int ev = row_fragments<NB>(v + at, live, s.d, 1.f, 1.f, vh, vl);
-  const int norm = values_norm(f.k_exponents + 4 * (static_cast<size_t>(b) * s.hk + hk) * f.k_blocks, (keys + kBlock - 1) / kBlock);
+  const int norm = values_norm(f.norms + (static_cast<size_t>(b) * s.hk + hk) * f.k_blocks, (keys + kBlock - 1) / kBlock);
   const float factor = fabsf(scale) * kLog2e;
   floatx16 ok[NB] = {}, ov[NB] = {};
   RunningScale qs, gs;
   tile_barrier();
-  for (int u = begin; u < end; u++) {
-    const char* now = lds[(u - begin) % 2];
-    if (u + 1 < end) copy_unit(u + 1, lds[(u + 1 - begin) % 2]);
+  auto step = [&](const char* now, char* next, int u) {
+    if (u + 1 < end) copy_unit(u + 1, next);
     const int q0 = (q_first + u % per_head) * kBlock;
     // Whether any of the block's queries sees any of the wave's keys.
     if (first < keys && (!s.causal || first <= q0 + kBlock - 1 + offset)) {
       const char* t = now + lane * 16;
-      const int* exponents = f.q_exponents + 4 * unit_block(u);
-      const int eq = exponents[0], eg = exponents[1], shift = clamp_power(kScoreShift - exponents[2] - norm);
+      const float* tail = reinterpret_cast<const float*>(now + kTile - kTail);
+      const int* exponents = reinterpret_cast<const int*>(tail) + 64;
+      const int eq = uniform(exponents[0]), eg = uniform(exponents[1]), shift = clamp_power(kScoreShift - uniform(exponents[2]) - norm);
       floatx16 x = {}, dp = {};
 #pragma unroll
       for (int n = 0; n < NB * 2; n++)
@@ -780,7 +804,6 @@ __device__ inline void key_grads(float* __restrict__ dk, float* __restrict__ dv,
       const int up = kProbShift - g_behind, off = shift - q_behind - up;
       const float of_dp = power(off - eg - ev), of_delta = power(off);
       const bool whole = !s.causal || first + 31 <= q0 + offset;
-      const float* tail = reinterpret_cast<const float*>(now + kTile - 256);
 #pragma unroll
       for (int c = 0; c < 4; c++) {
         const float4 mm = *reinterpret_cast<const float4*>(tail + 8 * c + 4 * half);
@@ -818,6 +841,10 @@ __device__ inline void key_grads(float* __restrict__ dk, float* __restrict__ dv,
       }
     }
     tile_barrier();
+  };
+  for (int u = begin; u < end; u += 2) {
+    step(even, odd, u);
+    if (u + 1 < end) step(odd, even, u + 1);
   }
   if (j >= s.sk) return;
   const size_t all = static_cast<size_t>(s.b) * s.sk * s.hk * s.d;

@@ -206,7 +206,7 @@ RenderedKernel render_attention(const UOp& call, bool grad) {
       rk.launches = {launch("fg_attention", (q_rows + 3) / 4, 256, "attention")};
     } else {
       const uint64_t blocks = static_cast<uint64_t>(batch * kv_heads * k_blocks);
-      rk.workspace_bytes = blocks * static_cast<uint64_t>(nb * 8192 + 8);
+      rk.workspace_bytes = blocks * static_cast<uint64_t>(nb * 8192 + 1024);
       rk.launches = {launch("fg_attention_pack_" + std::to_string(nb), 2 * blocks, 256, "attention"),
                      launch("fg_attention_tiles_" + std::to_string(nb),
                             static_cast<uint64_t>(batch * heads * ((sq + 127) / 128)), 256, "attention")};
@@ -224,8 +224,8 @@ RenderedKernel render_attention(const UOp& call, bool grad) {
     const int64_t tiles = batch * kv_heads * ((sk + 127) / 128);
     const int64_t parts = std::max<int64_t>(1, std::min((1024 + tiles - 1) / tiles, q_blocks * group / 4));
     const uint64_t all = static_cast<uint64_t>(batch * sk * kv_heads * dim);
-    rk.workspace_bytes = nk * static_cast<uint64_t>(nb * 12288 + 16) + nq * static_cast<uint64_t>(nb * 16384 + 256 + 16) +
-                         (parts > 1 ? 8 * all * static_cast<uint64_t>(parts) : 0);
+    rk.workspace_bytes = nk * static_cast<uint64_t>(nb * 12288 + 1024) + nq * static_cast<uint64_t>(nb * 16384 + 1024) +
+                         (nk + 3) / 4 * 16 + (parts > 1 ? 8 * all * static_cast<uint64_t>(parts) : 0);
     rk.launches = {launch("fg_attention_grad_pack" + nbs, 2 * (nk + nq), 256, "attention"),
                    launch("fg_attention_grad_kv" + nbs, static_cast<uint64_t>(tiles * parts), 256, "attention"),
                    launch("fg_attention_grad_q" + nbs, static_cast<uint64_t>(batch * heads * ((sq + 127) / 128)), 256, "attention")};
