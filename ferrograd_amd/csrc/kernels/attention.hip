@@ -5,8 +5,9 @@
 // lengths[b] are hidden, and with `causal` those past i + Sk - Sq. A query that
 // sees no key gives 0 and gradients of 0.
 // Matrices are one row per token: q, y [B Sq, Hq D], k, v [B Sk, Hk D].
-// stats holds per (b, h, i) the row's maximum in units of log2 (of S log2 e),
-// then 1 / sum, for the gradients to make the probabilities again.
+// stats holds per (b, h, i) m_i, no less than the row's maximum of S log2 e less
+// kLazy, then 1 / sum_j exp2(S_ij log2 e - m_i), for the gradients to make the
+// probabilities again.
 #include <hip/hip_runtime.h>
 
 namespace {
@@ -877,17 +878,190 @@ __device__ inline void sum_parts(float* __restrict__ dk, float* __restrict__ dv,
   }
 }
 
+// ── few queries ─────────────────────────────────────────────────────────────
+// At most 16 query rows per key head (queries times the heads that share it):
+// a token at a time, where reading the keys and values is all the work. They
+// are read once, as they are, by float32 matrix products, so nothing is cut or
+// staged. A wave takes 16 keys at a time: S (16 keys x 16 rows) = K Q^T, lane l
+// holding key l % 16 and every fourth group of 4 columns, and O^T += V^T P with
+// the four terms of a product taken as lane l's result rows, 4 (l / 16) + r: P
+// is used where it is. The keys of a head are split over workgroups until these
+// fill the chip, and joined by a second launch.
+
+// A workgroup's part of the keys of one (b, hk): the rows' sums so far.
+struct TokenPart {
+  float* o;  // [16][D]
+  float* m;  // [16], units of log2
+  float* l;  // [16]
+};
+
+__device__ inline TokenPart token_part(char* ws, size_t index, int D) {
+  float* at = reinterpret_cast<float*>(ws) + index * (16 * D + 32);
+  return {at, at + 16 * D, at + 16 * D + 16};
+}
+
+// ND: columns in units of 64.
+template <int ND>
+__device__ inline void token(float* __restrict__ y, const float* __restrict__ q, const float* __restrict__ k,
+                             const float* __restrict__ v, float* __restrict__ stats, const int* __restrict__ lengths,
+                             char* __restrict__ ws, const Shape& s, float scale, int splits, int per) {
+  __shared__ float merged[4][16 * ND * 64];
+  __shared__ float ms[4][16], ls[4][16];
+  const int split = blockIdx.x % splits, hk = blockIdx.x / splits % s.hk, b = blockIdx.x / splits / s.hk;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+  const int n = lane % 16, quad = lane / 16, group = s.hq / s.hk, rows = s.sq * group;
+  const int keys = key_count(s, lengths, b), begin = split * per, end = min(keys, begin + per);
+  // Row n of the products: query n / group, head hk * group + n % group.
+  const int i = min(n, rows - 1) / group, h = hk * group + min(n, rows - 1) % group;
+  const int seen = n < rows ? min(end, visible(s, keys, i)) : 0;
+  const float* q_row = q + (static_cast<size_t>(b) * s.sq + i) * s.hq * s.d + static_cast<size_t>(h) * s.d;
+  const size_t stride = static_cast<size_t>(s.hk) * s.d;
+  const size_t head = static_cast<size_t>(b) * s.sk * stride + static_cast<size_t>(hk) * s.d;
+  float4 qv[ND * 4];
+#pragma unroll
+  for (int t = 0; t < ND * 4; t++) qv[t] = load4(q_row, 16 * t + 4 * quad, s.d);
+  const float factor = scale * kLog2e;
+  float m = -INFINITY, l = 0.f;
+  floatx4 o[ND][4] = {};
+  for (int j0 = begin + wave * 16; j0 < end; j0 += 64) {
+    float4 kv[ND * 4], vv[4][ND];
+    const float* k_row = k + head + min(j0 + n, end - 1) * stride;
+#pragma unroll
+    for (int t = 0; t < ND * 4; t++) kv[t] = load4(k_row, 16 * t + 4 * quad, s.d);
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+#pragma unroll
+      for (int c = 0; c < ND; c++)
+        vv[r][c] = load4(v + head + min(j0 + 4 * quad + r, end - 1) * stride, 64 * c + 4 * n, s.d);
+    floatx4 x = {};
+#pragma unroll
+    for (int t = 0; t < ND * 4; t++) {
+      x = __builtin_amdgcn_mfma_f32_16x16x4f32(kv[t].x, qv[t].x, x, 0, 0, 0);
+      x = __builtin_amdgcn_mfma_f32_16x16x4f32(kv[t].y, qv[t].y, x, 0, 0, 0);
+      x = __builtin_amdgcn_mfma_f32_16x16x4f32(kv[t].z, qv[t].z, x, 0, 0, 0);
+      x = __builtin_amdgcn_mfma_f32_16x16x4f32(kv[t].w, qv[t].w, x, 0, 0, 0);
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      x[r] = j0 + 4 * quad + r < seen ? x[r] * factor : -INFINITY;
+      top = fmaxf(top, x[r]);
+    }
+    if (__any(top > m + kLazy)) {
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float to = top > m + kLazy ? top : m;
+      const float old = to == -INFINITY ? 1.f : exp2f(m - to);
+      m = to;
+      l *= old;
+#pragma unroll
+      for (int c = 0; c < ND; c++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[c][e] *= old;
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      x[r] = __builtin_amdgcn_exp2f(x[r] - base);
+      l += x[r];
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+#pragma unroll
+      for (int c = 0; c < ND; c++) {
+        o[c][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[r][c].x, x[r], o[c][0], 0, 0, 0);
+        o[c][1] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[r][c].y, x[r], o[c][1], 0, 0, 0);
+        o[c][2] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[r][c].z, x[r], o[c][2], 0, 0, 0);
+        o[c][3] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[r][c].w, x[r], o[c][3], 0, 0, 0);
+      }
+  }
+  // The four waves' sums, joined in LDS: o[c][e][r] is row n, column 64 c +
+  // 4 (4 quad + r) + e.
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  if (quad == 0) {
+    ms[wave][n] = m;
+    ls[wave][n] = l;
+  }
+#pragma unroll
+  for (int c = 0; c < ND; c++)
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+      *reinterpret_cast<float4*>(&merged[wave][n * ND * 64 + 64 * c + 4 * (4 * quad + r)]) =
+          make_float4(o[c][0][r], o[c][1][r], o[c][2][r], o[c][3][r]);
+  __syncthreads();
+  const TokenPart part = token_part(ws, blockIdx.x, s.d);
+  for (int at = threadIdx.x; at < rows * ND * 64; at += 256) {
+    const int row = at / (ND * 64), d = at % (ND * 64);
+    float top = fmaxf(fmaxf(ms[0][row], ms[1][row]), fmaxf(ms[2][row], ms[3][row]));
+    top = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, all = 0.f;
+    for (int w = 0; w < 4; w++) {
+      const float of = exp2f(ms[w][row] - top);
+      sum += of * ls[w][row];
+      all += of * merged[w][row * ND * 64 + d];
+    }
+    if (splits > 1) {
+      if (d < s.d) part.o[row * s.d + d] = all;
+      if (d == 0) {
+        part.m[row] = top;
+        part.l[row] = sum;
+      }
+    } else {
+      const int iq = row / group, hq = hk * group + row % group;
+      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      if (d < s.d) y[(static_cast<size_t>(b) * s.sq + iq) * s.hq * s.d + static_cast<size_t>(hq) * s.d + d] = all * inv;
+      if (d == 0) {
+        const size_t stat = (static_cast<size_t>(b) * s.hq + hq) * s.sq + iq;
+        stats[stat] = top;
+        stats[static_cast<size_t>(s.b) * s.hq * s.sq + stat] = inv;
+      }
+    }
+  }
+}
+
+// The parts of a row's keys joined: a workgroup of 128 columns per row.
+__device__ inline void join_token(float* __restrict__ y, float* __restrict__ stats, char* __restrict__ ws, const Shape& s, int splits) {
+  const int group = s.hq / s.hk, rows = s.sq * group;
+  const int row = blockIdx.x % rows, hk = blockIdx.x / rows % s.hk, b = blockIdx.x / rows / s.hk, d = threadIdx.x;
+  const size_t first = (static_cast<size_t>(b) * s.hk + hk) * splits;
+  // A part without keys has m = 0 and l = 0 and takes no part in the maximum.
+  float top = -INFINITY;
+  for (int p = 0; p < splits; p++) {
+    const TokenPart part = token_part(ws, first + p, s.d);
+    if (part.l[row] > 0.f) top = fmaxf(top, part.m[row]);
+  }
+  if (top == -INFINITY) top = 0.f;
+  float sum = 0.f, all = 0.f;
+  for (int p = 0; p < splits; p++) {
+    const TokenPart part = token_part(ws, first + p, s.d);
+    const float l = part.l[row];
+    if (!(l > 0.f)) continue;
+    const float of = exp2f(part.m[row] - top);
+    sum += of * l;
+    if (d < s.d) all += of * part.o[row * s.d + d];
+  }
+  const int i = row / group, h = hk * group + row % group;
+  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  if (d < s.d) y[(static_cast<size_t>(b) * s.sq + i) * s.hq * s.d + static_cast<size_t>(h) * s.d + d] = all * inv;
+  if (d == 0) {
+    const size_t stat = (static_cast<size_t>(b) * s.hq + h) * s.sq + i;
+    stats[stat] = top;
+    stats[static_cast<size_t>(s.b) * s.hq * s.sq + stat] = inv;
+  }
+}
+
 }  // namespace
 
 #define FG_ATTENTION(NB)                                                                                              \
   extern "C" __global__ void __launch_bounds__(256) fg_attention_pack_##NB(                                           \
       float* y, const float* q, const float* k, const float* v, float* stats, const int* lengths, char* ws, int B,    \
-      int Sq, int Sk, int Hq, int Hk, int D, int causal, float scale) {                                               \
+      int Sq, int Sk, int Hq, int Hk, int D, int causal, float scale, int splits, int per) {                          \
     pack_keys<NB>(k, v, lengths, ws, B, Sk, Hk, D);                                                                   \
   }                                                                                                                   \
   extern "C" __global__ void __launch_bounds__(256, 2) fg_attention_tiles_##NB(                                       \
       float* y, const float* q, const float* k, const float* v, float* stats, const int* lengths, char* ws, int B,    \
-      int Sq, int Sk, int Hq, int Hk, int D, int causal, float scale) {                                               \
+      int Sq, int Sk, int Hq, int Hk, int D, int causal, float scale, int splits, int per) {                          \
     forward_tiles<NB>(y, q, stats, lengths, ws, B, Sq, Sk, Hq, Hk, D, causal, scale);                                 \
   }                                                                                                                   \
   extern "C" __global__ void __launch_bounds__(256) fg_attention_grad_pack_##NB(                                      \
@@ -896,7 +1070,7 @@ __device__ inline void sum_parts(float* __restrict__ dk, float* __restrict__ dv,
       int causal, float scale) {                                                                                      \
     pack_grad<NB>(q, k, v, y, g, stats, lengths, ws, Shape{B, Sq, Sk, Hq, Hk, D, causal});                            \
   }                                                                                                                   \
-  extern "C" __global__ void __launch_bounds__(256, (NB) < 3 ? 2 : 1) fg_attention_grad_q_##NB(                       \
+  extern "C" __global__ void __launch_bounds__(256, (NB) < 4 ? 2 : 1) fg_attention_grad_q_##NB(                       \
       float* dq, const float* q, const float* k, const float* v, const float* y, const float* g, const float* stats,  \
       float* dk, float* dv, const int* lengths, char* ws, int parts, int B, int Sq, int Sk, int Hq, int Hk, int D,    \
       int causal, float scale) {                                                                                      \
@@ -921,48 +1095,18 @@ FG_ATTENTION(2)
 FG_ATTENTION(3)
 FG_ATTENTION(4)
 
-// One wave per query row.
-extern "C" __global__ void __launch_bounds__(256)
-    fg_attention(float* __restrict__ y, const float* __restrict__ q, const float* __restrict__ k,
-                 const float* __restrict__ v, float* __restrict__ stats, const int* __restrict__ lengths, char* ws, int B, int Sq,
-                 int Sk, int Hq, int Hk, int D, int causal, float scale) {
-  __shared__ float probs[4][64];
-  const Shape s{B, Sq, Sk, Hq, Hk, D, causal};
-  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-  const size_t row = static_cast<size_t>(blockIdx.x) * 4 + wave;  // (b, h, i)
-  const bool live = row < static_cast<size_t>(B) * Hq * Sq;
-  const int i = live ? row % Sq : 0, h = live ? row / Sq % Hq : 0, b = live ? row / Sq / Hq : 0;
-  const int hk = h / (Hq / Hk);
-  const int seen = live ? visible(s, key_count(s, lengths, b), i) : 0;
-  const float* qi = q + (static_cast<size_t>(b) * Sq + i) * Hq * D + static_cast<size_t>(h) * D;
-  const float* kb = k + static_cast<size_t>(b) * Sk * Hk * D + static_cast<size_t>(hk) * D;
-  const float* vb = v + static_cast<size_t>(b) * Sk * Hk * D + static_cast<size_t>(hk) * D;
-  const size_t stride = static_cast<size_t>(Hk) * D;
-  float m = -INFINITY, l = 0.f, o[2] = {0.f, 0.f};
-  for (int j0 = 0; j0 < seen; j0 += 64) {
-    const int j = j0 + lane;
-    const float x = j < seen ? dot(qi, kb + j * stride, D) * (scale * kLog2e) : -INFINITY;
-    const float top = fmaxf(m, wave_max(x)), base = top == -INFINITY ? 0.f : top;
-    const float p = exp2f(x - base), old = exp2f(m - base);
-    l = l * old + wave_sum(p);
-    m = top;
-    probs[wave][lane] = p;
-    __builtin_amdgcn_wave_barrier();
-    for (int t = 0; t < 2; t++) {
-      const int d = lane + 64 * t;
-      if (d >= D) continue;
-      float sum = 0.f;
-      for (int n = 0; n < min(64, seen - j0); n++) sum += probs[wave][n] * vb[(j0 + n) * stride + d];
-      o[t] = o[t] * old + sum;
-    }
-    __builtin_amdgcn_wave_barrier();
+#define FG_ATTENTION_TOKEN(ND)                                                                                        \
+  extern "C" __global__ void __launch_bounds__(256) fg_attention_token_##ND(                                          \
+      float* y, const float* q, const float* k, const float* v, float* stats, const int* lengths, char* ws, int B,    \
+      int Sq, int Sk, int Hq, int Hk, int D, int causal, float scale, int splits, int per) {                          \
+    token<ND>(y, q, k, v, stats, lengths, ws, Shape{B, Sq, Sk, Hq, Hk, D, causal}, scale, splits, per);               \
   }
-  if (!live) return;
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  for (int t = 0; t < 2; t++)
-    if (lane + 64 * t < D) y[(static_cast<size_t>(b) * Sq + i) * Hq * D + static_cast<size_t>(h) * D + lane + 64 * t] = o[t] * inv;
-  if (lane == 0) {
-    stats[row] = m == -INFINITY ? 0.f : m;
-    stats[static_cast<size_t>(B) * Hq * Sq + row] = inv;
-  }
+FG_ATTENTION_TOKEN(1)
+FG_ATTENTION_TOKEN(2)
+
+extern "C" __global__ void __launch_bounds__(128)
+    fg_attention_token_join(float* y, const float* q, const float* k, const float* v, float* stats, const int* lengths,
+                            char* ws, int B, int Sq, int Sk, int Hq, int Hk, int D, int causal, float scale, int splits,
+                            int per) {
+  join_token(y, stats, ws, Shape{B, Sq, Sk, Hq, Hk, D, causal}, splits);
 }

@@ -198,12 +198,26 @@ RenderedKernel render_attention(const UOp& call, bool grad) {
   const bool lengths = p[7] != 0;
   RenderedKernel rk;
   set_image(rk, fg_image_attention, fg_image_attention_end);
-  const uint64_t q_rows = static_cast<uint64_t>(batch * heads * sq);
+  std::vector<CallArg> tail;
+  for (int i = 0; i < 7; i++) tail.push_back(CallArg::i32(p[static_cast<size_t>(i)]));
+  tail.push_back(CallArg::f32(static_cast<float>(from_bits(p[8]))));
   const int64_t dim = p[5], nb = (dim + 31) / 32, k_blocks = (sk + 31) / 32;
   if (!grad) {
     rk.kind = "attention";
-    if (sq * (heads / kv_heads) < 8) {
-      rk.launches = {launch("fg_attention", (q_rows + 3) / 4, 256, "attention")};
+    int64_t splits = 1, per = sk;
+    if (sq * (heads / kv_heads) <= 16) {
+      // Few query rows: the keys of a head split until there are 1024
+      // workgroups, of at least 256 keys (four rounds of its waves).
+      const int64_t pairs = batch * kv_heads;
+      splits = std::max<int64_t>(1, std::min({(1024 + pairs - 1) / pairs, sk / 256, int64_t(64)}));
+      per = ((sk + splits - 1) / splits + 63) / 64 * 64;
+      splits = (sk + per - 1) / per;
+      rk.launches = {launch("fg_attention_token_" + std::to_string(dim <= 64 ? 1 : 2), static_cast<uint64_t>(pairs * splits), 256, "attention")};
+      rk.workspace_bytes = 4;
+      if (splits > 1) {
+        rk.workspace_bytes = static_cast<size_t>(pairs * splits) * static_cast<size_t>(16 * dim + 32) * 4;
+        rk.launches.push_back(launch("fg_attention_token_join", static_cast<uint64_t>(batch * heads * sq), 128, "attention"));
+      }
     } else {
       const uint64_t blocks = static_cast<uint64_t>(batch * kv_heads * k_blocks);
       rk.workspace_bytes = blocks * static_cast<uint64_t>(nb * 8192 + 1024);
@@ -213,6 +227,8 @@ RenderedKernel render_attention(const UOp& call, bool grad) {
     }
     rk.call_args = {CallArg::slot(0), CallArg::slot(1), CallArg::slot(2), CallArg::slot(3), CallArg::slot(lengths ? 5 : 4),
                     lengths ? CallArg::slot(4) : CallArg::null(), CallArg::workspace()};
+    tail.push_back(CallArg::i32(splits));
+    tail.push_back(CallArg::i32(per));
     rk.side_outputs = {lengths ? 5 : 4};
   } else {
     rk.kind = "attention_grad";
@@ -240,8 +256,7 @@ RenderedKernel render_attention(const UOp& call, bool grad) {
     rk.call_args.push_back(CallArg::i32(parts));
     rk.side_outputs = {dk, dk + 1};
   }
-  for (int i = 0; i < 7; i++) rk.call_args.push_back(CallArg::i32(p[static_cast<size_t>(i)]));
-  rk.call_args.push_back(CallArg::f32(static_cast<float>(from_bits(p[8]))));
+  rk.call_args.insert(rk.call_args.end(), tail.begin(), tail.end());
   return rk;
 }
 
