@@ -233,11 +233,11 @@ __device__ inline void pack_keys(const float* k, const float* v, const int* leng
 
 // Copies `Bytes` (a multiple of 1 KiB), contiguous, into LDS without passing
 // registers: each wave 1 KiB at a time.
-template <int Bytes>
+template <int Bytes, int Waves>
 __device__ inline void copy_tile(const char* from, char* to) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
 #pragma unroll
-  for (int at = wave * kPart; at < Bytes; at += 4 * kPart)
+  for (int at = wave * kPart; at < Bytes; at += Waves * kPart)
     __builtin_amdgcn_global_load_lds(
         (const __attribute__((address_space(1))) void*)(from + at + lane * 16),
         (__attribute__((address_space(3))) void*)(to + at), 16, 0, 0);
@@ -359,13 +359,13 @@ __device__ inline void store_columns(float* row, int n, int half, int D, const f
   }
 }
 
-// Which 128 queries, head and batch a workgroup takes. The last queries of
+// Which `rows` queries, head and batch a workgroup takes. The last queries of
 // every head come first: with `causal` they see the most keys, and what is
 // left for the end is small. Workgroups go to the 8 chiplets in turn, so
 // where the heads allow it each chiplet gets heads next to each other, which
 // share keys in its cache.
-__device__ inline void query_tile(const Shape& s, int* qt, int* h, int* b) {
-  const unsigned heads = static_cast<unsigned>(s.b) * s.hq, tiles = (s.sq + 127) / 128;
+__device__ inline void query_tile(const Shape& s, int rows, int* qt, int* h, int* b) {
+  const unsigned heads = static_cast<unsigned>(s.b) * s.hq, tiles = (s.sq + rows - 1) / rows;
   unsigned head = blockIdx.x % heads;
   if (heads % 8 == 0) head = head % 8 * (heads / 8) + head / 8;
   *qt = tiles - 1 - blockIdx.x / heads;
@@ -387,7 +387,7 @@ __device__ inline void forward_tiles(float* __restrict__ y, const float* __restr
   // wait for them first.
   __shared__ __attribute__((aligned(1024))) char even[kTile], odd[kTile];
   int qt, h, b;
-  query_tile(Shape{B, Sq, Sk, Hq, Hk, D, causal}, &qt, &h, &b);
+  query_tile(Shape{B, Sq, Sk, Hq, Hk, D, causal}, 128, &qt, &h, &b);
   const int hk = h / (Hq / Hk);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, half = lane / 32;
   const int i = qt * 128 + wave * 32 + lane % 32;  // this lane's query
@@ -403,7 +403,7 @@ __device__ inline void forward_tiles(float* __restrict__ y, const float* __restr
 
   const size_t head = static_cast<size_t>(b) * Hk + hk;
   const char* tile = ws + head * ((Sk + kBlock - 1) / kBlock) * kTile;
-  if (block_end > 0) copy_tile<kTile>(tile, even);
+  if (block_end > 0) copy_tile<kTile, 4>(tile, even);
 
   half8 qh[NB * 2], ql[NB * 2];
   const int eq = row_fragments<NB>(q + (static_cast<size_t>(b) * Sq + min(i, Sq - 1)) * Hq * D + static_cast<size_t>(h) * D, live,
@@ -414,7 +414,7 @@ __device__ inline void forward_tiles(float* __restrict__ y, const float* __restr
   RunningScale vs;
   tile_barrier();
   auto step = [&](const char* now, char* next, int kb) {
-    if (kb + 1 < block_end) copy_tile<kTile>(tile + static_cast<size_t>(kb + 1) * kTile, next);
+    if (kb + 1 < block_end) copy_tile<kTile, 4>(tile + static_cast<size_t>(kb + 1) * kTile, next);
     if (kb < wave_end) {
       const char* t = now + lane * 16;
       const int* tail = reinterpret_cast<const int*>(now + kTile - kTail);
@@ -631,9 +631,14 @@ __device__ inline int values_norm(const int* norms, int blocks) {
 
 __device__ inline int clamp_power(int a) { return min(max(a, -120), 120); }
 
-// dq. A workgroup: 128 queries of one head, 32 a wave, over all keys; scores
-// and their gradients transposed as in the forward pass.
+// dq. A workgroup: 32 queries of one head a wave, over all keys; scores and
+// their gradients transposed as in the forward pass. Tiles of four column
+// groups leave room for one workgroup a compute unit: eight waves share them,
+// so that each matrix core has two waves in turn.
 template <int NB>
+constexpr int kQueryGradWaves = NB < 4 ? 4 : 8;
+
+template <int NB, int Waves>
 __device__ inline void query_grads(float* __restrict__ dq, const float* __restrict__ q, const float* __restrict__ g,
                                    const float* __restrict__ stats, const int* __restrict__ lengths,
                                    char* __restrict__ ws, const Shape& s, float scale) {
@@ -641,20 +646,21 @@ __device__ inline void query_grads(float* __restrict__ dq, const float* __restri
   __shared__ __attribute__((aligned(1024))) char even[kTile], odd[kTile];
   const GradSpace f = grad_space<NB>(ws, s);
   int qt, h, b;
-  query_tile(s, &qt, &h, &b);
+  constexpr int kRows = 32 * Waves;
+  query_tile(s, kRows, &qt, &h, &b);
   const int hk = h / (s.hq / s.hk);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, half = lane / 32;
-  const int first = qt * 128 + wave * 32, i = first + lane % 32;
+  const int first = qt * kRows + wave * 32, i = first + lane % 32;
   const bool live = i < s.sq, wave_live = first < s.sq;
   const int keys = key_count(s, lengths, b);
-  const int block_end = (visible(s, keys, min(s.sq, qt * 128 + 128) - 1) + kBlock - 1) / kBlock;
+  const int block_end = (visible(s, keys, min(s.sq, qt * kRows + kRows) - 1) + kBlock - 1) / kBlock;
   const int wave_end = wave_live ? (visible(s, keys, min(s.sq, first + 32) - 1) + kBlock - 1) / kBlock : 0;
   const int wave_full = visible(s, keys, first) / kBlock;
   const int seen = live ? visible(s, keys, i) : 0;
 
   const size_t head = static_cast<size_t>(b) * s.hk + hk;
   const char* tile = f.k_tiles + head * f.k_blocks * kTile;
-  if (block_end > 0) copy_tile<kTile>(tile, even);
+  if (block_end > 0) copy_tile<kTile, Waves>(tile, even);
 
   const size_t at = (static_cast<size_t>(b) * s.sq + min(i, s.sq - 1)) * s.hq * s.d + static_cast<size_t>(h) * s.d;
   const size_t stat = (static_cast<size_t>(b) * s.hq + h) * s.sq + min(i, s.sq - 1);
@@ -673,7 +679,7 @@ __device__ inline void query_grads(float* __restrict__ dq, const float* __restri
   RunningScale ks;
   tile_barrier();
   auto step = [&](const char* now, char* next, int kb) {
-    if (kb + 1 < block_end) copy_tile<kTile>(tile + static_cast<size_t>(kb + 1) * kTile, next);
+    if (kb + 1 < block_end) copy_tile<kTile, Waves>(tile + static_cast<size_t>(kb + 1) * kTile, next);
     if (kb < wave_end) {
       const char* t = now + lane * 16;
       const int* tail = reinterpret_cast<const int*>(now + kTile - kTail);
@@ -729,23 +735,30 @@ __device__ inline void query_grads(float* __restrict__ dq, const float* __restri
   for (int n = 0; n < NB; n++) store_columns(dq + at, n, half, s.d, o[n], scale, -shift - ks.ref);
 }
 
-// dk and dv. A workgroup: 128 keys of one key head, 32 a wave, over its part
-// of the query blocks that see any of them, head after head of those that read
-// the key head. Scores are not transposed here: a lane holds 16 queries of one
-// key, which is what dv^T += G^T P and dk^T += Q^T dS take.
+// dk and dv. A workgroup: 128 keys of one key head over its part of the query
+// blocks that see any of them, head after head of those that read the key
+// head. Two waves share 32 keys: one makes the probabilities and dv, the other
+// the gradients' products with the values, and from both ds and dk. So neither
+// holds more than one operand and one result (a wave with both leaves a matrix
+// core to itself, waiting while it does anything else), at the price of the
+// probabilities' way through LDS. Scores are not transposed here: a lane holds
+// 16 queries of one key, which is what dv^T += G^T P and dk^T += Q^T dS take.
 template <int NB>
 __device__ inline void key_grads(float* __restrict__ dk, float* __restrict__ dv, const float* __restrict__ k,
                                  const float* __restrict__ v, const int* __restrict__ lengths, char* __restrict__ ws,
                                  const Shape& s, float scale, int parts) {
-  constexpr int kTile = kQueryTile<NB>;
+  constexpr int kTile = kQueryTile<NB>, Waves = 8;
   __shared__ __attribute__((aligned(1024))) char even[kTile], odd[kTile];
+  __shared__ float4 probs[4][4][64];  // [pair][registers 4 c .. 4 c + 3][lane]
   const GradSpace f = grad_space<NB>(ws, s);
   // The first keys are seen by the most queries: first.
   const unsigned inner = static_cast<unsigned>(s.b * s.hk) * parts;
   const int kt = blockIdx.x / inner, part = blockIdx.x % inner % parts;
   const int hk = blockIdx.x % inner / parts % s.hk, b = blockIdx.x % inner / parts / s.hk, group = s.hq / s.hk;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, half = lane / 32;
-  const int first = kt * 128 + wave * 32, j = first + lane % 32;
+  const int pair = wave % 4;
+  const bool of_keys = wave >= 4;  // makes dk, from ds; the other dv, from p
+  const int first = kt * 128 + pair * 32, j = first + lane % 32;
   const int keys = key_count(s, lengths, b), offset = s.sk - s.sq;
   const bool live = j < keys;
   // Query blocks that see a key of the workgroup: those from q_first on.
@@ -755,90 +768,92 @@ __device__ inline void key_grads(float* __restrict__ dk, float* __restrict__ dv,
   const int end = static_cast<int>(static_cast<long long>(units) * (part + 1) / parts);
 
   const size_t q_head = (static_cast<size_t>(b) * s.hq + static_cast<size_t>(hk) * group) * f.q_blocks;
-  auto unit_block = [&](int u) { return q_head + static_cast<size_t>(u / per_head) * f.q_blocks + q_first + u % per_head; };
-  auto copy_unit = [&](int u, char* to) { copy_tile<kTile>(f.q_tiles + unit_block(u) * kTile, to); };
+  auto copy_unit = [&](int u, char* to) {
+    const size_t block = q_head + static_cast<size_t>(u / per_head) * f.q_blocks + q_first + u % per_head;
+    copy_tile<kTile, Waves>(f.q_tiles + block * kTile, to);
+  };
   if (begin < end) copy_unit(begin, even);
 
   const size_t at = (static_cast<size_t>(b) * s.sk + min(j, s.sk - 1)) * s.hk * s.d + static_cast<size_t>(hk) * s.d;
-  half8 kh[NB * 2], kl[NB * 2], vh[NB * 2], vl[NB * 2];
-  const int ek = row_fragments<NB>(k + at, live, s.d, scale < 0.f ? -1.f : 1.f, 1.f, kh, kl);
-  const int ev = row_fragments<NB>(v + at, live, s.d, 1.f, 1.f, vh, vl);
+  half8 fh[NB * 2], fl[NB * 2];  // K for the probabilities (its sign with scale's), V for ds
+  const int e = row_fragments<NB>((of_keys ? v : k) + at, live, s.d, !of_keys && scale < 0.f ? -1.f : 1.f, 1.f, fh, fl);
   const int norm = values_norm(f.norms + (static_cast<size_t>(b) * s.hk + hk) * f.k_blocks, (keys + kBlock - 1) / kBlock);
   const float factor = fabsf(scale) * kLog2e;
-  floatx16 ok[NB] = {}, ov[NB] = {};
+  floatx16 o[NB] = {};
   RunningScale qs, gs;
   tile_barrier();
   auto step = [&](const char* now, char* next, int u) {
     if (u + 1 < end) copy_unit(u + 1, next);
     const int q0 = (q_first + u % per_head) * kBlock;
     // Whether any of the block's queries sees any of the wave's keys.
-    if (first < keys && (!s.causal || first <= q0 + kBlock - 1 + offset)) {
-      const char* t = now + lane * 16;
-      const float* tail = reinterpret_cast<const float*>(now + kTile - kTail);
-      const int* exponents = reinterpret_cast<const int*>(tail) + 64;
-      const int eq = uniform(exponents[0]), eg = uniform(exponents[1]), shift = clamp_power(kScoreShift - uniform(exponents[2]) - norm);
-      floatx16 x = {}, dp = {};
+    const bool any = first < keys && (!s.causal || first <= q0 + kBlock - 1 + offset);
+    const char* t = now + lane * 16 + (of_keys ? kRowBytes<NB> : 0);
+    const float* tail = reinterpret_cast<const float*>(now + kTile - kTail);
+    const int* exponents = reinterpret_cast<const int*>(tail) + 64;
+    const int eq = uniform(exponents[0]), eg = uniform(exponents[1]), shift = clamp_power(kScoreShift - uniform(exponents[2]) - norm);
+    floatx16 x = {};
+    int change = 0, up = 0, q_behind = 0;
+    if (any) {
+      int g_behind;
+      const int g_change = gs.take(eg, &g_behind), q_change = qs.take(shift + eq, &q_behind);
+      change = of_keys ? q_change : g_change;
+      up = kProbShift - g_behind;  // p carries 2^up
 #pragma unroll
       for (int n = 0; n < NB * 2; n++)
         x = mfma3(*reinterpret_cast<const half8*>(t + n * 2 * kPart), *reinterpret_cast<const half8*>(t + n * 2 * kPart + kPart),
-                  kh[n], kl[n], x);
+                  fh[n], fl[n], x);
+      if (!of_keys) {
+        const float fac = ldexpf(factor, -(eq + e));
+        const bool whole = !s.causal || first + 31 <= q0 + offset;
 #pragma unroll
-      for (int n = 0; n < NB * 2; n++)
-        dp = mfma3(*reinterpret_cast<const half8*>(t + kRowBytes<NB> + n * 2 * kPart),
-                   *reinterpret_cast<const half8*>(t + kRowBytes<NB> + n * 2 * kPart + kPart), vh[n], vl[n], dp);
-      int q_behind, g_behind;
-      const int q_change = qs.take(shift + eq, &q_behind), g_change = gs.take(eg, &g_behind);
-      if (q_change != 0) {
+        for (int c = 0; c < 4; c++) {
+          const float4 mm = *reinterpret_cast<const float4*>(tail + 8 * c + 4 * half);
+          const float m4[4] = {mm.x, mm.y, mm.z, mm.w};
 #pragma unroll
-        for (int n = 0; n < NB; n++)
-#pragma unroll
-          for (int r = 0; r < 16; r++) ok[n][r] = ldexpf(ok[n][r], q_change);
-      }
-      if (g_change != 0) {
-#pragma unroll
-        for (int n = 0; n < NB; n++)
-#pragma unroll
-          for (int r = 0; r < 16; r++) ov[n][r] = ldexpf(ov[n][r], g_change);
-      }
-      const float fac = ldexpf(factor, -(eq + ek));
-      // p carries 2^up; what multiplies it into ds takes that off again.
-      const int up = kProbShift - g_behind, off = shift - q_behind - up;
-      const float of_dp = power(off - eg - ev), of_delta = power(off);
-      const bool whole = !s.causal || first + 31 <= q0 + offset;
-#pragma unroll
-      for (int c = 0; c < 4; c++) {
-        const float4 mm = *reinterpret_cast<const float4*>(tail + 8 * c + 4 * half);
-        const float4 dd = *reinterpret_cast<const float4*>(tail + 32 + 8 * c + 4 * half);
-        const float m4[4] = {mm.x, mm.y, mm.z, mm.w}, d4[4] = {dd.x, dd.y, dd.z, dd.w};
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const int r = 4 * c + e;
-          float p = __builtin_amdgcn_exp2f(fmaf(x[r], fac, static_cast<float>(up) - m4[e]));
-          if (!whole) p = j <= q0 + result_row(r, half) + offset ? p : 0.f;
-          x[r] = p;
-          dp[r] = p * fmaf(dp[r], of_dp, -d4[e] * of_delta);
+          for (int i = 0; i < 4; i++) {
+            float p = __builtin_amdgcn_exp2f(fmaf(x[4 * c + i], fac, static_cast<float>(up) - m4[i]));
+            if (!whole) p = j <= q0 + 8 * c + 4 * half + i + offset ? p : 0.f;
+            x[4 * c + i] = p;
+          }
+          probs[pair][c][lane] = make_float4(x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]);
         }
       }
+    }
+    // The probabilities are in LDS. (No wait for the copies.)
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (any) {
+      if (of_keys) {
+        // ds, with what p carries taken off again.
+        const int off = shift - q_behind - up;
+        const float of_dp = power(off - eg - e), of_delta = power(off);
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          const float4 pp = probs[pair][c][lane], dd = *reinterpret_cast<const float4*>(tail + 32 + 8 * c + 4 * half);
+          const float p4[4] = {pp.x, pp.y, pp.z, pp.w}, d4[4] = {dd.x, dd.y, dd.z, dd.w};
+#pragma unroll
+          for (int i = 0; i < 4; i++) x[4 * c + i] = p4[i] * fmaf(x[4 * c + i], of_dp, -d4[i] * of_delta);
+        }
+      }
+      if (change != 0) {
+#pragma unroll
+        for (int n = 0; n < NB; n++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) o[n][r] = ldexpf(o[n][r], change);
+      }
+      const char* columns = now + lane * 16 + 2 * kRowBytes<NB> + (of_keys ? 0 : kColBytes<NB>);
 #pragma unroll
       for (int w = 0; w < 2; w++) {
-        float p[8], d[8];
+        float p[8];
 #pragma unroll
-        for (int r = 0; r < 8; r++) {
-          p[r] = x[8 * w + r];
-          d[r] = dp[8 * w + r];
-        }
-        half8 ph, pl, dh, dl;
+        for (int r = 0; r < 8; r++) p[r] = x[8 * w + r];
+        half8 ph, pl;
         cut_probs(p, &ph, &pl);
-        cut_probs(d, &dh, &dl);
-        const char* qt = t + 2 * kRowBytes<NB> + w * 2 * kPart;
-        const char* gt = qt + kColBytes<NB>;
 #pragma unroll
-        for (int n = 0; n < NB; n++) {
-          ov[n] = mfma3(*reinterpret_cast<const half8*>(gt + n * 4 * kPart),
-                        *reinterpret_cast<const half8*>(gt + n * 4 * kPart + kPart), ph, pl, ov[n]);
-          ok[n] = mfma3(*reinterpret_cast<const half8*>(qt + n * 4 * kPart),
-                        *reinterpret_cast<const half8*>(qt + n * 4 * kPart + kPart), dh, dl, ok[n]);
-        }
+        for (int n = 0; n < NB; n++)
+          o[n] = mfma3(*reinterpret_cast<const half8*>(columns + (2 * n + w) * 2 * kPart),
+                       *reinterpret_cast<const half8*>(columns + (2 * n + w) * 2 * kPart + kPart), ph, pl, o[n]);
       }
     }
     tile_barrier();
@@ -849,23 +864,16 @@ __device__ inline void key_grads(float* __restrict__ dk, float* __restrict__ dv,
   }
   if (j >= s.sk) return;
   const size_t all = static_cast<size_t>(s.b) * s.sk * s.hk * s.d;
-  if (parts > 1) {
-    dk = f.parts + 2 * all * part;
-    dv = dk + all;
-  }
+  float* out = of_keys ? dk : dv;
+  if (parts > 1) out = f.parts + 2 * all * part + (of_keys ? 0 : all);
   // Keys past the length take no gradient (their lanes' sums are not of it).
   if (!live) {
 #pragma unroll
-    for (int n = 0; n < NB; n++) {
-      ok[n] = floatx16{};
-      ov[n] = floatx16{};
-    }
+    for (int n = 0; n < NB; n++) o[n] = floatx16{};
   }
 #pragma unroll
-  for (int n = 0; n < NB; n++) {
-    store_columns(dk + at, n, half, s.d, ok[n], scale, -qs.ref);
-    store_columns(dv + at, n, half, s.d, ov[n], 1.f, -kProbShift - gs.ref);
-  }
+  for (int n = 0; n < NB; n++)
+    store_columns(out + at, n, half, s.d, o[n], of_keys ? scale : 1.f, of_keys ? -qs.ref : -kProbShift - gs.ref);
 }
 
 // dk and dv from their parts, in order.
@@ -1070,13 +1078,13 @@ __device__ inline void join_token(float* __restrict__ y, float* __restrict__ sta
       int causal, float scale) {                                                                                      \
     pack_grad<NB>(q, k, v, y, g, stats, lengths, ws, Shape{B, Sq, Sk, Hq, Hk, D, causal});                            \
   }                                                                                                                   \
-  extern "C" __global__ void __launch_bounds__(256, (NB) < 4 ? 2 : 1) fg_attention_grad_q_##NB(                       \
+  extern "C" __global__ void __launch_bounds__(64 * kQueryGradWaves<NB>, 2) fg_attention_grad_q_##NB(                  \
       float* dq, const float* q, const float* k, const float* v, const float* y, const float* g, const float* stats,  \
       float* dk, float* dv, const int* lengths, char* ws, int parts, int B, int Sq, int Sk, int Hq, int Hk, int D,    \
       int causal, float scale) {                                                                                      \
-    query_grads<NB>(dq, q, g, stats, lengths, ws, Shape{B, Sq, Sk, Hq, Hk, D, causal}, scale);                        \
+    query_grads<NB, kQueryGradWaves<NB>>(dq, q, g, stats, lengths, ws, Shape{B, Sq, Sk, Hq, Hk, D, causal}, scale);                        \
   }                                                                                                                   \
-  extern "C" __global__ void __launch_bounds__(256, (NB) < 3 ? 2 : 1) fg_attention_grad_kv_##NB(                      \
+  extern "C" __global__ void __launch_bounds__(512, 2) fg_attention_grad_kv_##NB(                                   \
       float* dq, const float* q, const float* k, const float* v, const float* y, const float* g, const float* stats,  \
       float* dk, float* dv, const int* lengths, char* ws, int parts, int B, int Sq, int Sk, int Hq, int Hk, int D,    \
       int causal, float scale) {                                                                                      \

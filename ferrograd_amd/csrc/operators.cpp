@@ -237,14 +237,15 @@ RenderedKernel render_attention(const UOp& call, bool grad) {
     const uint64_t nk = static_cast<uint64_t>(batch * kv_heads * k_blocks), nq = static_cast<uint64_t>(batch * heads * q_blocks);
     // Workgroups of 128 keys, each key tile's queries in parts until there are
     // 1024, of at least 4 query blocks.
-    const int64_t tiles = batch * kv_heads * ((sk + 127) / 128);
+    const int64_t tiles = batch * kv_heads * ((sk + 127) / 128), waves = nb < 4 ? 4 : 8;  // kQueryGradWaves
     const int64_t parts = std::max<int64_t>(1, std::min((1024 + tiles - 1) / tiles, q_blocks * group / 4));
     const uint64_t all = static_cast<uint64_t>(batch * sk * kv_heads * dim);
     rk.workspace_bytes = nk * static_cast<uint64_t>(nb * 12288 + 1024) + nq * static_cast<uint64_t>(nb * 16384 + 1024) +
                          (nk + 3) / 4 * 16 + (parts > 1 ? 8 * all * static_cast<uint64_t>(parts) : 0);
     rk.launches = {launch("fg_attention_grad_pack" + nbs, 2 * (nk + nq), 256, "attention"),
-                   launch("fg_attention_grad_kv" + nbs, static_cast<uint64_t>(tiles * parts), 256, "attention"),
-                   launch("fg_attention_grad_q" + nbs, static_cast<uint64_t>(batch * heads * ((sq + 127) / 128)), 256, "attention")};
+                   launch("fg_attention_grad_kv" + nbs, static_cast<uint64_t>(tiles * parts), 512, "attention"),
+                   launch("fg_attention_grad_q" + nbs, static_cast<uint64_t>(batch * heads * ((sq + 32 * waves - 1) / (32 * waves))),
+                          static_cast<unsigned>(64 * waves), "attention")};
     if (parts > 1)
       rk.launches.push_back(launch("fg_attention_grad_sum" + nbs, std::min<uint64_t>((2 * all + 255) / 256, 8192), 256, "attention"));
     const int dk = lengths ? 8 : 7;
