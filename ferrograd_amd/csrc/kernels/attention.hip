@@ -761,18 +761,19 @@ __device__ inline void key_grads(float* __restrict__ dk, float* __restrict__ dv,
   const int first = kt * 128 + pair * 32, j = first + lane % 32;
   const int keys = key_count(s, lengths, b), offset = s.sk - s.sq;
   const bool live = j < keys;
-  // Query blocks that see a key of the workgroup: those from q_first on.
+  // Query blocks that see a key of the workgroup: those from q_first on, the
+  // last first, each of all heads; a part takes every parts-th. Workgroups of
+  // other keys start with the same blocks and keep about the same pace, so
+  // that a chiplet's cache has what one of them read for the others.
   const int q_first = s.causal ? max(0, kt * 128 - offset) / kBlock : 0;
-  const int per_head = kt * 128 < keys ? max(0, f.q_blocks - q_first) : 0, units = per_head * group;
-  const int begin = static_cast<int>(static_cast<long long>(units) * part / parts);
-  const int end = static_cast<int>(static_cast<long long>(units) * (part + 1) / parts);
+  const int units = kt * 128 < keys ? max(0, f.q_blocks - q_first) * group : 0;
 
   const size_t q_head = (static_cast<size_t>(b) * s.hq + static_cast<size_t>(hk) * group) * f.q_blocks;
   auto copy_unit = [&](int u, char* to) {
-    const size_t block = q_head + static_cast<size_t>(u / per_head) * f.q_blocks + q_first + u % per_head;
+    const size_t block = q_head + static_cast<size_t>(u % group) * f.q_blocks + (f.q_blocks - 1 - u / group);
     copy_tile<kTile, Waves>(f.q_tiles + block * kTile, to);
   };
-  if (begin < end) copy_unit(begin, even);
+  if (part < units) copy_unit(part, even);
 
   const size_t at = (static_cast<size_t>(b) * s.sk + min(j, s.sk - 1)) * s.hk * s.d + static_cast<size_t>(hk) * s.d;
   half8 fh[NB * 2], fl[NB * 2];  // K for the probabilities (its sign with scale's), V for ds
@@ -783,8 +784,8 @@ __device__ inline void key_grads(float* __restrict__ dk, float* __restrict__ dv,
   RunningScale qs, gs;
   tile_barrier();
   auto step = [&](const char* now, char* next, int u) {
-    if (u + 1 < end) copy_unit(u + 1, next);
-    const int q0 = (q_first + u % per_head) * kBlock;
+    if (u + parts < units) copy_unit(u + parts, next);
+    const int q0 = (f.q_blocks - 1 - u / group) * kBlock;
     // Whether any of the block's queries sees any of the wave's keys.
     const bool any = first < keys && (!s.causal || first <= q0 + kBlock - 1 + offset);
     const char* t = now + lane * 16 + (of_keys ? kRowBytes<NB> : 0);
@@ -858,9 +859,9 @@ __device__ inline void key_grads(float* __restrict__ dk, float* __restrict__ dv,
     }
     tile_barrier();
   };
-  for (int u = begin; u < end; u += 2) {
+  for (int u = part; u < units; u += 2 * parts) {
     step(even, odd, u);
-    if (u + 1 < end) step(odd, even, u + 1);
+    if (u + parts < units) step(odd, even, u + parts);
   }
   if (j >= s.sk) return;
   const size_t all = static_cast<size_t>(s.b) * s.sk * s.hk * s.d;
