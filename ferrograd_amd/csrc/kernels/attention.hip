@@ -909,8 +909,16 @@ __device__ inline TokenPart token_part(char* ws, size_t index, int D) {
   return {at, at + 16 * D, at + 16 * D + 16};
 }
 
-// ND: columns in units of 64.
-template <int ND>
+// Columns c .. c + 3 of a row, any of the row's own where they lie past its end
+// (they meet zeros of the query, or are not kept).
+template <bool Aligned>
+__device__ inline float4 load4_any(const float* row, int c, int D) {
+  if constexpr (Aligned) return *reinterpret_cast<const float4*>(row + (c < D ? c : 0));
+  return make_float4(row[min(c, D - 1)], row[min(c + 1, D - 1)], row[min(c + 2, D - 1)], row[min(c + 3, D - 1)]);
+}
+
+// ND: columns in units of 64. Aligned: a row starts on 16 bytes.
+template <int ND, bool Aligned>
 __device__ inline void token(float* __restrict__ y, const float* __restrict__ q, const float* __restrict__ k,
                              const float* __restrict__ v, float* __restrict__ stats, const int* __restrict__ lengths,
                              char* __restrict__ ws, const Shape& s, float scale, int splits, int per) {
@@ -932,16 +940,24 @@ __device__ inline void token(float* __restrict__ y, const float* __restrict__ q,
   const float factor = scale * kLog2e;
   float m = -INFINITY, l = 0.f;
   floatx4 o[ND][4] = {};
-  for (int j0 = begin + wave * 16; j0 < end; j0 += 64) {
+  // 16 keys and values, loaded while the wave works on the 16 before.
+  struct Keys {
     float4 kv[ND * 4], vv[4][ND];
+  };
+  auto load = [&](Keys& to, int j0) {
     const float* k_row = k + head + min(j0 + n, end - 1) * stride;
 #pragma unroll
-    for (int t = 0; t < ND * 4; t++) kv[t] = load4(k_row, 16 * t + 4 * quad, s.d);
+    for (int t = 0; t < ND * 4; t++) to.kv[t] = load4_any<Aligned>(k_row, 16 * t + 4 * quad, s.d);
 #pragma unroll
     for (int r = 0; r < 4; r++)
 #pragma unroll
       for (int c = 0; c < ND; c++)
-        vv[r][c] = load4(v + head + min(j0 + 4 * quad + r, end - 1) * stride, 64 * c + 4 * n, s.d);
+        to.vv[r][c] = load4_any<Aligned>(v + head + min(j0 + 4 * quad + r, end - 1) * stride, 64 * c + 4 * n, s.d);
+  };
+  auto step = [&](const Keys& now, Keys& next, int j0) {
+    load(next, j0 + 64);
+    const auto& kv = now.kv;
+    const auto& vv = now.vv;
     floatx4 x = {};
 #pragma unroll
     for (int t = 0; t < ND * 4; t++) {
@@ -983,6 +999,14 @@ __device__ inline void token(float* __restrict__ y, const float* __restrict__ q,
         o[c][2] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[r][c].z, x[r], o[c][2], 0, 0, 0);
         o[c][3] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[r][c].w, x[r], o[c][3], 0, 0, 0);
       }
+  };
+  if (begin + wave * 16 < end) {
+    Keys even, odd;
+    load(even, begin + wave * 16);
+    for (int j0 = begin + wave * 16; j0 < end; j0 += 128) {
+      step(even, odd, j0);
+      if (j0 + 64 < end) step(odd, even, j0 + 64);
+    }
   }
   // The four waves' sums, joined in LDS: o[c][e][r] is row n, column 64 c +
   // 4 (4 quad + r) + e.
@@ -1029,35 +1053,48 @@ __device__ inline void token(float* __restrict__ y, const float* __restrict__ q,
   }
 }
 
-// The parts of a row's keys joined: a workgroup of 128 columns per row.
+// The parts of a row's keys joined, at most 64: a workgroup of 128 columns by
+// four quarters of the parts per row, so that a thread's loads are all in
+// flight at once. The first wave weighs the parts.
 __device__ inline void join_token(float* __restrict__ y, float* __restrict__ stats, char* __restrict__ ws, const Shape& s, int splits) {
+  __shared__ float weights[64], sums[4][128], total;
   const int group = s.hq / s.hk, rows = s.sq * group;
-  const int row = blockIdx.x % rows, hk = blockIdx.x / rows % s.hk, b = blockIdx.x / rows / s.hk, d = threadIdx.x;
+  const int row = blockIdx.x % rows, hk = blockIdx.x / rows % s.hk, b = blockIdx.x / rows / s.hk, lane = threadIdx.x;
   const size_t first = (static_cast<size_t>(b) * s.hk + hk) * splits;
-  // A part without keys has m = 0 and l = 0 and takes no part in the maximum.
-  float top = -INFINITY;
-  for (int p = 0; p < splits; p++) {
-    const TokenPart part = token_part(ws, first + p, s.d);
-    if (part.l[row] > 0.f) top = fmaxf(top, part.m[row]);
-  }
-  if (top == -INFINITY) top = 0.f;
-  float sum = 0.f, all = 0.f;
-  for (int p = 0; p < splits; p++) {
-    const TokenPart part = token_part(ws, first + p, s.d);
-    const float l = part.l[row];
-    if (!(l > 0.f)) continue;
-    const float of = exp2f(part.m[row] - top);
-    sum += of * l;
-    if (d < s.d) all += of * part.o[row * s.d + d];
-  }
   const int i = row / group, h = hk * group + row % group;
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
-  if (d < s.d) y[(static_cast<size_t>(b) * s.sq + i) * s.hq * s.d + static_cast<size_t>(h) * s.d + d] = all * inv;
-  if (d == 0) {
-    const size_t stat = (static_cast<size_t>(b) * s.hq + h) * s.sq + i;
-    stats[stat] = top;
-    stats[static_cast<size_t>(s.b) * s.hq * s.sq + stat] = inv;
+  if (threadIdx.x < 64) {
+    // A part without keys has l = 0 and no say in the maximum.
+    const TokenPart part = token_part(ws, first + min(lane, splits - 1), s.d);
+    const float l = lane < splits ? part.l[row] : 0.f, m = l > 0.f ? part.m[row] : -INFINITY;
+    float top = wave_max(m);
+    top = top == -INFINITY ? 0.f : top;
+    const float weight = l > 0.f ? exp2f(m - top) : 0.f, sum = wave_sum(weight * l);
+    weights[lane] = weight;
+    if (lane == 0) {
+      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      const size_t stat = (static_cast<size_t>(b) * s.hq + h) * s.sq + i;
+      total = inv;
+      stats[stat] = top;
+      stats[static_cast<size_t>(s.b) * s.hq * s.sq + stat] = inv;
+    }
   }
+  const int d = threadIdx.x % 128, quarter = threadIdx.x / 128;
+  float o[16];
+#pragma unroll
+  for (int n = 0; n < 16; n++)
+    o[n] = token_part(ws, first + min(quarter + 4 * n, splits - 1), s.d).o[row * s.d + min(d, s.d - 1)];
+  __syncthreads();
+  float all = 0.f;
+#pragma unroll
+  for (int n = 0; n < 16; n++) {
+    const int p = quarter + 4 * n;
+    if (p < splits && weights[p] > 0.f) all += weights[p] * o[n];  // one without keys holds nothing
+  }
+  sums[quarter][d] = all;
+  __syncthreads();
+  if (quarter == 0 && d < s.d)
+    y[(static_cast<size_t>(b) * s.sq + i) * s.hq * s.d + static_cast<size_t>(h) * s.d + d] =
+        ((sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d])) * total;
 }
 
 }  // namespace
@@ -1104,16 +1141,18 @@ FG_ATTENTION(2)
 FG_ATTENTION(3)
 FG_ATTENTION(4)
 
-#define FG_ATTENTION_TOKEN(ND)                                                                                        \
-  extern "C" __global__ void __launch_bounds__(256) fg_attention_token_##ND(                                          \
+#define FG_ATTENTION_TOKEN(ND, NAME, ALIGNED)                                                                         \
+  extern "C" __global__ void __launch_bounds__(256, 2) fg_attention_token_##NAME(                                     \
       float* y, const float* q, const float* k, const float* v, float* stats, const int* lengths, char* ws, int B,    \
       int Sq, int Sk, int Hq, int Hk, int D, int causal, float scale, int splits, int per) {                          \
-    token<ND>(y, q, k, v, stats, lengths, ws, Shape{B, Sq, Sk, Hq, Hk, D, causal}, scale, splits, per);               \
+    token<ND, ALIGNED>(y, q, k, v, stats, lengths, ws, Shape{B, Sq, Sk, Hq, Hk, D, causal}, scale, splits, per);      \
   }
-FG_ATTENTION_TOKEN(1)
-FG_ATTENTION_TOKEN(2)
+FG_ATTENTION_TOKEN(1, 1, true)
+FG_ATTENTION_TOKEN(2, 2, true)
+FG_ATTENTION_TOKEN(1, 1_any, false)
+FG_ATTENTION_TOKEN(2, 2_any, false)
 
-extern "C" __global__ void __launch_bounds__(128)
+extern "C" __global__ void __launch_bounds__(512)
     fg_attention_token_join(float* y, const float* q, const float* k, const float* v, float* stats, const int* lengths,
                             char* ws, int B, int Sq, int Sk, int Hq, int Hk, int D, int causal, float scale, int splits,
                             int per) {

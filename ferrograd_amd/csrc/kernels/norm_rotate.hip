@@ -258,20 +258,27 @@ FG_NORM_ROTATE(1, 64, 1)
 FG_NORM_ROTATE(1, 64, 2)
 FG_NORM_ROTATE(1, 64, 4)
 
-// dw from the workgroups' sums: 64 columns a workgroup, 16 slices of rows.
+// dw from the workgroups' sums: 16 columns a workgroup, 64 slices of them.
 extern "C" __global__ void __launch_bounds__(1024)
     fg_norm_rotate_weight(float* dx, const float* x, const float* w, const int* positions, const float* g, float* dw,
                           const float* partial, int blocks, int tokens, int heads, int dim, int heads_per, float eps,
                           float log2_base_hi, float log2_base_lo) {
-  __shared__ float sums[16][64];
-  const int col = threadIdx.x % 64, slice = threadIdx.x / 64, d = blockIdx.x * 64 + col;
+  __shared__ float sums[64][16];
+  const int col = threadIdx.x % 16, slice = threadIdx.x / 16, d = blockIdx.x * 16 + col;
   float t = 0.f;
-  if (d < dim)
-    for (int b = slice; b < blocks; b += 16) t += partial[static_cast<size_t>(b) * dim + d];
+  if (d < dim) {
+#pragma unroll 4
+    for (int b = slice; b < blocks; b += 64) t += partial[static_cast<size_t>(b) * dim + d];
+  }
   sums[slice][col] = t;
   __syncthreads();
-  if (slice == 0 && d < dim) {
-    for (int k = 1; k < 16; k++) t += sums[k][col];
-    dw[d] = t;
+  // Four runs of 16 slices, then their sum.
+  if (slice < 4) {
+    t = 0.f;
+    for (int k = 0; k < 16; k++) t += sums[16 * slice + k][col];
   }
+  __syncthreads();
+  if (slice < 4) sums[slice][col] = t;
+  __syncthreads();
+  if (slice == 0 && d < dim) dw[d] = (sums[0][col] + sums[1][col]) + (sums[2][col] + sums[3][col]);
 }

@@ -178,7 +178,7 @@ RenderedKernel render_norm_rotate(const UOp& call, bool grad) {
   } else {
     rk.kind = "norm_rotate_grad";
     rk.launches = {launch("fg_norm_rotate_grad" + r.suffix(), static_cast<uint64_t>(blocks), 256, "norm_rotate"),
-                   launch("fg_norm_rotate_weight", static_cast<uint64_t>((dim + 63) / 64), 1024, "norm_rotate")};
+                   launch("fg_norm_rotate_weight", static_cast<uint64_t>((dim + 15) / 16), 1024, "norm_rotate")};
     rk.workspace_bytes = static_cast<size_t>(blocks * dim) * 4;
     rk.side_outputs = {5};
     for (CallArg a : {CallArg::slot(4), CallArg::slot(5), CallArg::workspace(), CallArg::i32(blocks)}) rk.call_args.push_back(a);
@@ -192,10 +192,33 @@ RenderedKernel render_norm_rotate(const UOp& call, bool grad) {
 // lengths, bits of scale. Sources: q, k, v, [lengths], the stats' storage; of
 // the gradient: q, k, v, y, g, stats, [lengths], dk's and dv's storage.
 
+// In how many parts each 128 keys take their query blocks for dk and dv. The
+// launch fills 256 compute units with one workgroup each, and costs its longest
+// row of workgroups: rounds times (units + about 3 for a workgroup's start and
+// end); with `causal` the first keys' units are twice the average, and parts
+// even them out. Parts are written and summed: 8 bytes an element and part at
+// 5 TB/s, and a launch. A unit takes about 0.9 us per 32 columns.
+int64_t key_grad_parts(int64_t tiles, int64_t units, bool causal, double elements, int64_t nb) {
+  int64_t best = 1;
+  double least = 0;
+  for (int64_t parts = 1; parts <= std::min<int64_t>(units, 16); parts++) {
+    const double each = static_cast<double>(units) / static_cast<double>(parts);
+    const int64_t rounds = (tiles * parts + 255) / 256;
+    double cost = static_cast<double>(rounds) * (each + 3);
+    if (causal) cost = std::max(each + 3, 0.5 * static_cast<double>(tiles * units) / 256 + 3.0 * static_cast<double>(rounds));
+    if (parts > 1) cost += (elements * 8 * static_cast<double>(parts) / 5e6 + 5) / (0.9 * static_cast<double>(nb));
+    if (parts == 1 || cost < least) {
+      best = parts;
+      least = cost;
+    }
+  }
+  return best;
+}
+
 RenderedKernel render_attention(const UOp& call, bool grad) {
   const std::vector<int64_t> p = params_of(call);
   const int64_t batch = p[0], sq = p[1], sk = p[2], heads = p[3], kv_heads = p[4];
-  const bool lengths = p[7] != 0;
+  const bool causal = p[6] != 0, lengths = p[7] != 0;
   RenderedKernel rk;
   set_image(rk, fg_image_attention, fg_image_attention_end);
   std::vector<CallArg> tail;
@@ -212,11 +235,11 @@ RenderedKernel render_attention(const UOp& call, bool grad) {
       splits = std::max<int64_t>(1, std::min({(1024 + pairs - 1) / pairs, sk / 256, int64_t(64)}));
       per = ((sk + splits - 1) / splits + 63) / 64 * 64;
       splits = (sk + per - 1) / per;
-      rk.launches = {launch("fg_attention_token_" + std::to_string(dim <= 64 ? 1 : 2), static_cast<uint64_t>(pairs * splits), 256, "attention")};
+      rk.launches = {launch(std::string("fg_attention_token_") + (dim <= 64 ? "1" : "2") + (dim % 4 ? "_any" : ""), static_cast<uint64_t>(pairs * splits), 256, "attention")};
       rk.workspace_bytes = 4;
       if (splits > 1) {
         rk.workspace_bytes = static_cast<size_t>(pairs * splits) * static_cast<size_t>(16 * dim + 32) * 4;
-        rk.launches.push_back(launch("fg_attention_token_join", static_cast<uint64_t>(batch * heads * sq), 128, "attention"));
+        rk.launches.push_back(launch("fg_attention_token_join", static_cast<uint64_t>(batch * heads * sq), 512, "attention"));
       }
     } else {
       const uint64_t blocks = static_cast<uint64_t>(batch * kv_heads * k_blocks);
@@ -235,10 +258,8 @@ RenderedKernel render_attention(const UOp& call, bool grad) {
     const std::string nbs = "_" + std::to_string(nb);
     const int64_t q_blocks = (sq + 31) / 32, group = heads / kv_heads;
     const uint64_t nk = static_cast<uint64_t>(batch * kv_heads * k_blocks), nq = static_cast<uint64_t>(batch * heads * q_blocks);
-    // Workgroups of 128 keys, each key tile's queries in parts until there are
-    // 1024, of at least 4 query blocks.
     const int64_t tiles = batch * kv_heads * ((sk + 127) / 128), waves = nb < 4 ? 4 : 8;  // kQueryGradWaves
-    const int64_t parts = std::max<int64_t>(1, std::min((1024 + tiles - 1) / tiles, q_blocks * group / 4));
+    const int64_t parts = key_grad_parts(tiles, q_blocks * group, causal, 2.0 * static_cast<double>(batch * sk * kv_heads * dim), nb);
     const uint64_t all = static_cast<uint64_t>(batch * sk * kv_heads * dim);
     rk.workspace_bytes = nk * static_cast<uint64_t>(nb * 12288 + 1024) + nq * static_cast<uint64_t>(nb * 16384 + 1024) +
                          (nk + 3) / 4 * 16 + (parts > 1 ? 8 * all * static_cast<uint64_t>(parts) : 0);
