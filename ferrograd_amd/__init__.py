@@ -138,13 +138,6 @@ def _i64(xs: Iterable[int]):
     return (ctypes.c_int64 * max(1, len(xs)))(*xs), len(xs)
 
 
-def _u64(v, name: str) -> int:
-    v = int(v)
-    if not 0 <= v < 1 << 64:
-        raise FerrogradError(f"{name} must be in [0, 2**64), got {v}")
-    return v
-
-
 def _dev(device) -> int:
     """Device code of a name ("hip", "cpu"), a code, or None: the default
     device, which the DEVICE environment variable selects ("hip" unless set)."""
@@ -286,49 +279,13 @@ class Tensor(_fgc.TensorBase if _fgc is not None else object):
 
     # ── ops (tensor.rs:442-778): neg, reciprocal, exp2, log2, sqrt, relu, exp,
     # log, contiguous, detach, add, mul, sub, matmul, cross_entropy, reshape,
-    # permute, expand, narrow, sum, max, log_softmax, assign and realize are
-    # the extension type's methods (csrc/pymodule.c).
+    # permute, expand, narrow, sum, max, log_softmax, assign and realize,
+    # and the hand-written kernels' attention, norm_rotate and dropout, are the
+    # extension type's methods (csrc/pymodule.c).
 
     def replace(self, other: "Tensor") -> "Tensor":
         _check(lib().fg_tensor_replace(self._h, other._h))
         return self
-
-    # ── hand-written kernels (no reference counterpart) ──────────────────
-    def attention(self, k: "Tensor", v: "Tensor", heads: int, kv_heads: int | None = None, batch: int = 1,
-                  causal: bool = False, lengths: "Tensor | None" = None, scale: float | None = None) -> "Tensor":
-        """softmax(scale q k^T) v per head, with this tensor as q. Matrices
-        have one row per token, as Linear takes and gives them: q [batch * sq,
-        heads * dim], k and v [batch * sk, kv_heads * dim] (f32, dim at most
-        128); kv_heads defaults to heads, scale to dim ** -0.5. Query i of a
-        sequence sees the keys j < lengths[b] (an int32 tensor [batch], clamped
-        to [0, sk]; None: all of them) and, with causal, j <= i + sk - sq; one
-        that sees none gives 0 and gradients of 0. What keys and values past a
-        length hold never matters; everything else must be finite."""
-        if scale is None:
-            cols = self.shape[-1] if self.shape else 0
-            scale = (cols / heads) ** -0.5 if cols and heads > 0 else 1.0
-        return Tensor._out(lib().fg_tensor_attention, self._h, k._h, v._h, lengths._h if lengths is not None else None,
-                           int(batch), int(heads), int(heads if kv_heads is None else kv_heads), int(bool(causal)),
-                           float(scale))
-
-    def norm_rotate(self, weight: "Tensor", positions: "Tensor", heads: int, eps: float = 1e-6,
-                    base: float = 10000.0) -> "Tensor":
-        """RMS norm of each head and the rotation of its position in one pass,
-        for queries and keys [tokens, heads * dim] (f32, dim even and at most
-        512): z = x * (mean(x**2) + eps) ** -0.5 * weight (f32 [dim]), then the
-        pair (z_i, z_{i + dim/2}) turned by positions[token] * base**(-2i/dim)
-        (positions int32 [tokens])."""
-        return Tensor._out(lib().fg_tensor_norm_rotate, self._h, weight._h, positions._h, int(heads), float(eps),
-                           float(base))
-
-    def dropout(self, p: float, seed: int, offset: int = 0) -> "Tensor":
-        """x / (1 - p) where the element's random word is at least
-        floor(p * 2**32), else 0 (an f32 tensor of any shape; 0 <= p < 1). Element e's word is word e % 4 of Philox4x32-10 of the
-        counter (e // 4, offset) under the key `seed`: 64 bits each, so the
-        same seed and offset drop the same elements, and the gradient draws
-        the mask again. Use a new offset for every call that should draw
-        anew (Dropout does)."""
-        return Tensor._out(lib().fg_tensor_dropout, self._h, float(p), _u64(seed, "seed"), _u64(offset, "offset"))
 
     # ── realisation (tensor.rs:781-930) ──────────────────────────────────
     @staticmethod

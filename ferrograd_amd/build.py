@@ -54,7 +54,7 @@ def build_python_module() -> str:
     tmp = out + ".tmp"
     _run(["gcc", "-O2", "-g0", "-fPIC", "-shared", "-Wall", "-I" + sysconfig.get_paths()["include"],
           "-I" + os.path.join(ROOT, "include"), os.path.join(CSRC, "pymodule.c"), "-o", tmp,
-          "-L" + HERE, "-lferrograd_amd", "-Wl,-rpath,$ORIGIN"])
+          "-L" + HERE, "-lferrograd_amd", "-lm", "-Wl,-rpath,$ORIGIN"])
     os.replace(tmp, out)
     return out
 

@@ -359,16 +359,105 @@ __device__ inline void store_columns(float* row, int n, int half, int D, const f
   }
 }
 
-// Which `rows` queries, head and batch a workgroup takes. The last queries of
-// every head come first: with `causal` they see the most keys, and what is
-// left for the end is small. Workgroups go to the 8 chiplets in turn, so
+// ── keys in parts ───────────────────────────────────────────────────────────
+// Where the query rows alone are too few workgroups, each takes a part of the
+// keys and leaves, per row (b, h, i), the sum of exp2(S_ij log2 e - m) v_j, m,
+// and the sum of the exponentials (0: it saw no key, and the rest is nothing).
+struct RowParts {
+  float* o;   // [split][row][D]
+  float* ml;  // [split][row][2]
+  size_t rows;
+};
+
+__device__ inline RowParts row_parts(char* at, const Shape& s, int splits) {
+  RowParts p;
+  p.rows = static_cast<size_t>(s.b) * s.hq * s.sq;
+  p.o = reinterpret_cast<float*>(at);
+  p.ml = p.o + splits * p.rows * s.d;
+  return p;
+}
+
+// The parts joined: a thread per row and W columns, N parts at a time in flight.
+// The stats are written by the row's first column.
+template <int N, int W>
+__device__ inline void join_columns(float* __restrict__ y, float* __restrict__ stats, const RowParts& parts, const Shape& s,
+                                    int splits) {
+  const size_t e = (static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x) * W;
+  if (e >= parts.rows * s.d) return;
+  const size_t row = e / s.d;
+  const int d = e % s.d;
+  float top = -INFINITY, sum = 0.f, all[W] = {};
+  for (int p0 = 0; p0 < splits; p0 += N) {
+    float2 ml[N];
+    float o[N][W];
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+      const size_t part = min(p0 + n, splits - 1) * parts.rows + row;
+      ml[n] = *reinterpret_cast<const float2*>(parts.ml + 2 * part);
+      if constexpr (W == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(parts.o + part * s.d + d);
+        o[n][0] = v.x;
+        o[n][1] = v.y;
+        o[n][2] = v.z;
+        o[n][3] = v.w;
+      } else {
+        o[n][0] = parts.o[part * s.d + d];
+      }
+    }
+    float most = top;
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+      if (p0 + n >= splits) ml[n].y = 0.f;
+      if (ml[n].y > 0.f) most = fmaxf(most, ml[n].x);
+    }
+    if (most == -INFINITY) continue;
+    const float old = exp2f(top - most);
+    sum *= old;
+#pragma unroll
+    for (int w = 0; w < W; w++) all[w] *= old;
+    top = most;
+#pragma unroll
+    for (int n = 0; n < N; n++)
+      if (ml[n].y > 0.f) {
+        const float of = exp2f(ml[n].x - top);
+        sum += of * ml[n].y;
+#pragma unroll
+        for (int w = 0; w < W; w++) all[w] += of * o[n][w];
+      }
+  }
+  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  const int i = row % s.sq, h = row / s.sq % s.hq;
+  const size_t b = row / s.sq / s.hq;
+  float* out = y + (b * s.sq + i) * s.hq * s.d + static_cast<size_t>(h) * s.d + d;
+#pragma unroll
+  for (int w = 0; w < W; w++) all[w] *= inv;
+  if constexpr (W == 4) *reinterpret_cast<float4*>(out) = make_float4(all[0], all[1], all[2], all[3]);
+  else *out = all[0];
+  if (d == 0) {
+    stats[row] = top == -INFINITY ? 0.f : top;
+    stats[parts.rows + row] = inv;
+  }
+}
+
+template <int W>
+__device__ inline void join_parts(float* __restrict__ y, float* __restrict__ stats, char* __restrict__ at, const Shape& s,
+                                  int splits) {
+  const RowParts parts = row_parts(at, s, splits);
+  if (splits <= 4) join_columns<4, W>(y, stats, parts, s, splits);
+  else join_columns<16, W>(y, stats, parts, s, splits);
+}
+
+// Which `rows` queries, head, batch and part of the keys a workgroup takes. The
+// last queries of every head come first: with `causal` they see the most keys,
+// and what is left for the end is small. Workgroups go to the 8 chiplets in turn, so
 // where the heads allow it each chiplet gets heads next to each other, which
 // share keys in its cache.
-__device__ inline void query_tile(const Shape& s, int rows, int* qt, int* h, int* b) {
+__device__ inline void query_tile(const Shape& s, int rows, int splits, int* qt, int* h, int* b, int* split) {
   const unsigned heads = static_cast<unsigned>(s.b) * s.hq, tiles = (s.sq + rows - 1) / rows;
   unsigned head = blockIdx.x % heads;
   if (heads % 8 == 0) head = head % 8 * (heads / 8) + head / 8;
-  *qt = tiles - 1 - blockIdx.x / heads;
+  *split = blockIdx.x / heads % splits;
+  *qt = tiles - 1 - blockIdx.x / heads / splits;
   *h = head % s.hq;
   *b = head / s.hq;
 }
@@ -379,60 +468,62 @@ __device__ inline void query_tile(const Shape& s, int rows, int* qt, int* h, int
 // are in registers what O^T += V^T P^T takes as its second operand.
 template <int NB>
 __device__ inline void forward_tiles(float* __restrict__ y, const float* __restrict__ q, float* __restrict__ stats,
-                                     const int* __restrict__ lengths, char* __restrict__ ws, int B, int Sq, int Sk,
-                                     int Hq, int Hk, int D, int causal, float scale) {
+                                     const int* __restrict__ lengths, char* __restrict__ ws, const Shape& s, float scale,
+                                     int splits) {
   constexpr int kTile = kForwardTile<NB>;
   // Two buffers of their own, and a loop written out twice: the compiler then
   // knows that what a step reads is not what its copies write, and does not
   // wait for them first.
   __shared__ __attribute__((aligned(1024))) char even[kTile], odd[kTile];
-  int qt, h, b;
-  query_tile(Shape{B, Sq, Sk, Hq, Hk, D, causal}, 128, &qt, &h, &b);
-  const int hk = h / (Hq / Hk);
+  int qt, h, b, split;
+  query_tile(s, 128, splits, &qt, &h, &b, &split);
+  const int hk = h / (s.hq / s.hk);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, half = lane / 32;
   const int i = qt * 128 + wave * 32 + lane % 32;  // this lane's query
-  const bool live = i < Sq;
-  const int keys = lengths ? min(max(lengths[b], 0), Sk) : Sk;
-  // Keys that the last query of the workgroup, of the wave, and this lane's see.
-  auto seen_by = [&](int row) { return causal ? max(0, min(keys, row + Sk - Sq + 1)) : keys; };
-  const int block_end = (seen_by(min(Sq, qt * 128 + 128) - 1) + kBlock - 1) / kBlock;
-  const int wave_last = min(Sq, qt * 128 + wave * 32 + 32) - 1;
-  const int wave_end = wave_last >= qt * 128 + wave * 32 ? (seen_by(wave_last) + kBlock - 1) / kBlock : 0;
-  const int wave_full = seen_by(qt * 128 + wave * 32) / kBlock;  // blocks that every query of the wave sees whole
-  const int seen = live ? seen_by(i) : 0;
+  const bool live = i < s.sq;
+  const int keys = key_count(s, lengths, b), first = qt * 128 + wave * 32;
+  // Blocks of keys that the last query of the workgroup sees, of which this
+  // part takes those from `begin` to `end`; those that the last of the wave
+  // sees; those that every query of the wave sees whole.
+  const int blocks = (visible(s, keys, min(s.sq, qt * 128 + 128) - 1) + kBlock - 1) / kBlock;
+  const int begin = static_cast<int>(static_cast<long long>(blocks) * split / splits);
+  const int end = static_cast<int>(static_cast<long long>(blocks) * (split + 1) / splits);
+  const int wave_end = first < s.sq ? (visible(s, keys, min(s.sq, first + 32) - 1) + kBlock - 1) / kBlock : 0;
+  const int wave_full = visible(s, keys, first) / kBlock;
+  const int seen = live ? visible(s, keys, i) : 0;
 
-  const size_t head = static_cast<size_t>(b) * Hk + hk;
-  const char* tile = ws + head * ((Sk + kBlock - 1) / kBlock) * kTile;
-  if (block_end > 0) copy_tile<kTile, 4>(tile, even);
+  const size_t head = static_cast<size_t>(b) * s.hk + hk, head_blocks = (s.sk + kBlock - 1) / kBlock;
+  const char* tile = ws + head * head_blocks * kTile;
+  if (begin < end) copy_tile<kTile, 4>(tile + static_cast<size_t>(begin) * kTile, even);
 
   half8 qh[NB * 2], ql[NB * 2];
-  const int eq = row_fragments<NB>(q + (static_cast<size_t>(b) * Sq + min(i, Sq - 1)) * Hq * D + static_cast<size_t>(h) * D, live,
-                                   D, scale < 0.f ? -1.f : 1.f, 1.f, qh, ql);
+  const int eq = row_fragments<NB>(q + (static_cast<size_t>(b) * s.sq + min(i, s.sq - 1)) * s.hq * s.d + static_cast<size_t>(h) * s.d,
+                                   live, s.d, scale < 0.f ? -1.f : 1.f, 1.f, qh, ql);
   const float factor = fabsf(scale) * kLog2e;
   float m = -INFINITY, l = 0.f;
   floatx16 o[NB] = {};
   RunningScale vs;
   tile_barrier();
   auto step = [&](const char* now, char* next, int kb) {
-    if (kb + 1 < block_end) copy_tile<kTile, 4>(tile + static_cast<size_t>(kb + 1) * kTile, next);
+    if (kb + 1 < end) copy_tile<kTile, 4>(tile + static_cast<size_t>(kb + 1) * kTile, next);
     if (kb < wave_end) {
       const char* t = now + lane * 16;
       const int* tail = reinterpret_cast<const int*>(now + kTile - kTail);
       const int ek = uniform(tail[0]), ev = uniform(tail[1]);
-      floatx16 s = {};
+      floatx16 x = {};
 #pragma unroll
       for (int n = 0; n < NB * 2; n++)
-        s = mfma3(*reinterpret_cast<const half8*>(t + n * 2 * kPart), *reinterpret_cast<const half8*>(t + n * 2 * kPart + kPart),
-                  qh[n], ql[n], s);
+        x = mfma3(*reinterpret_cast<const half8*>(t + n * 2 * kPart), *reinterpret_cast<const half8*>(t + n * 2 * kPart + kPart),
+                  qh[n], ql[n], x);
       float fac = ldexpf(factor, -(eq + ek));
       if (kb >= wave_full) {
 #pragma unroll
-        for (int r = 0; r < 16; r++) s[r] = kb * kBlock + result_row(r, half) < seen ? s[r] * fac : -INFINITY;
+        for (int r = 0; r < 16; r++) x[r] = kb * kBlock + result_row(r, half) < seen ? x[r] * fac : -INFINITY;
         fac = 1.f;
       }
-      float top = s[0];
+      float top = x[0];
 #pragma unroll
-      for (int r = 1; r < 16; r++) top = fmaxf(top, s[r]);
+      for (int r = 1; r < 16; r++) top = fmaxf(top, x[r]);
       top = halves_max(top) * fac;
       int behind;
       const int change = vs.take(ev, &behind);
@@ -457,15 +548,15 @@ __device__ inline void forward_tiles(float* __restrict__ y, const float* __restr
       float sum = 0.f;
 #pragma unroll
       for (int r = 0; r < 16; r++) {
-        s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], fac, base));
-        sum += s[r];
+        x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], fac, base));
+        sum += x[r];
       }
       l += ldexpf(sum, behind - kProbShift);
 #pragma unroll
       for (int u = 0; u < 2; u++) {
         float p[8];
 #pragma unroll
-        for (int r = 0; r < 8; r++) p[r] = s[8 * u + r];
+        for (int r = 0; r < 8; r++) p[r] = x[8 * u + r];
         half8 ph, pl;
         cut_probs(p, &ph, &pl);
         const char* vt = t + kRowBytes<NB> + u * 2 * kPart;
@@ -477,20 +568,31 @@ __device__ inline void forward_tiles(float* __restrict__ y, const float* __restr
     }
     tile_barrier();
   };
-  for (int kb = 0; kb < block_end; kb += 2) {
+  for (int kb = begin; kb < end; kb += 2) {
     step(even, odd, kb);
-    if (kb + 1 < block_end) step(odd, even, kb + 1);
+    if (kb + 1 < end) step(odd, even, kb + 1);
   }
   l = halves_sum(l);
-  const float inv = l > 0.f ? 1.f / l : 0.f;
   if (!live) return;
-  float* row = y + (static_cast<size_t>(b) * Sq + i) * Hq * D + static_cast<size_t>(h) * D;
+  const size_t stat = (static_cast<size_t>(b) * s.hq + h) * s.sq + i, rows = static_cast<size_t>(s.b) * s.hq * s.sq;
+  if (splits > 1) {
+    const RowParts parts = row_parts(ws + static_cast<size_t>(s.b) * s.hk * head_blocks * kTile, s, splits);
+    const size_t out = split * rows + stat;
 #pragma unroll
-  for (int n = 0; n < NB; n++) store_columns(row, n, half, D, o[n], inv, -kProbShift - vs.ref);
+    for (int n = 0; n < NB; n++) store_columns(parts.o + out * s.d, n, half, s.d, o[n], 1.f, -kProbShift - vs.ref);
+    if (half == 0) {
+      parts.ml[2 * out] = m;
+      parts.ml[2 * out + 1] = l;
+    }
+    return;
+  }
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  float* row = y + (static_cast<size_t>(b) * s.sq + i) * s.hq * s.d + static_cast<size_t>(h) * s.d;
+#pragma unroll
+  for (int n = 0; n < NB; n++) store_columns(row, n, half, s.d, o[n], inv, -kProbShift - vs.ref);
   if (half == 0) {
-    const size_t at = (static_cast<size_t>(b) * Hq + h) * Sq + i;
-    stats[at] = m == -INFINITY ? 0.f : m;
-    stats[static_cast<size_t>(B) * Hq * Sq + at] = inv;
+    stats[stat] = m == -INFINITY ? 0.f : m;
+    stats[rows + stat] = inv;
   }
 }
 
@@ -511,7 +613,8 @@ constexpr int kScoreShift = 12;  // 15, less kLazy and one for the twice
 // head and block of 32 queries: the tile [Q rows | G rows | Q columns | G
 // columns | m, delta of each row, exponents of Q, G and of G's largest row
 // norm] (G = g'); then the exponents of the key blocks' largest row norms of V;
-// then dk and dv of each part.
+// then dk and dv of each part of the queries, and dq of each part of the keys,
+// where there is more than one.
 template <int NB>
 constexpr int kKeyTile = 2 * kRowBytes<NB> + kColBytes<NB> + kTail;
 template <int NB>
@@ -535,6 +638,11 @@ __device__ inline GradSpace grad_space(char* ws, const Shape& s) {
   g.norms = reinterpret_cast<int*>(g.q_tiles + nq * kQueryTile<NB>);
   g.parts = reinterpret_cast<float*>(g.norms + (nk + 3) / 4 * 4);
   return g;
+}
+
+// Floats of the parts of dk and dv.
+__device__ inline size_t key_parts(const Shape& s, int parts) {
+  return parts > 1 ? 2 * static_cast<size_t>(parts) * s.b * s.sk * s.hk * s.d : 0;
 }
 
 // The power of two above a norm, from the largest sum of squares of a block's
@@ -641,26 +749,28 @@ constexpr int kQueryGradWaves = NB < 4 ? 4 : 8;
 template <int NB, int Waves>
 __device__ inline void query_grads(float* __restrict__ dq, const float* __restrict__ q, const float* __restrict__ g,
                                    const float* __restrict__ stats, const int* __restrict__ lengths,
-                                   char* __restrict__ ws, const Shape& s, float scale) {
+                                   char* __restrict__ ws, const Shape& s, float scale, int parts, int q_parts) {
   constexpr int kTile = kKeyTile<NB>;
   __shared__ __attribute__((aligned(1024))) char even[kTile], odd[kTile];
   const GradSpace f = grad_space<NB>(ws, s);
-  int qt, h, b;
+  int qt, h, b, part;
   constexpr int kRows = 32 * Waves;
-  query_tile(s, kRows, &qt, &h, &b);
+  query_tile(s, kRows, q_parts, &qt, &h, &b, &part);
   const int hk = h / (s.hq / s.hk);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, half = lane / 32;
   const int first = qt * kRows + wave * 32, i = first + lane % 32;
   const bool live = i < s.sq, wave_live = first < s.sq;
   const int keys = key_count(s, lengths, b);
-  const int block_end = (visible(s, keys, min(s.sq, qt * kRows + kRows) - 1) + kBlock - 1) / kBlock;
+  const int blocks = (visible(s, keys, min(s.sq, qt * kRows + kRows) - 1) + kBlock - 1) / kBlock;
+  const int begin = static_cast<int>(static_cast<long long>(blocks) * part / q_parts);
+  const int end = static_cast<int>(static_cast<long long>(blocks) * (part + 1) / q_parts);
   const int wave_end = wave_live ? (visible(s, keys, min(s.sq, first + 32) - 1) + kBlock - 1) / kBlock : 0;
   const int wave_full = visible(s, keys, first) / kBlock;
   const int seen = live ? visible(s, keys, i) : 0;
 
   const size_t head = static_cast<size_t>(b) * s.hk + hk;
   const char* tile = f.k_tiles + head * f.k_blocks * kTile;
-  if (block_end > 0) copy_tile<kTile, Waves>(tile, even);
+  if (begin < end) copy_tile<kTile, Waves>(tile + static_cast<size_t>(begin) * kTile, even);
 
   const size_t at = (static_cast<size_t>(b) * s.sq + min(i, s.sq - 1)) * s.hq * s.d + static_cast<size_t>(h) * s.d;
   const size_t stat = (static_cast<size_t>(b) * s.hq + h) * s.sq + min(i, s.sq - 1);
@@ -679,7 +789,7 @@ __device__ inline void query_grads(float* __restrict__ dq, const float* __restri
   RunningScale ks;
   tile_barrier();
   auto step = [&](const char* now, char* next, int kb) {
-    if (kb + 1 < block_end) copy_tile<kTile, Waves>(tile + static_cast<size_t>(kb + 1) * kTile, next);
+    if (kb + 1 < end) copy_tile<kTile, Waves>(tile + static_cast<size_t>(kb + 1) * kTile, next);
     if (kb < wave_end) {
       const char* t = now + lane * 16;
       const int* tail = reinterpret_cast<const int*>(now + kTile - kTail);
@@ -726,11 +836,12 @@ __device__ inline void query_grads(float* __restrict__ dq, const float* __restri
     }
     tile_barrier();
   };
-  for (int kb = 0; kb < block_end; kb += 2) {
+  for (int kb = begin; kb < end; kb += 2) {
     step(even, odd, kb);
-    if (kb + 1 < block_end) step(odd, even, kb + 1);
+    if (kb + 1 < end) step(odd, even, kb + 1);
   }
   if (!live) return;
+  if (q_parts > 1) dq = f.parts + key_parts(s, parts) + part * (static_cast<size_t>(s.b) * s.sq * s.hq * s.d);
 #pragma unroll
   for (int n = 0; n < NB; n++) store_columns(dq + at, n, half, s.d, o[n], scale, -shift - ks.ref);
 }
@@ -743,12 +854,20 @@ __device__ inline void query_grads(float* __restrict__ dq, const float* __restri
 // core to itself, waiting while it does anything else), at the price of the
 // probabilities' way through LDS. Scores are not transposed here: a lane holds
 // 16 queries of one key, which is what dv^T += G^T P and dk^T += Q^T dS take.
+//
+// The rows of a tile are read before the probabilities' barrier, its columns
+// after it. Up to two column groups they have one buffer each, refilled while
+// the other is read, so that two workgroups fit a compute unit and
+// cover each other's waits. More groups leave room for one workgroup, with two
+// buffers of whole tiles.
 template <int NB>
 __device__ inline void key_grads(float* __restrict__ dk, float* __restrict__ dv, const float* __restrict__ k,
                                  const float* __restrict__ v, const int* __restrict__ lengths, char* __restrict__ ws,
                                  const Shape& s, float scale, int parts) {
   constexpr int kTile = kQueryTile<NB>, Waves = 8;
-  __shared__ __attribute__((aligned(1024))) char even[kTile], odd[kTile];
+  constexpr bool kTwo = NB > 2;  // two buffers
+  constexpr int kRows = 2 * kRowBytes<NB> + kTail, kCols = 2 * kColBytes<NB>;
+  __shared__ __attribute__((aligned(1024))) char rows_a[kRows], cols_a[kCols], rows_b[kTwo ? kRows : kPart], cols_b[kTwo ? kCols : kPart];
   __shared__ float4 probs[4][4][64];  // [pair][registers 4 c .. 4 c + 3][lane]
   const GradSpace f = grad_space<NB>(ws, s);
   // The first keys are seen by the most queries: first.
@@ -769,11 +888,18 @@ __device__ inline void key_grads(float* __restrict__ dk, float* __restrict__ dv,
   const int units = kt * 128 < keys ? max(0, f.q_blocks - q_first) * group : 0;
 
   const size_t q_head = (static_cast<size_t>(b) * s.hq + static_cast<size_t>(hk) * group) * f.q_blocks;
-  auto copy_unit = [&](int u, char* to) {
-    const size_t block = q_head + static_cast<size_t>(u % group) * f.q_blocks + (f.q_blocks - 1 - u / group);
-    copy_tile<kTile, Waves>(f.q_tiles + block * kTile, to);
+  auto unit_tile = [&](int u) {
+    return f.q_tiles + (q_head + static_cast<size_t>(u % group) * f.q_blocks + (f.q_blocks - 1 - u / group)) * kTile;
   };
-  if (part < units) copy_unit(part, even);
+  auto copy_rows = [&](int u, char* to) {
+    copy_tile<2 * kRowBytes<NB>, Waves>(unit_tile(u), to);
+    copy_tile<kTail, Waves>(unit_tile(u) + kTile - kTail, to + 2 * kRowBytes<NB>);
+  };
+  auto copy_cols = [&](int u, char* to) { copy_tile<kCols, Waves>(unit_tile(u) + 2 * kRowBytes<NB>, to); };
+  if (part < units) {
+    copy_rows(part, rows_a);
+    copy_cols(part, cols_a);
+  }
 
   const size_t at = (static_cast<size_t>(b) * s.sk + min(j, s.sk - 1)) * s.hk * s.d + static_cast<size_t>(hk) * s.d;
   half8 fh[NB * 2], fl[NB * 2];  // K for the probabilities (its sign with scale's), V for ds
@@ -783,15 +909,23 @@ __device__ inline void key_grads(float* __restrict__ dk, float* __restrict__ dv,
   floatx16 o[NB] = {};
   RunningScale qs, gs;
   tile_barrier();
-  auto step = [&](const char* now, char* next, int u) {
-    if (u + parts < units) copy_unit(u + parts, next);
+  auto step = [&](const char* rows, const char* cols, char* next_rows, char* next_cols, int u) {
+    const bool more = u + parts < units;
+    if (kTwo && more) {
+      copy_rows(u + parts, next_rows);
+      copy_cols(u + parts, next_cols);
+    }
     const int q0 = (f.q_blocks - 1 - u / group) * kBlock;
     // Whether any of the block's queries sees any of the wave's keys.
     const bool any = first < keys && (!s.causal || first <= q0 + kBlock - 1 + offset);
-    const char* t = now + lane * 16 + (of_keys ? kRowBytes<NB> : 0);
-    const float* tail = reinterpret_cast<const float*>(now + kTile - kTail);
+    const char* t = rows + lane * 16 + (of_keys ? kRowBytes<NB> : 0);
+    const float* tail = reinterpret_cast<const float*>(rows + 2 * kRowBytes<NB>);
     const int* exponents = reinterpret_cast<const int*>(tail) + 64;
     const int eq = uniform(exponents[0]), eg = uniform(exponents[1]), shift = clamp_power(kScoreShift - uniform(exponents[2]) - norm);
+    // m for the probabilities, delta for ds.
+    float4 of_row[4];
+#pragma unroll
+    for (int c = 0; c < 4; c++) of_row[c] = *reinterpret_cast<const float4*>(tail + (of_keys ? 32 : 0) + 8 * c + 4 * half);
     floatx16 x = {};
     int change = 0, up = 0, q_behind = 0;
     if (any) {
@@ -808,8 +942,7 @@ __device__ inline void key_grads(float* __restrict__ dk, float* __restrict__ dv,
         const bool whole = !s.causal || first + 31 <= q0 + offset;
 #pragma unroll
         for (int c = 0; c < 4; c++) {
-          const float4 mm = *reinterpret_cast<const float4*>(tail + 8 * c + 4 * half);
-          const float m4[4] = {mm.x, mm.y, mm.z, mm.w};
+          const float m4[4] = {of_row[c].x, of_row[c].y, of_row[c].z, of_row[c].w};
 #pragma unroll
           for (int i = 0; i < 4; i++) {
             float p = __builtin_amdgcn_exp2f(fmaf(x[4 * c + i], fac, static_cast<float>(up) - m4[i]));
@@ -820,10 +953,17 @@ __device__ inline void key_grads(float* __restrict__ dk, float* __restrict__ dv,
         }
       }
     }
-    // The probabilities are in LDS. (No wait for the copies.)
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
+    // The probabilities are in LDS, every wave is done with the rows, and, with
+    // one buffer, the columns are there. (With two they are since the step
+    // began, and its copies are not waited for.)
+    if constexpr (kTwo) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+    } else {
+      tile_barrier();
+      if (more) copy_rows(u + parts, next_rows);
+    }
     if (any) {
       if (of_keys) {
         // ds, with what p carries taken off again.
@@ -831,8 +971,8 @@ __device__ inline void key_grads(float* __restrict__ dk, float* __restrict__ dv,
         const float of_dp = power(off - eg - e), of_delta = power(off);
 #pragma unroll
         for (int c = 0; c < 4; c++) {
-          const float4 pp = probs[pair][c][lane], dd = *reinterpret_cast<const float4*>(tail + 32 + 8 * c + 4 * half);
-          const float p4[4] = {pp.x, pp.y, pp.z, pp.w}, d4[4] = {dd.x, dd.y, dd.z, dd.w};
+          const float4 pp = probs[pair][c][lane];
+          const float p4[4] = {pp.x, pp.y, pp.z, pp.w}, d4[4] = {of_row[c].x, of_row[c].y, of_row[c].z, of_row[c].w};
 #pragma unroll
           for (int i = 0; i < 4; i++) x[4 * c + i] = p4[i] * fmaf(x[4 * c + i], of_dp, -d4[i] * of_delta);
         }
@@ -843,7 +983,7 @@ __device__ inline void key_grads(float* __restrict__ dk, float* __restrict__ dv,
 #pragma unroll
           for (int r = 0; r < 16; r++) o[n][r] = ldexpf(o[n][r], change);
       }
-      const char* columns = now + lane * 16 + 2 * kRowBytes<NB> + (of_keys ? 0 : kColBytes<NB>);
+      const char* columns = cols + lane * 16 + (of_keys ? 0 : kColBytes<NB>);
 #pragma unroll
       for (int w = 0; w < 2; w++) {
         float p[8];
@@ -858,10 +998,15 @@ __device__ inline void key_grads(float* __restrict__ dk, float* __restrict__ dv,
       }
     }
     tile_barrier();
+    if (!kTwo && more) copy_cols(u + parts, next_cols);
   };
-  for (int u = part; u < units; u += 2 * parts) {
-    step(even, odd, u);
-    if (u + parts < units) step(odd, even, u + parts);
+  if constexpr (kTwo) {
+    for (int u = part; u < units; u += 2 * parts) {
+      step(rows_a, cols_a, rows_b, cols_b, u);
+      if (u + parts < units) step(rows_b, cols_b, rows_a, cols_a, u + parts);
+    }
+  } else {
+    for (int u = part; u < units; u += parts) step(rows_a, cols_a, rows_a, cols_a, u);
   }
   if (j >= s.sk) return;
   const size_t all = static_cast<size_t>(s.b) * s.sk * s.hk * s.d;
@@ -877,37 +1022,26 @@ __device__ inline void key_grads(float* __restrict__ dk, float* __restrict__ dv,
     store_columns(out + at, n, half, s.d, o[n], of_keys ? scale : 1.f, of_keys ? -qs.ref : -kProbShift - gs.ref);
 }
 
-// dk and dv from their parts, in order.
-__device__ inline void sum_parts(float* __restrict__ dk, float* __restrict__ dv, const float* __restrict__ partial,
-                                 size_t n, int parts) {
-  for (size_t e = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x; e < 2 * n; e += static_cast<size_t>(gridDim.x) * 256) {
+// Sums of parts, in order: element e of two arrays of n in a row.
+__device__ inline void sum_parts(float* __restrict__ first, float* __restrict__ second, const float* __restrict__ parts,
+                                 size_t n, size_t all, int count) {
+  for (size_t e = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x; e < all; e += static_cast<size_t>(gridDim.x) * 256) {
     float t = 0.f;
-    for (int part = 0; part < parts; part++) t += partial[2 * n * part + e];
-    (e < n ? dk : dv - n)[e] = t;
+    for (int part = 0; part < count; part++) t += parts[all * part + e];
+    if (e < n) first[e] = t;
+    else second[e - n] = t;
   }
 }
 
-// ── few queries ─────────────────────────────────────────────────────────────
-// At most 16 query rows per key head (queries times the heads that share it):
-// a token at a time, where reading the keys and values is all the work. They
-// are read once, as they are, by float32 matrix products, so nothing is cut or
-// staged. A wave takes 16 keys at a time: S (16 keys x 16 rows) = K Q^T, lane l
-// holding key l % 16 and every fourth group of 4 columns, and O^T += V^T P with
-// the four terms of a product taken as lane l's result rows, 4 (l / 16) + r: P
-// is used where it is. The keys of a head are split over workgroups until these
-// fill the chip, and joined by a second launch.
-
-// A workgroup's part of the keys of one (b, hk): the rows' sums so far.
-struct TokenPart {
-  float* o;  // [16][D]
-  float* m;  // [16], units of log2
-  float* l;  // [16]
-};
-
-__device__ inline TokenPart token_part(char* ws, size_t index, int D) {
-  float* at = reinterpret_cast<float*>(ws) + index * (16 * D + 32);
-  return {at, at + 16 * D, at + 16 * D + 16};
-}
+// ── small calls ─────────────────────────────────────────────────────────────
+// A token at a time, where reading the keys and values is all the work, and
+// calls too small to cut their operands for. 16 query rows of one key head
+// (query times the heads that share it) a workgroup; keys and values are read
+// as they are, by float32 matrix products. A wave takes 16 keys at a time: S
+// (16 keys x 16 rows) = K Q^T, lane l holding key l % 16 and every fourth group
+// of 4 columns, and O^T += V^T P with the four terms of a product taken as lane
+// l's result rows, 4 (l / 16) + r: P is used where it is. Keys are split over
+// workgroups until these fill the chip, and joined by a second launch.
 
 // Columns c .. c + 3 of a row, any of the row's own where they lie past its end
 // (they meet zeros of the query, or are not kept).
@@ -922,14 +1056,18 @@ template <int ND, bool Aligned>
 __device__ inline void token(float* __restrict__ y, const float* __restrict__ q, const float* __restrict__ k,
                              const float* __restrict__ v, float* __restrict__ stats, const int* __restrict__ lengths,
                              char* __restrict__ ws, const Shape& s, float scale, int splits, int per) {
+  // blockIdx.x: (b, hk, 16 rows, split)
   __shared__ float merged[4][16 * ND * 64];
   __shared__ float ms[4][16], ls[4][16];
-  const int split = blockIdx.x % splits, hk = blockIdx.x / splits % s.hk, b = blockIdx.x / splits / s.hk;
+  const int group = s.hq / s.hk, tiles = (s.sq * group + 15) / 16;
+  const int split = blockIdx.x % splits, tile = blockIdx.x / splits % tiles;
+  const int hk = blockIdx.x / splits / tiles % s.hk, b = blockIdx.x / splits / tiles / s.hk;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
-  const int n = lane % 16, quad = lane / 16, group = s.hq / s.hk, rows = s.sq * group;
-  const int keys = key_count(s, lengths, b), begin = split * per, end = min(keys, begin + per);
-  // Row n of the products: query n / group, head hk * group + n % group.
-  const int i = min(n, rows - 1) / group, h = hk * group + min(n, rows - 1) % group;
+  const int n = lane % 16, quad = lane / 16, first = tile * 16, rows = min(16, s.sq * group - first);
+  // Row n of the products: query (first + n) / group, head hk * group + (first + n) % group.
+  const int row = first + min(n, rows - 1), i = row / group, h = hk * group + row % group;
+  const int keys = key_count(s, lengths, b), begin = split * per;
+  const int end = min(visible(s, keys, (first + rows - 1) / group), begin + per);
   const int seen = n < rows ? min(end, visible(s, keys, i)) : 0;
   const float* q_row = q + (static_cast<size_t>(b) * s.sq + i) * s.hq * s.d + static_cast<size_t>(h) * s.d;
   const size_t stride = static_cast<size_t>(s.hk) * s.d;
@@ -1023,7 +1161,7 @@ __device__ inline void token(float* __restrict__ y, const float* __restrict__ q,
       *reinterpret_cast<float4*>(&merged[wave][n * ND * 64 + 64 * c + 4 * (4 * quad + r)]) =
           make_float4(o[c][0][r], o[c][1][r], o[c][2][r], o[c][3][r]);
   __syncthreads();
-  const TokenPart part = token_part(ws, blockIdx.x, s.d);
+  const RowParts parts = row_parts(ws, s, splits);
   for (int at = threadIdx.x; at < rows * ND * 64; at += 256) {
     const int row = at / (ND * 64), d = at % (ND * 64);
     float top = fmaxf(fmaxf(ms[0][row], ms[1][row]), fmaxf(ms[2][row], ms[3][row]));
@@ -1034,67 +1172,24 @@ __device__ inline void token(float* __restrict__ y, const float* __restrict__ q,
       sum += of * ls[w][row];
       all += of * merged[w][row * ND * 64 + d];
     }
+    const int iq = (first + row) / group, hq = hk * group + (first + row) % group;
+    const size_t stat = (static_cast<size_t>(b) * s.hq + hq) * s.sq + iq;
     if (splits > 1) {
-      if (d < s.d) part.o[row * s.d + d] = all;
+      const size_t out = split * parts.rows + stat;
+      if (d < s.d) parts.o[out * s.d + d] = all;
       if (d == 0) {
-        part.m[row] = top;
-        part.l[row] = sum;
+        parts.ml[2 * out] = top;
+        parts.ml[2 * out + 1] = sum;
       }
     } else {
-      const int iq = row / group, hq = hk * group + row % group;
       const float inv = sum > 0.f ? 1.f / sum : 0.f;
       if (d < s.d) y[(static_cast<size_t>(b) * s.sq + iq) * s.hq * s.d + static_cast<size_t>(hq) * s.d + d] = all * inv;
       if (d == 0) {
-        const size_t stat = (static_cast<size_t>(b) * s.hq + hq) * s.sq + iq;
         stats[stat] = top;
-        stats[static_cast<size_t>(s.b) * s.hq * s.sq + stat] = inv;
+        stats[parts.rows + stat] = inv;
       }
     }
   }
-}
-
-// The parts of a row's keys joined, at most 64: a workgroup of 128 columns by
-// four quarters of the parts per row, so that a thread's loads are all in
-// flight at once. The first wave weighs the parts.
-__device__ inline void join_token(float* __restrict__ y, float* __restrict__ stats, char* __restrict__ ws, const Shape& s, int splits) {
-  __shared__ float weights[64], sums[4][128], total;
-  const int group = s.hq / s.hk, rows = s.sq * group;
-  const int row = blockIdx.x % rows, hk = blockIdx.x / rows % s.hk, b = blockIdx.x / rows / s.hk, lane = threadIdx.x;
-  const size_t first = (static_cast<size_t>(b) * s.hk + hk) * splits;
-  const int i = row / group, h = hk * group + row % group;
-  if (threadIdx.x < 64) {
-    // A part without keys has l = 0 and no say in the maximum.
-    const TokenPart part = token_part(ws, first + min(lane, splits - 1), s.d);
-    const float l = lane < splits ? part.l[row] : 0.f, m = l > 0.f ? part.m[row] : -INFINITY;
-    float top = wave_max(m);
-    top = top == -INFINITY ? 0.f : top;
-    const float weight = l > 0.f ? exp2f(m - top) : 0.f, sum = wave_sum(weight * l);
-    weights[lane] = weight;
-    if (lane == 0) {
-      const float inv = sum > 0.f ? 1.f / sum : 0.f;
-      const size_t stat = (static_cast<size_t>(b) * s.hq + h) * s.sq + i;
-      total = inv;
-      stats[stat] = top;
-      stats[static_cast<size_t>(s.b) * s.hq * s.sq + stat] = inv;
-    }
-  }
-  const int d = threadIdx.x % 128, quarter = threadIdx.x / 128;
-  float o[16];
-#pragma unroll
-  for (int n = 0; n < 16; n++)
-    o[n] = token_part(ws, first + min(quarter + 4 * n, splits - 1), s.d).o[row * s.d + min(d, s.d - 1)];
-  __syncthreads();
-  float all = 0.f;
-#pragma unroll
-  for (int n = 0; n < 16; n++) {
-    const int p = quarter + 4 * n;
-    if (p < splits && weights[p] > 0.f) all += weights[p] * o[n];  // one without keys holds nothing
-  }
-  sums[quarter][d] = all;
-  __syncthreads();
-  if (quarter == 0 && d < s.d)
-    y[(static_cast<size_t>(b) * s.sq + i) * s.hq * s.d + static_cast<size_t>(h) * s.d + d] =
-        ((sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d])) * total;
 }
 
 }  // namespace
@@ -1102,38 +1197,41 @@ __device__ inline void join_token(float* __restrict__ y, float* __restrict__ sta
 #define FG_ATTENTION(NB)                                                                                              \
   extern "C" __global__ void __launch_bounds__(256) fg_attention_pack_##NB(                                           \
       float* y, const float* q, const float* k, const float* v, float* stats, const int* lengths, char* ws, int B,    \
-      int Sq, int Sk, int Hq, int Hk, int D, int causal, float scale, int splits, int per) {                          \
+      int Sq, int Sk, int Hq, int Hk, int D, int causal, float scale, int splits, int per, unsigned, unsigned) {                          \
     pack_keys<NB>(k, v, lengths, ws, B, Sk, Hk, D);                                                                   \
   }                                                                                                                   \
   extern "C" __global__ void __launch_bounds__(256, 2) fg_attention_tiles_##NB(                                       \
       float* y, const float* q, const float* k, const float* v, float* stats, const int* lengths, char* ws, int B,    \
-      int Sq, int Sk, int Hq, int Hk, int D, int causal, float scale, int splits, int per) {                          \
-    forward_tiles<NB>(y, q, stats, lengths, ws, B, Sq, Sk, Hq, Hk, D, causal, scale);                                 \
+      int Sq, int Sk, int Hq, int Hk, int D, int causal, float scale, int splits, int per, unsigned, unsigned) {                          \
+    forward_tiles<NB>(y, q, stats, lengths, ws, Shape{B, Sq, Sk, Hq, Hk, D, causal}, scale, splits);                  \
   }                                                                                                                   \
   extern "C" __global__ void __launch_bounds__(256) fg_attention_grad_pack_##NB(                                      \
       float* dq, const float* q, const float* k, const float* v, const float* y, const float* g, const float* stats,  \
-      float* dk, float* dv, const int* lengths, char* ws, int parts, int B, int Sq, int Sk, int Hq, int Hk, int D,    \
+      float* dk, float* dv, const int* lengths, char* ws, int parts, int q_parts, int B, int Sq, int Sk, int Hq, int Hk, int D, \
       int causal, float scale) {                                                                                      \
     pack_grad<NB>(q, k, v, y, g, stats, lengths, ws, Shape{B, Sq, Sk, Hq, Hk, D, causal});                            \
   }                                                                                                                   \
   extern "C" __global__ void __launch_bounds__(64 * kQueryGradWaves<NB>, 2) fg_attention_grad_q_##NB(                  \
       float* dq, const float* q, const float* k, const float* v, const float* y, const float* g, const float* stats,  \
-      float* dk, float* dv, const int* lengths, char* ws, int parts, int B, int Sq, int Sk, int Hq, int Hk, int D,    \
+      float* dk, float* dv, const int* lengths, char* ws, int parts, int q_parts, int B, int Sq, int Sk, int Hq, int Hk, int D, \
       int causal, float scale) {                                                                                      \
-    query_grads<NB, kQueryGradWaves<NB>>(dq, q, g, stats, lengths, ws, Shape{B, Sq, Sk, Hq, Hk, D, causal}, scale);                        \
+    query_grads<NB, kQueryGradWaves<NB>>(dq, q, g, stats, lengths, ws, Shape{B, Sq, Sk, Hq, Hk, D, causal}, scale, parts, q_parts);        \
   }                                                                                                                   \
-  extern "C" __global__ void __launch_bounds__(512, 2) fg_attention_grad_kv_##NB(                                   \
+  extern "C" __global__ void __launch_bounds__(512, (NB) < 3 ? 4 : 2) fg_attention_grad_kv_##NB(                                   \
       float* dq, const float* q, const float* k, const float* v, const float* y, const float* g, const float* stats,  \
-      float* dk, float* dv, const int* lengths, char* ws, int parts, int B, int Sq, int Sk, int Hq, int Hk, int D,    \
+      float* dk, float* dv, const int* lengths, char* ws, int parts, int q_parts, int B, int Sq, int Sk, int Hq, int Hk, int D, \
       int causal, float scale) {                                                                                      \
     key_grads<NB>(dk, dv, k, v, lengths, ws, Shape{B, Sq, Sk, Hq, Hk, D, causal}, scale, parts);                      \
   }                                                                                                                   \
   extern "C" __global__ void __launch_bounds__(256) fg_attention_grad_sum_##NB(                                       \
       float* dq, const float* q, const float* k, const float* v, const float* y, const float* g, const float* stats,  \
-      float* dk, float* dv, const int* lengths, char* ws, int parts, int B, int Sq, int Sk, int Hq, int Hk, int D,    \
+      float* dk, float* dv, const int* lengths, char* ws, int parts, int q_parts, int B, int Sq, int Sk, int Hq, int Hk, int D, \
       int causal, float scale) {                                                                                      \
-    const GradSpace f = grad_space<NB>(ws, Shape{B, Sq, Sk, Hq, Hk, D, causal});                                      \
-    sum_parts(dk, dv, f.parts, static_cast<size_t>(B) * Sk * Hk * D, parts);                                          \
+    const Shape s{B, Sq, Sk, Hq, Hk, D, causal};                                                                      \
+    const GradSpace f = grad_space<NB>(ws, s);                                                                        \
+    const size_t n = static_cast<size_t>(B) * Sk * Hk * D, m = static_cast<size_t>(B) * Sq * Hq * D;                  \
+    if (parts > 1) sum_parts(dk, dv, f.parts, n, 2 * n, parts);                                                       \
+    if (q_parts > 1) sum_parts(dq, dq, f.parts + key_parts(s, parts), m, m, q_parts);                                 \
   }
 
 FG_ATTENTION(1)
@@ -1144,7 +1242,7 @@ FG_ATTENTION(4)
 #define FG_ATTENTION_TOKEN(ND, NAME, ALIGNED)                                                                         \
   extern "C" __global__ void __launch_bounds__(256, 2) fg_attention_token_##NAME(                                     \
       float* y, const float* q, const float* k, const float* v, float* stats, const int* lengths, char* ws, int B,    \
-      int Sq, int Sk, int Hq, int Hk, int D, int causal, float scale, int splits, int per) {                          \
+      int Sq, int Sk, int Hq, int Hk, int D, int causal, float scale, int splits, int per, unsigned, unsigned) {                          \
     token<ND, ALIGNED>(y, q, k, v, stats, lengths, ws, Shape{B, Sq, Sk, Hq, Hk, D, causal}, scale, splits, per);      \
   }
 FG_ATTENTION_TOKEN(1, 1, true)
@@ -1152,9 +1250,15 @@ FG_ATTENTION_TOKEN(2, 2, true)
 FG_ATTENTION_TOKEN(1, 1_any, false)
 FG_ATTENTION_TOKEN(2, 2_any, false)
 
-extern "C" __global__ void __launch_bounds__(512)
-    fg_attention_token_join(float* y, const float* q, const float* k, const float* v, float* stats, const int* lengths,
-                            char* ws, int B, int Sq, int Sk, int Hq, int Hk, int D, int causal, float scale, int splits,
-                            int per) {
-  join_token(y, stats, ws, Shape{B, Sq, Sk, Hq, Hk, D, causal}, splits);
-}
+// The parts begin `tiles` bytes into the workspace (given as two words). W
+// columns a thread.
+#define FG_ATTENTION_JOIN(W)                                                                                          \
+  extern "C" __global__ void __launch_bounds__(256) fg_attention_join_##W(                                            \
+      float* y, const float* q, const float* k, const float* v, float* stats, const int* lengths, char* ws, int B,    \
+      int Sq, int Sk, int Hq, int Hk, int D, int causal, float scale, int splits, int per, unsigned tiles_lo,         \
+      unsigned tiles_hi) {                                                                                            \
+    join_parts<W>(y, stats, ws + (static_cast<size_t>(tiles_hi) << 32 | tiles_lo),                                    \
+                  Shape{B, Sq, Sk, Hq, Hk, D, causal}, splits);                                                       \
+  }
+FG_ATTENTION_JOIN(1)
+FG_ATTENTION_JOIN(4)

@@ -192,21 +192,31 @@ RenderedKernel render_norm_rotate(const UOp& call, bool grad) {
 // lengths, bits of scale. Sources: q, k, v, [lengths], the stats' storage; of
 // the gradient: q, k, v, y, g, stats, [lengths], dk's and dv's storage.
 
-// In how many parts each 128 keys take their query blocks for dk and dv. The
-// launch fills 256 compute units with one workgroup each, and costs its longest
-// row of workgroups: rounds times (units + about 3 for a workgroup's start and
-// end); with `causal` the first keys' units are twice the average, and parts
-// even them out. Parts are written and summed: 8 bytes an element and part at
-// 5 TB/s, and a launch. A unit takes about 0.9 us per 32 columns.
-int64_t key_grad_parts(int64_t tiles, int64_t units, bool causal, double elements, int64_t nb) {
+// Calls of up to this many operations (of both products, all keys counted) run
+// on the float32 path, in one launch. Float32 path against cut operands, us of
+// the kernels, 8 heads of 64, causal: batch 8 of 128 tokens (2^28) 10.5 and
+// 14.6 (in two launches), one of 512 (2^29) 16.8 and 20.2, 8 of 256 (2^30) 21.6
+// and 21.8; 16 heads of 128 over 512 tokens (2^31) 47 and 34.
+constexpr double kSmallAttention = 1073741824.0;
+
+// In how many parts each of `tiles` workgroups' rows takes its `units` blocks of
+// 32. A launch fills `slots` with a workgroup each and costs its longest row of
+// them: rounds times (units + about 4 for a workgroup's start and end) units of
+// `unit_us`. With `causal` the longest is twice the average, and long ones start
+// first: the launch takes as long as the longest, or as all of them together.
+// Parts cost `extra_us` (a launch that joins them) and their `bytes`, written
+// and read at 5 TB/s.
+int64_t count_parts(int64_t tiles, int64_t units, bool causal, int64_t slots, double unit_us, double bytes, double extra_us,
+                    int64_t most) {
   int64_t best = 1;
   double least = 0;
-  for (int64_t parts = 1; parts <= std::min<int64_t>(units, 16); parts++) {
-    const double each = static_cast<double>(units) / static_cast<double>(parts);
-    const int64_t rounds = (tiles * parts + 255) / 256;
-    double cost = static_cast<double>(rounds) * (each + 3);
-    if (causal) cost = std::max(each + 3, 0.5 * static_cast<double>(tiles * units) / 256 + 3.0 * static_cast<double>(rounds));
-    if (parts > 1) cost += (elements * 8 * static_cast<double>(parts) / 5e6 + 5) / (0.9 * static_cast<double>(nb));
+  for (int64_t parts = 1; parts <= std::min(units, most); parts++) {
+    const double each = static_cast<double>(units) / static_cast<double>(parts) + 4;
+    const double rounds = static_cast<double>((tiles * parts + slots - 1) / slots);
+    double cost = rounds * each;
+    if (causal) cost = std::max(each, 0.5 * static_cast<double>(tiles * units) / static_cast<double>(slots) + 4 * rounds);
+    cost *= unit_us;
+    if (parts > 1) cost += 2 * bytes * static_cast<double>(parts) / 5e6 + extra_us;
     if (parts == 1 || cost < least) {
       best = parts;
       least = cost;
@@ -225,50 +235,59 @@ RenderedKernel render_attention(const UOp& call, bool grad) {
   for (int i = 0; i < 7; i++) tail.push_back(CallArg::i32(p[static_cast<size_t>(i)]));
   tail.push_back(CallArg::f32(static_cast<float>(from_bits(p[8]))));
   const int64_t dim = p[5], nb = (dim + 31) / 32, k_blocks = (sk + 31) / 32;
+  const uint64_t all_q = static_cast<uint64_t>(batch * sq * heads * dim), all_k = static_cast<uint64_t>(batch * sk * kv_heads * dim);
   if (!grad) {
     rk.kind = "attention";
     int64_t splits = 1, per = sk;
-    if (sq * (heads / kv_heads) <= 16) {
-      // Few query rows: the keys of a head split until there are 1024
-      // workgroups, of at least 256 keys (four rounds of its waves).
-      const int64_t pairs = batch * kv_heads;
+    uint64_t tile_bytes = 0;
+    const int64_t rows = sq * (heads / kv_heads);
+    if (rows <= 16 || 4.0 * static_cast<double>(all_q) * static_cast<double>(sk) <= kSmallAttention) {
+      // 16 rows a workgroup; the keys of each split until there are 1024, of
+      // at least 256 keys (four rounds of its waves).
+      const int64_t pairs = batch * kv_heads * ((rows + 15) / 16);
       splits = std::max<int64_t>(1, std::min({(1024 + pairs - 1) / pairs, sk / 256, int64_t(64)}));
       per = ((sk + splits - 1) / splits + 63) / 64 * 64;
       splits = (sk + per - 1) / per;
       rk.launches = {launch(std::string("fg_attention_token_") + (dim <= 64 ? "1" : "2") + (dim % 4 ? "_any" : ""), static_cast<uint64_t>(pairs * splits), 256, "attention")};
-      rk.workspace_bytes = 4;
-      if (splits > 1) {
-        rk.workspace_bytes = static_cast<size_t>(pairs * splits) * static_cast<size_t>(16 * dim + 32) * 4;
-        rk.launches.push_back(launch("fg_attention_token_join", static_cast<uint64_t>(batch * heads * sq), 512, "attention"));
-      }
     } else {
+      const int64_t tiles = batch * heads * ((sq + 127) / 128);
       const uint64_t blocks = static_cast<uint64_t>(batch * kv_heads * k_blocks);
-      rk.workspace_bytes = blocks * static_cast<uint64_t>(nb * 8192 + 1024);
+      splits = count_parts(tiles, k_blocks, causal, 512, 0.5 + 0.4 * static_cast<double>(nb), 4.0 * static_cast<double>(all_q), 6, 64);
+      tile_bytes = blocks * static_cast<uint64_t>(nb * 8192 + 1024);
       rk.launches = {launch("fg_attention_pack_" + std::to_string(nb), 2 * blocks, 256, "attention"),
-                     launch("fg_attention_tiles_" + std::to_string(nb),
-                            static_cast<uint64_t>(batch * heads * ((sq + 127) / 128)), 256, "attention")};
+                     launch("fg_attention_tiles_" + std::to_string(nb), static_cast<uint64_t>(tiles * splits), 256, "attention")};
+    }
+    rk.workspace_bytes = std::max<uint64_t>(tile_bytes, 4);
+    if (splits > 1) {
+      const uint64_t all_rows = static_cast<uint64_t>(batch * heads * sq);
+      rk.workspace_bytes = tile_bytes + static_cast<uint64_t>(splits) * (4 * all_q + 8 * all_rows);
+      const uint64_t columns = dim % 4 ? 1 : 4;  // a thread's
+      rk.launches.push_back(launch("fg_attention_join_" + std::to_string(columns), (all_q / columns + 255) / 256, 256, "attention"));
     }
     rk.call_args = {CallArg::slot(0), CallArg::slot(1), CallArg::slot(2), CallArg::slot(3), CallArg::slot(lengths ? 5 : 4),
                     lengths ? CallArg::slot(4) : CallArg::null(), CallArg::workspace()};
-    tail.push_back(CallArg::i32(splits));
-    tail.push_back(CallArg::i32(per));
+    for (int64_t x : {splits, per, static_cast<int64_t>(static_cast<int32_t>(tile_bytes & 0xffffffffu)), static_cast<int64_t>(tile_bytes >> 32)})
+      tail.push_back(CallArg::i32(x));
     rk.side_outputs = {lengths ? 5 : 4};
   } else {
     rk.kind = "attention_grad";
     const std::string nbs = "_" + std::to_string(nb);
     const int64_t q_blocks = (sq + 31) / 32, group = heads / kv_heads;
     const uint64_t nk = static_cast<uint64_t>(batch * kv_heads * k_blocks), nq = static_cast<uint64_t>(batch * heads * q_blocks);
-    const int64_t tiles = batch * kv_heads * ((sk + 127) / 128), waves = nb < 4 ? 4 : 8;  // kQueryGradWaves
-    const int64_t parts = key_grad_parts(tiles, q_blocks * group, causal, 2.0 * static_cast<double>(batch * sk * kv_heads * dim), nb);
-    const uint64_t all = static_cast<uint64_t>(batch * sk * kv_heads * dim);
+    const int64_t waves = nb < 4 ? 4 : 8;  // kQueryGradWaves
+    const int64_t k_tiles = batch * kv_heads * ((sk + 127) / 128), q_tiles = batch * heads * ((sq + 32 * waves - 1) / (32 * waves));
+    const double unit_us = 0.9 * static_cast<double>(nb);
+    const int64_t parts = count_parts(k_tiles, q_blocks * group, causal, nb < 3 ? 512 : 256, unit_us, 8.0 * static_cast<double>(all_k), 6, 16);
+    const int64_t q_parts = count_parts(q_tiles, k_blocks, causal, nb < 4 ? 512 : 256, unit_us, 4.0 * static_cast<double>(all_q),
+                                        parts > 1 ? 0 : 6, 16);
+    const uint64_t summed = std::max(parts > 1 ? 2 * all_k : 0, q_parts > 1 ? all_q : 0);
     rk.workspace_bytes = nk * static_cast<uint64_t>(nb * 12288 + 1024) + nq * static_cast<uint64_t>(nb * 16384 + 1024) +
-                         (nk + 3) / 4 * 16 + (parts > 1 ? 8 * all * static_cast<uint64_t>(parts) : 0);
+                         (nk + 3) / 4 * 16 + (parts > 1 ? 8 * all_k * static_cast<uint64_t>(parts) : 0) +
+                         (q_parts > 1 ? 4 * all_q * static_cast<uint64_t>(q_parts) : 0);
     rk.launches = {launch("fg_attention_grad_pack" + nbs, 2 * (nk + nq), 256, "attention"),
-                   launch("fg_attention_grad_kv" + nbs, static_cast<uint64_t>(tiles * parts), 512, "attention"),
-                   launch("fg_attention_grad_q" + nbs, static_cast<uint64_t>(batch * heads * ((sq + 32 * waves - 1) / (32 * waves))),
-                          static_cast<unsigned>(64 * waves), "attention")};
-    if (parts > 1)
-      rk.launches.push_back(launch("fg_attention_grad_sum" + nbs, std::min<uint64_t>((2 * all + 255) / 256, 8192), 256, "attention"));
+                   launch("fg_attention_grad_kv" + nbs, static_cast<uint64_t>(k_tiles * parts), 512, "attention"),
+                   launch("fg_attention_grad_q" + nbs, static_cast<uint64_t>(q_tiles * q_parts), static_cast<unsigned>(64 * waves), "attention")};
+    if (summed) rk.launches.push_back(launch("fg_attention_grad_sum" + nbs, std::min<uint64_t>((summed + 255) / 256, 8192), 256, "attention"));
     const int dk = lengths ? 8 : 7;
     for (int i = 0; i < 7; i++) rk.call_args.push_back(CallArg::slot(i));
     rk.call_args.push_back(CallArg::slot(dk));
@@ -276,6 +295,7 @@ RenderedKernel render_attention(const UOp& call, bool grad) {
     rk.call_args.push_back(lengths ? CallArg::slot(7) : CallArg::null());
     rk.call_args.push_back(CallArg::workspace());
     rk.call_args.push_back(CallArg::i32(parts));
+    rk.call_args.push_back(CallArg::i32(q_parts));
     rk.side_outputs = {dk, dk + 1};
   }
   rk.call_args.insert(rk.call_args.end(), tail.begin(), tail.end());

@@ -12,6 +12,7 @@
  * Python class, which subclasses this type. */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
+#include <math.h>
 
 #include "ferrograd.h"
 
@@ -202,6 +203,106 @@ static PyObject* t_log_softmax(TensorObject* self, PyObject* axis) {
   return wrap(Py_TYPE(self), out);
 }
 
+PyDoc_STRVAR(attention_doc,
+"attention(k, v, heads, kv_heads=None, batch=1, causal=False, lengths=None, scale=None)\n--\n\n"
+"softmax(scale q k^T) v per head, with this tensor as q. Matrices have one row\n"
+"per token, as Linear takes and gives them: q [batch * sq, heads * dim], k and v\n"
+"[batch * sk, kv_heads * dim] (f32, dim at most 128); kv_heads defaults to heads,\n"
+"scale to dim ** -0.5. Query i of a sequence sees the keys j < lengths[b] (an\n"
+"int32 tensor [batch], clamped to [0, sk]; None: all of them) and, with causal,\n"
+"j <= i + sk - sq; one that sees none gives 0 and gradients of 0. What keys and\n"
+"values past a length hold never matters; everything else must be finite.");
+
+static PyObject* t_attention(TensorObject* self, PyObject* args, PyObject* kw) {
+  static char* names[] = {"k", "v", "heads", "kv_heads", "batch", "causal", "lengths", "scale", NULL};
+  PyObject *kv_heads = Py_None, *lengths = Py_None, *scale = Py_None;
+  TensorObject *k, *v, *l = NULL;
+  PyObject *ko, *vo;
+  long long heads, kvh, batch = 1;
+  int causal = 0;
+  if (!PyArg_ParseTupleAndKeywords(args, kw, "OOL|OLpOO:attention", names, &ko, &vo, &heads, &kv_heads, &batch, &causal,
+                                   &lengths, &scale))
+    return NULL;
+  if (check_tensor(ko, &k) || check_tensor(vo, &v) || (lengths != Py_None && check_tensor(lengths, &l))) return NULL;
+  if (!has_handle(self) || !has_handle(k) || !has_handle(v) || (l && !has_handle(l))) return NULL;
+  kvh = heads;
+  if (kv_heads != Py_None) {
+    kvh = PyLong_AsLongLong(kv_heads);
+    if (kvh == -1 && PyErr_Occurred()) return NULL;
+  }
+  double s = 1.0;
+  if (scale != Py_None) {
+    s = PyFloat_AsDouble(scale);
+    if (s == -1.0 && PyErr_Occurred()) return NULL;
+  } else {
+    int64_t shape[16];
+    int n = 16;
+    if (fg_tensor_shape(self->h, shape, &n)) return raise_last();
+    /* A shape that does not split is refused below. */
+    if (n == 2 && heads > 0 && shape[1] >= heads) s = 1.0 / sqrt((double)(shape[1] / heads));
+  }
+  fg_tensor* out = NULL;
+  if (fg_tensor_attention(self->h, k->h, v->h, l ? l->h : NULL, batch, heads, kvh, causal, s, &out)) return raise_last();
+  return wrap(Py_TYPE(self), out);
+}
+
+PyDoc_STRVAR(norm_rotate_doc,
+"norm_rotate(weight, positions, heads, eps=1e-6, base=10000.0)\n--\n\n"
+"RMS norm of each head and the rotation of its position in one pass, for queries\n"
+"and keys [tokens, heads * dim] (f32, dim even and at most 512): z = x *\n"
+"(mean(x**2) + eps) ** -0.5 * weight (f32 [dim]), then the pair (z_i,\n"
+"z_{i + dim/2}) turned by positions[token] * base**(-2i/dim) (positions int32\n"
+"[tokens]).");
+
+static PyObject* t_norm_rotate(TensorObject* self, PyObject* args, PyObject* kw) {
+  static char* names[] = {"weight", "positions", "heads", "eps", "base", NULL};
+  PyObject *wo, *po;
+  TensorObject *w, *p;
+  long long heads;
+  double eps = 1e-6, base = 10000.0;
+  if (!PyArg_ParseTupleAndKeywords(args, kw, "OOL|dd:norm_rotate", names, &wo, &po, &heads, &eps, &base)) return NULL;
+  if (check_tensor(wo, &w) || check_tensor(po, &p) || !has_handle(self) || !has_handle(w) || !has_handle(p)) return NULL;
+  fg_tensor* out = NULL;
+  if (fg_tensor_norm_rotate(self->h, w->h, p->h, heads, eps, base, &out)) return raise_last();
+  return wrap(Py_TYPE(self), out);
+}
+
+PyDoc_STRVAR(dropout_doc,
+"dropout(p, seed, offset=0)\n--\n\n"
+"x / (1 - p) where the element's random word is at least floor(p * 2**32), else\n"
+"0 (an f32 tensor of any shape; 0 <= p < 1). Element e's word is word e % 4 of\n"
+"Philox4x32-10 of the counter (e // 4, offset) under the key `seed`: 64 bits\n"
+"each, so the same seed and offset drop the same elements, and the gradient draws\n"
+"the mask again. Use a new offset for every call that should draw anew (Dropout\n"
+"does).");
+
+/* An int of [0, 2^64). */
+static int u64_arg(PyObject* o, const char* name, uint64_t* out) {
+  PyObject* i = PyNumber_Index(o);
+  if (!i) return -1;
+  *out = PyLong_AsUnsignedLongLong(i);
+  if (*out == (uint64_t)-1 && PyErr_Occurred()) {
+    PyErr_Clear();
+    PyErr_Format(g_error_class ? g_error_class : PyExc_RuntimeError, "%s must be in [0, 2**64), got %S", name, i);
+    Py_DECREF(i);
+    return -1;
+  }
+  Py_DECREF(i);
+  return 0;
+}
+
+static PyObject* t_dropout(TensorObject* self, PyObject* args, PyObject* kw) {
+  static char* names[] = {"p", "seed", "offset", NULL};
+  PyObject *so, *oo = NULL;
+  double p;
+  uint64_t seed, offset = 0;
+  if (!PyArg_ParseTupleAndKeywords(args, kw, "dO|O:dropout", names, &p, &so, &oo)) return NULL;
+  if (u64_arg(so, "seed", &seed) || (oo && u64_arg(oo, "offset", &offset)) || !has_handle(self)) return NULL;
+  fg_tensor* out = NULL;
+  if (fg_tensor_dropout(self->h, p, seed, offset, &out)) return raise_last();
+  return wrap(Py_TYPE(self), out);
+}
+
 static PyObject* t_realize(TensorObject* self, PyObject* unused) {
   (void)unused;
   if (!has_handle(self)) return NULL;
@@ -242,6 +343,9 @@ static PyMethodDef t_methods[] = {
     {"expand", (PyCFunction)t_expand, METH_O, NULL},
     {"narrow", (PyCFunction)(void (*)(void))t_narrow, METH_FASTCALL, NULL},
     {"log_softmax", (PyCFunction)t_log_softmax, METH_O, NULL},
+    {"attention", (PyCFunction)(void (*)(void))t_attention, METH_VARARGS | METH_KEYWORDS, attention_doc},
+    {"norm_rotate", (PyCFunction)(void (*)(void))t_norm_rotate, METH_VARARGS | METH_KEYWORDS, norm_rotate_doc},
+    {"dropout", (PyCFunction)(void (*)(void))t_dropout, METH_VARARGS | METH_KEYWORDS, dropout_doc},
     {"_u", (PyCFunction)t_u, METH_O, NULL},
     {"_b", (PyCFunction)(void (*)(void))t_b, METH_FASTCALL, NULL},
     {"realize", (PyCFunction)t_realize, METH_NOARGS, "Tensor::realize (tensor.rs:781-830)."},
