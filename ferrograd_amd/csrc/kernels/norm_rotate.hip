@@ -44,11 +44,15 @@ __device__ inline Vec<VEC> load(const float* p) {
   return r;
 }
 
+// `stream`: past the caches.
 template <int VEC>
-__device__ inline void store(float* p, const Vec<VEC>& r) {
-  if constexpr (VEC == 4) *reinterpret_cast<float4*>(p) = make_float4(r.v[0], r.v[1], r.v[2], r.v[3]);
-  else if constexpr (VEC == 2) *reinterpret_cast<float2*>(p) = make_float2(r.v[0], r.v[1]);
-  else *p = r.v[0];
+__device__ inline void store(float* p, const Vec<VEC>& r, bool stream) {
+  typedef float vec __attribute__((ext_vector_type(VEC)));
+  vec v;
+#pragma unroll
+  for (int e = 0; e < VEC; e++) v[e] = r.v[e];
+  if (stream) __builtin_nontemporal_store(v, reinterpret_cast<vec*>(p));
+  else *reinterpret_cast<vec*>(p) = v;
 }
 
 template <int G>
@@ -77,11 +81,15 @@ __device__ inline void turn(double freq, int pos, float* c, float* s) {
 }
 
 // Units of work: `heads_per` heads of a token; group g of the launch takes
-// units g, g + groups, ...
+// units g, g + groups, ... Heads are taken kHeads at a time, loaded before the
+// first is worked on: a row is a few hundred bytes, and the memory needs more
+// of them under way than there are waves.
+constexpr int kHeads = 4, kGradHeads = 2;
+
 template <int VEC, int G, int NV>
 __device__ inline void forward(float* __restrict__ out, const float* __restrict__ x, const float* __restrict__ w,
                                const int* __restrict__ positions, int tokens, int heads, int dim, int heads_per,
-                               float eps, float log2_base_hi, float log2_base_lo) {
+                               float eps, float log2_base_hi, float log2_base_lo, bool stream) {
   const int half = dim / 2, sub = threadIdx.x % G;
   const unsigned groups = gridDim.x * (kThreads / G);
   const unsigned chunks = (heads + heads_per - 1) / heads_per;
@@ -106,34 +114,46 @@ __device__ inline void forward(float* __restrict__ out, const float* __restrict_
     for (int v = 0; v < NV; v++)
 #pragma unroll
       for (int e = 0; e < VEC; e++) turn(freq[v][e], pos, &c[v][e], &s[v][e]);
-    size_t row = (static_cast<size_t>(token) * heads + h0) * dim;
-    for (int h = h0; h < h1; h++, row += dim) {
-      Vec<VEC> a[NV], b[NV];
-      float ss = 0.f;
+    for (int h = h0; h < h1; h += kHeads) {
+      Vec<VEC> a[kHeads][NV], b[kHeads][NV];
 #pragma unroll
-      for (int v = 0; v < NV; v++) {
-        const int i = (v * G + sub) * VEC;
-        if (i < half) {
-          a[v] = load<VEC>(x + row + i);
-          b[v] = load<VEC>(x + row + half + i);
+      for (int k = 0; k < kHeads; k++) {
+        const float* row = x + (static_cast<size_t>(token) * heads + min(h + k, h1 - 1)) * dim;
 #pragma unroll
-          for (int e = 0; e < VEC; e++) ss += a[v].v[e] * a[v].v[e] + b[v].v[e] * b[v].v[e];
+        for (int v = 0; v < NV; v++) {
+          const int i = (v * G + sub) * VEC;
+          if (i < half) {
+            a[k][v] = load<VEC>(row + i);
+            b[k][v] = load<VEC>(row + half + i);
+          }
         }
       }
-      const float r = 1.f / sqrtf(group_sum<G>(ss) / dim + eps);
 #pragma unroll
-      for (int v = 0; v < NV; v++) {
-        const int i = (v * G + sub) * VEC;
-        if (i >= half) continue;
-        Vec<VEC> ya, yb;
+      for (int k = 0; k < kHeads; k++) {
+        float ss = 0.f;
 #pragma unroll
-        for (int e = 0; e < VEC; e++) {
-          const float za = a[v].v[e] * r * wa[v].v[e], zb = b[v].v[e] * r * wb[v].v[e];
-          ya.v[e] = za * c[v][e] - zb * s[v][e];
-          yb.v[e] = zb * c[v][e] + za * s[v][e];
+        for (int v = 0; v < NV; v++)
+          if ((v * G + sub) * VEC < half) {
+#pragma unroll
+            for (int e = 0; e < VEC; e++) ss += a[k][v].v[e] * a[k][v].v[e] + b[k][v].v[e] * b[k][v].v[e];
+          }
+        const float r = 1.f / sqrtf(group_sum<G>(ss) / dim + eps);
+        if (h + k >= h1) continue;
+        float* row = out + (static_cast<size_t>(token) * heads + h + k) * dim;
+#pragma unroll
+        for (int v = 0; v < NV; v++) {
+          const int i = (v * G + sub) * VEC;
+          if (i >= half) continue;
+          Vec<VEC> ya, yb;
+#pragma unroll
+          for (int e = 0; e < VEC; e++) {
+            const float za = a[k][v].v[e] * r * wa[v].v[e], zb = b[k][v].v[e] * r * wb[v].v[e];
+            ya.v[e] = za * c[v][e] - zb * s[v][e];
+            yb.v[e] = zb * c[v][e] + za * s[v][e];
+          }
+          store<VEC>(row + i, ya, stream);
+          store<VEC>(row + half + i, yb, stream);
         }
-        store<VEC>(out + row + i, ya);
-        store<VEC>(out + row + half + i, yb);
       }
     }
   }
@@ -143,7 +163,7 @@ template <int VEC, int G, int NV>
 __device__ inline void backward(float* __restrict__ dx, const float* __restrict__ x, const float* __restrict__ w,
                                 const int* __restrict__ positions, const float* __restrict__ g,
                                 float* __restrict__ partial, int tokens, int heads, int dim, int heads_per, float eps,
-                                float log2_base_hi, float log2_base_lo) {
+                                float log2_base_hi, float log2_base_lo, bool stream) {
   __shared__ float sums[kThreads * 2 * NV * VEC];  // [group of the workgroup][half][index], index < G * NV * VEC
   const int half = dim / 2, sub = threadIdx.x % G, group = threadIdx.x / G;
   const unsigned groups = gridDim.x * (kThreads / G);
@@ -170,42 +190,58 @@ __device__ inline void backward(float* __restrict__ dx, const float* __restrict_
     for (int v = 0; v < NV; v++)
 #pragma unroll
       for (int e = 0; e < VEC; e++) turn(freq[v][e], pos, &c[v][e], &s[v][e]);
-    size_t row = (static_cast<size_t>(token) * heads + h0) * dim;
-    for (int h = h0; h < h1; h++, row += dim) {
-      Vec<VEC> a[NV], b[NV], ga[NV], gb[NV];  // x, and g rotated back
-      float ss = 0.f, sg = 0.f;               // sums of x^2 and of g' w x
+    for (int h = h0; h < h1; h += kGradHeads) {
+      Vec<VEC> a[kGradHeads][NV], b[kGradHeads][NV], p[kGradHeads][NV], q[kGradHeads][NV];  // x and g
 #pragma unroll
-      for (int v = 0; v < NV; v++) {
-        const int i = (v * G + sub) * VEC;
-        if (i >= half) continue;
-        a[v] = load<VEC>(x + row + i);
-        b[v] = load<VEC>(x + row + half + i);
-        const Vec<VEC> p = load<VEC>(g + row + i), q = load<VEC>(g + row + half + i);
+      for (int k = 0; k < kGradHeads; k++) {
+        const size_t row = (static_cast<size_t>(token) * heads + min(h + k, h1 - 1)) * dim;
 #pragma unroll
-        for (int e = 0; e < VEC; e++) {
-          ga[v].v[e] = p.v[e] * c[v][e] + q.v[e] * s[v][e];
-          gb[v].v[e] = q.v[e] * c[v][e] - p.v[e] * s[v][e];
-          ss += a[v].v[e] * a[v].v[e] + b[v].v[e] * b[v].v[e];
-          sg += ga[v].v[e] * wa[v].v[e] * a[v].v[e] + gb[v].v[e] * wb[v].v[e] * b[v].v[e];
+        for (int v = 0; v < NV; v++) {
+          const int i = (v * G + sub) * VEC;
+          if (i < half) {
+            a[k][v] = load<VEC>(x + row + i);
+            b[k][v] = load<VEC>(x + row + half + i);
+            p[k][v] = load<VEC>(g + row + i);
+            q[k][v] = load<VEC>(g + row + half + i);
+          }
         }
       }
-      const float r = 1.f / sqrtf(group_sum<G>(ss) / dim + eps);
-      const float mean = group_sum<G>(sg) * r / dim;
 #pragma unroll
-      for (int v = 0; v < NV; v++) {
-        const int i = (v * G + sub) * VEC;
-        if (i >= half) continue;
-        Vec<VEC> oa, ob;
+      for (int k = 0; k < kGradHeads; k++) {
+        float ss = 0.f, sg = 0.f;  // sums of x^2 and of g' w x
 #pragma unroll
-        for (int e = 0; e < VEC; e++) {
-          const float na = a[v].v[e] * r, nb = b[v].v[e] * r;
-          oa.v[e] = r * (ga[v].v[e] * wa[v].v[e] - na * mean);
-          ob.v[e] = r * (gb[v].v[e] * wb[v].v[e] - nb * mean);
-          da[v][e] += ga[v].v[e] * na;
-          db[v][e] += gb[v].v[e] * nb;
+        for (int v = 0; v < NV; v++) {
+          if ((v * G + sub) * VEC >= half) continue;
+#pragma unroll
+          for (int e = 0; e < VEC; e++) {
+            const float ga = p[k][v].v[e] * c[v][e] + q[k][v].v[e] * s[v][e];
+            const float gb = q[k][v].v[e] * c[v][e] - p[k][v].v[e] * s[v][e];
+            p[k][v].v[e] = ga;
+            q[k][v].v[e] = gb;
+            ss += a[k][v].v[e] * a[k][v].v[e] + b[k][v].v[e] * b[k][v].v[e];
+            sg += ga * wa[v].v[e] * a[k][v].v[e] + gb * wb[v].v[e] * b[k][v].v[e];
+          }
         }
-        store<VEC>(dx + row + i, oa);
-        store<VEC>(dx + row + half + i, ob);
+        const float r = 1.f / sqrtf(group_sum<G>(ss) / dim + eps);
+        const float mean = group_sum<G>(sg) * r / dim;
+        if (h + k >= h1) continue;
+        float* row = dx + (static_cast<size_t>(token) * heads + h + k) * dim;
+#pragma unroll
+        for (int v = 0; v < NV; v++) {
+          const int i = (v * G + sub) * VEC;
+          if (i >= half) continue;
+          Vec<VEC> oa, ob;
+#pragma unroll
+          for (int e = 0; e < VEC; e++) {
+            const float na = a[k][v].v[e] * r, nb = b[k][v].v[e] * r;
+            oa.v[e] = r * (p[k][v].v[e] * wa[v].v[e] - na * mean);
+            ob.v[e] = r * (q[k][v].v[e] * wb[v].v[e] - nb * mean);
+            da[v][e] += p[k][v].v[e] * na;
+            db[v][e] += q[k][v].v[e] * nb;
+          }
+          store<VEC>(row + i, oa, stream);
+          store<VEC>(row + half + i, ob, stream);
+        }
       }
     }
   }
@@ -232,14 +268,16 @@ __device__ inline void backward(float* __restrict__ dx, const float* __restrict_
 #define FG_NORM_ROTATE(VEC, G, NV)                                                                                     \
   extern "C" __global__ void __launch_bounds__(kThreads) fg_norm_rotate_##VEC##_##G##_##NV(                            \
       float* out, const float* x, const float* w, const int* positions, int tokens, int heads, int dim, int heads_per, \
-      float eps, float log2_base_hi, float log2_base_lo) {                                                             \
-    forward<VEC, G, NV>(out, x, w, positions, tokens, heads, dim, heads_per, eps, log2_base_hi, log2_base_lo);         \
+      float eps, float log2_base_hi, float log2_base_lo, int stream) {                                                 \
+    forward<VEC, G, NV>(out, x, w, positions, tokens, heads, dim, heads_per, eps, log2_base_hi, log2_base_lo,          \
+                          stream);                                                                                     \
   }                                                                                                                    \
   extern "C" __global__ void __launch_bounds__(kThreads) fg_norm_rotate_grad_##VEC##_##G##_##NV(                       \
       float* dx, const float* x, const float* w, const int* positions, const float* g, float* dw, float* partial,      \
-      int blocks, int tokens, int heads, int dim, int heads_per, float eps, float log2_base_hi, float log2_base_lo) {  \
+      int blocks, int tokens, int heads, int dim, int heads_per, float eps, float log2_base_hi, float log2_base_lo,    \
+      int stream) {                                                                                                    \
     backward<VEC, G, NV>(dx, x, w, positions, g, partial, tokens, heads, dim, heads_per, eps, log2_base_hi,            \
-                         log2_base_lo);                                                                                \
+                         log2_base_lo, stream);                                                                        \
   }
 
 FG_NORM_ROTATE(4, 8, 1)
@@ -262,7 +300,7 @@ FG_NORM_ROTATE(1, 64, 4)
 extern "C" __global__ void __launch_bounds__(1024)
     fg_norm_rotate_weight(float* dx, const float* x, const float* w, const int* positions, const float* g, float* dw,
                           const float* partial, int blocks, int tokens, int heads, int dim, int heads_per, float eps,
-                          float log2_base_hi, float log2_base_lo) {
+                          float log2_base_hi, float log2_base_lo, int stream) {
   __shared__ float sums[64][16];
   const int col = threadIdx.x % 16, slice = threadIdx.x / 16, d = blockIdx.x * 16 + col;
   float t = 0.f;

@@ -25,6 +25,10 @@ void set_image(RenderedKernel& rk, const unsigned char* begin, const unsigned ch
   rk.image_size = static_cast<size_t>(end - begin);
 }
 
+// Outputs from this size on are written past the caches: they would not stay in
+// the Infinity Cache (256 MB) for their reader, and push out what it holds.
+constexpr uint64_t kStreamBytes = uint64_t(64) << 20;
+
 // The products of a fixed grid dimension: HIP takes 2^31 - 1 workgroups.
 unsigned grid_of(uint64_t n, const char* what) {
   FG_CHECK(n >= 1 && n <= 0x7fffffffULL, std::string(what) + ": " + std::to_string(n) + " workgroups in one launch");
@@ -112,7 +116,7 @@ RenderedKernel render_dropout(const UOp& call) {
   set_image(rk, fg_image_dropout, fg_image_dropout_end);
   const uint64_t threshold = static_cast<uint64_t>(p * 4294967296.0);
   // 4 elements a thread (one block of four random words).
-  rk.launches = {launch("fg_dropout", (n + 1023) / 1024, 256, "dropout")};
+  rk.launches = {launch(4 * n >= kStreamBytes ? "fg_dropout_stream" : "fg_dropout", (n + 511) / 512, 128, "dropout")};
   rk.call_args = {CallArg::slot(0), CallArg::slot(1), CallArg::slot(2), CallArg::slot(3), CallArg::slot(4),
                   CallArg::slot(5), CallArg::i32(static_cast<int32_t>(n & 0xffffffffu)),
                   CallArg::i32(static_cast<int64_t>(n >> 32)), CallArg::i32(static_cast<int32_t>(threshold)),
@@ -160,9 +164,8 @@ RenderedKernel render_norm_rotate(const UOp& call, bool grad) {
   const int64_t tokens = p[0], heads = p[1], dim = p[2];
   const double eps = from_bits(p[3]), log2_base = std::log2(from_bits(p[4]));
   const RowSplit r = row_split(dim);
-  // Heads of a token that share its cosines: more while 16384 groups are left
-  // (every lane of the chip four waves deep at 16 lanes a group).
-  const int64_t heads_per = std::max<int64_t>(1, std::min<int64_t>({heads, 8, tokens * heads / 16384}));
+  // Heads of a token that share its cosines: more while 8192 groups are left.
+  const int64_t heads_per = std::max<int64_t>(1, std::min<int64_t>({heads, 8, tokens * heads / 8192}));
   const int64_t units = tokens * ((heads + heads_per - 1) / heads_per), per_block = 256 / r.lanes;
   const int64_t blocks = std::min<int64_t>((units + per_block - 1) / per_block, grad ? 1024 : 4096);
   RenderedKernel rk;
@@ -170,7 +173,8 @@ RenderedKernel render_norm_rotate(const UOp& call, bool grad) {
   const float hi = static_cast<float>(log2_base);
   const std::vector<CallArg> tail = {CallArg::i32(tokens), CallArg::i32(heads), CallArg::i32(dim), CallArg::i32(heads_per),
                                      CallArg::f32(static_cast<float>(eps)), CallArg::f32(hi),
-                                     CallArg::f32(static_cast<float>(log2_base - hi))};
+                                     CallArg::f32(static_cast<float>(log2_base - hi)),
+                                     CallArg::i32(4 * tokens * heads * dim >= static_cast<int64_t>(kStreamBytes))};
   rk.call_args = {CallArg::slot(0), CallArg::slot(1), CallArg::slot(2), CallArg::slot(3)};
   if (!grad) {
     rk.kind = "norm_rotate";
