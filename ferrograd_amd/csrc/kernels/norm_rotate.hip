@@ -12,9 +12,11 @@
 // backward reads x and g and writes dx (12). So a row lives in the registers
 // of G lanes (the least power of two that holds half a row in vectors of VEC,
 // so lane i has both numbers of its pairs), its sums run over the G lanes, and
-// the cosines of a token are made once and serve several of its heads. Angles
-// are formed in 64 bits as revolutions and reduced there: a far position times
-// a frequency has more whole turns than 32 bits can hold beside the fraction.
+// a workgroup makes the cosines of a few tokens once, in LDS, for all of their
+// heads, then goes through their rows in order, a stretch of memory at a time.
+// Angles are formed in 64 bits as revolutions and reduced there: a far position
+// times a frequency has more whole turns than 32 bits can hold beside the
+// fraction.
 // dw is summed in registers over all rows of a group, then over the workgroup
 // in LDS, then over the workgroups by a second launch: a fixed order, no
 // atomics.
@@ -29,29 +31,25 @@ struct Vec {
   float v[VEC];
 };
 
-template <int VEC>
+// `Stream`: past the caches, for what is read once and outputs that would not
+// stay in the Infinity Cache.
+template <int VEC, bool Stream = false>
 __device__ inline Vec<VEC> load(const float* p) {
+  typedef float vec __attribute__((ext_vector_type(VEC)));
+  const vec v = Stream ? __builtin_nontemporal_load(reinterpret_cast<const vec*>(p)) : *reinterpret_cast<const vec*>(p);
   Vec<VEC> r;
-  if constexpr (VEC == 4) {
-    const float4 t = *reinterpret_cast<const float4*>(p);
-    r = {{t.x, t.y, t.z, t.w}};
-  } else if constexpr (VEC == 2) {
-    const float2 t = *reinterpret_cast<const float2*>(p);
-    r = {{t.x, t.y}};
-  } else {
-    r.v[0] = *p;
-  }
+#pragma unroll
+  for (int e = 0; e < VEC; e++) r.v[e] = v[e];
   return r;
 }
 
-// `stream`: past the caches.
-template <int VEC>
-__device__ inline void store(float* p, const Vec<VEC>& r, bool stream) {
+template <int VEC, bool Stream>
+__device__ inline void store(float* p, const Vec<VEC>& r) {
   typedef float vec __attribute__((ext_vector_type(VEC)));
   vec v;
 #pragma unroll
   for (int e = 0; e < VEC; e++) v[e] = r.v[e];
-  if (stream) __builtin_nontemporal_store(v, reinterpret_cast<vec*>(p));
+  if (Stream) __builtin_nontemporal_store(v, reinterpret_cast<vec*>(p));
   else *reinterpret_cast<vec*>(p) = v;
 }
 
@@ -62,40 +60,43 @@ __device__ inline float group_sum(float x) {
   return x;
 }
 
-// The frequencies (revolutions per position) of a lane's pairs.
-template <int VEC, int G, int NV>
-__device__ inline void frequencies(double (&freq)[NV][VEC], int sub, int half, double log2_base) {
-#pragma unroll
-  for (int v = 0; v < NV; v++)
-#pragma unroll
-    for (int e = 0; e < VEC; e++) {
-      const int i = (v * G + sub) * VEC + e;
-      freq[v][e] = exp2(-(static_cast<double>(i) / half) * log2_base) * 0.15915494309189533577;  // 1 / (2 pi)
-    }
+constexpr int kAngles = 1024;  // of a workgroup's tokens, at most
+constexpr int kMaxHalf = 256;
+
+struct Angles {
+  double freq[kMaxHalf];  // revolutions per position
+  float2 turn[kAngles];   // cos, sin of [token][pair]
+};
+
+__device__ inline void frequencies(Angles& a, int half, double log2_base) {
+  for (int i = threadIdx.x; i < half; i += kThreads)
+    a.freq[i] = exp2(-(static_cast<double>(i) / half) * log2_base) * 0.15915494309189533577;  // 1 / (2 pi)
+  __syncthreads();
 }
 
-// cos and sin of pos * frequency; the whole turns go in 64 bits.
-__device__ inline void turn(double freq, int pos, float* c, float* s) {
-  const double t = freq * pos;
-  sincospif(2.f * static_cast<float>(t - rint(t)), s, c);
+// The angles of `count` tokens; the whole turns go in 64 bits.
+__device__ inline void turns(Angles& a, const int* positions, int count, int half) {
+  __syncthreads();  // the last tokens' are read
+  for (int n = threadIdx.x; n < count * half; n += kThreads) {
+    const double t = a.freq[n % half] * positions[n / half];
+    sincospif(2.f * static_cast<float>(t - rint(t)), &a.turn[n].y, &a.turn[n].x);
+  }
+  __syncthreads();
 }
 
-// Units of work: `heads_per` heads of a token; group g of the launch takes
-// units g, g + groups, ... Heads are taken kHeads at a time, loaded before the
-// first is worked on: a row is a few hundred bytes, and the memory needs more
-// of them under way than there are waves.
-constexpr int kHeads = 4, kGradHeads = 2;
+// Rows are taken kRows at a time, loaded before the first is worked on: a row is
+// a few hundred bytes, and the memory needs more of them under way than there
+// are waves.
+constexpr int kRows = 2, kGradRows = 2;
 
-template <int VEC, int G, int NV>
+template <int VEC, int G, int NV, bool Stream>
 __device__ inline void forward(float* __restrict__ out, const float* __restrict__ x, const float* __restrict__ w,
-                               const int* __restrict__ positions, int tokens, int heads, int dim, int heads_per,
-                               float eps, float log2_base_hi, float log2_base_lo, bool stream) {
-  const int half = dim / 2, sub = threadIdx.x % G;
-  const unsigned groups = gridDim.x * (kThreads / G);
-  const unsigned chunks = (heads + heads_per - 1) / heads_per;
-  const unsigned units = static_cast<unsigned>(tokens) * chunks;
-  double freq[NV][VEC];
-  frequencies<VEC, G, NV>(freq, sub, half, static_cast<double>(log2_base_hi) + log2_base_lo);
+                               const int* __restrict__ positions, int tokens, int heads, int dim, int per, float eps,
+                               float log2_base_hi, float log2_base_lo) {
+  __shared__ Angles angles;
+  const int half = dim / 2, sub = threadIdx.x % G, group = threadIdx.x / G;
+  constexpr int kGroups = kThreads / G;
+  frequencies(angles, half, static_cast<double>(log2_base_hi) + log2_base_lo);
   Vec<VEC> wa[NV], wb[NV];
 #pragma unroll
   for (int v = 0; v < NV; v++) {
@@ -105,31 +106,27 @@ __device__ inline void forward(float* __restrict__ out, const float* __restrict_
       wb[v] = load<VEC>(w + half + i);
     }
   }
-  for (unsigned u = blockIdx.x * (kThreads / G) + threadIdx.x / G; u < units; u += groups) {
-    const unsigned token = u / chunks;
-    const int h0 = static_cast<int>(u % chunks) * heads_per, h1 = min(heads, h0 + heads_per);
-    const int pos = positions[token];
-    float c[NV][VEC], s[NV][VEC];
+  for (int first = blockIdx.x * per; first < tokens; first += gridDim.x * per) {
+    const int count = min(per, tokens - first), rows = count * heads;
+    turns(angles, positions + first, count, half);
+    const size_t base = static_cast<size_t>(first) * heads * dim;
+    for (int r0 = group; r0 < rows; r0 += kRows * kGroups) {
+      Vec<VEC> a[kRows][NV], b[kRows][NV];
 #pragma unroll
-    for (int v = 0; v < NV; v++)
-#pragma unroll
-      for (int e = 0; e < VEC; e++) turn(freq[v][e], pos, &c[v][e], &s[v][e]);
-    for (int h = h0; h < h1; h += kHeads) {
-      Vec<VEC> a[kHeads][NV], b[kHeads][NV];
-#pragma unroll
-      for (int k = 0; k < kHeads; k++) {
-        const float* row = x + (static_cast<size_t>(token) * heads + min(h + k, h1 - 1)) * dim;
+      for (int k = 0; k < kRows; k++) {
+        const float* row = x + base + static_cast<size_t>(min(r0 + k * kGroups, rows - 1)) * dim;
 #pragma unroll
         for (int v = 0; v < NV; v++) {
           const int i = (v * G + sub) * VEC;
           if (i < half) {
-            a[k][v] = load<VEC>(row + i);
-            b[k][v] = load<VEC>(row + half + i);
+            a[k][v] = load<VEC, Stream>(row + i);
+            b[k][v] = load<VEC, Stream>(row + half + i);
           }
         }
       }
 #pragma unroll
-      for (int k = 0; k < kHeads; k++) {
+      for (int k = 0; k < kRows; k++) {
+        const int r = r0 + k * kGroups;
         float ss = 0.f;
 #pragma unroll
         for (int v = 0; v < NV; v++)
@@ -137,9 +134,10 @@ __device__ inline void forward(float* __restrict__ out, const float* __restrict_
 #pragma unroll
             for (int e = 0; e < VEC; e++) ss += a[k][v].v[e] * a[k][v].v[e] + b[k][v].v[e] * b[k][v].v[e];
           }
-        const float r = 1.f / sqrtf(group_sum<G>(ss) / dim + eps);
-        if (h + k >= h1) continue;
-        float* row = out + (static_cast<size_t>(token) * heads + h + k) * dim;
+        const float inv = 1.f / sqrtf(group_sum<G>(ss) / dim + eps);
+        if (r >= rows) continue;
+        const float2* turn = angles.turn + r / heads * half;
+        float* row = out + base + static_cast<size_t>(r) * dim;
 #pragma unroll
         for (int v = 0; v < NV; v++) {
           const int i = (v * G + sub) * VEC;
@@ -147,30 +145,29 @@ __device__ inline void forward(float* __restrict__ out, const float* __restrict_
           Vec<VEC> ya, yb;
 #pragma unroll
           for (int e = 0; e < VEC; e++) {
-            const float za = a[k][v].v[e] * r * wa[v].v[e], zb = b[k][v].v[e] * r * wb[v].v[e];
-            ya.v[e] = za * c[v][e] - zb * s[v][e];
-            yb.v[e] = zb * c[v][e] + za * s[v][e];
+            const float2 cs = turn[i + e];
+            const float za = a[k][v].v[e] * inv * wa[v].v[e], zb = b[k][v].v[e] * inv * wb[v].v[e];
+            ya.v[e] = za * cs.x - zb * cs.y;
+            yb.v[e] = zb * cs.x + za * cs.y;
           }
-          store<VEC>(row + i, ya, stream);
-          store<VEC>(row + half + i, yb, stream);
+          store<VEC, Stream>(row + i, ya);
+          store<VEC, Stream>(row + half + i, yb);
         }
       }
     }
   }
 }
 
-template <int VEC, int G, int NV>
+template <int VEC, int G, int NV, bool Stream>
 __device__ inline void backward(float* __restrict__ dx, const float* __restrict__ x, const float* __restrict__ w,
                                 const int* __restrict__ positions, const float* __restrict__ g,
-                                float* __restrict__ partial, int tokens, int heads, int dim, int heads_per, float eps,
-                                float log2_base_hi, float log2_base_lo, bool stream) {
+                                float* __restrict__ partial, int tokens, int heads, int dim, int per, float eps,
+                                float log2_base_hi, float log2_base_lo) {
+  __shared__ Angles angles;
   __shared__ float sums[kThreads * 2 * NV * VEC];  // [group of the workgroup][half][index], index < G * NV * VEC
   const int half = dim / 2, sub = threadIdx.x % G, group = threadIdx.x / G;
-  const unsigned groups = gridDim.x * (kThreads / G);
-  const unsigned chunks = (heads + heads_per - 1) / heads_per;
-  const unsigned units = static_cast<unsigned>(tokens) * chunks;
-  double freq[NV][VEC];
-  frequencies<VEC, G, NV>(freq, sub, half, static_cast<double>(log2_base_hi) + log2_base_lo);
+  constexpr int kGroups = kThreads / G;
+  frequencies(angles, half, static_cast<double>(log2_base_hi) + log2_base_lo);
   Vec<VEC> wa[NV], wb[NV];
   float da[NV][VEC] = {}, db[NV][VEC] = {};
 #pragma unroll
@@ -181,51 +178,50 @@ __device__ inline void backward(float* __restrict__ dx, const float* __restrict_
       wb[v] = load<VEC>(w + half + i);
     }
   }
-  for (unsigned u = blockIdx.x * (kThreads / G) + group; u < units; u += groups) {
-    const unsigned token = u / chunks;
-    const int h0 = static_cast<int>(u % chunks) * heads_per, h1 = min(heads, h0 + heads_per);
-    const int pos = positions[token];
-    float c[NV][VEC], s[NV][VEC];
+  for (int first = blockIdx.x * per; first < tokens; first += gridDim.x * per) {
+    const int count = min(per, tokens - first), rows = count * heads;
+    turns(angles, positions + first, count, half);
+    const size_t base = static_cast<size_t>(first) * heads * dim;
+    for (int r0 = group; r0 < rows; r0 += kGradRows * kGroups) {
+      Vec<VEC> a[kGradRows][NV], b[kGradRows][NV], p[kGradRows][NV], q[kGradRows][NV];  // x and g
 #pragma unroll
-    for (int v = 0; v < NV; v++)
-#pragma unroll
-      for (int e = 0; e < VEC; e++) turn(freq[v][e], pos, &c[v][e], &s[v][e]);
-    for (int h = h0; h < h1; h += kGradHeads) {
-      Vec<VEC> a[kGradHeads][NV], b[kGradHeads][NV], p[kGradHeads][NV], q[kGradHeads][NV];  // x and g
-#pragma unroll
-      for (int k = 0; k < kGradHeads; k++) {
-        const size_t row = (static_cast<size_t>(token) * heads + min(h + k, h1 - 1)) * dim;
+      for (int k = 0; k < kGradRows; k++) {
+        const size_t row = base + static_cast<size_t>(min(r0 + k * kGroups, rows - 1)) * dim;
 #pragma unroll
         for (int v = 0; v < NV; v++) {
           const int i = (v * G + sub) * VEC;
           if (i < half) {
-            a[k][v] = load<VEC>(x + row + i);
-            b[k][v] = load<VEC>(x + row + half + i);
-            p[k][v] = load<VEC>(g + row + i);
-            q[k][v] = load<VEC>(g + row + half + i);
+            a[k][v] = load<VEC, Stream>(x + row + i);
+            b[k][v] = load<VEC, Stream>(x + row + half + i);
+            p[k][v] = load<VEC, Stream>(g + row + i);
+            q[k][v] = load<VEC, Stream>(g + row + half + i);
           }
         }
       }
 #pragma unroll
-      for (int k = 0; k < kGradHeads; k++) {
+      for (int k = 0; k < kGradRows; k++) {
+        const int r = r0 + k * kGroups;
+        const float2* turn = angles.turn + min(r, rows - 1) / heads * half;
         float ss = 0.f, sg = 0.f;  // sums of x^2 and of g' w x
 #pragma unroll
         for (int v = 0; v < NV; v++) {
-          if ((v * G + sub) * VEC >= half) continue;
+          const int i = (v * G + sub) * VEC;
+          if (i >= half) continue;
 #pragma unroll
           for (int e = 0; e < VEC; e++) {
-            const float ga = p[k][v].v[e] * c[v][e] + q[k][v].v[e] * s[v][e];
-            const float gb = q[k][v].v[e] * c[v][e] - p[k][v].v[e] * s[v][e];
+            const float2 cs = turn[i + e];
+            const float ga = p[k][v].v[e] * cs.x + q[k][v].v[e] * cs.y;
+            const float gb = q[k][v].v[e] * cs.x - p[k][v].v[e] * cs.y;
             p[k][v].v[e] = ga;
             q[k][v].v[e] = gb;
             ss += a[k][v].v[e] * a[k][v].v[e] + b[k][v].v[e] * b[k][v].v[e];
             sg += ga * wa[v].v[e] * a[k][v].v[e] + gb * wb[v].v[e] * b[k][v].v[e];
           }
         }
-        const float r = 1.f / sqrtf(group_sum<G>(ss) / dim + eps);
-        const float mean = group_sum<G>(sg) * r / dim;
-        if (h + k >= h1) continue;
-        float* row = dx + (static_cast<size_t>(token) * heads + h + k) * dim;
+        const float inv = 1.f / sqrtf(group_sum<G>(ss) / dim + eps);
+        const float mean = group_sum<G>(sg) * inv / dim;
+        if (r >= rows) continue;
+        float* row = dx + base + static_cast<size_t>(r) * dim;
 #pragma unroll
         for (int v = 0; v < NV; v++) {
           const int i = (v * G + sub) * VEC;
@@ -233,14 +229,14 @@ __device__ inline void backward(float* __restrict__ dx, const float* __restrict_
           Vec<VEC> oa, ob;
 #pragma unroll
           for (int e = 0; e < VEC; e++) {
-            const float na = a[k][v].v[e] * r, nb = b[k][v].v[e] * r;
-            oa.v[e] = r * (p[k][v].v[e] * wa[v].v[e] - na * mean);
-            ob.v[e] = r * (q[k][v].v[e] * wb[v].v[e] - nb * mean);
+            const float na = a[k][v].v[e] * inv, nb = b[k][v].v[e] * inv;
+            oa.v[e] = inv * (p[k][v].v[e] * wa[v].v[e] - na * mean);
+            ob.v[e] = inv * (q[k][v].v[e] * wb[v].v[e] - nb * mean);
             da[v][e] += p[k][v].v[e] * na;
             db[v][e] += q[k][v].v[e] * nb;
           }
-          store<VEC>(row + i, oa, stream);
-          store<VEC>(row + half + i, ob, stream);
+          store<VEC, Stream>(row + i, oa);
+          store<VEC, Stream>(row + half + i, ob);
         }
       }
     }
@@ -265,20 +261,23 @@ __device__ inline void backward(float* __restrict__ dx, const float* __restrict_
 
 }  // namespace
 
-#define FG_NORM_ROTATE(VEC, G, NV)                                                                                     \
-  extern "C" __global__ void __launch_bounds__(kThreads) fg_norm_rotate_##VEC##_##G##_##NV(                            \
-      float* out, const float* x, const float* w, const int* positions, int tokens, int heads, int dim, int heads_per, \
-      float eps, float log2_base_hi, float log2_base_lo, int stream) {                                                 \
-    forward<VEC, G, NV>(out, x, w, positions, tokens, heads, dim, heads_per, eps, log2_base_hi, log2_base_lo,          \
-                          stream);                                                                                     \
-  }                                                                                                                    \
-  extern "C" __global__ void __launch_bounds__(kThreads) fg_norm_rotate_grad_##VEC##_##G##_##NV(                       \
-      float* dx, const float* x, const float* w, const int* positions, const float* g, float* dw, float* partial,      \
-      int blocks, int tokens, int heads, int dim, int heads_per, float eps, float log2_base_hi, float log2_base_lo,    \
-      int stream) {                                                                                                    \
-    backward<VEC, G, NV>(dx, x, w, positions, g, partial, tokens, heads, dim, heads_per, eps, log2_base_hi,            \
-                         log2_base_lo, stream);                                                                        \
+#define FG_NORM_ROTATE_AS(VEC, G, NV, NAME, STREAM)                                                                   \
+  extern "C" __global__ void __launch_bounds__(kThreads) fg_norm_rotate_##NAME(                                       \
+      float* out, const float* x, const float* w, const int* positions, int tokens, int heads, int dim,               \
+      int per, float eps, float log2_base_hi, float log2_base_lo) {                                             \
+    forward<VEC, G, NV, STREAM>(out, x, w, positions, tokens, heads, dim, per, eps, log2_base_hi,               \
+                                log2_base_lo);                                                                        \
+  }                                                                                                                   \
+  extern "C" __global__ void __launch_bounds__(kThreads) fg_norm_rotate_grad_##NAME(                                  \
+      float* dx, const float* x, const float* w, const int* positions, const float* g, float* dw, float* partial,     \
+      int blocks, int tokens, int heads, int dim, int per, float eps, float log2_base_hi,                       \
+      float log2_base_lo) {                                                                                           \
+    backward<VEC, G, NV, STREAM>(dx, x, w, positions, g, partial, tokens, heads, dim, per, eps, log2_base_hi,   \
+                                 log2_base_lo);                                                                       \
   }
+#define FG_NORM_ROTATE(VEC, G, NV)                         \
+  FG_NORM_ROTATE_AS(VEC, G, NV, VEC##_##G##_##NV, false)   \
+  FG_NORM_ROTATE_AS(VEC, G, NV, VEC##_##G##_##NV##_stream, true)
 
 FG_NORM_ROTATE(4, 8, 1)
 FG_NORM_ROTATE(4, 16, 1)
@@ -299,8 +298,8 @@ FG_NORM_ROTATE(1, 64, 4)
 // dw from the workgroups' sums: 16 columns a workgroup, 64 slices of them.
 extern "C" __global__ void __launch_bounds__(1024)
     fg_norm_rotate_weight(float* dx, const float* x, const float* w, const int* positions, const float* g, float* dw,
-                          const float* partial, int blocks, int tokens, int heads, int dim, int heads_per, float eps,
-                          float log2_base_hi, float log2_base_lo, int stream) {
+                          const float* partial, int blocks, int tokens, int heads, int dim, int per, float eps,
+                          float log2_base_hi, float log2_base_lo) {
   __shared__ float sums[64][16];
   const int col = threadIdx.x % 16, slice = threadIdx.x / 16, d = blockIdx.x * 16 + col;
   float t = 0.f;

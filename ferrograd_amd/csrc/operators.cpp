@@ -164,24 +164,28 @@ RenderedKernel render_norm_rotate(const UOp& call, bool grad) {
   const int64_t tokens = p[0], heads = p[1], dim = p[2];
   const double eps = from_bits(p[3]), log2_base = std::log2(from_bits(p[4]));
   const RowSplit r = row_split(dim);
-  // Heads of a token that share its cosines: more while 8192 groups are left.
-  const int64_t heads_per = std::max<int64_t>(1, std::min<int64_t>({heads, 8, tokens * heads / 8192}));
-  const int64_t units = tokens * ((heads + heads_per - 1) / heads_per), per_block = 256 / r.lanes;
-  const int64_t blocks = std::min<int64_t>((units + per_block - 1) / per_block, grad ? 1024 : 4096);
+  // Tokens whose angles a workgroup makes at a time: as many as it has threads
+  // for, more until its groups of lanes have four rows each, fewer while there
+  // are not four workgroups a compute unit.
+  const int64_t half = dim / 2, groups = 256 / r.lanes;
+  int64_t per = std::max<int64_t>(1, 256 / half);
+  while (per * heads < 4 * groups && 2 * per * half <= 1024) per *= 2;
+  while (per > 1 && (tokens + per - 1) / per < 1024) per /= 2;
+  const int64_t blocks = std::min<int64_t>((tokens + per - 1) / per, grad ? 1024 : 2048);
   RenderedKernel rk;
   set_image(rk, fg_image_norm_rotate, fg_image_norm_rotate_end);
   const float hi = static_cast<float>(log2_base);
-  const std::vector<CallArg> tail = {CallArg::i32(tokens), CallArg::i32(heads), CallArg::i32(dim), CallArg::i32(heads_per),
+  const std::vector<CallArg> tail = {CallArg::i32(tokens), CallArg::i32(heads), CallArg::i32(dim), CallArg::i32(per),
                                      CallArg::f32(static_cast<float>(eps)), CallArg::f32(hi),
-                                     CallArg::f32(static_cast<float>(log2_base - hi)),
-                                     CallArg::i32(4 * tokens * heads * dim >= static_cast<int64_t>(kStreamBytes))};
+                                     CallArg::f32(static_cast<float>(log2_base - hi))};
+  const std::string name = r.suffix() + (4 * tokens * heads * dim >= static_cast<int64_t>(kStreamBytes) ? "_stream" : "");
   rk.call_args = {CallArg::slot(0), CallArg::slot(1), CallArg::slot(2), CallArg::slot(3)};
   if (!grad) {
     rk.kind = "norm_rotate";
-    rk.launches = {launch("fg_norm_rotate" + r.suffix(), static_cast<uint64_t>(blocks), 256, "norm_rotate")};
+    rk.launches = {launch("fg_norm_rotate" + name, static_cast<uint64_t>(blocks), 256, "norm_rotate")};
   } else {
     rk.kind = "norm_rotate_grad";
-    rk.launches = {launch("fg_norm_rotate_grad" + r.suffix(), static_cast<uint64_t>(blocks), 256, "norm_rotate"),
+    rk.launches = {launch("fg_norm_rotate_grad" + name, static_cast<uint64_t>(blocks), 256, "norm_rotate"),
                    launch("fg_norm_rotate_weight", static_cast<uint64_t>((dim + 15) / 16), 1024, "norm_rotate")};
     rk.workspace_bytes = static_cast<size_t>(blocks * dim) * 4;
     rk.side_outputs = {5};
