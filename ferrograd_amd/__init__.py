@@ -18,7 +18,7 @@ from typing import Iterable, Sequence
 
 import numpy as np
 
-__all__ = ["Tensor", "Linear", "Sgd", "FerrogradError", "lib", "stats", "synchronize", "reset_init_seed",
+__all__ = ["Tensor", "Linear", "Dropout", "Sgd", "FerrogradError", "lib", "stats", "synchronize", "reset_init_seed",
            "debug_plan", "F32", "I32", "BOOL", "clear_caches"]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -375,6 +375,27 @@ class Linear:
         if _lib is not None and getattr(self, "_h", None):
             _lib.fg_linear_free(self._h)
             self._h = None
+
+
+class Dropout:
+    """Dropout as a layer (no reference counterpart): Tensor.dropout under a seed
+    of its own, each call with the next offset and so a mask of its own. Layers
+    that should draw apart need different seeds. With `training` off it hands its
+    input on."""
+
+    def __init__(self, p: float, seed: int = 42):
+        if not 0.0 <= p < 1.0:
+            raise FerrogradError(f"Dropout: p must be in [0, 1), got {p}")
+        self.p, self.seed, self.offset, self.training = float(p), int(seed), 0, True
+
+    def forward(self, x: Tensor) -> Tensor:
+        if not self.training or self.p == 0.0:
+            return x
+        y = x.dropout(self.p, self.seed, self.offset)
+        self.offset += 1
+        return y
+
+    __call__ = forward
 
 
 class Sgd:

@@ -7,7 +7,7 @@ from typing import Callable, Sequence
 
 import numpy as np
 
-from . import Linear, Sgd, Tensor
+from . import Dropout, FerrogradError, Linear, Sgd, Tensor
 
 
 def one_hot(labels: np.ndarray, num_classes: int) -> np.ndarray:
@@ -18,10 +18,20 @@ def one_hot(labels: np.ndarray, num_classes: int) -> np.ndarray:
 
 
 class Mlp:
-    """Linear -> ReLU -> ... -> Linear (mnist.rs:30-54 is dims = (784, 128, 10))."""
+    """Linear -> ReLU -> ... -> Linear (mnist.rs:30-54 is dims = (784, 128, 10)).
+    With `dropout` above 0, every hidden layer's ReLU is followed by a Dropout of
+    that probability under the seed `seed` + its index, while train() is on (as
+    it is at first)."""
 
-    def __init__(self, dims: Sequence[int], device=None):
+    def __init__(self, dims: Sequence[int], device=None, dropout: float = 0.0, seed: int = 42):
         self.layers = [Linear(dims[i], dims[i + 1], device) for i in range(len(dims) - 1)]
+        self.dropouts = [Dropout(dropout, seed + i) for i in range(len(dims) - 2)] if dropout else []
+
+    def train(self, on: bool = True) -> "Mlp":
+        """Turn dropout on or off."""
+        for d in self.dropouts:
+            d.training = on
+        return self
 
     def forward(self, x: Tensor) -> Tensor:
         return self.forward_preactivations(x)[-1]
@@ -38,6 +48,8 @@ class Mlp:
             zs.append(h)
             if i + 1 < len(self.layers):
                 h = h.relu()
+                if self.dropouts:
+                    h = self.dropouts[i](h)
         return zs
 
     def parameters(self) -> list:
@@ -58,12 +70,19 @@ def train_step(model: Mlp, opt: Sgd, x: Tensor, targets: Tensor, preactivations:
     return loss
 
 
+def _without_dropout(model: Mlp) -> None:
+    if model.dropouts:
+        raise FerrogradError("the native train loops run no dropout: drive the model with train_step")
+
+
 def train_steps_native(model: Mlp, opt: Sgd, x: Tensor, targets: Tensor, steps: int) -> list:
     """`steps` train steps as train_step, looped in native code
     (fg_mlp_train_steps), with each step's loss read back as
-    examples/mnist.rs:98 does; returns the losses."""
+    examples/mnist.rs:98 does; returns the losses. Models with dropout are
+    trained by train_step."""
     from . import train_steps_native as native
 
+    _without_dropout(model)
     return native(model.layers, opt, x, targets, steps)
 
 
@@ -72,9 +91,11 @@ def train_batches_native(model: Mlp, opt: Sgd, images: Tensor, targets: Tensor, 
     """`steps` train steps over narrow()ed batches of the resident `images`
     and `targets` (examples/mnist.rs:84-98), batch index first_batch + i
     wrapping over the whole batches, looped in native code
-    (fg_mlp_train_batches); returns the losses."""
+    (fg_mlp_train_batches); returns the losses. Models with dropout are
+    trained by train_step."""
     from . import train_batches_native as native
 
+    _without_dropout(model)
     return native(model.layers, opt, images, targets, batch_size, steps, first_batch)
 
 
@@ -113,16 +134,17 @@ def predictions(logits: np.ndarray) -> np.ndarray:
 
 
 def train_mnist(dataset, device=None, epochs: int = 5, batch_size: int = 256, lr: float = 0.01,
-                max_batches: int | None = None, log=print, native: bool = False) -> dict:
+                max_batches: int | None = None, log=print, native: bool = False, dropout: float = 0.0) -> dict:
     """examples/mnist.rs:59-126 on `device`: Linear(784,128) -> ReLU ->
     Linear(128,10), cross-entropy, SGD; batches are narrow()ed views of the
     resident training set. Returns per-batch losses and per-epoch average loss
     and test accuracy (percent). With `native`, each epoch's batch loop runs
     in native code (fg_mlp_train_batches: the same steps, captured and
-    replayed with each batch's start as an argument)."""
+    replayed with each batch's start as an argument). `dropout` is the hidden
+    layer's while it trains, off for the accuracy (not with `native`)."""
     train_targets = Tensor.new(one_hot(dataset.train_labels, dataset.num_classes),
                                [dataset.train_len(), dataset.num_classes], device)
-    model = Mlp((784, 128, 10), device)
+    model = Mlp((784, 128, 10), device, dropout=dropout)
     opt = Sgd(model.parameters(), lr)
     num_batches = dataset.train_len() // batch_size
     if max_batches is None:
@@ -154,7 +176,9 @@ def train_mnist(dataset, device=None, epochs: int = 5, batch_size: int = 256, lr
             if log:
                 log(f"  epoch {epoch} batch {b:>4}/{num_batches}  loss={v:.4f}")
         avg = float(epoch_loss / np.float32(runs))
+        model.train(False)
         logits = model.forward(dataset.test_images).numpy().reshape(dataset.test_len(), dataset.num_classes)
+        model.train()
         acc = float(np.float32(np.sum(predictions(logits) == dataset.test_labels)) / np.float32(dataset.test_len())
                     * np.float32(100.0))
         history["epoch_loss"].append(avg)
@@ -173,5 +197,6 @@ if __name__ == "__main__":
     ap.add_argument("--data", default="data/mnist")
     ap.add_argument("--device", default="hip")
     ap.add_argument("--epochs", type=int, default=5)
+    ap.add_argument("--dropout", type=float, default=0.0)
     a = ap.parse_args()
-    train_mnist(MNISTDataset.load(a.data, a.device), a.device, epochs=a.epochs)
+    train_mnist(MNISTDataset.load(a.data, a.device), a.device, epochs=a.epochs, dropout=a.dropout)

@@ -449,3 +449,157 @@ def test_the_same_inputs_give_the_same_bits(fg, hip):
     a, b = run_attention(fg, q, k, v, g, **kw), run_attention(fg, q, k, v, g, **kw)
     for n in a:
         assert np.array_equal(a[n], b[n]), n
+
+
+# ── together, as layers ─────────────────────────────────────────────────────
+
+
+def test_layers_refuse_what_their_calls_would(fg, cpu):
+    from ferrograd_amd.attention import SelfAttention
+    from ferrograd_amd.mlp import Mlp, train_steps_native
+
+    for kw, match in [(dict(heads=5), "do not split"), (dict(heads=32), "must be even"),
+                      (dict(heads=4, kv_heads=3), "do not share"), (dict(heads=1, head_dim=130), "at most 128")]:
+        with pytest.raises(fg.FerrogradError, match=match):
+            SelfAttention(32, device=cpu, **kw)
+    with pytest.raises(fg.FerrogradError, match="p must be in"):
+        fg.Dropout(1.0)
+    model = Mlp((4, 3, 2), cpu, dropout=0.5)
+    with pytest.raises(fg.FerrogradError, match="run no dropout"):
+        train_steps_native(model, None, None, None, 1)
+    x = cpu_tensor(fg, (5, 4))
+    assert model.train(False).forward(x).shape == (5, 2)  # and without dropout any device does
+
+
+class Torch64:
+    """The layers in float64 on the CPU."""
+
+    @staticmethod
+    def norm_rotate(x, w, pos, heads, eps, base):
+        import torch
+
+        n, d = x.shape[0], x.shape[1] // heads
+        z = x.reshape(n, heads, d)
+        z = z / torch.sqrt((z * z).mean(2, keepdim=True) + eps) * w
+        a = pos[:, None].double() * base ** (-torch.arange(d // 2).double() * 2 / d)
+        c, s = torch.cos(a)[:, None], torch.sin(a)[:, None]
+        l, r = z[..., :d // 2], z[..., d // 2:]
+        return torch.cat([l * c - r * s, r * c + l * s], 2).reshape(n, -1)
+
+    @staticmethod
+    def attention(q, k, v, heads, kv_heads, batch, lengths):
+        import torch
+
+        split = lambda t, h: t.reshape(batch, -1, h, t.shape[1] // h).transpose(1, 2)  # noqa: E731
+        q, k, v = split(q, heads), *(split(t, kv_heads).repeat_interleave(heads // kv_heads, 1) for t in (k, v))
+        s = q @ k.transpose(2, 3) / q.shape[3] ** 0.5
+        n = s.shape[2]
+        hide = torch.ones(n, n, dtype=torch.bool).triu(1)[None, None] | (
+            torch.arange(n)[None, None, None] >= lengths[:, None, None, None])
+        y = torch.softmax(s.masked_fill(hide, float("-inf")), 3) @ v
+        return y.transpose(1, 2).reshape(batch * n, -1)
+
+
+@pytest.mark.gpu
+def test_a_self_attention_layer_and_its_gradients(fg, hip):
+    import torch
+
+    from ferrograd_amd.attention import SelfAttention
+
+    batch, n, features, heads, kv_heads = 3, 41, 48, 6, 2
+    fg.reset_init_seed(3)
+    layer = SelfAttention(features, heads, kv_heads, head_dim=16, device=hip, dropout=0.25, seed=9)
+    r = seeded(31)
+    x, g = (r.standard_normal((batch * n, features)).astype(np.float32) for _ in range(2))
+    pos = np.tile(np.arange(n, dtype=np.int32), batch)
+    lengths = np.array([41, 7, 30], np.int32)
+    tx, tp, tl, tg = new(fg, x, True), new(fg, pos), new(fg, lengths), new(fg, g)
+    for step in range(3):  # the plan of the first step, then its replays, each with the next mask
+        y = layer(tx, tp, batch, tl)
+        params = layer.parameters()
+        grads = y.mul(tg).sum([0, 1]).gradient([tx, *params])
+        fg.Tensor.realize_many([y, *grads])
+        ps = [torch.tensor(p.numpy().astype(np.float64), requires_grad=True) for p in (tx, *params)]
+        px, wq, wk, wv, wo, nq, nk = ps
+        q = Torch64.norm_rotate(px @ wq.T, nq, torch.tensor(pos), heads, 1e-6, 10000.0)
+        k = Torch64.norm_rotate(px @ wk.T, nk, torch.tensor(pos), kv_heads, 1e-6, 10000.0)
+        out = Torch64.attention(q, k, px @ wv.T, heads, kv_heads, batch, torch.tensor(lengths)) @ wo.T
+        keep = philox(out.numel(), 9, step).reshape(out.shape) >= 1 << 30
+        want = out * torch.tensor(keep / 0.75)
+        want_grads = torch.autograd.grad((want * torch.tensor(g.astype(np.float64))).sum(), ps)
+        # Each of the nine products, norms and softmaxes on a value's way is off
+        # by at most its terms (features, heads' sizes, keys, tokens summed over)
+        # times half a step of its terms' magnitudes; 16 for magnitudes over sums.
+        tol = 9 * 16 * (features + heads * 16 + n + batch * n) * U
+        for name, got, ref in [("y", y, want)] + list(zip("x wq wk wv wo nq nk".split(), grads, want_grads)):
+            ref = ref.detach().numpy()
+            off = np.linalg.norm(got.numpy() - ref) / np.linalg.norm(ref)
+            assert off <= tol, (step, name, off, tol)
+    before = layer.train(False)(tx, tp, batch, tl).numpy()
+    assert np.array_equal(before, layer(tx, tp, batch, tl).numpy())  # no dropout
+
+
+@pytest.mark.gpu
+def test_a_sequence_classifier_trains(fg, hip):
+    # Two layers around a residual, a classifier on top, SGD in place: every
+    # parameter moves and the loss is the one that the parameters before it give.
+    from ferrograd_amd.attention import SelfAttention
+
+    fg.reset_init_seed(5)
+    layers = [SelfAttention(32, 4, 2, device=hip, dropout=0.1, seed=i) for i in range(2)]
+    head = fg.Linear(32, 5, hip)
+    params = [p for l in layers for p in l.parameters()] + head.parameters()
+    opt = fg.Sgd(params, 0.05)
+    r = seeded(32)
+    pos = new(fg, np.tile(np.arange(20, dtype=np.int32), 4))
+    before = [p.numpy().copy() for p in params]
+    for step in range(4):
+        h = new(fg, r.standard_normal((80, 32)).astype(np.float32))
+        t = new(fg, np.eye(5, dtype=np.float32)[r.integers(0, 5, 80)])
+        for l in layers:
+            h = h.add(l(h, pos, 4))
+        loss = head(h).cross_entropy(t)
+        opt.zero_grad()
+        loss.backward()
+        opt.step()
+        assert np.isfinite(loss.to_vec()[0])
+    for p, b in zip(params, before):
+        assert np.isfinite(p.numpy()).all() and not np.array_equal(p.numpy(), b)
+
+
+@pytest.mark.gpu
+def test_an_mlp_with_dropout_takes_the_masks_gradient(fg, hip):
+    from ferrograd_amd.mlp import Mlp, synthetic_batch, train_step
+
+    dims, lr = (24, 40, 33, 6), 0.5
+    fg.reset_init_seed(7)
+    model = Mlp(dims, hip, dropout=0.5, seed=70)
+    opt = fg.Sgd(model.parameters(), lr)
+    xs, ts = synthetic_batch(50, 24, 6, 1, 2)
+    x, t = new(fg, xs), new(fg, ts)
+    for step in range(4):
+        p0 = [p.numpy().astype(np.float64) for p in model.parameters()]
+        zs = []
+        loss = train_step(model, opt, x, t, zs).to_vec()[0]
+        hs, h = [xs.astype(np.float64)], xs.astype(np.float64)
+        masks = []
+        for i in range(3):
+            z = h @ p0[2 * i].T + p0[2 * i + 1]
+            if i < 2:
+                # The device's own signs: a value within rounding of 0 may fall on either side.
+                on = zs[i].numpy() > 0
+                masks.append((philox(z.size, 70 + i, step).reshape(z.shape) >= 1 << 31) * 2.0 * on)
+                h = z * masks[-1]
+                hs.append(h)
+        logp = z - z.max(1, keepdims=True)
+        logp -= np.log(np.exp(logp).sum(1, keepdims=True))
+        assert abs(loss + (ts * logp).sum() / 50) <= 1e-5
+        dz = (np.exp(logp) - ts) / 50
+        for i in reversed(range(3)):
+            for j, want in ((2 * i, dz.T @ hs[i]), (2 * i + 1, dz.sum(0))):
+                got = (p0[j] - model.parameters()[j].numpy()) / lr
+                # The update's rounding, half a step of the parameter over lr, and 128 for the products before.
+                bound = U * (np.abs(p0[j]) + 1) * 2 / lr + 128 * U * np.abs(want).max()
+                assert np.abs(got - want).max() <= bound.max(), (step, j)
+            if i:
+                dz = (dz @ p0[2 * i]) * masks[i - 1]
