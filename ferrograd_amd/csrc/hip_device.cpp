@@ -472,6 +472,12 @@ class HipDevice : public Device {
       a[2].v.i = rb->words;
       return a;
     };
+    // The largest workspace of the sequence first: all of its arguments are
+    // marshalled before any of it is launched, and an address must not be
+    // given back in between.
+    size_t workspace_need = 0;
+    for (Program* p : progs) workspace_need = std::max(workspace_need, p->meta.workspace_bytes);
+    if (workspace_need) workspace(workspace_need);
     std::vector<fg_prog*> lp;
     std::vector<unsigned> grids, blocks, lds;
     std::vector<int> nargs;

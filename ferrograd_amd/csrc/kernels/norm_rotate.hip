@@ -106,8 +106,8 @@ __device__ inline void forward(float* __restrict__ out, const float* __restrict_
       wb[v] = load<VEC>(w + half + i);
     }
   }
-  for (int first = blockIdx.x * per; first < tokens; first += gridDim.x * per) {
-    const int count = min(per, tokens - first), rows = count * heads;
+  for (unsigned first = blockIdx.x * per; first < static_cast<unsigned>(tokens); first += gridDim.x * per) {
+    const int count = min(per, static_cast<int>(tokens - first)), rows = count * heads;
     turns(angles, positions + first, count, half);
     const size_t base = static_cast<size_t>(first) * heads * dim;
     for (int r0 = group; r0 < rows; r0 += kRows * kGroups) {
@@ -178,8 +178,8 @@ __device__ inline void backward(float* __restrict__ dx, const float* __restrict_
       wb[v] = load<VEC>(w + half + i);
     }
   }
-  for (int first = blockIdx.x * per; first < tokens; first += gridDim.x * per) {
-    const int count = min(per, tokens - first), rows = count * heads;
+  for (unsigned first = blockIdx.x * per; first < static_cast<unsigned>(tokens); first += gridDim.x * per) {
+    const int count = min(per, static_cast<int>(tokens - first)), rows = count * heads;
     turns(angles, positions + first, count, half);
     const size_t base = static_cast<size_t>(first) * heads * dim;
     for (int r0 = group; r0 < rows; r0 += kGradRows * kGroups) {

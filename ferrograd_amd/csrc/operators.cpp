@@ -58,8 +58,9 @@ Shape shape_of(const UOp& call) {
   return Shape(a.v.begin(), a.v.begin() + a.b);
 }
 
-// A matrix a call reads: as it is, except that a literal or a value behind an
-// in-place store is copied first (both need a kernel that writes them out).
+// A matrix a call reads: as it is, except that a literal is written out first,
+// and a tensor with an in-place update not yet realised goes the way it goes in
+// every other op.
 UOp source(const UOp& u) {
   UOp b = u;
   while (b.op() == Op::Reshape) b = b.src(0);
@@ -363,6 +364,7 @@ Tensor Tensor::attention(const Tensor& k, const Tensor& v, const Tensor* lengths
     FG_CHECK(lengths->dtype() == DType::I32() && lengths->shape() == Shape{batch},
              "attention: the lengths must be i32 of shape " + shape_str(Shape{batch}) + ", got " + shape_str(lengths->shape()));
   FG_CHECK(std::isfinite(scale) && std::isfinite(static_cast<float>(scale)), "attention: scale must be finite");
+  FG_CHECK(batch <= 0x7fffffffu && heads <= 0x7fffffffu, "attention: more than 2^31 - 1 sequences or heads");
   const size_t sq = qs[0] / batch, sk = ks[0] / batch;
   FG_CHECK(sq <= (1u << 28) && sk <= (1u << 28), "attention: sequences of more than 2^28 tokens");
   need_hip(*this, "attention");

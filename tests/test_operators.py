@@ -443,6 +443,52 @@ def test_gradients_realised_after_their_loss(fg, hip):
 
 
 @pytest.mark.gpu
+def test_calls_read_views_and_literals_and_update_in_place(fg, hip):
+    r = seeded(40)
+    x, m = r.standard_normal((12, 8)).astype(np.float32), r.standard_normal((8, 12)).astype(np.float32)
+    t, tm = new(fg, x, True), new(fg, m)
+    assert np.array_equal(t.permute([1, 0]).dropout(0.5, 1).numpy(), dropped(x.T, 0.5, 1, 0))
+    assert np.array_equal(t.narrow(0, 5, 6).dropout(0.5, 1).numpy(), dropped(x[5:11], 0.5, 1, 0))
+    assert np.array_equal(t.narrow(1, 3, 4).dropout(0.5, 1).numpy(), dropped(x[:, 3:7], 0.5, 1, 0))
+    # Read by the call and by another root: both see the same values.
+    h = t.permute([1, 0]).add(tm)
+    y = h.dropout(0.5, 2)
+    fg.Tensor.realize_many([h, y])
+    assert np.array_equal(h.numpy(), x.T + m) and np.array_equal(y.numpy(), dropped(x.T + m, 0.5, 2, 0))
+    # A gradient that is a literal, and one that sums over a broadcast.
+    ones = t.dropout(0.5, 3).sum([0, 1]).gradient([t])[0].numpy()
+    assert np.array_equal(ones, dropped(np.ones_like(x), 0.5, 3, 0))
+    row = new(fg, x[:1], True)
+    d = row.expand([12, 8]).dropout(0.5, 4).sum([0, 1]).gradient([row])[0].numpy()
+    assert np.array_equal(d, dropped(np.ones_like(x), 0.5, 4, 0).sum(0, keepdims=True))
+    # Attention over transposed, narrowed keys.
+    kv = r.standard_normal((16, 20)).astype(np.float32)
+    tkv = new(fg, kv)
+    k, v = tkv.narrow(0, 0, 8).permute([1, 0]), tkv.narrow(0, 8, 8).permute([1, 0])
+    check("y", t.attention(k, v, heads=2).numpy(), *attention_ref.attention(x, kv[:8].T, kv[8:].T, 1, 2, 2)["y"])
+    # In place: the call reads what the store replaces.
+    z = new(fg, x)
+    for step in range(3):
+        z.assign(z.dropout(0.5, 5, step))
+        z.realize()
+    assert np.array_equal(z.numpy(), dropped(dropped(dropped(x, 0.5, 5, 0), 0.5, 5, 1), 0.5, 5, 2))
+
+
+@pytest.mark.gpu
+def test_two_calls_of_one_realisation_share_the_workspace(fg, hip):
+    q, k, v, _ = attention_inputs(41, 1, 300, 300, 4, 4, 64)
+    tq, tk, tv = (new(fg, x) for x in (q, k, v))
+    want = attention_ref.attention(q, k, v, 1, 4, 4)["y"]
+    for step in range(3):
+        small = tq.attention(tk, tv, heads=4)
+        big = tq.attention(tk.permute([1, 0]).permute([1, 0]).contiguous(), tv, heads=4, causal=True)
+        fg.Tensor.realize_many([small, big])
+        check("small", small.numpy(), *want)
+        check("big", big.numpy(), *attention_ref.attention(q, k, v, 1, 4, 4, causal=True)["y"])
+        fg.clear_caches() if step == 1 else None
+
+
+@pytest.mark.gpu
 def test_the_same_inputs_give_the_same_bits(fg, hip):
     q, k, v, g = attention_inputs(13, 2, 300, 300, 4, 2, 64)
     kw = dict(batch=2, heads=4, kv_heads=2, causal=True)
