@@ -452,12 +452,12 @@ __device__ inline void join_parts(float* __restrict__ y, float* __restrict__ sta
 // and what is left for the end is small. Workgroups go to the 8 chiplets in turn, so
 // where the heads allow it each chiplet gets heads next to each other, which
 // share keys in its cache.
-__device__ inline void query_tile(const Shape& s, int rows, int splits, int* qt, int* h, int* b, int* split) {
+__device__ inline void query_tile(const Shape& s, int rows, int splits, unsigned block, int* qt, int* h, int* b, int* split) {
   const unsigned heads = static_cast<unsigned>(s.b) * s.hq, tiles = (s.sq + rows - 1) / rows;
-  unsigned head = blockIdx.x % heads;
+  unsigned head = block % heads;
   if (heads % 8 == 0) head = head % 8 * (heads / 8) + head / 8;
-  *split = blockIdx.x / heads % splits;
-  *qt = tiles - 1 - blockIdx.x / heads / splits;
+  *split = block / heads % splits;
+  *qt = tiles - 1 - block / heads / splits;
   *h = head % s.hq;
   *b = head / s.hq;
 }
@@ -476,7 +476,7 @@ __device__ inline void forward_tiles(float* __restrict__ y, const float* __restr
   // wait for them first.
   __shared__ __attribute__((aligned(1024))) char even[kTile], odd[kTile];
   int qt, h, b, split;
-  query_tile(s, 128, splits, &qt, &h, &b, &split);
+  query_tile(s, 128, splits, blockIdx.x, &qt, &h, &b, &split);
   const int hk = h / (s.hq / s.hk);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, half = lane / 32;
   const int i = qt * 128 + wave * 32 + lane % 32;  // this lane's query
@@ -749,13 +749,13 @@ constexpr int kQueryGradWaves = NB < 4 ? 4 : 8;
 template <int NB, int Waves>
 __device__ inline void query_grads(float* __restrict__ dq, const float* __restrict__ q, const float* __restrict__ g,
                                    const float* __restrict__ stats, const int* __restrict__ lengths,
-                                   char* __restrict__ ws, const Shape& s, float scale, int parts, int q_parts) {
+                                   char* __restrict__ ws, const Shape& s, float scale, int parts, int q_parts,
+                                   unsigned block, char* even, char* odd) {
   constexpr int kTile = kKeyTile<NB>;
-  __shared__ __attribute__((aligned(1024))) char even[kTile], odd[kTile];
   const GradSpace f = grad_space<NB>(ws, s);
   int qt, h, b, part;
   constexpr int kRows = 32 * Waves;
-  query_tile(s, kRows, q_parts, &qt, &h, &b, &part);
+  query_tile(s, kRows, q_parts, block, &qt, &h, &b, &part);
   const int hk = h / (s.hq / s.hk);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, half = lane / 32;
   const int first = qt * kRows + wave * 32, i = first + lane % 32;
@@ -861,19 +861,23 @@ __device__ inline void query_grads(float* __restrict__ dq, const float* __restri
 // cover each other's waits. More groups leave room for one workgroup, with two
 // buffers of whole tiles.
 template <int NB>
+constexpr int kGradRows = 2 * kRowBytes<NB> + kTail;
+template <int NB>
+constexpr int kGradCols = 2 * kColBytes<NB>;
+typedef float4 Probs[4][64];  // of a pair: [registers 4 c .. 4 c + 3][lane]
+
+template <int NB, bool kTwo>
 __device__ inline void key_grads(float* __restrict__ dk, float* __restrict__ dv, const float* __restrict__ k,
                                  const float* __restrict__ v, const int* __restrict__ lengths, char* __restrict__ ws,
-                                 const Shape& s, float scale, int parts) {
+                                 const Shape& s, float scale, int parts, unsigned block, char* rows_a, char* cols_a,
+                                 char* rows_b, char* cols_b, Probs* probs) {
   constexpr int kTile = kQueryTile<NB>, Waves = 8;
-  constexpr bool kTwo = NB > 2;  // two buffers
-  constexpr int kRows = 2 * kRowBytes<NB> + kTail, kCols = 2 * kColBytes<NB>;
-  __shared__ __attribute__((aligned(1024))) char rows_a[kRows], cols_a[kCols], rows_b[kTwo ? kRows : kPart], cols_b[kTwo ? kCols : kPart];
-  __shared__ float4 probs[4][4][64];  // [pair][registers 4 c .. 4 c + 3][lane]
+  constexpr int kCols = kGradCols<NB>;
   const GradSpace f = grad_space<NB>(ws, s);
   // The first keys are seen by the most queries: first.
   const unsigned inner = static_cast<unsigned>(s.b * s.hk) * parts;
-  const int kt = blockIdx.x / inner, part = blockIdx.x % inner % parts;
-  const int hk = blockIdx.x % inner / parts % s.hk, b = blockIdx.x % inner / parts / s.hk, group = s.hq / s.hk;
+  const int kt = block / inner, part = block % inner % parts;
+  const int hk = block % inner / parts % s.hk, b = block % inner / parts / s.hk, group = s.hq / s.hk;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, half = lane / 32;
   const int pair = wave % 4;
   const bool of_keys = wave >= 4;  // makes dk, from ds; the other dv, from p
@@ -1057,7 +1061,8 @@ __device__ inline void token(float* __restrict__ y, const float* __restrict__ q,
                              const float* __restrict__ v, float* __restrict__ stats, const int* __restrict__ lengths,
                              char* __restrict__ ws, const Shape& s, float scale, int splits, int per) {
   // blockIdx.x: (b, hk, 16 rows, split)
-  __shared__ float merged[4][16 * ND * 64];
+  constexpr int kRow = ND * 64 + 4;  // lanes of unlike rows at unlike banks
+  __shared__ __attribute__((aligned(16))) float merged[4][16 * kRow];
   __shared__ float ms[4][16], ls[4][16];
   const int group = s.hq / s.hk, tiles = (s.sq * group + 15) / 16;
   const int split = blockIdx.x % splits, tile = blockIdx.x / splits % tiles;
@@ -1158,7 +1163,7 @@ __device__ inline void token(float* __restrict__ y, const float* __restrict__ q,
   for (int c = 0; c < ND; c++)
 #pragma unroll
     for (int r = 0; r < 4; r++)
-      *reinterpret_cast<float4*>(&merged[wave][n * ND * 64 + 64 * c + 4 * (4 * quad + r)]) =
+      *reinterpret_cast<float4*>(&merged[wave][n * kRow + 64 * c + 4 * (4 * quad + r)]) =
           make_float4(o[c][0][r], o[c][1][r], o[c][2][r], o[c][3][r]);
   __syncthreads();
   const RowParts parts = row_parts(ws, s, splits);
@@ -1170,7 +1175,7 @@ __device__ inline void token(float* __restrict__ y, const float* __restrict__ q,
     for (int w = 0; w < 4; w++) {
       const float of = exp2f(ms[w][row] - top);
       sum += of * ls[w][row];
-      all += of * merged[w][row * ND * 64 + d];
+      all += of * merged[w][row * kRow + d];
     }
     const int iq = (first + row) / group, hq = hk * group + (first + row) % group;
     const size_t stat = (static_cast<size_t>(b) * s.hq + hq) * s.sq + iq;
@@ -1194,44 +1199,49 @@ __device__ inline void token(float* __restrict__ y, const float* __restrict__ q,
 
 }  // namespace
 
-#define FG_ATTENTION(NB)                                                                                              \
-  extern "C" __global__ void __launch_bounds__(256) fg_attention_pack_##NB(                                           \
-      float* y, const float* q, const float* k, const float* v, float* stats, const int* lengths, char* ws, int B,    \
-      int Sq, int Sk, int Hq, int Hk, int D, int causal, float scale, int splits, int per, unsigned, unsigned) {                          \
-    pack_keys<NB>(k, v, lengths, ws, B, Sk, Hk, D);                                                                   \
-  }                                                                                                                   \
-  extern "C" __global__ void __launch_bounds__(256, 2) fg_attention_tiles_##NB(                                       \
-      float* y, const float* q, const float* k, const float* v, float* stats, const int* lengths, char* ws, int B,    \
-      int Sq, int Sk, int Hq, int Hk, int D, int causal, float scale, int splits, int per, unsigned, unsigned) {                          \
-    forward_tiles<NB>(y, q, stats, lengths, ws, Shape{B, Sq, Sk, Hq, Hk, D, causal}, scale, splits);                  \
-  }                                                                                                                   \
-  extern "C" __global__ void __launch_bounds__(256) fg_attention_grad_pack_##NB(                                      \
-      float* dq, const float* q, const float* k, const float* v, const float* y, const float* g, const float* stats,  \
-      float* dk, float* dv, const int* lengths, char* ws, int parts, int q_parts, int B, int Sq, int Sk, int Hq, int Hk, int D, \
-      int causal, float scale) {                                                                                      \
-    pack_grad<NB>(q, k, v, y, g, stats, lengths, ws, Shape{B, Sq, Sk, Hq, Hk, D, causal});                            \
-  }                                                                                                                   \
-  extern "C" __global__ void __launch_bounds__(64 * kQueryGradWaves<NB>, 2) fg_attention_grad_q_##NB(                  \
-      float* dq, const float* q, const float* k, const float* v, const float* y, const float* g, const float* stats,  \
-      float* dk, float* dv, const int* lengths, char* ws, int parts, int q_parts, int B, int Sq, int Sk, int Hq, int Hk, int D, \
-      int causal, float scale) {                                                                                      \
-    query_grads<NB, kQueryGradWaves<NB>>(dq, q, g, stats, lengths, ws, Shape{B, Sq, Sk, Hq, Hk, D, causal}, scale, parts, q_parts);        \
-  }                                                                                                                   \
-  extern "C" __global__ void __launch_bounds__(512, (NB) < 3 ? 4 : 2) fg_attention_grad_kv_##NB(                                   \
-      float* dq, const float* q, const float* k, const float* v, const float* y, const float* g, const float* stats,  \
-      float* dk, float* dv, const int* lengths, char* ws, int parts, int q_parts, int B, int Sq, int Sk, int Hq, int Hk, int D, \
-      int causal, float scale) {                                                                                      \
-    key_grads<NB>(dk, dv, k, v, lengths, ws, Shape{B, Sq, Sk, Hq, Hk, D, causal}, scale, parts);                      \
-  }                                                                                                                   \
-  extern "C" __global__ void __launch_bounds__(256) fg_attention_grad_sum_##NB(                                       \
-      float* dq, const float* q, const float* k, const float* v, const float* y, const float* g, const float* stats,  \
-      float* dk, float* dv, const int* lengths, char* ws, int parts, int q_parts, int B, int Sq, int Sk, int Hq, int Hk, int D, \
-      int causal, float scale) {                                                                                      \
-    const Shape s{B, Sq, Sk, Hq, Hk, D, causal};                                                                      \
-    const GradSpace f = grad_space<NB>(ws, s);                                                                        \
-    const size_t n = static_cast<size_t>(B) * Sk * Hk * D, m = static_cast<size_t>(B) * Sq * Hq * D;                  \
-    if (parts > 1) sum_parts(dk, dv, f.parts, n, 2 * n, parts);                                                       \
-    if (q_parts > 1) sum_parts(dq, dq, f.parts + key_parts(s, parts), m, m, q_parts);                                 \
+// Every launch of a call takes the call's arguments.
+#define FG_ARGS                                                                                                  \
+  float *y, const float *q, const float *k, const float *v, float *stats, const int *lengths, char *ws, int B,   \
+      int Sq, int Sk, int Hq, int Hk, int D, int causal, float scale, int splits, int per, unsigned tiles_lo,    \
+      unsigned tiles_hi
+#define FG_GRAD_ARGS                                                                                             \
+  float *dq, const float *q, const float *k, const float *v, const float *y, const float *g, const float *stats, \
+      float *dk, float *dv, const int *lengths, char *ws, int parts, int q_parts, int B, int Sq, int Sk, int Hq, \
+      int Hk, int D, int causal, float scale
+#define FG_SHAPE \
+  Shape { B, Sq, Sk, Hq, Hk, D, causal }
+
+#define FG_ATTENTION(NB)                                                                                         \
+  extern "C" __global__ void __launch_bounds__(256) fg_attention_pack_##NB(FG_ARGS) {                            \
+    pack_keys<NB>(k, v, lengths, ws, B, Sk, Hk, D);                                                              \
+  }                                                                                                              \
+  extern "C" __global__ void __launch_bounds__(256, 2) fg_attention_tiles_##NB(FG_ARGS) {                        \
+    forward_tiles<NB>(y, q, stats, lengths, ws, FG_SHAPE, scale, splits);                                        \
+  }                                                                                                              \
+  extern "C" __global__ void __launch_bounds__(256) fg_attention_grad_pack_##NB(FG_GRAD_ARGS) {                  \
+    pack_grad<NB>(q, k, v, y, g, stats, lengths, ws, FG_SHAPE);                                                  \
+  }                                                                                                              \
+  extern "C" __global__ void __launch_bounds__(64 * kQueryGradWaves<NB>, 2)                                      \
+      fg_attention_grad_q_##NB(FG_GRAD_ARGS) {                                                                   \
+    __shared__ __attribute__((aligned(1024))) char even[kKeyTile<NB>], odd[kKeyTile<NB>];                        \
+    query_grads<NB, kQueryGradWaves<NB>>(dq, q, g, stats, lengths, ws, FG_SHAPE, scale, parts, q_parts,          \
+                                         blockIdx.x, even, odd);                                                 \
+  }                                                                                                              \
+  extern "C" __global__ void __launch_bounds__(512, (NB) < 3 ? 4 : 2) fg_attention_grad_kv_##NB(FG_GRAD_ARGS) {  \
+    constexpr bool kTwo = (NB) > 2;                                                                              \
+    __shared__ __attribute__((aligned(1024))) char rows_a[kGradRows<NB>], cols_a[kGradCols<NB>];                 \
+    __shared__ __attribute__((aligned(1024))) char rows_b[kTwo ? kGradRows<NB> : kPart];                         \
+    __shared__ __attribute__((aligned(1024))) char cols_b[kTwo ? kGradCols<NB> : kPart];                         \
+    __shared__ Probs probs[4];                                                                                   \
+    key_grads<NB, kTwo>(dk, dv, k, v, lengths, ws, FG_SHAPE, scale, parts, blockIdx.x, rows_a, cols_a, rows_b,   \
+                        cols_b, probs);                                                                          \
+  }                                                                                                              \
+  extern "C" __global__ void __launch_bounds__(256) fg_attention_grad_sum_##NB(FG_GRAD_ARGS) {                   \
+    const Shape s = FG_SHAPE;                                                                                    \
+    const GradSpace f = grad_space<NB>(ws, s);                                                                   \
+    const size_t n = static_cast<size_t>(B) * Sk * Hk * D, m = static_cast<size_t>(B) * Sq * Hq * D;             \
+    if (parts > 1) sum_parts(dk, dv, f.parts, n, 2 * n, parts);                                                  \
+    if (q_parts > 1) sum_parts(dq, dq, f.parts + key_parts(s, parts), m, m, q_parts);                            \
   }
 
 FG_ATTENTION(1)
@@ -1239,11 +1249,31 @@ FG_ATTENTION(2)
 FG_ATTENTION(3)
 FG_ATTENTION(4)
 
-#define FG_ATTENTION_TOKEN(ND, NAME, ALIGNED)                                                                         \
-  extern "C" __global__ void __launch_bounds__(256, 2) fg_attention_token_##NAME(                                     \
-      float* y, const float* q, const float* k, const float* v, float* stats, const int* lengths, char* ws, int B,    \
-      int Sq, int Sk, int Hq, int Hk, int D, int causal, float scale, int splits, int per, unsigned, unsigned) {                          \
-    token<ND, ALIGNED>(y, q, k, v, stats, lengths, ws, Shape{B, Sq, Sk, Hq, Hk, D, causal}, scale, splits, per);      \
+// Both gradients of a call whose workgroups all fit the chip at once: those of
+// dk and dv, then those of dq, of whose eight waves the ones that have no part
+// in a tile leave at once. They share the two buffers.
+#define FG_ATTENTION_GRADS(NB)                                                                                   \
+  extern "C" __global__ void __launch_bounds__(512, 2) fg_attention_grads_##NB(FG_GRAD_ARGS) {                   \
+    constexpr int kOdd = kGradCols<NB> + 4 * static_cast<int>(sizeof(Probs)), kTile = kKeyTile<NB>;              \
+    __shared__ __attribute__((aligned(1024))) char even[kTile > kGradRows<NB> ? kTile : kGradRows<NB>];          \
+    __shared__ __attribute__((aligned(1024))) char odd[kTile > kOdd ? kTile : kOdd];                             \
+    const unsigned key_blocks = static_cast<unsigned>(B * Hk) * parts * ((Sk + 127) / 128);                      \
+    if (blockIdx.x < key_blocks) {                                                                               \
+      key_grads<NB, false>(dk, dv, k, v, lengths, ws, FG_SHAPE, scale, parts, blockIdx.x, even, odd, even, odd,  \
+                           reinterpret_cast<Probs*>(odd + kGradCols<NB>));                                       \
+    } else if (threadIdx.x < 64 * kQueryGradWaves<NB>) {                                                         \
+      query_grads<NB, kQueryGradWaves<NB>>(dq, q, g, stats, lengths, ws, FG_SHAPE, scale, parts, q_parts,        \
+                                           blockIdx.x - key_blocks, even, odd);                                  \
+    }                                                                                                            \
+  }
+FG_ATTENTION_GRADS(1)
+FG_ATTENTION_GRADS(2)
+FG_ATTENTION_GRADS(3)
+FG_ATTENTION_GRADS(4)
+
+#define FG_ATTENTION_TOKEN(ND, NAME, ALIGNED)                                                                    \
+  extern "C" __global__ void __launch_bounds__(256, 2) fg_attention_token_##NAME(FG_ARGS) {                      \
+    token<ND, ALIGNED>(y, q, k, v, stats, lengths, ws, FG_SHAPE, scale, splits, per);                            \
   }
 FG_ATTENTION_TOKEN(1, 1, true)
 FG_ATTENTION_TOKEN(2, 2, true)
@@ -1252,13 +1282,9 @@ FG_ATTENTION_TOKEN(2, 2_any, false)
 
 // The parts begin `tiles` bytes into the workspace (given as two words). W
 // columns a thread.
-#define FG_ATTENTION_JOIN(W)                                                                                          \
-  extern "C" __global__ void __launch_bounds__(256) fg_attention_join_##W(                                            \
-      float* y, const float* q, const float* k, const float* v, float* stats, const int* lengths, char* ws, int B,    \
-      int Sq, int Sk, int Hq, int Hk, int D, int causal, float scale, int splits, int per, unsigned tiles_lo,         \
-      unsigned tiles_hi) {                                                                                            \
-    join_parts<W>(y, stats, ws + (static_cast<size_t>(tiles_hi) << 32 | tiles_lo),                                    \
-                  Shape{B, Sq, Sk, Hq, Hk, D, causal}, splits);                                                       \
+#define FG_ATTENTION_JOIN(W)                                                                                     \
+  extern "C" __global__ void __launch_bounds__(256) fg_attention_join_##W(FG_ARGS) {                             \
+    join_parts<W>(y, stats, ws + (static_cast<size_t>(tiles_hi) << 32 | tiles_lo), FG_SHAPE, splits);            \
   }
 FG_ATTENTION_JOIN(1)
 FG_ATTENTION_JOIN(4)

@@ -286,16 +286,29 @@ RenderedKernel render_attention(const UOp& call, bool grad) {
     const int64_t waves = nb < 4 ? 4 : 8;  // kQueryGradWaves
     const int64_t k_tiles = batch * kv_heads * ((sk + 127) / 128), q_tiles = batch * heads * ((sq + 32 * waves - 1) / (32 * waves));
     const double unit_us = 0.9 * static_cast<double>(nb);
-    const int64_t parts = count_parts(k_tiles, q_blocks * group, causal, nb < 3 ? 512 : 256, unit_us, 8.0 * static_cast<double>(all_k), 6, 16);
-    const int64_t q_parts = count_parts(q_tiles, k_blocks, causal, nb < 4 ? 512 : 256, unit_us, 4.0 * static_cast<double>(all_q),
+    // Where all workgroups of both kinds find room on the chip, one launch has
+    // them, and each kind's share of the room goes by its tiles. Two launches
+    // against one, us a pass with its forward, causal: 8 x 8 heads of 64 over
+    // 256 tokens 78 and 59, 4 x 16 of 32 over 512 96 and 77, 8 of 128 over 1024
+    // 141 and 120; 256 workgroups over a chip of 256 units are one each.
+    const int64_t all_slots = nb == 1 ? 512 : 256;
+    const bool together = k_tiles + q_tiles <= all_slots;
+    const int64_t k_slots = together ? all_slots * k_tiles / (k_tiles + q_tiles) : nb < 3 ? 512 : 256;
+    const int64_t q_slots = together ? all_slots - k_slots : nb < 4 ? 512 : 256;
+    const int64_t parts = count_parts(k_tiles, q_blocks * group, causal, k_slots, unit_us, 8.0 * static_cast<double>(all_k), 6, 16);
+    const int64_t q_parts = count_parts(q_tiles, k_blocks, causal, q_slots, unit_us, 4.0 * static_cast<double>(all_q),
                                         parts > 1 ? 0 : 6, 16);
     const uint64_t summed = std::max(parts > 1 ? 2 * all_k : 0, q_parts > 1 ? all_q : 0);
     rk.workspace_bytes = nk * static_cast<uint64_t>(nb * 12288 + 1024) + nq * static_cast<uint64_t>(nb * 16384 + 1024) +
                          (nk + 3) / 4 * 16 + (parts > 1 ? 8 * all_k * static_cast<uint64_t>(parts) : 0) +
                          (q_parts > 1 ? 4 * all_q * static_cast<uint64_t>(q_parts) : 0);
-    rk.launches = {launch("fg_attention_grad_pack" + nbs, 2 * (nk + nq), 256, "attention"),
-                   launch("fg_attention_grad_kv" + nbs, static_cast<uint64_t>(k_tiles * parts), 512, "attention"),
-                   launch("fg_attention_grad_q" + nbs, static_cast<uint64_t>(q_tiles * q_parts), static_cast<unsigned>(64 * waves), "attention")};
+    rk.launches = {launch("fg_attention_grad_pack" + nbs, 2 * (nk + nq), 256, "attention")};
+    if (together) {
+      rk.launches.push_back(launch("fg_attention_grads" + nbs, static_cast<uint64_t>(k_tiles * parts + q_tiles * q_parts), 512, "attention"));
+    } else {
+      rk.launches.push_back(launch("fg_attention_grad_kv" + nbs, static_cast<uint64_t>(k_tiles * parts), 512, "attention"));
+      rk.launches.push_back(launch("fg_attention_grad_q" + nbs, static_cast<uint64_t>(q_tiles * q_parts), static_cast<unsigned>(64 * waves), "attention"));
+    }
     if (summed) rk.launches.push_back(launch("fg_attention_grad_sum" + nbs, std::min<uint64_t>((summed + 255) / 256, 8192), 256, "attention"));
     const int dk = lengths ? 8 : 7;
     for (int i = 0; i < 7; i++) rk.call_args.push_back(CallArg::slot(i));

@@ -181,6 +181,33 @@ def test_attention_and_its_gradients(fg, hip, shape):
     assert np.array_equal(y, got["y"])  # the same without the gradients
 
 
+# Calls of over 2^30 operations, whose forward pass cuts its operands, and of
+# more workgroups than one launch of both gradients takes.
+LARGE_SHAPES = [
+    (17, 130, 130, 32, 16, 32, True, None),
+    (8, 200, 260, 16, 8, 50, True, [260, 0, 1, 32, 33, 128, 129, 255]),
+    (4, 300, 300, 16, 16, 80, False, [300, 299, 96, 7]),
+    (4, 300, 270, 16, 4, 128, True, None),  # the first 30 queries see nothing
+    (4, 130, 257, 32, 32, 127, False, None),
+    (1, 64, 5000, 16, 16, 64, False, None),  # keys of a query tile in parts
+    (1, 520, 300, 64, 1, 64, True, [290]),  # queries of a key tile in parts
+    (1, 600, 600, 24, 24, 100, True, None),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", LARGE_SHAPES, ids=lambda s: "x".join(str(x) for x in s[:6]))
+def test_larger_attention_and_its_gradients(fg, hip, shape):
+    batch, sq, sk, heads, kv_heads, dim, causal, lengths = shape
+    q, k, v, g = attention_inputs(4, batch, sq, sk, heads, kv_heads, dim)
+    lengths = None if lengths is None else np.asarray(lengths, np.int32)
+    kw = dict(batch=batch, heads=heads, kv_heads=kv_heads, causal=causal, lengths=lengths)
+    want = attention_ref.attention(q, k, v, g=g, **kw)
+    got = run_attention(fg, q, k, v, g, **kw)
+    for name in ("y", "dq", "dk", "dv"):
+        check(name, got[name], *want[name])
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("sq", [1, 90])
 def test_hidden_keys_may_hold_anything(fg, hip, sq):
@@ -223,6 +250,47 @@ def test_attention_with_sharp_rows_and_values_of_unlike_sizes(fg, hip):
     got = run_attention(fg, q, k, v, g, **kw)
     for name in want:
         check(name, got[name], *want[name])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [1e-18, 1e15])
+def test_larger_attention_of_small_and_large_values(fg, hip, size):
+    q, k, v, g = attention_inputs(12, 1, 300, 520, 32, 32, 64)
+    q, k, v, g = (q / np.float32(size)), (k * np.float32(size)), v * np.float32(size), g / np.float32(size)
+    kw = dict(batch=1, heads=32, kv_heads=32, causal=True)
+    want = attention_ref.attention(q, k, v, g=g, **kw)
+    got = run_attention(fg, q, k, v, g, **kw)
+    for name in want:
+        check(name, got[name], *want[name])
+
+
+@pytest.mark.gpu
+def test_larger_attention_with_sharp_rows_and_values_of_unlike_sizes(fg, hip):
+    q, k, v, g = attention_inputs(13, 1, 300, 520, 32, 8, 64, spread=40.0)
+    v *= (2.0 ** np.linspace(-20, 20, 520))[:, None].astype(np.float32)
+    v[64:128] = 0
+    g *= (2.0 ** np.linspace(10, -10, 300))[:, None].astype(np.float32)
+    kw = dict(batch=1, heads=32, kv_heads=8, scale=0.3)
+    want = attention_ref.attention(q, k, v, g=g, **kw)
+    got = run_attention(fg, q, k, v, g, **kw)
+    for name in want:
+        check(name, got[name], *want[name])
+
+
+@pytest.mark.gpu
+def test_larger_attention_with_anything_behind_the_lengths(fg, hip):
+    q, k, v, g = attention_inputs(14, 2, 150, 520, 32, 16, 64)
+    kw = dict(batch=2, heads=32, kv_heads=16, lengths=np.array([500, 3], np.int32))
+    clean = run_attention(fg, q, k, v, g, **kw)
+    junk = np.array([np.nan, np.inf, -np.inf, np.finfo(np.float32).max, np.finfo(np.float32).min], np.float32)
+    for x in (k, v):
+        for rows in (slice(500, 520), slice(523, 1040)):
+            x[rows] = junk[np.arange(x[rows].size) % 5].reshape(x[rows].shape)
+    dirty = run_attention(fg, q, k, v, g, **kw)
+    for n in clean:
+        assert np.array_equal(clean[n], dirty[n]), n
+    for n in ("dk", "dv"):
+        assert not dirty[n][500:520].any() and not dirty[n][523:].any()
 
 
 @pytest.mark.gpu
