@@ -139,24 +139,17 @@ UOp output_of(const UOp& storage, const UOp& call) {
 // params: tokens, heads, dim, bits of eps, bits of base. Sources: x, weight,
 // positions; of the gradient also g and dweight's storage.
 
-// A head in vectors of `vec` on `lanes` lanes, `turns` vectors of each half a
-// lane (kernels/norm_rotate.hip).
+// A head in vectors of `vec` of each half on `lanes` lanes
+// (kernels/norm_rotate.hip).
 struct RowSplit {
-  int vec, lanes, turns;
-  std::string suffix() const {
-    return "_" + std::to_string(vec) + "_" + std::to_string(lanes) + "_" + std::to_string(turns);
-  }
+  int vec, lanes;
+  std::string suffix() const { return "_" + std::to_string(vec) + "_" + std::to_string(lanes); }
 };
 
 RowSplit row_split(int64_t dim) {
   const int64_t half = dim / 2;
-  RowSplit r;
-  r.vec = half % 4 == 0 ? 4 : half % 2 == 0 ? 2 : 1;  // halves of a row start on a vector's alignment
-  const int64_t vectors = half / r.vec;
-  r.lanes = 8;
-  while (r.lanes < vectors && r.lanes < 64) r.lanes *= 2;
-  r.turns = 1;
-  while (r.lanes * r.turns < vectors) r.turns *= 2;
+  RowSplit r{half < 4 ? 1 : 4, 8};
+  while (r.lanes * r.vec < half) r.lanes *= 2;
   return r;
 }
 

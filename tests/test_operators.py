@@ -380,6 +380,24 @@ def test_norm_rotate_and_its_gradients(fg, hip, tokens, heads, dim, far):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dim", [4, 10, 14, 66, 130, 250, 258, 386])
+def test_norm_rotate_of_halves_that_end_within_a_vector(fg, hip, dim):
+    r = seeded(1000 + dim)
+    tokens, heads = 37, 3
+    x = (3 * r.standard_normal((tokens, heads * dim))).astype(np.float32)
+    w = (1 + 0.3 * r.standard_normal(dim)).astype(np.float32)
+    g = r.standard_normal(x.shape).astype(np.float32)
+    pos = r.integers(0, 4096, tokens).astype(np.int32)
+    want = norm_rotate_ref(x, w, pos, heads, 1e-6, 10000.0, g)
+    tx, tw = new(fg, x, True), new(fg, w, True)
+    y = tx.norm_rotate(tw, new(fg, pos), heads)
+    dx, dw = y.mul(new(fg, g)).sum([0, 1]).gradient([tx, tw])
+    fg.Tensor.realize_many([y, dx, dw])
+    for name, t in (("y", y), ("dx", dx), ("dweight", dw)):
+        check(name, t.numpy(), *want[name])
+
+
+@pytest.mark.gpu
 def test_norm_rotate_of_zero_rows_and_gradients_against_differences(fg, hip):
     r = seeded(2)
     x = r.standard_normal((6, 32)).astype(np.float32)
