@@ -162,20 +162,36 @@ __device__ inline float block_max(float x, float* shared) {
   return x;
 }
 
+// Four numbers of a row, which starts on any float: odd head sizes take the
+// same 16-byte loads and stores. (As single floats a token over 8 x 8192 keys of
+// 63 columns took 80 us, of 127 251; so 29 and 77, as 64 and 128 do.)
+typedef float floatu4 __attribute__((ext_vector_type(4), aligned(4)));
+
+// Columns c .. c + 3 of a row of D >= 4, or the row's last four where those would
+// pass its end; `turn_to` then moves them to their places.
+__device__ inline float4 load4_within(const float* row, int c, int D) {
+  const floatu4 v = *reinterpret_cast<const floatu4*>(row + min(c, D - 4));
+  return make_float4(v[0], v[1], v[2], v[3]);
+}
+
+// The columns past the end are then any of the row's own.
+__device__ inline float4 turn_to(float4 v, int c, int D) {
+  const int by = c - (D - 4);
+  if (by > 0 && by & 1) v = make_float4(v.y, v.z, v.w, v.w);
+  if (by > 0 && by & 2) v = make_float4(v.z, v.w, v.w, v.w);
+  return v;
+}
+
 // Columns c .. c + 3 of a row of D, 0 past its end. Every lane loads from the
 // row whatever it keeps: loads under conditions would wait for one another.
 __device__ inline float4 load4(const float* row, int c, int D) {
   float4 v;
-  if (D % 4 == 0) {
-    v = *reinterpret_cast<const float4*>(row + (c < D ? c : 0));
-    if (c >= D) v = make_float4(0.f, 0.f, 0.f, 0.f);
-  } else {
-    v = make_float4(row[c < D ? c : 0], row[c + 1 < D ? c + 1 : 0], row[c + 2 < D ? c + 2 : 0], row[c + 3 < D ? c + 3 : 0]);
-    if (c >= D) v.x = 0.f;
-    if (c + 1 >= D) v.y = 0.f;
-    if (c + 2 >= D) v.z = 0.f;
-    if (c + 3 >= D) v.w = 0.f;
-  }
+  if (D >= 4) v = turn_to(load4_within(row, c, D), c, D);
+  else v = make_float4(row[c < D ? c : 0], row[c + 1 < D ? c + 1 : 0], row[c + 2 < D ? c + 2 : 0], 0.f);
+  if (c >= D) v.x = 0.f;
+  if (c + 1 >= D) v.y = 0.f;
+  if (c + 2 >= D) v.z = 0.f;
+  if (c + 3 >= D) v.w = 0.f;
   return v;
 }
 
@@ -349,8 +365,8 @@ __device__ inline void store_columns(float* row, int n, int half, int D, const f
     float v[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) v[i] = ldexpf(o[4 * g + i] * scale, e);
-    if (D % 4 == 0) {
-      if (c < D) *reinterpret_cast<float4*>(row + c) = make_float4(v[0], v[1], v[2], v[3]);
+    if (c + 3 < D) {
+      *reinterpret_cast<floatu4*>(row + c) = floatu4{v[0], v[1], v[2], v[3]};
     } else {
 #pragma unroll
       for (int i = 0; i < 4; i++)
@@ -378,14 +394,16 @@ __device__ inline RowParts row_parts(char* at, const Shape& s, int splits) {
 }
 
 // The parts joined: a thread per row and W columns, N parts at a time in flight.
-// The stats are written by the row's first column.
+// Where a row is no whole number of W its last thread takes its last W columns,
+// some of them a second time. The stats are written by the row's first column.
 template <int N, int W>
 __device__ inline void join_columns(float* __restrict__ y, float* __restrict__ stats, const RowParts& parts, const Shape& s,
                                     int splits) {
-  const size_t e = (static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x) * W;
-  if (e >= parts.rows * s.d) return;
-  const size_t row = e / s.d;
-  const int d = e % s.d;
+  const size_t e = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int columns = (s.d + W - 1) / W;
+  if (e >= parts.rows * columns) return;
+  const size_t row = e / columns;
+  const int d = min(static_cast<int>(e % columns) * W, s.d - W);
   float top = -INFINITY, sum = 0.f, all[W] = {};
   for (int p0 = 0; p0 < splits; p0 += N) {
     float2 ml[N];
@@ -395,11 +413,9 @@ __device__ inline void join_columns(float* __restrict__ y, float* __restrict__ s
       const size_t part = min(p0 + n, splits - 1) * parts.rows + row;
       ml[n] = *reinterpret_cast<const float2*>(parts.ml + 2 * part);
       if constexpr (W == 4) {
-        const float4 v = *reinterpret_cast<const float4*>(parts.o + part * s.d + d);
-        o[n][0] = v.x;
-        o[n][1] = v.y;
-        o[n][2] = v.z;
-        o[n][3] = v.w;
+        const floatu4 v = *reinterpret_cast<const floatu4*>(parts.o + part * s.d + d);
+#pragma unroll
+        for (int w = 0; w < 4; w++) o[n][w] = v[w];
       } else {
         o[n][0] = parts.o[part * s.d + d];
       }
@@ -431,7 +447,7 @@ __device__ inline void join_columns(float* __restrict__ y, float* __restrict__ s
   float* out = y + (b * s.sq + i) * s.hq * s.d + static_cast<size_t>(h) * s.d + d;
 #pragma unroll
   for (int w = 0; w < W; w++) all[w] *= inv;
-  if constexpr (W == 4) *reinterpret_cast<float4*>(out) = make_float4(all[0], all[1], all[2], all[3]);
+  if constexpr (W == 4) *reinterpret_cast<floatu4*>(out) = floatu4{all[0], all[1], all[2], all[3]};
   else *out = all[0];
   if (d == 0) {
     stats[row] = top == -INFINITY ? 0.f : top;
@@ -1047,16 +1063,12 @@ __device__ inline void sum_parts(float* __restrict__ first, float* __restrict__ 
 // l's result rows, 4 (l / 16) + r: P is used where it is. Keys are split over
 // workgroups until these fill the chip, and joined by a second launch.
 
-// Columns c .. c + 3 of a row, any of the row's own where they lie past its end
-// (they meet zeros of the query, or are not kept).
-template <bool Aligned>
-__device__ inline float4 load4_any(const float* row, int c, int D) {
-  if constexpr (Aligned) return *reinterpret_cast<const float4*>(row + (c < D ? c : 0));
-  return make_float4(row[min(c, D - 1)], row[min(c + 1, D - 1)], row[min(c + 2, D - 1)], row[min(c + 3, D - 1)]);
-}
+// Whether rows are whole vectors of four columns, end within one, or are less
+// than one.
+enum class Columns { Whole, Odd, Few };
 
-// ND: columns in units of 64. Aligned: a row starts on 16 bytes.
-template <int ND, bool Aligned>
+// ND: columns in units of 64.
+template <int ND, Columns C>
 __device__ inline void token(float* __restrict__ y, const float* __restrict__ q, const float* __restrict__ k,
                              const float* __restrict__ v, float* __restrict__ stats, const int* __restrict__ lengths,
                              char* __restrict__ ws, const Shape& s, float scale, int splits, int per) {
@@ -1083,6 +1095,16 @@ __device__ inline void token(float* __restrict__ y, const float* __restrict__ q,
   const float factor = scale * kLog2e;
   float m = -INFINITY, l = 0.f;
   floatx4 o[ND][4] = {};
+  // Columns c .. c + 3 of a row, any of the row's own where they lie past its end
+  // (they meet zeros of the query, or are not kept).
+  auto columns = [&](const float* row, int c) {
+    if constexpr (C == Columns::Few) return make_float4(row[min(c, s.d - 1)], row[min(c + 1, s.d - 1)], row[min(c + 2, s.d - 1)], 0.f);
+    else return load4_within(row, c, s.d);
+  };
+  auto placed = [&](const float4& x, int c) {
+    if constexpr (C == Columns::Odd) return turn_to(x, c, s.d);
+    else return x;
+  };
   // 16 keys and values, loaded while the wave works on the 16 before.
   struct Keys {
     float4 kv[ND * 4], vv[4][ND];
@@ -1090,24 +1112,23 @@ __device__ inline void token(float* __restrict__ y, const float* __restrict__ q,
   auto load = [&](Keys& to, int j0) {
     const float* k_row = k + head + min(j0 + n, end - 1) * stride;
 #pragma unroll
-    for (int t = 0; t < ND * 4; t++) to.kv[t] = load4_any<Aligned>(k_row, 16 * t + 4 * quad, s.d);
+    for (int t = 0; t < ND * 4; t++) to.kv[t] = columns(k_row, 16 * t + 4 * quad);
 #pragma unroll
     for (int r = 0; r < 4; r++)
 #pragma unroll
       for (int c = 0; c < ND; c++)
-        to.vv[r][c] = load4_any<Aligned>(v + head + min(j0 + 4 * quad + r, end - 1) * stride, 64 * c + 4 * n, s.d);
+        to.vv[r][c] = columns(v + head + min(j0 + 4 * quad + r, end - 1) * stride, 64 * c + 4 * n);
   };
   auto step = [&](const Keys& now, Keys& next, int j0) {
     load(next, j0 + 64);
-    const auto& kv = now.kv;
-    const auto& vv = now.vv;
     floatx4 x = {};
 #pragma unroll
     for (int t = 0; t < ND * 4; t++) {
-      x = __builtin_amdgcn_mfma_f32_16x16x4f32(kv[t].x, qv[t].x, x, 0, 0, 0);
-      x = __builtin_amdgcn_mfma_f32_16x16x4f32(kv[t].y, qv[t].y, x, 0, 0, 0);
-      x = __builtin_amdgcn_mfma_f32_16x16x4f32(kv[t].z, qv[t].z, x, 0, 0, 0);
-      x = __builtin_amdgcn_mfma_f32_16x16x4f32(kv[t].w, qv[t].w, x, 0, 0, 0);
+      const float4 kv = placed(now.kv[t], 16 * t + 4 * quad);
+      x = __builtin_amdgcn_mfma_f32_16x16x4f32(kv.x, qv[t].x, x, 0, 0, 0);
+      x = __builtin_amdgcn_mfma_f32_16x16x4f32(kv.y, qv[t].y, x, 0, 0, 0);
+      x = __builtin_amdgcn_mfma_f32_16x16x4f32(kv.z, qv[t].z, x, 0, 0, 0);
+      x = __builtin_amdgcn_mfma_f32_16x16x4f32(kv.w, qv[t].w, x, 0, 0, 0);
     }
     float top = -INFINITY;
 #pragma unroll
@@ -1137,10 +1158,11 @@ __device__ inline void token(float* __restrict__ y, const float* __restrict__ q,
     for (int r = 0; r < 4; r++)
 #pragma unroll
       for (int c = 0; c < ND; c++) {
-        o[c][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[r][c].x, x[r], o[c][0], 0, 0, 0);
-        o[c][1] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[r][c].y, x[r], o[c][1], 0, 0, 0);
-        o[c][2] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[r][c].z, x[r], o[c][2], 0, 0, 0);
-        o[c][3] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[r][c].w, x[r], o[c][3], 0, 0, 0);
+        const float4 vv = placed(now.vv[r][c], 64 * c + 4 * n);
+        o[c][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv.x, x[r], o[c][0], 0, 0, 0);
+        o[c][1] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv.y, x[r], o[c][1], 0, 0, 0);
+        o[c][2] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv.z, x[r], o[c][2], 0, 0, 0);
+        o[c][3] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv.w, x[r], o[c][3], 0, 0, 0);
       }
   };
   if (begin + wave * 16 < end) {
@@ -1271,14 +1293,15 @@ FG_ATTENTION_GRADS(2)
 FG_ATTENTION_GRADS(3)
 FG_ATTENTION_GRADS(4)
 
-#define FG_ATTENTION_TOKEN(ND, NAME, ALIGNED)                                                                    \
+#define FG_ATTENTION_TOKEN(ND, NAME, COLUMNS)                                                                    \
   extern "C" __global__ void __launch_bounds__(256, 2) fg_attention_token_##NAME(FG_ARGS) {                      \
-    token<ND, ALIGNED>(y, q, k, v, stats, lengths, ws, FG_SHAPE, scale, splits, per);                            \
+    token<ND, Columns::COLUMNS>(y, q, k, v, stats, lengths, ws, FG_SHAPE, scale, splits, per);                   \
   }
-FG_ATTENTION_TOKEN(1, 1, true)
-FG_ATTENTION_TOKEN(2, 2, true)
-FG_ATTENTION_TOKEN(1, 1_any, false)
-FG_ATTENTION_TOKEN(2, 2_any, false)
+FG_ATTENTION_TOKEN(1, 1, Whole)
+FG_ATTENTION_TOKEN(2, 2, Whole)
+FG_ATTENTION_TOKEN(1, 1_odd, Odd)
+FG_ATTENTION_TOKEN(2, 2_odd, Odd)
+FG_ATTENTION_TOKEN(1, 1_few, Few)
 
 // The parts begin `tiles` bytes into the workspace (given as two words). W
 // columns a thread.

@@ -250,7 +250,7 @@ RenderedKernel render_attention(const UOp& call, bool grad) {
       splits = std::max<int64_t>(1, std::min({(1024 + pairs - 1) / pairs, sk / 256, int64_t(64)}));
       per = ((sk + splits - 1) / splits + 63) / 64 * 64;
       splits = (sk + per - 1) / per;
-      rk.launches = {launch(std::string("fg_attention_token_") + (dim <= 64 ? "1" : "2") + (dim % 4 ? "_any" : ""), static_cast<uint64_t>(pairs * splits), 256, "attention")};
+      rk.launches = {launch(std::string("fg_attention_token_") + (dim <= 64 ? "1" : "2") + (dim < 4 ? "_few" : dim % 4 ? "_odd" : ""), static_cast<uint64_t>(pairs * splits), 256, "attention")};
     } else {
       const int64_t tiles = batch * heads * ((sq + 127) / 128);
       const uint64_t blocks = static_cast<uint64_t>(batch * kv_heads * k_blocks);
@@ -263,8 +263,8 @@ RenderedKernel render_attention(const UOp& call, bool grad) {
     if (splits > 1) {
       const uint64_t all_rows = static_cast<uint64_t>(batch * heads * sq);
       rk.workspace_bytes = tile_bytes + static_cast<uint64_t>(splits) * (4 * all_q + 8 * all_rows);
-      const uint64_t columns = dim % 4 ? 1 : 4;  // a thread's
-      rk.launches.push_back(launch("fg_attention_join_" + std::to_string(columns), (all_q / columns + 255) / 256, 256, "attention"));
+      const uint64_t columns = dim < 4 ? 1 : 4;  // a thread's
+      rk.launches.push_back(launch("fg_attention_join_" + std::to_string(columns), (all_rows * ((static_cast<uint64_t>(dim) + columns - 1) / columns) + 255) / 256, 256, "attention"));
     }
     rk.call_args = {CallArg::slot(0), CallArg::slot(1), CallArg::slot(2), CallArg::slot(3), CallArg::slot(lengths ? 5 : 4),
                     lengths ? CallArg::slot(4) : CallArg::null(), CallArg::workspace()};

@@ -209,6 +209,18 @@ def test_larger_attention_and_its_gradients(fg, hip, shape):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dim", [1, 2, 3, 5, 6, 7, 61, 62, 66, 125, 126])
+@pytest.mark.parametrize("sq,sk", [(2, 1200), (40, 45)])
+def test_attention_of_heads_that_end_within_a_vector(fg, hip, sq, sk, dim):
+    q, k, v, g = attention_inputs(100 + dim, 2, sq, sk, 6, 3, dim)
+    kw = dict(batch=2, heads=6, kv_heads=3, causal=True, lengths=np.array([sk - 3, 31], np.int32))
+    want = attention_ref.attention(q, k, v, g=g, **kw)
+    got = run_attention(fg, q, k, v, g, **kw)
+    for name in ("y", "dq", "dk", "dv"):
+        check(name, got[name], *want[name])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("sq", [1, 90])
 def test_hidden_keys_may_hold_anything(fg, hip, sq):
     q, k, v, g = attention_inputs(5, 2, sq, 90, 4, 2, 48)
