@@ -201,28 +201,57 @@ RenderedKernel render_norm_rotate(const UOp& call, bool grad) {
 // and 21.8; 16 heads of 128 over 512 tokens (2^31) 47 and 34.
 constexpr double kSmallAttention = 1073741824.0;
 
-// In how many parts each of `tiles` workgroups' rows takes its `units` blocks of
-// 32. A launch fills `slots` with a workgroup each and costs its longest row of
-// them: rounds times (units + about 4 for a workgroup's start and end) units of
-// `unit_us`. With `causal` the longest is twice the average, and long ones start
-// first: the launch takes as long as the longest, or as all of them together.
-// Parts cost `extra_us` (a launch that joins them) and their `bytes`, written
-// and read at 5 TB/s.
-int64_t count_parts(int64_t tiles, int64_t units, bool causal, int64_t slots, double unit_us, double bytes, double extra_us,
-                    int64_t most) {
-  int64_t best = 1;
-  double least = 0;
-  for (int64_t parts = 1; parts <= std::min(units, most); parts++) {
-    const double each = static_cast<double>(units) / static_cast<double>(parts) + 4;
-    const double rounds = static_cast<double>((tiles * parts + slots - 1) / slots);
-    double cost = rounds * each;
-    if (causal) cost = std::max(each, 0.5 * static_cast<double>(tiles * units) / static_cast<double>(slots) + 4 * rounds);
-    cost *= unit_us;
-    if (parts > 1) cost += 2 * bytes * static_cast<double>(parts) / 5e6 + extra_us;
-    if (parts == 1 || cost < least) {
-      best = parts;
-      least = cost;
-    }
+// Units of attention's launches: 32 query rows by 32 keys of every wave of a
+// workgroup. A unit's us, measured where workgroups fill the chip (16 heads,
+// 2048 queries, 1024 to 4096 keys): two of them a compute unit, or one where
+// their tiles leave no room for another. A workgroup with a compute unit to
+// itself takes less than each of two do, by these factors.
+constexpr double kForwardUnit[] = {1.2, 1.7, 2.3, 3.0}, kKeyUnit[] = {2.7, 3.6, 2.8, 3.3}, kQueryUnit[] = {1.4, 2.3, 3.3, 4.0};
+constexpr double kForwardAlone = 0.75, kGradAlone = 0.72;
+constexpr int64_t kUnits = 256;   // compute units
+constexpr double kSumLaunch = 8;  // us of a launch that joins parts, beside its bytes
+
+// One kind of workgroups of a launch: `tiles` of them, each over `units` blocks
+// of 32 (with `causal` the longest; the average is half of that), or in parts of
+// them, which cost `bytes` each, written and read at 5 TB/s. A workgroup's start
+// and end cost as much as some units: `ends_alone` where every one has a compute
+// unit to itself, 4 otherwise.
+struct Work {
+  int64_t tiles, units;
+  bool causal;
+  double us, alone_us, ends_alone, bytes;
+  double joined(int64_t parts) const { return parts > 1 ? 2 * bytes * static_cast<double>(parts) / 5e6 : 0; }
+};
+
+// A launch's us with `slots` workgroups on the chip at once and the work cut into
+// these parts: as long as its longest workgroup, or as all of them together, of
+// which the last end half of one after the others (with `causal` they are
+// short). Equal workgroups take whole rounds.
+double launch_us(const Work* work, const int64_t* parts, int kinds, int64_t slots) {
+  int64_t n = 0;
+  for (int i = 0; i < kinds; i++) n += work[i].tiles * parts[i];
+  double longest = 0, sum = 0, last = 0;
+  for (int i = 0; i < kinds; i++) {
+    const Work& w = work[i];
+    const double p = static_cast<double>(parts[i]), units = static_cast<double>(w.units) / p, ends = n <= kUnits ? w.ends_alone : 4;
+    longest = std::max(longest, (units + ends) * (n <= kUnits || kinds > 1 ? w.alone_us : w.us));
+    sum += static_cast<double>(w.tiles) * p * (units * (w.causal ? 0.5 : 1) + ends) * w.us;
+    last = w.causal || n <= slots ? 0 : (units + ends) * w.us;
+  }
+  if (kinds == 1 && !work[0].causal) return static_cast<double>((n + slots - 1) / slots) * longest;
+  return std::max(longest, sum / static_cast<double>(slots) + 0.5 * last);
+}
+
+struct Split {
+  int64_t parts;
+  double us;
+};
+
+Split count_parts(const Work& work, int64_t slots, double join_us, int64_t most) {
+  Split best{1, 0};
+  for (int64_t parts = 1; parts <= std::min(work.units, most); parts++) {
+    const double us = launch_us(&work, &parts, 1, slots) + (parts > 1 ? work.joined(parts) + join_us : 0);
+    if (parts == 1 || us < best.us) best = {parts, us};
   }
   return best;
 }
@@ -254,7 +283,8 @@ RenderedKernel render_attention(const UOp& call, bool grad) {
     } else {
       const int64_t tiles = batch * heads * ((sq + 127) / 128);
       const uint64_t blocks = static_cast<uint64_t>(batch * kv_heads * k_blocks);
-      splits = count_parts(tiles, k_blocks, causal, 512, 0.5 + 0.4 * static_cast<double>(nb), 4.0 * static_cast<double>(all_q), 6, 64);
+      splits = count_parts({tiles, k_blocks, causal, kForwardUnit[nb - 1], kForwardAlone * kForwardUnit[nb - 1], 4, 4.0 * static_cast<double>(all_q)}, 2 * kUnits,
+                           kSumLaunch, std::clamp<int64_t>(2 * kUnits / tiles, 1, 64)).parts;
       tile_bytes = blocks * static_cast<uint64_t>(nb * 8192 + 1024);
       rk.launches = {launch("fg_attention_pack_" + std::to_string(nb), 2 * blocks, 256, "attention"),
                      launch("fg_attention_tiles_" + std::to_string(nb), static_cast<uint64_t>(tiles * splits), 256, "attention")};
@@ -278,19 +308,40 @@ RenderedKernel render_attention(const UOp& call, bool grad) {
     const uint64_t nk = static_cast<uint64_t>(batch * kv_heads * k_blocks), nq = static_cast<uint64_t>(batch * heads * q_blocks);
     const int64_t waves = nb < 4 ? 4 : 8;  // kQueryGradWaves
     const int64_t k_tiles = batch * kv_heads * ((sk + 127) / 128), q_tiles = batch * heads * ((sq + 32 * waves - 1) / (32 * waves));
-    const double unit_us = 0.9 * static_cast<double>(nb);
-    // Where all workgroups of both kinds find room on the chip, one launch has
-    // them, and each kind's share of the room goes by its tiles. Two launches
-    // against one, us a pass with its forward, causal: 8 x 8 heads of 64 over
-    // 256 tokens 78 and 59, 4 x 16 of 32 over 512 96 and 77, 8 of 128 over 1024
-    // 141 and 120; 256 workgroups over a chip of 256 units are one each.
-    const int64_t all_slots = nb == 1 ? 512 : 256;
-    const bool together = k_tiles + q_tiles <= all_slots;
-    const int64_t k_slots = together ? all_slots * k_tiles / (k_tiles + q_tiles) : nb < 3 ? 512 : 256;
-    const int64_t q_slots = together ? all_slots - k_slots : nb < 4 ? 512 : 256;
-    const int64_t parts = count_parts(k_tiles, q_blocks * group, causal, k_slots, unit_us, 8.0 * static_cast<double>(all_k), 6, 16);
-    const int64_t q_parts = count_parts(q_tiles, k_blocks, causal, q_slots, unit_us, 4.0 * static_cast<double>(all_q),
-                                        parts > 1 ? 0 : 6, 16);
+    // Two workgroups a compute unit where they fit.
+    const int64_t k_slots = nb < 3 ? 2 * kUnits : kUnits, q_slots = nb < 4 ? 2 * kUnits : kUnits;
+    const double k_us = kKeyUnit[nb - 1], q_us = kQueryUnit[nb - 1], k_alone = (nb < 3 ? kGradAlone : 1) * k_us, q_alone = (nb < 4 ? kGradAlone : 1) * q_us;
+    Work work[2] = {{k_tiles, q_blocks * group, causal, k_us, k_alone, 2, 8.0 * static_cast<double>(all_k)},
+                    {q_tiles, k_blocks, causal, q_us, q_alone, 2, 4.0 * static_cast<double>(all_q)}};
+    const Split k_split = count_parts(work[0], k_slots, kSumLaunch, 16);
+    const Split q_split = count_parts(work[1], q_slots, k_split.parts > 1 ? 0 : kSumLaunch, 16);
+    int64_t parts = k_split.parts, q_parts = q_split.parts;
+    // One launch can have both kinds where all their tiles find room (two
+    // workgroups a compute unit of one column group, one of more), and has them
+    // where it takes less than two. Two launches against one, us a pass with its
+    // forward, causal: 8 x 8 heads of 64 over 256 tokens 78 and 59, 4 x 16 of 32
+    // over 512 96 and 77, 8 of 128 over 1024 141 and 120.
+    bool together = false;
+    const int64_t slots = nb == 1 ? 2 * kUnits : kUnits;
+    if (k_tiles + q_tiles <= slots) {
+      if (nb > 1) {
+        work[0].us = k_alone;
+        work[1].us = q_alone;
+      }
+      double least = k_split.us + q_split.us;
+      for (int64_t both[2] = {1, 1}; both[0] <= std::min<int64_t>(16, work[0].units); both[0]++)
+        for (both[1] = 1; both[1] <= std::min<int64_t>(16, work[1].units); both[1]++) {
+          // The kind that comes first leaves room for the other's longest.
+          if (k_tiles * both[0] + q_tiles * both[1] > slots && 8 * k_tiles * both[0] > 7 * slots) continue;
+          const double us = launch_us(work, both, 2, slots) + work[0].joined(both[0]) + work[1].joined(both[1]) +
+                            (both[0] > 1 || both[1] > 1 ? kSumLaunch : 0);
+          if (us >= least) continue;
+          together = true;
+          least = us;
+          parts = both[0];
+          q_parts = both[1];
+        }
+    }
     const uint64_t summed = std::max(parts > 1 ? 2 * all_k : 0, q_parts > 1 ? all_q : 0);
     rk.workspace_bytes = nk * static_cast<uint64_t>(nb * 12288 + 1024) + nq * static_cast<uint64_t>(nb * 16384 + 1024) +
                          (nk + 3) / 4 * 16 + (parts > 1 ? 8 * all_k * static_cast<uint64_t>(parts) : 0) +
