@@ -876,6 +876,45 @@ __device__ inline void query_grads(float* __restrict__ dq, const float* __restri
 // the other is read, so that two workgroups fit a compute unit and
 // cover each other's waits. More groups leave room for one workgroup, with two
 // buffers of whole tiles.
+// Which 128 keys, key head, batch and part of the queries a workgroup takes. The
+// first keys, seen by the most queries, come first. With lengths, tiles that are
+// no sequence's come last, so that those with work to do are spread evenly over
+// the chiplets and take no more rounds than they must: 5 x 12 heads of 80 over
+// up to 777 keys, where 240 of 420 tiles had work, took 141 us with the tiles in
+// one order for all lengths, and 90 so. Lane l counts the tiles of sequence l, for as many
+// sequences as there are lanes.
+__device__ inline void key_tile(const Shape& s, const int* lengths, int parts, unsigned block, int* kt, int* part, int* hk,
+                                int* b) {
+  const unsigned each = static_cast<unsigned>(s.hk) * parts;
+  unsigned rest = block % each;
+  if (lengths && s.b <= 64) {
+    const int lane = threadIdx.x % 64, tiles = (s.sk + 127) / 128;
+    const int mine = lane < s.b ? (key_count(s, lengths, lane) + 127) / 128 : 0;
+    const unsigned long long every = ~0ull >> (64 - s.b);
+    for (int t = 0; t < 2 * tiles; t++) {
+      const bool empty = t >= tiles;
+      const int at = empty ? t - tiles : t;
+      const unsigned long long with = __ballot(mine > at);
+      unsigned long long left = empty ? every & ~with : with;
+      const unsigned count = __popcll(left) * each;
+      if (block >= count) {
+        block -= count;
+        continue;
+      }
+      for (unsigned n = block / each; n > 0; n--) left &= left - 1;
+      *kt = at;
+      *b = __ffsll(left) - 1;
+      rest = block % each;
+      break;
+    }
+  } else {
+    *kt = block / (each * s.b);
+    *b = block / each % s.b;
+  }
+  *part = rest % parts;
+  *hk = rest / parts;
+}
+
 template <int NB>
 constexpr int kGradRows = 2 * kRowBytes<NB> + kTail;
 template <int NB>
@@ -890,10 +929,9 @@ __device__ inline void key_grads(float* __restrict__ dk, float* __restrict__ dv,
   constexpr int kTile = kQueryTile<NB>, Waves = 8;
   constexpr int kCols = kGradCols<NB>;
   const GradSpace f = grad_space<NB>(ws, s);
-  // The first keys are seen by the most queries: first.
-  const unsigned inner = static_cast<unsigned>(s.b * s.hk) * parts;
-  const int kt = block / inner, part = block % inner % parts;
-  const int hk = block % inner / parts % s.hk, b = block % inner / parts / s.hk, group = s.hq / s.hk;
+  const int group = s.hq / s.hk;
+  int kt, part, hk, b;
+  key_tile(s, lengths, parts, block, &kt, &part, &hk, &b);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, half = lane / 32;
   const int pair = wave % 4;
   const bool of_keys = wave >= 4;  // makes dk, from ds; the other dv, from p

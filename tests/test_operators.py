@@ -209,6 +209,18 @@ def test_larger_attention_and_its_gradients(fg, hip, shape):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("batch", [63, 64, 65, 130])
+def test_attention_of_many_short_sequences(fg, hip, batch):
+    q, k, v, g = attention_inputs(15, batch, 5, 300, 2, 1, 16)
+    lengths = seeded(batch).integers(0, 301, batch).astype(np.int32)
+    kw = dict(batch=batch, heads=2, kv_heads=1, lengths=lengths)
+    want = attention_ref.attention(q, k, v, g=g, **kw)
+    got = run_attention(fg, q, k, v, g, **kw)
+    for name in ("y", "dq", "dk", "dv"):
+        check(name, got[name], *want[name])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dim", [1, 2, 3, 5, 6, 7, 61, 62, 66, 125, 126])
 @pytest.mark.parametrize("sq,sk", [(2, 1200), (40, 45)])
 def test_attention_of_heads_that_end_within_a_vector(fg, hip, sq, sk, dim):
