@@ -946,17 +946,20 @@ __device__ inline void key_grads(float* __restrict__ dk, float* __restrict__ dv,
   const int units = kt * 128 < keys ? max(0, f.q_blocks - q_first) * group : 0;
 
   const size_t q_head = (static_cast<size_t>(b) * s.hq + static_cast<size_t>(hk) * group) * f.q_blocks;
-  auto unit_tile = [&](int u) {
-    return f.q_tiles + (q_head + static_cast<size_t>(u % group) * f.q_blocks + (f.q_blocks - 1 - u / group)) * kTile;
+  // Unit u is query block q_blocks - 1 - u / group of head u % group.
+  int back = part / group, of_group = part % group;
+  const int back_step = parts / group, head_step = parts % group;
+  auto unit_tile = [&](int back, int of_group) {
+    return f.q_tiles + (q_head + static_cast<size_t>(of_group) * f.q_blocks + (f.q_blocks - 1 - back)) * kTile;
   };
-  auto copy_rows = [&](int u, char* to) {
-    copy_tile<2 * kRowBytes<NB>, Waves>(unit_tile(u), to);
-    copy_tile<kTail, Waves>(unit_tile(u) + kTile - kTail, to + 2 * kRowBytes<NB>);
+  auto copy_rows = [&](const char* tile, char* to) {
+    copy_tile<2 * kRowBytes<NB>, Waves>(tile, to);
+    copy_tile<kTail, Waves>(tile + kTile - kTail, to + 2 * kRowBytes<NB>);
   };
-  auto copy_cols = [&](int u, char* to) { copy_tile<kCols, Waves>(unit_tile(u) + 2 * kRowBytes<NB>, to); };
+  auto copy_cols = [&](const char* tile, char* to) { copy_tile<kCols, Waves>(tile + 2 * kRowBytes<NB>, to); };
   if (part < units) {
-    copy_rows(part, rows_a);
-    copy_cols(part, cols_a);
+    copy_rows(unit_tile(back, of_group), rows_a);
+    copy_cols(unit_tile(back, of_group), cols_a);
   }
 
   const size_t at = (static_cast<size_t>(b) * s.sk + min(j, s.sk - 1)) * s.hk * s.d + static_cast<size_t>(hk) * s.d;
@@ -969,11 +972,18 @@ __device__ inline void key_grads(float* __restrict__ dk, float* __restrict__ dv,
   tile_barrier();
   auto step = [&](const char* rows, const char* cols, char* next_rows, char* next_cols, int u) {
     const bool more = u + parts < units;
-    if (kTwo && more) {
-      copy_rows(u + parts, next_rows);
-      copy_cols(u + parts, next_cols);
+    const int q0 = (f.q_blocks - 1 - back) * kBlock;
+    back += back_step;
+    of_group += head_step;
+    if (of_group >= group) {
+      of_group -= group;
+      back++;
     }
-    const int q0 = (f.q_blocks - 1 - u / group) * kBlock;
+    const char* next = unit_tile(back, of_group);
+    if (kTwo && more) {
+      copy_rows(next, next_rows);
+      copy_cols(next, next_cols);
+    }
     // Whether any of the block's queries sees any of the wave's keys.
     const bool any = first < keys && (!s.causal || first <= q0 + kBlock - 1 + offset);
     const char* t = rows + lane * 16 + (of_keys ? kRowBytes<NB> : 0);
@@ -1020,7 +1030,7 @@ __device__ inline void key_grads(float* __restrict__ dk, float* __restrict__ dv,
       asm volatile("" ::: "memory");
     } else {
       tile_barrier();
-      if (more) copy_rows(u + parts, next_rows);
+      if (more) copy_rows(next, next_rows);
     }
     if (any) {
       if (of_keys) {
@@ -1056,7 +1066,7 @@ __device__ inline void key_grads(float* __restrict__ dk, float* __restrict__ dv,
       }
     }
     tile_barrier();
-    if (!kTwo && more) copy_cols(u + parts, next_cols);
+    if (!kTwo && more) copy_cols(next, next_cols);
   };
   if constexpr (kTwo) {
     for (int u = part; u < units; u += 2 * parts) {
