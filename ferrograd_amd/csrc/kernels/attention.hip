@@ -393,17 +393,36 @@ __device__ inline RowParts row_parts(char* at, const Shape& s, int splits) {
   return p;
 }
 
+// Keys a part where all sequences' keys go into about `units` parts of the same
+// length, no more than `splits` of a sequence: where lengths differ a short
+// sequence takes few workgroups, and all of them end together. For up to 64
+// sequences; lane l has sequence l's keys.
+__device__ inline unsigned keys_a_part(const Shape& s, int keys, int splits, int units) {
+  unsigned all = (keys + 63u) / 64;  // in 64 keys, of which a wave takes 16
+  for (int d = 32; d > 0; d /= 2) all += __shfl_xor(all, d);
+  const unsigned longest = (s.sk + 63u) / 64;
+  return __builtin_amdgcn_readfirstlane(64 * max(max((all + units - 1) / units, (longest + splits - 1) / splits), 2u));
+}
+
 // The parts joined: a thread per row and W columns, N parts at a time in flight.
 // Where a row is no whole number of W its last thread takes its last W columns,
 // some of them a second time. The stats are written by the row's first column.
-template <int N, int W>
-__device__ inline void join_columns(float* __restrict__ y, float* __restrict__ stats, const RowParts& parts, const Shape& s,
-                                    int splits) {
+template <int N, int W, bool OneLength>
+__device__ inline void join_columns(float* __restrict__ y, float* __restrict__ stats, const int* __restrict__ lengths,
+                                    const RowParts& parts, const Shape& s, int splits, int units) {
+  int each = 0;
+  if (OneLength) {
+    const int lane = threadIdx.x % 64;
+    each = keys_a_part(s, lane < s.b ? key_count(s, lengths, lane) : 0, splits, units);
+  }
   const size_t e = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
   const int columns = (s.d + W - 1) / W;
   if (e >= parts.rows * columns) return;
   const size_t row = e / columns;
   const int d = min(static_cast<int>(e % columns) * W, s.d - W);
+  const int i = row % s.sq, h = row / s.sq % s.hq;
+  const size_t b = row / s.sq / s.hq;
+  if (OneLength) splits = (static_cast<unsigned>(key_count(s, lengths, b)) + each - 1) / each;
   float top = -INFINITY, sum = 0.f, all[W] = {};
   for (int p0 = 0; p0 < splits; p0 += N) {
     float2 ml[N];
@@ -442,8 +461,6 @@ __device__ inline void join_columns(float* __restrict__ y, float* __restrict__ s
       }
   }
   const float inv = sum > 0.f ? 1.f / sum : 0.f;
-  const int i = row % s.sq, h = row / s.sq % s.hq;
-  const size_t b = row / s.sq / s.hq;
   float* out = y + (b * s.sq + i) * s.hq * s.d + static_cast<size_t>(h) * s.d + d;
 #pragma unroll
   for (int w = 0; w < W; w++) all[w] *= inv;
@@ -455,12 +472,13 @@ __device__ inline void join_columns(float* __restrict__ y, float* __restrict__ s
   }
 }
 
-template <int W>
-__device__ inline void join_parts(float* __restrict__ y, float* __restrict__ stats, char* __restrict__ at, const Shape& s,
-                                  int splits) {
+template <int W, bool OneLength>
+__device__ inline void join_parts(float* __restrict__ y, float* __restrict__ stats, const int* __restrict__ lengths,
+                                  char* __restrict__ at, const Shape& s, int splits, int units) {
   const RowParts parts = row_parts(at, s, splits);
-  if (splits <= 4) join_columns<4, W>(y, stats, parts, s, splits);
-  else join_columns<16, W>(y, stats, parts, s, splits);
+  if constexpr (OneLength) join_columns<16, W, true>(y, stats, lengths, parts, s, splits, units);
+  else if (splits <= 4) join_columns<4, W, false>(y, stats, lengths, parts, s, splits, units);
+  else join_columns<16, W, false>(y, stats, lengths, parts, s, splits, units);
 }
 
 // Which `rows` queries, head, batch and part of the keys a workgroup takes. The
@@ -482,6 +500,14 @@ __device__ inline void query_tile(const Shape& s, int rows, int splits, unsigned
 // S^T = K Q^T, so that a lane holds 16 scores of one query: the row's maximum
 // and sum cost one exchange between the wave's halves, and the probabilities
 // are in registers what O^T += V^T P^T takes as its second operand.
+//
+// Bound by the matrix cores at the clock the card's power leaves them: 4096
+// causal tokens, 32 heads of 128 over 8: 421 us, 980 TFLOP/s of float16 products
+// (327 of the float32 ones they stand for; float32's own matrix rate is 151 and a
+// library's large float16 product reaches 1076), cores busy 53% of the time at
+// 1.9 GHz. Four waves a workgroup and two workgroups a compute unit, so that one
+// has the cores while the other makes its probabilities; keys are cut by a launch
+// of their own (14 us), once for all the query tiles that read them.
 template <int NB>
 __device__ inline void forward_tiles(float* __restrict__ y, const float* __restrict__ q, float* __restrict__ stats,
                                      const int* __restrict__ lengths, char* __restrict__ ws, const Shape& s, float scale,
@@ -675,7 +701,9 @@ __device__ inline int norm_exponent(float squares, int e) {
 __device__ inline float power(int a) { return ldexpf(1.f, a); }
 
 // Keys, values, queries and gradients cut once per call, one workgroup per
-// block and matrix.
+// block and matrix. Bound by memory, 4.0 TB/s: 16 heads of 128 over 8192 tokens
+// 138 us for 237 MB read and 320 written (queries and gradients by rows for the
+// scores, and by columns for dk and dv).
 template <int NB>
 __device__ inline void pack_grad(const float* __restrict__ q, const float* __restrict__ k, const float* __restrict__ v,
                                  const float* __restrict__ y, const float* __restrict__ g,
@@ -758,7 +786,9 @@ __device__ inline int clamp_power(int a) { return min(max(a, -120), 120); }
 // dq. A workgroup: 32 queries of one head a wave, over all keys; scores and
 // their gradients transposed as in the forward pass. Tiles of four column
 // groups leave room for one workgroup a compute unit: eight waves share them,
-// so that each matrix core has two waves in turn.
+// so that each matrix core has two waves in turn. Bound like the forward pass: 16
+// heads of 128 over 8192 causal tokens 1044 us, 1185 TFLOP/s of float16 products,
+// cores busy 60% of the time at 1.9 GHz.
 template <int NB>
 constexpr int kQueryGradWaves = NB < 4 ? 4 : 8;
 
@@ -870,6 +900,12 @@ __device__ inline void query_grads(float* __restrict__ dq, const float* __restri
 // core to itself, waiting while it does anything else), at the price of the
 // probabilities' way through LDS. Scores are not transposed here: a lane holds
 // 16 queries of one key, which is what dv^T += G^T P and dk^T += Q^T dS take.
+//
+// 16 heads of 128 over 4 key heads and 8192 causal tokens: 1737 us, 950 TFLOP/s of
+// float16 products, cores busy 45% of the time at 2.0 GHz: what the power leaves
+// and the two barriers of a step, at which the pair waits for its probabilities
+// and all for the next tile. (With one wave for both, and four for dq, forward and
+// gradients took 4.21 ms instead of 3.65.)
 //
 // The rows of a tile are read before the probabilities' barrier, its columns
 // after it. Up to two column groups they have one buffer each, refilled while
@@ -1110,6 +1146,13 @@ __device__ inline void sum_parts(float* __restrict__ first, float* __restrict__ 
 // of 4 columns, and O^T += V^T P with the four terms of a product taken as lane
 // l's result rows, 4 (l / 16) + r: P is used where it is. Keys are split over
 // workgroups until these fill the chip, and joined by a second launch.
+//
+// Bound by memory: one token of 32 heads of 128 over 8 key heads and 8 x 8192 keys
+// reads 537 MB in 89 us, 6.0 TB/s (268 MB, at lengths of half that on the average,
+// in 66 to 73 us), and joins in 5. A wave loads its next 16 keys and values while
+// it works on the last (126 us without, for the shorter). Small calls are bound by
+// their few dependent steps: 2 x 4 heads of 32 over 33 tokens 6 us, 8 x 8 of 64
+// over 256 causal tokens 22.
 
 // Whether rows are whole vectors of four columns, end within one, or are less
 // than one.
@@ -1119,19 +1162,37 @@ enum class Columns { Whole, Odd, Few };
 template <int ND, Columns C>
 __device__ inline void token(float* __restrict__ y, const float* __restrict__ q, const float* __restrict__ k,
                              const float* __restrict__ v, float* __restrict__ stats, const int* __restrict__ lengths,
-                             char* __restrict__ ws, const Shape& s, float scale, int splits, int per) {
-  // blockIdx.x: (b, hk, 16 rows, split)
+                             char* __restrict__ ws, const Shape& s, float scale, int splits, int units) {
   constexpr int kRow = ND * 64 + 4;  // lanes of unlike rows at unlike banks
   __shared__ __attribute__((aligned(16))) float merged[4][16 * kRow];
   __shared__ float ms[4][16], ls[4][16];
   const int group = s.hq / s.hk, tiles = (s.sq * group + 15) / 16;
-  const int split = blockIdx.x % splits, tile = blockIdx.x / splits % tiles;
-  const int hk = blockIdx.x / splits / tiles % s.hk, b = blockIdx.x / splits / tiles / s.hk;
+  // The workgroup's 16 rows, key head, sequence and part of its keys.
+  int split = blockIdx.x % splits, tile = blockIdx.x / splits % tiles;
+  int hk = blockIdx.x / splits / tiles % s.hk, b = blockIdx.x / splits / tiles / s.hk;
+  unsigned each = 0;
+  if (units > 0) {
+    const unsigned inner = s.hk * tiles;
+    const int unit = blockIdx.x / inner, l = threadIdx.x % 64, mine = l < s.b ? key_count(s, lengths, l) : 0;
+    each = keys_a_part(s, mine, splits, units);
+    int ends = (mine + each - 1) / each;  // of the parts up to and of sequence l
+    for (int d = 1; d < 64; d *= 2) {
+      const int before = __shfl_up(ends, d);
+      if (l >= d) ends += before;
+    }
+    b = __popcll(__ballot(l < s.b && ends <= unit));
+    if (b == s.b) return;  // there are fewer parts
+    split = unit - (b > 0 ? __builtin_amdgcn_readlane(ends, max(b - 1, 0)) : 0);
+    tile = blockIdx.x % inner % tiles;
+    hk = blockIdx.x % inner / tiles;
+  }
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
   const int n = lane % 16, quad = lane / 16, first = tile * 16, rows = min(16, s.sq * group - first);
   // Row n of the products: query (first + n) / group, head hk * group + (first + n) % group.
   const int row = first + min(n, rows - 1), i = row / group, h = hk * group + row % group;
-  const int keys = key_count(s, lengths, b), begin = split * per;
+  const int keys = key_count(s, lengths, b);
+  const int per = units > 0 ? each : ((static_cast<unsigned>(keys) + splits - 1) / splits + 63) / 64 * 64;
+  const int begin = split * per;
   const int end = min(visible(s, keys, (first + rows - 1) / group), begin + per);
   const int seen = n < rows ? min(end, visible(s, keys, i)) : 0;
   const float* q_row = q + (static_cast<size_t>(b) * s.sq + i) * s.hq * s.d + static_cast<size_t>(h) * s.d;
@@ -1272,7 +1333,7 @@ __device__ inline void token(float* __restrict__ y, const float* __restrict__ q,
 // Every launch of a call takes the call's arguments.
 #define FG_ARGS                                                                                                  \
   float *y, const float *q, const float *k, const float *v, float *stats, const int *lengths, char *ws, int B,   \
-      int Sq, int Sk, int Hq, int Hk, int D, int causal, float scale, int splits, int per, unsigned tiles_lo,    \
+      int Sq, int Sk, int Hq, int Hk, int D, int causal, float scale, int splits, int units, unsigned tiles_lo,    \
       unsigned tiles_hi
 #define FG_GRAD_ARGS                                                                                             \
   float *dq, const float *q, const float *k, const float *v, const float *y, const float *g, const float *stats, \
@@ -1346,7 +1407,7 @@ FG_ATTENTION_GRADS(4)
 
 #define FG_ATTENTION_TOKEN(ND, NAME, COLUMNS)                                                                    \
   extern "C" __global__ void __launch_bounds__(256, 2) fg_attention_token_##NAME(FG_ARGS) {                      \
-    token<ND, Columns::COLUMNS>(y, q, k, v, stats, lengths, ws, FG_SHAPE, scale, splits, per);                   \
+    token<ND, Columns::COLUMNS>(y, q, k, v, stats, lengths, ws, FG_SHAPE, scale, splits, units);                   \
   }
 FG_ATTENTION_TOKEN(1, 1, Whole)
 FG_ATTENTION_TOKEN(2, 2, Whole)
@@ -1356,9 +1417,12 @@ FG_ATTENTION_TOKEN(1, 1_few, Few)
 
 // The parts begin `tiles` bytes into the workspace (given as two words). W
 // columns a thread.
-#define FG_ATTENTION_JOIN(W)                                                                                     \
-  extern "C" __global__ void __launch_bounds__(256) fg_attention_join_##W(FG_ARGS) {                             \
-    join_parts<W>(y, stats, ws + (static_cast<size_t>(tiles_hi) << 32 | tiles_lo), FG_SHAPE, splits);            \
+#define FG_ATTENTION_JOIN(W, NAME, ONE_LENGTH)                                                                   \
+  extern "C" __global__ void __launch_bounds__(256) fg_attention_join_##NAME(FG_ARGS) {                          \
+    join_parts<W, ONE_LENGTH>(y, stats, lengths, ws + (static_cast<size_t>(tiles_hi) << 32 | tiles_lo),          \
+                              FG_SHAPE, splits, units);                                                          \
   }
-FG_ATTENTION_JOIN(1)
-FG_ATTENTION_JOIN(4)
+FG_ATTENTION_JOIN(1, 1, false)
+FG_ATTENTION_JOIN(4, 4, false)
+FG_ATTENTION_JOIN(1, 1_even, true)
+FG_ATTENTION_JOIN(4, 4_even, true)

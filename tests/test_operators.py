@@ -221,6 +221,19 @@ def test_attention_of_many_short_sequences(fg, hip, batch):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("sq", [1, 3])
+@pytest.mark.parametrize("dim", [3, 30, 128])
+@pytest.mark.parametrize("lengths", [[0, 2500, 7, 1300, 0, 128, 129, 2499, 1, 0], [0] * 10, [2500] * 10, [0] * 9 + [2500],
+                                     [64, 0, 0, 0, 0, 0, 0, 0, 0, 0]], ids=["mixed", "none", "all", "last", "first"])
+def test_tokens_of_sequences_of_unlike_lengths(fg, hip, lengths, dim, sq):
+    q, k, v, _ = attention_inputs(16, 10, sq, 2500, 12, 6, dim)
+    lengths = np.asarray(lengths, np.int32)
+    kw = dict(batch=10, heads=12, kv_heads=6, causal=sq > 1, lengths=lengths)
+    want = attention_ref.attention(q, k, v, **kw)
+    check("y", run_attention(fg, q, k, v, None, **kw)["y"], *want["y"])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dim", [1, 2, 3, 5, 6, 7, 61, 62, 66, 125, 126])
 @pytest.mark.parametrize("sq,sk", [(2, 1200), (40, 45)])
 def test_attention_of_heads_that_end_within_a_vector(fg, hip, sq, sk, dim):
