@@ -1148,11 +1148,10 @@ __device__ inline void sum_parts(float* __restrict__ first, float* __restrict__ 
 // workgroups until these fill the chip, and joined by a second launch.
 //
 // Bound by memory: one token of 32 heads of 128 over 8 key heads and 8 x 8192 keys
-// reads 537 MB in 89 us, 6.0 TB/s (268 MB, at lengths of half that on the average,
-// in 66 to 73 us), and joins in 5. A wave loads its next 16 keys and values while
-// it works on the last (126 us without, for the shorter). Small calls are bound by
-// their few dependent steps: 2 x 4 heads of 32 over 33 tokens 6 us, 8 x 8 of 64
-// over 256 causal tokens 22.
+// reads 537 MB in 94 us, 5.7 TB/s, and with lengths of half that on the average 268
+// MB in 46 us, 5.9 TB/s; the join takes 5. A wave loads its next 16 keys and values
+// while it works on the last. Small calls are bound by their few dependent steps: 2
+// x 4 heads of 32 over 33 tokens 6 us, 8 x 8 of 64 over 256 causal tokens 22.
 
 // Whether rows are whole vectors of four columns, end within one, or are less
 // than one.
@@ -1380,8 +1379,8 @@ FG_ATTENTION(2)
 FG_ATTENTION(3)
 FG_ATTENTION(4)
 
-// Both gradients of a call whose tiles all fit the chip at once: the workgroups
-// of dk and dv, then those of dq, of whose eight waves the ones that have no part
+// Both gradients of a call of few tiles in one launch: the workgroups of dk and
+// dv, then those of dq, of whose eight waves the ones that have no part
 // in a tile leave at once. In this order the units that take two workgroups have
 // one of each kind (with the kinds in turn, 16 heads of 32 over 2048 tokens took
 // 229 us with their forward pass instead of 189). Both share the two buffers.

@@ -332,14 +332,16 @@ RenderedKernel render_attention(const UOp& call, bool grad) {
     const Split k_split = count_parts(work[0], k_slots, kSumLaunch, 16);
     const Split q_split = count_parts(work[1], q_slots, k_split.parts > 1 ? 0 : kSumLaunch, 16);
     int64_t parts = k_split.parts, q_parts = q_split.parts;
-    // One launch can have both kinds where all their tiles find room (two
-    // workgroups a compute unit of one column group, one of more), and has them
-    // where it takes less than two. Two launches against one, us a pass with its
-    // forward, causal: 8 x 8 heads of 64 over 256 tokens 78 and 59, 4 x 16 of 32
-    // over 512 96 and 77, 8 of 128 over 1024 141 and 120.
+    // One launch can have both kinds (two workgroups a compute unit of one column
+    // group, one of more), and has them where that takes less than two: their
+    // starts, ends and last rounds go together. Two launches against one, us a
+    // pass with its forward, causal: 8 x 8 heads of 64 over 256 tokens 78 and 59,
+    // 4 x 16 of 32 over 512 96 and 77, 8 of 128 over 1024 141 and 120, 2 x 12 of 64
+    // over 900 152 and 115. From twice as many tiles as the chip takes on, no call
+    // tried was better so.
     bool together = false;
     const int64_t slots = nb == 1 ? 2 * kUnits : kUnits;
-    if (k_tiles + q_tiles <= slots) {
+    if (k_tiles + q_tiles <= 2 * slots) {
       if (nb > 1) {
         work[0].us = k_alone;
         work[1].us = q_alone;
