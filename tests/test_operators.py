@@ -192,6 +192,9 @@ LARGE_SHAPES = [
     (1, 64, 5000, 16, 16, 64, False, None),  # keys of a query tile in parts
     (1, 520, 300, 64, 1, 64, True, [290]),  # queries of a key tile in parts
     (1, 600, 600, 24, 24, 100, True, None),
+    (16, 130, 130, 20, 20, 64, True, [130 - 8 * i for i in range(16)]),
+    (16, 130, 130, 20, 10, 96, False, None),
+    (16, 130, 260, 20, 10, 120, True, None),
 ]
 
 
