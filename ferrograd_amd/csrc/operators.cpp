@@ -194,13 +194,6 @@ RenderedKernel render_norm_rotate(const UOp& call, bool grad) {
 // lengths, bits of scale. Sources: q, k, v, [lengths], the stats' storage; of
 // the gradient: q, k, v, y, g, stats, [lengths], dk's and dv's storage.
 
-// Calls of up to this many operations (of both products, all keys counted) run
-// on the float32 path, in one launch. Float32 path against cut operands, us of
-// the kernels, 8 heads of 64, causal: batch 8 of 128 tokens (2^28) 10.5 and
-// 14.6 (in two launches), one of 512 (2^29) 16.8 and 20.2, 8 of 256 (2^30) 21.6
-// and 21.8; 16 heads of 128 over 512 tokens (2^31) 47 and 34.
-constexpr double kSmallAttention = 1073741824.0;
-
 // Units of attention's launches: 32 query rows by 32 keys of every wave of a
 // workgroup. A unit's us, measured where workgroups fill the chip (16 heads,
 // 2048 queries, 1024 to 4096 keys): two of them a compute unit, or one where
@@ -269,40 +262,52 @@ RenderedKernel render_attention(const UOp& call, bool grad) {
   const uint64_t all_q = static_cast<uint64_t>(batch * sq * heads * dim), all_k = static_cast<uint64_t>(batch * sk * kv_heads * dim);
   if (!grad) {
     rk.kind = "attention";
-    int64_t splits = 1, units = 0;
     uint64_t tile_bytes = 0;
-    const int64_t rows = sq * (heads / kv_heads);
-    if (rows <= 16 || 4.0 * static_cast<double>(all_q) * static_cast<double>(sk) <= kSmallAttention) {
-      // 16 rows a workgroup, and each sequence's keys in parts until there are
-      // 1024 workgroups, of at least 256 keys in the longest (four rounds of a
-      // workgroup's waves). Where these are more than 512 and sequences have
-      // lengths, parts are of one length for all sequences: 8 sequences of up to
-      // 8192 keys, 32 heads of 128 over 8, 50 to 62 us instead of 51 to 66 with
-      // their joins, 4 of up to 16384, 16 heads of 64 over 4, 18 instead of 21;
-      // 2 of up to 3000, 12 heads of 80, 19 instead of 16.
-      const int64_t each = kv_heads * ((rows + 15) / 16), pairs = batch * each;
-      uint64_t blocks;
-      splits = std::max<int64_t>(1, std::min({(1024 + pairs - 1) / pairs, sk / 256, int64_t(64)}));
-      if (lengths && batch > 1 && batch <= 64 && splits > 1 && pairs * splits > 512) {
-        units = (512 + each - 1) / each;
-        splits = std::min({units, sk / 128, int64_t(64)});
-        blocks = static_cast<uint64_t>(std::min(units + batch, splits * batch) * each);
-      } else {
-        const int64_t per = ((sk + splits - 1) / splits + 63) / 64 * 64;
-        splits = (sk + per - 1) / per;
-        blocks = static_cast<uint64_t>(pairs * splits);
-      }
-      rk.launches = {launch(std::string("fg_attention_token_") + (dim <= 64 ? "1" : "2") + (dim < 4 ? "_few" : dim % 4 ? "_odd" : ""), blocks, 256, "attention")};
+    // The float32 path: 16 rows a workgroup, and each sequence's keys in parts
+    // until there are 1024 workgroups, of at least 256 keys in the longest (four
+    // rounds of a workgroup's waves). Where these are more than 512 and sequences
+    // have lengths, parts are of one length for all sequences: 8 sequences of up
+    // to 8192 keys, 32 heads of 128 over 8, 50 to 62 us instead of 51 to 66 with
+    // their joins, 4 of up to 16384, 16 heads of 64 over 4, 18 instead of 21; 2 of
+    // up to 3000, 12 heads of 80, 19 instead of 16.
+    const int64_t rows = sq * (heads / kv_heads), each = kv_heads * ((rows + 15) / 16), pairs = batch * each;
+    int64_t splits = std::max<int64_t>(1, std::min({(1024 + pairs - 1) / pairs, sk / 256, int64_t(64)})), units = 0;
+    int64_t blocks, per = ((sk + splits - 1) / splits + 63) / 64 * 64;
+    if (lengths && batch > 1 && batch <= 64 && splits > 1 && pairs * splits > 512) {
+      units = (512 + each - 1) / each;
+      splits = std::min({units, sk / 128, int64_t(64)});
+      blocks = std::min(units + batch, splits * batch) * each;
     } else {
-      const int64_t tiles = batch * heads * ((sq + 127) / 128);
-      const uint64_t blocks = static_cast<uint64_t>(batch * kv_heads * k_blocks);
-      // Up to four parts are joined in one go; more only until they fill the
-      // chip (2 x 8 heads of 64 over 800 causal tokens: 22 us with its join in
-      // four parts, 26 in six).
-      const Work work{tiles, k_blocks, causal, kForwardUnit[nb - 1], kForwardAlone * kForwardUnit[nb - 1], 4, 4.0 * static_cast<double>(all_q)};
-      splits = count_parts(work, 2 * kUnits, kSumLaunch, std::clamp<int64_t>(2 * kUnits / tiles, 4, 64)).parts;
-      tile_bytes = blocks * static_cast<uint64_t>(nb * 8192 + 1024);
-      rk.launches = {launch("fg_attention_pack_" + std::to_string(nb), 2 * blocks, 256, "attention"),
+      splits = (sk + per - 1) / per;
+      blocks = pairs * splits;
+    }
+    // The other cuts its operands first. It is taken where that and its tiles take
+    // less than the float32 workgroups: as long as one of them alone, or as all of
+    // them, each a start and rounds of 64 keys. Float32 path against cut operands,
+    // us: 8 x 8 heads of 64 over 256 causal tokens 22 and 22, one sequence of 512
+    // 17 and 20, 2 x 4 heads of 128 over 500 20 and 32, 16 of 128 over 512 47 and
+    // 34, 4 x 50 of 128 over 10 and 99 tokens 29 and 20.
+    const bool narrow = dim <= 64;
+    const double rounds = static_cast<double>((per + 63) / 64) * (causal && splits == 1 ? 0.75 : 1);
+    const double token_us = std::max(narrow ? 4 + 1.5 * rounds : 5 + 2 * rounds,
+                                     static_cast<double>(blocks) / static_cast<double>(kUnits) * (narrow ? 1 + 1.2 * rounds : 3 + 2.7 * rounds)) +
+                            (splits > 1 ? 5 : 0);
+    // Up to four parts are joined in one go; more only until they fill the chip
+    // (2 x 8 heads of 64 over 800 causal tokens: 22 us with its join in four
+    // parts, 26 in six).
+    const int64_t tiles = batch * heads * ((sq + 127) / 128);
+    const Work work{tiles, k_blocks, causal, kForwardUnit[nb - 1], kForwardAlone * kForwardUnit[nb - 1], 4, 4.0 * static_cast<double>(all_q)};
+    const Split split = count_parts(work, 2 * kUnits, kSumLaunch, std::clamp<int64_t>(2 * kUnits / tiles, 4, 64));
+    const double tiles_us = 9 + 16.0 * static_cast<double>(all_k) / 4e6 + split.us;
+    if (rows <= 16 || token_us <= tiles_us) {
+      rk.launches = {launch(std::string("fg_attention_token_") + (narrow ? "1" : "2") + (dim < 4 ? "_few" : dim % 4 ? "_odd" : ""),
+                            static_cast<uint64_t>(blocks), 256, "attention")};
+    } else {
+      units = 0;
+      splits = split.parts;
+      const uint64_t key_blocks = static_cast<uint64_t>(batch * kv_heads * k_blocks);
+      tile_bytes = key_blocks * static_cast<uint64_t>(nb * 8192 + 1024);
+      rk.launches = {launch("fg_attention_pack_" + std::to_string(nb), 2 * key_blocks, 256, "attention"),
                      launch("fg_attention_tiles_" + std::to_string(nb), static_cast<uint64_t>(tiles * splits), 256, "attention")};
     }
     rk.workspace_bytes = std::max<uint64_t>(tile_bytes, 4);

@@ -181,15 +181,16 @@ def test_attention_and_its_gradients(fg, hip, shape):
     assert np.array_equal(y, got["y"])  # the same without the gradients
 
 
-# Calls of over 2^30 operations, whose forward pass cuts its operands, and of
-# more workgroups than one launch of both gradients takes.
+# Calls large enough for their forward pass to cut its operands, and of more
+# workgroups than one launch of both gradients takes.
 LARGE_SHAPES = [
     (17, 130, 130, 32, 16, 32, True, None),
     (8, 200, 260, 16, 8, 50, True, [260, 0, 1, 32, 33, 128, 129, 255]),
     (4, 300, 300, 16, 16, 80, False, [300, 299, 96, 7]),
     (4, 300, 270, 16, 4, 128, True, None),  # the first 30 queries see nothing
     (4, 130, 257, 32, 32, 127, False, None),
-    (1, 64, 5000, 16, 16, 64, False, None),  # keys of a query tile in parts
+    (1, 64, 5000, 16, 16, 64, False, None),
+    (1, 256, 4000, 16, 16, 64, False, None),  # keys of a query tile in parts
     (1, 520, 300, 64, 1, 64, True, [290]),  # queries of a key tile in parts
     (1, 600, 600, 24, 24, 100, True, None),
     (16, 130, 130, 20, 20, 64, True, [130 - 8 * i for i in range(16)]),
@@ -295,7 +296,7 @@ def test_attention_with_sharp_rows_and_values_of_unlike_sizes(fg, hip):
 @pytest.mark.gpu
 @pytest.mark.parametrize("size", [1e-18, 1e15])
 def test_larger_attention_of_small_and_large_values(fg, hip, size):
-    q, k, v, g = attention_inputs(12, 1, 300, 520, 32, 32, 64)
+    q, k, v, g = attention_inputs(12, 1, 400, 800, 32, 32, 64)
     q, k, v, g = (q / np.float32(size)), (k * np.float32(size)), v * np.float32(size), g / np.float32(size)
     kw = dict(batch=1, heads=32, kv_heads=32, causal=True)
     want = attention_ref.attention(q, k, v, g=g, **kw)
@@ -306,10 +307,10 @@ def test_larger_attention_of_small_and_large_values(fg, hip, size):
 
 @pytest.mark.gpu
 def test_larger_attention_with_sharp_rows_and_values_of_unlike_sizes(fg, hip):
-    q, k, v, g = attention_inputs(13, 1, 300, 520, 32, 8, 64, spread=40.0)
-    v *= (2.0 ** np.linspace(-20, 20, 520))[:, None].astype(np.float32)
+    q, k, v, g = attention_inputs(13, 1, 400, 800, 32, 8, 64, spread=40.0)
+    v *= (2.0 ** np.linspace(-20, 20, 800))[:, None].astype(np.float32)
     v[64:128] = 0
-    g *= (2.0 ** np.linspace(10, -10, 300))[:, None].astype(np.float32)
+    g *= (2.0 ** np.linspace(10, -10, 400))[:, None].astype(np.float32)
     kw = dict(batch=1, heads=32, kv_heads=8, scale=0.3)
     want = attention_ref.attention(q, k, v, g=g, **kw)
     got = run_attention(fg, q, k, v, g, **kw)
@@ -319,18 +320,18 @@ def test_larger_attention_with_sharp_rows_and_values_of_unlike_sizes(fg, hip):
 
 @pytest.mark.gpu
 def test_larger_attention_with_anything_behind_the_lengths(fg, hip):
-    q, k, v, g = attention_inputs(14, 2, 150, 520, 32, 16, 64)
+    q, k, v, g = attention_inputs(14, 2, 300, 700, 32, 16, 64)
     kw = dict(batch=2, heads=32, kv_heads=16, lengths=np.array([500, 3], np.int32))
     clean = run_attention(fg, q, k, v, g, **kw)
     junk = np.array([np.nan, np.inf, -np.inf, np.finfo(np.float32).max, np.finfo(np.float32).min], np.float32)
     for x in (k, v):
-        for rows in (slice(500, 520), slice(523, 1040)):
+        for rows in (slice(500, 700), slice(703, 1400)):
             x[rows] = junk[np.arange(x[rows].size) % 5].reshape(x[rows].shape)
     dirty = run_attention(fg, q, k, v, g, **kw)
     for n in clean:
         assert np.array_equal(clean[n], dirty[n]), n
     for n in ("dk", "dv"):
-        assert not dirty[n][500:520].any() and not dirty[n][523:].any()
+        assert not dirty[n][500:700].any() and not dirty[n][703:].any()
 
 
 @pytest.mark.gpu
