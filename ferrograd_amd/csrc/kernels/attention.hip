@@ -905,7 +905,9 @@ __device__ inline void query_grads(float* __restrict__ dq, const float* __restri
 // float16 products, cores busy 45% of the time at 2.0 GHz: what the power leaves
 // and the two barriers of a step, at which the pair waits for its probabilities
 // and all for the next tile. (With one wave for both, and four for dq, forward and
-// gradients took 4.21 ms instead of 3.65.)
+// gradients took 4.21 ms instead of 3.65; with 64 keys a workgroup and two of
+// them a compute unit, out of step with each other, 3.70 instead of 3.56: the
+// query tiles are then copied twice as often.)
 //
 // The rows of a tile are read before the probabilities' barrier, its columns
 // after it. Up to two column groups they have one buffer each, refilled while
