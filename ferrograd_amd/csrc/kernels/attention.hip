@@ -709,7 +709,7 @@ __device__ inline void pack_grad(const float* __restrict__ q, const float* __res
                                  const float* __restrict__ y, const float* __restrict__ g,
                                  const float* __restrict__ stats, const int* __restrict__ lengths,
                                  char* __restrict__ ws, const Shape& s) {
-  __shared__ float x[kBlock * kStride<NB>];
+  __shared__ __attribute__((aligned(16))) float x[kBlock * kStride<NB>];
   __shared__ float tops[4];
   const GradSpace f = grad_space<NB>(ws, s);
   const size_t nk = static_cast<size_t>(s.b) * s.hk * f.k_blocks;
@@ -724,31 +724,43 @@ __device__ inline void pack_grad(const float* __restrict__ q, const float* __res
   const size_t stride = static_cast<size_t>(heads) * s.d;
   const size_t first = (static_cast<size_t>(b) * n + at) * stride + static_cast<size_t>(h) * s.d;
   const float* src = (of_keys ? (second ? v : k) : (second ? g : q)) + first;
+  const int row = threadIdx.x / 8, part = threadIdx.x % 8 * 4;  // eight threads a row, for its sums: columns part .. part + 3 of every 32
+  const bool of_grads = !of_keys && second, live = at + row < s.sq;
+  float4 yv[NB];
+  float m = 0.f, inv = 0.f;
+  if (of_grads) {
+    const int to_load = min(row, rows - at - 1);
+#pragma unroll
+    for (int n = 0; n < NB; n++) yv[n] = load4(y + first + to_load * stride, 32 * n + part, s.d);
+    const size_t stat = (static_cast<size_t>(b) * s.hq + h) * s.sq + at + to_load;
+    m = stats[stat];
+    inv = stats[static_cast<size_t>(s.b) * s.hq * s.sq + stat];
+  }
   float top = load_block<NB>(src, stride, min(kBlock, rows - at), s.d, x);
   char* tile = of_keys ? f.k_tiles + block * kKeyTile<NB> : f.q_tiles + block * kQueryTile<NB>;
   char* tail = tile + (of_keys ? kKeyTile<NB> : kQueryTile<NB>) - kTail;
   int* exponents = reinterpret_cast<int*>(tail) + (of_keys ? 0 : 64);
-  const int row = threadIdx.x / 8, part = threadIdx.x % 8;  // eight threads a row, for its sums
-  if (!of_keys && second) {
+  float4* mine = reinterpret_cast<float4*>(x + row * kStride<NB> + part);  // every eighth
+  if (of_grads) {
     // g' and delta; rows past the last query stay 0.
     __syncthreads();
-    const size_t rows_all = static_cast<size_t>(s.b) * s.hq * s.sq;
-    const size_t stat = (static_cast<size_t>(b) * s.hq + h) * s.sq + at + row;
-    const bool live = at + row < s.sq;
-    const float inv = live ? stats[rows_all + stat] : 0.f;
     float delta = 0.f;
     top = 0.f;
-    for (int c = part; c < s.d; c += 8) {
-      const float gx = x[row * kStride<NB> + c] * inv;
-      x[row * kStride<NB> + c] = gx;
-      top = gx == gx ? fmaxf(top, fabsf(gx)) : INFINITY;
-      if (live) delta += gx * y[first + row * stride + c];
+#pragma unroll
+    for (int n = 0; n < NB; n++) {
+      float4 gx = mine[8 * n];
+      gx = live ? make_float4(gx.x * inv, gx.y * inv, gx.z * inv, gx.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f);
+      mine[8 * n] = gx;
+      const float of[4] = {gx.x, gx.y, gx.z, gx.w};
+#pragma unroll
+      for (int i = 0; i < 4; i++) top = of[i] == of[i] ? fmaxf(top, fabsf(of[i])) : INFINITY;
+      if (live) delta += gx.x * yv[n].x + gx.y * yv[n].y + gx.z * yv[n].z + gx.w * yv[n].w;
     }
     delta += __shfl_xor(delta, 1);
     delta += __shfl_xor(delta, 2);
     delta += __shfl_xor(delta, 4);
     if (part == 0) {
-      reinterpret_cast<float*>(tail)[row] = live ? stats[stat] : 0.f;
+      reinterpret_cast<float*>(tail)[row] = live ? m : 0.f;
       reinterpret_cast<float*>(tail)[32 + row] = delta;
     }
   }
@@ -756,9 +768,12 @@ __device__ inline void pack_grad(const float* __restrict__ q, const float* __res
   const float scale = power(e);
   if (second) {
     float squares = 0.f;
-    for (int c = part; c < s.d; c += 8) {
-      const float t = x[row * kStride<NB> + c] * scale;
-      squares += t * t;
+#pragma unroll
+    for (int n = 0; n < NB; n++) {
+      const float4 v = mine[8 * n];
+      const float of[4] = {v.x * scale, v.y * scale, v.z * scale, v.w * scale};
+#pragma unroll
+      for (int i = 0; i < 4; i++) squares += of[i] * of[i];
     }
     squares += __shfl_xor(squares, 1);
     squares += __shfl_xor(squares, 2);
