@@ -701,9 +701,10 @@ __device__ inline int norm_exponent(float squares, int e) {
 __device__ inline float power(int a) { return ldexpf(1.f, a); }
 
 // Keys, values, queries and gradients cut once per call, one workgroup per
-// block and matrix. Bound by memory, 4.0 TB/s: 16 heads of 128 over 8192 tokens
-// 138 us for 237 MB read and 320 written (queries and gradients by rows for the
-// scores, and by columns for dk and dv).
+// block and matrix. Bound by memory: 16 heads of 128 over 8192 tokens 102 us for
+// 236 MB read and 320 written, 5.4 TB/s (queries and gradients by rows for the
+// scores, and by columns for dk and dv). With the outputs read after the gradients
+// were in LDS it took 138.
 template <int NB>
 __device__ inline void pack_grad(const float* __restrict__ q, const float* __restrict__ k, const float* __restrict__ v,
                                  const float* __restrict__ y, const float* __restrict__ g,
@@ -916,8 +917,8 @@ __device__ inline void query_grads(float* __restrict__ dq, const float* __restri
 // probabilities' way through LDS. Scores are not transposed here: a lane holds
 // 16 queries of one key, which is what dv^T += G^T P and dk^T += Q^T dS take.
 //
-// 16 heads of 128 over 4 key heads and 8192 causal tokens: 1737 us, 950 TFLOP/s of
-// float16 products, cores busy 45% of the time at 2.0 GHz: what the power leaves
+// 16 heads of 128 over 4 key heads and 8192 causal tokens: 1685 us, 980 TFLOP/s of
+// float16 products, cores busy 46% of the time at 2.0 GHz: what the power leaves
 // and the two barriers of a step, at which the pair waits for its probabilities
 // and all for the next tile. (With one wave for both, and four for dq, forward and
 // gradients took 4.21 ms instead of 3.65; with 64 keys a workgroup and two of
@@ -1168,7 +1169,7 @@ __device__ inline void sum_parts(float* __restrict__ first, float* __restrict__ 
 // reads 537 MB in 94 us, 5.7 TB/s, and with lengths of half that on the average 268
 // MB in 46 us, 5.9 TB/s; the join takes 5. A wave loads its next 16 keys and values
 // while it works on the last. Small calls are bound by their few dependent steps: 2
-// x 4 heads of 32 over 33 tokens 6 us, 8 x 8 of 64 over 256 causal tokens 22.
+// x 4 heads of 32 over 33 tokens 6 us, 8 x 8 of 64 over 256 causal tokens 18.
 
 // Whether rows are whole vectors of four columns, end within one, or are less
 // than one.

@@ -284,8 +284,8 @@ RenderedKernel render_attention(const UOp& call, bool grad) {
     // The other cuts its operands first. It is taken where that and its tiles take
     // less than the float32 workgroups: as long as one of them alone, or as all of
     // them, each a start and rounds of 64 keys. Float32 path against cut operands,
-    // us: 8 x 8 heads of 64 over 256 causal tokens 22 and 22, one sequence of 512
-    // 17 and 20, 2 x 4 heads of 128 over 500 20 and 32, 16 of 128 over 512 47 and
+    // us: 8 x 8 heads of 64 over 256 causal tokens 18 and 22, one sequence of 512
+    // 16 and 20, 2 x 4 heads of 128 over 500 20 and 32, 16 of 128 over 512 47 and
     // 34, 4 x 50 of 128 over 10 and 99 tokens 29 and 20.
     const bool narrow = dim <= 64;
     const double rounds = static_cast<double>((per + 63) / 64) * (causal && splits == 1 ? 0.75 : 1);
