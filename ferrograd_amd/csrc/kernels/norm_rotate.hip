@@ -17,7 +17,12 @@
 // Rows need not start on a vector's alignment, nor halves be whole vectors: the
 // last lane of a half then begins where its vector ends with the half, and
 // leaves what it shares with the lane before it out of the sums (its stores are
-// the same values again).
+// the same values again). With vectors as wide as the alignment allowed instead,
+// 5001 x 7 x 74 took 11 us forward and 16 backward, now 8 and 9.
+//
+// 16384 tokens of 32 heads of 128: 94 us forward (5.7 TB/s), 140 backward (5.8);
+// elementwise kernels reach 6.3 here. Walking rows token by token in waves of
+// their own, with angles made per row, backward took 167.
 // Angles are formed in 64 bits as revolutions and reduced there: a far position
 // times a frequency has more whole turns than 32 bits can hold beside the
 // fraction.
@@ -109,7 +114,8 @@ __device__ inline void turns(Angles& a, const int* positions, int count, int hal
 
 // Rows are taken kRows at a time, loaded before the first is worked on: a row is
 // a few hundred bytes, and the memory needs more of them under way than there
-// are waves.
+// are waves. Forward the first are on their way while the angles are made;
+// backward that holds too many registers (149 us instead of 143).
 constexpr int kRows = 2, kGradRows = 2;
 
 // A lane's part of a row: where its vectors start in the halves, whether it has
