@@ -570,6 +570,22 @@ def test_gradients_realised_after_their_loss(fg, hip):
 
 
 @pytest.mark.gpu
+def test_gradients_of_gradients(fg, hip):
+    # Dropout's is its own again; the others' are refused.
+    x = seeded(30).standard_normal((12, 16)).astype(np.float32)
+    t = new(fg, x, True)
+    g = t.dropout(0.5, 3).mul(t).sum([0, 1]).gradient([t])[0]  # 2 m x, m the mask times 2
+    d = g.mul(g).sum([0, 1]).gradient([t])[0].numpy()
+    m = dropped(np.ones_like(x), 0.5, 3, 0)
+    assert np.array_equal(d, 8 * m * m * x)  # all powers of two but x
+    w, pos = new(fg, np.ones(8, np.float32), True), new(fg, np.arange(12, dtype=np.int32))
+    for y in (t.attention(t, t, heads=2), t.norm_rotate(w, pos, heads=2)):
+        g = y.sum([0, 1]).gradient([t])[0]
+        with pytest.raises(fg.FerrogradError, match="gradient not implemented"):
+            g.mul(g).sum([0, 1]).gradient([t])
+
+
+@pytest.mark.gpu
 def test_calls_read_views_and_literals_and_update_in_place(fg, hip):
     r = seeded(40)
     x, m = r.standard_normal((12, 8)).astype(np.float32), r.standard_normal((8, 12)).astype(np.float32)
