@@ -126,9 +126,13 @@ RenderedKernel render_dropout(const UOp& call) {
 }
 
 // Output i (from 1 on) of a call with sources `srcs`: its storage, a source of
-// the call besides them.
-UOp output_storage(KernelId id, int64_t i, const Shape& shape, const std::vector<UOp>& srcs) {
-  return UOp::make_new(Op::KernelBuf, DType::F32(), srcs, Arg::kernel(static_cast<int64_t>(id), shape, {i}));
+// the call besides them. Nodes that are alike are one node, so it carries all
+// that tells the call from others on the same sources: without the call's
+// parameters two calls that differ in nothing else would write one buffer.
+UOp output_storage(KernelId id, int64_t i, const Shape& shape, const std::vector<UOp>& srcs, const std::vector<int64_t>& params) {
+  std::vector<int64_t> key{i};
+  key.insert(key.end(), params.begin(), params.end());
+  return UOp::make_new(Op::KernelBuf, DType::F32(), srcs, Arg::kernel(static_cast<int64_t>(id), shape, key));
 }
 
 UOp output_of(const UOp& storage, const UOp& call) {
@@ -453,7 +457,7 @@ Tensor Tensor::attention(const Tensor& k, const Tensor& v, const Tensor* lengths
                                        static_cast<int64_t>(dim), causal, lengths != nullptr, to_bits(scale)};
   std::vector<UOp> srcs = {source(uop()), source(k.uop()), source(v.uop())};
   if (lengths) srcs.push_back(source(lengths->uop()));
-  srcs.push_back(output_storage(KernelId::Attention, 1, Shape{2, batch * heads * sq}, srcs));
+  srcs.push_back(output_storage(KernelId::Attention, 1, Shape{2, batch * heads * sq}, srcs, params));
   return from_uop(make_call(KernelId::Attention, qs, srcs, params), requires_grad() || k.requires_grad() || v.requires_grad());
 }
 
@@ -475,7 +479,7 @@ std::vector<UOp> kernel_gradient(const UOp& call, const UOp& grad) {
     case KernelId::NormRotate: {
       std::vector<UOp> srcs = call.srcs();
       srcs.push_back(gradient_source(grad));
-      UOp dw = output_storage(KernelId::NormRotateGrad, 1, call.src(1).shape(), srcs);
+      UOp dw = output_storage(KernelId::NormRotateGrad, 1, call.src(1).shape(), srcs, params_of(call));
       srcs.push_back(dw);
       UOp dx = make_call(KernelId::NormRotateGrad, call.src(0).shape(), srcs, params_of(call));
       return {dx, output_of(dw, dx), UOp()};
@@ -485,8 +489,8 @@ std::vector<UOp> kernel_gradient(const UOp& call, const UOp& grad) {
       std::vector<UOp> srcs = {call.src(0), call.src(1), call.src(2), call, gradient_source(grad)};
       srcs.push_back(output_of(call.srcs().back(), call));
       if (params[7]) srcs.push_back(call.src(3));
-      UOp dk = output_storage(KernelId::AttentionGrad, 1, call.src(1).shape(), srcs);
-      UOp dv = output_storage(KernelId::AttentionGrad, 2, call.src(2).shape(), srcs);
+      UOp dk = output_storage(KernelId::AttentionGrad, 1, call.src(1).shape(), srcs, params);
+      UOp dv = output_storage(KernelId::AttentionGrad, 2, call.src(2).shape(), srcs, params);
       srcs.push_back(dk);
       srcs.push_back(dv);
       UOp dq = make_call(KernelId::AttentionGrad, call.src(0).shape(), srcs, params);
