@@ -28,6 +28,10 @@ __device__ inline int visible(const Shape& s, int keys, int i) {
   return s.causal ? max(0, min(keys, i + s.sk - s.sq + 1)) : keys;
 }
 
+// 1 / a row's sum: 0 where it saw no key, and NaN where one of its scores was, so
+// that its gradients are not finite either.
+__device__ inline float inverse_sum(float sum) { return sum == 0.f ? 0.f : 1.f / sum; }
+
 __device__ inline float wave_max(float x) {
   for (int d = 32; d > 0; d /= 2) x = fmaxf(x, __shfl_xor(x, d));
   return x;
@@ -443,24 +447,24 @@ __device__ inline void join_columns(float* __restrict__ y, float* __restrict__ s
 #pragma unroll
     for (int n = 0; n < N; n++) {
       if (p0 + n >= splits) ml[n].y = 0.f;
-      if (ml[n].y > 0.f) most = fmaxf(most, ml[n].x);
+      if (ml[n].y != 0.f) most = fmaxf(most, ml[n].x);
     }
-    if (most == -INFINITY) continue;
-    const float old = exp2f(top - most);
+    // A part whose sum is NaN counts: only 0 says that it saw no key.
+    const float base = most == -INFINITY ? 0.f : most, old = exp2f(top - base);
     sum *= old;
 #pragma unroll
     for (int w = 0; w < W; w++) all[w] *= old;
     top = most;
 #pragma unroll
     for (int n = 0; n < N; n++)
-      if (ml[n].y > 0.f) {
-        const float of = exp2f(ml[n].x - top);
+      if (ml[n].y != 0.f) {
+        const float of = exp2f(ml[n].x - base);
         sum += of * ml[n].y;
 #pragma unroll
         for (int w = 0; w < W; w++) all[w] += of * o[n][w];
       }
   }
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  const float inv = inverse_sum(sum);
   float* out = y + (b * s.sq + i) * s.hq * s.d + static_cast<size_t>(h) * s.d + d;
 #pragma unroll
   for (int w = 0; w < W; w++) all[w] *= inv;
@@ -628,7 +632,7 @@ __device__ inline void forward_tiles(float* __restrict__ y, const float* __restr
     }
     return;
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const float inv = inverse_sum(l);
   float* row = y + (static_cast<size_t>(b) * s.sq + i) * s.hq * s.d + static_cast<size_t>(h) * s.d;
 #pragma unroll
   for (int n = 0; n < NB; n++) store_columns(row, n, half, s.d, o[n], inv, -kProbShift - vs.ref);
@@ -690,7 +694,7 @@ __device__ inline size_t key_parts(const Shape& s, int parts) {
 // The power of two above a norm, from the largest sum of squares of a block's
 // numbers times 2^e.
 __device__ inline int norm_exponent(float squares, int e) {
-  if (!(squares > 0.f)) return -120;
+  if (squares == 0.f) return -120;
   if (!(squares < INFINITY)) return 0;
   int k;
   frexpf(squares, &k);
@@ -1339,7 +1343,7 @@ __device__ inline void token(float* __restrict__ y, const float* __restrict__ q,
         parts.ml[2 * out + 1] = sum;
       }
     } else {
-      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      const float inv = inverse_sum(sum);
       if (d < s.d) y[(static_cast<size_t>(b) * s.sq + iq) * s.hq * s.d + static_cast<size_t>(hq) * s.d + d] = all * inv;
       if (d == 0) {
         stats[stat] = top;

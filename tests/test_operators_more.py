@@ -103,3 +103,100 @@ def test_gradients_of_two_norms_on_the_same_tensors(fg, hip, kw):
         fg.Tensor.realize_many([y, dx, dw])
         for name, t in (("y", y), ("dx", dx), ("dweight", dw)):
             check((step, name), t.numpy(), *both(a[name], b[name]))
+
+
+# ── NaN and infinities that are seen ────────────────────────────────────────
+
+# batch, sq, sk, heads, kv_heads, dim, lengths, and the launches of the forward pass
+PATHS = {
+    "small": (2, 3, 200, 4, 2, 24, None, ["token"]),
+    "small in parts": (2, 1, 3000, 4, 2, 24, None, ["token", "join"]),
+    "three columns in parts": (1, 1, 1300, 1, 1, 3, None, ["token", "join"]),
+    "parts of one length": (10, 1, 2500, 12, 6, 24, [2500, 0, 2400, 1300, 2, 128, 129, 2499, 1, 2500], ["token", "join"]),
+    "large": (4, 130, 257, 32, 32, 40, None, ["pack", "tiles"]),
+    "large in parts": (1, 256, 4000, 16, 8, 64, None, ["pack", "tiles", "join"]),
+}
+
+
+def forward_launches(fg, batch, sq, sk, heads, kv_heads, dim, lengths):
+    q, k = fg.Tensor.zeros([batch * sq, heads * dim], "hip"), fg.Tensor.zeros([batch * sk, kv_heads * dim], "hip")
+    y = q.attention(k, k, heads=heads, kv_heads=kv_heads, batch=batch,
+                    lengths=None if lengths is None else fg.Tensor.zeros([batch], "hip", fg.I32))
+    call = [it for it in fg.debug_plan([y], fuse=True, render_hip=True)["items"] if it["class"] == "attention"]
+    return [l["name"].split("_")[2] for it in call for l in it["launches"]]
+
+
+@pytest.mark.parametrize("path", PATHS)
+def test_the_shapes_below_take_their_paths(fg, path):
+    *shape, launches = PATHS[path]
+    assert forward_launches(fg, *shape) == launches
+
+
+def run_both(fg, q, k, v, g, **kw):
+    """y and the gradients of attention, as arrays."""
+    tq, tk, tv = (new(fg, t, True) for t in (q, k, v))
+    if kw.get("lengths") is not None:
+        kw["lengths"] = new(fg, np.asarray(kw["lengths"], np.int32))
+    y = tq.attention(tk, tv, **kw)
+    grads = y.mul(new(fg, g)).sum([0, 1]).gradient([tq, tk, tv])
+    fg.Tensor.realize_many([y, *grads])
+    return {n: t.numpy() for n, t in zip(("y", "dq", "dk", "dv"), (y, *grads))}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", [np.nan, np.inf], ids=["nan", "inf"])
+@pytest.mark.parametrize("path", PATHS)
+def test_rows_that_see_a_key_that_is_not_finite_are_not_finite(fg, hip, path, what):
+    batch, sq, sk, heads, kv_heads, dim, lengths, _ = PATHS[path]
+    kw = dict(batch=batch, heads=heads, kv_heads=kv_heads, lengths=lengths)
+    q, k, v, g = attention_inputs(60, batch, sq, sk, heads, kv_heads, dim)
+    q[:sq, 0] = np.abs(q[:sq, 0]) + 0.1  # an infinite key scores +infinity
+    clean = run_both(fg, q, k, v, g, **kw)
+    at = sk * 3 // 5
+    k[at, 0] = what  # a visible key of the first sequence and key head
+    got = run_both(fg, q, k, v, g, **kw)
+    group = heads // kv_heads
+    for name, rows, cols in (("y", sq, dim if what == np.inf else group * dim), ("dq", sq, dim), ("dk", sk, dim), ("dv", sk, dim)):
+        bad = np.zeros(got[name].shape, bool)
+        bad[:rows, :cols] = True
+        assert not np.isfinite(got[name][bad]).any(), name
+        rest = np.ones(got[name].shape, bool)  # what other key heads and sequences see
+        rest[:rows, :(group if name in ("y", "dq") else 1) * dim] = False
+        assert np.array_equal(got[name][rest], clean[name][rest]), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("path", PATHS)
+def test_a_query_that_is_nan_has_a_row_of_nan(fg, hip, path):
+    batch, sq, sk, heads, kv_heads, dim, lengths, _ = PATHS[path]
+    kw = dict(batch=batch, heads=heads, kv_heads=kv_heads, lengths=lengths)
+    q, k, v, g = attention_inputs(61, batch, sq, sk, heads, kv_heads, dim)
+    clean = run_both(fg, q, k, v, g, **kw)
+    at = sq // 2
+    q[at, dim - 1] = np.nan  # of the first sequence and head
+    got = run_both(fg, q, k, v, g, **kw)
+    bad = np.zeros(q.shape, bool)
+    bad[at, :dim] = True
+    assert np.isnan(got["y"][bad]).all() and np.isnan(got["dq"][bad]).all()
+    assert np.array_equal(got["y"][~bad], clean["y"][~bad])
+    seen = np.zeros(k.shape, bool)
+    seen[:sk, :dim] = True
+    for name in ("dk", "dv"):
+        assert np.isnan(got[name][seen]).all(), name
+        assert np.array_equal(got[name][~seen], clean[name][~seen]), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("path", PATHS)
+def test_a_value_that_is_nan_makes_its_column_nan(fg, hip, path):
+    batch, sq, sk, heads, kv_heads, dim, lengths, _ = PATHS[path]
+    kw = dict(batch=batch, heads=heads, kv_heads=kv_heads, lengths=lengths)
+    q, k, v, g = attention_inputs(62, batch, sq, sk, heads, kv_heads, dim)
+    v[sk // 2, 1] = np.nan
+    got = run_both(fg, q, k, v, g, **kw)
+    group = heads // kv_heads
+    assert np.isnan(got["y"][:sq].reshape(sq, heads, dim)[:, :group, 1]).all()
+    assert np.isnan(got["dq"][:sq, :group * dim]).all() and np.isnan(got["dk"][:sk, :dim]).all()
+    rest = np.ones(q.shape, bool)
+    rest[:sq, :group * dim] = False
+    assert np.isfinite(got["y"][rest]).all() and np.isfinite(got["dq"][rest]).all()
