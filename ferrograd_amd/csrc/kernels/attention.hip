@@ -60,8 +60,9 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 
 // Rows of a block that shares a scale, and of a tile.
 constexpr int kBlock = 32;
-// The scale of a block of zeros.
-constexpr int kZeroExponent = 127;
+// The exponents of blocks: at most kMostExponent, or that of a block of zeros,
+// which takes part in nothing.
+constexpr int kMostExponent = 127, kZeroExponent = 1000;
 constexpr int kPart = 1024;  // bytes of one fragment: 64 lanes of 8 float16
 
 // The power of two that brings `top`, a block's largest magnitude, into
@@ -71,8 +72,11 @@ __device__ inline int block_exponent(float top) {
   if (!(top < INFINITY)) return 0;
   int e;
   frexpf(top, &e);  // top = f 2^e with f in [1/2, 1)
-  return min(15 - e, kZeroExponent);
+  return min(15 - e, kMostExponent);
 }
+
+// The scale of a block of exponent e.
+__device__ inline float block_scale(int e) { return e == kZeroExponent ? 0.f : ldexpf(1.f, e); }
 
 // Eight scaled numbers as two parts, both rounded to nearest.
 __device__ inline void cut(const float (&x)[8], half8* hi, half8* lo) {
@@ -244,7 +248,7 @@ __device__ inline void pack_keys(const float* k, const float* v, const int* leng
   const float top = block_max(
       load_block<NB>((values ? v : k) + at, static_cast<size_t>(Hk) * D, min(kBlock, keys - kb * kBlock), D, x), tops);
   const int e = block_exponent(top);
-  const float scale = ldexpf(1.f, e);
+  const float scale = block_scale(e);
   char* tile = ws + block * kForwardTile<NB>;
   if (values) write_cols<NB>(x, scale, tile + kRowBytes<NB>);
   else write_rows<NB>(x, scale, tile);
@@ -282,9 +286,13 @@ struct RunningScale {
   bool any = false;
   // Takes block exponent e; returns the power of two that accumulators have
   // to be multiplied by (0: none), and leaves in *behind how far the block's
-  // operand is above ref (what the other operand makes up for).
+  // operand is above ref (what the other operand makes up for). A block of zeros
+  // changes nothing: were its exponent a scale like any other, probabilities
+  // would be cut to meet it, and their row's sum with them.
   __device__ int take(int e, int* behind) {
     int change = 0;
+    *behind = 0;
+    if (e >= kZeroExponent / 2) return 0;  // with another exponent added or not
     if (!any) {
       any = true;
       ref = least = e;
@@ -349,7 +357,7 @@ __device__ inline int row_fragments(const float* row, bool live, int D, float si
       top = v[t][i] == v[t][i] ? fmaxf(top, fabsf(v[t][i])) : INFINITY;
     }
   const int e = block_exponent(halves_max(top));
-  const float scale = ldexpf(sign, e);
+  const float scale = sign * block_scale(e);
 #pragma unroll
   for (int t = 0; t < NB * 2; t++) {
 #pragma unroll
@@ -770,7 +778,7 @@ __device__ inline void pack_grad(const float* __restrict__ q, const float* __res
     }
   }
   const int e = block_exponent(block_max(top, tops));
-  const float scale = power(e);
+  const float scale = block_scale(e);
   if (second) {
     float squares = 0.f;
 #pragma unroll

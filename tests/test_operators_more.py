@@ -200,3 +200,22 @@ def test_a_value_that_is_nan_makes_its_column_nan(fg, hip, path):
     rest = np.ones(q.shape, bool)
     rest[:sq, :group * dim] = False
     assert np.isfinite(got["y"][rest]).all() and np.isfinite(got["dq"][rest]).all()
+
+
+# ── values of unlike sizes ──────────────────────────────────────────────────
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [1e20, 1e26, 1e30])
+@pytest.mark.parametrize("zeros", ["last", "first", "between"])
+def test_values_of_zero_beside_large_ones_take_their_probability(fg, hip, size, zeros):
+    batch, sq, sk, heads, kv_heads, dim, lengths, _ = PATHS["large"]
+    q, k, v, g = attention_inputs(63, batch, sq, sk, heads, kv_heads, dim, spread=0.5)
+    v = (v * np.float32(size)).reshape(batch, sk, -1)
+    v[:, {"last": slice(128, None), "first": slice(0, 128), "between": slice(64, 192)}[zeros]] = 0
+    v = v.reshape(batch * sk, -1)
+    g /= np.float32(size)
+    kw = dict(batch=batch, heads=heads, kv_heads=kv_heads)
+    got, want = run_both(fg, q, k, v, g, **kw), attention_ref.attention(q, k, v, g=g, **kw)
+    for name in want:
+        check(name, got[name], *want[name])
