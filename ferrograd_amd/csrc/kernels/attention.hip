@@ -32,20 +32,29 @@ __device__ inline int visible(const Shape& s, int keys, int i) {
 // that its gradients are not finite either.
 __device__ inline float inverse_sum(float sum) { return sum == 0.f ? 0.f : 1.f / sum; }
 
-__device__ inline float wave_max(float x) {
-  for (int d = 32; d > 0; d /= 2) x = fmaxf(x, __shfl_xor(x, d));
-  return x;
+// The word joined over eight lanes next to each other, and over a wave, in all
+// of them: by lane permutations of the vector unit, none of which passes LDS.
+template <class Join>
+__device__ inline int join8(int x, Join join) {
+  x = join(x, __builtin_amdgcn_mov_dpp(x, 0xB1, 0xF, 0xF, false));   // lanes 1, 0, 3, 2 of four
+  x = join(x, __builtin_amdgcn_mov_dpp(x, 0x4E, 0xF, 0xF, false));   // lanes 2, 3, 0, 1 of four
+  return join(x, __builtin_amdgcn_mov_dpp(x, 0x141, 0xF, 0xF, false));  // eight mirrored
 }
-__device__ inline float wave_sum(float x) {
-  for (int d = 32; d > 0; d /= 2) x += __shfl_xor(x, d);
-  return x;
+template <class Join>
+__device__ inline int join_wave(int x, Join join) {
+  x = join8(x, join);
+  x = join(x, __builtin_amdgcn_mov_dpp(x, 0x140, 0xF, 0xF, false));  // sixteen mirrored
+  const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = join(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return join(b[0], b[1]);
 }
+__device__ inline int max_of_floats(int a, int b) { return __float_as_int(fmaxf(__int_as_float(a), __int_as_float(b))); }
 
-__device__ inline float dot(const float* a, const float* b, int d) {
-  float t = 0.f;
-  for (int e = 0; e < d; e++) t += a[e] * b[e];
-  return t;
+__device__ inline float sum8(float x) {
+  return __int_as_float(join8(__float_as_int(x), [](int a, int b) { return __float_as_int(__int_as_float(a) + __int_as_float(b)); }));
 }
+__device__ inline float wave_max(float x) { return __int_as_float(join_wave(__float_as_int(x), max_of_floats)); }
 
 // ── products of cut operands ────────────────────────────────────────────────
 // A float32 product on the float16 matrix cores: each operand is scaled by a
@@ -60,23 +69,24 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 
 // Rows of a block that shares a scale, and of a tile.
 constexpr int kBlock = 32;
-// The exponents of blocks: at most kMostExponent, or that of a block of zeros,
-// which takes part in nothing.
-constexpr int kMostExponent = 127, kZeroExponent = 1000;
+// The exponents of blocks: at most kMostExponent, or, beyond every sum of two of
+// these, that of a block of zeros, which takes part in nothing, and that of one
+// that is not finite, nor is what it takes part in.
+constexpr int kMostExponent = 127, kNoExponent = 500, kNotFiniteExponent = 900, kZeroExponent = 1000;
 constexpr int kPart = 1024;  // bytes of one fragment: 64 lanes of 8 float16
 
 // The power of two that brings `top`, a block's largest magnitude, into
-// [2^14, 2^15). Not finite: 0, and what the block takes part in is not finite.
+// [2^14, 2^15).
 __device__ inline int block_exponent(float top) {
   if (top == 0.f) return kZeroExponent;
-  if (!(top < INFINITY)) return 0;
+  if (!(top < INFINITY)) return kNotFiniteExponent;
   int e;
   frexpf(top, &e);  // top = f 2^e with f in [1/2, 1)
   return min(15 - e, kMostExponent);
 }
 
 // The scale of a block of exponent e.
-__device__ inline float block_scale(int e) { return e == kZeroExponent ? 0.f : ldexpf(1.f, e); }
+__device__ inline float block_scale(int e) { return e < kNoExponent ? ldexpf(1.f, e) : e == kZeroExponent ? 0.f : 1.f; }
 
 // Eight scaled numbers as two parts, both rounded to nearest.
 __device__ inline void cut(const float (&x)[8], half8* hi, half8* lo) {
@@ -170,6 +180,176 @@ __device__ inline float block_max(float x, float* shared) {
   return x;
 }
 
+// A block's largest magnitude (infinite where it holds a NaN) and its smallest
+// that is not zero.
+struct Extremes {
+  float top = 0.f, least = INFINITY;
+  __device__ void take(const float4& v) {
+    const float a[4] = {fabsf(v.x), fabsf(v.y), fabsf(v.z), fabsf(v.w)};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      top = a[i] == a[i] ? fmaxf(top, a[i]) : INFINITY;
+      least = fminf(least, a[i] > 0.f ? a[i] : INFINITY);
+    }
+  }
+  // Those of the 256 threads, in all of them. `shared`: 8 floats.
+  __device__ void join(float* shared) {
+    const float t = wave_max(top), l = wave_max(-least);
+    if (threadIdx.x % 64 == 0) {
+      shared[threadIdx.x / 64] = t;
+      shared[4 + threadIdx.x / 64] = l;
+    }
+    __syncthreads();
+    top = fmaxf(fmaxf(shared[0], shared[1]), fmaxf(shared[2], shared[3]));
+    least = -fmaxf(fmaxf(shared[4], shared[5]), fmaxf(shared[6], shared[7]));
+  }
+};
+
+// ── even blocks ─────────────────────────────────────────────────────────────
+// A number of a cut block is off by up to 2^-22 of itself or 2^-40 of the block's
+// largest, whichever is more, and probabilities and gradients of scores are cut
+// at 2^-37 of what they can be at most. So where rows or columns are of very
+// unlike sizes, float32 would keep of the small ones what this loses, and a
+// key that a query does not even see would set the scale of those it sees. The
+// launches that cut operands write how even each block is, and workgroups that
+// meet blocks (or scores, or sizes of blocks) beyond these bounds take float32
+// matrix products of the operands as they are instead:
+constexpr int kSpread = 16;         // rows of one block, and of all blocks of a matrix but g', to the largest: errors 2^-24 of each row's largest
+constexpr int kColumnSpread = 20;   // columns of one block: a block's last row alone is a column each
+constexpr int kGradSpread = 40;     // blocks of g': dv and dk follow each block's scale, up to 60
+constexpr int kMostScore = 16;      // scores: 2^-40 of the largest is 2^-24, an error of p as rounding leaves it
+constexpr int kNoRange = 1000;      // beyond every power of two of a float, up or down
+constexpr int kUneven = 4096;       // added to an exponent: the block is uneven in itself
+
+// How even a block is: the power of two above its largest number, and minus
+// that of its smallest row that is not zero (kNoRange more where its columns
+// or too many of its numbers are small). Both are least for a block of zeros,
+// and both beyond every bound for one that is not finite, so that blocks taken
+// together have the largest of each.
+typedef short Range __attribute__((ext_vector_type(2)));
+constexpr int kNotFinite = 8 * kNoRange;
+
+__device__ inline Range no_range() { return Range{static_cast<short>(-kNoRange), static_cast<short>(-kNoRange)}; }
+__device__ inline Range widest(Range a, Range b) { return __builtin_elementwise_max(a, b); }
+__device__ inline int spread(Range r) { return r[0] + r[1]; }
+// A block's range without its rows': what its largest number spreads over blocks.
+__device__ inline Range top_only(Range r) { return r[0] == -kNoRange ? r : Range{r[0], static_cast<short>(-r[0])}; }
+
+// The range of one number.
+__device__ inline Range top_range(float top) {
+  if (top == 0.f) return no_range();
+  if (!(top < INFINITY)) return Range{static_cast<short>(kNotFinite), static_cast<short>(kNotFinite)};
+  int e;
+  frexpf(top, &e);
+  return Range{static_cast<short>(e), static_cast<short>(-e)};
+}
+
+// The widest of a wave's lanes, in scalar registers.
+__device__ inline Range wave_widest(Range r) {
+  const int x = join_wave(__builtin_bit_cast(int, r), [](int a, int b) {
+    return __builtin_bit_cast(int, widest(__builtin_bit_cast(Range, a), __builtin_bit_cast(Range, b)));
+  });
+  return __builtin_bit_cast(Range, __builtin_amdgcn_readfirstlane(x));
+}
+
+// Two matrices' ranges: of keys and values, or of queries and gradients.
+struct Ranges {
+  Range first, second;
+};
+
+// The widest of `n` blocks, for a whole wave.
+__device__ inline Ranges widest_of(const Ranges* ranges, int n) {
+  Ranges r = {no_range(), no_range()};
+  for (int i = threadIdx.x % 64; i < n; i += 64) {
+    const Ranges b = ranges[i];
+    r.first = widest(r.first, b.first);
+    r.second = widest(r.second, b.second);
+  }
+  return {wave_widest(r.first), wave_widest(r.second)};
+}
+
+// ... of the blocks' largest numbers alone, and whether any is uneven in itself.
+struct Tops {
+  Range first, second;
+  bool uneven;
+};
+__device__ inline Tops tops_of(const Ranges* ranges, int n) {
+  Tops r = {no_range(), no_range(), false};
+  for (int i = threadIdx.x % 64; i < n; i += 64) {
+    const Ranges b = ranges[i];
+    r.first = widest(r.first, top_only(b.first));
+    r.second = widest(r.second, top_only(b.second));
+    r.uneven |= max(spread(b.first), spread(b.second)) > kSpread;
+  }
+  return {wave_widest(r.first), wave_widest(r.second), __any(r.uneven) != 0};
+}
+
+// The power of two above |scale| log2 e D: what the largest numbers of a query
+// and a key are multiplied by to bound their score.
+__device__ inline int score_exponent(float scale, int D) {
+  int e;
+  frexpf(fabsf(scale) * kLog2e * D, &e);
+  return e;
+}
+
+// The range of a block in LDS, in the threads of the first wave. `top` and
+// `least` are its largest magnitude and its smallest that is not zero, in all
+// threads; every thread takes part. Where no number is 2^-kColumnSpread of the
+// largest, nor is a column (nearly all blocks of numbers drawn alike), and only
+// its rows are looked at: the launches that cut operands took up to 4 us more
+// with the columns of every block looked at.
+struct RangeSpace {
+  float lows[4], columns[256];
+  int counts[4];
+};
+template <int NB>
+__device__ inline Range block_range(const float* x, float top, float least, RangeSpace& shared, int D) {
+  const int wave = threadIdx.x / 64, row = threadIdx.x / 8, part = threadIdx.x % 8 * 4;
+  float of_row = 0.f;
+#pragma unroll
+  for (int n = 0; n < NB; n++) {
+    const float4 v = *reinterpret_cast<const float4*>(x + row * kStride<NB> + 32 * n + part);
+    of_row = fmaxf(of_row, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+  }
+  of_row = __int_as_float(join8(__float_as_int(of_row), max_of_floats));
+  int e;
+  frexpf(of_row, &e);
+  const float low = wave_max(of_row > 0.f ? static_cast<float>(-e) : -kNoRange);
+  if (threadIdx.x % 64 == 0) shared.lows[wave] = low;
+  bool uneven = false;
+  if (least < ldexpf(top, -kColumnSpread)) {
+    // A thread has a column's rows of its slice.
+    constexpr int kColumns = NB * 32, kSlices = NB == 3 ? 2 : 256 / kColumns, kRows = 32 / kSlices;
+    const int column = threadIdx.x % kColumns, slice = threadIdx.x / kColumns;
+    float of_column = 0.f;
+    int small = 0;
+    if (slice < kSlices)
+      for (int i = 0; i < kRows; i++) {
+        const float a = fabsf(x[(slice * kRows + i) * kStride<NB> + column]);
+        of_column = fmaxf(of_column, a);
+        small += a > 0.f && a < ldexpf(top, -kSpread) ? 1 : 0;
+      }
+    shared.columns[threadIdx.x] = of_column;
+    small = join_wave(small, [](int a, int b) { return a + b; });
+    if (threadIdx.x % 64 == 0) shared.counts[wave] = small;
+    __syncthreads();
+    if (wave == 0) {
+      for (int c = threadIdx.x; c < kColumns; c += 64) {
+        float most = 0.f;
+        for (int i = 0; i < kSlices; i++) most = fmaxf(most, shared.columns[i * kColumns + c]);
+        uneven |= most > 0.f && most < ldexpf(top, -kColumnSpread);
+      }
+      uneven = __any(uneven) || shared.counts[0] + shared.counts[1] + shared.counts[2] + shared.counts[3] > 2 * D;
+    }
+  } else {
+    __syncthreads();
+  }
+  if (wave > 0) return no_range();
+  const float lows = fmaxf(fmaxf(shared.lows[0], shared.lows[1]), fmaxf(shared.lows[2], shared.lows[3]));
+  const Range r = top_range(top);
+  return r[0] == -kNoRange || r[0] == kNotFinite ? r : Range{r[0], static_cast<short>(uneven ? kNoRange : static_cast<int>(lows))};
+}
+
 // Four numbers of a row, which starts on any float: odd head sizes take the
 // same 16-byte loads and stores. (As single floats a token over 8 x 8192 keys of
 // 63 columns took 80 us, of 127 251; so 29 and 77, as 64 and 128 do.)
@@ -203,11 +383,11 @@ __device__ inline float4 load4(const float* row, int c, int D) {
   return v;
 }
 
-// A block of up to 32 rows of `rows` rows of D numbers into LDS, the rest 0;
-// the largest magnitude among this thread's.
+// A block of up to 32 rows of `rows` rows of D numbers into LDS, the rest 0; the
+// extremes of this thread's.
 template <int NB>
-__device__ inline float load_block(const float* src, size_t stride, int rows, int D, float* x) {
-  float top = 0.f;
+__device__ inline Extremes load_block(const float* src, size_t stride, int rows, int D, float* x) {
+  Extremes of;
   float4 loaded[NB];
 #pragma unroll
   for (int n = 0; n < NB; n++) {
@@ -218,26 +398,31 @@ __device__ inline float load_block(const float* src, size_t stride, int rows, in
   for (int n = 0; n < NB; n++) {
     const int at = n * 256 + threadIdx.x, row = at / (NB * 8), c = at % (NB * 8) * 4;
     const float4 v = row < rows ? loaded[n] : make_float4(0.f, 0.f, 0.f, 0.f);
-    // NaN counts as infinite: fmaxf would drop it.
-    const float m = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
-    top = v.x + v.y + v.z + v.w == v.x + v.y + v.z + v.w ? fmaxf(top, m) : INFINITY;
+    of.take(v);
     *reinterpret_cast<float4*>(x + row * kStride<NB> + c) = v;
   }
-  return top;
+  return of;
 }
 
 // The forward pass's workspace: per batch and key head and block of 32 keys the
-// tile [K rows | V columns | exponents of K, V].
+// tile [K rows | V columns | exponents of K, V]; then the blocks' ranges; then
+// the parts, where there is more than one.
 template <int NB>
 constexpr int kForwardTile = kRowBytes<NB> + kColBytes<NB> + kTail;
+
+template <int NB>
+__device__ inline Ranges* forward_ranges(char* ws, size_t key_blocks) {
+  return reinterpret_cast<Ranges*>(ws + key_blocks * kForwardTile<NB>);
+}
 
 // Keys and values cut once per call: one workgroup per block and matrix.
 // Every query tile of a head reads them, so the main loop only copies.
 template <int NB>
 __device__ inline void pack_keys(const float* k, const float* v, const int* lengths, char* ws, int B, int Sk, int Hk,
                                  int D) {
-  __shared__ float x[kBlock * kStride<NB>];
-  __shared__ float tops[4];
+  __shared__ __attribute__((aligned(16))) float x[kBlock * kStride<NB>];
+  __shared__ float tops[8];
+  __shared__ RangeSpace ranges;
   const int blocks = (Sk + kBlock - 1) / kBlock;
   const bool values = blockIdx.x % 2;
   const size_t block = blockIdx.x / 2;  // (b, hk, kb)
@@ -245,14 +430,20 @@ __device__ inline void pack_keys(const float* k, const float* v, const int* leng
   const int keys = lengths ? min(max(lengths[b], 0), Sk) : Sk;
   if (kb * kBlock >= keys) return;
   const size_t at = (static_cast<size_t>(b) * Sk + kb * kBlock) * Hk * D + static_cast<size_t>(hk) * D;
-  const float top = block_max(
-      load_block<NB>((values ? v : k) + at, static_cast<size_t>(Hk) * D, min(kBlock, keys - kb * kBlock), D, x), tops);
-  const int e = block_exponent(top);
+  Extremes of = load_block<NB>((values ? v : k) + at, static_cast<size_t>(Hk) * D, min(kBlock, keys - kb * kBlock), D, x);
+  of.join(tops);
+  const int e = block_exponent(of.top);
   const float scale = block_scale(e);
   char* tile = ws + block * kForwardTile<NB>;
+  // Keys are multiplied into scores, which only their largest number bounds.
+  const Range range = values ? block_range<NB>(x, of.top, of.least, ranges, D) : top_range(of.top);
   if (values) write_cols<NB>(x, scale, tile + kRowBytes<NB>);
   else write_rows<NB>(x, scale, tile);
-  if (threadIdx.x == 0) reinterpret_cast<int*>(tile + kRowBytes<NB> + kColBytes<NB>)[values] = e;
+  if (threadIdx.x == 0) {
+    reinterpret_cast<int*>(tile + kRowBytes<NB> + kColBytes<NB>)[values] = e;
+    Range* of_block = &forward_ranges<NB>(ws, static_cast<size_t>(B) * Hk * blocks)[block].first;
+    of_block[values] = range;
+  }
 }
 
 // Copies `Bytes` (a multiple of 1 KiB), contiguous, into LDS without passing
@@ -292,7 +483,7 @@ struct RunningScale {
   __device__ int take(int e, int* behind) {
     int change = 0;
     *behind = 0;
-    if (e >= kZeroExponent / 2) return 0;  // with another exponent added or not
+    if (e >= kNoExponent) return 0;
     if (!any) {
       any = true;
       ref = least = e;
@@ -384,6 +575,69 @@ __device__ inline void store_columns(float* row, int n, int half, int D, const f
       for (int i = 0; i < 4; i++)
         if (c + i < D) row[c + i] = v[i];
     }
+  }
+}
+
+// ── products in float32 ─────────────────────────────────────────────────────
+// What uneven operands take: float32 matrix products of 32 x 32 x 2, with
+// operands loaded as they are, by waves that share nothing. Lane l has row (or
+// column) l % 32 of an operand and terms 4 (l / 32) .. + 3 of every eight; results
+// lie as those of cut operands do. Right, not fast, in as few registers as the
+// loops over even blocks leave: with one value 10^8 times the others 4096 causal
+// tokens, 32 heads of 128 over 8, take 2.4 ms instead of 0.4, and 8192 with
+// gradients, 16 heads over 4, 34 ms instead of 3.4; with such a gradient in every
+// 20th block of queries 11 ms. Looking for it costs even operands 0 to 3 in 100.
+
+// The kernel's arguments, read again: held in registers through the loops over
+// even blocks they would be spilled there.
+struct ForwardArgs {
+  float* y;
+  const float *q, *k, *v;
+};
+struct GradArgs {
+  float* dq;
+  const float *q, *k, *v, *y, *g, *stats;
+};
+template <class Args>
+__device__ inline const Args* args_again() {
+  auto p = __builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return (const Args*)p;  // of the constant address space
+}
+
+// Products of two rows of D numbers.
+template <int NB>
+__device__ inline floatx16 exact_dots(const float* a, const float* b, int D) {
+  const int half = threadIdx.x % 64 / 32;
+  floatx16 x = {};
+#pragma unroll 1
+  for (int c = 4 * half; c < NB * 32; c += 8) {
+    const float4 av = load4(a, c, D), bv = load4(b, c, D);
+    x = __builtin_amdgcn_mfma_f32_32x32x2f32(av.x, bv.x, x, 0, 0, 0);
+    x = __builtin_amdgcn_mfma_f32_32x32x2f32(av.y, bv.y, x, 0, 0, 0);
+    x = __builtin_amdgcn_mfma_f32_32x32x2f32(av.z, bv.z, x, 0, 0, 0);
+    x = __builtin_amdgcn_mfma_f32_32x32x2f32(av.w, bv.w, x, 0, 0, 0);
+  }
+  return x;
+}
+
+// o += X^T p with the first `rows` of 32 rows of X, multiplied by `times(row)`
+// 2^e, and p as a product leaves it: 0 for the rows past them, for which the
+// last is read again. Columns past D are any.
+template <int NB, class Times>
+__device__ inline void exact_outer(floatx16 (&o)[NB], const float* x, size_t stride, int rows, int D, const floatx16& p,
+                                   int e, Times times) {
+  const int column = threadIdx.x % 32, half = threadIdx.x % 64 / 32;
+  asm volatile("" : "+s"(rows));  // or the caller's sixteen numbers of rows stay in registers
+#pragma unroll
+  for (int r = 0; r < 16; r++) {
+    const int row = result_row(r, half);
+    const float* at = x + min(row, rows - 1) * stride;
+    const float by = times(min(row, rows - 1));
+#pragma unroll
+    for (int n = 0; n < NB; n++)
+      o[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(ldexpf(at[min(32 * n + column, D - 1)] * by, e), p[r], o[n], 0, 0, 0);
+    if (r % 2) __builtin_amdgcn_sched_barrier(0);  // few loads in flight: the even blocks' registers are not to be more for these
   }
 }
 
@@ -529,6 +783,7 @@ __device__ inline void forward_tiles(float* __restrict__ y, const float* __restr
   // knows that what a step reads is not what its copies write, and does not
   // wait for them first.
   __shared__ __attribute__((aligned(1024))) char even[kTile], odd[kTile];
+  __shared__ int uneven[4];
   int qt, h, b, split;
   query_tile(s, 128, splits, blockIdx.x, &qt, &h, &b, &split);
   const int hk = h / (s.hq / s.hk);
@@ -550,14 +805,78 @@ __device__ inline void forward_tiles(float* __restrict__ y, const float* __restr
   const char* tile = ws + head * head_blocks * kTile;
   if (begin < end) copy_tile<kTile, 4>(tile + static_cast<size_t>(begin) * kTile, even);
 
+  const size_t tiles = static_cast<size_t>(s.b) * s.hk * head_blocks;
+  const float* q_row = q + (static_cast<size_t>(b) * s.sq + min(i, s.sq - 1)) * s.hq * s.d + static_cast<size_t>(h) * s.d;
   half8 qh[NB * 2], ql[NB * 2];
-  const int eq = row_fragments<NB>(q + (static_cast<size_t>(b) * s.sq + min(i, s.sq - 1)) * s.hq * s.d + static_cast<size_t>(h) * s.d,
-                                   live, s.d, scale < 0.f ? -1.f : 1.f, 1.f, qh, ql);
+  const int eq = row_fragments<NB>(q_row, live, s.d, scale < 0.f ? -1.f : 1.f, 1.f, qh, ql);
+  const Ranges seen_keys = widest_of(forward_ranges<NB>(ws, tiles) + head * head_blocks, blocks);
+  if (lane == 0) uneven[wave] = 0;
+  // The query's largest number is below 2^(15 - eq).
+  if (__any(eq < kNoExponent && 15 - eq + seen_keys.first[0] + score_exponent(scale, s.d) > kMostScore) ||
+      spread(seen_keys.second) > kSpread)
+    uneven[wave] = 1;
   const float factor = fabsf(scale) * kLog2e;
   float m = -INFINITY, l = 0.f;
   floatx16 o[NB] = {};
   RunningScale vs;
   tile_barrier();
+  const bool exact = uniform(uneven[0] | uneven[1] | uneven[2] | uneven[3]) != 0;
+  auto finish = [&](int exponent) {
+    l = halves_sum(l);
+    if (!live) return;
+    const size_t stat = (static_cast<size_t>(b) * s.hq + h) * s.sq + i, rows = static_cast<size_t>(s.b) * s.hq * s.sq;
+    if (splits > 1) {
+      const RowParts parts = row_parts(reinterpret_cast<char*>(forward_ranges<NB>(ws, tiles) + tiles), s, splits);
+      const size_t out = split * rows + stat;
+#pragma unroll
+      for (int n = 0; n < NB; n++) store_columns(parts.o + out * s.d, n, half, s.d, o[n], 1.f, exponent);
+      if (half == 0) {
+        parts.ml[2 * out] = m;
+        parts.ml[2 * out + 1] = l;
+      }
+      return;
+    }
+    const float inv = inverse_sum(l);
+    float* row = y + (static_cast<size_t>(b) * s.sq + i) * s.hq * s.d + static_cast<size_t>(h) * s.d;
+#pragma unroll
+    for (int n = 0; n < NB; n++) store_columns(row, n, half, s.d, o[n], inv, exponent);
+    if (half == 0) {
+      stats[stat] = m == -INFINITY ? 0.f : m;
+      stats[rows + stat] = inv;
+    }
+  };
+  if (__builtin_expect(exact, 0)) {
+    const size_t stride = static_cast<size_t>(s.hk) * s.d, of_head = static_cast<size_t>(b) * s.sk * stride + static_cast<size_t>(hk) * s.d;
+    const auto* again = args_again<ForwardArgs>();
+    const float *k = again->k, *v = again->v;
+    for (int kb = begin; kb < min(end, wave_end); kb++) {
+      const size_t at = of_head + static_cast<size_t>(kb) * kBlock * stride;
+      const int rows = min(kBlock, keys - kb * kBlock);
+      floatx16 x = exact_dots<NB>(k + at + min(lane % 32, rows - 1) * stride, q_row, s.d);
+      float top = m;
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        x[r] = kb * kBlock + result_row(r, half) < seen ? x[r] * (scale * kLog2e) : -INFINITY;
+        top = fmaxf(top, x[r]);
+      }
+      top = halves_max(top);
+      const float base = top == -INFINITY ? 0.f : top, old = exp2f(m - base);
+      m = top;
+      l *= old;
+#pragma unroll
+      for (int n = 0; n < NB; n++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) o[n][r] *= old;
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        x[r] = exp2f(x[r] - base);
+        l += x[r];
+      }
+      exact_outer<NB>(o, v + at, stride, rows, s.d, x, 0, [](int) { return 1.f; });
+    }
+    finish(0);
+    return;
+  }
   auto step = [&](const char* now, char* next, int kb) {
     if (kb + 1 < end) copy_tile<kTile, 4>(tile + static_cast<size_t>(kb + 1) * kTile, next);
     if (kb < wave_end) {
@@ -626,28 +945,7 @@ __device__ inline void forward_tiles(float* __restrict__ y, const float* __restr
     step(even, odd, kb);
     if (kb + 1 < end) step(odd, even, kb + 1);
   }
-  l = halves_sum(l);
-  if (!live) return;
-  const size_t stat = (static_cast<size_t>(b) * s.hq + h) * s.sq + i, rows = static_cast<size_t>(s.b) * s.hq * s.sq;
-  if (splits > 1) {
-    const RowParts parts = row_parts(ws + static_cast<size_t>(s.b) * s.hk * head_blocks * kTile, s, splits);
-    const size_t out = split * rows + stat;
-#pragma unroll
-    for (int n = 0; n < NB; n++) store_columns(parts.o + out * s.d, n, half, s.d, o[n], 1.f, -kProbShift - vs.ref);
-    if (half == 0) {
-      parts.ml[2 * out] = m;
-      parts.ml[2 * out + 1] = l;
-    }
-    return;
-  }
-  const float inv = inverse_sum(l);
-  float* row = y + (static_cast<size_t>(b) * s.sq + i) * s.hq * s.d + static_cast<size_t>(h) * s.d;
-#pragma unroll
-  for (int n = 0; n < NB; n++) store_columns(row, n, half, s.d, o[n], inv, -kProbShift - vs.ref);
-  if (half == 0) {
-    stats[stat] = m == -INFINITY ? 0.f : m;
-    stats[rows + stat] = inv;
-  }
+  finish(-kProbShift - vs.ref);
 }
 
 // ── gradients ───────────────────────────────────────────────────────────────
@@ -665,9 +963,10 @@ constexpr int kScoreShift = 12;  // 15, less kLazy and one for the twice
 // The gradients' workspace. Per batch and key head and block of 32 keys: the
 // tile [K rows | V rows | K columns | exponents of K, V]; per batch and query
 // head and block of 32 queries: the tile [Q rows | G rows | Q columns | G
-// columns | m, delta of each row, exponents of Q, G and of G's largest row
-// norm] (G = g'); then the exponents of the key blocks' largest row norms of V;
-// then dk and dv of each part of the queries, and dq of each part of the keys,
+// columns | m, delta of each row, exponents of Q, G (kUneven more where the block
+// is uneven in itself) and of G's largest row norm] (G = g'); then the ranges of
+// the key blocks and of the query blocks; then the exponents of the key blocks'
+// largest row norms of V; then dk and dv of each part of the queries, and dq of each part of the keys,
 // where there is more than one.
 template <int NB>
 constexpr int kKeyTile = 2 * kRowBytes<NB> + kColBytes<NB> + kTail;
@@ -677,6 +976,7 @@ constexpr int kQueryTile = 2 * kRowBytes<NB> + 2 * kColBytes<NB> + kTail;
 struct GradSpace {
   int k_blocks, q_blocks;
   char *k_tiles, *q_tiles;
+  Ranges *k_ranges, *q_ranges;
   int* norms;
   float* parts;
 };
@@ -689,7 +989,9 @@ __device__ inline GradSpace grad_space(char* ws, const Shape& s) {
   const size_t nk = static_cast<size_t>(s.b) * s.hk * g.k_blocks, nq = static_cast<size_t>(s.b) * s.hq * g.q_blocks;
   g.k_tiles = ws;
   g.q_tiles = ws + nk * kKeyTile<NB>;
-  g.norms = reinterpret_cast<int*>(g.q_tiles + nq * kQueryTile<NB>);
+  g.k_ranges = reinterpret_cast<Ranges*>(g.q_tiles + nq * kQueryTile<NB>);
+  g.q_ranges = g.k_ranges + nk;
+  g.norms = reinterpret_cast<int*>(g.q_ranges + nq);
   g.parts = reinterpret_cast<float*>(g.norms + (nk + 3) / 4 * 4);
   return g;
 }
@@ -723,7 +1025,8 @@ __device__ inline void pack_grad(const float* __restrict__ q, const float* __res
                                  const float* __restrict__ stats, const int* __restrict__ lengths,
                                  char* __restrict__ ws, const Shape& s) {
   __shared__ __attribute__((aligned(16))) float x[kBlock * kStride<NB>];
-  __shared__ float tops[4];
+  __shared__ float tops[8];
+  __shared__ RangeSpace ranges;
   const GradSpace f = grad_space<NB>(ws, s);
   const size_t nk = static_cast<size_t>(s.b) * s.hk * f.k_blocks;
   const bool second = blockIdx.x % 2;  // V, or G
@@ -749,7 +1052,7 @@ __device__ inline void pack_grad(const float* __restrict__ q, const float* __res
     m = stats[stat];
     inv = stats[static_cast<size_t>(s.b) * s.hq * s.sq + stat];
   }
-  float top = load_block<NB>(src, stride, min(kBlock, rows - at), s.d, x);
+  Extremes of = load_block<NB>(src, stride, min(kBlock, rows - at), s.d, x);
   char* tile = of_keys ? f.k_tiles + block * kKeyTile<NB> : f.q_tiles + block * kQueryTile<NB>;
   char* tail = tile + (of_keys ? kKeyTile<NB> : kQueryTile<NB>) - kTail;
   int* exponents = reinterpret_cast<int*>(tail) + (of_keys ? 0 : 64);
@@ -758,55 +1061,53 @@ __device__ inline void pack_grad(const float* __restrict__ q, const float* __res
     // g' and delta; rows past the last query stay 0.
     __syncthreads();
     float delta = 0.f;
-    top = 0.f;
+    of = Extremes();
 #pragma unroll
     for (int n = 0; n < NB; n++) {
       float4 gx = mine[8 * n];
       gx = live ? make_float4(gx.x * inv, gx.y * inv, gx.z * inv, gx.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f);
       mine[8 * n] = gx;
-      const float of[4] = {gx.x, gx.y, gx.z, gx.w};
-#pragma unroll
-      for (int i = 0; i < 4; i++) top = of[i] == of[i] ? fmaxf(top, fabsf(of[i])) : INFINITY;
+      of.take(gx);
       if (live) delta += gx.x * yv[n].x + gx.y * yv[n].y + gx.z * yv[n].z + gx.w * yv[n].w;
     }
-    delta += __shfl_xor(delta, 1);
-    delta += __shfl_xor(delta, 2);
-    delta += __shfl_xor(delta, 4);
+    delta = sum8(delta);
     if (part == 0) {
       reinterpret_cast<float*>(tail)[row] = live ? m : 0.f;
       reinterpret_cast<float*>(tail)[32 + row] = delta;
     }
   }
-  const int e = block_exponent(block_max(top, tops));
+  of.join(tops);
+  const int e = block_exponent(of.top);
   const float scale = block_scale(e);
+  const Range range = block_range<NB>(x, of.top, of.least, ranges, s.d);
   if (second) {
     float squares = 0.f;
 #pragma unroll
     for (int n = 0; n < NB; n++) {
       const float4 v = mine[8 * n];
-      const float of[4] = {v.x * scale, v.y * scale, v.z * scale, v.w * scale};
+      const float a[4] = {v.x * scale, v.y * scale, v.z * scale, v.w * scale};
 #pragma unroll
-      for (int i = 0; i < 4; i++) squares += of[i] * of[i];
+      for (int i = 0; i < 4; i++) squares += a[i] * a[i];
     }
-    squares += __shfl_xor(squares, 1);
-    squares += __shfl_xor(squares, 2);
-    squares += __shfl_xor(squares, 4);
+    squares = sum8(squares);
     __syncthreads();  // tops is read
     squares = block_max(squares, tops);
     if (threadIdx.x == 0) *(of_keys ? f.norms + block : exponents + 2) = norm_exponent(squares, e);
   }
-  if (threadIdx.x == 0) exponents[second] = e;
+  if (threadIdx.x == 0) {
+    exponents[second] = e + (!of_keys && spread(range) > kSpread ? kUneven : 0);
+    (&(of_keys ? f.k_ranges : f.q_ranges)[block].first)[second] = range;
+  }
   write_rows<NB>(x, scale, tile + (second ? kRowBytes<NB> : 0));
   if (of_keys && !second) write_cols<NB>(x, scale, tile + 2 * kRowBytes<NB>);
   if (!of_keys) write_cols<NB>(x, scale, tile + 2 * kRowBytes<NB> + (second ? kColBytes<NB> : 0));
 }
 
-// The exponent above the norms of every value row of a head.
+// The exponent above the norms of the value rows of a head's first blocks.
 __device__ inline int values_norm(const int* norms, int blocks) {
   int top = -120;
   for (int n = threadIdx.x % 64; n < blocks; n += 64) top = max(top, norms[n]);
-  for (int d = 32; d > 0; d /= 2) top = max(top, __shfl_xor(top, d));
-  return __builtin_amdgcn_readfirstlane(top);
+  return __builtin_amdgcn_readfirstlane(join_wave(top, [](int a, int b) { return max(a, b); }));
 }
 
 __device__ inline int clamp_power(int a) { return min(max(a, -120), 120); }
@@ -853,14 +1154,47 @@ __device__ inline void query_grads(float* __restrict__ dq, const float* __restri
   const float m = live ? stats[stat] : 0.f;
   const char* q_tail = f.q_tiles + (q_block + 1) * kQueryTile<NB> - kTail;
   const float delta = reinterpret_cast<const float*>(q_tail)[32 + lane % 32];
-  half8 qh[NB * 2], ql[NB * 2], gh[NB * 2], gl[NB * 2];
-  const int eq = row_fragments<NB>(q + at, live, s.d, scale < 0.f ? -1.f : 1.f, 1.f, qh, ql);
-  const int eg = row_fragments<NB>(g + at, live, s.d, 1.f, inv, gh, gl);
+  // Whether the keys and values that the workgroup's queries see are even, and
+  // their own blocks.
   const int shift = uniform(clamp_power(kScoreShift - reinterpret_cast<const int*>(q_tail)[66] -
-                                        values_norm(f.norms + head * f.k_blocks, (keys + kBlock - 1) / kBlock)));
+                                        values_norm(f.norms + head * f.k_blocks, blocks)));
+  const Ranges seen_keys = widest_of(f.k_ranges + head * f.k_blocks, blocks);
+  const int own = (static_cast<size_t>(qt) * kRows) / kBlock;
+  const Ranges of_rows = widest_of(f.q_ranges + (static_cast<size_t>(b) * s.hq + h) * f.q_blocks + own, min(Waves, f.q_blocks - own));
+  const bool exact = max(spread(seen_keys.first), max(spread(seen_keys.second), spread(of_rows.second))) > kSpread ||
+                     of_rows.first[0] + seen_keys.first[0] + score_exponent(scale, s.d) > kMostScore;
   const float factor = fabsf(scale) * kLog2e;
   floatx16 o[NB] = {};
   RunningScale ks;
+  auto store = [&](int exponent) {
+    if (!live) return;
+    float* out = dq;
+    if (q_parts > 1) out = f.parts + key_parts(s, parts) + part * (static_cast<size_t>(s.b) * s.sq * s.hq * s.d);
+#pragma unroll
+    for (int n = 0; n < NB; n++) store_columns(out + at, n, half, s.d, o[n], scale, exponent);
+  };
+  if (__builtin_expect(exact, 0)) {
+    tile_barrier();
+    const size_t stride = static_cast<size_t>(s.hk) * s.d, of_head = static_cast<size_t>(b) * s.sk * stride + static_cast<size_t>(hk) * s.d;
+    const auto* again = args_again<GradArgs>();
+    const float *k = again->k, *v = again->v;
+    for (int kb = begin; kb < min(end, wave_end); kb++) {
+      const size_t from = of_head + static_cast<size_t>(kb) * kBlock * stride;
+      const int rows = min(kBlock, keys - kb * kBlock);
+      const size_t key = min(lane % 32, rows - 1) * stride;
+      const floatx16 x = exact_dots<NB>(k + from + key, q + at, s.d);
+      floatx16 ds = exact_dots<NB>(v + from + key, g + at, s.d);
+#pragma unroll
+      for (int r = 0; r < 16; r++)
+        ds[r] = kb * kBlock + result_row(r, half) < seen ? exp2f(fmaf(x[r], scale * kLog2e, -m)) * fmaf(ds[r], inv, -delta) : 0.f;
+      exact_outer<NB>(o, k + from, stride, rows, s.d, ds, 0, [](int) { return 1.f; });
+    }
+    store(0);
+    return;
+  }
+  half8 qh[NB * 2], ql[NB * 2], gh[NB * 2], gl[NB * 2];
+  const int eq = row_fragments<NB>(q + at, live, s.d, scale < 0.f ? -1.f : 1.f, 1.f, qh, ql);
+  const int eg = row_fragments<NB>(g + at, live, s.d, 1.f, inv, gh, gl);
   tile_barrier();
   auto step = [&](const char* now, char* next, int kb) {
     if (kb + 1 < end) copy_tile<kTile, Waves>(tile + static_cast<size_t>(kb + 1) * kTile, next);
@@ -914,10 +1248,7 @@ __device__ inline void query_grads(float* __restrict__ dq, const float* __restri
     step(even, odd, kb);
     if (kb + 1 < end) step(odd, even, kb + 1);
   }
-  if (!live) return;
-  if (q_parts > 1) dq = f.parts + key_parts(s, parts) + part * (static_cast<size_t>(s.b) * s.sq * s.hq * s.d);
-#pragma unroll
-  for (int n = 0; n < NB; n++) store_columns(dq + at, n, half, s.d, o[n], scale, -shift - ks.ref);
+  store(-shift - ks.ref);
 }
 
 // dk and dv. A workgroup: 128 keys of one key head over its part of the query
@@ -1032,6 +1363,12 @@ __device__ inline void key_grads(float* __restrict__ dk, float* __restrict__ dv,
   half8 fh[NB * 2], fl[NB * 2];  // K for the probabilities (its sign with scale's), V for ds
   const int e = row_fragments<NB>((of_keys ? v : k) + at, live, s.d, !of_keys && scale < 0.f ? -1.f : 1.f, 1.f, fh, fl);
   const int norm = values_norm(f.norms + (static_cast<size_t>(b) * s.hk + hk) * f.k_blocks, (keys + kBlock - 1) / kBlock);
+  // Whether all of the head's keys and values and of the group's queries and
+  // gradients take float32 products, or some blocks of queries.
+  const Ranges of_head = widest_of(f.k_ranges + (static_cast<size_t>(b) * s.hk + hk) * f.k_blocks, (keys + kBlock - 1) / kBlock);
+  const Tops of_rows = tops_of(f.q_ranges + q_head, group * f.q_blocks);
+  const bool exact = spread(of_head.second) > kSpread || spread(of_rows.first) > kSpread || spread(of_rows.second) > kGradSpread ||
+                     of_rows.first[0] + of_head.first[0] + score_exponent(scale, s.d) > kMostScore;
   const float factor = fabsf(scale) * kLog2e;
   floatx16 o[NB] = {};
   RunningScale qs, gs;
@@ -1050,12 +1387,18 @@ __device__ inline void key_grads(float* __restrict__ dk, float* __restrict__ dv,
       copy_rows(next, next_rows);
       copy_cols(next, next_cols);
     }
-    // Whether any of the block's queries sees any of the wave's keys.
-    const bool any = first < keys && (!s.causal || first <= q0 + kBlock - 1 + offset);
     const char* t = rows + lane * 16 + (of_keys ? kRowBytes<NB> : 0);
     const float* tail = reinterpret_cast<const float*>(rows + 2 * kRowBytes<NB>);
     const int* exponents = reinterpret_cast<const int*>(tail) + 64;
     const int eq = uniform(exponents[0]), eg = uniform(exponents[1]), shift = clamp_power(kScoreShift - uniform(exponents[2]) - norm);
+    // Whether any of the block's queries sees any of the wave's keys, and it is
+    // not among the uneven ones. (Only where there are some does the step wait for
+    // the exponents here.)
+    bool any = first < keys && (!s.causal || first <= q0 + kBlock - 1 + offset);
+    if (__builtin_expect(of_rows.uneven, 0)) {
+      asm volatile("");
+      any = any && max(eq, eg) < kUneven / 2;
+    }
     // m for the probabilities, delta for ds.
     float4 of_row[4];
 #pragma unroll
@@ -1135,25 +1478,84 @@ __device__ inline void key_grads(float* __restrict__ dk, float* __restrict__ dv,
     if (!kTwo && more) copy_cols(next, next_cols);
   };
   if constexpr (kTwo) {
-    for (int u = part; u < units; u += 2 * parts) {
+    for (int u = exact ? units : part; u < units; u += 2 * parts) {
       step(rows_a, cols_a, rows_b, cols_b, u);
       if (u + parts < units) step(rows_b, cols_b, rows_a, cols_a, u + parts);
     }
   } else {
-    for (int u = part; u < units; u += parts) step(rows_a, cols_a, rows_a, cols_a, u);
+    for (int u = exact ? units : part; u < units; u += parts) step(rows_a, cols_a, rows_a, cols_a, u);
   }
-  if (j >= s.sk) return;
+  if (exact) gs.ref = -kProbShift;  // sums as they are
+  if (exact || of_rows.uneven) {
+    // All blocks of queries, or those that are uneven in themselves, by waves
+    // that share nothing: both of a pair make the probabilities. Sums keep the
+    // scales that they have from the even blocks.
+    const auto* again = args_again<GradArgs>();
+    const float *q = again->q, *k = again->k, *v = again->v, *g = again->g, *stats = again->stats;
+    const size_t q_stride = static_cast<size_t>(s.hq) * s.d;
+    for (int u = part; u < units; u += parts) {
+      const int block = f.q_blocks - 1 - u / group, h = hk * group + u % group, q0 = block * kBlock, rows = min(kBlock, s.sq - q0);
+      const float* tail = reinterpret_cast<const float*>(unit_tile(u / group, u % group) + kTile - kTail);
+      const int* exponents = reinterpret_cast<const int*>(tail) + 64;
+      const int eq = uniform(exponents[0]), eg = uniform(exponents[1]);
+      if (!exact && max(eq, eg) < kUneven / 2) continue;
+      if (first >= keys || (s.causal && first > q0 + kBlock - 1 + offset)) continue;
+      const size_t q_at = (static_cast<size_t>(b) * s.sq + q0) * q_stride + static_cast<size_t>(h) * s.d;
+      // A row's and the key's places, made where they are used.
+      auto row = [&] {
+        int thread = threadIdx.x;
+        asm volatile("" : "+v"(thread));
+        return min(thread % 32, rows - 1) * q_stride;
+      };
+      const float* inv = stats + (static_cast<size_t>(s.b) * s.hq + static_cast<size_t>(b) * s.hq + h) * s.sq + q0;
+      int change = 0, behind, shift = 0;
+      if (!exact) {
+        shift = clamp_power(kScoreShift - uniform(exponents[2]) - norm);
+        change = of_keys ? qs.take(shift + (eq < kUneven / 2 ? eq : eq - kUneven), &behind)
+                         : gs.take(eg < kUneven / 2 ? eg : eg - kUneven, &behind);
+      }
+#pragma unroll
+      for (int n = 0; n < NB; n++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) o[n][r] = ldexpf(o[n][r], change);
+      floatx16 x = exact_dots<NB>(q + q_at + row(), k + at, s.d);
+      __builtin_amdgcn_sched_barrier(0);
+      auto seen = [&](int i) { return i < rows && (!s.causal || j <= q0 + i + offset); };
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        const int i = result_row(r, half);
+        x[r] = seen(i) ? exp2f(fmaf(x[r], scale * kLog2e, -tail[i])) : 0.f;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (of_keys) {
+        floatx16 ds = exact_dots<NB>(g + q_at + row(), v + at, s.d);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          const int i = result_row(r, half);
+          ds[r] = seen(i) ? ldexpf(x[r] * fmaf(ds[r], inv[min(i, rows - 1)], -tail[32 + i]), shift) : 0.f;
+        }
+        exact_outer<NB>(o, q + q_at, q_stride, rows, s.d, ds, qs.ref - shift, [](int) { return 1.f; });
+      } else {
+        exact_outer<NB>(o, g + q_at, q_stride, rows, s.d, x, gs.ref + kProbShift, [&](int i) { return inv[i]; });
+      }
+    }
+  }
+  int thread = threadIdx.x;
+  asm volatile("" : "+v"(thread));  // the key's place is made again: held through the uneven blocks it would be spilled
+  const int key = first + thread % 32;
+  if (key >= s.sk) return;
   const size_t all = static_cast<size_t>(s.b) * s.sk * s.hk * s.d;
   float* out = of_keys ? dk : dv;
   if (parts > 1) out = f.parts + 2 * all * part + (of_keys ? 0 : all);
   // Keys past the length take no gradient (their lanes' sums are not of it).
-  if (!live) {
+  if (key >= keys) {
 #pragma unroll
     for (int n = 0; n < NB; n++) o[n] = floatx16{};
   }
 #pragma unroll
   for (int n = 0; n < NB; n++)
-    store_columns(out + at, n, half, s.d, o[n], of_keys ? scale : 1.f, of_keys ? -qs.ref : -kProbShift - gs.ref);
+    store_columns(out + (static_cast<size_t>(b) * s.sk + key) * s.hk * s.d + static_cast<size_t>(hk) * s.d, n, thread % 64 / 32, s.d, o[n], of_keys ? scale : 1.f, of_keys ? -qs.ref : -kProbShift - gs.ref);
 }
 
 // Sums of parts, in order: element e of two arrays of n in a row.
@@ -1379,7 +1781,7 @@ __device__ inline void token(float* __restrict__ y, const float* __restrict__ q,
   extern "C" __global__ void __launch_bounds__(256) fg_attention_pack_##NB(FG_ARGS) {                            \
     pack_keys<NB>(k, v, lengths, ws, B, Sk, Hk, D);                                                              \
   }                                                                                                              \
-  extern "C" __global__ void __launch_bounds__(256, 2) fg_attention_tiles_##NB(FG_ARGS) {                        \
+  extern "C" __global__ void __launch_bounds__(256, (NB) < 4 ? 6 - (NB) : 2) fg_attention_tiles_##NB(FG_ARGS) {                        \
     forward_tiles<NB>(y, q, stats, lengths, ws, FG_SHAPE, scale, splits);                                        \
   }                                                                                                              \
   extern "C" __global__ void __launch_bounds__(256) fg_attention_grad_pack_##NB(FG_GRAD_ARGS) {                  \
@@ -1419,7 +1821,7 @@ FG_ATTENTION(4)
 // one of each kind (with the kinds in turn, 16 heads of 32 over 2048 tokens took
 // 229 us with their forward pass instead of 189). Both share the two buffers.
 #define FG_ATTENTION_GRADS(NB)                                                                                   \
-  extern "C" __global__ void __launch_bounds__(512, 2) fg_attention_grads_##NB(FG_GRAD_ARGS) {                   \
+  extern "C" __global__ void __launch_bounds__(512, (NB) < 2 ? 4 : 2) fg_attention_grads_##NB(FG_GRAD_ARGS) {                   \
     constexpr int kOdd = kGradCols<NB> + 4 * static_cast<int>(sizeof(Probs)), kTile = kKeyTile<NB>;              \
     constexpr int Waves = kQueryGradWaves<NB>;                                                                   \
     __shared__ __attribute__((aligned(1024))) char even[kTile > kGradRows<NB> ? kTile : kGradRows<NB>];          \

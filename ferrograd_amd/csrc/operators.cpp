@@ -206,6 +206,7 @@ RenderedKernel render_norm_rotate(const UOp& call, bool grad) {
 constexpr double kForwardUnit[] = {1.2, 1.7, 2.3, 3.0}, kKeyUnit[] = {2.7, 3.6, 2.8, 3.3}, kQueryUnit[] = {1.4, 2.3, 3.3, 4.0};
 constexpr double kForwardAlone = 0.75, kGradAlone = 0.72;
 constexpr int64_t kUnits = 256;   // compute units
+constexpr int64_t kRangeBytes = 8;  // of a block of cut operands: its ranges
 constexpr double kSumLaunch = 8;  // us of a launch that joins parts, beside its bytes
 
 // One kind of workgroups of a launch: `tiles` of them, each over `units` blocks
@@ -310,7 +311,7 @@ RenderedKernel render_attention(const UOp& call, bool grad) {
       units = 0;
       splits = split.parts;
       const uint64_t key_blocks = static_cast<uint64_t>(batch * kv_heads * k_blocks);
-      tile_bytes = key_blocks * static_cast<uint64_t>(nb * 8192 + 1024);
+      tile_bytes = key_blocks * static_cast<uint64_t>(nb * 8192 + 1024 + kRangeBytes);
       rk.launches = {launch("fg_attention_pack_" + std::to_string(nb), 2 * key_blocks, 256, "attention"),
                      launch("fg_attention_tiles_" + std::to_string(nb), static_cast<uint64_t>(tiles * splits), 256, "attention")};
     }
@@ -370,7 +371,7 @@ RenderedKernel render_attention(const UOp& call, bool grad) {
         }
     }
     const uint64_t summed = std::max(parts > 1 ? 2 * all_k : 0, q_parts > 1 ? all_q : 0);
-    rk.workspace_bytes = nk * static_cast<uint64_t>(nb * 12288 + 1024) + nq * static_cast<uint64_t>(nb * 16384 + 1024) +
+    rk.workspace_bytes = nk * static_cast<uint64_t>(nb * 12288 + 1024 + kRangeBytes) + nq * static_cast<uint64_t>(nb * 16384 + 1024 + kRangeBytes) +
                          (nk + 3) / 4 * 16 + (parts > 1 ? 8 * all_k * static_cast<uint64_t>(parts) : 0) +
                          (q_parts > 1 ? 4 * all_q * static_cast<uint64_t>(q_parts) : 0);
     rk.launches = {launch("fg_attention_grad_pack" + nbs, 2 * (nk + nq), 256, "attention")};

@@ -219,3 +219,130 @@ def test_values_of_zero_beside_large_ones_take_their_probability(fg, hip, size, 
     got, want = run_both(fg, q, k, v, g, **kw), attention_ref.attention(q, k, v, g=g, **kw)
     for name in want:
         check(name, got[name], *want[name])
+
+
+# What a query does not see, or weighs with nothing, and columns beside large
+# ones: each against the call without the large numbers, whose values and bounds
+# are those of numbers of one size.
+
+UNLIKE = {  # batch, sq, sk, heads, kv_heads, dim
+    "small": (1, 100, 100, 2, 1, 24),
+    "large": (4, 130, 257, 32, 32, 40),
+    "large in parts": (1, 256, 4000, 16, 8, 64),
+    "wide": (2, 200, 200, 32, 16, 128),
+    "wide and ragged": (2, 300, 300, 16, 16, 100),
+    "narrow": (2, 300, 300, 32, 16, 20),
+}
+
+
+def unlike_inputs(path, seed):
+    batch, sq, sk, heads, kv_heads, dim = UNLIKE[path]
+    return attention_inputs(seed, batch, sq, sk, heads, kv_heads, dim), dict(batch=batch, heads=heads, kv_heads=kv_heads)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [1e6, 1e9, 1e12, 1e20])
+@pytest.mark.parametrize("of", ["k", "v", "kv"])
+@pytest.mark.parametrize("path", UNLIKE)
+def test_a_large_key_or_value_changes_nothing_for_queries_that_do_not_see_it(fg, hip, path, of, size):
+    (q, k, v, g), kw = unlike_inputs(path, 70)
+    batch, sq, sk = UNLIKE[path][:3]
+    at = 3 * sq // 4  # the query that sees it first, and its key
+    want = attention_ref.attention(q, k, v, causal=True, g=g, **kw)
+    g = g.reshape(batch, sq, -1).copy()
+    g[:, at:] = 0  # the others' gradients
+    g = g.reshape(batch * sq, -1)
+    want_grads = attention_ref.attention(q, k, v, causal=True, g=g, **kw)
+    for x, name in ((k, "k"), (v, "v")):
+        if name in of:
+            x.reshape(batch, sk, -1)[:, at + sk - sq] *= np.float32(size)
+    got = run_both(fg, q, k, v, g, causal=True, **kw)
+    rows = (np.arange(batch * sq) % sq) < at
+    check("y", got["y"][rows], *(x[rows] for x in want["y"]))
+    check("dq", got["dq"][rows], *(x[rows] for x in want_grads["dq"]))
+    if "k" not in of:  # a large key makes the probabilities of those that see it what they are not here
+        keys = (np.arange(batch * sk) % sk) < at + sk - sq
+        for name in ("dk", "dv"):
+            check(name, got[name][keys], *(x[keys] for x in want_grads[name]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [1e6, 1e9, 1e12])
+@pytest.mark.parametrize("path", UNLIKE)
+def test_a_value_that_weighs_nothing_changes_nothing(fg, hip, path, size):
+    # Its key scores -10^4 or less, so that its probability is 0 in float32 and
+    # in float64: the call without that key.
+    (q, k, v, g), kw = unlike_inputs(path, 71)
+    batch, sq, sk, heads, kv_heads, dim = UNLIKE[path]
+    q[:, ::dim] = np.abs(q[:, ::dim]) + 0.5
+    at = sk // 3
+    rest = np.arange(batch * sk) % sk != at
+    want = attention_ref.attention(q, k[rest], v[rest], g=g, **kw)
+    k.reshape(batch, sk, kv_heads, dim)[:, at, :, 0] = -4e4 * np.sqrt(dim)
+    v.reshape(batch, sk, -1)[:, at] *= np.float32(size)
+    got = run_both(fg, q, k, v, g, **kw)
+    check("y", got["y"], *want["y"])
+    check("dq", got["dq"], *want["dq"])
+    for name in ("dk", "dv"):
+        check(name, got[name][rest], *want[name])
+        assert not got[name][~rest].any(), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [1e6, 1e9, 1e12])
+@pytest.mark.parametrize("path", UNLIKE)
+def test_columns_beside_a_large_one(fg, hip, path, size):
+    # A column of the values that is large in each head, where the gradient is 0:
+    # the other columns, and the gradients, are as without it. A column of the
+    # keys that is large where the queries are 0, the same.
+    (q, k, v, g), kw = unlike_inputs(path, 72)
+    batch, sq, sk, heads, kv_heads, dim = UNLIKE[path]
+    q[:, 1::dim] = 0
+    g[:, ::dim] = 0
+    want = attention_ref.attention(q, k, v, g=g, **kw)
+    v[:, ::dim] *= np.float32(size)
+    k[:, 1::dim] *= np.float32(size)
+    got = run_both(fg, q, k, v, g, **kw)
+    for name, large in (("y", 0), ("dq", 1), ("dk", None), ("dv", None)):
+        columns = np.arange(got[name].shape[1]) % dim != (-1 if large is None else large)
+        check(name, got[name][:, columns], *(x[:, columns] for x in want[name]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [1e6, 1e9, 1e12])
+@pytest.mark.parametrize("of", ["q", "g"])
+@pytest.mark.parametrize("path", UNLIKE)
+def test_a_large_query_or_gradient_changes_nothing_for_keys_that_it_does_not_see(fg, hip, path, of, size):
+    (q, k, v, g), kw = unlike_inputs(path, 73)
+    batch, sq, sk = UNLIKE[path][:3]
+    at = sq // 3
+    want = attention_ref.attention(q, k, v, causal=True, g=g, **kw)
+    x = {"q": q, "g": g}[of]
+    x.reshape(batch, sq, -1)[:, at] *= np.float32(size)
+    got = run_both(fg, q, k, v, g, causal=True, **kw)
+    keys = (np.arange(batch * sk) % sk) > at + sk - sq
+    rows = (np.arange(batch * sq) % sq) != at
+    for name in ("dk", "dv"):
+        check(name, got[name][keys], *(x[keys] for x in want[name]))
+    for name in ("y", "dq"):
+        check(name, got[name][rows], *(x[rows] for x in want[name]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("path", UNLIKE)
+def test_gradients_that_grow_over_the_sequence(fg, hip, path):
+    # Blocks of queries 2^12 apart, 2^50 and more in all: the last keys are seen
+    # by the last, smallest gradients only.
+    (q, k, v, g), kw = unlike_inputs(path, 74)
+    batch, sq, sk = UNLIKE[path][:3]
+    g = g.reshape(batch, sq, -1)
+    want = attention_ref.attention(q, k, v, causal=True, g=g.reshape(batch * sq, -1), **kw)
+    scale = 2.0 ** (12 * ((sq - 1 - np.arange(sq)) // 32))
+    g = (g * scale[:, None].astype(np.float32)).reshape(batch * sq, -1)
+    got = run_both(fg, q, k, v, g, causal=True, **kw)
+    rows = np.tile(scale[:, None], (batch, 1))
+    check("dq", got["dq"] / rows, *want["dq"])
+    last = (np.arange(batch * sq) % sq) >= sq - sq % 32 if sq % 32 else (np.arange(batch * sq) % sq) >= sq - 32
+    keys = (np.arange(batch * sk) % sk) >= sk - last[:sq].sum()
+    for name in ("dk", "dv"):
+        check(name, got[name][keys], *(x[keys] for x in want[name]))
