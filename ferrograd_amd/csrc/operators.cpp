@@ -418,7 +418,8 @@ Tensor Tensor::norm_rotate(const Tensor& weight, const Tensor& positions, size_t
            "norm_rotate: the positions must be i32 of shape " + shape_str(Shape{s[0]}) + ", got " + shape_str(positions.shape()));
   FG_CHECK(eps >= 0 && std::isfinite(eps), "norm_rotate: eps must be finite and not negative");
   FG_CHECK(base > 0 && std::isfinite(base), "norm_rotate: base must be finite and positive");
-  FG_CHECK(s[0] * heads <= 0x7fffffffu, "norm_rotate: more than 2^31 - 1 heads of tokens");
+  // The kernels count rows in 32 bits, some workgroups' rows past the last.
+  FG_CHECK(s[0] * heads <= 0x7fffffffu - 1024, "norm_rotate: more than 2^31 - 1025 heads of tokens");
   need_hip(*this, "norm_rotate");
   return from_uop(make_call(KernelId::NormRotate, s, {source(uop()), source(weight.uop()), source(positions.uop())},
                             {static_cast<int64_t>(s[0]), static_cast<int64_t>(heads), static_cast<int64_t>(dim),
@@ -452,6 +453,7 @@ Tensor Tensor::attention(const Tensor& k, const Tensor& v, const Tensor* lengths
   FG_CHECK(batch <= 0x7fffffffu && heads <= 0x7fffffffu, "attention: more than 2^31 - 1 sequences or heads");
   const size_t sq = qs[0] / batch, sk = ks[0] / batch;
   FG_CHECK(sq <= (1u << 28) && sk <= (1u << 28), "attention: sequences of more than 2^28 tokens");
+  FG_CHECK(sq * (heads / kv_heads) <= (1u << 30), "attention: more than 2^30 queries of a sequence share a key head");
   need_hip(*this, "attention");
   const std::vector<int64_t> params = {static_cast<int64_t>(batch), static_cast<int64_t>(sq), static_cast<int64_t>(sk),
                                        static_cast<int64_t>(heads), static_cast<int64_t>(kv_heads),

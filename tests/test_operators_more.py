@@ -346,3 +346,18 @@ def test_gradients_that_grow_over_the_sequence(fg, hip, path):
     keys = (np.arange(batch * sk) % sk) >= sk - last[:sq].sum()
     for name in ("dk", "dv"):
         check(name, got[name][keys], *(x[keys] for x in want[name]))
+
+
+# ── the largest sizes ───────────────────────────────────────────────────────
+
+
+def test_more_rows_than_the_kernels_count_are_refused(fg):
+    # Nothing of these sizes is allocated: a call past its limit is refused before.
+    z = lambda *s: fg.Tensor.zeros(list(s), "hip")  # noqa: E731
+    for heads in ((1 << 31) - 1, (1 << 31) - 1024):
+        with pytest.raises(fg.FerrogradError, match="heads of tokens"):
+            z(1, 2 * heads).norm_rotate(z(2), fg.Tensor.zeros([1], "hip", fg.I32), heads=heads)
+    k = z(5, 1)
+    with pytest.raises(fg.FerrogradError, match="share a key head"):
+        z(1 << 28, 8).attention(k, k, heads=8, kv_heads=1)
+    z(1 << 27, 8).attention(k, k, heads=8, kv_heads=1)
