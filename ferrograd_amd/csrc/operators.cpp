@@ -29,12 +29,6 @@ void set_image(RenderedKernel& rk, const unsigned char* begin, const unsigned ch
 // the Infinity Cache (256 MB) for their reader, and push out what it holds.
 constexpr uint64_t kStreamBytes = uint64_t(64) << 20;
 
-// The products of a fixed grid dimension: HIP takes 2^31 - 1 workgroups.
-unsigned grid_of(uint64_t n, const char* what) {
-  FG_CHECK(n >= 1 && n <= 0x7fffffffULL, std::string(what) + ": " + std::to_string(n) + " workgroups in one launch");
-  return static_cast<unsigned>(n);
-}
-
 int64_t to_bits(double f) {
   int64_t b;
   std::memcpy(&b, &f, 8);
@@ -97,10 +91,14 @@ void need_hip(const Tensor& t, const char* what) {
                                             " device has no kernel for it (only hip has)");
 }
 
+// A launch of `grid` workgroups. The device counts a launch's threads in 32 bits.
 LaunchSpec launch(const std::string& func, uint64_t grid, unsigned block, const char* what, unsigned lds = 0) {
+  FG_CHECK(grid >= 1 && grid <= 0xffffffffULL / block,
+           std::string(what) + ": " + std::to_string(grid) + " workgroups of " + std::to_string(block) +
+               " threads in one launch, which takes 2^32 - 1 threads");
   LaunchSpec l;
   l.func = func;
-  l.grid[0] = grid_of(grid, what);
+  l.grid[0] = static_cast<unsigned>(grid);
   l.block[0] = block;
   l.lds_bytes = lds;
   return l;

@@ -361,3 +361,16 @@ def test_more_rows_than_the_kernels_count_are_refused(fg):
     with pytest.raises(fg.FerrogradError, match="share a key head"):
         z(1 << 28, 8).attention(k, k, heads=8, kv_heads=1)
     z(1 << 27, 8).attention(k, k, heads=8, kv_heads=1)
+
+
+def test_more_threads_than_a_launch_takes_are_refused(fg):
+    plan = lambda t: fg.debug_plan([t], fuse=True, render_hip=True)  # noqa: E731
+    n = (1 << 34) - 512  # 512 elements a workgroup of 128
+    assert plan(fg.Tensor.zeros([n], "hip").dropout(0.5, 1))["items"][0]["launches"][0]["grid"] == (1 << 25) - 1
+    with pytest.raises(fg.FerrogradError, match="threads in one launch"):
+        plan(fg.Tensor.zeros([n + 1], "hip").dropout(0.5, 1))
+    q = fg.Tensor.zeros([1 << 23, 8], "hip").with_requires_grad(True)  # 2^23 sequences of one token: 2^25 blocks to cut
+    y = q.attention(q, q, heads=1, batch=1 << 23)
+    plan(y)
+    with pytest.raises(fg.FerrogradError, match="threads in one launch"):
+        plan(y.sum([0, 1]).gradient([q])[0])
