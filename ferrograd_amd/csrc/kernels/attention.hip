@@ -646,16 +646,16 @@ __device__ inline void exact_outer(floatx16 (&o)[NB], const float* x, size_t str
 // keys and leaves, per row (b, h, i), the sum of exp2(S_ij log2 e - m) v_j, m,
 // and the sum of the exponentials (0: it saw no key, and the rest is nothing).
 struct RowParts {
+  float* ml;  // [split][row][2]: first, so that pairs are on the alignment of pairs whatever D
   float* o;   // [split][row][D]
-  float* ml;  // [split][row][2]
   size_t rows;
 };
 
 __device__ inline RowParts row_parts(char* at, const Shape& s, int splits) {
   RowParts p;
   p.rows = static_cast<size_t>(s.b) * s.hq * s.sq;
-  p.o = reinterpret_cast<float*>(at);
-  p.ml = p.o + splits * p.rows * s.d;
+  p.ml = reinterpret_cast<float*>(at);
+  p.o = p.ml + 2 * splits * p.rows;
   return p;
 }
 

@@ -348,6 +348,16 @@ def test_gradients_that_grow_over_the_sequence(fg, hip, path):
         check(name, got[name][keys], *(x[keys] for x in want[name]))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [1, 3, 63, 127])
+@pytest.mark.parametrize("sk", [1300, 2000])
+def test_one_token_of_an_odd_head_in_an_odd_number_of_parts(fg, hip, dim, sk):
+    # The parts' sums are an odd number of floats.
+    q, k, v, _ = attention_inputs(80 + dim, 1, 1, sk, 1, 1, dim)
+    want = attention_ref.attention(q, k, v, 1, 1, 1)
+    check("y", new(fg, q).attention(new(fg, k), new(fg, v), heads=1).numpy(), *want["y"])
+
+
 # ── the largest sizes ───────────────────────────────────────────────────────
 
 
