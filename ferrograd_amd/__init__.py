@@ -484,6 +484,8 @@ def stats() -> dict:
 
 
 def clear_caches() -> None:
+    """Drop recorded plans and compiled programs, and hand the hand-written
+    kernels' workspace back to the allocator."""
     _check(lib().fg_clear_caches())
 
 

@@ -215,6 +215,9 @@ class Device {
   std::shared_ptr<Program> cached_program(const UOp& sink);
   void insert_program(const UOp& sink, std::shared_ptr<Program> p);
   void clear_for_tests();
+  // Hand the memory that calls of hand-written kernels share back to the
+  // allocator (the next call takes what it needs again).
+  virtual void release_workspace() {}
   size_t cache_size() const { return programs_.size(); }
 
  protected:

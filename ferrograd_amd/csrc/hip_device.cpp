@@ -258,13 +258,17 @@ class HipDevice : public Device {
   // recorded graph never keeps an old address.
   void* workspace(size_t nbytes) {
     if (nbytes > workspace_bytes_) {
-      if (workspace_) check(fg_hip_free(ctx(), workspace_), "fg_hip_free (workspace)");
-      workspace_ = nullptr;
-      workspace_bytes_ = 0;
+      release_workspace();
       check(fg_hip_alloc(ctx(), nbytes, 0, &workspace_), "fg_hip_alloc (workspace)");
       workspace_bytes_ = nbytes;
     }
     return workspace_;
+  }
+
+  void release_workspace() override {
+    if (workspace_) check(fg_hip_free(ctx(), workspace_), "fg_hip_free (workspace)");
+    workspace_ = nullptr;
+    workspace_bytes_ = 0;
   }
 
   void execute(Program& prog, std::vector<KernelArg>& args) override {  // cpu.rs:328-380

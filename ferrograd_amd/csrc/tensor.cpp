@@ -56,7 +56,9 @@ void clear_kernel_caches() {
   clear_plan_cache();
   for (int d = 0; d < 2; d++) {
     lowering_cache(static_cast<DeviceId>(d)).clear();
-    if (has_device(static_cast<DeviceId>(d))) get_device(static_cast<DeviceId>(d)).clear_for_tests();
+    if (!has_device(static_cast<DeviceId>(d))) continue;
+    get_device(static_cast<DeviceId>(d)).clear_for_tests();
+    get_device(static_cast<DeviceId>(d)).release_workspace();
   }
 }
 

@@ -181,6 +181,8 @@ int fg_step_capture_stats(uint64_t* captured, uint64_t* replayed);
 /* Cumulative host nanoseconds in: schedule, lowering-cache/compile, launch,
  * live-tensor rewrite after realisation, backward graph construction. */
 int fg_host_times(uint64_t out[5]);
+/* Drop recorded plans and compiled programs, and hand the hand-written kernels'
+ * workspace back to the allocator (fg_hip_trim returns that to the device). */
 int fg_clear_caches(void);
 /* Realisation plans: realize_many records each distinct lazy-graph structure
  * (with its buffer sharing and which leaves still hold zeros) together with

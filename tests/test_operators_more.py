@@ -384,3 +384,37 @@ def test_more_threads_than_a_launch_takes_are_refused(fg):
     plan(y)
     with pytest.raises(fg.FerrogradError, match="threads in one launch"):
         plan(y.sum([0, 1]).gradient([q])[0])
+
+
+# ── the workspace ───────────────────────────────────────────────────────────
+
+
+@pytest.mark.gpu
+def test_cleared_caches_give_the_workspace_back(fg, hip):
+    import gc
+
+    import torch
+
+    from ferrograd_amd.hip import Context, api, check as hip_check
+
+    ctx = Context.of_device()
+    q = fg.Tensor.zeros([4096, 16 * 64], "hip").with_requires_grad(True)
+    x = new(fg, seeded(90).standard_normal((4096, 16 * 64)).astype(np.float32))
+
+    def gradient():
+        return q.add(x).attention(x, x, heads=16, causal=True).sum([0, 1]).gradient([q])[0]
+
+    workspace = max(it.get("workspace", 0) for it in fg.debug_plan([gradient()], fuse=True, render_hip=True)["items"])
+    assert workspace > 1 << 26
+
+    def free():
+        gc.collect()
+        hip_check(api().fg_hip_trim(ctx.h))
+        return torch.cuda.mem_get_info()[0]
+
+    first = gradient().numpy()
+    held = free()
+    fg.clear_caches()
+    cleared = free()
+    assert cleared - held >= workspace * 9 // 10, (held, cleared, workspace)
+    assert np.array_equal(gradient().numpy(), first)  # and it is taken again
