@@ -414,7 +414,9 @@ Tensor Tensor::norm_rotate(const Tensor& weight, const Tensor& positions, size_t
            "norm_rotate: the weight must be f32 of shape " + shape_str(Shape{dim}) + ", got " + shape_str(weight.shape()));
   FG_CHECK(positions.dtype() == DType::I32() && positions.shape() == Shape{s[0]},
            "norm_rotate: the positions must be i32 of shape " + shape_str(Shape{s[0]}) + ", got " + shape_str(positions.shape()));
-  FG_CHECK(eps >= 0 && std::isfinite(eps), "norm_rotate: eps must be finite and not negative");
+  // As float32, which the kernels add: infinity would give 0, and 0 NaN for a row of zeros.
+  FG_CHECK(eps >= 0 && std::isfinite(static_cast<float>(eps)) && (eps == 0 || static_cast<float>(eps) > 0),
+           "norm_rotate: eps must be finite and not negative, and not 0 in float32 unless it is 0");
   FG_CHECK(base > 0 && std::isfinite(base), "norm_rotate: base must be finite and positive");
   // The kernels count rows in 32 bits, some workgroups' rows past the last.
   FG_CHECK(s[0] * heads <= 0x7fffffffu - 1024, "norm_rotate: more than 2^31 - 1025 heads of tokens");

@@ -386,6 +386,15 @@ def test_more_threads_than_a_launch_takes_are_refused(fg):
         plan(y.sum([0, 1]).gradient([q])[0])
 
 
+def test_an_eps_that_float32_does_not_hold_is_refused(fg):
+    x, w, pos = lazy(fg, 6, 8), lazy(fg, 4), lazy(fg, 6, dtype=fg.I32)
+    for eps in (1e39, 1e-50, float("inf"), float("nan"), -1e-9):
+        with pytest.raises(fg.FerrogradError, match="eps"):
+            x.norm_rotate(w, pos, heads=2, eps=eps)
+    for eps in (0.0, 1e-40, 3e38):
+        x.norm_rotate(w, pos, heads=2, eps=eps)
+
+
 # ── the workspace ───────────────────────────────────────────────────────────
 
 
