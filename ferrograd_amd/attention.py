@@ -17,6 +17,8 @@ class SelfAttention:
 
     def __init__(self, features: int, heads: int, kv_heads: int | None = None, head_dim: int | None = None, device=None,
                  causal: bool = True, dropout: float = 0.0, seed: int = 42, eps: float = 1e-6, base: float = 10000.0):
+        if heads < 1:
+            raise FerrogradError(f"SelfAttention: there must be at least one head, got {heads}")
         if head_dim is None:
             if features % heads:
                 raise FerrogradError(f"SelfAttention: {features} features do not split into {heads} heads")

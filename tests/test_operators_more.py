@@ -395,6 +395,15 @@ def test_an_eps_that_float32_does_not_hold_is_refused(fg):
         x.norm_rotate(w, pos, heads=2, eps=eps)
 
 
+@pytest.mark.parametrize("kw", [dict(heads=0), dict(heads=-2), dict(heads=2, kv_heads=0), dict(heads=2, kv_heads=-2),
+                                dict(heads=2, head_dim=0)])
+def test_a_layer_of_no_heads_is_refused(fg, kw):
+    from ferrograd_amd.attention import SelfAttention
+
+    with pytest.raises(fg.FerrogradError, match="SelfAttention"):
+        SelfAttention(32, device="hip", **kw)
+
+
 # ── the workspace ───────────────────────────────────────────────────────────
 
 
