@@ -436,3 +436,56 @@ def test_cleared_caches_give_the_workspace_back(fg, hip):
     cleared = free()
     assert cleared - held >= workspace * 9 // 10, (held, cleared, workspace)
     assert np.array_equal(gradient().numpy(), first)  # and it is taken again
+
+
+# ── layers, trained ─────────────────────────────────────────────────────────
+
+
+@pytest.mark.gpu
+def test_a_sequence_classifier_has_the_loss_and_the_updates_of_its_parameters(fg, hip):
+    import torch
+
+    from ferrograd_amd.attention import SelfAttention
+    from test_operators import Torch64, philox
+
+    features, heads, kv_heads, batch, n, classes, lr = 32, 4, 2, 4, 20, 5, 0.25
+    fg.reset_init_seed(6)
+    layers = [SelfAttention(features, heads, kv_heads, device=hip, dropout=0.125, seed=i) for i in range(2)]
+    head = fg.Linear(features, classes, hip)
+    params = [p for l in layers for p in l.parameters()] + head.parameters()
+    opt = fg.Sgd(params, lr)
+    r = seeded(91)
+    pos = np.tile(np.arange(n, dtype=np.int32), batch)
+    lengths = np.array([20, 7, 13, 1], np.int32)
+    tp, tl = new(fg, pos), new(fg, lengths)
+    # Each layer's values are off by at most 9 * 16 half steps times the terms
+    # summed over (as for one layer's), and there are two and the classifier.
+    tol = 3 * 9 * 16 * (2 * features + n + batch * n) * U
+    for step in range(3):
+        xs = r.standard_normal((batch * n, features)).astype(np.float32)
+        ts = np.eye(classes, dtype=np.float32)[r.integers(0, classes, batch * n)]
+        before = [p.numpy().astype(np.float64) for p in params]
+        h = new(fg, xs)
+        for l in layers:
+            h = h.add(l(h, tp, batch, tl))
+        loss = head(h).cross_entropy(new(fg, ts))
+        opt.zero_grad()
+        loss.backward()
+        opt.step()
+        got = float(loss.to_vec()[0])
+        ps = [torch.tensor(p, requires_grad=True) for p in before]
+        z, at = torch.tensor(xs.astype(np.float64)), 0
+        for i in range(2):
+            wq, wk, wv, wo, nq, nk = ps[at:at + 6]
+            at += 6
+            q = Torch64.norm_rotate(z @ wq.T, nq, torch.tensor(pos), heads, 1e-6, 10000.0)
+            k = Torch64.norm_rotate(z @ wk.T, nk, torch.tensor(pos), kv_heads, 1e-6, 10000.0)
+            out = Torch64.attention(q, k, z @ wv.T, heads, kv_heads, batch, torch.tensor(lengths)) @ wo.T
+            keep = philox(out.numel(), i, step).reshape(out.shape) >= 1 << 29
+            z = z + out * torch.tensor(keep / 0.875)
+        want = -(torch.log_softmax(z @ ps[at].T + ps[at + 1], 1) * torch.tensor(ts.astype(np.float64))).sum() / (batch * n)
+        assert abs(got - float(want.detach())) <= tol * abs(float(want.detach())), (step, got, float(want.detach()))
+        for i, (p, b, g) in enumerate(zip(params, before, torch.autograd.grad(want, ps))):
+            update, g = (b - p.numpy()) / lr, g.numpy()
+            rounding = U * np.linalg.norm(b) / lr  # of the updated parameter
+            assert np.linalg.norm(update - g) <= tol * np.linalg.norm(g) + 2 * rounding, (step, i)
