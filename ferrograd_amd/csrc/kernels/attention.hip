@@ -214,10 +214,12 @@ struct Extremes {
 // launches that cut operands write how even each block is, and workgroups that
 // meet blocks (or scores, or sizes of blocks) beyond these bounds take float32
 // matrix products of the operands as they are instead:
-constexpr int kSpread = 16;         // rows of one block, and of all blocks of a matrix but g', to the largest: errors 2^-24 of each row's largest
+constexpr int kSpread = 10;         // rows of all keys, of all values and of queries, to the largest: 2^-37 of a probability times that is 2^-27 of the least row's
+constexpr int kGradRowSpread = 13;  // rows of one block of g': gradients of scores are cut at 2^-24 of the least row's
 constexpr int kColumnSpread = 20;   // columns of one block: a block's last row alone is a column each
+constexpr int kSmall = 16;          // numbers so far below the largest are few
 constexpr int kGradSpread = 40;     // blocks of g': dv and dk follow each block's scale, up to 60
-constexpr int kMostScore = 16;      // scores: 2^-40 of the largest is 2^-24, an error of p as rounding leaves it
+constexpr int kMostScore = 20;      // scores: 2^-40 of the largest is 2^-20, which a float32 score of 16 is rounded by
 constexpr int kNoRange = 1000;      // beyond every power of two of a float, up or down
 constexpr int kUneven = 4096;       // added to an exponent: the block is uneven in itself
 
@@ -232,6 +234,8 @@ constexpr int kNotFinite = 8 * kNoRange;
 __device__ inline Range no_range() { return Range{static_cast<short>(-kNoRange), static_cast<short>(-kNoRange)}; }
 __device__ inline Range widest(Range a, Range b) { return __builtin_elementwise_max(a, b); }
 __device__ inline int spread(Range r) { return r[0] + r[1]; }
+// Whether a block of queries, or of their gradients, is uneven in itself.
+__device__ inline bool uneven_in_itself(Range r, bool grads) { return spread(r) > (grads ? kGradRowSpread : kSpread); }
 // A block's range without its rows': what its largest number spreads over blocks.
 __device__ inline Range top_only(Range r) { return r[0] == -kNoRange ? r : Range{r[0], static_cast<short>(-r[0])}; }
 
@@ -279,7 +283,7 @@ __device__ inline Tops tops_of(const Ranges* ranges, int n) {
     const Ranges b = ranges[i];
     r.first = widest(r.first, top_only(b.first));
     r.second = widest(r.second, top_only(b.second));
-    r.uneven |= max(spread(b.first), spread(b.second)) > kSpread;
+    r.uneven |= uneven_in_itself(b.first, false) || uneven_in_itself(b.second, true);
   }
   return {wave_widest(r.first), wave_widest(r.second), __any(r.uneven) != 0};
 }
@@ -327,7 +331,7 @@ __device__ inline Range block_range(const float* x, float top, float least, Rang
       for (int i = 0; i < kRows; i++) {
         const float a = fabsf(x[(slice * kRows + i) * kStride<NB> + column]);
         of_column = fmaxf(of_column, a);
-        small += a > 0.f && a < ldexpf(top, -kSpread) ? 1 : 0;
+        small += a > 0.f && a < ldexpf(top, -kSmall) ? 1 : 0;
       }
     shared.columns[threadIdx.x] = of_column;
     small = join_wave(small, [](int a, int b) { return a + b; });
@@ -955,9 +959,10 @@ __device__ inline void forward_tiles(float* __restrict__ y, const float* __restr
 //   ds_ij = p_ij (g'_i . v_j - delta_i)
 //   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i
 // so that both p and ds are cut where their largest is, whatever the row's sum.
-// |g'_i . v_j - delta_i| is at most twice the largest |g'_i| (of the block)
-// times the largest |v_j| (of the head), and p less than 2^kLazy: ds times
-// 2^(kScoreShift - the norms' exponents) is less than 2^15.
+// |g'_i . v_j - delta_i| is at most twice |g'_i| times the largest |v_j| that i
+// sees, and p less than 2^kLazy: ds times 2^(kScoreShift - the norms' exponents)
+// is less than 2^15, with the largest |g'_i| of the block and the largest |v_j|
+// that the workgroup's queries see (dq) or of the head (dk).
 constexpr int kScoreShift = 12;  // 15, less kLazy and one for the twice
 
 // The gradients' workspace. Per batch and key head and block of 32 keys: the
@@ -1095,7 +1100,7 @@ __device__ inline void pack_grad(const float* __restrict__ q, const float* __res
     if (threadIdx.x == 0) *(of_keys ? f.norms + block : exponents + 2) = norm_exponent(squares, e);
   }
   if (threadIdx.x == 0) {
-    exponents[second] = e + (!of_keys && spread(range) > kSpread ? kUneven : 0);
+    exponents[second] = e + (!of_keys && uneven_in_itself(range, second) ? kUneven : 0);
     (&(of_keys ? f.k_ranges : f.q_ranges)[block].first)[second] = range;
   }
   write_rows<NB>(x, scale, tile + (second ? kRowBytes<NB> : 0));
@@ -1154,14 +1159,14 @@ __device__ inline void query_grads(float* __restrict__ dq, const float* __restri
   const float m = live ? stats[stat] : 0.f;
   const char* q_tail = f.q_tiles + (q_block + 1) * kQueryTile<NB> - kTail;
   const float delta = reinterpret_cast<const float*>(q_tail)[32 + lane % 32];
-  // Whether the keys and values that the workgroup's queries see are even, and
-  // their own blocks.
   const int shift = uniform(clamp_power(kScoreShift - reinterpret_cast<const int*>(q_tail)[66] -
                                         values_norm(f.norms + head * f.k_blocks, blocks)));
+  // Whether the keys and values that the workgroup's queries see and each block of
+  // its own are even, and their scores small enough.
   const Ranges seen_keys = widest_of(f.k_ranges + head * f.k_blocks, blocks);
   const int own = (static_cast<size_t>(qt) * kRows) / kBlock;
-  const Ranges of_rows = widest_of(f.q_ranges + (static_cast<size_t>(b) * s.hq + h) * f.q_blocks + own, min(Waves, f.q_blocks - own));
-  const bool exact = max(spread(seen_keys.first), max(spread(seen_keys.second), spread(of_rows.second))) > kSpread ||
+  const Tops of_rows = tops_of(f.q_ranges + (static_cast<size_t>(b) * s.hq + h) * f.q_blocks + own, min(Waves, f.q_blocks - own));
+  const bool exact = max(spread(seen_keys.first), spread(seen_keys.second)) > kSpread || of_rows.uneven ||
                      of_rows.first[0] + seen_keys.first[0] + score_exponent(scale, s.d) > kMostScore;
   const float factor = fabsf(scale) * kLog2e;
   floatx16 o[NB] = {};
