@@ -60,8 +60,10 @@ __device__ inline float wave_max(float x) { return __int_as_float(join_wave(__fl
 // A float32 product on the float16 matrix cores: each operand is scaled by a
 // power of two that brings its block's largest value below 2^15 and cut into
 // two float16 parts, 11 bits each, and a b = a1 b1 + a1 b2 + a2 b1 with sums in
-// float32; a2 b2, 2^-20 of the product at most, is left out. Three float16
-// products cost less than a fifth of one float32 product's matrix-core time.
+// float32; a2 b2, 2^-21 of the product at most, is left out. Three float16
+// products cost less than a fifth of one float32 product's matrix-core time. That
+// is 22 bits of each number instead of float32's 24; measured against 64 bits,
+// results are off by 5e-7 to 1e-6, which is what float32's own sums of this length are.
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
@@ -508,7 +510,9 @@ constexpr float kLazy = 2.f;
 constexpr int kProbShift = 13;
 
 // p[0..7] as two parts, cut off (not rounded: one instruction for two
-// numbers), the second from what the first leaves.
+// numbers), the second from what the first leaves: low by up to 2^-21 of each, or
+// by 2^-37 of the largest a row can have. So what a key takes that every query
+// weighs less than 2^-27 keeps fewer bits than float32's, by up to that.
 __device__ inline void cut_probs(const float* p, half8* hi, half8* lo) {
   typedef __fp16 fp16x2 __attribute__((ext_vector_type(2)));
   union {
@@ -771,13 +775,15 @@ __device__ inline void query_tile(const Shape& s, int rows, int splits, unsigned
 // and sum cost one exchange between the wave's halves, and the probabilities
 // are in registers what O^T += V^T P^T takes as its second operand.
 //
-// Bound by the matrix cores at the clock the card's power leaves them: 4096
-// causal tokens, 32 heads of 128 over 8: 421 us, 980 TFLOP/s of float16 products
-// (327 of the float32 ones they stand for; float32's own matrix rate is 151 and a
-// library's large float16 product reaches 1076), cores busy 53% of the time at
-// 1.9 GHz. Four waves a workgroup and two workgroups a compute unit, so that one
-// has the cores while the other makes its probabilities; keys are cut by a launch
-// of their own (14 us), once for all the query tiles that read them.
+// 4096 causal tokens, 32 heads of 128 over 8: 407 us, 1013 TFLOP/s of float16
+// products (338 of the float32 ones they stand for; float32's own matrix rate is
+// 152 and a library's large float16 product reaches 1084). Nothing is at its
+// limit: the matrix cores are busy 58% of the cycles in which a compute unit has
+// waves, and waves wait 43% of theirs, for tiles and for results, at 1.9 GHz of
+// 2.4, which the power leaves. Four waves a workgroup and two workgroups a compute
+// unit, so that one has the cores while the other makes its probabilities; keys
+// are cut by a launch of their own (15 us), once for all the query tiles that read
+// them.
 template <int NB>
 __device__ inline void forward_tiles(float* __restrict__ y, const float* __restrict__ q, float* __restrict__ stats,
                                      const int* __restrict__ lengths, char* __restrict__ ws, const Shape& s, float scale,
@@ -1020,7 +1026,7 @@ __device__ inline int norm_exponent(float squares, int e) {
 __device__ inline float power(int a) { return ldexpf(1.f, a); }
 
 // Keys, values, queries and gradients cut once per call, one workgroup per
-// block and matrix. Bound by memory: 16 heads of 128 over 8192 tokens 102 us for
+// block and matrix, with how even each block is. Bound by memory: 16 heads of 128 over 8192 tokens 102 us for
 // 236 MB read and 320 written, 5.4 TB/s (queries and gradients by rows for the
 // scores, and by columns for dk and dv). With the outputs read after the gradients
 // were in LDS it took 138.
@@ -1120,9 +1126,9 @@ __device__ inline int clamp_power(int a) { return min(max(a, -120), 120); }
 // dq. A workgroup: 32 queries of one head a wave, over all keys; scores and
 // their gradients transposed as in the forward pass. Tiles of four column
 // groups leave room for one workgroup a compute unit: eight waves share them,
-// so that each matrix core has two waves in turn. Bound like the forward pass: 16
-// heads of 128 over 8192 causal tokens 1044 us, 1185 TFLOP/s of float16 products,
-// cores busy 60% of the time at 1.9 GHz.
+// so that each matrix core has two waves in turn. 16 heads of 128 over 8192 causal
+// tokens: 1021-1042 us, up to 1210 TFLOP/s of float16 products, the cores busy 66%
+// and waves waiting 46% of their cycles, at 1.9 GHz.
 template <int NB>
 constexpr int kQueryGradWaves = NB < 4 ? 4 : 8;
 
@@ -1265,10 +1271,10 @@ __device__ inline void query_grads(float* __restrict__ dq, const float* __restri
 // probabilities' way through LDS. Scores are not transposed here: a lane holds
 // 16 queries of one key, which is what dv^T += G^T P and dk^T += Q^T dS take.
 //
-// 16 heads of 128 over 4 key heads and 8192 causal tokens: 1685 us, 980 TFLOP/s of
-// float16 products, cores busy 46% of the time at 2.0 GHz: what the power leaves
-// and the two barriers of a step, at which the pair waits for its probabilities
-// and all for the next tile. (With one wave for both, and four for dq, forward and
+// 16 heads of 128 over 4 key heads and 8192 causal tokens: 1624-1700 us, up to 1015
+// TFLOP/s of float16 products, the cores busy 50% of the cycles at 2.0 GHz. Bound
+// by the two barriers of a step, at which the pair waits for its probabilities and
+// all for the next tile: waves wait 43% of their cycles. (With one wave for both, and four for dq, forward and
 // gradients took 4.21 ms instead of 3.65; with 64 keys a workgroup and two of
 // them a compute unit, out of step with each other, 3.70 instead of 3.56: the
 // query tiles are then copied twice as often.)

@@ -202,6 +202,18 @@ def test_a_value_that_is_nan_makes_its_column_nan(fg, hip, path):
     assert np.isfinite(got["y"][rest]).all() and np.isfinite(got["dq"][rest]).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("path", [p for p in PATHS if PATHS[p][6] is None])
+def test_a_key_that_scores_minus_infinity_weighs_nothing(fg, hip, path):
+    batch, sq, sk, heads, kv_heads, dim, _, _ = PATHS[path]
+    q, k, v, _ = attention_inputs(64, batch, sq, sk, heads, kv_heads, dim)
+    q[:, ::dim] = np.abs(q[:, ::dim]) + 0.1
+    rest = np.arange(batch * sk) % sk != sk // 4
+    want = attention_ref.attention(q, k[rest], v[rest], batch, heads, kv_heads)["y"]
+    k.reshape(batch, sk, kv_heads, dim)[:, sk // 4, :, 0] = -np.inf
+    check("y", new(fg, q).attention(new(fg, k), new(fg, v), heads=heads, kv_heads=kv_heads, batch=batch).numpy(), *want)
+
+
 # ── values of unlike sizes ──────────────────────────────────────────────────
 
 
