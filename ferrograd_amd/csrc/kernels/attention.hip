@@ -52,7 +52,9 @@ __device__ inline int join_wave(int x, Join join) {
 __device__ inline int max_of_floats(int a, int b) { return __float_as_int(fmaxf(__int_as_float(a), __int_as_float(b))); }
 
 __device__ inline float sum8(float x) {
-  return __int_as_float(join8(__float_as_int(x), [](int a, int b) { return __float_as_int(__int_as_float(a) + __int_as_float(b)); }));
+  return __int_as_float(join8(__float_as_int(x), [](int a, int b) {
+    return __float_as_int(__int_as_float(a) + __int_as_float(b));
+  }));
 }
 __device__ inline float wave_max(float x) { return __int_as_float(join_wave(__float_as_int(x), max_of_floats)); }
 
@@ -216,14 +218,20 @@ struct Extremes {
 // launches that cut operands write how even each block is, and workgroups that
 // meet blocks (or scores, or sizes of blocks) beyond these bounds take float32
 // matrix products of the operands as they are instead:
-constexpr int kSpread = 10;         // rows of all keys, of all values and of queries, to the largest: 2^-37 of a probability times that is 2^-27 of the least row's
-constexpr int kGradRowSpread = 13;  // rows of one block of g': gradients of scores are cut at 2^-24 of the least row's
-constexpr int kColumnSpread = 20;   // columns of one block: a block's last row alone is a column each
-constexpr int kSmall = 16;          // numbers so far below the largest are few
-constexpr int kGradSpread = 40;     // blocks of g': dv and dk follow each block's scale, up to 60
-constexpr int kMostScore = 20;      // scores: 2^-40 of the largest is 2^-20, which a float32 score of 16 is rounded by
-constexpr int kNoRange = 1000;      // beyond every power of two of a float, up or down
-constexpr int kUneven = 4096;       // added to an exponent: the block is uneven in itself
+//   rows of all values, of all keys (dq) and of all queries (dk), to the largest:
+//   2^-37 of a probability is then 2^-27 of what the least row adds;
+constexpr int kSpread = 10;
+//   rows of one block of g': gradients of scores are cut at 2^-24 of the least;
+constexpr int kGradRowSpread = 13;
+//   blocks of g': the sums of dv and dk follow each block's scale, but 60 at most;
+constexpr int kGradSpread = 40;
+//   columns of one block (one row alone is a column each, so no less), or more
+//   than a sixteenth of its numbers 2^-kSmall of the largest;
+constexpr int kColumnSpread = 20, kSmall = 16;
+//   scores: 2^-40 of the largest is 2^-20, half a step of a float32 score of 16.
+constexpr int kMostScore = 20;
+constexpr int kNoRange = 1000;  // beyond every power of two of a float, up or down
+constexpr int kUneven = 4096;   // added to an exponent: the block is uneven in itself
 
 // How even a block is: the power of two above its largest number, and minus
 // that of its smallest row that is not zero (kNoRange more where its columns
@@ -353,7 +361,8 @@ __device__ inline Range block_range(const float* x, float top, float least, Rang
   if (wave > 0) return no_range();
   const float lows = fmaxf(fmaxf(shared.lows[0], shared.lows[1]), fmaxf(shared.lows[2], shared.lows[3]));
   const Range r = top_range(top);
-  return r[0] == -kNoRange || r[0] == kNotFinite ? r : Range{r[0], static_cast<short>(uneven ? kNoRange : static_cast<int>(lows))};
+  if (r[0] == -kNoRange || r[0] == kNotFinite) return r;
+  return Range{r[0], static_cast<short>(uneven ? kNoRange : static_cast<int>(lows))};
 }
 
 // Four numbers of a row, which starts on any float: odd head sizes take the
@@ -594,7 +603,7 @@ __device__ inline void store_columns(float* row, int n, int half, int D, const f
 // loops over even blocks leave: with one value 10^8 times the others 4096 causal
 // tokens, 32 heads of 128 over 8, take 2.4 ms instead of 0.4, and 8192 with
 // gradients, 16 heads over 4, 34 ms instead of 3.4; with such a gradient in every
-// 20th block of queries 11 ms. Looking for it costs even operands 0 to 3 in 100.
+// 20th block of queries 11 ms. Looking for it costs even operands 0 to 5 in 100.
 
 // The kernel's arguments, read again: held in registers through the loops over
 // even blocks they would be spilled there.
@@ -645,7 +654,8 @@ __device__ inline void exact_outer(floatx16 (&o)[NB], const float* x, size_t str
 #pragma unroll
     for (int n = 0; n < NB; n++)
       o[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(ldexpf(at[min(32 * n + column, D - 1)] * by, e), p[r], o[n], 0, 0, 0);
-    if (r % 2) __builtin_amdgcn_sched_barrier(0);  // few loads in flight: the even blocks' registers are not to be more for these
+    // Few loads in flight, so that even blocks have no fewer registers for these.
+    if (r % 2) __builtin_amdgcn_sched_barrier(0);
   }
 }
 

@@ -349,6 +349,45 @@ def test_a_large_query_or_gradient_changes_nothing_for_keys_that_it_does_not_see
         check(name, got[name][rows], *(x[rows] for x in want[name]))
 
 
+# The same through every launch of the gradients: both in one, one for each, and
+# queries or keys in parts, at every number of column groups.
+EVERY = {
+    "one launch, 1": (3, 70, 90, 4, 2, 30),
+    "one launch, 2": (3, 70, 90, 4, 2, 50),
+    "one launch, 3": (3, 70, 90, 4, 2, 80),
+    "one launch, 4": (3, 70, 90, 4, 2, 128),
+    "parts, 2": (1, 520, 300, 64, 1, 64),
+    "parts, 4": (1, 300, 900, 6, 2, 100),
+    "two launches, 1": (17, 130, 140, 40, 40, 16),
+    "two launches, 2": (16, 130, 130, 24, 24, 50),
+    "two launches, 3": (16, 130, 130, 20, 20, 70),
+    "two launches, 4": (16, 130, 130, 20, 20, 110),
+}
+
+
+def test_the_shapes_reach_every_launch_of_the_gradients(fg):
+    names = set()
+    for batch, sq, sk, heads, kv_heads, dim in EVERY.values():
+        q, k = lazy(fg, batch * sq, heads * dim), fg.Tensor.zeros([batch * sk, kv_heads * dim], "hip")
+        g = q.attention(k, k, heads=heads, kv_heads=kv_heads, batch=batch, causal=True).sum([0, 1]).gradient([q])[0]
+        for it in fg.debug_plan([g], fuse=True, render_hip=True)["items"]:
+            names |= {l["name"] for l in it["launches"]} if it["class"] == "attention_grad" else set()
+    want = {f"fg_attention_{n}_{i}" for n in ("grad_pack", "grads", "grad_kv", "grad_q") for i in (1, 2, 3, 4)}
+    assert want <= names and {"fg_attention_grad_sum_2", "fg_attention_grad_sum_4"} <= names, want - names
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("path", EVERY)
+def test_operands_of_unlike_sizes_in_every_launch(fg, hip, path, monkeypatch):
+    monkeypatch.setitem(UNLIKE, path, EVERY[path])
+    for of in ("v", "kv"):
+        test_a_large_key_or_value_changes_nothing_for_queries_that_do_not_see_it(fg, hip, path, of, 1e9)
+    for of in ("q", "g"):
+        test_a_large_query_or_gradient_changes_nothing_for_keys_that_it_does_not_see(fg, hip, path, of, 1e9)
+    test_a_value_that_weighs_nothing_changes_nothing(fg, hip, path, 1e9)
+    test_columns_beside_a_large_one(fg, hip, path, 1e9)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("path", UNLIKE)
 def test_gradients_that_grow_over_the_sequence(fg, hip, path):
