@@ -118,9 +118,9 @@ PATHS = {
 }
 
 
-def forward_launches(fg, batch, sq, sk, heads, kv_heads, dim, lengths):
+def forward_launches(fg, batch, sq, sk, heads, kv_heads, dim, lengths, causal=False):
     q, k = fg.Tensor.zeros([batch * sq, heads * dim], "hip"), fg.Tensor.zeros([batch * sk, kv_heads * dim], "hip")
-    y = q.attention(k, k, heads=heads, kv_heads=kv_heads, batch=batch,
+    y = q.attention(k, k, heads=heads, kv_heads=kv_heads, batch=batch, causal=causal,
                     lengths=None if lengths is None else fg.Tensor.zeros([batch], "hip", fg.I32))
     call = [it for it in fg.debug_plan([y], fuse=True, render_hip=True)["items"] if it["class"] == "attention"]
     return [l["name"].split("_")[2] for it in call for l in it["launches"]]
@@ -239,12 +239,20 @@ def test_values_of_zero_beside_large_ones_take_their_probability(fg, hip, size, 
 
 UNLIKE = {  # batch, sq, sk, heads, kv_heads, dim
     "small": (1, 100, 100, 2, 1, 24),
-    "large": (4, 130, 257, 32, 32, 40),
-    "large in parts": (1, 256, 4000, 16, 8, 64),
-    "wide": (2, 200, 200, 32, 16, 128),
-    "wide and ragged": (2, 300, 300, 16, 16, 100),
+    "large": (4, 200, 257, 32, 32, 40),
+    "large in parts": (1, 256, 1600, 16, 8, 64),
+    "wide": (2, 300, 300, 24, 12, 128),
+    "wide and odd": (2, 257, 300, 24, 24, 70),
     "narrow": (2, 300, 300, 32, 16, 20),
 }
+
+
+def test_the_unlike_shapes_take_their_paths(fg):
+    cut = ["pack", "tiles"]
+    for causal in (False, True):
+        launches = {p: forward_launches(fg, *s, None, causal) for p, s in UNLIKE.items()}
+        assert launches == {"small": ["token"], "large": cut, "large in parts": cut + ["join"], "wide": cut,
+                            "wide and odd": cut, "narrow": cut}
 
 
 def unlike_inputs(path, seed):
