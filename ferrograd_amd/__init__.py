@@ -18,8 +18,8 @@ from typing import Iterable, Sequence
 
 import numpy as np
 
-__all__ = ["Tensor", "Linear", "Dropout", "Sgd", "FerrogradError", "lib", "stats", "synchronize", "reset_init_seed",
-           "debug_plan", "F32", "I32", "BOOL", "clear_caches"]
+__all__ = ["Tensor", "Linear", "Dropout", "Embedding", "LayerNorm", "Sgd", "clip_norm", "global_norm", "FerrogradError",
+           "lib", "stats", "synchronize", "reset_init_seed", "debug_plan", "F32", "I32", "BOOL", "clear_caches"]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libferrograd_amd.so")
@@ -82,6 +82,11 @@ def _declare(l: ctypes.CDLL) -> None:
         "fg_tensor_attention": (c_int, [P, P, P, P] + [ctypes.c_int64] * 3 + [c_int, ctypes.c_double, PP]),
         "fg_tensor_norm_rotate": (c_int, [P, P, P, ctypes.c_int64, ctypes.c_double, ctypes.c_double, PP]),
         "fg_tensor_dropout": (c_int, [P, ctypes.c_double, ctypes.c_uint64, ctypes.c_uint64, PP]),
+        "fg_tensor_embedding": (c_int, [P, P, ctypes.c_double, PP]),
+        "fg_tensor_layer_norm": (c_int, [P, P, P, ctypes.c_double, PP]),
+        "fg_tensor_token_cross_entropy": (c_int, [P, P, PP]),
+        "fg_global_norm": (c_int, [PP, c_int, PP]),
+        "fg_clip_norm": (c_int, [PP, c_int, ctypes.c_double, PP, PP]),
         "fg_tensor_log_softmax": (c_int, [P, ctypes.c_int64, PP]),
         "fg_tensor_assign": (c_int, [P, P]),
         "fg_tensor_replace": (c_int, [P, P]),
@@ -104,6 +109,7 @@ def _declare(l: ctypes.CDLL) -> None:
         "fg_linear_free": (c_int, [P]),
         "fg_sgd_new": (c_int, [PP, c_int, ctypes.c_float, PP]),
         "fg_sgd_zero_grad": (c_int, [P]),
+        "fg_sgd_clip_grad_norm": (c_int, [P, ctypes.c_double, PP]),
         "fg_sgd_step": (c_int, [P]),
         "fg_mlp_train_steps": (c_int, [P, c_int, P, P, P, c_int, ctypes.POINTER(ctypes.c_float)]),
         "fg_mlp_train_batches": (c_int, [P, c_int, P, P, P, ctypes.c_int64, ctypes.c_int64, c_int,
@@ -280,8 +286,9 @@ class Tensor(_fgc.TensorBase if _fgc is not None else object):
     # ── ops (tensor.rs:442-778): neg, reciprocal, exp2, log2, sqrt, relu, exp,
     # log, contiguous, detach, add, mul, sub, matmul, cross_entropy, reshape,
     # permute, expand, narrow, sum, max, log_softmax, assign and realize,
-    # and the hand-written kernels' attention, norm_rotate and dropout, are the
-    # extension type's methods (csrc/pymodule.c).
+    # and the hand-written kernels' attention, norm_rotate, dropout, embedding,
+    # layer_norm and token_cross_entropy, are the extension type's methods
+    # (csrc/pymodule.c).
 
     def replace(self, other: "Tensor") -> "Tensor":
         _check(lib().fg_tensor_replace(self._h, other._h))
@@ -398,6 +405,67 @@ class Dropout:
     __call__ = forward
 
 
+class Embedding:
+    """Rows of a weight [vocab, dim] by token id, times `scale`, as a layer (no
+    reference counterpart): Tensor.embedding. The weight is drawn as that of
+    Linear(dim, vocab), whose rows it can share: pass that layer's weight as
+    `weight`."""
+
+    def __init__(self, vocab: int, dim: int, device=None, scale: float = 1.0, weight: Tensor | None = None):
+        if weight is None:
+            weight = Linear(dim, vocab, device, bias=False).weight
+        elif weight.shape != (vocab, dim):
+            raise FerrogradError(f"Embedding: the weight must have shape [{vocab}, {dim}], got {list(weight.shape)}")
+        self.weight, self.scale = weight, float(scale)
+
+    def forward(self, ids: Tensor) -> Tensor:
+        return self.weight.embedding(ids, self.scale)
+
+    __call__ = forward
+
+    def parameters(self) -> list:
+        return [self.weight]
+
+
+class LayerNorm:
+    """Layer norm over `features` columns with a weight of ones and a bias of
+    zeros (`bias` off: none), as a layer (no reference counterpart):
+    Tensor.layer_norm."""
+
+    def __init__(self, features: int, device=None, bias: bool = True, eps: float = 1e-5):
+        self.weight = Tensor.ones([features], device).with_requires_grad(True)
+        self.bias = Tensor.zeros([features], device).with_requires_grad(True) if bias else None
+        self.eps = float(eps)
+
+    def forward(self, x: Tensor) -> Tensor:
+        return x.layer_norm(self.weight, self.bias, self.eps)
+
+    __call__ = forward
+
+    def parameters(self) -> list:
+        return [self.weight] + ([self.bias] if self.bias is not None else [])
+
+
+def _handles(tensors: Sequence[Tensor]):
+    return (ctypes.c_void_p * max(1, len(tensors)))(*[t._h for t in tensors]), len(tensors)
+
+
+def global_norm(tensors: Sequence[Tensor]) -> Tensor:
+    """The root of the sum of the squares of all elements of the tensors (f32, any
+    shapes), as a tensor [1], with squares and sums in 64 bits. No gradient flows
+    through it."""
+    return Tensor._out(lib().fg_global_norm, *_handles(tensors))
+
+
+def clip_norm(tensors: Sequence[Tensor], max_norm: float) -> tuple:
+    """global_norm, and the list of the tensors times max_norm / max(norm,
+    max_norm), all in a pass over them for the norm and one for the products."""
+    hs, n = _handles(tensors)
+    norm, outs = ctypes.c_void_p(), (ctypes.c_void_p * max(1, n))()
+    _check(lib().fg_clip_norm(hs, n, max_norm, ctypes.byref(norm), outs))
+    return _fgc.from_handle(Tensor, norm.value), [_fgc.from_handle(Tensor, outs[i]) for i in range(n)]
+
+
 class Sgd:
     """optim::Sgd (optim.rs:16-71)."""
 
@@ -409,6 +477,11 @@ class Sgd:
 
     def zero_grad(self) -> None:
         _check(lib().fg_sgd_zero_grad(self._h))
+
+    def clip_grad_norm(self, max_norm: float) -> Tensor:
+        """Between backward and step: the parameters' gradients clipped together
+        (clip_norm); the norm they had (no reference counterpart)."""
+        return Tensor._out(lib().fg_sgd_clip_grad_norm, self._h, max_norm)
 
     def step(self) -> None:
         _check(lib().fg_sgd_step(self._h))

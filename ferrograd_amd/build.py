@@ -24,7 +24,7 @@ SOURCES = ["ir.cpp", "device.cpp", "schedule.cpp", "tensor.cpp", "gpu_lower.cpp"
            "hip_runtime.cpp", "kernel_text.cpp", "hip_kernel.cpp", "dataset.cpp", "operators.cpp", "capi.cpp"]
 # Hand-written kernels (csrc/kernels/*.hip): device code objects, linked into
 # the library as data.
-KERNELS = ["attention", "dropout", "norm_rotate"]
+KERNELS = ["attention", "clip", "dropout", "embedding", "layer_norm", "norm_rotate", "token_loss"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 CXXFLAGS = ["-O2", "-g0", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function",

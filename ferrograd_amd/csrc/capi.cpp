@@ -218,6 +218,39 @@ int fg_tensor_dropout(fg_tensor* t, double p, uint64_t seed, uint64_t offset, fg
   return guard([&] { *out = wrap(t->t.dropout(p, seed, offset)); });
 }
 
+int fg_tensor_embedding(fg_tensor* weight, fg_tensor* ids, double scale, fg_tensor** out) {
+  return guard([&] { *out = wrap(weight->t.embedding(ids->t, scale)); });
+}
+
+int fg_tensor_layer_norm(fg_tensor* x, fg_tensor* weight, fg_tensor* bias, double eps, fg_tensor** out) {
+  return guard([&] { *out = wrap(x->t.layer_norm(weight->t, bias ? &bias->t : nullptr, eps)); });
+}
+
+int fg_tensor_token_cross_entropy(fg_tensor* logits, fg_tensor* labels, fg_tensor** out) {
+  return guard([&] { *out = wrap(logits->t.token_cross_entropy(labels->t)); });
+}
+
+namespace {
+std::vector<fg::Tensor> tensors_of(fg_tensor* const* ts, int n, const char* what) {
+  FG_CHECK(n >= 0 && (ts || n == 0), std::string(what) + ": no tensors");
+  std::vector<fg::Tensor> v;
+  for (int i = 0; i < n; i++) v.push_back(ts[i]->t);
+  return v;
+}
+}  // namespace
+
+int fg_global_norm(fg_tensor* const* ts, int n, fg_tensor** out) {
+  return guard([&] { *out = wrap(fg::Tensor::global_norm(tensors_of(ts, n, "global_norm"))); });
+}
+
+int fg_clip_norm(fg_tensor* const* ts, int n, double max_norm, fg_tensor** norm, fg_tensor** outs) {
+  return guard([&] {
+    auto [total, clipped] = fg::Tensor::clip_norm(tensors_of(ts, n, "clip_norm"), max_norm);
+    *norm = wrap(total);
+    for (size_t i = 0; i < clipped.size(); i++) outs[i] = wrap(clipped[i]);
+  });
+}
+
 int fg_tensor_log_softmax(fg_tensor* t, int64_t axis, fg_tensor** out) {
   return guard([&] {
     FG_CHECK(axis >= 0, "log_softmax: negative axis");
@@ -385,6 +418,10 @@ int fg_sgd_new(fg_tensor** params, int n, float lr, fg_sgd** out) {
     for (int i = 0; i < n; i++) ps.push_back(params[i]->t);
     *out = new fg_sgd{fg::Sgd(ps, lr)};
   });
+}
+
+int fg_sgd_clip_grad_norm(fg_sgd* s, double max_norm, fg_tensor** norm) {
+  return guard([&] { *norm = wrap(s->s.clip_grad_norm(max_norm)); });
 }
 
 int fg_sgd_zero_grad(fg_sgd* s) {

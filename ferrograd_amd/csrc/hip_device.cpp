@@ -241,6 +241,7 @@ class HipDevice : public Device {
         }
         case CallArg::Kind::I32: x.kind = FG_ARG_I32; x.v.i = ca.i; break;
         case CallArg::Kind::F32: x.kind = FG_ARG_F32; x.v.f = ca.f; break;
+        case CallArg::Kind::Bits64: x.kind = FG_ARG_PTR; std::memcpy(&x.v.p, &ca.bits, 8); break;
         case CallArg::Kind::Null: x.kind = FG_ARG_PTR; break;
         case CallArg::Kind::Workspace: x.kind = FG_ARG_PTR; x.v.p = workspace(p.meta.workspace_bytes); break;
       }

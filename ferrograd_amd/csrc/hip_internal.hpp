@@ -9,6 +9,9 @@ extern "C" {
 int fg_hip_set_error(int code, const char* msg);
 // Function `func` of a code object in memory (the hand-written kernels, linked
 // into the library), loaded once per context and device.
+// Its launches take up to FG_MAX_BUILTIN_ARGS arguments (a clip's has three for
+// each of 64 tensors).
+#define FG_MAX_BUILTIN_ARGS 256
 int fg_hip_builtin_function(fg_ctx* c, const void* image, size_t size, const char* func, int num_args, fg_prog** out);
 // The device ordinal a context was created on.
 int fg_hip_context_device(const fg_ctx* c);

@@ -148,6 +148,7 @@ struct fg_prog {
   std::shared_ptr<ModuleRef> module;
   hipFunction_t func = nullptr;
   int num_args = 0;
+  bool builtin = false;  // of the library's own code objects
   std::string name;
   // The kernel as the HSA queue dispatches it: its descriptor and segment
   // sizes (read on the first dispatch).
@@ -792,6 +793,7 @@ int fg_hip_builtin_function(fg_ctx* c, const void* image, size_t size, const cha
   }
   auto p = std::make_unique<fg_prog>();
   p->num_args = num_args;
+  p->builtin = true;
   p->name = func;
   p->module = module;
   hipError_t e = hipModuleGetFunction(&p->func, p->module->module, func);
@@ -833,8 +835,9 @@ int fg_hip_program_num_args(const fg_prog* p) { return p ? p->num_args : -1; }
 
 namespace {
 // Points params[i] at the value of args[i] (kernelParams for a HIP launch).
-int marshal_args(const fg_arg* args, int nargs, void** params) {
-  if (nargs > FG_MAX_LAUNCH_ARGS) return set_err(FG_ERR_ARGS, "fg_hip_launch: at most 64 arguments");
+int marshal_args(const fg_prog* p, const fg_arg* args, int nargs, void** params) {
+  const int most = p->builtin ? FG_MAX_BUILTIN_ARGS : FG_MAX_LAUNCH_ARGS;
+  if (nargs > most) return set_err(FG_ERR_ARGS, "fg_hip_launch: at most " + std::to_string(most) + " arguments");
   for (int i = 0; i < nargs; i++) {
     switch (args[i].kind) {
       case FG_ARG_PTR: params[i] = const_cast<void**>(&args[i].v.p); break;
@@ -878,8 +881,8 @@ int fg_hip_launch_direct(fg_ctx* c, fg_prog* p, const fg_arg* args, int nargs, c
                          const unsigned block[3], unsigned lds) {
   if (int rc = check_launch(c, p, nargs, grid, block)) return rc;
   if (int rc = aql_interlude(c)) return rc;
-  void* params[FG_MAX_LAUNCH_ARGS];
-  if (int rc = marshal_args(args, nargs, params)) return rc;
+  void* params[FG_MAX_BUILTIN_ARGS];
+  if (int rc = marshal_args(p, args, nargs, params)) return rc;
   HIP_TRY(hipModuleLaunchKernel(p->func, grid[0], grid[1], grid[2], block[0], block[1], block[2], lds, c->stream,
                                 params, nullptr));
   return FG_OK;
@@ -1228,8 +1231,8 @@ int fg_hip_launch(fg_ctx* c, fg_prog* p, const fg_arg* args, int nargs, const un
                   const unsigned block[3], unsigned lds) {
   if (int rc = check_launch(c, p, nargs, grid, block)) return rc;
   if (int rc = aql_interlude(c)) return rc;
-  void* params[FG_MAX_LAUNCH_ARGS];
-  if (int rc = marshal_args(args, nargs, params)) return rc;
+  void* params[FG_MAX_BUILTIN_ARGS];
+  if (int rc = marshal_args(p, args, nargs, params)) return rc;
   if (c->profiling) {
     // Start/stop events attached to the dispatch itself, so the duration
     // excludes any host gap before the launch reaches the queue.
@@ -1278,8 +1281,8 @@ int fg_hip_graph_create(fg_ctx* c, int n, fg_prog* const* progs, const unsigned*
   HIP_TRY(hipStreamBeginCapture(c->stream, hipStreamCaptureModeThreadLocal));
   int rc = FG_OK;
   for (auto& l : g->launches) {
-    void* params[FG_MAX_LAUNCH_ARGS];
-    rc = marshal_args(l.args.data(), static_cast<int>(l.args.size()), params);
+    void* params[FG_MAX_BUILTIN_ARGS];
+    rc = marshal_args(l.prog, l.args.data(), static_cast<int>(l.args.size()), params);
     if (rc) break;
     hipError_t e = hipModuleLaunchKernel(l.prog->func, l.grid[0], l.grid[1], l.grid[2], l.block[0], l.block[1],
                                          l.block[2], l.lds, c->stream, params, nullptr);
@@ -1330,8 +1333,8 @@ int fg_hip_graph_launch(fg_ctx* c, fg_graph* g, const fg_arg* args, int* updated
     const int n = static_cast<int>(l.args.size());
     if (!same_args(l.args.data(), args + off, n)) {
       std::copy(args + off, args + off + n, l.args.begin());
-      void* params[FG_MAX_LAUNCH_ARGS];
-      if (int rc = marshal_args(l.args.data(), n, params)) return rc;
+      void* params[FG_MAX_BUILTIN_ARGS];
+      if (int rc = marshal_args(l.prog, l.args.data(), n, params)) return rc;
       hipKernelNodeParams p = l.params;
       p.kernelParams = params;
       p.extra = nullptr;

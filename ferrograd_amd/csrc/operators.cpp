@@ -15,6 +15,10 @@
 FG_IMAGE(dropout)
 FG_IMAGE(norm_rotate)
 FG_IMAGE(attention)
+FG_IMAGE(embedding)
+FG_IMAGE(layer_norm)
+FG_IMAGE(token_loss)
+FG_IMAGE(clip)
 
 namespace fg {
 
@@ -394,6 +398,196 @@ RenderedKernel render_attention(const UOp& call, bool grad) {
   return rk;
 }
 
+// ── embedding ───────────────────────────────────────────────────────────────
+// params: tokens, vocab, dim, bits of scale. Sources: weight, ids; of the
+// gradient ids, g.
+
+RenderedKernel render_embedding(const UOp& call, bool grad) {
+  const std::vector<int64_t> p = params_of(call);
+  const int64_t tokens = p[0], vocab = p[1];
+  RenderedKernel rk;
+  set_image(rk, fg_image_embedding, fg_image_embedding_end);
+  if (!grad) {
+    rk.kind = "embedding";
+    rk.launches = {launch("fg_embedding", static_cast<uint64_t>(std::min<int64_t>(tokens, 65536)), 256, "embedding")};
+  } else {
+    rk.kind = "embedding_grad";
+    rk.launches = {launch("fg_embedding_grad", static_cast<uint64_t>(std::min<int64_t>(vocab, 65536)), 256, "embedding")};
+  }
+  for (int i = 0; i < 3; i++) rk.call_args.push_back(CallArg::slot(i));
+  for (size_t i = 0; i < 3; i++) rk.call_args.push_back(CallArg::i32(p[i]));
+  rk.call_args.push_back(CallArg::f32(static_cast<float>(from_bits(p[3]))));
+  return rk;
+}
+
+// ── layer_norm ──────────────────────────────────────────────────────────────
+// params: rows, dim, whether there is a bias, bits of eps. Sources: x, weight,
+// [bias]; of the gradient x, weight, g, dweight's and [dbias's] storage.
+
+RenderedKernel render_layer_norm(const UOp& call, bool grad) {
+  const std::vector<int64_t> p = params_of(call);
+  const int64_t rows = p[0], dim = p[1];
+  const bool bias = p[2] != 0;
+  RenderedKernel rk;
+  set_image(rk, fg_image_layer_norm, fg_image_layer_norm_end);
+  const uint64_t blocks = static_cast<uint64_t>(std::min<int64_t>(rows, 65536));
+  for (int i = 0; i < 3; i++) rk.call_args.push_back(CallArg::slot(i));
+  if (!grad) {
+    rk.kind = "layer_norm";
+    rk.launches = {launch("fg_layer_norm", blocks, 256, "layer_norm")};
+    rk.call_args.push_back(bias ? CallArg::slot(3) : CallArg::null());
+  } else {
+    rk.kind = "layer_norm_grad";
+    rk.launches = {launch("fg_layer_norm_grad", blocks, 256, "layer_norm"),
+                   launch("fg_layer_norm_weight", static_cast<uint64_t>((dim + 255) / 256), 256, "layer_norm")};
+    rk.workspace_bytes = static_cast<size_t>(rows) * 8;
+    rk.side_outputs = {4};
+    if (bias) rk.side_outputs.push_back(5);
+    for (CallArg a : {CallArg::slot(3), CallArg::slot(4), bias ? CallArg::slot(5) : CallArg::null(), CallArg::workspace()})
+      rk.call_args.push_back(a);
+  }
+  rk.call_args.push_back(CallArg::i32(rows));
+  rk.call_args.push_back(CallArg::i32(dim));
+  rk.call_args.push_back(CallArg::f32(static_cast<float>(from_bits(p[3]))));
+  return rk;
+}
+
+// ── token_cross_entropy ─────────────────────────────────────────────────────
+// params: rows, classes. Sources: logits, labels; of the gradient also g.
+
+RenderedKernel render_token_loss(const UOp& call, bool grad) {
+  const std::vector<int64_t> p = params_of(call);
+  const uint64_t rows = static_cast<uint64_t>(p[0]);
+  RenderedKernel rk;
+  set_image(rk, fg_image_token_loss, fg_image_token_loss_end);
+  for (int i = 0; i < 3; i++) rk.call_args.push_back(CallArg::slot(i));
+  if (!grad) {
+    rk.kind = "token_loss";
+    rk.launches = {launch("fg_token_loss", std::min<uint64_t>(rows, 65536), 256, "token_cross_entropy"),
+                   launch("fg_token_loss_mean", 1, 256, "token_cross_entropy")};
+    rk.workspace_bytes = rows * 4;
+    rk.call_args.push_back(CallArg::workspace());
+  } else {
+    rk.kind = "token_loss_grad";
+    rk.launches = {launch("fg_token_loss_grad", std::min<uint64_t>(rows, 1024), 256, "token_cross_entropy")};
+    rk.call_args.push_back(CallArg::slot(3));
+  }
+  rk.call_args.push_back(CallArg::i32(p[0]));
+  rk.call_args.push_back(CallArg::i32(p[1]));
+  return rk;
+}
+
+// ── clip_norm ───────────────────────────────────────────────────────────────
+// Square sums' params: workgroups, whether other sums are added, then the
+// tensors' sizes; sources: the tensors, [the other sums]. Their result is
+// as many numbers of 64 bits, two elements each. Clipping's params: bits of
+// max_norm, workgroups of the sums, whether it writes the norm, then the sizes;
+// sources: the tensors, the sums, the storage of its outputs after the first,
+// [of the norm].
+
+constexpr size_t kClipTensors = 64;  // of a launch (kernels/clip.hip)
+constexpr int64_t kClipChunk = 4096;
+// Workgroups of a pass over the tensors: enough to fill the chip, each with some
+// chunks where there are many.
+constexpr int64_t kClipBlocks = 2048;
+
+int64_t clip_chunks(const std::vector<int64_t>& p, size_t first) {
+  int64_t chunks = 0;
+  for (size_t i = first; i < p.size(); i++) chunks += (p[i] + kClipChunk - 1) / kClipChunk;
+  return chunks;
+}
+
+// Addresses and sizes of up to kClipTensors tensors, from slot 1 on.
+std::vector<CallArg> clip_args(const std::vector<int64_t>& p, size_t first) {
+  const size_t count = p.size() - first;
+  std::vector<CallArg> a;
+  for (size_t i = 0; i < kClipTensors; i++) a.push_back(i < count ? CallArg::slot(static_cast<int32_t>(i) + 1) : CallArg::null());
+  for (size_t i = 0; i < kClipTensors; i++) a.push_back(CallArg::bits64(i < count ? p[first + i] : 0));
+  return a;
+}
+
+RenderedKernel render_square_sums(const UOp& call) {
+  const std::vector<int64_t> p = params_of(call);
+  const int32_t count = static_cast<int32_t>(p.size() - 2);
+  RenderedKernel rk;
+  set_image(rk, fg_image_clip, fg_image_clip_end);
+  rk.kind = "square_sums";
+  rk.launches = {launch("fg_square_sums", static_cast<uint64_t>(p[0]), 256, "clip_norm")};
+  rk.call_args = clip_args(p, 2);
+  rk.call_args.push_back(CallArg::slot(0));
+  rk.call_args.push_back(p[1] ? CallArg::slot(count + 1) : CallArg::null());
+  rk.call_args.push_back(CallArg::i32(count));
+  return rk;
+}
+
+RenderedKernel render_norm_of_sums(const UOp& call) {
+  RenderedKernel rk;
+  set_image(rk, fg_image_clip, fg_image_clip_end);
+  rk.kind = "norm_of_sums";
+  rk.launches = {launch("fg_norm_of_sums", 1, 256, "global_norm")};
+  rk.call_args = {CallArg::slot(0), CallArg::slot(1), CallArg::i32(params_of(call)[0])};
+  return rk;
+}
+
+RenderedKernel render_clip(const UOp& call) {
+  const std::vector<int64_t> p = params_of(call);
+  const bool norm = p[2] != 0;
+  const int32_t count = static_cast<int32_t>(p.size() - 3);
+  RenderedKernel rk;
+  set_image(rk, fg_image_clip, fg_image_clip_end);
+  rk.kind = "clip";
+  rk.launches = {launch("fg_clip", static_cast<uint64_t>(std::min(clip_chunks(p, 3), kClipBlocks)), 256, "clip_norm")};
+  rk.call_args = clip_args(p, 3);
+  // Slots: the first output, the tensors, the sums, the further outputs, the norm.
+  for (int32_t i = 0; i < static_cast<int32_t>(kClipTensors); i++)
+    rk.call_args.push_back(i >= count ? CallArg::null() : CallArg::slot(i ? count + 1 + i : 0));
+  for (int32_t i = 1; i < count + norm; i++) rk.side_outputs.push_back(count + 1 + i);
+  rk.call_args.push_back(CallArg::slot(count + 1));
+  rk.call_args.push_back(norm ? CallArg::slot(2 * count + 1) : CallArg::null());
+  rk.call_args.push_back(CallArg::bits64(p[0]));
+  rk.call_args.push_back(CallArg::i32(p[1]));
+  rk.call_args.push_back(CallArg::i32(count));
+  return rk;
+}
+
+// The tensors of a clip as their calls read them.
+std::vector<UOp> clip_sources(const std::vector<Tensor>& tensors, const char* what) {
+  const std::string name = what;
+  FG_CHECK(!tensors.empty(), name + ": there must be at least one tensor");
+  std::vector<UOp> out;
+  uint64_t chunks = 0;
+  for (size_t i = 0; i < tensors.size(); i++) {
+    const Tensor& t = tensors[i];
+    FG_CHECK(t.dtype() == DType::F32(), name + ": tensor " + std::to_string(i) + " must be f32");
+    FG_CHECK(t.numel() > 0, name + ": tensor " + std::to_string(i) + " is empty");
+    FG_CHECK(t.device() == tensors[0].device(), name + ": all tensors must be on the same device");
+    chunks += (t.numel() + kClipChunk - 1) / kClipChunk;
+    out.push_back(source(t.uop()));
+  }
+  // The kernels count chunks in 32 bits, some workgroups' past the last.
+  FG_CHECK(chunks <= (1u << 30), name + ": more than 2^42 elements");
+  need_hip(tensors[0], what);
+  return out;
+}
+
+// The sums of squares of the tensors' chunks, of as many workgroups as `blocks`
+// says: kClipTensors tensors a call.
+UOp square_sums(const std::vector<UOp>& srcs, int64_t* blocks) {
+  int64_t chunks = 0;
+  for (const UOp& u : srcs) chunks += (static_cast<int64_t>(numel(u.shape())) + kClipChunk - 1) / kClipChunk;
+  *blocks = std::min(chunks, kClipBlocks);
+  UOp sums;
+  for (size_t first = 0; first < srcs.size(); first += kClipTensors) {
+    std::vector<UOp> part(srcs.begin() + static_cast<std::ptrdiff_t>(first),
+                          srcs.begin() + static_cast<std::ptrdiff_t>(std::min(srcs.size(), first + kClipTensors)));
+    std::vector<int64_t> params{*blocks, first ? 1 : 0};
+    for (const UOp& u : part) params.push_back(static_cast<int64_t>(numel(u.shape())));
+    if (first) part.push_back(sums);
+    sums = make_call(KernelId::SquareSums, Shape{2 * static_cast<size_t>(*blocks)}, part, params);
+  }
+  return sums;
+}
+
 void check_matrix(const Tensor& t, const char* what) {
   FG_CHECK(t.dtype() == DType::F32(), std::string(what) + " must be f32");
   FG_CHECK(t.ndim() == 2, std::string(what) + " must be 2D (one row per token), got shape " + shape_str(t.shape()));
@@ -477,6 +671,93 @@ Tensor Tensor::dropout(double p, uint64_t seed, uint64_t offset) const {
                   requires_grad());
 }
 
+Tensor Tensor::embedding(const Tensor& ids, double scale) const {
+  FG_CHECK(dtype() == DType::F32(), "embedding: the weight must be f32");
+  FG_CHECK(ndim() == 2, "embedding: the weight must be 2D (one row per id), got shape " + shape_str(shape()));
+  FG_CHECK(numel() > 0, "embedding: the weight is empty");
+  FG_CHECK(ids.dtype() == DType::I32() && ids.ndim() == 1,
+           "embedding: the ids must be i32 of one dimension, got shape " + shape_str(ids.shape()));
+  FG_CHECK(ids.numel() > 0, "embedding: the ids are empty");
+  FG_CHECK(device() == ids.device(), "embedding: all tensors must be on the same device");
+  FG_CHECK(std::isfinite(scale) && std::isfinite(static_cast<float>(scale)), "embedding: scale must be finite");
+  const Shape s = shape();
+  const size_t tokens = ids.numel();
+  // Sizes that the kernels count in 32 bits, some workgroups' past the last.
+  FG_CHECK(s[0] <= (1u << 30) && s[1] <= (1u << 30) && tokens <= (1u << 30), "embedding: more than 2^30 rows, columns or ids");
+  need_hip(*this, "embedding");
+  return from_uop(make_call(KernelId::Embedding, Shape{tokens, s[1]}, {source(uop()), source(ids.uop())},
+                            {static_cast<int64_t>(tokens), static_cast<int64_t>(s[0]), static_cast<int64_t>(s[1]), to_bits(scale)}),
+                  requires_grad());
+}
+
+Tensor Tensor::layer_norm(const Tensor& weight, const Tensor* bias, double eps) const {
+  check_matrix(*this, "layer_norm: the input");
+  FG_CHECK(device() == weight.device() && (!bias || device() == bias->device()), "layer_norm: all tensors must be on the same device");
+  const Shape s = shape();
+  for (const Tensor* t : {&weight, bias})
+    if (t)
+      FG_CHECK(t->dtype() == DType::F32() && t->shape() == Shape{s[1]},
+               std::string("layer_norm: the ") + (t == bias ? "bias" : "weight") + " must be f32 of shape " +
+                   shape_str(Shape{s[1]}) + ", got " + shape_str(t->shape()));
+  // As float32, which the kernels add: infinity would give 0, and 0 NaN for a row of equal numbers.
+  FG_CHECK(eps >= 0 && std::isfinite(static_cast<float>(eps)) && (eps == 0 || static_cast<float>(eps) > 0),
+           "layer_norm: eps must be finite and not negative, and not 0 in float32 unless it is 0");
+  FG_CHECK(s[0] <= (1u << 30) && s[1] <= (1u << 30), "layer_norm: more than 2^30 rows or columns");
+  need_hip(*this, "layer_norm");
+  std::vector<UOp> srcs = {source(uop()), source(weight.uop())};
+  if (bias) srcs.push_back(source(bias->uop()));
+  return from_uop(make_call(KernelId::LayerNorm, s, srcs,
+                            {static_cast<int64_t>(s[0]), static_cast<int64_t>(s[1]), bias != nullptr, to_bits(eps)}),
+                  requires_grad() || weight.requires_grad() || (bias && bias->requires_grad()));
+}
+
+Tensor Tensor::token_cross_entropy(const Tensor& labels) const {
+  check_matrix(*this, "token_cross_entropy: the logits");
+  const Shape s = shape();
+  FG_CHECK(device() == labels.device(), "token_cross_entropy: all tensors must be on the same device");
+  FG_CHECK(labels.dtype() == DType::I32() && labels.shape() == Shape{s[0]},
+           "token_cross_entropy: the labels must be i32 of shape " + shape_str(Shape{s[0]}) + ", got " + shape_str(labels.shape()));
+  FG_CHECK(s[0] <= (1u << 30) && s[1] <= (1u << 30), "token_cross_entropy: more than 2^30 rows or classes");
+  need_hip(*this, "token_cross_entropy");
+  return from_uop(make_call(KernelId::TokenLoss, Shape{1}, {source(uop()), source(labels.uop())},
+                            {static_cast<int64_t>(s[0]), static_cast<int64_t>(s[1])}),
+                  requires_grad());
+}
+
+Tensor Tensor::global_norm(const std::vector<Tensor>& tensors) {
+  int64_t blocks = 0;
+  const UOp sums = square_sums(clip_sources(tensors, "global_norm"), &blocks);
+  return from_uop(make_call(KernelId::NormOfSums, Shape{1}, {sums}, {blocks}), false);
+}
+
+std::pair<Tensor, std::vector<Tensor>> Tensor::clip_norm(const std::vector<Tensor>& tensors, double max_norm) {
+  FG_CHECK(max_norm > 0 && std::isfinite(max_norm), "clip_norm: max_norm must be finite and positive");
+  const std::vector<UOp> all = clip_sources(tensors, "clip_norm");
+  int64_t blocks = 0;
+  const UOp sums = square_sums(all, &blocks);
+  Tensor norm;
+  std::vector<Tensor> out;
+  for (size_t first = 0; first < all.size(); first += kClipTensors) {
+    const size_t count = std::min(kClipTensors, all.size() - first);
+    std::vector<UOp> srcs(all.begin() + static_cast<std::ptrdiff_t>(first), all.begin() + static_cast<std::ptrdiff_t>(first + count));
+    std::vector<int64_t> params{to_bits(max_norm), blocks, first == 0};
+    for (const UOp& u : srcs) params.push_back(static_cast<int64_t>(fg::numel(u.shape())));
+    // A further output is told from other calls' by its tensor, the sums (of
+    // all tensors) and its place.
+    srcs.push_back(sums);
+    std::vector<UOp> storage;
+    for (size_t i = 1; i < count; i++)
+      storage.push_back(output_storage(KernelId::Clip, static_cast<int64_t>(first + i), srcs[i].shape(), {srcs[i], sums}, {to_bits(max_norm)}));
+    if (first == 0) storage.push_back(output_storage(KernelId::Clip, 0, Shape{1}, {sums}, {to_bits(max_norm)}));
+    srcs.insert(srcs.end(), storage.begin(), storage.end());
+    const UOp call = make_call(KernelId::Clip, srcs[0].shape(), srcs, params);
+    out.push_back(from_uop(call, false));
+    for (size_t i = 1; i < count; i++) out.push_back(from_uop(output_of(storage[i - 1], call), false));
+    if (first == 0) norm = from_uop(output_of(storage.back(), call), false);
+  }
+  return {norm, out};
+}
+
 std::vector<UOp> kernel_gradient(const UOp& call, const UOp& grad) {
   switch (static_cast<KernelId>(call.arg().a)) {
     case KernelId::NormRotate: {
@@ -501,8 +782,33 @@ std::vector<UOp> kernel_gradient(const UOp& call, const UOp& grad) {
       grads.resize(call.srcs().size());
       return grads;
     }
+    case KernelId::Embedding: {
+      const Shape weight = call.src(0).shape();
+      return {make_call(KernelId::EmbeddingGrad, weight, {call.src(1), gradient_source(grad)}, params_of(call)), UOp()};
+    }
+    case KernelId::LayerNorm: {
+      const std::vector<int64_t> params = params_of(call);
+      std::vector<UOp> srcs = {call.src(0), call.src(1), gradient_source(grad)}, storage;
+      for (size_t i = 1; i < call.srcs().size(); i++)
+        storage.push_back(output_storage(KernelId::LayerNormGrad, static_cast<int64_t>(i), call.src(1).shape(), srcs, params));
+      srcs.insert(srcs.end(), storage.begin(), storage.end());
+      UOp dx = make_call(KernelId::LayerNormGrad, call.src(0).shape(), srcs, params);
+      std::vector<UOp> grads{dx};
+      for (const UOp& u : storage) grads.push_back(output_of(u, dx));
+      return grads;
+    }
+    case KernelId::TokenLoss: {
+      std::vector<UOp> srcs = {call.src(0), call.src(1), gradient_source(grad)};
+      return {make_call(KernelId::TokenLossGrad, call.src(0).shape(), srcs, params_of(call)), UOp()};
+    }
     case KernelId::NormRotateGrad:
-    case KernelId::AttentionGrad: break;  // no second gradients
+    case KernelId::AttentionGrad:
+    case KernelId::EmbeddingGrad:
+    case KernelId::LayerNormGrad:
+    case KernelId::TokenLossGrad: break;  // no second gradients
+    case KernelId::SquareSums:
+    case KernelId::NormOfSums:
+    case KernelId::Clip: break;  // none through a norm
     case KernelId::Dropout: {
       // The same words again: the mask is never stored.
       std::vector<UOp> srcs = call.srcs();
@@ -521,6 +827,15 @@ RenderedKernel render_hip_call(const UOp& call) {
     case KernelId::NormRotateGrad: rk = render_norm_rotate(call, true); break;
     case KernelId::Attention: rk = render_attention(call, false); break;
     case KernelId::AttentionGrad: rk = render_attention(call, true); break;
+    case KernelId::Embedding: rk = render_embedding(call, false); break;
+    case KernelId::EmbeddingGrad: rk = render_embedding(call, true); break;
+    case KernelId::LayerNorm: rk = render_layer_norm(call, false); break;
+    case KernelId::LayerNormGrad: rk = render_layer_norm(call, true); break;
+    case KernelId::TokenLoss: rk = render_token_loss(call, false); break;
+    case KernelId::TokenLossGrad: rk = render_token_loss(call, true); break;
+    case KernelId::SquareSums: rk = render_square_sums(call); break;
+    case KernelId::NormOfSums: rk = render_norm_of_sums(call); break;
+    case KernelId::Clip: rk = render_clip(call); break;
   }
   rk.name = rk.launches.at(0).func;
   rk.out_slot = 0;

@@ -1,7 +1,8 @@
 // Hand-written kernels behind Tensor methods: attention, per-head norms with
-// the position rotation, dropout. No reference counterpart: the reference
-// composes every op out of its IR, which has no random numbers, no sine and
-// only two-dimensional products.
+// the position rotation, dropout; embedding, layer norm, the loss of token
+// labels, and clipping to a global norm. No reference counterpart: the
+// reference composes every op out of its IR, which has no random numbers, no
+// sine, no indexing by data and only two-dimensional products.
 //
 // A call is one Op::Kernel node whose sources are its arguments: matrices read
 // as whole buffers (the scheduler gives what computes them a kernel of its
@@ -16,7 +17,10 @@
 
 namespace fg {
 
-enum class KernelId : int64_t { Dropout = 0, NormRotate, NormRotateGrad, Attention, AttentionGrad };
+enum class KernelId : int64_t {
+  Dropout = 0, NormRotate, NormRotateGrad, Attention, AttentionGrad, Embedding, EmbeddingGrad, LayerNorm, LayerNormGrad,
+  TokenLoss, TokenLossGrad, SquareSums, NormOfSums, Clip
+};
 
 // The gradients of a call's sources (null where there is none), for
 // gradient_for_op.

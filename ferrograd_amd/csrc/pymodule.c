@@ -303,6 +303,63 @@ static PyObject* t_dropout(TensorObject* self, PyObject* args, PyObject* kw) {
   return wrap(Py_TYPE(self), out);
 }
 
+PyDoc_STRVAR(embedding_doc,
+"embedding(ids, scale=1.0)\n--\n\n"
+"Rows of this weight [vocab, dim] (f32) by id, times scale: [tokens, dim] of ids\n"
+"(an int32 tensor [tokens]). An id outside of [0, vocab) is no token: a row of\n"
+"zeros, and no gradient. The weight's gradient sums its tokens' rows in their\n"
+"order, the same in every run.");
+
+static PyObject* t_embedding(TensorObject* self, PyObject* args, PyObject* kw) {
+  static char* names[] = {"ids", "scale", NULL};
+  PyObject* io;
+  TensorObject* ids;
+  double scale = 1.0;
+  if (!PyArg_ParseTupleAndKeywords(args, kw, "O|d:embedding", names, &io, &scale)) return NULL;
+  if (check_tensor(io, &ids) || !has_handle(self) || !has_handle(ids)) return NULL;
+  fg_tensor* out = NULL;
+  if (fg_tensor_embedding(self->h, ids->h, scale, &out)) return raise_last();
+  return wrap(Py_TYPE(self), out);
+}
+
+PyDoc_STRVAR(layer_norm_doc,
+"layer_norm(weight, bias=None, eps=1e-5)\n--\n\n"
+"Layer norm of each row [rows, dim] (f32): (x - mean) / sqrt(variance + eps) *\n"
+"weight + bias, with weight and bias f32 [dim] (bias None: none).");
+
+static PyObject* t_layer_norm(TensorObject* self, PyObject* args, PyObject* kw) {
+  static char* names[] = {"weight", "bias", "eps", NULL};
+  PyObject *wo, *bo = Py_None;
+  TensorObject *w, *b = NULL;
+  double eps = 1e-5;
+  if (!PyArg_ParseTupleAndKeywords(args, kw, "O|Od:layer_norm", names, &wo, &bo, &eps)) return NULL;
+  if (check_tensor(wo, &w) || (bo != Py_None && check_tensor(bo, &b))) return NULL;
+  if (!has_handle(self) || !has_handle(w) || (b && !has_handle(b))) return NULL;
+  fg_tensor* out = NULL;
+  if (fg_tensor_layer_norm(self->h, w->h, b ? b->h : NULL, eps, &out)) return raise_last();
+  return wrap(Py_TYPE(self), out);
+}
+
+PyDoc_STRVAR(token_cross_entropy_doc,
+"token_cross_entropy(labels)\n--\n\n"
+"The mean of logsumexp(row) - row[label] over the rows of these logits [rows,\n"
+"classes] (f32) whose label (an int32 tensor [rows]) is in [0, classes), as a\n"
+"tensor [1]. Rows of other labels are ignored and get gradients of 0; a loss of 0\n"
+"where all are. With every label valid it is cross_entropy of one-hot rows, which\n"
+"need not be made. Logits of -inf are classes that a row cannot take; a row of\n"
+"nothing else, or with a NaN or +inf, makes the loss and its own gradients NaN.");
+
+static PyObject* t_token_cross_entropy(TensorObject* self, PyObject* args, PyObject* kw) {
+  static char* names[] = {"labels", NULL};
+  PyObject* lo;
+  TensorObject* labels;
+  if (!PyArg_ParseTupleAndKeywords(args, kw, "O:token_cross_entropy", names, &lo)) return NULL;
+  if (check_tensor(lo, &labels) || !has_handle(self) || !has_handle(labels)) return NULL;
+  fg_tensor* out = NULL;
+  if (fg_tensor_token_cross_entropy(self->h, labels->h, &out)) return raise_last();
+  return wrap(Py_TYPE(self), out);
+}
+
 static PyObject* t_realize(TensorObject* self, PyObject* unused) {
   (void)unused;
   if (!has_handle(self)) return NULL;
@@ -346,6 +403,10 @@ static PyMethodDef t_methods[] = {
     {"attention", (PyCFunction)(void (*)(void))t_attention, METH_VARARGS | METH_KEYWORDS, attention_doc},
     {"norm_rotate", (PyCFunction)(void (*)(void))t_norm_rotate, METH_VARARGS | METH_KEYWORDS, norm_rotate_doc},
     {"dropout", (PyCFunction)(void (*)(void))t_dropout, METH_VARARGS | METH_KEYWORDS, dropout_doc},
+    {"embedding", (PyCFunction)(void (*)(void))t_embedding, METH_VARARGS | METH_KEYWORDS, embedding_doc},
+    {"layer_norm", (PyCFunction)(void (*)(void))t_layer_norm, METH_VARARGS | METH_KEYWORDS, layer_norm_doc},
+    {"token_cross_entropy", (PyCFunction)(void (*)(void))t_token_cross_entropy, METH_VARARGS | METH_KEYWORDS,
+     token_cross_entropy_doc},
     {"_u", (PyCFunction)t_u, METH_O, NULL},
     {"_b", (PyCFunction)(void (*)(void))t_b, METH_FASTCALL, NULL},
     {"realize", (PyCFunction)t_realize, METH_NOARGS, "Tensor::realize (tensor.rs:781-830)."},

@@ -186,6 +186,7 @@ std::optional<Tensor> Tensor::grad() const {
   return Tensor(p_->grad);
 }
 void Tensor::clear_grad() const { p_->grad.reset(); }
+void Tensor::set_grad(const Tensor& g) const { p_->grad = g.p_; }
 Tensor Tensor::with_requires_grad(bool rg) const {
   p_->requires_grad = rg;
   return *this;
@@ -1434,6 +1435,18 @@ Sgd::Sgd(const std::vector<Tensor>& ps, float lr_) : lr(lr_) {  // optim.rs:23-4
 
 void Sgd::zero_grad() const {
   for (auto& p : params) p.clear_grad();
+}
+
+Tensor Sgd::clip_grad_norm(double max_norm) const {
+  std::vector<Tensor> grads;
+  for (auto& p : params) {
+    auto g = p.grad();
+    FG_CHECK(g.has_value(), "clip_grad_norm requires parameter gradients");
+    grads.push_back(*g);
+  }
+  auto [norm, clipped] = Tensor::clip_norm(grads, max_norm);
+  for (size_t i = 0; i < params.size(); i++) params[i].set_grad(clipped[i]);
+  return norm;
 }
 
 void Sgd::step() const {  // optim.rs:60-71

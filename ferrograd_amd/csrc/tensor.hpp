@@ -5,6 +5,7 @@
 #include <memory>
 #include <optional>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "device.hpp"
@@ -41,6 +42,7 @@ class Tensor {
   bool requires_grad() const;
   std::optional<Tensor> grad() const;
   void clear_grad() const;
+  void set_grad(const Tensor& g) const;
   Tensor with_requires_grad(bool rg) const;
   Tensor detach() const;
   Tensor replace(const Tensor& other) const;
@@ -85,6 +87,19 @@ class Tensor {
   Tensor attention(const Tensor& k, const Tensor& v, const Tensor* lengths, size_t batch, size_t heads, size_t kv_heads,
                    bool causal, double scale) const;
   Tensor dropout(double p, uint64_t seed, uint64_t offset) const;
+  // Rows of *this = weight [vocab, dim] by id (i32 [tokens]), times scale; an id
+  // outside of [0, vocab) gives a row of zeros.
+  Tensor embedding(const Tensor& ids, double scale) const;
+  // (x - mean) / sqrt(variance + eps) of each row, times weight [dim], plus bias
+  // [dim] (or null).
+  Tensor layer_norm(const Tensor& weight, const Tensor* bias, double eps) const;
+  // The mean over the rows whose label (i32 [rows]) is in [0, classes) of
+  // logsumexp(row) - row[label], with *this = logits [rows, classes].
+  Tensor token_cross_entropy(const Tensor& labels) const;
+  // The root of the sum of all tensors' squares, and the tensors times max_norm
+  // / max(norm, max_norm). No gradients flow through either.
+  static Tensor global_norm(const std::vector<Tensor>& tensors);
+  static std::pair<Tensor, std::vector<Tensor>> clip_norm(const std::vector<Tensor>& tensors, double max_norm);
 
   // Realisation (tensor.rs:781-930).
   static void realize_many(const std::vector<Tensor>& tensors);
@@ -145,6 +160,9 @@ struct Sgd {
   mutable std::vector<std::pair<DeviceId, Tensor>> lr_buffers;
   Sgd(const std::vector<Tensor>& params, float lr);
   void zero_grad() const;
+  // Gradients of a larger norm (of all elements together) are scaled to
+  // max_norm; the norm they had. No reference counterpart.
+  Tensor clip_grad_norm(double max_norm) const;
   void step() const;
 };
 

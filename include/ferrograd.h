@@ -87,6 +87,39 @@ int fg_tensor_norm_rotate(fg_tensor* x, fg_tensor* weight, fg_tensor* positions,
  * device only. No reference counterpart. */
 int fg_tensor_dropout(fg_tensor* t, double p, uint64_t seed, uint64_t offset, fg_tensor** out);
 
+/* Rows of weight [vocab, dim] (f32) by id, times scale: [tokens, dim] of ids
+ * (i32 [tokens]). An id outside of [0, vocab) is no token: it gives a row of
+ * zeros and has no gradient. The weight's gradient sums its tokens' rows in
+ * their order, without atomics: the same in every run. HIP device only. No
+ * reference counterpart. */
+int fg_tensor_embedding(fg_tensor* weight, fg_tensor* ids, double scale, fg_tensor** out);
+
+/* Layer norm of each row of x [rows, dim] (f32): (x - mean(x)) *
+ * (mean((x - mean(x))^2) + eps)^(-1/2) * weight + bias, weight and bias f32 [dim]
+ * (bias NULL: none). Gradients flow to all three. HIP device only. No reference
+ * counterpart. */
+int fg_tensor_layer_norm(fg_tensor* x, fg_tensor* weight, fg_tensor* bias, double eps, fg_tensor** out);
+
+/* Cross-entropy of labels: the mean of logsumexp(row) - row[label] over the rows
+ * of logits [rows, classes] (f32) whose label (i32 [rows]) is in [0, classes);
+ * the other rows are ignored, and get gradients of 0. 0 where all are. With every
+ * label valid it is fg_tensor_binary's FG_BINARY_CROSS_ENTROPY of the labels as
+ * one-hot rows, which need not be written. A class that no row may take can
+ * have logits of -infinity; a row of nothing else, or with a NaN or +infinity,
+ * makes the loss and its own gradients NaN. HIP device only. No reference
+ * counterpart. */
+int fg_tensor_token_cross_entropy(fg_tensor* logits, fg_tensor* labels, fg_tensor** out);
+
+/* The root of the sum of the squares of all elements of n tensors (f32, any
+ * shapes), as a tensor [1]; squares and sums are f64. The same tensor given twice
+ * counts twice. No gradient flows through it. HIP device only. No reference
+ * counterpart. */
+int fg_global_norm(fg_tensor* const* ts, int n, fg_tensor** out);
+/* That norm, and every tensor times max_norm / max(norm, max_norm) (max_norm
+ * finite and above 0) into outs[0, n). A norm of NaN makes them NaN, one of
+ * infinity 0 (NaN where a tensor is infinite). */
+int fg_clip_norm(fg_tensor* const* ts, int n, double max_norm, fg_tensor** norm, fg_tensor** outs);
+
 /* In-place graph updates (tensor.rs:399-440). */
 int fg_tensor_assign(fg_tensor* t, fg_tensor* value);
 int fg_tensor_replace(fg_tensor* t, fg_tensor* value);
@@ -150,6 +183,10 @@ int fg_mlp_train_batches(fg_linear* const* layers, int nlayers, fg_sgd* opt, fg_
 /* optim::Sgd (optim.rs:16-71). */
 int fg_sgd_new(fg_tensor** params, int n, float lr, fg_sgd** out);
 int fg_sgd_zero_grad(fg_sgd* s);
+/* Between the backward pass and the step: the parameters' gradients clipped as
+ * by fg_clip_norm, together; *norm is the norm they had. No reference
+ * counterpart. */
+int fg_sgd_clip_grad_norm(fg_sgd* s, double max_norm, fg_tensor** norm);
 int fg_sgd_step(fg_sgd* s);
 int fg_sgd_free(fg_sgd* s);
 

@@ -209,6 +209,12 @@ extern "C" {
     pub fn fg_tensor_attention(q: *mut fg_tensor, k: *mut fg_tensor, v: *mut fg_tensor, lengths: *mut fg_tensor, batch: i64, heads: i64, kv_heads: i64, causal: i32, scale: f64, out: *mut *mut fg_tensor) -> i32;
     pub fn fg_tensor_norm_rotate(x: *mut fg_tensor, weight: *mut fg_tensor, positions: *mut fg_tensor, heads: i64, eps: f64, base: f64, out: *mut *mut fg_tensor) -> i32;
     pub fn fg_tensor_dropout(t: *mut fg_tensor, p: f64, seed: u64, offset: u64, out: *mut *mut fg_tensor) -> i32;
+    pub fn fg_tensor_embedding(weight: *mut fg_tensor, ids: *mut fg_tensor, scale: f64, out: *mut *mut fg_tensor) -> i32;
+    pub fn fg_tensor_layer_norm(x: *mut fg_tensor, weight: *mut fg_tensor, bias: *mut fg_tensor, eps: f64, out: *mut *mut fg_tensor) -> i32;
+    pub fn fg_tensor_token_cross_entropy(logits: *mut fg_tensor, labels: *mut fg_tensor, out: *mut *mut fg_tensor) -> i32;
+    pub fn fg_global_norm(ts: *const *mut fg_tensor, n: i32, out: *mut *mut fg_tensor) -> i32;
+    pub fn fg_clip_norm(ts: *const *mut fg_tensor, n: i32, max_norm: f64, norm: *mut *mut fg_tensor,
+                        outs: *mut *mut fg_tensor) -> i32;
     pub fn fg_tensor_log_softmax(t: *mut fg_tensor, axis: i64, out: *mut *mut fg_tensor) -> i32;
     pub fn fg_tensor_assign(t: *mut fg_tensor, value: *mut fg_tensor) -> i32;
     pub fn fg_tensor_replace(t: *mut fg_tensor, value: *mut fg_tensor) -> i32;
@@ -238,6 +244,7 @@ extern "C" {
                                 images: *mut fg_tensor, targets: *mut fg_tensor, batch_size: i64,
                                 first_batch: i64, steps: i32, losses: *mut f32) -> i32;
     pub fn fg_sgd_new(params: *mut *mut fg_tensor, n: i32, lr: f32, out: *mut *mut fg_sgd) -> i32;
+    pub fn fg_sgd_clip_grad_norm(s: *mut fg_sgd, max_norm: f64, norm: *mut *mut fg_tensor) -> i32;
     pub fn fg_sgd_zero_grad(s: *mut fg_sgd) -> i32;
     pub fn fg_sgd_step(s: *mut fg_sgd) -> i32;
     pub fn fg_sgd_free(s: *mut fg_sgd) -> i32;
