@@ -64,19 +64,19 @@ struct LaunchSpec {
 // One argument of a hand-written kernel's launches, in the order of its
 // signature: a parameter slot of the call (a buffer, or a scalar that changes
 // from call to call), a number fixed by the call's shapes (of 32 bits, or of the
-// 64 that a pointer has), a null pointer (an absent input), or the device's
-// workspace.
+// 64 that a pointer has), a null pointer (an absent input), or a place in the
+// device's workspace.
 struct CallArg {
   enum class Kind : uint8_t { Slot, I32, F32, Bits64, Null, Workspace } kind = Kind::Null;
   int32_t i = 0;  // the slot, or the number
   float f = 0.f;
-  int64_t bits = 0;
+  int64_t bits = 0;  // the number of 64, or the place
   static CallArg slot(int32_t s) { CallArg a; a.kind = Kind::Slot; a.i = s; return a; }
   static CallArg i32(int64_t v) { CallArg a; a.kind = Kind::I32; a.i = static_cast<int32_t>(v); return a; }
   static CallArg f32(float v) { CallArg a; a.kind = Kind::F32; a.f = v; return a; }
   static CallArg bits64(int64_t v) { CallArg a; a.kind = Kind::Bits64; a.bits = v; return a; }
   static CallArg null() { return CallArg(); }
-  static CallArg workspace() { CallArg a; a.kind = Kind::Workspace; return a; }
+  static CallArg workspace(uint64_t at = 0) { CallArg a; a.kind = Kind::Workspace; a.bits = static_cast<int64_t>(at); return a; }
 };
 
 // What a renderer hands to `Device::compile`: the source and everything the

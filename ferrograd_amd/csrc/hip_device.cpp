@@ -243,7 +243,7 @@ class HipDevice : public Device {
         case CallArg::Kind::F32: x.kind = FG_ARG_F32; x.v.f = ca.f; break;
         case CallArg::Kind::Bits64: x.kind = FG_ARG_PTR; std::memcpy(&x.v.p, &ca.bits, 8); break;
         case CallArg::Kind::Null: x.kind = FG_ARG_PTR; break;
-        case CallArg::Kind::Workspace: x.kind = FG_ARG_PTR; x.v.p = workspace(p.meta.workspace_bytes); break;
+        case CallArg::Kind::Workspace: x.kind = FG_ARG_PTR; x.v.p = static_cast<char*>(workspace(p.meta.workspace_bytes)) + ca.bits; break;
       }
       a.push_back(x);
     }

@@ -1,40 +1,377 @@
 // Rows of an embedding by token, scaled, and the weight's gradient.
 //
 //   y_t = s W[id_t],  dW_v = s sum over the tokens t with id_t = v of g_t,
-// in the order of t. An id outside of [0, vocab) is no token: its row is of
-// zeros, and it has no gradient.
+// in an order that the ids alone decide. An id outside of [0, vocab) is no
+// token: its row is of zeros, and it has no gradient.
+//
+// Both are bound by memory: the lookup reads and writes each token's row once,
+// the gradient reads each token's row once and writes every row of dW.
+//
+// Gradient. The tokens are sorted by id, those of an id in their own order,
+// while other workgroups of the same launches fill dW with zeros. Then the
+// sorted tokens are cut into chunks of one length, however many of them are of
+// one id: a group of lanes sums a chunk's rows, writes the sum of an id that
+// begins and ends within it to dW, and that of one which goes over its ends to
+// the workspace, where a last launch joins it with its other parts. So a padding
+// token that is a third of the batch costs no more than any other.
+//
+// 65536 tokens of 2048 columns, 50001 rows, a third of the tokens one: lookup 150
+// us (1.07 GB through the Infinity Cache, 5.9 TB/s of the output and the rows that
+// differ would be 110), sort and zeros 64 (6.4 TB/s of zeros; the sort alone would
+// take 24), sums 130 (5.2 TB/s; 174 with loads that stay in the caches), joins 12.
+// What is written twice, the rows that have tokens, is 120 MB of 1.2 GB.
 #include <hip/hip_runtime.h>
+
+#include "vectors.hpp"
 
 namespace {
 
-constexpr int kThreads = 256;
+// A row in slices of G * VEC columns, a slice on G lanes. The last lane of a row
+// begins where its vector ends with the row: what it shares with the lane before
+// it is the same value again.
+template <int VEC, int G>
+__device__ inline int column(int slice, int dim) {
+  return min((slice * G + static_cast<int>(threadIdx.x) % G) * VEC, dim - VEC);
+}
 
-}  // namespace
+constexpr int kRows = 4;  // tokens that a group of lanes looks up at a time
 
-extern "C" __global__ void __launch_bounds__(kThreads)
-    fg_embedding(float* out, const float* weight, const int* ids, int tokens, int vocab, int dim, float scale) {
-  for (int t = blockIdx.x; t < tokens; t += gridDim.x) {
-    const int id = ids[t];
-    const bool inside = id >= 0 && id < vocab;
-    const float* from = weight + static_cast<size_t>(inside ? id : 0) * dim;
-    float* to = out + static_cast<size_t>(t) * dim;
-    for (int c = threadIdx.x; c < dim; c += kThreads) to[c] = inside ? from[c] * scale : 0.f;
+template <int VEC, int G, bool Stream>
+__device__ inline void lookup(float* __restrict__ out, const float* __restrict__ weight, const int* __restrict__ ids,
+                              int tokens, int vocab, int dim, int slices, float scale) {
+  const unsigned group = (blockIdx.x * 256u + threadIdx.x) / G;
+  const int slice = static_cast<int>(group % slices), first = static_cast<int>(group / slices) * kRows;
+  if (first >= tokens) return;
+  const int at = column<VEC, G>(slice, dim);
+  int id[kRows];
+#pragma unroll
+  for (int k = 0; k < kRows; k++) id[k] = ids[min(first + k, tokens - 1)];
+  Vec<VEC> v[kRows];
+#pragma unroll
+  for (int k = 0; k < kRows; k++)
+    v[k] = load<VEC>(weight + static_cast<size_t>(static_cast<unsigned>(id[k]) < static_cast<unsigned>(vocab) ? id[k] : 0) * dim + at);
+#pragma unroll
+  for (int k = 0; k < kRows; k++) {
+    if (first + k >= tokens) return;
+    const bool inside = static_cast<unsigned>(id[k]) < static_cast<unsigned>(vocab);
+#pragma unroll
+    for (int e = 0; e < VEC; e++) v[k].v[e] = inside ? v[k].v[e] * scale : 0.f;
+    store<VEC, Stream>(out + static_cast<size_t>(first + k) * dim + at, v[k]);
   }
 }
 
-// A workgroup goes through all ids for each of its rows.
-extern "C" __global__ void __launch_bounds__(kThreads)
-    fg_embedding_grad(float* dw, const int* ids, const float* g, int tokens, int vocab, int dim, float scale) {
-  const int lane = threadIdx.x % 64;
-  for (int v = blockIdx.x; v < vocab; v += gridDim.x)
-    for (int c0 = 0; c0 < dim; c0 += kThreads) {
-      const int c = c0 + threadIdx.x;
-      float sum = 0.f;
-      for (int t0 = 0; t0 < tokens; t0 += 64) {
-        unsigned long long mine = __ballot(t0 + lane < tokens && ids[min(t0 + lane, tokens - 1)] == v);
-        for (; mine; mine &= mine - 1)
-          if (c < dim) sum += g[static_cast<size_t>(t0 + __ffsll(mine) - 1) * dim + c];
-      }
-      if (c < dim) dw[static_cast<size_t>(v) * dim + c] = sum * scale;
-    }
+// ── the tokens in the order of their ids ────────────────────────────────────
+
+// The key that a token is sorted by: its id, or `vocab` where it is none.
+__device__ inline unsigned key_of(int id, int vocab) { return min(static_cast<unsigned>(id), static_cast<unsigned>(vocab)); }
+
+// Part `part` of `parts` of dW set to zero, by the workgroups from `first` on.
+__device__ inline void fill(float* __restrict__ dw, int vocab, int dim, int first, int part, int parts) {
+  typedef float floatx4 __attribute__((ext_vector_type(4)));
+  const size_t n = static_cast<size_t>(vocab) * dim, vectors = n / 4, per = (vectors + parts - 1) / parts;
+  const size_t end = part + 1 == parts ? vectors : per * (part + 1), step = static_cast<size_t>(gridDim.x - first) * blockDim.x;
+  floatx4* to = reinterpret_cast<floatx4*>(dw);
+  for (size_t i = per * part + static_cast<size_t>(blockIdx.x - first) * blockDim.x + threadIdx.x; i < end; i += step)
+    to[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+  if (part == 0 && blockIdx.x == static_cast<unsigned>(first) && threadIdx.x < n % 4) dw[4 * vectors + threadIdx.x] = 0.f;
 }
+
+constexpr int kRankThreads = 1024;
+
+// Of up to 16384 tokens: a token's place is the number of tokens before it in
+// the order, all of which are looked at. A workgroup ranks 64 tokens, one a
+// lane, each of its waves against a part of all, which come through the scalar
+// cache: two vector instructions for 64 pairs.
+__device__ inline void rank_tokens(int2* __restrict__ sorted, const int* __restrict__ ids, int tokens, int vocab) {
+  __shared__ int places[kRankThreads / 64][64];
+  typedef const __attribute__((address_space(4))) int* Scalars;
+  const Scalars all = (Scalars)ids;
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int block = blockIdx.x, t = block * 64 + lane;
+  const unsigned mine = t < tokens ? key_of(ids[t], vocab) : 0;
+  const int blocks = (tokens + 63) / 64, per = (blocks + kRankThreads / 64 - 1) / (kRankThreads / 64);
+  int before = 0;
+  for (int b = wave * per; b < min((wave + 1) * per, blocks); b++) {
+    const int u0 = b * 64;
+    if (b == block || u0 + 64 > tokens) {  // one after the other through a vector register
+      const unsigned theirs = key_of(ids[min(u0 + lane, tokens - 1)], vocab);
+      const int n = min(64, tokens - u0), equal = b < block ? 64 : b == block ? lane : 0;
+#pragma unroll 8
+      for (int j = 0; j < n; j++) {
+        const unsigned u = __builtin_amdgcn_readlane(theirs, j);
+        before += u < mine || (u == mine && j < equal);
+      }
+    } else if (b < block) {
+#pragma unroll 32
+      for (int j = 0; j < 64; j++) before += key_of(all[u0 + j], vocab) <= mine;
+    } else {
+#pragma unroll 32
+      for (int j = 0; j < 64; j++) before += key_of(all[u0 + j], vocab) < mine;
+    }
+  }
+  places[wave][lane] = before;
+  __syncthreads();
+  if (wave != 0 || t >= tokens) return;
+  before = 0;
+#pragma unroll
+  for (int w = 0; w < kRankThreads / 64; w++) before += places[w][lane];
+  sorted[before] = make_int2(static_cast<int>(mine), t);
+}
+
+// Of more: passes over digits of the key from the lowest on, each keeping the
+// order of tokens that it does not tell apart. A workgroup takes a tile of
+// tokens; one launch counts the digits of every tile, the next one places them.
+constexpr int kSortThreads = 1024, kWaves = kSortThreads / 64, kItems = 4, kTile = kSortThreads * kItems;
+constexpr int kMaxDigits = 1024;
+
+// Token i of a pass: of the first from the ids, later from the last one's order.
+__device__ inline int2 token_at(const int2* from, const int* ids, int i, int vocab) {
+  return from ? from[i] : make_int2(static_cast<int>(key_of(ids[i], vocab)), i);
+}
+
+__device__ inline void count_digits(int* __restrict__ table, const int2* __restrict__ from, const int* __restrict__ ids,
+                                    int tokens, int vocab, int shift, int bits) {
+  __shared__ int count[kMaxDigits];
+  const int digits = 1 << bits;
+  for (int d = threadIdx.x; d < digits; d += kSortThreads) count[d] = 0;
+  __syncthreads();
+  for (int k = 0; k < kItems; k++) {
+    const int i = blockIdx.x * kTile + k * kSortThreads + threadIdx.x;
+    if (i < tokens) atomicAdd(&count[(token_at(from, ids, i, vocab).x >> shift) & (digits - 1)], 1);
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < digits; d += kSortThreads) table[blockIdx.x * digits + d] = count[d];
+}
+
+__device__ inline void place_tokens(int2* __restrict__ to, const int* __restrict__ table, const int2* __restrict__ from,
+                                    const int* __restrict__ ids, int tokens, int vocab, int shift, int bits, int tiles) {
+  // Of each wave's digits: how many so far, then how many of the tile's are before them.
+  __shared__ int count[kWaves][kMaxDigits];
+  __shared__ int base[kMaxDigits], part[kWaves];
+  const int digits = 1 << bits, lane = threadIdx.x % 64, wave = threadIdx.x / 64, d = threadIdx.x;
+  if (d < digits)
+    for (int w = 0; w < kWaves; w++) count[w][d] = 0;
+  // Where the digit's tokens of this tile begin: after all tokens of lower digits
+  // and the earlier tiles' of this one. One digit a thread.
+  int all = 0, earlier = 0;
+  if (d < digits)
+#pragma unroll 8
+    for (int b = 0; b < tiles; b++) {
+      const int n = table[b * digits + d];
+      all += n;
+      earlier += b < static_cast<int>(blockIdx.x) ? n : 0;
+    }
+  int lower = all;
+#pragma unroll
+  for (int k = 1; k < 64; k *= 2) {
+    const int x = __shfl_up(lower, k);
+    if (lane >= k) lower += x;
+  }
+  if (lane == 63) part[wave] = lower;
+  __syncthreads();
+  lower -= all;
+  for (int w = 0; w < wave; w++) lower += part[w];
+  if (d < digits) base[d] = lower + earlier;
+  // A wave's tokens in their order, 64 at a time; those of one digit find each
+  // other by ballots, and the first of them adds them to the wave's count.
+  int2 token[kItems];
+  int digit[kItems], place[kItems];
+#pragma unroll
+  for (int k = 0; k < kItems; k++) {
+    const int i = blockIdx.x * kTile + (wave * kItems + k) * 64 + lane;
+    token[k] = token_at(from, ids, min(i, tokens - 1), vocab);
+    digit[k] = i < tokens ? (token[k].x >> shift) & (digits - 1) : -1;
+  }
+#pragma unroll
+  for (int k = 0; k < kItems; k++) {
+    unsigned long long same = __ballot(digit[k] >= 0);
+    for (int b = 0; b < bits; b++) {
+      const bool set = (digit[k] >> b) & 1;
+      const unsigned long long ones = __ballot(set);
+      same &= set ? ones : ~ones;
+    }
+    if (digit[k] < 0) same = 1ull << lane;
+    const int leader = __ffsll(same) - 1;
+    int n = 0;
+    if (digit[k] >= 0 && lane == leader) n = atomicAdd(&count[wave][digit[k]], __popcll(same));
+    place[k] = __shfl(n, leader) + __popcll(same & ((1ull << lane) - 1));
+  }
+  __syncthreads();
+  if (d < digits) {
+    int n = 0;
+    for (int w = 0; w < kWaves; w++) {
+      const int x = count[w][d];
+      count[w][d] = n;
+      n += x;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kItems; k++)
+    if (digit[k] >= 0) to[base[digit[k]] + count[wave][digit[k]] + place[k]] = token[k];
+}
+
+// ── their rows, summed ──────────────────────────────────────────────────────
+
+constexpr int kBatch = 8;  // rows on their way at a time
+
+// A chunk's parts in the workspace: [chunk][of an id that began before it, of one
+// that goes on after it][dim].
+template <int VEC, int G, bool Stream>
+__device__ inline void sum_chunks(float* __restrict__ dw, const float* __restrict__ g, const int2* __restrict__ sorted,
+                                  float* __restrict__ parts, int tokens, int vocab, int dim, int slices, int chunk, int chunks,
+                                  float scale) {
+  const unsigned group = (blockIdx.x * 256u + threadIdx.x) / G;
+  const int slice = static_cast<int>(group % slices), c = static_cast<int>(group / slices);
+  if (c >= chunks) return;
+  const int at = column<VEC, G>(slice, dim), begin = c * chunk, end = min(begin + chunk, tokens);
+  int id = sorted[begin].x;
+  if (id >= vocab) return;  // and all behind it
+  bool before = begin > 0 && sorted[begin - 1].x == id;
+  const int next = end < tokens ? sorted[end].x : vocab;
+  Vec<VEC> sum{};
+  auto flush = [&](bool after) {
+    if (before || after) {
+      store<VEC>(parts + (static_cast<size_t>(c) * 2 + (before ? 0 : 1)) * dim + at, sum);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; e++) sum.v[e] *= scale;
+      store<VEC>(dw + static_cast<size_t>(id) * dim + at, sum);
+    }
+  };
+  for (int i0 = begin; i0 < end; i0 += kBatch) {
+    int2 token[kBatch];
+    Vec<VEC> v[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; k++) token[k] = sorted[min(i0 + k, end - 1)];
+#pragma unroll
+    for (int k = 0; k < kBatch; k++) v[k] = load<VEC, Stream>(g + static_cast<size_t>(token[k].y) * dim + at);
+#pragma unroll
+    for (int k = 0; k < kBatch; k++) {
+      if (i0 + k >= end || token[k].x >= vocab) break;
+      if (token[k].x != id) {
+        flush(false);
+        before = false;
+        id = token[k].x;
+        sum = v[k];
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; e++) sum.v[e] += v[k].v[e];
+      }
+    }
+  }
+  flush(next == id);
+}
+
+constexpr int kJoinThreads = 256;
+
+// An id that begins in chunk c and goes on: its parts, in 64 bits, those of the
+// later chunks shared out to the workgroup's groups of lanes.
+template <int VEC, int G>
+__device__ inline void join_chunks(float* __restrict__ dw, const int2* __restrict__ sorted, const float* __restrict__ parts,
+                                   int tokens, int vocab, int dim, int slices, int chunk, int chunks, float scale) {
+  constexpr int kGroups = kJoinThreads / G;
+  __shared__ double sums[kGroups][G * VEC];
+  const int slice = static_cast<int>(blockIdx.x) % slices, c = static_cast<int>(blockIdx.x) / slices;
+  const int begin = c * chunk, end = begin + chunk, id = sorted[end].x;
+  if (id >= vocab || sorted[end - 1].x != id || (begin > 0 && sorted[begin].x == id && sorted[begin - 1].x == id)) return;
+  // The chunks that begin with it.
+  int more = 0;
+  for (unsigned long long all = ~0ull; all == ~0ull;) {
+    const int d = c + 1 + more + static_cast<int>(threadIdx.x) % 64;
+    all = __ballot(d < chunks && sorted[min(d, chunks - 1) * chunk].x == id);
+    more += all == ~0ull ? 64 : __ffsll(~all) - 1;
+  }
+  const int at = column<VEC, G>(slice, dim), group = threadIdx.x / G, lane = threadIdx.x % G;
+  double sum[VEC] = {};
+  const float* of = parts + static_cast<size_t>(c) * 2 * dim + at;
+  if (group == 0) {
+    const Vec<VEC> v = load<VEC>(of + dim);
+#pragma unroll
+    for (int e = 0; e < VEC; e++) sum[e] = v.v[e];
+  }
+#pragma unroll 8
+  for (int k = group; k < more; k += kGroups) {
+    const Vec<VEC> v = load<VEC>(of + static_cast<size_t>(k + 1) * 2 * dim);
+#pragma unroll
+    for (int e = 0; e < VEC; e++) sum[e] += v.v[e];
+  }
+#pragma unroll
+  for (int e = 0; e < VEC; e++) sums[group][lane * VEC + e] = sum[e];
+  __syncthreads();
+  if (group != 0) return;
+  Vec<VEC> total;
+#pragma unroll
+  for (int e = 0; e < VEC; e++) {
+    double t = 0.0;
+    for (int k = 0; k < kGroups; k++) t += sums[k][lane * VEC + e];
+    total.v[e] = static_cast<float>(t * scale);
+  }
+  store<VEC>(dw + static_cast<size_t>(id) * dim + at, total);
+}
+
+}  // namespace
+
+#define FG_LOOKUP_AS(VEC, G, NAME, STREAM)                                                                             \
+  extern "C" __global__ void __launch_bounds__(256) fg_embedding_##NAME(                                               \
+      float* out, const float* weight, const int* ids, int tokens, int vocab, int dim, int slices, float scale) {      \
+    lookup<VEC, G, STREAM>(out, weight, ids, tokens, vocab, dim, slices, scale);                                       \
+  }
+
+// Of the gradient's launches: `sort` workgroups that sort, before those that fill;
+// the sorted tokens are at `sorted`, of digits of `bits` bits; `other` is the
+// second place of tokens, `table` the counts of digits.
+#define FG_GRAD_ARGS                                                                                                    \
+  float *dw, const int *ids, const float *g, int2 *sorted, int2 *other, int *table, float *parts, int tokens, int vocab, \
+      int dim, int slices, int chunk, int chunks, int sort, int bits, float scale
+
+#define FG_SUM_AS(VEC, G, NAME, STREAM)                                                                                 \
+  extern "C" __global__ void __launch_bounds__(256) fg_embedding_grad_sum_##NAME(FG_GRAD_ARGS) {                        \
+    sum_chunks<VEC, G, STREAM>(dw, g, sorted, parts, tokens, vocab, dim, slices, chunk, chunks, scale);                 \
+  }
+
+#define FG_EMBEDDING(VEC, G)                                                                                            \
+  FG_LOOKUP_AS(VEC, G, VEC##_##G, false)                                                                                \
+  FG_LOOKUP_AS(VEC, G, VEC##_##G##_stream, true)                                                                        \
+  FG_SUM_AS(VEC, G, VEC##_##G, false)                                                                                   \
+  FG_SUM_AS(VEC, G, VEC##_##G##_stream, true)                                                                           \
+  extern "C" __global__ void __launch_bounds__(kJoinThreads) fg_embedding_grad_join_##VEC##_##G(FG_GRAD_ARGS) {         \
+    join_chunks<VEC, G>(dw, sorted, parts, tokens, vocab, dim, slices, chunk, chunks, scale);                           \
+  }
+
+FG_EMBEDDING(1, 8)
+FG_EMBEDDING(4, 8)
+FG_EMBEDDING(4, 16)
+FG_EMBEDDING(4, 32)
+FG_EMBEDDING(4, 64)
+
+extern "C" __global__ void __launch_bounds__(kRankThreads) fg_embedding_grad_rank(FG_GRAD_ARGS) {
+  if (static_cast<int>(blockIdx.x) < sort) rank_tokens(sorted, ids, tokens, vocab);
+  else fill(dw, vocab, dim, sort, 0, 1);
+}
+
+// Pass P of `PASSES`: the tokens go from place to place so that the last pass
+// leaves them at `sorted`.
+#define FG_SORT(P, PASSES)                                                                                              \
+  extern "C" __global__ void __launch_bounds__(kSortThreads) fg_embedding_grad_count_##P##_##PASSES(FG_GRAD_ARGS) {     \
+    const int2* from = P == 0 ? nullptr : (PASSES - P) % 2 ? other : sorted;                                            \
+    if (static_cast<int>(blockIdx.x) < sort) count_digits(table, from, ids, tokens, vocab, P * bits, bits);             \
+    else fill(dw, vocab, dim, sort, 2 * P, 2 * PASSES);                                                                 \
+  }                                                                                                                     \
+  extern "C" __global__ void __launch_bounds__(kSortThreads) fg_embedding_grad_place_##P##_##PASSES(FG_GRAD_ARGS) {     \
+    const int2* from = P == 0 ? nullptr : (PASSES - P) % 2 ? other : sorted;                                            \
+    if (static_cast<int>(blockIdx.x) < sort)                                                                            \
+      place_tokens((PASSES - P) % 2 ? sorted : other, table, from, ids, tokens, vocab, P * bits, bits, sort);           \
+    else fill(dw, vocab, dim, sort, 2 * P + 1, 2 * PASSES);                                                             \
+  }
+
+FG_SORT(0, 1)
+FG_SORT(0, 2)
+FG_SORT(1, 2)
+FG_SORT(0, 3)
+FG_SORT(1, 3)
+FG_SORT(2, 3)
+FG_SORT(0, 4)
+FG_SORT(1, 4)
+FG_SORT(2, 4)
+FG_SORT(3, 4)

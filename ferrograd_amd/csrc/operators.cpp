@@ -402,21 +402,73 @@ RenderedKernel render_attention(const UOp& call, bool grad) {
 // params: tokens, vocab, dim, bits of scale. Sources: weight, ids; of the
 // gradient ids, g.
 
+// Rows in slices of `lanes` times `vec` columns.
+struct ColumnSplit {
+  int64_t vec, lanes, slices;
+  std::string suffix() const { return "_" + std::to_string(vec) + "_" + std::to_string(lanes); }
+};
+
+ColumnSplit column_split(int64_t dim) {
+  ColumnSplit r{dim < 4 ? 1 : 4, 8, 1};
+  while (r.lanes < 64 && r.lanes * r.vec < dim) r.lanes *= 2;
+  r.slices = (dim + r.lanes * r.vec - 1) / (r.lanes * r.vec);
+  return r;
+}
+
+constexpr int64_t kSortTile = 4096, kSortDigitBits = 10, kRankTokens = 16384;  // kernels/embedding.hip
+
 RenderedKernel render_embedding(const UOp& call, bool grad) {
   const std::vector<int64_t> p = params_of(call);
-  const int64_t tokens = p[0], vocab = p[1];
+  const int64_t tokens = p[0], vocab = p[1], dim = p[2];
+  const ColumnSplit split = column_split(dim);
+  const float scale = static_cast<float>(from_bits(p[3]));
   RenderedKernel rk;
   set_image(rk, fg_image_embedding, fg_image_embedding_end);
+  for (int i = 0; i < 3; i++) rk.call_args.push_back(CallArg::slot(i));
   if (!grad) {
     rk.kind = "embedding";
-    rk.launches = {launch("fg_embedding", static_cast<uint64_t>(std::min<int64_t>(tokens, 65536)), 256, "embedding")};
-  } else {
-    rk.kind = "embedding_grad";
-    rk.launches = {launch("fg_embedding_grad", static_cast<uint64_t>(std::min<int64_t>(vocab, 65536)), 256, "embedding")};
+    const uint64_t groups = static_cast<uint64_t>((tokens + 3) / 4 * split.slices);  // of four tokens each
+    rk.launches = {launch("fg_embedding" + split.suffix() + (4 * tokens * dim >= static_cast<int64_t>(kStreamBytes) ? "_stream" : ""),
+                          (groups * static_cast<uint64_t>(split.lanes) + 255) / 256, 256, "embedding")};
+    for (int64_t x : {tokens, vocab, dim, split.slices}) rk.call_args.push_back(CallArg::i32(x));
+    rk.call_args.push_back(CallArg::f32(scale));
+    return rk;
   }
-  for (int i = 0; i < 3; i++) rk.call_args.push_back(CallArg::slot(i));
-  for (size_t i = 0; i < 3; i++) rk.call_args.push_back(CallArg::i32(p[i]));
-  rk.call_args.push_back(CallArg::f32(static_cast<float>(from_bits(p[3]))));
+  rk.kind = "embedding_grad";
+  // Chunks of 32 sorted tokens, shorter while they are too few to fill the chip
+  // (up to 2048 of them: the joining launch has a workgroup for each), longer
+  // where one id could be in more than 256 for each group of lanes that joins
+  // them. Sums and joins: 1000 tokens of 4 columns 9 + 4 us in chunks of 32, 4 + 4
+  // in 8; 65536 of 4 columns 5 + 17 in 8, 11 + 7 in 32, 17 + 5 in 64; 65536 of 2048
+  // columns 174 + 18 in 32, 174 + 12 in 64.
+  int64_t chunk = 32;
+  while (chunk > 8 && tokens / chunk < 1024 && tokens / chunk * split.slices * split.lanes < 2048 * 64) chunk /= 2;
+  while (tokens / chunk > 256 * (256 / split.lanes)) chunk *= 2;
+  const int64_t chunks = (tokens + chunk - 1) / chunk;
+  const uint64_t pairs = static_cast<uint64_t>(tokens + tokens % 2) * 8;
+  const bool rank = tokens <= kRankTokens;
+  int64_t key_bits = 1;
+  while (vocab >> key_bits) key_bits++;
+  const int64_t passes = rank ? 0 : (key_bits + kSortDigitBits - 1) / kSortDigitBits;
+  const int64_t bits = rank ? 0 : (key_bits + passes - 1) / passes;
+  const int64_t sort = rank ? (tokens + 63) / 64 : (tokens + kSortTile - 1) / kSortTile;
+  const uint64_t table = rank ? 0 : static_cast<uint64_t>(sort << bits) * 4;
+  const uint64_t table_at = pairs + (rank ? 0 : pairs), parts_at = table_at + (table + 15) / 16 * 16;
+  rk.workspace_bytes = parts_at + (chunks > 1 ? static_cast<uint64_t>(chunks * 2 * dim) * 4 : 0);
+  // Workgroups that fill, four vectors a thread or more.
+  const int64_t fill = std::clamp<int64_t>(vocab * dim / 16384 / std::max<int64_t>(1, 2 * passes), 1, 512);
+  const uint64_t both = static_cast<uint64_t>(sort + fill);
+  if (rank) rk.launches.push_back(launch("fg_embedding_grad_rank", both, 1024, "embedding"));
+  for (int64_t i = 0; i < passes; i++)
+    for (const char* step : {"count", "place"})
+      rk.launches.push_back(launch(std::string("fg_embedding_grad_") + step + "_" + std::to_string(i) + "_" + std::to_string(passes), both, 1024, "embedding"));
+  rk.launches.push_back(launch("fg_embedding_grad_sum" + split.suffix() + (4 * tokens * dim >= static_cast<int64_t>(kStreamBytes) ? "_stream" : ""),
+                               (static_cast<uint64_t>(chunks * split.slices * split.lanes) + 255) / 256, 256, "embedding"));
+  if (chunks > 1)
+    rk.launches.push_back(launch("fg_embedding_grad_join" + split.suffix(), static_cast<uint64_t>((chunks - 1) * split.slices), 256, "embedding"));
+  for (uint64_t at : {uint64_t(0), pairs, table_at, parts_at}) rk.call_args.push_back(CallArg::workspace(at));
+  for (int64_t x : {tokens, vocab, dim, split.slices, chunk, chunks, sort, bits}) rk.call_args.push_back(CallArg::i32(x));
+  rk.call_args.push_back(CallArg::f32(scale));
   return rk;
 }
 

@@ -185,6 +185,7 @@ def embedding64(w, ids, g, scale):
 EMBEDDINGS = [  # tokens, vocab, dim
     (1, 1, 1), (1, 7, 5), (2, 3, 4), (63, 100, 3), (64, 2, 64), (65, 1000, 130), (257, 31, 77), (1000, 5000, 36),
     (4097, 300, 20), (5000, 70000, 12), (2049, 2048, 257), (300, 4, 1028), (9000, 3, 8),
+    (16384, 900, 4), (16385, 1000, 5), (20000, 700, 6), (40000, 1500000, 3), (66000, 40, 4), (17000, 1023, 9), (17000, 1024, 8),
 ]
 
 
