@@ -476,26 +476,51 @@ RenderedKernel render_embedding(const UOp& call, bool grad) {
 // params: rows, dim, whether there is a bias, bits of eps. Sources: x, weight,
 // [bias]; of the gradient x, weight, g, dweight's and [dbias's] storage.
 
+// A row on `lanes` lanes, up to `vectors` vectors of four each
+// (kernels/layer_norm.hip).
+struct LayerNormSplit {
+  int64_t lanes, vectors;
+};
+constexpr LayerNormSplit kLayerNormSplits[] = {{8, 1},  {16, 1},  {32, 1},  {64, 1},  {64, 2},
+                                               {64, 4}, {256, 2}, {256, 4}, {512, 4}, {1024, 4}};
+
 RenderedKernel render_layer_norm(const UOp& call, bool grad) {
   const std::vector<int64_t> p = params_of(call);
   const int64_t rows = p[0], dim = p[1];
   const bool bias = p[2] != 0;
   RenderedKernel rk;
   set_image(rk, fg_image_layer_norm, fg_image_layer_norm_end);
-  const uint64_t blocks = static_cast<uint64_t>(std::min<int64_t>(rows, 65536));
+  const LayerNormSplit* split = nullptr;
+  for (const LayerNormSplit& s : kLayerNormSplits)
+    if (!split && 4 * s.lanes * s.vectors >= dim) split = &s;
+  const std::string name = !split ? "_long" : "_" + std::to_string(split->lanes) + "_" + std::to_string(split->vectors) +
+                                                  (dim % 4 ? "_odd" : "") +
+                                                  (4 * rows * dim >= static_cast<int64_t>(kStreamBytes) ? "_stream" : "");
+  const int64_t threads = !split ? 1024 : std::max<int64_t>(256, split->lanes), groups = split ? threads / split->lanes : 1;
+  const int64_t turns = (rows + groups - 1) / groups;  // workgroups, if each had its rows at once
   for (int i = 0; i < 3; i++) rk.call_args.push_back(CallArg::slot(i));
   if (!grad) {
     rk.kind = "layer_norm";
-    rk.launches = {launch("fg_layer_norm", blocks, 256, "layer_norm")};
+    rk.launches = {launch("fg_layer_norm" + name, static_cast<uint64_t>(std::min<int64_t>(turns, 8 * kUnits * 256 / threads)),
+                          static_cast<unsigned>(threads), "layer_norm")};
     rk.call_args.push_back(bias ? CallArg::slot(3) : CallArg::null());
   } else {
     rk.kind = "layer_norm_grad";
-    rk.launches = {launch("fg_layer_norm_grad", blocks, 256, "layer_norm"),
-                   launch("fg_layer_norm_weight", static_cast<uint64_t>((dim + 255) / 256), 256, "layer_norm")};
-    rk.workspace_bytes = static_cast<size_t>(rows) * 8;
+    // Workgroups that fit the chip together, so that each adds up what it can
+    // before its sums go to memory.
+    int64_t blocks = std::min<int64_t>(turns, 4 * kUnits * 256 / threads);
+    rk.launches = {launch("fg_layer_norm_grad" + name, static_cast<uint64_t>(blocks), static_cast<unsigned>(threads), "layer_norm")};
+    if (!split) {
+      blocks = std::min<int64_t>(rows, 32);
+      rk.launches.push_back(launch("fg_layer_norm_grad_long_sums", static_cast<uint64_t>((dim + 255) / 256 * blocks), 256, "layer_norm"));
+    }
+    rk.launches.push_back(launch("fg_layer_norm_weight", static_cast<uint64_t>((2 * dim + 31) / 32), 1024, "layer_norm"));
+    const uint64_t stats_at = static_cast<uint64_t>(blocks * 2 * dim) * 4;
+    rk.workspace_bytes = stats_at + (split ? 0 : static_cast<uint64_t>(rows) * 8);
     rk.side_outputs = {4};
     if (bias) rk.side_outputs.push_back(5);
-    for (CallArg a : {CallArg::slot(3), CallArg::slot(4), bias ? CallArg::slot(5) : CallArg::null(), CallArg::workspace()})
+    for (CallArg a : {CallArg::slot(3), CallArg::slot(4), bias ? CallArg::slot(5) : CallArg::null(), CallArg::workspace(),
+                      CallArg::workspace(stats_at), CallArg::i32(blocks)})
       rk.call_args.push_back(a);
   }
   rk.call_args.push_back(CallArg::i32(rows));
