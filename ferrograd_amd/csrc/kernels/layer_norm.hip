@@ -12,7 +12,15 @@
 // second read. L is a part of a wave for short rows, a workgroup for long ones.
 // dw and db are summed in registers over all rows that a lane sees, then over the
 // workgroup, then over the workgroups by a second launch: a fixed order, no
-// atomics. Rows of more than 16384 columns are read again for each sum.
+// atomics. Registers do not hold these sums of more than 16384 columns: x and g
+// are then read again for them. Rows of more than 32768 columns are read again for
+// each of their sums.
+//
+// 16384 rows of 4096: forward 98 us (5.4 TB/s), backward 126 (6.4); of 4095, whose
+// vectors are unaligned, 101 and 150 (184 where registers left room for three
+// waves a SIMD, not four). 65536 of 1024: 92 and 120 (5.8 and 6.7). 3000 of 20000:
+// 138 (199 with weight and bias read for each row), and backward 133 + 90, where reading each row for each sum took 186, and 392
+// + 98.
 #include <hip/hip_runtime.h>
 
 #include "vectors.hpp"
@@ -79,8 +87,11 @@ struct Columns {
 };
 
 // The row less its mean (0 past its end), and the inverse of its deviation.
+struct Moments {
+  float mean, inv;
+};
 template <int L, int K, bool Whole>
-__device__ inline float centre(Vec<4> (&x)[K], const Columns<L, K, Whole>& cols, float eps) {
+__device__ inline Moments centre(Vec<4> (&x)[K], const Columns<L, K, Whole>& cols, float eps) {
   float s[1] = {};
 #pragma unroll
   for (int k = 0; k < K; k++)
@@ -97,7 +108,7 @@ __device__ inline float centre(Vec<4> (&x)[K], const Columns<L, K, Whole>& cols,
       s[0] += x[k].v[e] * x[k].v[e];
     }
   row_sums<L>(s);
-  return 1.f / sqrtf(s[0] / cols.dim + eps);
+  return {mean, 1.f / sqrtf(s[0] / cols.dim + eps)};
 }
 
 constexpr int threads_of(int L) { return L > 256 ? L : 256; }
@@ -114,7 +125,7 @@ __device__ inline void forward(float* __restrict__ out, const float* __restrict_
     const int r = r0 + static_cast<int>(threadIdx.x) / L;
     Vec<4> v[K];
     cols.template read<false>(v, x + static_cast<size_t>(min(r, rows - 1)) * dim);
-    const float inv = centre<L, K, Whole>(v, cols, eps);
+    const float inv = centre<L, K, Whole>(v, cols, eps).inv;
     if (r >= rows) continue;
 #pragma unroll
     for (int k = 0; k < K; k++) {
@@ -127,10 +138,13 @@ __device__ inline void forward(float* __restrict__ out, const float* __restrict_
 
 // A workgroup's sums for dw and db go to partial[workgroup][2][dim]. Rows of more
 // than one workgroup's 256 lanes keep the weight in LDS: in registers as well it
-// would leave room for half the waves.
+// would leave room for half the waves. Where K is 8 there is room for no sums: the
+// rows' means and deviations go to `stats` for a launch that makes them.
 template <int L, int K, bool Whole, bool Stream>
 __device__ inline void backward(float* __restrict__ dx, const float* __restrict__ x, const float* __restrict__ w,
-                                const float* __restrict__ g, float* __restrict__ partial, int rows, int dim, float eps) {
+                                const float* __restrict__ g, float* __restrict__ partial, float* __restrict__ stats, int rows,
+                                int dim, float eps) {
+  constexpr bool kSums = K < 8;
   constexpr int kGroups = threads_of(L) / L;
   constexpr bool kHeld = L <= 256;
   __shared__ Vec<4> weights[kHeld ? 1 : K * L];
@@ -146,7 +160,12 @@ __device__ inline void backward(float* __restrict__ dx, const float* __restrict_
     Vec<4> h[K], u[K];
     cols.template read<Stream>(h, x + at);
     cols.template read<Stream>(u, g + at);
-    const float inv = centre<L, K, Whole>(h, cols, eps);
+    const Moments m = centre<L, K, Whole>(h, cols, eps);
+    const float inv = m.inv;
+    if (!kSums && threadIdx.x == 0) {
+      stats[2 * static_cast<size_t>(r)] = m.mean;
+      stats[2 * static_cast<size_t>(r) + 1] = m.inv;
+    }
     float s[2] = {};
 #pragma unroll
     for (int k = 0; k < K; k++) {
@@ -156,8 +175,8 @@ __device__ inline void backward(float* __restrict__ dx, const float* __restrict_
         // A group past the last row has that row again, and adds none of it.
         const float own = kGroups == 1 || r < rows ? u[k].v[e] : 0.f;
         h[k].v[e] *= inv;
-        dw[k].v[e] += own * h[k].v[e];
-        db[k].v[e] += own;
+        if (kSums) dw[k].v[e] += own * h[k].v[e];
+        if (kSums) db[k].v[e] += own;
         u[k].v[e] *= wk.v[e];
         s[0] += u[k].v[e];
         s[1] += u[k].v[e] * h[k].v[e];
@@ -174,6 +193,7 @@ __device__ inline void backward(float* __restrict__ dx, const float* __restrict_
       cols.template write<Stream>(dx + at, k, d);
     }
   }
+  if (!kSums) return;
   float* to = partial + static_cast<size_t>(blockIdx.x) * 2 * dim;
   if constexpr (kGroups == 1) {
 #pragma unroll
@@ -205,10 +225,6 @@ __device__ inline void backward(float* __restrict__ dx, const float* __restrict_
 
 constexpr int kLong = 1024;  // threads
 
-struct Moments {
-  float mean, inv;
-};
-
 __device__ inline Moments moments(const float* x, int dim, float eps) {
   float s[1] = {};
   for (int c = threadIdx.x; c < dim; c += kLong) s[0] += x[c];
@@ -232,8 +248,9 @@ __device__ inline Moments moments(const float* x, int dim, float eps) {
   extern "C" __global__ void __launch_bounds__(threads_of(L)) fg_layer_norm_##NAME(FG_FORWARD_ARGS) {                 \
     forward<L, K, WHOLE, STREAM>(out, x, w, b, rows, dim, eps);                                                       \
   }                                                                                                                   \
-  extern "C" __global__ void __launch_bounds__(threads_of(L)) fg_layer_norm_grad_##NAME(FG_BACKWARD_ARGS) {           \
-    backward<L, K, WHOLE, STREAM>(dx, x, w, g, partial, rows, dim, eps);                                              \
+  extern "C" __global__ void __launch_bounds__(threads_of(L)) __attribute__((amdgpu_waves_per_eu(4)))                 \
+      fg_layer_norm_grad_##NAME(FG_BACKWARD_ARGS) {                                                                   \
+    backward<L, K, WHOLE, STREAM>(dx, x, w, g, partial, stats, rows, dim, eps);                                              \
   }
 #define FG_LAYER_NORM(L, K)                                  \
   FG_LAYER_NORM_AS(L, K, L##_##K, true, false)               \
@@ -251,6 +268,7 @@ FG_LAYER_NORM(256, 2)
 FG_LAYER_NORM(256, 4)
 FG_LAYER_NORM(512, 4)
 FG_LAYER_NORM(1024, 4)
+FG_LAYER_NORM(1024, 8)
 
 extern "C" __global__ void __launch_bounds__(kLong) fg_layer_norm_long(FG_FORWARD_ARGS) {
   for (int r = blockIdx.x; r < rows; r += gridDim.x) {

@@ -482,7 +482,7 @@ struct LayerNormSplit {
   int64_t lanes, vectors;
 };
 constexpr LayerNormSplit kLayerNormSplits[] = {{8, 1},  {16, 1},  {32, 1},  {64, 1},  {64, 2},
-                                               {64, 4}, {256, 2}, {256, 4}, {512, 4}, {1024, 4}};
+                                               {64, 4}, {256, 2}, {256, 4}, {512, 4}, {1024, 4}, {1024, 8}};
 
 RenderedKernel render_layer_norm(const UOp& call, bool grad) {
   const std::vector<int64_t> p = params_of(call);
@@ -510,13 +510,14 @@ RenderedKernel render_layer_norm(const UOp& call, bool grad) {
     // before its sums go to memory.
     int64_t blocks = std::min<int64_t>(turns, 4 * kUnits * 256 / threads);
     rk.launches = {launch("fg_layer_norm_grad" + name, static_cast<uint64_t>(blocks), static_cast<unsigned>(threads), "layer_norm")};
-    if (!split) {
+    const bool sums = split && split->vectors < 8;
+    if (!sums) {
       blocks = std::min<int64_t>(rows, 32);
       rk.launches.push_back(launch("fg_layer_norm_grad_long_sums", static_cast<uint64_t>((dim + 255) / 256 * blocks), 256, "layer_norm"));
     }
     rk.launches.push_back(launch("fg_layer_norm_weight", static_cast<uint64_t>((2 * dim + 31) / 32), 1024, "layer_norm"));
     const uint64_t stats_at = static_cast<uint64_t>(blocks * 2 * dim) * 4;
-    rk.workspace_bytes = stats_at + (split ? 0 : static_cast<uint64_t>(rows) * 8);
+    rk.workspace_bytes = stats_at + (sums ? 0 : static_cast<uint64_t>(rows) * 8);
     rk.side_outputs = {4};
     if (bias) rk.side_outputs.push_back(5);
     for (CallArg a : {CallArg::slot(3), CallArg::slot(4), bias ? CallArg::slot(5) : CallArg::null(), CallArg::workspace(),
