@@ -23,68 +23,9 @@
 // + 98.
 #include <hip/hip_runtime.h>
 
-#include "vectors.hpp"
+#include "rows.hpp"
 
 namespace {
-
-// Sums over a row's L lanes, in each of them, N at a time.
-
-template <int L, int N>
-__device__ inline void row_sums(float (&s)[N]) {
-#pragma unroll
-  for (int d = (L < 64 ? L : 64) / 2; d > 0; d /= 2)
-#pragma unroll
-    for (int n = 0; n < N; n++) s[n] += __shfl_xor(s[n], d);
-  if constexpr (L > 64) {
-    constexpr int kWaves = L / 64;
-    __shared__ float part[kWaves][N];
-    __syncthreads();  // the last sums are read
-    if (threadIdx.x % 64 == 0)
-#pragma unroll
-      for (int n = 0; n < N; n++) part[threadIdx.x / 64][n] = s[n];
-    __syncthreads();
-#pragma unroll
-    for (int n = 0; n < N; n++) {
-      s[n] = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWaves; w++) s[n] += part[w][n];
-    }
-  }
-}
-
-// A row's columns on a lane: vector k is of the columns from at(k) on. With
-// `Whole` rows are of whole vectors, else the last one may end within.
-template <int L, int K, bool Whole>
-struct Columns {
-  int lane, dim;
-  __device__ explicit Columns(int d) : lane(static_cast<int>(threadIdx.x) % L), dim(d) {}
-  __device__ int at(int k) const { return (k * L + lane) * 4; }
-  __device__ bool has(int k, int e) const { return at(k) + (Whole ? 0 : e) < dim; }
-  template <bool Stream>
-  __device__ void read(Vec<4> (&v)[K], const float* row) const {
-#pragma unroll
-    for (int k = 0; k < K; k++) {
-      v[k] = Vec<4>{};
-      if (Whole ? at(k) < dim : at(k) + 4 <= dim) {
-        v[k] = load<4, Stream>(row + at(k));
-      } else if (!Whole) {
-#pragma unroll
-        for (int e = 0; e < 3; e++)
-          if (at(k) + e < dim) v[k].v[e] = row[at(k) + e];
-      }
-    }
-  }
-  template <bool Stream>
-  __device__ void write(float* row, int k, const Vec<4>& v) const {
-    if (Whole ? at(k) < dim : at(k) + 4 <= dim) {
-      store<4, Stream>(row + at(k), v);
-    } else if (!Whole) {
-#pragma unroll
-      for (int e = 0; e < 3; e++)
-        if (at(k) + e < dim) row[at(k) + e] = v.v[e];
-    }
-  }
-};
 
 // The row less its mean (0 past its end), and the inverse of its deviation.
 struct Moments {
@@ -110,8 +51,6 @@ __device__ inline Moments centre(Vec<4> (&x)[K], const Columns<L, K, Whole>& col
   row_sums<L>(s);
   return {mean, 1.f / sqrtf(s[0] / cols.dim + eps)};
 }
-
-constexpr int threads_of(int L) { return L > 256 ? L : 256; }
 
 template <int L, int K, bool Whole, bool Stream>
 __device__ inline void forward(float* __restrict__ out, const float* __restrict__ x, const float* __restrict__ w,

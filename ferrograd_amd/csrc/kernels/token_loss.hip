@@ -4,90 +4,258 @@
 // others are ignored):
 //   loss = 1/N sum over the N rows of logsumexp(x) - x[label]   (0 if N is 0)
 //   dx = g/N (softmax(x) - onehot(label)), 0 in ignored rows.
+//
+// Bound by memory: the loss reads a row once, the gradient reads and writes it
+// once. So a row of up to 65536 logits lives in the registers of L lanes, K
+// vectors of four each, from its maximum to its gradient; a longer one is read
+// once with a running maximum and sum, and again for its gradient, out of the
+// Infinity Cache. A gradient whose g is 1 makes the loss as well: a training step
+// reads its logits once. Ignored rows are not read.
 #include <hip/hip_runtime.h>
+
+#include "rows.hpp"
 
 namespace {
 
-constexpr int kThreads = 256;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 
-template <class T, class F>
-__device__ inline T block_all(T x, F join) {
-  __shared__ T part[kThreads / 64];
+// Sum of whole numbers or of doubles over a workgroup, in every thread.
+template <int THREADS, class T>
+__device__ inline T block_sum(T x) {
+  __shared__ T part[THREADS / 64];
 #pragma unroll
-  for (int d = 32; d > 0; d /= 2) x = join(x, __shfl_xor(x, d));
+  for (int d = 32; d > 0; d /= 2) x += __shfl_xor(x, d);
   __syncthreads();
   if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = x;
   __syncthreads();
   x = part[0];
 #pragma unroll
-  for (int i = 1; i < kThreads / 64; i++) x = join(x, part[i]);
+  for (int i = 1; i < THREADS / 64; i++) x += part[i];
   return x;
 }
 
-template <class T>
-__device__ inline T block_sum(T x) {
-  return block_all(x, [](T a, T b) { return a + b; });
-}
+__device__ inline bool is_class(int label, int classes) { return label >= 0 && label < classes; }
 
-struct Row {
-  float top, sum;  // the largest logit, and the sum of exp(x - top)
-};
-
-__device__ inline Row row_sum(const float* x, int classes) {
-  // NaN is kept: fmaxf would drop it, but the sum below has it.
-  float top = -INFINITY;
-  for (int c = threadIdx.x; c < classes; c += kThreads) top = fmaxf(top, x[c]);
-  top = block_all(top, [](float a, float b) { return fmaxf(a, b); });
-  float s = 0.f;
-  for (int c = threadIdx.x; c < classes; c += kThreads) s += exp2f((x[c] - top) * kLog2e);
-  return {top, block_sum(s)};
-}
-
-__device__ inline int count_valid(const int* labels, int rows, int classes) {
+template <int THREADS>
+__device__ inline int count_valid(const int* __restrict__ labels, int rows, int classes) {
   int n = 0;
-  for (int r = threadIdx.x; r < rows; r += kThreads) n += labels[r] >= 0 && labels[r] < classes;
-  return block_sum(n);
+#pragma unroll 8
+  for (int r = threadIdx.x; r < rows; r += THREADS) n += is_class(labels[r], classes);
+  return block_sum<THREADS>(n);
+}
+
+// The mean of the rows' losses, by one workgroup.
+template <int THREADS>
+__device__ inline void mean_loss(float* loss, const float* each, const int* labels, int rows, int classes) {
+  int n = 0;
+  double s = 0.0;
+#pragma unroll 8
+  for (int r = threadIdx.x; r < rows; r += THREADS) {
+    n += is_class(labels[r], classes);
+    s += each[r];
+  }
+  n = block_sum<THREADS>(n);
+  s = block_sum<THREADS>(s);
+  if (threadIdx.x == 0) *loss = static_cast<float>(s / max(n, 1));
+}
+
+// A row's loss: its label's logit, its largest one, and the sum of exp(x - top).
+__device__ inline float row_loss(float picked, float top, float sum) { return (top - picked) + log2f(sum) * kLn2; }
+
+// Rows on L lanes each. `each` (or null) takes the rows' losses; with `Grad` dx
+// their gradients, g (or null: 1) over the number of valid labels times what it
+// says above. One workgroup alone also makes the mean.
+template <int L, int K, bool Whole, bool Grad, bool Stream>
+__device__ inline void rows_of(float* __restrict__ dx, const float* __restrict__ x, const int* __restrict__ labels,
+                               const float* __restrict__ g, const int* __restrict__ count, float* __restrict__ each,
+                               float* __restrict__ loss, int rows, int classes) {
+  constexpr int kThreads = threads_of(L), kGroups = kThreads / L;
+  const Columns<L, K, Whole> cols(classes);
+  float scale = 0.f;
+  if (Grad) scale = (g ? *g : 1.f) / max(count ? *count : count_valid<kThreads>(labels, rows, classes), 1);
+  for (int r0 = blockIdx.x * kGroups; r0 < rows; r0 += gridDim.x * kGroups) {
+    const int r = r0 + static_cast<int>(threadIdx.x) / L, label = labels[min(r, rows - 1)];
+    const bool valid = is_class(label, classes);
+    const size_t at = static_cast<size_t>(min(r, rows - 1)) * classes;
+    Vec<4> v[K];
+    if (L > 64 && !valid) {  // the same in all of the workgroup
+      if (each && threadIdx.x == 0) each[r] = 0.f;
+      if (Grad)
+#pragma unroll
+        for (int k = 0; k < K; k++) cols.template write<Stream>(dx + at, k, Vec<4>{});
+      continue;
+    }
+    const float picked = x[at + (valid ? label : 0)];
+    cols.template read<Stream>(v, x + at, -INFINITY);
+    float top[1] = {-INFINITY}, sum[1] = {};
+#pragma unroll
+    for (int k = 0; k < K; k++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) top[0] = fmaxf(top[0], v[k].v[e]);
+    join_row<L>(top, Largest());
+#pragma unroll
+    for (int k = 0; k < K; k++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        v[k].v[e] = exp2f((v[k].v[e] - top[0]) * kLog2e);
+        sum[0] += v[k].v[e];
+      }
+    row_sums<L>(sum);
+    if (r >= rows) continue;
+    if (each && cols.lane == 0) each[r] = valid ? row_loss(picked, top[0], sum[0]) : 0.f;
+    if (!Grad) continue;
+    const float inv = 1.f / sum[0];
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const float p = v[k].v[e] * inv - (cols.at(k) + e == label ? 1.f : 0.f);
+        v[k].v[e] = valid ? p * scale : 0.f;
+      }
+      cols.template write<Stream>(dx + at, k, v[k]);
+    }
+  }
+  if (!each || gridDim.x != 1) return;
+  __syncthreads();
+  mean_loss<kThreads>(loss, each, labels, rows, classes);
+}
+
+// ── rows of more than registers hold ────────────────────────────────────────
+
+constexpr int kLong = 1024;  // threads
+constexpr int kBatch = 8;    // vectors of a thread on their way at a time
+
+// f(first column, up to four logits) over the row, a thread's vectors in batches.
+template <bool Stream, class F>
+__device__ inline void over_row(const float* __restrict__ row, int classes, F f) {
+  for (int c0 = 0; c0 < classes; c0 += kBatch * kLong * 4) {
+    Vec<4> v[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; k++) {
+      const int c = c0 + (k * kLong + static_cast<int>(threadIdx.x)) * 4;
+      if (c + 4 <= classes) {
+        v[k] = load<4, Stream>(row + c);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[k].v[e] = c + e < classes ? row[c + e] : -INFINITY;
+      }
+    }
+    f(c0, v);
+  }
+}
+
+template <bool Grad>
+__device__ inline void long_rows(float* __restrict__ dx, const float* __restrict__ x, const int* __restrict__ labels,
+                                 const float* __restrict__ g, const int* __restrict__ count, float* __restrict__ each,
+                                 float* __restrict__ loss, int rows, int classes) {
+  float scale = 0.f;
+  if (Grad) scale = (g ? *g : 1.f) / max(count ? *count : count_valid<kLong>(labels, rows, classes), 1);
+  for (int r = blockIdx.x; r < rows; r += gridDim.x) {
+    const int label = labels[r];
+    const size_t at = static_cast<size_t>(r) * classes;
+    if (!is_class(label, classes)) {
+      if (each && threadIdx.x == 0) each[r] = 0.f;
+      if (Grad)
+        for (int c = threadIdx.x; c < classes; c += kLong) dx[at + c] = 0.f;
+      continue;
+    }
+    const float picked = x[at + label];
+    // A running maximum, and the sum of exp(x - it). While all are -inf the sum
+    // is of exp(x): 0.
+    float top[1] = {-INFINITY}, sum[1] = {};
+    over_row<false>(x + at, classes, [&](int, Vec<4>(&v)[kBatch]) {
+      float now = top[0];
+#pragma unroll
+      for (int k = 0; k < kBatch; k++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) now = fmaxf(now, v[k].v[e]);
+      const float from = now == -INFINITY ? 0.f : now;
+      sum[0] *= exp2f((top[0] - from) * kLog2e);
+      top[0] = now;
+#pragma unroll
+      for (int k = 0; k < kBatch; k++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) sum[0] += exp2f((v[k].v[e] - from) * kLog2e);
+    });
+    const float mine = top[0];
+    join_row<kLong>(top, Largest());
+    sum[0] *= exp2f((mine - (top[0] == -INFINITY ? 0.f : top[0])) * kLog2e);
+    row_sums<kLong>(sum);
+    if (each && threadIdx.x == 0) each[r] = row_loss(picked, top[0], sum[0]);
+    if (!Grad) continue;
+    const float inv = 1.f / sum[0], from = top[0];
+    over_row<false>(x + at, classes, [&](int c0, Vec<4>(&v)[kBatch]) {
+#pragma unroll
+      for (int k = 0; k < kBatch; k++) {
+        const int c = c0 + (k * kLong + static_cast<int>(threadIdx.x)) * 4;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          v[k].v[e] = (exp2f((v[k].v[e] - from) * kLog2e) * inv - (c + e == label ? 1.f : 0.f)) * scale;
+        if (c + 4 <= classes) {
+          store<4, true>(dx + at + c, v[k]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 3; e++)
+            if (c + e < classes) dx[at + c + e] = v[k].v[e];
+        }
+      }
+    });
+  }
+  if (!each || gridDim.x != 1) return;
+  __syncthreads();
+  mean_loss<kLong>(loss, each, labels, rows, classes);
 }
 
 }  // namespace
 
-extern "C" __global__ void __launch_bounds__(kThreads)
-    fg_token_loss(float* out, const float* x, const int* labels, float* each, int rows, int classes) {
-  for (int r = blockIdx.x; r < rows; r += gridDim.x) {
-    const int label = labels[r];
-    float v = 0.f;
-    if (label >= 0 && label < classes) {
-      const float* row = x + static_cast<size_t>(r) * classes;
-      const Row s = row_sum(row, classes);
-      v = (s.top - row[label]) + log2f(s.sum) * kLn2;
-    }
-    if (threadIdx.x == 0) each[r] = v;
+// The first output is the loss of a forward call, dx of a gradient.
+#define FG_LOSS_ARGS float *loss, const float *x, const int *labels, float *each, int rows, int classes
+#define FG_GRAD_ARGS \
+  float *dx, const float *x, const int *labels, const float *g, float *loss, float *each, int *count, int rows, int classes
+
+#define FG_LOSS_AS(L, K, NAME, WHOLE)                                                                                     \
+  extern "C" __global__ void __launch_bounds__(threads_of(L)) fg_token_loss_##NAME(FG_LOSS_ARGS) {                        \
+    rows_of<L, K, WHOLE, false, false>(nullptr, x, labels, nullptr, nullptr, each, loss, rows, classes);                  \
   }
+#define FG_GRAD_AS(L, K, NAME, WHOLE, STREAM)                                                                             \
+  extern "C" __global__ void __launch_bounds__(threads_of(L)) fg_token_loss_grad_##NAME(FG_GRAD_ARGS) {                   \
+    rows_of<L, K, WHOLE, true, STREAM>(dx, x, labels, g, count, each, loss, rows, classes);                               \
+  }
+#define FG_TOKEN_LOSS(L, K)                             \
+  FG_LOSS_AS(L, K, L##_##K, true)                       \
+  FG_LOSS_AS(L, K, L##_##K##_odd, false)                \
+  FG_GRAD_AS(L, K, L##_##K, true, false)                \
+  FG_GRAD_AS(L, K, L##_##K##_stream, true, true)        \
+  FG_GRAD_AS(L, K, L##_##K##_odd, false, false)         \
+  FG_GRAD_AS(L, K, L##_##K##_odd_stream, false, true)
+
+FG_TOKEN_LOSS(8, 1)
+FG_TOKEN_LOSS(16, 1)
+FG_TOKEN_LOSS(32, 1)
+FG_TOKEN_LOSS(64, 1)
+FG_TOKEN_LOSS(64, 2)
+FG_TOKEN_LOSS(64, 4)
+FG_TOKEN_LOSS(256, 2)
+FG_TOKEN_LOSS(256, 4)
+FG_TOKEN_LOSS(256, 8)
+FG_TOKEN_LOSS(512, 8)
+FG_TOKEN_LOSS(1024, 8)
+FG_TOKEN_LOSS(1024, 16)
+
+extern "C" __global__ void __launch_bounds__(kLong) fg_token_loss_long(FG_LOSS_ARGS) {
+  long_rows<false>(nullptr, x, labels, nullptr, nullptr, each, loss, rows, classes);
+}
+extern "C" __global__ void __launch_bounds__(kLong) fg_token_loss_grad_long(FG_GRAD_ARGS) {
+  long_rows<true>(dx, x, labels, g, count, each, loss, rows, classes);
 }
 
-extern "C" __global__ void __launch_bounds__(kThreads)
-    fg_token_loss_mean(float* out, const float* x, const int* labels, float* each, int rows, int classes) {
-  const int n = count_valid(labels, rows, classes);
-  double s = 0.0;
-  for (int r = threadIdx.x; r < rows; r += kThreads) s += each[r];
-  s = block_sum(s);
-  if (threadIdx.x == 0) *out = static_cast<float>(s / max(n, 1));
+extern "C" __global__ void __launch_bounds__(kLong) fg_token_loss_mean(FG_LOSS_ARGS) {
+  mean_loss<kLong>(loss, each, labels, rows, classes);
 }
-
-extern "C" __global__ void __launch_bounds__(kThreads)
-    fg_token_loss_grad(float* dx, const float* x, const int* labels, const float* g, int rows, int classes) {
-  const float scale = *g / max(count_valid(labels, rows, classes), 1);
-  for (int r = blockIdx.x; r < rows; r += gridDim.x) {
-    const int label = labels[r];
-    const size_t at = static_cast<size_t>(r) * classes;
-    if (label >= 0 && label < classes) {
-      const Row s = row_sum(x + at, classes);
-      const float inv = 1.f / s.sum;
-      for (int c = threadIdx.x; c < classes; c += kThreads)
-        dx[at + c] = (exp2f((x[at + c] - s.top) * kLog2e) * inv - (c == label ? 1.f : 0.f)) * scale;
-    } else {
-      for (int c = threadIdx.x; c < classes; c += kThreads) dx[at + c] = 0.f;
-    }
-  }
+extern "C" __global__ void __launch_bounds__(kLong) fg_token_loss_grad_mean(FG_GRAD_ARGS) {
+  mean_loss<kLong>(loss, each, labels, rows, classes);
+}
+extern "C" __global__ void __launch_bounds__(kLong) fg_token_loss_grad_count(FG_GRAD_ARGS) {
+  const int n = count_valid<kLong>(labels, rows, classes);
+  if (threadIdx.x == 0) *count = n;
 }

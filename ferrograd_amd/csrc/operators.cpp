@@ -478,10 +478,10 @@ RenderedKernel render_embedding(const UOp& call, bool grad) {
 
 // A row on `lanes` lanes, up to `vectors` vectors of four each
 // (kernels/layer_norm.hip).
-struct LayerNormSplit {
+struct RegisterSplit {
   int64_t lanes, vectors;
 };
-constexpr LayerNormSplit kLayerNormSplits[] = {{8, 1},  {16, 1},  {32, 1},  {64, 1},  {64, 2},
+constexpr RegisterSplit kLayerNormSplits[] = {{8, 1},  {16, 1},  {32, 1},  {64, 1},  {64, 2},
                                                {64, 4}, {256, 2}, {256, 4}, {512, 4}, {1024, 4}, {1024, 8}};
 
 RenderedKernel render_layer_norm(const UOp& call, bool grad) {
@@ -490,8 +490,8 @@ RenderedKernel render_layer_norm(const UOp& call, bool grad) {
   const bool bias = p[2] != 0;
   RenderedKernel rk;
   set_image(rk, fg_image_layer_norm, fg_image_layer_norm_end);
-  const LayerNormSplit* split = nullptr;
-  for (const LayerNormSplit& s : kLayerNormSplits)
+  const RegisterSplit* split = nullptr;
+  for (const RegisterSplit& s : kLayerNormSplits)
     if (!split && 4 * s.lanes * s.vectors >= dim) split = &s;
   const std::string name = !split ? "_long" : "_" + std::to_string(split->lanes) + "_" + std::to_string(split->vectors) +
                                                   (dim % 4 ? "_odd" : "") +
@@ -531,27 +531,53 @@ RenderedKernel render_layer_norm(const UOp& call, bool grad) {
 }
 
 // ── token_cross_entropy ─────────────────────────────────────────────────────
-// params: rows, classes. Sources: logits, labels; of the gradient also g.
+// params: rows, classes. Sources: logits, labels. Of the gradient also whether it
+// makes the loss; sources: logits, labels, and the loss's storage, or else g.
+
+// A row on `lanes` lanes, up to `vectors` vectors of four each
+// (kernels/token_loss.hip).
+constexpr RegisterSplit kTokenLossSplits[] = {{8, 1},   {16, 1},  {32, 1},  {64, 1},  {64, 2},   {64, 4},
+                                               {256, 2}, {256, 4}, {256, 8}, {512, 8}, {1024, 8}, {1024, 16}};
 
 RenderedKernel render_token_loss(const UOp& call, bool grad) {
   const std::vector<int64_t> p = params_of(call);
-  const uint64_t rows = static_cast<uint64_t>(p[0]);
+  const int64_t rows = p[0], classes = p[1];
+  const bool joint = grad && p[2] != 0;
   RenderedKernel rk;
   set_image(rk, fg_image_token_loss, fg_image_token_loss_end);
+  const RegisterSplit* split = nullptr;
+  for (const RegisterSplit& s : kTokenLossSplits)
+    if (!split && 4 * s.lanes * s.vectors >= classes) split = &s;
+  std::string name = !split ? "_long" : "_" + std::to_string(split->lanes) + "_" + std::to_string(split->vectors) + (classes % 4 ? "_odd" : "");
+  if (split && grad && 4 * rows * classes >= static_cast<int64_t>(kStreamBytes)) name += "_stream";
+  const int64_t threads = !split ? 1024 : std::max<int64_t>(256, split->lanes), groups = split ? threads / split->lanes : 1;
+  // As many workgroups as the chip has room for; one alone for rows that it goes
+  // through in 8 turns, as it then needs no other launch.
+  const int64_t turns = (rows + groups - 1) / groups;
+  const int64_t blocks = groups > 1 && turns <= 8 ? 1 : std::min<int64_t>(turns, 8 * kUnits * 256 / threads);
   for (int i = 0; i < 3; i++) rk.call_args.push_back(CallArg::slot(i));
   if (!grad) {
     rk.kind = "token_loss";
-    rk.launches = {launch("fg_token_loss", std::min<uint64_t>(rows, 65536), 256, "token_cross_entropy"),
-                   launch("fg_token_loss_mean", 1, 256, "token_cross_entropy")};
-    rk.workspace_bytes = rows * 4;
+    rk.launches = {launch("fg_token_loss" + name, static_cast<uint64_t>(blocks), static_cast<unsigned>(threads), "token_cross_entropy")};
+    if (blocks > 1) rk.launches.push_back(launch("fg_token_loss_mean", 1, 1024, "token_cross_entropy"));
+    rk.workspace_bytes = static_cast<uint64_t>(rows) * 4;
     rk.call_args.push_back(CallArg::workspace());
   } else {
     rk.kind = "token_loss_grad";
-    rk.launches = {launch("fg_token_loss_grad", std::min<uint64_t>(rows, 1024), 256, "token_cross_entropy")};
-    rk.call_args.push_back(CallArg::slot(3));
+    // The valid labels are counted by each workgroup, or once where they are many.
+    const bool count = rows > 8192;
+    if (count) rk.launches.push_back(launch("fg_token_loss_grad_count", 1, 1024, "token_cross_entropy"));
+    rk.launches.push_back(launch("fg_token_loss_grad" + name, static_cast<uint64_t>(blocks), static_cast<unsigned>(threads), "token_cross_entropy"));
+    if (joint && blocks > 1) rk.launches.push_back(launch("fg_token_loss_grad_mean", 1, 1024, "token_cross_entropy"));
+    rk.workspace_bytes = 16 + static_cast<uint64_t>(rows) * 4;
+    rk.call_args.push_back(joint ? CallArg::null() : CallArg::slot(3));
+    rk.call_args.push_back(joint ? CallArg::slot(3) : CallArg::null());
+    rk.call_args.push_back(joint ? CallArg::workspace(16) : CallArg::null());
+    rk.call_args.push_back(count ? CallArg::workspace() : CallArg::null());
+    if (joint) rk.side_outputs = {3};
   }
-  rk.call_args.push_back(CallArg::i32(p[0]));
-  rk.call_args.push_back(CallArg::i32(p[1]));
+  rk.call_args.push_back(CallArg::i32(rows));
+  rk.call_args.push_back(CallArg::i32(classes));
   return rk;
 }
 
@@ -876,8 +902,12 @@ std::vector<UOp> kernel_gradient(const UOp& call, const UOp& grad) {
       return grads;
     }
     case KernelId::TokenLoss: {
-      std::vector<UOp> srcs = {call.src(0), call.src(1), gradient_source(grad)};
-      return {make_call(KernelId::TokenLossGrad, call.src(0).shape(), srcs, params_of(call)), UOp()};
+      std::vector<int64_t> params = params_of(call);
+      // Of a gradient of 1, the seed of a backward pass, the call makes the loss too.
+      const bool joint = is_ones(grad);
+      params.push_back(joint);
+      UOp last = joint ? output_storage(KernelId::TokenLossGrad, 1, call.shape(), {call}, params) : gradient_source(grad);
+      return {make_call(KernelId::TokenLossGrad, call.src(0).shape(), {call.src(0), call.src(1), last}, params), UOp()};
     }
     case KernelId::NormRotateGrad:
     case KernelId::AttentionGrad:
@@ -895,6 +925,11 @@ std::vector<UOp> kernel_gradient(const UOp& call, const UOp& grad) {
     }
   }
   fail("gradient not implemented for this kernel");
+}
+
+UOp kernel_also_made(const UOp& call) {
+  if (call.op() != Op::Kernel || static_cast<KernelId>(call.arg().a) != KernelId::TokenLossGrad || !params_of(call)[2]) return UOp();
+  return call.srcs().back().src(0);
 }
 
 RenderedKernel render_hip_call(const UOp& call) {

@@ -26,6 +26,11 @@ enum class KernelId : int64_t {
 // gradient_for_op.
 std::vector<UOp> kernel_gradient(const UOp& call, const UOp& grad);
 
+// The other call whose result `call` makes as well, in the storage that is its
+// last source (of the loss of token labels, its gradient does), or null. That
+// storage has the other call as its source, so a graph that has `call` has both.
+UOp kernel_also_made(const UOp& call);
+
 // The launches of a call on the MI355X (Device::render_call): functions of the
 // library's code object, their geometry and arguments.
 RenderedKernel render_hip_call(const UOp& call);

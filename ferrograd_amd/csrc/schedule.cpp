@@ -4,6 +4,8 @@
 // src/schedule/indexing.rs:22-242.
 #include "schedule.hpp"
 
+#include "operators.hpp"
+
 #include <algorithm>
 #include <unordered_set>
 
@@ -609,26 +611,43 @@ SchedulePlan schedule_many(const std::vector<UOp>& exprs, const ScheduleOptions&
   // applies the same elementwise ops to the same reduced values.
   UOpMap<UOp> deferred;
   const UOpSet kernel_reads = kernel_sources(order);
+  // Calls that another call of the graph makes along with its own result.
+  UOpMap<UOp> made_by;
+  for (auto& node : order)
+    if (UOp made = kernel_also_made(node)) made_by[made] = node;
+  auto run_kernel = [&](const UOp& node) {
+    if (plan.replacements.count(node)) return;  // it ran in another one's place
+    UOp call = substitute_materialized(node, plan.replacements);
+    if (node.op() == Op::KernelOut) {
+      plan.replacements[node] = call.src(0);
+      return;
+    }
+    ScheduleItem item;
+    if (node.op() == Op::KernelBuf) {
+      item.out_shape = node.shape();
+      item.output_buffer = get_device(node.device()).reserve_buffer(node.dtype(), numel(item.out_shape));
+      item.sink = UOp::sink({UOp::param_buffer(0, node.dtype(), static_cast<int64_t>(numel(item.out_shape)), node.device())});
+      item.storage_only = true;
+    } else {
+      item = parameterize_kernel(call);
+    }
+    plan.replacements[node] = buffer_replacement(item);
+    plan.items.push_back(std::move(item));
+  };
   for (auto& node : order) {
     if (is_kernel(node.op())) {
       // Hand-written kernels run in phase 1 even where they are roots, so that
       // every reader of theirs reads a buffer.
-      UOp call = substitute_materialized(node, plan.replacements);
-      if (node.op() == Op::KernelOut) {
-        plan.replacements[node] = call.src(0);
-        continue;
-      }
-      ScheduleItem item;
-      if (node.op() == Op::KernelBuf) {
-        item.out_shape = node.shape();
-        item.output_buffer = get_device(node.device()).reserve_buffer(node.dtype(), numel(item.out_shape));
-        item.sink = UOp::sink({UOp::param_buffer(0, node.dtype(), static_cast<int64_t>(numel(item.out_shape)), node.device())});
-        item.storage_only = true;
+      auto by = made_by.find(node);
+      if (by != made_by.end()) {
+        // Both read the same tensors: the other call can run here already.
+        const UOp storage = by->second.srcs().back();
+        run_kernel(storage);
+        run_kernel(by->second);
+        plan.replacements[node] = plan.replacements.at(storage);
       } else {
-        item = parameterize_kernel(call);
+        run_kernel(node);
       }
-      plan.replacements[node] = buffer_replacement(item);
-      plan.items.push_back(std::move(item));
       continue;
     }
     auto d = deferred.find(node);
