@@ -11,6 +11,13 @@
 // once with a running maximum and sum, and again for its gradient, out of the
 // Infinity Cache. A gradient whose g is 1 makes the loss as well: a training step
 // reads its logits once. Ignored rows are not read.
+//
+// 8192 rows of 32000, a tenth ignored, loss and gradient: 363 us (5.5 TB/s; 396
+// with the library's exp2, 389 with registers for two workgroups a compute unit,
+// 397 with the next row's loads behind this one's stores, which they then wait for).
+// 2047 of 50001, a fifth ignored: 162 (4.6 TB/s: a row fills a compute unit, so
+// its loads, sums and stores take turns; 176 read twice). Read twice, 8192 of 32000
+// take 403.
 #include <hip/hip_runtime.h>
 
 #include "rows.hpp"
@@ -18,6 +25,11 @@
 namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
+
+// 2^x by the hardware's instruction alone: within a step, and 0 below the normal
+// range, where the library's function scales twice. Here 0 stands for what is
+// below 2^-126 of a sum that is 1 or more.
+__device__ inline float power2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Sum of whole numbers or of doubles over a workgroup, in every thread.
 template <int THREADS, class T>
@@ -97,7 +109,7 @@ __device__ inline void rows_of(float* __restrict__ dx, const float* __restrict__
     for (int k = 0; k < K; k++)
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        v[k].v[e] = exp2f((v[k].v[e] - top[0]) * kLog2e);
+        v[k].v[e] = power2((v[k].v[e] - top[0]) * kLog2e);
         sum[0] += v[k].v[e];
       }
     row_sums<L>(sum);
@@ -170,16 +182,16 @@ __device__ inline void long_rows(float* __restrict__ dx, const float* __restrict
 #pragma unroll
         for (int e = 0; e < 4; e++) now = fmaxf(now, v[k].v[e]);
       const float from = now == -INFINITY ? 0.f : now;
-      sum[0] *= exp2f((top[0] - from) * kLog2e);
+      sum[0] *= power2((top[0] - from) * kLog2e);
       top[0] = now;
 #pragma unroll
       for (int k = 0; k < kBatch; k++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) sum[0] += exp2f((v[k].v[e] - from) * kLog2e);
+        for (int e = 0; e < 4; e++) sum[0] += power2((v[k].v[e] - from) * kLog2e);
     });
     const float mine = top[0];
     join_row<kLong>(top, Largest());
-    sum[0] *= exp2f((mine - (top[0] == -INFINITY ? 0.f : top[0])) * kLog2e);
+    sum[0] *= power2((mine - (top[0] == -INFINITY ? 0.f : top[0])) * kLog2e);
     row_sums<kLong>(sum);
     if (each && threadIdx.x == 0) each[r] = row_loss(picked, top[0], sum[0]);
     if (!Grad) continue;
@@ -190,7 +202,7 @@ __device__ inline void long_rows(float* __restrict__ dx, const float* __restrict
         const int c = c0 + (k * kLong + static_cast<int>(threadIdx.x)) * 4;
 #pragma unroll
         for (int e = 0; e < 4; e++)
-          v[k].v[e] = (exp2f((v[k].v[e] - from) * kLog2e) * inv - (c + e == label ? 1.f : 0.f)) * scale;
+          v[k].v[e] = (power2((v[k].v[e] - from) * kLog2e) * inv - (c + e == label ? 1.f : 0.f)) * scale;
         if (c + 4 <= classes) {
           store<4, true>(dx + at + c, v[k]);
         } else {
