@@ -5,6 +5,10 @@
 // rate of a double's multiply-add hides behind the memory's. A norm of NaN
 // makes every y NaN, one of infinity 0 (NaN where x is infinite).
 //
+// 151 million numbers: squares 93 us (6.5 TB/s), products 216 (5.6); 136 and 211
+// where everything goes through the caches in its order. 67 million: 42 + 83 (6.3
+// and 6.5), and 70 + 84.
+//
 // A launch takes up to 64 tensors, one for each lane of a wave: the lanes hold
 // the tensors' addresses and sizes, read out of the launch's arguments, and the
 // running count of their chunks, so that a ballot finds a chunk's tensor. More
@@ -13,30 +17,35 @@
 
 namespace {
 
-constexpr int kThreads = 256, kTensors = 64;
+constexpr int kThreads = 256;
 constexpr int kChunk = 4096;  // elements a workgroup takes at a time
 constexpr int kVectors = kChunk / 4 / kThreads;
+// The second pass goes through the chunks from the last one on: of many, the
+// first pass leaves this many in the Infinity Cache for it, and reads the others
+// past it.
+constexpr int kKept = 8192;
 
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 #define FG_CONSTANT __attribute__((address_space(4)))
 #define FG_GLOBAL __attribute__((address_space(1)))
 
-// A lane's tensor.
+// A lane's tensor, of a launch's TENSORS.
+template <int TENSORS>
 struct Mine {
   unsigned long long in, out;
   int end;   // chunks of the tensors up to this one
   int last;  // elements of its last chunk
 
-  // The launch's arguments begin with 64 addresses and 64 sizes, and, where
-  // there are `outputs`, 64 addresses of theirs.
+  // The launch's arguments begin with their addresses and sizes, and, where there
+  // are `outputs`, those' addresses.
   __device__ Mine(int count, bool outputs) : in(0), out(0) {
     const auto* args = (const FG_CONSTANT unsigned long long*)__builtin_amdgcn_kernarg_segment_ptr();
     const int lane = threadIdx.x % 64;
     unsigned long long n = 0;
     if (lane < count) {
       in = args[lane];
-      n = args[kTensors + lane];
-      if (outputs) out = args[2 * kTensors + lane];
+      n = args[TENSORS + lane];
+      if (outputs) out = args[2 * TENSORS + lane];
     }
     end = static_cast<int>((n + kChunk - 1) / kChunk);
     last = static_cast<int>((n - 1) % kChunk) + 1;
@@ -61,7 +70,8 @@ struct Chunk {
   const FG_GLOBAL float* in;
   FG_GLOBAL float* out;
   int n;
-  __device__ Chunk(const Mine& t, int c) {
+  template <int TENSORS>
+  __device__ Chunk(const Mine<TENSORS>& t, int c) {
     const int i = __popcll(__ballot(t.end <= c));
     const size_t at = static_cast<size_t>(c - (i ? __builtin_amdgcn_readlane(t.end, i - 1) : 0)) * kChunk;
     in = reinterpret_cast<const FG_GLOBAL float*>(of_lane(t.in, i)) + at;
@@ -69,6 +79,14 @@ struct Chunk {
     n = c + 1 == __builtin_amdgcn_readlane(t.end, i) ? __builtin_amdgcn_readlane(t.last, i) : kChunk;
   }
 };
+
+// A whole chunk's vectors of a thread; `Past` the caches.
+template <bool Past>
+__device__ inline void read(floatx4 (&v)[kVectors], const FG_GLOBAL float* in) {
+  const FG_GLOBAL floatx4* from = reinterpret_cast<const FG_GLOBAL floatx4*>(in) + threadIdx.x;
+#pragma unroll
+  for (int i = 0; i < kVectors; i++) v[i] = Past ? __builtin_nontemporal_load(from + i * kThreads) : from[i * kThreads];
+}
 
 // The sum over a workgroup, in every thread, the same in each launch.
 __device__ inline double block_sum(double x) {
@@ -89,23 +107,41 @@ __device__ inline double norm_of(const double* sums, int blocks) {
   return sqrt(block_sum(s));
 }
 
-}  // namespace
-
-#define FG_8(T, p) T p##0, T p##1, T p##2, T p##3, T p##4, T p##5, T p##6, T p##7
-#define FG_64(T, p) FG_8(T, p##0), FG_8(T, p##1), FG_8(T, p##2), FG_8(T, p##3), FG_8(T, p##4), FG_8(T, p##5), FG_8(T, p##6), FG_8(T, p##7)
-
-// A workgroup's sum of squares, and what `before` (if any) has in its place.
-extern "C" __global__ void __launch_bounds__(kThreads)
-    fg_square_sums(FG_64(const float*, in), FG_64(long long, n), double* sums, const double* before, int count) {
-  const Mine t(count, false);
+// `Stream`: outputs past the caches, for those that would not stay there.
+template <int TENSORS, bool Stream>
+__device__ inline void clip(const double* sums, float* total, double max_norm, int blocks, int count) {
+  const Mine<TENSORS> t(count, true);
   const int chunks = t.chunks();
-  double s = 0.0;
+  const double norm = norm_of(sums, blocks);
+  if (total && blockIdx.x == 0 && threadIdx.x == 0) *total = static_cast<float>(norm);
+  // Not fmax, which would take max_norm for a NaN.
+  const float scale = static_cast<float>(max_norm / (norm <= max_norm ? max_norm : norm));
   for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
+    const Chunk k(t, chunks - 1 - c);
+    if (k.n == kChunk) {
+      floatx4 v[kVectors];
+      read<false>(v, k.in);
+      FG_GLOBAL floatx4* to = reinterpret_cast<FG_GLOBAL floatx4*>(k.out) + threadIdx.x;
+#pragma unroll
+      for (int i = 0; i < kVectors; i++) {
+        if (Stream) __builtin_nontemporal_store(v[i] * scale, to + i * kThreads);
+        else to[i * kThreads] = v[i] * scale;
+      }
+    } else {
+      for (int i = threadIdx.x; i < k.n; i += kThreads) k.out[i] = k.in[i] * scale;
+    }
+  }
+}
+
+// A workgroup's squares in its chunks from c on that are below `end`.
+template <bool Past, int TENSORS>
+__device__ inline double squares(const Mine<TENSORS>& t, int& c, int end) {
+  double s = 0.0;
+  for (; c < end; c += gridDim.x) {
     const Chunk k(t, c);
     if (k.n == kChunk) {
       floatx4 v[kVectors];
-#pragma unroll
-      for (int i = 0; i < kVectors; i++) v[i] = reinterpret_cast<const FG_GLOBAL floatx4*>(k.in)[i * kThreads + threadIdx.x];
+      read<Past>(v, k.in);
 #pragma unroll
       for (int i = 0; i < kVectors; i++)
 #pragma unroll
@@ -114,34 +150,46 @@ extern "C" __global__ void __launch_bounds__(kThreads)
       for (int i = threadIdx.x; i < k.n; i += kThreads) s += static_cast<double>(k.in[i]) * k.in[i];
     }
   }
+  return s;
+}
+
+// A workgroup's sum of squares, and what `before` (if any) has in its place.
+template <int TENSORS>
+__device__ inline void square_sums(double* sums, const double* before, int count) {
+  const Mine<TENSORS> t(count, false);
+  const int chunks = t.chunks();
+  int c = blockIdx.x;
+  double s = squares<true>(t, c, chunks - kKept);
+  s += squares<false>(t, c, chunks);
   s = block_sum(s);
   if (threadIdx.x == 0) sums[blockIdx.x] = before ? before[blockIdx.x] + s : s;
 }
 
+}  // namespace
+
+#define FG_8(T, p) T p##0, T p##1, T p##2, T p##3, T p##4, T p##5, T p##6, T p##7
+#define FG_16(T, p) FG_8(T, p##0), FG_8(T, p##1)
+#define FG_64(T, p) FG_16(T, p##0), FG_16(T, p##1), FG_16(T, p##2), FG_16(T, p##3)
+
+// Of up to 16 tensors, with fewer arguments to pass, and of up to 64.
+#define FG_CLIP_AS(N, NAME, STREAM)                                                                               \
+  extern "C" __global__ void __launch_bounds__(kThreads)                                                          \
+      fg_clip_##NAME(FG_##N(const float*, in), FG_##N(long long, n), FG_##N(float*, out), const double* sums,     \
+                     float* total, double max_norm, int blocks, int count) {                                      \
+    clip<N, STREAM>(sums, total, max_norm, blocks, count);                                                        \
+  }
+#define FG_CLIP(N)                                                                                                \
+  extern "C" __global__ void __launch_bounds__(kThreads)                                                          \
+      fg_square_sums_##N(FG_##N(const float*, in), FG_##N(long long, n), double* sums, const double* before, int count) { \
+    square_sums<N>(sums, before, count);                                                                          \
+  }                                                                                                               \
+  FG_CLIP_AS(N, N, false)                                                                                         \
+  FG_CLIP_AS(N, N##_stream, true)
+
+FG_CLIP(16)
+FG_CLIP(64)
+
 extern "C" __global__ void __launch_bounds__(kThreads) fg_norm_of_sums(float* out, const double* sums, int blocks) {
   const double norm = norm_of(sums, blocks);
   if (threadIdx.x == 0) *out = static_cast<float>(norm);
-}
-
-extern "C" __global__ void __launch_bounds__(kThreads)
-    fg_clip(FG_64(const float*, in), FG_64(long long, n), FG_64(float*, out), const double* sums, float* total,
-            double max_norm, int blocks, int count) {
-  const Mine t(count, true);
-  const int chunks = t.chunks();
-  const double norm = norm_of(sums, blocks);
-  if (total && blockIdx.x == 0 && threadIdx.x == 0) *total = static_cast<float>(norm);
-  // Not fmax, which would take max_norm for a NaN.
-  const float scale = static_cast<float>(max_norm / (norm <= max_norm ? max_norm : norm));
-  for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
-    const Chunk k(t, c);
-    if (k.n == kChunk) {
-      floatx4 v[kVectors];
-#pragma unroll
-      for (int i = 0; i < kVectors; i++) v[i] = reinterpret_cast<const FG_GLOBAL floatx4*>(k.in)[i * kThreads + threadIdx.x];
-#pragma unroll
-      for (int i = 0; i < kVectors; i++) reinterpret_cast<FG_GLOBAL floatx4*>(k.out)[i * kThreads + threadIdx.x] = v[i] * scale;
-    } else {
-      for (int i = threadIdx.x; i < k.n; i += kThreads) k.out[i] = k.in[i] * scale;
-    }
-  }
 }

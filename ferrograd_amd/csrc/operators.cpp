@@ -601,12 +601,15 @@ int64_t clip_chunks(const std::vector<int64_t>& p, size_t first) {
   return chunks;
 }
 
-// Addresses and sizes of up to kClipTensors tensors, from slot 1 on.
+// The tensors that a launch has arguments for.
+size_t clip_places(size_t count) { return count <= 16 ? 16 : kClipTensors; }
+
+// Addresses and sizes of the tensors, from slot 1 on.
 std::vector<CallArg> clip_args(const std::vector<int64_t>& p, size_t first) {
-  const size_t count = p.size() - first;
+  const size_t count = p.size() - first, places = clip_places(count);
   std::vector<CallArg> a;
-  for (size_t i = 0; i < kClipTensors; i++) a.push_back(i < count ? CallArg::slot(static_cast<int32_t>(i) + 1) : CallArg::null());
-  for (size_t i = 0; i < kClipTensors; i++) a.push_back(CallArg::bits64(i < count ? p[first + i] : 0));
+  for (size_t i = 0; i < places; i++) a.push_back(i < count ? CallArg::slot(static_cast<int32_t>(i) + 1) : CallArg::null());
+  for (size_t i = 0; i < places; i++) a.push_back(CallArg::bits64(i < count ? p[first + i] : 0));
   return a;
 }
 
@@ -616,7 +619,7 @@ RenderedKernel render_square_sums(const UOp& call) {
   RenderedKernel rk;
   set_image(rk, fg_image_clip, fg_image_clip_end);
   rk.kind = "square_sums";
-  rk.launches = {launch("fg_square_sums", static_cast<uint64_t>(p[0]), 256, "clip_norm")};
+  rk.launches = {launch("fg_square_sums_" + std::to_string(clip_places(p.size() - 2)), static_cast<uint64_t>(p[0]), 256, "clip_norm")};
   rk.call_args = clip_args(p, 2);
   rk.call_args.push_back(CallArg::slot(0));
   rk.call_args.push_back(p[1] ? CallArg::slot(count + 1) : CallArg::null());
@@ -640,10 +643,13 @@ RenderedKernel render_clip(const UOp& call) {
   RenderedKernel rk;
   set_image(rk, fg_image_clip, fg_image_clip_end);
   rk.kind = "clip";
-  rk.launches = {launch("fg_clip", static_cast<uint64_t>(std::min(clip_chunks(p, 3), kClipBlocks)), 256, "clip_norm")};
+  const int64_t chunks = clip_chunks(p, 3);
+  rk.launches = {launch("fg_clip_" + std::to_string(clip_places(p.size() - 3)) +
+                            (4 * kClipChunk * chunks >= static_cast<int64_t>(kStreamBytes) ? "_stream" : ""),
+                        static_cast<uint64_t>(std::min(chunks, kClipBlocks)), 256, "clip_norm")};
   rk.call_args = clip_args(p, 3);
   // Slots: the first output, the tensors, the sums, the further outputs, the norm.
-  for (int32_t i = 0; i < static_cast<int32_t>(kClipTensors); i++)
+  for (int32_t i = 0; i < static_cast<int32_t>(clip_places(p.size() - 3)); i++)
     rk.call_args.push_back(i >= count ? CallArg::null() : CallArg::slot(i ? count + 1 + i : 0));
   for (int32_t i = 1; i < count + norm; i++) rk.side_outputs.push_back(count + 1 + i);
   rk.call_args.push_back(CallArg::slot(count + 1));

@@ -450,7 +450,7 @@ def test_large_logits_and_labels_of_all_rows(fg, hip):
 SHAPES = {
     "one": [(1,)], "classifier": [(128, 784), (128,), (10, 128), (10,)],
     "ragged": [(4095,), (4096,), (4097,), (3, 5, 7), (1, 1), (8192,), (12289,), (2, 2)],
-    "64": [(1 + 37 * i,) for i in range(64)], "65": [(1 + 37 * i,) for i in range(65)],
+    "16": [(1 + 37 * i,) for i in range(16)], "17": [(1 + 37 * i,) for i in range(17)], "64": [(1 + 37 * i,) for i in range(64)], "65": [(1 + 37 * i,) for i in range(65)],
     "200": [(3 + i % 5, 700) for i in range(200)],
 }
 
