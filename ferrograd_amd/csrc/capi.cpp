@@ -234,7 +234,10 @@ namespace {
 std::vector<fg::Tensor> tensors_of(fg_tensor* const* ts, int n, const char* what) {
   FG_CHECK(n >= 0 && (ts || n == 0), std::string(what) + ": no tensors");
   std::vector<fg::Tensor> v;
-  for (int i = 0; i < n; i++) v.push_back(ts[i]->t);
+  for (int i = 0; i < n; i++) {
+    FG_CHECK(ts[i], std::string(what) + ": tensor " + std::to_string(i) + " is null");
+    v.push_back(ts[i]->t);
+  }
   return v;
 }
 }  // namespace

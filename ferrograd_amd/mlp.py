@@ -7,7 +7,7 @@ from typing import Callable, Sequence
 
 import numpy as np
 
-from . import Dropout, FerrogradError, Linear, Sgd, Tensor
+from . import I32, Dropout, FerrogradError, Linear, Sgd, Tensor
 
 
 def one_hot(labels: np.ndarray, num_classes: int) -> np.ndarray:
@@ -56,16 +56,22 @@ class Mlp:
         return [p for layer in self.layers for p in layer.parameters()]
 
 
-def train_step(model: Mlp, opt: Sgd, x: Tensor, targets: Tensor, preactivations: list | None = None) -> Tensor:
+def train_step(model: Mlp, opt: Sgd, x: Tensor, targets: Tensor, preactivations: list | None = None,
+               max_norm: float | None = None) -> Tensor:
     """One step as mnist.rs:90-97: forward, cross-entropy, zero_grad, backward,
     SGD. With a list for `preactivations`, the layers' outputs before ReLU
-    (logits last) are appended to it, realised by the step itself."""
+    (logits last) are appended to it, realised by the step itself. Targets may
+    also be int32 labels [rows], rows of other than a class ignored
+    (Tensor.token_cross_entropy). With `max_norm` the gradients are clipped to it
+    together (Sgd.clip_grad_norm)."""
     zs = model.forward_preactivations(x)
     if preactivations is not None:
         preactivations.extend(zs)
-    loss = zs[-1].cross_entropy(targets)
+    loss = (zs[-1].token_cross_entropy if targets.dtype == I32 else zs[-1].cross_entropy)(targets)
     opt.zero_grad()
     loss.backward()
+    if max_norm is not None:
+        opt.clip_grad_norm(max_norm)
     opt.step()
     return loss
 

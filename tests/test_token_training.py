@@ -353,6 +353,7 @@ def loss64(x, labels, gout=1.0):
 LOSSES = [  # rows, classes
     (1, 1), (1, 2), (3, 2), (256, 10), (5, 31), (64, 64), (7, 65), (33, 257), (130, 1000), (9, 1027), (300, 77), (4, 4096),
     (3, 5001), (2, 16384), (5, 16387), (3, 32768), (2, 32771), (2, 50001), (1, 70000), (2, 128000), (2000, 3),
+    (2100, 9), (2500, 520),
 ]
 
 
@@ -619,6 +620,169 @@ def test_gradients_against_differences(fg, hip):
         terms = [(g * d) for g, d in zip(grads, ds)]
         # The difference is off by step^2 times a third derivative of order 10; the gradients by a few hundred roundings.
         assert abs(sum(t.sum() for t in terms) - slope) <= 1e-8 + 500 * U * sum(np.abs(t).sum() for t in terms)
+
+
+@pytest.mark.gpu
+def test_a_loss_and_what_is_made_of_it_beside_its_gradient(fg, hip):
+    # The gradient's call makes the loss, for its own readers too, whichever is realised first.
+    x, labels = 3 * normal(90, 30, 40), seeded(91).integers(0, 40, 30).astype(np.int32)
+    tx, tl, two = new(fg, x, True), new(fg, labels), new(fg, np.array([2.0], np.float32))
+    (want, bound), (dwant, dbound) = loss64(x, labels)
+    loss = tx.token_cross_entropy(tl)
+    double, dx = loss.mul(two), loss.gradient([tx])[0]
+    got = classes(fg, [double, dx])
+    assert "token_loss" not in got and got.count("token_loss_grad") == 1
+    fg.Tensor.realize_many([double, dx])
+    assert loss.is_realized()
+    check("double", double.numpy(), 2 * want, 2.1 * bound)
+    check("dx", dx.numpy(), dwant, dbound)
+    # Only the gradient: the loss is there as well.
+    loss = tx.token_cross_entropy(tl)
+    dx = loss.gradient([tx])[0].realize()
+    assert loss.is_realized()
+    check("loss", loss.numpy(), want, bound)
+    # The loss first, then its gradient; a gradient through a function of the loss.
+    loss = tx.token_cross_entropy(tl)
+    dx = loss.gradient([tx])[0]
+    check("loss", loss.numpy(), want, bound)
+    check("dx", dx.numpy(), dwant, dbound)
+    loss = tx.token_cross_entropy(tl)
+    square = loss.mul(loss)
+    dsq = square.gradient([tx])[0]
+    fg.Tensor.realize_many([dsq, square, loss])
+    check("square", square.numpy(), want * want, 2.2 * bound * want)
+    check("dsq", dsq.numpy(), 2 * want * dwant, 2.2 * (want * dbound + bound * np.abs(dwant)) + 4 * U * np.abs(2 * want * dwant))
+
+
+@pytest.mark.gpu
+def test_weights_read_twice_and_gradients_that_are_broadcast(fg, hip):
+    w, a, b = normal(92, 9, 6), np.array([1, 2, 2, 8], np.int32), np.array([2, 0, 5, 5], np.int32)
+    tw = new(fg, w, True)
+    y = tw.embedding(new(fg, a)).add(tw.embedding(new(fg, b), 2.0))
+    dw = y.sum([0, 1]).gradient([tw])[0].numpy()
+    want = np.bincount(a, minlength=9) + 2.0 * np.bincount(b, minlength=9)
+    assert np.array_equal(dw, np.repeat(want[:, None], 6, 1))
+    x, n = normal(93, 5, 6), normal(94, 6)
+    tx, tn = new(fg, x, True), new(fg, n, True)
+    y = tx.layer_norm(tn, tn)  # one tensor as weight and bias
+    dx, dn = (t.numpy() for t in y.sum([0, 1]).gradient([tx, tn]))
+    _, (wx, ex), (ww, ew), (wb, eb) = layer_norm64(x, n, n, np.ones((5, 6), np.float32), 1e-5)
+    check("dx", dx, wx, ex)
+    check("dn", dn, ww + wb, ew + eb + U * np.abs(ww + wb))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_norm", [None, 0.05])
+def test_a_train_step_takes_labels_and_clips(fg, hip, max_norm):
+    from ferrograd_amd.mlp import Mlp, synthetic_batch, train_step
+
+    xs, ts = synthetic_batch(64, 20, 7, 1, 2)
+    labels = ts.argmax(1).astype(np.int32)
+    got = []
+    for targets in (ts, labels):
+        fg.reset_init_seed(11)
+        model = Mlp((20, 16, 7), hip)
+        params = model.parameters()
+        before = [p.numpy().astype(np.float64) for p in params]
+        loss = train_step(model, fg.Sgd(params, 0.5), new(fg, xs), new(fg, targets), max_norm=max_norm)
+        got.append([loss.numpy().reshape(-1)] + [(b - p.numpy()) / 0.5 for p, b in zip(params, before)])
+    # The same step, by sums in other orders: a few hundred roundings of terms no larger than their sums' norms.
+    for a, b, p in zip(*got, [np.zeros(1)] + before):
+        assert np.linalg.norm(a - b) <= 500 * U * np.linalg.norm(b) + 4 * U * np.linalg.norm(p) / 0.5
+    norm = np.sqrt(sum((g ** 2).sum() for g in got[1][1:]))
+    assert norm > 0.06 if max_norm is None else abs(norm - max_norm) <= 1e-5
+
+
+def view(t):
+    """A realised tensor's buffer, for torch to look at where it is."""
+    import torch
+
+    class Buffer:
+        __cuda_array_interface__ = {"shape": t.shape, "typestr": "<f4", "data": (t.data_ptr()[0], False), "version": 2}
+
+    return torch.as_tensor(Buffer(), device="cuda")
+
+
+def large(fg, rows, cols):
+    """A tensor of ones that torch may write, larger than generated kernels make."""
+    ones = fg.Tensor.ones([cols], "hip")
+    t = fg.Tensor.zeros([rows, cols], "hip").layer_norm(ones, ones).realize().detach()
+    fg.synchronize("hip")
+    return t
+
+
+@pytest.mark.gpu
+def test_ids_of_four_passes_and_rows_past_32_bits(fg, hip):
+    import torch
+
+    # 2^30 ids, whose keys have 31 bits.
+    tokens = 17000
+    ids = seeded(95).integers(0, 1 << 30, tokens).astype(np.int32)
+    ids[:9] = [0, (1 << 30) - 1, 7, 7, 1 << 30, -1, (1 << 30) - 1, 12345678, 7]
+    g = normal(96, tokens, 1)
+    w = fg.Tensor.zeros([1 << 30, 1], "hip").with_requires_grad(True)
+    dw = w.embedding(new(fg, ids)).mul(new(fg, g)).sum([0, 1]).gradient([w])[0].realize()
+    inside = (ids >= 0) & (ids < 1 << 30)
+    names, at = np.unique(ids[inside], return_inverse=True)
+    want, size = np.zeros(len(names)), np.zeros(len(names))
+    np.add.at(want, at, g[inside, 0].astype(np.float64))
+    np.add.at(size, at, np.abs(g[inside, 0]))
+    fg.synchronize("hip")
+    got = view(dw)[:, 0]
+    check("dw", got[torch.tensor(names.astype(np.int64), device="cuda")].cpu().numpy(), want, 4 * U * size)
+    assert int(torch.count_nonzero(got)) == np.count_nonzero(want)
+    del w, dw, got
+    # A weight of 2^32 elements and more: its last rows are read and written.
+    rows, dim = (1 << 22) + 5, 1028
+    w = large(fg, rows, dim).with_requires_grad(True)
+    view(w)[-1] = torch.arange(dim, device="cuda", dtype=torch.float32)
+    torch.cuda.synchronize()
+    ids = np.array([rows - 1, 3, rows - 2, rows - 1], np.int32)
+    g = normal(97, 4, dim)
+    y = w.embedding(new(fg, ids))
+    dw = y.mul(new(fg, g)).sum([0, 1]).gradient([w])[0]
+    fg.Tensor.realize_many([y, dw])
+    assert np.array_equal(y.numpy(), np.stack([np.arange(dim), np.ones(dim), np.ones(dim), np.arange(dim)]))
+    fg.synchronize("hip")
+    got = view(dw)
+    check("last", got[-1].cpu().numpy(), g[0].astype(np.float64) + g[3], U * np.abs(g[0] + g[3]))
+    assert np.array_equal(got[-2].cpu().numpy(), g[2]) and np.array_equal(got[3].cpu().numpy(), g[1])
+    assert int(torch.count_nonzero(got)) == 3 * dim
+
+
+@pytest.mark.gpu
+def test_rows_of_matrices_past_32_bits(fg, hip):
+    import torch
+
+    rows, cols = (1 << 21) + 3, 2052  # over 2^32 elements
+    x = large(fg, rows, cols).with_requires_grad(True)
+    last = normal(98, 2, cols)
+    view(x)[-2:] = torch.tensor(last, device="cuda")
+    torch.cuda.synchronize()
+    w, b = normal(99, cols), normal(100, cols)
+    y = x.layer_norm(new(fg, w), new(fg, b)).realize()
+    (want, bound), *_ = layer_norm64(last, w, b, np.zeros_like(last), 1e-5)
+    fg.synchronize("hip")
+    check("y", view(y)[-2:].cpu().numpy(), want, bound)
+    assert np.array_equal(view(y)[0].cpu().numpy(), b)
+    del y
+    labels = np.full(rows, -1, np.int32)
+    labels[-2:] = [7, 2051]
+    loss = x.token_cross_entropy(new(fg, labels))
+    dx = loss.gradient([x])[0]
+    fg.Tensor.realize_many([loss, dx])
+    (want, bound), (dwant, dbound) = loss64(last, labels[-2:])
+    check("loss", loss.numpy(), want, bound)
+    fg.synchronize("hip")
+    check("dx", view(dx)[-2:].cpu().numpy(), dwant, dbound)
+    assert not bool(view(dx)[:-2].any())
+    del dx, loss
+    norm, (c,) = fg.clip_norm([x], 1.0)
+    fg.Tensor.realize_many([norm, c])
+    total = np.sqrt((rows - 2) * float(cols) + (last.astype(np.float64) ** 2).sum())
+    check("norm", norm.numpy(), np.array([total]), 1.01 * U * total)
+    fg.synchronize("hip")
+    check("clipped", view(c)[-2:].cpu().numpy(), last / total, 2.01 * U * np.abs(last / total))
 
 
 def model64(torch, ps, ids, labels, pos, heads, batch):
