@@ -78,44 +78,45 @@ __device__ inline void fill(float* __restrict__ dw, int vocab, int dim, int firs
 
 constexpr int kRankThreads = 1024;
 
-// Of up to 16384 tokens: a token's place is the number of tokens before it in
-// the order, all of which are looked at. A workgroup ranks 64 tokens, one a
-// lane, each of its waves against a part of all, which come through the scalar
-// cache: two vector instructions for 64 pairs.
+// Of up to 12288 tokens: a token's place is the number of tokens before it in
+// the order, all of which are looked at. A workgroup ranks 16 tokens against all
+// keys, held in LDS: a lane has one of them and every 64th part of the keys, four
+// at a time, two and a half vector instructions for 64 pairs. 1000 tokens 3.5 us,
+// 5001 7, 16384 would be 31: the four launches below take 25, and more of the host.
+constexpr int kRankTokens = 12288, kRanked = 16, kParts = kRankThreads / kRanked;
 __device__ inline void rank_tokens(int2* __restrict__ sorted, const int* __restrict__ ids, int tokens, int vocab) {
-  __shared__ int places[kRankThreads / 64][64];
-  typedef const __attribute__((address_space(4))) int* Scalars;
-  const Scalars all = (Scalars)ids;
-  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  const int block = blockIdx.x, t = block * 64 + lane;
-  const unsigned mine = t < tokens ? key_of(ids[t], vocab) : 0;
-  const int blocks = (tokens + 63) / 64, per = (blocks + kRankThreads / 64 - 1) / (kRankThreads / 64);
-  int before = 0;
-  for (int b = wave * per; b < min((wave + 1) * per, blocks); b++) {
-    const int u0 = b * 64;
-    if (b == block || u0 + 64 > tokens) {  // one after the other through a vector register
-      const unsigned theirs = key_of(ids[min(u0 + lane, tokens - 1)], vocab);
-      const int n = min(64, tokens - u0), equal = b < block ? 64 : b == block ? lane : 0;
-#pragma unroll 8
-      for (int j = 0; j < n; j++) {
-        const unsigned u = __builtin_amdgcn_readlane(theirs, j);
-        before += u < mine || (u == mine && j < equal);
-      }
-    } else if (b < block) {
-#pragma unroll 32
-      for (int j = 0; j < 64; j++) before += key_of(all[u0 + j], vocab) <= mine;
-    } else {
-#pragma unroll 32
-      for (int j = 0; j < 64; j++) before += key_of(all[u0 + j], vocab) < mine;
-    }
-  }
-  places[wave][lane] = before;
+  __shared__ uint4 keys[kRankTokens / 4];
+  __shared__ int places[kParts][kRanked];
+  const int part = threadIdx.x / kRanked, own = threadIdx.x % kRanked, t0 = blockIdx.x * kRanked, t = t0 + own;
+  unsigned* key = reinterpret_cast<unsigned*>(keys);
+  // Past the last token: behind all others.
+  // An odd number of vectors a part: the parts that a wave reads are in other banks.
+  const int groups = (tokens + 3) / 4, per = (groups + kParts - 1) / kParts | 1;
+  for (int i = threadIdx.x; i < 4 * groups; i += kRankThreads) key[i] = i < tokens ? key_of(ids[i], vocab) : 0xffffffffu;
   __syncthreads();
-  if (wave != 0 || t >= tokens) return;
+  const unsigned mine = key[min(t, tokens - 1)];
+  int before = 0;
+#pragma unroll 4
+  for (int i = part * per; i < min((part + 1) * per, groups); i++) {
+    const uint4 u = keys[i];
+    const unsigned below = mine + (4 * i < t0 ? 1u : 0u);  // of the tokens before these also its own key
+    before += u.x < below;
+    before += u.y < below;
+    before += u.z < below;
+    before += u.w < below;
+  }
+  if (part == 0)
+    for (int j = 0; j < own; j++) before += key[min(t0 + j, tokens - 1)] == mine;
+  places[part][own] = before;
+  __syncthreads();
+  // A wave sums the parts of 16 tokens, four lanes each.
+  if (threadIdx.x >= 64) return;
   before = 0;
 #pragma unroll
-  for (int w = 0; w < kRankThreads / 64; w++) before += places[w][lane];
-  sorted[before] = make_int2(static_cast<int>(mine), t);
+  for (int k = 0; k < kParts / 4; k++) before += places[4 * k + threadIdx.x / kRanked][own];
+  before += __shfl_xor(before, 16);
+  before += __shfl_xor(before, 32);
+  if (threadIdx.x < kRanked && t < tokens) sorted[before] = make_int2(static_cast<int>(mine), t);
 }
 
 // Of more: passes over digits of the key from the lowest on, each keeping the

@@ -415,7 +415,7 @@ ColumnSplit column_split(int64_t dim) {
   return r;
 }
 
-constexpr int64_t kSortTile = 4096, kSortDigitBits = 10, kRankTokens = 16384;  // kernels/embedding.hip
+constexpr int64_t kSortTile = 4096, kSortDigitBits = 10, kRankTokens = 12288;  // kernels/embedding.hip
 
 RenderedKernel render_embedding(const UOp& call, bool grad) {
   const std::vector<int64_t> p = params_of(call);
@@ -451,7 +451,7 @@ RenderedKernel render_embedding(const UOp& call, bool grad) {
   while (vocab >> key_bits) key_bits++;
   const int64_t passes = rank ? 0 : (key_bits + kSortDigitBits - 1) / kSortDigitBits;
   const int64_t bits = rank ? 0 : (key_bits + passes - 1) / passes;
-  const int64_t sort = rank ? (tokens + 63) / 64 : (tokens + kSortTile - 1) / kSortTile;
+  const int64_t sort = rank ? (tokens + 15) / 16 : (tokens + kSortTile - 1) / kSortTile;
   const uint64_t table = rank ? 0 : static_cast<uint64_t>(sort << bits) * 4;
   const uint64_t table_at = pairs + (rank ? 0 : pairs), parts_at = table_at + (table + 15) / 16 * 16;
   rk.workspace_bytes = parts_at + (chunks > 1 ? static_cast<uint64_t>(chunks * 2 * dim) * 4 : 0);
