@@ -46,12 +46,14 @@ __device__ inline void row_sums(float (&s)[N]) {
 }
 
 // A row's columns on a lane: vector k is of the columns from at(k) on. With
-// `Whole` rows are of whole vectors, else the last one may end within.
+// `Whole` rows are of whole vectors, else the last one may end within, and the
+// first one begin before the row: `from` is 0, or less.
 template <int L, int K, bool Whole>
 struct Columns {
-  int lane, dim;
+  int lane, dim, from = 0;
   __device__ explicit Columns(int d) : lane(static_cast<int>(threadIdx.x) % L), dim(d) {}
-  __device__ int at(int k) const { return (k * L + lane) * 4; }
+  __device__ int at(int k) const { return (k * L + lane) * 4 + (Whole ? 0 : from); }
+  __device__ bool whole(int k) const { return Whole ? at(k) < dim : at(k) >= 0 && at(k) + 4 <= dim; }
   __device__ bool has(int k, int e) const { return at(k) + (Whole ? 0 : e) < dim; }
   // The row, and `past` behind its end.
   template <bool Stream>
@@ -60,23 +62,23 @@ struct Columns {
     for (int k = 0; k < K; k++) {
 #pragma unroll
       for (int e = 0; e < 4; e++) v[k].v[e] = past;
-      if (Whole ? at(k) < dim : at(k) + 4 <= dim) {
+      if (whole(k)) {
         v[k] = load<4, Stream>(row + at(k));
       } else if (!Whole) {
 #pragma unroll
-        for (int e = 0; e < 3; e++)
-          if (at(k) + e < dim) v[k].v[e] = row[at(k) + e];
+        for (int e = 0; e < 4; e++)
+          if (at(k) + e >= 0 && at(k) + e < dim) v[k].v[e] = row[at(k) + e];
       }
     }
   }
   template <bool Stream>
   __device__ void write(float* row, int k, const Vec<4>& v) const {
-    if (Whole ? at(k) < dim : at(k) + 4 <= dim) {
+    if (whole(k)) {
       store<4, Stream>(row + at(k), v);
     } else if (!Whole) {
 #pragma unroll
-      for (int e = 0; e < 3; e++)
-        if (at(k) + e < dim) row[at(k) + e] = v.v[e];
+      for (int e = 0; e < 4; e++)
+        if (at(k) + e >= 0 && at(k) + e < dim) row[at(k) + e] = v.v[e];
     }
   }
 };

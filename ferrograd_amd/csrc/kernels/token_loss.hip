@@ -15,7 +15,7 @@
 // 8192 rows of 32000, a tenth ignored, loss and gradient: 363 us (5.5 TB/s; 396
 // with the library's exp2, 389 with registers for two workgroups a compute unit,
 // 397 with the next row's loads behind this one's stores, which they then wait for).
-// 2047 of 50001, a fifth ignored: 162 (4.6 TB/s: a row fills a compute unit, so
+// 2047 of 50001, a fifth ignored: 148 (5.0 TB/s: a row fills a compute unit, so
 // its loads, sums and stores take turns; 176 read twice). Read twice, 8192 of 32000
 // take 403.
 #include <hip/hip_runtime.h>
@@ -71,6 +71,8 @@ __device__ inline void mean_loss(float* loss, const float* each, const int* labe
   if (threadIdx.x == 0) *loss = static_cast<float>(s / max(n, 1));
 }
 
+constexpr int kLine = 32;  // floats
+
 // A row's loss: its label's logit, its largest one, and the sum of exp(x - top).
 __device__ inline float row_loss(float picked, float top, float sum) { return (top - picked) + log2f(sum) * kLn2; }
 
@@ -82,13 +84,16 @@ __device__ inline void rows_of(float* __restrict__ dx, const float* __restrict__
                                const float* __restrict__ g, const int* __restrict__ count, float* __restrict__ each,
                                float* __restrict__ loss, int rows, int classes) {
   constexpr int kThreads = threads_of(L), kGroups = kThreads / L;
-  const Columns<L, K, Whole> cols(classes);
+  Columns<L, K, Whole> cols(classes);
   float scale = 0.f;
   if (Grad) scale = (g ? *g : 1.f) / max(count ? *count : count_valid<kThreads>(labels, rows, classes), 1);
   for (int r0 = blockIdx.x * kGroups; r0 < rows; r0 += gridDim.x * kGroups) {
     const int r = r0 + static_cast<int>(threadIdx.x) / L, label = labels[min(r, rows - 1)];
     const bool valid = is_class(label, classes);
     const size_t at = static_cast<size_t>(min(r, rows - 1)) * classes;
+    // Long rows begin on cache lines, whatever their width: 2047 of 50001 148 us,
+    // not 158; 8192 of 4001 would take 45.4, not 44.5.
+    if (!Whole && L * K >= 2048) cols.from = -static_cast<int>(at % kLine);
     Vec<4> v[K];
     if (L > 64 && !valid) {  // the same in all of the workgroup
       if (each && threadIdx.x == 0) each[r] = 0.f;

@@ -546,8 +546,9 @@ RenderedKernel render_token_loss(const UOp& call, bool grad) {
   RenderedKernel rk;
   set_image(rk, fg_image_token_loss, fg_image_token_loss_end);
   const RegisterSplit* split = nullptr;
+  // Long rows of broken vectors begin on the cache line that their first one is in.
   for (const RegisterSplit& s : kTokenLossSplits)
-    if (!split && 4 * s.lanes * s.vectors >= classes) split = &s;
+    if (!split && 4 * s.lanes * s.vectors - (s.lanes * s.vectors >= 2048 && classes % 4 ? 31 : 0) >= classes) split = &s;
   std::string name = !split ? "_long" : "_" + std::to_string(split->lanes) + "_" + std::to_string(split->vectors) + (classes % 4 ? "_odd" : "");
   if (split && grad && 4 * rows * classes >= static_cast<int64_t>(kStreamBytes)) name += "_stream";
   const int64_t threads = !split ? 1024 : std::max<int64_t>(256, split->lanes), groups = split ? threads / split->lanes : 1;

@@ -354,6 +354,7 @@ LOSSES = [  # rows, classes
     (1, 1), (1, 2), (3, 2), (256, 10), (5, 31), (64, 64), (7, 65), (33, 257), (130, 1000), (9, 1027), (300, 77), (4, 4096),
     (3, 5001), (2, 16384), (5, 16387), (3, 32768), (2, 32771), (2, 50001), (1, 70000), (2, 128000), (2000, 3),
     (2100, 9), (2500, 520),
+    (3, 2017), (3, 2018), (40, 4099), (33, 8161), (3, 8162), (9, 32737), (2, 32738), (2, 65505), (2, 65506),
 ]
 
 
