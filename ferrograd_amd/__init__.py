@@ -179,9 +179,9 @@ def _dtype_code(dtype) -> int:
 class Tensor(_fgc.TensorBase if _fgc is not None else object):
     """A lazily evaluated tensor (tensor.rs:95-97). Handles alias shared state.
 
-    The handle (`_h`, an int) and the graph-building ops (unary, binary,
-    reductions, movement, narrow, log_softmax, realize, assign, alias) come
-    from the extension type; `Tensor(handle)` adopts a handle the C-ABI
+    The handle (`_h`, an int), the shape, data_ptr and the graph-building ops
+    (unary, binary, reductions, movement, narrow, log_softmax, realize,
+    realize_many, gradient, assign, alias) come from the extension type; `Tensor(handle)` adopts a handle the C-ABI
     returned."""
 
     __slots__ = ()
@@ -242,13 +242,6 @@ class Tensor(_fgc.TensorBase if _fgc is not None else object):
         return d.value, dev.value, bool(r.value), bool(g.value)
 
     @property
-    def shape(self) -> tuple:
-        buf = (ctypes.c_int64 * 16)()
-        nd = ctypes.c_int(16)
-        _check(lib().fg_tensor_shape(self._h, buf, ctypes.byref(nd)))
-        return tuple(buf[i] for i in range(nd.value))
-
-    @property
     def dtype(self) -> int:
         return self._info()[0]
 
@@ -272,12 +265,6 @@ class Tensor(_fgc.TensorBase if _fgc is not None else object):
         _check(lib().fg_tensor_set_requires_grad(self._h, int(requires_grad)))
         return self
 
-    def data_ptr(self) -> tuple:
-        """(device pointer, byte size) of a realised tensor's storage."""
-        p, n = ctypes.c_void_p(), ctypes.c_size_t()
-        _check(lib().fg_tensor_data_ptr(self._h, ctypes.byref(p), ctypes.byref(n)))
-        return p.value, n.value
-
     def same(self, other: "Tensor") -> bool:
         s = ctypes.c_int()
         _check(lib().fg_tensor_same(self._h, other._h, ctypes.byref(s)))
@@ -295,11 +282,6 @@ class Tensor(_fgc.TensorBase if _fgc is not None else object):
         return self
 
     # ── realisation (tensor.rs:781-930) ──────────────────────────────────
-    @staticmethod
-    def realize_many(tensors: Sequence["Tensor"]) -> None:
-        arr = (ctypes.c_void_p * max(1, len(tensors)))(*[t._h for t in tensors])
-        _check(lib().fg_tensor_realize_many(arr, len(tensors)))
-
     def numpy(self) -> np.ndarray:
         code = self.dtype
         shape = self.shape
@@ -342,13 +324,6 @@ class Tensor(_fgc.TensorBase if _fgc is not None else object):
 
     def backward(self) -> None:
         _check(lib().fg_tensor_backward(self._h))
-
-    def gradient(self, targets: Sequence["Tensor"]) -> list:
-        n = len(targets)
-        ins = (ctypes.c_void_p * max(1, n))(*[t._h for t in targets])
-        outs = (ctypes.c_void_p * max(1, n))()
-        _check(lib().fg_tensor_gradient(self._h, ins, n, outs))
-        return [_fgc.from_handle(Tensor, outs[i]) for i in range(n)]
 
     def __repr__(self) -> str:
         try:
@@ -446,24 +421,19 @@ class LayerNorm:
         return [self.weight] + ([self.bias] if self.bias is not None else [])
 
 
-def _handles(tensors: Sequence[Tensor]):
-    return (ctypes.c_void_p * max(1, len(tensors)))(*[t._h for t in tensors]), len(tensors)
-
-
 def global_norm(tensors: Sequence[Tensor]) -> Tensor:
     """The root of the sum of the squares of all elements of the tensors (f32, any
     shapes), as a tensor [1], with squares and sums in 64 bits. No gradient flows
     through it."""
-    return Tensor._out(lib().fg_global_norm, *_handles(tensors))
+    lib()
+    return _fgc.global_norm(Tensor, tensors)
 
 
 def clip_norm(tensors: Sequence[Tensor], max_norm: float) -> tuple:
     """global_norm, and the list of the tensors times max_norm / max(norm,
     max_norm), all in a pass over them for the norm and one for the products."""
-    hs, n = _handles(tensors)
-    norm, outs = ctypes.c_void_p(), (ctypes.c_void_p * max(1, n))()
-    _check(lib().fg_clip_norm(hs, n, max_norm, ctypes.byref(norm), outs))
-    return _fgc.from_handle(Tensor, norm.value), [_fgc.from_handle(Tensor, outs[i]) for i in range(n)]
+    lib()
+    return _fgc.clip_norm(Tensor, tensors, max_norm)
 
 
 class Sgd:

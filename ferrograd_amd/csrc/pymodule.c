@@ -8,10 +8,11 @@
  * each op is one C call from the interpreter: the handle lives in the object,
  * results are new objects of the caller's type, and errors raise the
  * package's FerrogradError with fg_last_error()'s message. Everything else
- * (construction from host data, reads, autograd entry points) stays in the
- * Python class, which subclasses this type. */
+ * (construction from host data, reads, backward) stays in the Python class,
+ * which subclasses this type. */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
+#include <limits.h>
 #include <math.h>
 
 #include "ferrograd.h"
@@ -376,6 +377,102 @@ static PyObject* t_assign(TensorObject* self, PyObject* other) {
   return (PyObject*)self;
 }
 
+/* The handles of a sequence of Tensors (and room for as many more behind them),
+ * with the reference that keeps the tensors: free_handles returns both. */
+static fg_tensor** handles_of(PyObject* tensors, PyObject** seq, int* n) {
+  *seq = PySequence_Fast(tensors, "expected a sequence of Tensors");
+  if (!*seq) return NULL;
+  const Py_ssize_t count = PySequence_Fast_GET_SIZE(*seq);
+  fg_tensor** hs = count <= INT_MAX ? PyMem_New(fg_tensor*, 2 * (size_t)count + 1) : NULL;
+  if (!hs) {
+    Py_DECREF(*seq);
+    return (fg_tensor**)PyErr_NoMemory();
+  }
+  for (Py_ssize_t i = 0; i < count; i++) {
+    TensorObject* t;
+    if (check_tensor(PySequence_Fast_GET_ITEM(*seq, i), &t) || !has_handle(t)) {
+      PyMem_Free(hs);
+      Py_DECREF(*seq);
+      return NULL;
+    }
+    hs[i] = t->h;
+  }
+  *n = (int)count;
+  return hs;
+}
+
+static void free_handles(fg_tensor** hs, PyObject* seq) {
+  PyMem_Free(hs);
+  Py_DECREF(seq);
+}
+
+/* A list of objects of `tp` owning the handles; what is not wrapped is freed. */
+static PyObject* wrap_list(PyTypeObject* tp, fg_tensor** hs, int n) {
+  PyObject* list = PyList_New(n);
+  for (int i = 0; i < n; i++) {
+    PyObject* t = list ? wrap(tp, hs[i]) : NULL;
+    if (!list) fg_tensor_free(hs[i]);
+    else if (!t) Py_CLEAR(list); /* wrap freed this one */
+    else PyList_SET_ITEM(list, i, t);
+  }
+  return list;
+}
+
+PyDoc_STRVAR(realize_many_doc, "realize_many(tensors)\n--\n\nTensor::realize_many (tensor.rs:781-830).");
+
+static PyObject* t_realize_many(PyObject* unused, PyObject* tensors) {
+  (void)unused;
+  PyObject* seq;
+  int n;
+  fg_tensor** hs = handles_of(tensors, &seq, &n);
+  if (!hs) return NULL;
+  const int rc = fg_tensor_realize_many(hs, n);
+  free_handles(hs, seq);
+  if (rc) return raise_last();
+  Py_RETURN_NONE;
+}
+
+PyDoc_STRVAR(gradient_doc, "gradient(targets)\n--\n\nTensor::gradient (tensor.rs:938-964): the list of d self / d target.");
+
+static PyObject* t_gradient(TensorObject* self, PyObject* targets) {
+  PyObject* seq;
+  int n;
+  if (!has_handle(self)) return NULL;
+  fg_tensor** hs = handles_of(targets, &seq, &n);
+  if (!hs) return NULL;
+  PyObject* list = NULL;
+  if (fg_tensor_gradient(self->h, hs, n, hs + n)) raise_last();
+  else list = wrap_list(Py_TYPE(self), hs + n, n);
+  free_handles(hs, seq);
+  return list;
+}
+
+PyDoc_STRVAR(data_ptr_doc, "data_ptr()\n--\n\n(device pointer, byte size) of a realised tensor's storage.");
+
+static PyObject* t_data_ptr(TensorObject* self, PyObject* unused) {
+  (void)unused;
+  void* p = NULL;
+  size_t nbytes = 0;
+  if (!has_handle(self)) return NULL;
+  if (fg_tensor_data_ptr(self->h, &p, &nbytes)) return raise_last();
+  return Py_BuildValue("(NN)", p ? PyLong_FromVoidPtr(p) : Py_NewRef(Py_None), PyLong_FromSize_t(nbytes));
+}
+
+static PyObject* t_get_shape(TensorObject* self, void* closure) {
+  (void)closure;
+  int64_t shape[16];
+  int n = 16;
+  if (!has_handle(self)) return NULL;
+  if (fg_tensor_shape(self->h, shape, &n)) return raise_last();
+  PyObject* t = PyTuple_New(n);
+  for (int i = 0; t && i < n; i++) {
+    PyObject* d = PyLong_FromLongLong(shape[i]);
+    if (!d) Py_CLEAR(t);
+    else PyTuple_SET_ITEM(t, i, d);
+  }
+  return t;
+}
+
 static PyMethodDef t_methods[] = {
     {"neg", (PyCFunction)t_neg, METH_NOARGS, NULL},
     {"reciprocal", (PyCFunction)t_reciprocal, METH_NOARGS, NULL},
@@ -411,11 +508,15 @@ static PyMethodDef t_methods[] = {
     {"_b", (PyCFunction)(void (*)(void))t_b, METH_FASTCALL, NULL},
     {"realize", (PyCFunction)t_realize, METH_NOARGS, "Tensor::realize (tensor.rs:781-830)."},
     {"assign", (PyCFunction)t_assign, METH_O, "Tensor::assign (tensor.rs:421-440)."},
+    {"realize_many", (PyCFunction)t_realize_many, METH_O | METH_STATIC, realize_many_doc},
+    {"gradient", (PyCFunction)t_gradient, METH_O, gradient_doc},
+    {"data_ptr", (PyCFunction)t_data_ptr, METH_NOARGS, data_ptr_doc},
     {NULL, NULL, 0, NULL},
 };
 
 static PyGetSetDef t_getset[] = {
     {"_h", (getter)t_get_h, NULL, "the fg_tensor handle, as an int (None when empty)", NULL},
+    {"shape", (getter)t_get_shape, NULL, "the shape, as a tuple", NULL},
     {NULL, NULL, NULL, NULL, NULL},
 };
 
@@ -463,7 +564,49 @@ static PyObject* m_set_error_class(PyObject* mod, PyObject* cls) {
   Py_RETURN_NONE;
 }
 
+/* global_norm(cls, tensors): a `cls`. */
+static PyObject* m_global_norm(PyObject* mod, PyObject* args) {
+  (void)mod;
+  PyTypeObject* cls;
+  PyObject *tensors, *seq;
+  int n;
+  if (!PyArg_ParseTuple(args, "O!O:global_norm", &PyType_Type, &cls, &tensors)) return NULL;
+  fg_tensor** hs = handles_of(tensors, &seq, &n);
+  if (!hs) return NULL;
+  fg_tensor* norm = NULL;
+  const int rc = fg_global_norm(hs, n, &norm);
+  free_handles(hs, seq);
+  return rc ? raise_last() : wrap(cls, norm);
+}
+
+/* clip_norm(cls, tensors, max_norm): (a `cls`, a list of them). */
+static PyObject* m_clip_norm(PyObject* mod, PyObject* args) {
+  (void)mod;
+  PyTypeObject* cls;
+  PyObject *tensors, *seq;
+  double max_norm;
+  int n;
+  if (!PyArg_ParseTuple(args, "O!Od:clip_norm", &PyType_Type, &cls, &tensors, &max_norm)) return NULL;
+  fg_tensor** hs = handles_of(tensors, &seq, &n);
+  if (!hs) return NULL;
+  fg_tensor* norm = NULL;
+  PyObject* out = NULL;
+  if (fg_clip_norm(hs, n, max_norm, &norm, hs + n)) {
+    raise_last();
+  } else {
+    PyObject* list = wrap_list(cls, hs + n, n);
+    PyObject* t = wrap(cls, norm);
+    if (list && t) out = PyTuple_Pack(2, t, list);
+    Py_XDECREF(t);
+    Py_XDECREF(list);
+  }
+  free_handles(hs, seq);
+  return out;
+}
+
 static PyMethodDef m_methods[] = {
+    {"global_norm", m_global_norm, METH_VARARGS, NULL},
+    {"clip_norm", m_clip_norm, METH_VARARGS, NULL},
     {"from_handle", (PyCFunction)(void (*)(void))m_from_handle, METH_FASTCALL, NULL},
     {"set_error_class", (PyCFunction)m_set_error_class, METH_O, NULL},
     {NULL, NULL, 0, NULL},

@@ -122,6 +122,17 @@ def test_norm_and_clip_refusals(fg, cpu):
     for bad in (0.0, -1.0, float("nan"), float("inf")):
         with pytest.raises(fg.FerrogradError, match="max_norm must be finite and positive"):
             fg.clip_norm([a], bad)
+    for bad in (None, 3, [a, 2.0], "ab"):
+        with pytest.raises(TypeError):
+            fg.clip_norm(bad, 1.0)
+        with pytest.raises(TypeError):
+            fg.Tensor.realize_many(bad)
+        with pytest.raises(TypeError):
+            a.gradient(bad)
+    with pytest.raises(fg.FerrogradError, match="no handle"):
+        fg.global_norm([a, fg.Tensor()])
+    with pytest.raises(fg.FerrogradError, match="not realized"):
+        a.add(a).data_ptr()
     p = cpu_tensor(fg, (2, 2)).with_requires_grad(True)
     with pytest.raises(fg.FerrogradError, match="clip_grad_norm requires parameter gradients"):
         fg.Sgd([p], 0.1).clip_grad_norm(1.0)
@@ -486,6 +497,42 @@ def test_clip_norm_of_small_and_large_values(fg, hip, size):
     for x, y in zip(xs, clipped):
         want = 0.5 * x.astype(np.float64)
         check("clipped", y.numpy(), want, 2.01 * U * np.abs(want) + step)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("graphs", [False, True])
+def test_replayed_clips_of_many_tensors(fg, hip, graphs):
+    with graphs_on(fg, 2 if graphs else 0):
+        fg.clear_caches()
+        for turn in range(5):
+            xs = [(turn + 1) * normal(200 + 7 * turn + i, 5 + 61 * i) for i in range(70)]
+            norm = np.sqrt(sum((x.astype(np.float64) ** 2).sum() for x in xs))
+            got, clipped = fg.clip_norm([new(fg, x) for x in xs], 2.0)
+            fg.Tensor.realize_many(clipped + [got])
+            new(fg, normal(60, 1000)).exp().numpy()  # other work in between
+            check("norm", got.numpy(), np.array([norm]), 1.01 * U * norm)
+            for x, y in zip(xs, clipped):
+                check("clipped", y.numpy(), x * (2.0 / norm), 2.01 * U * np.abs(x * (2.0 / norm)))
+
+
+@pytest.mark.gpu
+def test_clipped_gradients_are_clipped_again_and_added_to(fg, hip):
+    p = new(fg, normal(280, 40), True)
+    w = new(fg, normal(281, 40))
+    opt = fg.Sgd([p], 0.5)
+    g = w.numpy().astype(np.float64)
+    size = np.linalg.norm(g)
+    p.mul(w).sum([0]).backward()
+    first = opt.clip_grad_norm(1.0)
+    second = opt.clip_grad_norm(0.5)
+    check("first", first.numpy(), np.array([size]), 2 * U * size)
+    check("second", second.numpy(), np.array([1.0]), np.array([6 * U]))
+    p.mul(w).sum([0]).backward()  # gradients add up
+    want = g * (1 + 0.5 / size)
+    check("sum", p.grad().numpy(), want, 8 * U * np.abs(want))
+    before = p.numpy().astype(np.float64)
+    opt.step()
+    check("step", p.numpy(), before - 0.5 * want, 2 * U * (np.abs(before) + 10 * np.abs(want)))
 
 
 @pytest.mark.gpu
