@@ -423,15 +423,16 @@ class LayerNorm:
 
 def global_norm(tensors: Sequence[Tensor]) -> Tensor:
     """The root of the sum of the squares of all elements of the tensors (f32, any
-    shapes), as a tensor [1], with squares and sums in 64 bits. No gradient flows
-    through it."""
+    shapes), as a tensor [1], with squares and sums in 64 bits. Gradients through
+    it are refused."""
     lib()
     return _fgc.global_norm(Tensor, tensors)
 
 
 def clip_norm(tensors: Sequence[Tensor], max_norm: float) -> tuple:
     """global_norm, and the list of the tensors times max_norm / max(norm,
-    max_norm), all in a pass over them for the norm and one for the products."""
+    max_norm), all in a pass over them for the norm and one for the products.
+    Gradients through either are refused."""
     lib()
     return _fgc.clip_norm(Tensor, tensors, max_norm)
 

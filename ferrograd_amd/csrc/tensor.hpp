@@ -97,7 +97,7 @@ class Tensor {
   // logsumexp(row) - row[label], with *this = logits [rows, classes].
   Tensor token_cross_entropy(const Tensor& labels) const;
   // The root of the sum of all tensors' squares, and the tensors times max_norm
-  // / max(norm, max_norm). No gradients flow through either.
+  // / max(norm, max_norm). Gradients through either are refused.
   static Tensor global_norm(const std::vector<Tensor>& tensors);
   static std::pair<Tensor, std::vector<Tensor>> clip_norm(const std::vector<Tensor>& tensors, double max_norm);
 

@@ -112,8 +112,8 @@ int fg_tensor_token_cross_entropy(fg_tensor* logits, fg_tensor* labels, fg_tenso
 
 /* The root of the sum of the squares of all elements of n tensors (f32, any
  * shapes), as a tensor [1]; squares and sums are f64. The same tensor given twice
- * counts twice. No gradient flows through it. HIP device only. No reference
- * counterpart. */
+ * counts twice. A gradient through it is refused, as through what fg_clip_norm
+ * gives. HIP device only. No reference counterpart. */
 int fg_global_norm(fg_tensor* const* ts, int n, fg_tensor** out);
 /* That norm, and every tensor times max_norm / max(norm, max_norm) (max_norm
  * finite and above 0) into outs[0, n). A norm of NaN makes them NaN, one of
