@@ -22,6 +22,8 @@
 // What is written twice, the rows that have tokens, is 120 MB of 1.2 GB.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "vectors.hpp"
 
 namespace {
@@ -40,23 +42,31 @@ template <int VEC, int G, bool Stream>
 __device__ inline void lookup(float* __restrict__ out, const float* __restrict__ weight, const int* __restrict__ ids,
                               int tokens, int vocab, int dim, int slices, float scale) {
   const unsigned group = (blockIdx.x * 256u + threadIdx.x) / G;
-  const int slice = static_cast<int>(group % slices), first = static_cast<int>(group / slices) * kRows;
-  if (first >= tokens) return;
+  const int slice = static_cast<int>(group % slices);
+  int first = static_cast<int>(group / slices) * kRows;
   const int at = column<VEC, G>(slice, dim);
-  int id[kRows];
+  auto look_up = [&](auto count) {
+    constexpr int N = decltype(count)::value;
+    int id[N];
 #pragma unroll
-  for (int k = 0; k < kRows; k++) id[k] = ids[min(first + k, tokens - 1)];
-  Vec<VEC> v[kRows];
+    for (int k = 0; k < N; k++) id[k] = ids[first + k];
+    Vec<VEC> v[N];
 #pragma unroll
-  for (int k = 0; k < kRows; k++)
-    v[k] = load<VEC>(weight + static_cast<size_t>(static_cast<unsigned>(id[k]) < static_cast<unsigned>(vocab) ? id[k] : 0) * dim + at);
+    for (int k = 0; k < N; k++)
+      v[k] = load<VEC>(weight + static_cast<size_t>(static_cast<unsigned>(id[k]) < static_cast<unsigned>(vocab) ? id[k] : 0) * dim + at);
 #pragma unroll
-  for (int k = 0; k < kRows; k++) {
-    if (first + k >= tokens) return;
-    const bool inside = static_cast<unsigned>(id[k]) < static_cast<unsigned>(vocab);
+    for (int k = 0; k < N; k++) {
+      const bool inside = static_cast<unsigned>(id[k]) < static_cast<unsigned>(vocab);
 #pragma unroll
-    for (int e = 0; e < VEC; e++) v[k].v[e] = inside ? v[k].v[e] * scale : 0.f;
-    store<VEC, Stream>(out + static_cast<size_t>(first + k) * dim + at, v[k]);
+      for (int e = 0; e < VEC; e++) v[k].v[e] = inside ? v[k].v[e] * scale : 0.f;
+      store<VEC, Stream>(out + static_cast<size_t>(first + k) * dim + at, v[k]);
+    }
+  };
+  // Whole groups without a branch between their loads, which would wait for each other.
+  if (first + kRows <= tokens) {
+    look_up(std::integral_constant<int, kRows>());
+  } else {
+    for (; first < tokens; first++) look_up(std::integral_constant<int, 1>());
   }
 }
 
