@@ -15,11 +15,12 @@
 // the workspace, where a last launch joins it with its other parts. So a padding
 // token that is a third of the batch costs no more than any other.
 //
-// 65536 tokens of 2048 columns, 50001 rows, a third of the tokens one: lookup 150
-// us (1.07 GB through the Infinity Cache, 5.9 TB/s of the output and the rows that
-// differ would be 110), sort and zeros 64 (6.4 TB/s of zeros; the sort alone would
-// take 24), sums 130 (5.2 TB/s; 174 with loads that stay in the caches), joins 12.
-// What is written twice, the rows that have tokens, is 120 MB of 1.2 GB.
+// 65536 tokens of 2048 columns, 50001 rows, a third of the tokens one: lookup 138
+// us (5.2 TB/s of the output and the rows that differ; 155 with a branch between a
+// group's loads, which then wait for each other), sort and zeros 64 (6.4 TB/s of
+// zeros; the sort alone would take 24), sums 130 (5.2 TB/s; 174 with loads that
+// stay in the caches), joins 12. What is written twice, the rows that have tokens,
+// is 120 MB of 1.2 GB.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>

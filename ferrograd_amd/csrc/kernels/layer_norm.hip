@@ -17,27 +17,72 @@
 // each of their sums.
 //
 // 16384 rows of 4096: forward 98 us (5.4 TB/s), backward 126 (6.4); of 4095, whose
-// vectors are unaligned, 101 and 150 (184 where registers left room for three
-// waves a SIMD, not four). 65536 of 1024: 92 and 120 (5.8 and 6.7). 3000 of 20000:
-// 138 (199 with weight and bias read for each row), and backward 133 + 90, where reading each row for each sum took 186, and 392
-// + 98.
+// vectors are unaligned, 102 and 136. 65536 of 1024: 92 and 120 (5.8 and 6.7); of
+// 1023, 101 and 132. 3000 of 20000: 138 (199 with weight and bias read for each
+// row), and backward 133 + 90, where reading each row for each sum took 186, and
+// 392 + 98.
 #include <hip/hip_runtime.h>
 
 #include "rows.hpp"
 
 namespace {
 
-// The row less its mean (0 past its end), and the inverse of its deviation.
+// A row's columns on a lane: its vector k is of those from at(k) on. With `Whole`
+// rows are of whole vectors; else the one over the row's end is moved into the
+// row, where it shares columns with the lane's before it: sums leave out what a
+// lane does not own, and what it does not own it writes as the same value again.
+// So each vector is one load and one store (with the last one's elements one by
+// one, for which the wave waits, 16384 rows of 4095 took 150 us backward, not 136,
+// 131072 of 33 18.4, not 16.1, and 4096 of 16383, which lacks the registers for
+// what is moved, 189, not 195). Rows of less than a vector have no other way.
+template <int L, int K, bool Whole>
+struct Moved {
+  int lane, dim;
+  __device__ explicit Moved(int d) : lane(static_cast<int>(threadIdx.x) % L), dim(d) {}
+  __device__ int nominal(int k) const { return (k * L + lane) * 4; }
+  __device__ bool any(int k) const { return nominal(k) < dim; }
+  __device__ int at(int k) const { return Whole ? nominal(k) : max(0, min(nominal(k), dim - 4)); }
+  __device__ bool owns(int k, int e) const { return any(k) && (Whole || (at(k) + e >= nominal(k) && at(k) + e < dim)); }
+  __device__ bool few() const { return !Whole && L == 8 && dim < 4; }
+  // The row's vectors, 0 where there is no column.
+  template <bool Stream>
+  __device__ void read(Vec<4> (&v)[K], const float* row) const {
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+      v[k] = Vec<4>{};
+      if (few()) {
+#pragma unroll
+        for (int e = 0; e < 3; e++)
+          if (owns(k, e)) v[k].v[e] = row[e];
+      } else if (any(k)) {
+        v[k] = load<4, Stream>(row + at(k));
+      }
+    }
+  }
+  template <bool Stream>
+  __device__ void write(float* row, int k, const Vec<4>& v) const {
+    if (few()) {
+#pragma unroll
+      for (int e = 0; e < 3; e++)
+        if (owns(k, e)) row[e] = v.v[e];
+    } else if (any(k)) {
+      store<4, Stream>(row + at(k), v);
+    }
+  }
+};
+
+// The row less its mean, and the inverse of its deviation. What a lane has of no
+// column is 0 where rows are of whole vectors; else sums leave it out.
 struct Moments {
   float mean, inv;
 };
 template <int L, int K, bool Whole>
-__device__ inline Moments centre(Vec<4> (&x)[K], const Columns<L, K, Whole>& cols, float eps) {
+__device__ inline Moments centre(Vec<4> (&x)[K], const Moved<L, K, Whole>& cols, float eps) {
   float s[1] = {};
 #pragma unroll
   for (int k = 0; k < K; k++)
 #pragma unroll
-    for (int e = 0; e < 4; e++) s[0] += x[k].v[e];
+    for (int e = 0; e < 4; e++) s[0] += Whole || cols.owns(k, e) ? x[k].v[e] : 0.f;
   row_sums<L>(s);
   const float mean = s[0] / cols.dim;
   s[0] = 0.f;
@@ -45,8 +90,8 @@ __device__ inline Moments centre(Vec<4> (&x)[K], const Columns<L, K, Whole>& col
   for (int k = 0; k < K; k++)
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      x[k].v[e] = cols.has(k, e) ? x[k].v[e] - mean : 0.f;
-      s[0] += x[k].v[e] * x[k].v[e];
+      x[k].v[e] = !Whole || cols.any(k) ? x[k].v[e] - mean : 0.f;
+      s[0] += Whole || cols.owns(k, e) ? x[k].v[e] * x[k].v[e] : 0.f;
     }
   row_sums<L>(s);
   return {mean, 1.f / sqrtf(s[0] / cols.dim + eps)};
@@ -56,7 +101,7 @@ template <int L, int K, bool Whole, bool Stream>
 __device__ inline void forward(float* __restrict__ out, const float* __restrict__ x, const float* __restrict__ w,
                                const float* __restrict__ b, int rows, int dim, float eps) {
   constexpr int kGroups = threads_of(L) / L;
-  const Columns<L, K, Whole> cols(dim);
+  const Moved<L, K, Whole> cols(dim);
   Vec<4> vw[K], vb[K] = {};
   cols.template read<false>(vw, w);
   if (b) cols.template read<false>(vb, b);
@@ -87,7 +132,7 @@ __device__ inline void backward(float* __restrict__ dx, const float* __restrict_
   constexpr int kGroups = threads_of(L) / L;
   constexpr bool kHeld = L <= 256;
   __shared__ Vec<4> weights[kHeld ? 1 : K * L];
-  const Columns<L, K, Whole> cols(dim);
+  const Moved<L, K, Whole> cols(dim);
   Vec<4> vw[K], dw[K] = {}, db[K] = {};
   cols.template read<false>(vw, w);
   if (!kHeld)  // a lane reads back what it wrote
@@ -117,8 +162,8 @@ __device__ inline void backward(float* __restrict__ dx, const float* __restrict_
         if (kSums) dw[k].v[e] += own * h[k].v[e];
         if (kSums) db[k].v[e] += own;
         u[k].v[e] *= wk.v[e];
-        s[0] += u[k].v[e];
-        s[1] += u[k].v[e] * h[k].v[e];
+        s[0] += Whole || cols.owns(k, e) ? u[k].v[e] : 0.f;
+        s[1] += Whole || cols.owns(k, e) ? u[k].v[e] * h[k].v[e] : 0.f;
       }
     }
     row_sums<L>(s);
@@ -146,10 +191,11 @@ __device__ inline void backward(float* __restrict__ dx, const float* __restrict_
 #pragma unroll
     for (int k = 0; k < K; k++)
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        sums[group][0][cols.at(k) + e] = dw[k].v[e];
-        sums[group][1][cols.at(k) + e] = db[k].v[e];
-      }
+      for (int e = 0; e < 4; e++)
+        if (cols.any(k)) {
+          sums[group][0][cols.at(k) + e] = dw[k].v[e];
+          sums[group][1][cols.at(k) + e] = db[k].v[e];
+        }
     __syncthreads();
     for (int c = threadIdx.x; c < 2 * dim; c += threads_of(L)) {
       float t = 0.f;

@@ -54,10 +54,9 @@ struct Columns {
   __device__ explicit Columns(int d) : lane(static_cast<int>(threadIdx.x) % L), dim(d) {}
   __device__ int at(int k) const { return (k * L + lane) * 4 + (Whole ? 0 : from); }
   __device__ bool whole(int k) const { return Whole ? at(k) < dim : at(k) >= 0 && at(k) + 4 <= dim; }
-  __device__ bool has(int k, int e) const { return at(k) + (Whole ? 0 : e) < dim; }
   // The row, and `past` behind its end.
   template <bool Stream>
-  __device__ void read(Vec<4> (&v)[K], const float* row, float past = 0.f) const {
+  __device__ void read(Vec<4> (&v)[K], const float* row, float past) const {
 #pragma unroll
     for (int k = 0; k < K; k++) {
 #pragma unroll
