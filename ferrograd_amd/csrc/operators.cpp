@@ -415,7 +415,7 @@ ColumnSplit column_split(int64_t dim) {
   return r;
 }
 
-constexpr int64_t kSortTile = 4096, kSortDigitBits = 10, kRankTokens = 12288;  // kernels/embedding.hip
+constexpr int64_t kSortTile = 4096, kSortGroups = 256, kSortDigitBits = 10, kRankTokens = 12288;  // kernels/embedding.hip
 
 RenderedKernel render_embedding(const UOp& call, bool grad) {
   const std::vector<int64_t> p = params_of(call);
@@ -451,7 +451,8 @@ RenderedKernel render_embedding(const UOp& call, bool grad) {
   while (vocab >> key_bits) key_bits++;
   const int64_t passes = rank ? 0 : (key_bits + kSortDigitBits - 1) / kSortDigitBits;
   const int64_t bits = rank ? 0 : (key_bits + passes - 1) / passes;
-  const int64_t sort = rank ? (tokens + 15) / 16 : (tokens + kSortTile - 1) / kSortTile;
+  const int64_t tiles = (tokens + kSortTile - 1) / kSortTile, turns = (tiles + kSortGroups - 1) / kSortGroups;
+  const int64_t sort = rank ? (tokens + 15) / 16 : (tiles + turns - 1) / turns;
   const uint64_t table = rank ? 0 : static_cast<uint64_t>(sort << bits) * 4;
   const uint64_t table_at = pairs + (rank ? 0 : pairs), parts_at = table_at + (table + 15) / 16 * 16;
   rk.workspace_bytes = parts_at + (chunks > 1 ? static_cast<uint64_t>(chunks * 2 * dim) * 4 : 0);
@@ -467,7 +468,7 @@ RenderedKernel render_embedding(const UOp& call, bool grad) {
   if (chunks > 1)
     rk.launches.push_back(launch("fg_embedding_grad_join" + split.suffix(), static_cast<uint64_t>((chunks - 1) * split.slices), 256, "embedding"));
   for (uint64_t at : {uint64_t(0), pairs, table_at, parts_at}) rk.call_args.push_back(CallArg::workspace(at));
-  for (int64_t x : {tokens, vocab, dim, split.slices, chunk, chunks, sort, bits}) rk.call_args.push_back(CallArg::i32(x));
+  for (int64_t x : {tokens, vocab, dim, split.slices, chunk, chunks, sort, turns, bits}) rk.call_args.push_back(CallArg::i32(x));
   rk.call_args.push_back(CallArg::f32(scale));
   return rk;
 }

@@ -216,6 +216,21 @@ def test_embedding_and_its_gradient(fg, hip, shape, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tokens,vocab,dim", [(1048577, 1000, 1), (4300001, 1000, 1), (8400000, 1500, 1), (8400000, 70000, 4)])
+def test_embedding_gradient_of_millions_of_tokens(fg, hip, tokens, vocab, dim):
+    # More than 256 tiles of 4096 tokens: some share a workgroup.
+    ids, g = some_ids("words", tokens, vocab + 50, 5), normal(6, tokens, dim)
+    w = fg.Tensor.zeros([vocab, dim], "hip").with_requires_grad(True)
+    dw = w.embedding(new(fg, ids)).mul(new(fg, g)).sum([0, 1]).gradient([w])[0].numpy()
+    inside = ids < vocab
+    n = np.bincount(ids[inside], minlength=vocab)
+    for c in range(dim):
+        col = g[inside, c].astype(np.float64)
+        want, size = (np.bincount(ids[inside], weights=x, minlength=vocab) for x in (col, np.abs(col)))
+        check("dw", dw[:, c], want, 1.01 * (n + 2) * U * size)
+
+
+@pytest.mark.gpu
 def test_embedding_rows_may_hold_anything(fg, hip):
     # A row that no token reads, and gradients of ids that are no tokens, never matter.
     w, g = normal(4, 9, 6), normal(5, 8, 6)
