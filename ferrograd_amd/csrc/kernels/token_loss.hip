@@ -48,23 +48,46 @@ __device__ inline T block_sum(T x) {
 
 __device__ inline bool is_class(int label, int classes) { return label >= 0 && label < classes; }
 
+// How many of the labels are classes: those of a workgroup's part of the rows, and
+// of all of them: the sum of what a launch of kParts workgroups counted, or, without
+// it, counted by each workgroup for itself.
+constexpr int kParts = 16;
 template <int THREADS>
-__device__ inline int count_valid(const int* __restrict__ labels, int rows, int classes) {
+__device__ inline int count_valid(const int* __restrict__ labels, int rows, int classes, unsigned part, unsigned parts) {
   int n = 0;
 #pragma unroll 8
-  for (int r = threadIdx.x; r < rows; r += THREADS) n += is_class(labels[r], classes);
+  for (int r = part * THREADS + threadIdx.x; r < rows; r += parts * THREADS) n += is_class(labels[r], classes);
   return block_sum<THREADS>(n);
 }
-
-// The mean of the rows' losses, by one workgroup.
 template <int THREADS>
-__device__ inline void mean_loss(float* loss, const float* each, const int* labels, int rows, int classes) {
+__device__ inline int all_valid(const int* __restrict__ counts, const int* __restrict__ labels, int rows, int classes) {
+  if (!counts) return count_valid<THREADS>(labels, rows, classes, 0, 1);
+  int n = 0;
+#pragma unroll
+  for (int i = 0; i < kParts; i++) n += counts[i];
+  return n;
+}
+
+// A part of the loss: the sum of losses of some rows, and how many of them are
+// valid, by one thread. The only one makes the mean; others are left to a launch of
+// one workgroup.
+__device__ inline void give_loss(float* loss, float* sums, int* valid, int at, double s, int n) {
+  if (gridDim.x == 1) {
+    *loss = static_cast<float>(s / max(n, 1));
+  } else {
+    // A rounding of a sum of losses, which are rounded themselves.
+    sums[at] = static_cast<float>(s);
+    valid[at] = n;
+  }
+}
+template <int THREADS>
+__device__ inline void mean_loss(float* loss, const float* __restrict__ sums, const int* __restrict__ valid, int parts) {
   int n = 0;
   double s = 0.0;
 #pragma unroll 8
-  for (int r = threadIdx.x; r < rows; r += THREADS) {
-    n += is_class(labels[r], classes);
-    s += each[r];
+  for (int i = threadIdx.x; i < parts; i += THREADS) {
+    n += valid[i];
+    s += sums[i];
   }
   n = block_sum<THREADS>(n);
   s = block_sum<THREADS>(s);
@@ -76,17 +99,19 @@ constexpr int kLine = 32;  // floats
 // A row's loss: its label's logit, its largest one, and the sum of exp(x - top).
 __device__ inline float row_loss(float picked, float top, float sum) { return (top - picked) + log2f(sum) * kLn2; }
 
-// Rows on L lanes each. `each` (or null) takes the rows' losses; with `Grad` dx
-// their gradients, g (or null: 1) over the number of valid labels times what it
-// says above. One workgroup alone also makes the mean.
+// Rows on L lanes each: the loss where `sums` is not null; with `Grad` dx, their
+// gradients, g (or null: 1) over the number of valid labels times what it says
+// above.
 template <int L, int K, bool Whole, bool Grad, bool Stream>
 __device__ inline void rows_of(float* __restrict__ dx, const float* __restrict__ x, const int* __restrict__ labels,
-                               const float* __restrict__ g, const int* __restrict__ count, float* __restrict__ each,
-                               float* __restrict__ loss, int rows, int classes) {
+                               const float* __restrict__ g, const int* __restrict__ counts, float* __restrict__ loss,
+                               float* __restrict__ sums, int* __restrict__ valids, int rows, int classes) {
   constexpr int kThreads = threads_of(L), kGroups = kThreads / L;
   Columns<L, K, Whole> cols(classes);
   float scale = 0.f;
-  if (Grad) scale = (g ? *g : 1.f) / max(count ? *count : count_valid<kThreads>(labels, rows, classes), 1);
+  if (Grad) scale = (g ? *g : 1.f) / max(all_valid<kThreads>(counts, labels, rows, classes), 1);
+  double total = 0.0;
+  int in = 0;
   for (int r0 = blockIdx.x * kGroups; r0 < rows; r0 += gridDim.x * kGroups) {
     const int r = r0 + static_cast<int>(threadIdx.x) / L, label = labels[min(r, rows - 1)];
     const bool valid = is_class(label, classes);
@@ -96,7 +121,7 @@ __device__ inline void rows_of(float* __restrict__ dx, const float* __restrict__
     if (!Whole && L * K >= 2048) cols.from = -static_cast<int>(at % kLine);
     Vec<4> v[K];
     if (L > 64 && !valid) {  // the same in all of the workgroup
-      if (each && threadIdx.x == 0) each[r] = 0.f;
+      if (sums && threadIdx.x == 0) give_loss(loss, sums, valids, r, 0.0, 0);
       if (Grad)
 #pragma unroll
         for (int k = 0; k < K; k++) cols.template write<Stream>(dx + at, k, Vec<4>{});
@@ -119,7 +144,13 @@ __device__ inline void rows_of(float* __restrict__ dx, const float* __restrict__
       }
     row_sums<L>(sum);
     if (r >= rows) continue;
-    if (each && cols.lane == 0) each[r] = valid ? row_loss(picked, top[0], sum[0]) : 0.f;
+    // Of long rows each is a part, of others those of a workgroup.
+    if (L > 64) {
+      if (sums && threadIdx.x == 0) give_loss(loss, sums, valids, r, row_loss(picked, top[0], sum[0]), 1);
+    } else if (cols.lane == 0 && valid) {
+      total += row_loss(picked, top[0], sum[0]);
+      in++;
+    }
     if (!Grad) continue;
     const float inv = 1.f / sum[0];
 #pragma unroll
@@ -132,9 +163,10 @@ __device__ inline void rows_of(float* __restrict__ dx, const float* __restrict__
       cols.template write<Stream>(dx + at, k, v[k]);
     }
   }
-  if (!each || gridDim.x != 1) return;
-  __syncthreads();
-  mean_loss<kThreads>(loss, each, labels, rows, classes);
+  if (L > 64 || !sums) return;
+  total = block_sum<kThreads>(total);
+  in = block_sum<kThreads>(in);
+  if (threadIdx.x == 0) give_loss(loss, sums, valids, blockIdx.x, total, in);
 }
 
 // ── rows of more than registers hold ────────────────────────────────────────
@@ -163,15 +195,15 @@ __device__ inline void over_row(const float* __restrict__ row, int classes, F f)
 
 template <bool Grad>
 __device__ inline void long_rows(float* __restrict__ dx, const float* __restrict__ x, const int* __restrict__ labels,
-                                 const float* __restrict__ g, const int* __restrict__ count, float* __restrict__ each,
-                                 float* __restrict__ loss, int rows, int classes) {
+                                 const float* __restrict__ g, const int* __restrict__ counts, float* __restrict__ loss,
+                                 float* __restrict__ sums, int* __restrict__ valids, int rows, int classes) {
   float scale = 0.f;
-  if (Grad) scale = (g ? *g : 1.f) / max(count ? *count : count_valid<kLong>(labels, rows, classes), 1);
+  if (Grad) scale = (g ? *g : 1.f) / max(all_valid<kLong>(counts, labels, rows, classes), 1);
   for (int r = blockIdx.x; r < rows; r += gridDim.x) {
     const int label = labels[r];
     const size_t at = static_cast<size_t>(r) * classes;
     if (!is_class(label, classes)) {
-      if (each && threadIdx.x == 0) each[r] = 0.f;
+      if (sums && threadIdx.x == 0) give_loss(loss, sums, valids, r, 0.0, 0);
       if (Grad)
         for (int c = threadIdx.x; c < classes; c += kLong) dx[at + c] = 0.f;
       continue;
@@ -198,7 +230,7 @@ __device__ inline void long_rows(float* __restrict__ dx, const float* __restrict
     join_row<kLong>(top, Largest());
     sum[0] *= power2((mine - (top[0] == -INFINITY ? 0.f : top[0])) * kLog2e);
     row_sums<kLong>(sum);
-    if (each && threadIdx.x == 0) each[r] = row_loss(picked, top[0], sum[0]);
+    if (sums && threadIdx.x == 0) give_loss(loss, sums, valids, r, row_loss(picked, top[0], sum[0]), 1);
     if (!Grad) continue;
     const float inv = 1.f / sum[0], from = top[0];
     over_row<false>(x + at, classes, [&](int c0, Vec<4>(&v)[kBatch]) {
@@ -218,25 +250,24 @@ __device__ inline void long_rows(float* __restrict__ dx, const float* __restrict
       }
     });
   }
-  if (!each || gridDim.x != 1) return;
-  __syncthreads();
-  mean_loss<kLong>(loss, each, labels, rows, classes);
 }
 
 }  // namespace
 
 // The first output is the loss of a forward call, dx of a gradient.
-#define FG_LOSS_ARGS float *loss, const float *x, const int *labels, float *each, int rows, int classes
-#define FG_GRAD_ARGS \
-  float *dx, const float *x, const int *labels, const float *g, float *loss, float *each, int *count, int rows, int classes
+#define FG_LOSS_ARGS \
+  float *loss, const float *x, const int *labels, float *sums, int *valids, int parts, int rows, int classes
+#define FG_GRAD_ARGS                                                                                                    \
+  float *dx, const float *x, const int *labels, const float *g, float *loss, float *sums, int *valids, int parts,       \
+      int *counts, int rows, int classes
 
 #define FG_LOSS_AS(L, K, NAME, WHOLE)                                                                                     \
   extern "C" __global__ void __launch_bounds__(threads_of(L)) fg_token_loss_##NAME(FG_LOSS_ARGS) {                        \
-    rows_of<L, K, WHOLE, false, false>(nullptr, x, labels, nullptr, nullptr, each, loss, rows, classes);                  \
+    rows_of<L, K, WHOLE, false, false>(nullptr, x, labels, nullptr, nullptr, loss, sums, valids, rows, classes);       \
   }
 #define FG_GRAD_AS(L, K, NAME, WHOLE, STREAM)                                                                             \
   extern "C" __global__ void __launch_bounds__(threads_of(L)) fg_token_loss_grad_##NAME(FG_GRAD_ARGS) {                   \
-    rows_of<L, K, WHOLE, true, STREAM>(dx, x, labels, g, count, each, loss, rows, classes);                               \
+    rows_of<L, K, WHOLE, true, STREAM>(dx, x, labels, g, counts, loss, sums, valids, rows, classes);               \
   }
 #define FG_TOKEN_LOSS(L, K)                             \
   FG_LOSS_AS(L, K, L##_##K, true)                       \
@@ -260,19 +291,19 @@ FG_TOKEN_LOSS(1024, 8)
 FG_TOKEN_LOSS(1024, 16)
 
 extern "C" __global__ void __launch_bounds__(kLong) fg_token_loss_long(FG_LOSS_ARGS) {
-  long_rows<false>(nullptr, x, labels, nullptr, nullptr, each, loss, rows, classes);
+  long_rows<false>(nullptr, x, labels, nullptr, nullptr, loss, sums, valids, rows, classes);
 }
 extern "C" __global__ void __launch_bounds__(kLong) fg_token_loss_grad_long(FG_GRAD_ARGS) {
-  long_rows<true>(dx, x, labels, g, count, each, loss, rows, classes);
+  long_rows<true>(dx, x, labels, g, counts, loss, sums, valids, rows, classes);
 }
 
 extern "C" __global__ void __launch_bounds__(kLong) fg_token_loss_mean(FG_LOSS_ARGS) {
-  mean_loss<kLong>(loss, each, labels, rows, classes);
+  mean_loss<kLong>(loss, sums, valids, parts);
 }
 extern "C" __global__ void __launch_bounds__(kLong) fg_token_loss_grad_mean(FG_GRAD_ARGS) {
-  mean_loss<kLong>(loss, each, labels, rows, classes);
+  mean_loss<kLong>(loss, sums, valids, parts);
 }
 extern "C" __global__ void __launch_bounds__(kLong) fg_token_loss_grad_count(FG_GRAD_ARGS) {
-  const int n = count_valid<kLong>(labels, rows, classes);
-  if (threadIdx.x == 0) *count = n;
+  const int n = count_valid<kLong>(labels, rows, classes, blockIdx.x, gridDim.x);
+  if (threadIdx.x == 0) counts[blockIdx.x] = n;
 }

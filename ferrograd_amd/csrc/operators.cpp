@@ -540,6 +540,8 @@ RenderedKernel render_layer_norm(const UOp& call, bool grad) {
 constexpr RegisterSplit kTokenLossSplits[] = {{8, 1},   {16, 1},  {32, 1},  {64, 1},  {64, 2},   {64, 4},
                                                {256, 2}, {256, 4}, {256, 8}, {512, 8}, {1024, 8}, {1024, 16}};
 
+constexpr uint64_t kLossCounts = 16;  // workgroups that count the valid labels
+
 RenderedKernel render_token_loss(const UOp& call, bool grad) {
   const std::vector<int64_t> p = params_of(call);
   const int64_t rows = p[0], classes = p[1];
@@ -560,25 +562,29 @@ RenderedKernel render_token_loss(const UOp& call, bool grad) {
   // launch.
   const int64_t turns = (rows + groups - 1) / groups;
   const int64_t blocks = groups == 1 ? std::min<int64_t>(turns, 1 << 20) : turns <= 8 ? 1 : std::min<int64_t>(turns, 8 * kUnits);
+  const int64_t parts = groups == 1 ? rows : blocks;  // of the loss
   for (int i = 0; i < 3; i++) rk.call_args.push_back(CallArg::slot(i));
   if (!grad) {
     rk.kind = "token_loss";
     rk.launches = {launch("fg_token_loss" + name, static_cast<uint64_t>(blocks), static_cast<unsigned>(threads), "token_cross_entropy")};
     if (blocks > 1) rk.launches.push_back(launch("fg_token_loss_mean", 1, 1024, "token_cross_entropy"));
-    rk.workspace_bytes = static_cast<uint64_t>(rows) * 4;
-    rk.call_args.push_back(CallArg::workspace());
+    rk.workspace_bytes = static_cast<uint64_t>(parts) * 8;
+    for (CallArg a : {CallArg::workspace(), CallArg::workspace(static_cast<uint64_t>(parts) * 4), CallArg::i32(parts)})
+      rk.call_args.push_back(a);
   } else {
     rk.kind = "token_loss_grad";
-    // The valid labels are counted by each workgroup, or once (2 to 5 us) where
-    // they are many.
+    // The valid labels are counted by each workgroup, or once (3 us) where they are
+    // many.
     const bool count = rows > 2048;
-    if (count) rk.launches.push_back(launch("fg_token_loss_grad_count", 1, 1024, "token_cross_entropy"));
+    if (count) rk.launches.push_back(launch("fg_token_loss_grad_count", kLossCounts, 1024, "token_cross_entropy"));
     rk.launches.push_back(launch("fg_token_loss_grad" + name, static_cast<uint64_t>(blocks), static_cast<unsigned>(threads), "token_cross_entropy"));
     if (joint && blocks > 1) rk.launches.push_back(launch("fg_token_loss_grad_mean", 1, 1024, "token_cross_entropy"));
-    rk.workspace_bytes = 16 + static_cast<uint64_t>(rows) * 4;
+    rk.workspace_bytes = 4 * kLossCounts + static_cast<uint64_t>(parts) * 8;
     rk.call_args.push_back(joint ? CallArg::null() : CallArg::slot(3));
     rk.call_args.push_back(joint ? CallArg::slot(3) : CallArg::null());
-    rk.call_args.push_back(joint ? CallArg::workspace(16) : CallArg::null());
+    rk.call_args.push_back(joint ? CallArg::workspace(4 * kLossCounts) : CallArg::null());
+    rk.call_args.push_back(joint ? CallArg::workspace(4 * kLossCounts + static_cast<uint64_t>(parts) * 4) : CallArg::null());
+    rk.call_args.push_back(CallArg::i32(parts));
     rk.call_args.push_back(count ? CallArg::workspace() : CallArg::null());
     if (joint) rk.side_outputs = {3};
   }

@@ -407,6 +407,12 @@ def test_token_cross_entropy_and_its_gradient(fg, hip, shape, ignored):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(131072, 10), (70001, 33), (20001, 270), (17000, 1025)], ids=lambda s: "x".join(map(str, s)))
+def test_token_cross_entropy_of_many_rows(fg, hip, shape):
+    test_token_cross_entropy_and_its_gradient(fg, hip, shape, 0.4)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("classes", [9, 300, 20000, 60000])
 def test_banned_classes_take_no_part(fg, hip, classes):
     # Logits of -inf and of the type's lowest value are classes of probability 0, wherever they are.
