@@ -864,11 +864,15 @@ void replay_plan(Device& backend, const GraphKey& k, const std::shared_ptr<Cache
   uint64_t t2 = now_ns();
   UOpMap<UOp> repl;
   repl.reserve(plan.replacements.size() * 2);
+  // Made once where nodes share a kernel's result: a call's further output and its storage.
+  std::vector<UOp> made(plan.kernels.size());
   for (auto& pr : plan.replacements) {
     const UOp& node = k.order[pr.node];
     if (pr.kernel >= 0) {
       const PlanKernel& pk = plan.kernels[pr.kernel];
-      repl[node] = UOp::reshape(UOp::buffer(outs[pr.kernel], pk.out_dtype, node.device()), pk.out_shape);
+      UOp& u = made[static_cast<size_t>(pr.kernel)];
+      if (!u) u = UOp::reshape(UOp::buffer(outs[pr.kernel], pk.out_dtype, node.device()), pk.out_shape);
+      repl[node] = u;
     } else {
       repl[node] = k.order[pr.value];
     }
