@@ -418,13 +418,27 @@ static PyObject* wrap_list(PyTypeObject* tp, fg_tensor** hs, int n) {
   return list;
 }
 
+/* The one argument of `func`, by position or as `name`. */
+static PyObject* one_argument(const char* func, const char* name, PyObject* const* args, Py_ssize_t n, PyObject* kwnames) {
+  const Py_ssize_t named = kwnames ? PyTuple_GET_SIZE(kwnames) : 0;
+  if (n + named != 1) {
+    PyErr_Format(PyExc_TypeError, "%s() takes exactly one argument (%zd given)", func, n + named);
+  } else if (named && PyUnicode_CompareWithASCIIString(PyTuple_GET_ITEM(kwnames, 0), name) != 0) {
+    PyErr_Format(PyExc_TypeError, "%s() got an unexpected keyword argument '%U'", func, PyTuple_GET_ITEM(kwnames, 0));
+  } else {
+    return args[0];
+  }
+  return NULL;
+}
+
 PyDoc_STRVAR(realize_many_doc, "realize_many(tensors)\n--\n\nTensor::realize_many (tensor.rs:781-830).");
 
-static PyObject* t_realize_many(PyObject* unused, PyObject* tensors) {
+static PyObject* t_realize_many(PyObject* unused, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
   (void)unused;
   PyObject* seq;
   int n;
-  fg_tensor** hs = handles_of(tensors, &seq, &n);
+  PyObject* tensors = one_argument("realize_many", "tensors", args, nargs, kwnames);
+  fg_tensor** hs = tensors ? handles_of(tensors, &seq, &n) : NULL;
   if (!hs) return NULL;
   const int rc = fg_tensor_realize_many(hs, n);
   free_handles(hs, seq);
@@ -432,12 +446,13 @@ static PyObject* t_realize_many(PyObject* unused, PyObject* tensors) {
   Py_RETURN_NONE;
 }
 
-PyDoc_STRVAR(gradient_doc, "gradient(targets)\n--\n\nTensor::gradient (tensor.rs:938-964): the list of d self / d target.");
+PyDoc_STRVAR(gradient_doc, "gradient($self, targets)\n--\n\nTensor::gradient (tensor.rs:938-964): the list of d self / d target.");
 
-static PyObject* t_gradient(TensorObject* self, PyObject* targets) {
+static PyObject* t_gradient(TensorObject* self, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
   PyObject* seq;
   int n;
-  if (!has_handle(self)) return NULL;
+  PyObject* targets = one_argument("gradient", "targets", args, nargs, kwnames);
+  if (!targets || !has_handle(self)) return NULL;
   fg_tensor** hs = handles_of(targets, &seq, &n);
   if (!hs) return NULL;
   PyObject* list = NULL;
@@ -508,8 +523,8 @@ static PyMethodDef t_methods[] = {
     {"_b", (PyCFunction)(void (*)(void))t_b, METH_FASTCALL, NULL},
     {"realize", (PyCFunction)t_realize, METH_NOARGS, "Tensor::realize (tensor.rs:781-830)."},
     {"assign", (PyCFunction)t_assign, METH_O, "Tensor::assign (tensor.rs:421-440)."},
-    {"realize_many", (PyCFunction)t_realize_many, METH_O | METH_STATIC, realize_many_doc},
-    {"gradient", (PyCFunction)t_gradient, METH_O, gradient_doc},
+    {"realize_many", (PyCFunction)(void (*)(void))t_realize_many, METH_FASTCALL | METH_KEYWORDS | METH_STATIC, realize_many_doc},
+    {"gradient", (PyCFunction)(void (*)(void))t_gradient, METH_FASTCALL | METH_KEYWORDS, gradient_doc},
     {"data_ptr", (PyCFunction)t_data_ptr, METH_NOARGS, data_ptr_doc},
     {NULL, NULL, 0, NULL},
 };
