@@ -9,7 +9,11 @@
  * results are new objects of the caller's type, and errors raise the
  * package's FerrogradError with fg_last_error()'s message. Everything else
  * (construction from host data, reads, backward) stays in the Python class,
- * which subclasses this type. */
+ * which subclasses this type.
+ *
+ * realize_many and gradient let other Python threads run meanwhile, as the
+ * calls through ctypes do: they compile kernels, wait for devices and walk
+ * whole graphs. The library itself is used by one thread at a time. */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <limits.h>
@@ -378,11 +382,12 @@ static PyObject* t_assign(TensorObject* self, PyObject* other) {
 }
 
 /* The handles of a sequence of Tensors (and room for as many more behind them),
- * with the reference that keeps the tensors: free_handles returns both. */
+ * with a tuple that keeps the tensors, whatever another thread does to a list of
+ * them: free_handles returns both. */
 static fg_tensor** handles_of(PyObject* tensors, PyObject** seq, int* n) {
-  *seq = PySequence_Fast(tensors, "expected a sequence of Tensors");
+  *seq = PySequence_Tuple(tensors);
   if (!*seq) return NULL;
-  const Py_ssize_t count = PySequence_Fast_GET_SIZE(*seq);
+  const Py_ssize_t count = PyTuple_GET_SIZE(*seq);
   fg_tensor** hs = count <= INT_MAX ? PyMem_New(fg_tensor*, 2 * (size_t)count + 1) : NULL;
   if (!hs) {
     Py_DECREF(*seq);
@@ -390,7 +395,7 @@ static fg_tensor** handles_of(PyObject* tensors, PyObject** seq, int* n) {
   }
   for (Py_ssize_t i = 0; i < count; i++) {
     TensorObject* t;
-    if (check_tensor(PySequence_Fast_GET_ITEM(*seq, i), &t) || !has_handle(t)) {
+    if (check_tensor(PyTuple_GET_ITEM(*seq, i), &t) || !has_handle(t)) {
       PyMem_Free(hs);
       Py_DECREF(*seq);
       return NULL;
@@ -440,7 +445,10 @@ static PyObject* t_realize_many(PyObject* unused, PyObject* const* args, Py_ssiz
   PyObject* tensors = one_argument("realize_many", "tensors", args, nargs, kwnames);
   fg_tensor** hs = tensors ? handles_of(tensors, &seq, &n) : NULL;
   if (!hs) return NULL;
-  const int rc = fg_tensor_realize_many(hs, n);
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = fg_tensor_realize_many(hs, n);
+  Py_END_ALLOW_THREADS
   free_handles(hs, seq);
   if (rc) return raise_last();
   Py_RETURN_NONE;
@@ -456,7 +464,12 @@ static PyObject* t_gradient(TensorObject* self, PyObject* const* args, Py_ssize_
   fg_tensor** hs = handles_of(targets, &seq, &n);
   if (!hs) return NULL;
   PyObject* list = NULL;
-  if (fg_tensor_gradient(self->h, hs, n, hs + n)) raise_last();
+  fg_tensor* const h = self->h;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = fg_tensor_gradient(h, hs, n, hs + n);
+  Py_END_ALLOW_THREADS
+  if (rc) raise_last();
   else list = wrap_list(Py_TYPE(self), hs + n, n);
   free_handles(hs, seq);
   return list;

@@ -1,6 +1,8 @@
 """Embedding, layer norm, the loss of token labels and clipping, further: how
 Python reaches them, and each of their kernels against float64."""
 import inspect
+import threading
+import time
 
 import numpy as np
 import pytest
@@ -24,3 +26,50 @@ def test_tensors_are_given_by_position_or_by_name(fg, cpu):
         for args, kw in (((), {}), (([a], [a]), {}), ((), dict(other=[a])), (([a],), dict(targets=[a])), (([a],), dict(tensors=[a]))):
             with pytest.raises(TypeError):
                 bad(*args, **kw)
+
+
+def while_it_runs(call, meanwhile):
+    """Seconds that call() took, and how often another thread ran meanwhile, once a millisecond."""
+    ticks, go, stop = [], threading.Event(), threading.Event()
+
+    def tick():
+        go.set()
+        while not stop.wait(0.001):
+            meanwhile()
+            ticks.append(time.perf_counter())
+
+    thread = threading.Thread(target=tick)
+    thread.start()
+    go.wait()
+    begin = time.perf_counter()
+    call()
+    end = time.perf_counter()
+    stop.set()
+    thread.join()
+    # Not those next to its ends, where the interpreter itself hands over.
+    inside = [t for t in ticks if begin + 0.1 * (end - begin) < t < end - 0.1 * (end - begin)]
+    return end - begin, len(inside)
+
+
+def long_call(fg, kind, size):
+    """A call of a time that grows with `size`, and a list of tensors that it was given."""
+    a = fg.Tensor.new(np.ones(1 << 12, np.float32), [1 << 12], "cpu").with_requires_grad(True)
+    if kind == "realize_many":
+        ts = [fg.Tensor.new(np.full(1 << size, i + 1.0, np.float32), [1 << size], "cpu").sqrt().exp().log().sum([0]) for i in range(2)]
+        return ts, lambda: fg.Tensor.realize_many(ts)
+    y = a
+    for _ in range(1 << (size - 10)):
+        y = y.mul(a)
+    loss, ts = y.sum([0]), [a]
+    return ts, lambda: loss.gradient(ts)
+
+
+@pytest.mark.parametrize("kind", ["realize_many", "gradient"])
+def test_other_threads_run_while_the_library_works(fg, cpu, kind):
+    for size in range(20, 26):
+        # The other thread empties the list, which alone has the tensors: the call keeps them.
+        ts, call = long_call(fg, kind, size)
+        seconds, ticks = while_it_runs(call, ts.clear)
+        if seconds > 0.08:
+            break
+    assert seconds > 0.08 and ticks >= 3, (seconds, ticks)
