@@ -115,7 +115,15 @@ __device__ inline void clip(const double* sums, float* total, double max_norm, i
   const double norm = norm_of(sums, blocks);
   if (total && blockIdx.x == 0 && threadIdx.x == 0) *total = static_cast<float>(norm);
   // Not fmax, which would take max_norm for a NaN.
-  const float scale = static_cast<float>(max_norm / (norm <= max_norm ? max_norm : norm));
+  double factor = max_norm / (norm <= max_norm ? max_norm : norm);
+  // A factor below float32's normal range would lose its digits, though not all
+  // products with it are that small: it goes in two steps, its digits and its
+  // power of two.
+  int power = 0;
+  if (factor < 0x1p-126) factor = frexp(factor, &power);
+  const float scale = static_cast<float>(factor);
+  power = __builtin_amdgcn_readfirstlane(power);  // the same in all threads
+  auto clipped = [&](float x) { return power ? ldexpf(x * scale, power) : x * scale; };
   for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
     const Chunk k(t, chunks - 1 - c);
     if (k.n == kChunk) {
@@ -124,11 +132,13 @@ __device__ inline void clip(const double* sums, float* total, double max_norm, i
       FG_GLOBAL floatx4* to = reinterpret_cast<FG_GLOBAL floatx4*>(k.out) + threadIdx.x;
 #pragma unroll
       for (int i = 0; i < kVectors; i++) {
-        if (Stream) __builtin_nontemporal_store(v[i] * scale, to + i * kThreads);
-        else to[i * kThreads] = v[i] * scale;
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[i][e] = clipped(v[i][e]);
+        if (Stream) __builtin_nontemporal_store(v[i], to + i * kThreads);
+        else to[i * kThreads] = v[i];
       }
     } else {
-      for (int i = threadIdx.x; i < k.n; i += kThreads) k.out[i] = k.in[i] * scale;
+      for (int i = threadIdx.x; i < k.n; i += kThreads) k.out[i] = clipped(k.in[i]);
     }
   }
 }

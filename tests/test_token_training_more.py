@@ -7,6 +7,8 @@ import time
 import numpy as np
 import pytest
 
+from test_token_training import U, check, new, normal
+
 
 # ── from Python (no GPU) ────────────────────────────────────────────────────
 
@@ -73,3 +75,22 @@ def test_other_threads_run_while_the_library_works(fg, cpu, kind):
         if seconds > 0.08:
             break
     assert seconds > 0.08 and ticks >= 3, (seconds, ticks)
+
+
+# ── clipping (GPU) ──────────────────────────────────────────────────────────
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_norm", [1e-6, 1e-9, 1e-12, 1e-20, 1e-36, 1e-43, 1e-60])
+def test_clip_norm_by_factors_below_the_normal_range(fg, hip, max_norm):
+    # Norms of about 1e33 and more: factors of 1e-39 and less, of products that are numbers of full precision.
+    xs = [(normal(300 + i, n) * 1e31).astype(np.float32) for i, n in enumerate((4096, 5001, 3))]
+    norm = np.sqrt(sum((x.astype(np.float64) ** 2).sum() for x in xs))
+    got, clipped = fg.clip_norm([new(fg, x) for x in xs], max_norm)
+    fg.Tensor.realize_many([got] + clipped)
+    check("norm", got.numpy(), np.array([norm]), 1.01 * U * norm)
+    step = 2.0 ** -149  # of numbers below the normal range
+    for x, y in zip(xs, clipped):
+        want = x.astype(np.float64) * (max_norm / norm)
+        # The factor's digits are rounded once and the product once, and where it is below the normal range once more.
+        assert np.all(np.abs(y.numpy() - want) <= 2.01 * U * np.abs(want) + 0.51 * step), max_norm
