@@ -77,6 +77,24 @@ def test_other_threads_run_while_the_library_works(fg, cpu, kind):
     assert seconds > 0.08 and ticks >= 3, (seconds, ticks)
 
 
+# ── embedding (GPU) ─────────────────────────────────────────────────────────
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,dim", [(600001, 132), (1100001, 68), (4200001, 5)])
+def test_embedding_gradient_of_a_frequent_id_adds_up(fg, hip, tokens, dim):
+    # The rows of one id are alike, so that the roundings of a long sum all go one way. A sum of 64 rows has 63
+    # additions in float32; all else is in 64 bits, but for the rounding of a chunk's part and of the result.
+    row = (1 + np.arange(dim) / dim).astype(np.float32)[None]
+    g = new(fg, row).embedding(new(fg, np.zeros(tokens, np.int32))).realize()
+    r = np.random.default_rng(310)
+    ids = np.where(r.random(tokens) < 0.9, 3, r.integers(0, 7, tokens)).astype(np.int32)
+    w = fg.Tensor.zeros([7, dim], "hip").with_requires_grad(True)
+    dw = w.embedding(new(fg, ids)).mul(g).sum([0, 1]).gradient([w])[0].numpy()
+    want = np.bincount(ids, minlength=7)[:, None] * row.astype(np.float64)
+    check("dw", dw, want, 66 * U * want)
+
+
 # ── clipping (GPU) ──────────────────────────────────────────────────────────
 
 
