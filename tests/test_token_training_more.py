@@ -7,7 +7,8 @@ import time
 import numpy as np
 import pytest
 
-from test_token_training import U, check, new, normal
+from conftest import seeded
+from test_token_training import U, check, layer_norm64, loss64, new, normal, some_ids, weighted
 
 
 # ── from Python (no GPU) ────────────────────────────────────────────────────
@@ -112,3 +113,63 @@ def test_clip_norm_by_factors_below_the_normal_range(fg, hip, max_norm):
         want = x.astype(np.float64) * (max_norm / norm)
         # The factor's digits are rounded once and the product once, and where it is below the normal range once more.
         assert np.all(np.abs(y.numpy() - want) <= 2.01 * U * np.abs(want) + 0.51 * step), max_norm
+
+
+# ── every kernel, over many rows (GPU) ──────────────────────────────────────
+#
+# Rows are of a few different ones, so that float64 has these alone to make, and
+# equal rows have to come out equal in every bit wherever they are (where no note
+# says otherwise). Sums over all
+# rows are of small whole numbers, of which every partial sum is exact, where they
+# can be. Each width goes through its kernel twice: with more rows than one round
+# of workgroups takes, and with outputs of 64 MB, which go past the caches.
+
+KINDS = 61  # of rows
+STREAM = 1 << 24  # floats of an output past the caches
+
+
+def drawn(seed, rows):
+    """Which of the kinds of rows each row is, every kind among them, and how many there are of each."""
+    which = seeded(seed).integers(0, KINDS, rows)
+    which[:KINDS] = np.arange(KINDS)[:rows]
+    return which, np.bincount(which, minlength=KINDS)
+
+
+def whole_numbers(seed, *shape):
+    return seeded(seed).integers(-2, 3, shape).astype(np.float32)
+
+
+def check_kinds(name, got, which, want, bound, alike=True):
+    """Rows against those of their kind; equal rows are alike, or else each is within the bound."""
+    if alike:
+        assert np.array_equal(got, got[:KINDS][which]), name
+        check(name, got[:KINDS], want, bound)
+    else:
+        check(name, got, want[which], bound[which])
+
+
+WIDTHS = [  # whole and broken vectors of every split of a row over lanes
+    8, 32, 3, 27, 64, 51, 128, 117, 256, 203, 512, 473, 1024, 1001, 2048, 1999, 4096, 4001, 8192, 8155, 16384, 16001, 32768, 32003,
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [1, 3, 4, 27, 64, 51, 128, 117, 256, 203, 1028])
+@pytest.mark.parametrize("kind", ["words", "padded", "one"])
+@pytest.mark.parametrize("many", [False, True])
+def test_embedding_and_its_gradient_are_exact(fg, hip, dim, kind, many):
+    tokens, vocab = STREAM // dim + 3 if many else 70001, 2999
+    r = seeded(320)
+    ids = some_ids("words" if kind == "padded" else kind, tokens, vocab, 321)
+    if kind == "padded":
+        ids[r.random(tokens) < 1 / 3] = 5
+        ids[r.random(tokens) < 0.1] = -1
+    w, table = whole_numbers(322, vocab, dim), whole_numbers(323, KINDS, dim)
+    which = r.integers(0, KINDS, tokens)
+    tw = new(fg, w, True)
+    y, dw = weighted(fg, tw.embedding(new(fg, ids), 0.5), table[which], [tw])
+    inside = ids >= 0
+    assert np.array_equal(y, np.where(inside[:, None], 0.5 * w[ids], 0.0))
+    # Of each id, how many tokens have each kind of gradient. All sums are below 2^24.
+    counts = np.bincount(ids[inside] * KINDS + which[inside], minlength=vocab * KINDS).reshape(vocab, KINDS)
+    assert np.array_equal(dw, 0.5 * (counts @ table.astype(np.float64)))
