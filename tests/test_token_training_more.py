@@ -173,3 +173,123 @@ def test_embedding_and_its_gradient_are_exact(fg, hip, dim, kind, many):
     # Of each id, how many tokens have each kind of gradient. All sums are below 2^24.
     counts = np.bincount(ids[inside] * KINDS + which[inside], minlength=vocab * KINDS).reshape(vocab, KINDS)
     assert np.array_equal(dw, 0.5 * (counts @ table.astype(np.float64)))
+
+
+def norm_splits(rows, dim):
+    """Rows that a lane sums the weights' gradients of, and the additions that its sums go through after it: the rows of
+    a workgroup, of a slice of the workgroups, and of the slices."""
+    lanes = next((l for l, k in ((8, 1), (16, 1), (32, 1), (64, 4), (256, 4), (512, 4), (1024, 4)) if 4 * l * k >= dim), None)
+    if lanes is None:
+        return -(-rows // min(rows, 32)), 6
+    threads = max(256, lanes)
+    groups = threads // lanes
+    blocks = min(-(-rows // groups), 4 * 256 * 256 // threads)
+    return -(-rows // (groups * blocks)), groups + -(-blocks // 32) + 5
+
+
+def norm_rows(rows, dim):
+    if rows == "many":
+        return STREAM // dim + 3
+    lanes = max(8, 1 << max(0, (dim - 1).bit_length() - 2)) if dim <= 256 else 64 if dim <= 1024 else 256
+    # More than two rounds of the gradient's workgroups, the last one not full.
+    return min(2 * 1024 * 256 // lanes + 77, STREAM // dim - 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", WIDTHS + [40001])
+@pytest.mark.parametrize("rows", ["some", "many"])
+def test_layer_norm_of_all_widths_over_many_rows(fg, hip, dim, rows):
+    n = norm_rows(rows, dim)
+    x, g, w = 2 + 3 * normal(330, KINDS, dim), whole_numbers(331, KINDS, dim), 1 + 0.1 * normal(332, dim)
+    b = 0.1 * normal(333, dim)
+    which, counts = drawn(334, n)
+    tx, tw, tb = new(fg, x[which], True), new(fg, w, True), new(fg, b, True)
+    y, dx, dw, db = weighted(fg, tx.layer_norm(tw, tb), g[which], [tx, tw, tb])
+    (wy, ey), (wx, ex), *_ = layer_norm64(x, w, b, g, 1e-5)
+    check_kinds("y", y, which, wy, ey)
+    check_kinds("dx", dx, which, wx, ex)
+    assert np.array_equal(db, counts @ g.astype(np.float64))  # below 2^24
+    # dw: each row's term with its bound, and the additions of a lane's rows and after them.
+    want, bound, size = np.zeros(dim), np.zeros(dim), np.zeros(dim)
+    for i in np.flatnonzero(counts):
+        _, _, (term, off), _ = layer_norm64(x[i:i + 1], w, b, g[i:i + 1], 1e-5)
+        want += counts[i] * term
+        bound += counts[i] * off
+        size += counts[i] * np.abs(term)
+    lane, after = norm_splits(n, dim)
+    check("dw", dw, want, bound + 1.01 * (lane + after) * U * size)
+    # Without a bias, and forward alone.
+    assert np.array_equal(tx.layer_norm(tw, tb).numpy(), y)
+    y, dx, dw2 = weighted(fg, tx.layer_norm(tw), g[which], [tx, tw])
+    (wy, ey), (wx, ex), *_ = layer_norm64(x, w, None, g, 1e-5)
+    check_kinds("y", y, which, wy, ey)
+    check_kinds("dx", dx, which, wx, ex)
+    assert np.array_equal(dw2, dw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 2, 31, 33, 67, 100])
+@pytest.mark.parametrize("dim", [20000, 40001])
+def test_layer_norm_weights_of_parts_of_the_rows(fg, hip, rows, dim):
+    # Rows in up to 32 parts of equal length, of which the last ones may have none.
+    g, x = whole_numbers(340, rows, dim), normal(341, rows, dim)
+    tx, tw, tb = new(fg, x, True), new(fg, 1 + 0.1 * normal(342, dim), True), new(fg, normal(343, dim), True)
+    y, dx, dw, db = weighted(fg, tx.layer_norm(tw, tb), g, [tx, tw, tb])
+    assert np.array_equal(db, g.astype(np.float64).sum(0))
+    for name, a, (want, bound) in zip(("y", "dx", "dw"), (y, dx, dw), layer_norm64(x, tw.numpy(), tb.numpy(), g, 1e-5)):
+        check(name, a, want, bound)
+
+
+LOSS_WIDTHS = WIDTHS + [65536, 65003, 70000, 70003]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("classes", LOSS_WIDTHS)
+@pytest.mark.parametrize("many", [False, True])
+def test_token_cross_entropy_of_all_widths_over_many_rows(fg, hip, classes, many):
+    # Short rows: more than a round of workgroups, of two rows each and more. Long ones are one a workgroup.
+    n = STREAM // classes + 3 if many else min(70001, STREAM // classes - 1)
+    r = seeded(350)
+    x, labels = 3 * normal(351, KINDS, classes), r.integers(0, classes, KINDS).astype(np.int32)
+    x[r.random(x.shape) < 0.1] = -np.inf
+    x[np.arange(KINDS), labels] = r.standard_normal(KINDS)
+    labels[r.random(KINDS) < 0.3] = -1
+    labels[7] = classes
+    which, counts = drawn(352, n)
+    total = counts[(labels >= 0) & (labels < classes)].sum()
+    tx, tl = new(fg, x[which], True), new(fg, labels[which])
+    loss = tx.token_cross_entropy(tl)
+    dx = loss.gradient([tx])[0]
+    fg.Tensor.realize_many([loss, dx])
+    want, bound = 0.0, 0.0
+    for i in np.flatnonzero(counts):
+        (each, off), _ = loss64(x[i:i + 1], labels[i:i + 1])
+        want, bound = want + counts[i] * each / total, bound + counts[i] * off / total
+    # The rows of a workgroup are rounded once, and the mean.
+    check("loss", loss.numpy(), want, bound + 2 * U * want)
+    valid = ((labels >= 0) & (labels < classes)).sum()
+    # Long rows of broken vectors are read from the cache line that they begin in: sums of equal rows that begin
+    # elsewhere in theirs are of other numbers, and as good.
+    alike = classes % 4 == 0 or classes <= 4096
+    check_kinds("dx", dx.numpy(), which, *loss64(x, labels, valid / total)[1], alike)
+    # Alone, and under a gradient that is not 1.
+    assert np.array_equal(tx.token_cross_entropy(tl).numpy(), loss.numpy())
+    scaled = tx.token_cross_entropy(tl).mul(new(fg, np.array([-2.5], np.float32))).gradient([tx])[0].numpy()
+    check_kinds("scaled", scaled, which, *loss64(x, labels, -2.5 * valid / total)[1], alike)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("count", [3, 20, 70])
+def test_clip_norm_of_more_than_the_caches_hold(fg, hip, count):
+    # Squares of whole numbers: the norm is rounded once. Products past the caches, squares of the first chunks too.
+    r = seeded(360)
+    pattern = whole_numbers(361, 1 << 20)
+    xs = [np.resize(np.roll(pattern, 1000 * i), 2 * STREAM // count + int(r.integers(9000))) for i in range(count)]
+    total = np.sqrt(sum(float((x.astype(np.float64) ** 2).sum()) for x in xs))
+    norm, clipped = fg.clip_norm([new(fg, x) for x in xs], 1.0)
+    fg.Tensor.realize_many([norm] + clipped)
+    check("norm", norm.numpy(), np.array([total]), 1.01 * U * total)
+    for x, y in zip(xs, clipped):
+        for value in range(-2, 3):  # a number's products are all the same
+            got = np.unique(y.numpy()[x == value])
+            assert len(got) == 1 and abs(float(got[0]) - value / total) <= 2.01 * U * abs(value / total)
