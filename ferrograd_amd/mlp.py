@@ -7,7 +7,7 @@ from typing import Callable, Sequence
 
 import numpy as np
 
-from . import I32, Dropout, FerrogradError, Linear, Sgd, Tensor
+from . import Dropout, FerrogradError, Linear, Sgd, Tensor
 
 
 def one_hot(labels: np.ndarray, num_classes: int) -> np.ndarray:
@@ -67,7 +67,8 @@ def train_step(model: Mlp, opt: Sgd, x: Tensor, targets: Tensor, preactivations:
     zs = model.forward_preactivations(x)
     if preactivations is not None:
         preactivations.extend(zs)
-    loss = (zs[-1].token_cross_entropy if targets.dtype == I32 else zs[-1].cross_entropy)(targets)
+    # Told apart by their shapes, which cost less to ask for than their types.
+    loss = (zs[-1].token_cross_entropy if len(targets.shape) == 1 else zs[-1].cross_entropy)(targets)
     opt.zero_grad()
     loss.backward()
     if max_norm is not None:

@@ -31,6 +31,30 @@ def test_tensors_are_given_by_position_or_by_name(fg, cpu):
                 bad(*args, **kw)
 
 
+def test_a_train_step_tells_labels_by_their_shape(fg, cpu):
+    # One number a row is a label. Rows of numbers are cross_entropy's targets, of whichever type, as before there were labels.
+    from ferrograd_amd.mlp import Mlp, train_step
+
+    x, rows = fg.Tensor.new(seeded(4).standard_normal((2, 3)).astype(np.float32), [2, 3], "cpu"), np.eye(4)[[1, 3]]
+    for targets in (rows.astype(np.float32), rows.astype(np.int32)):
+        t, got = fg.Tensor.new(targets, [2, 4], "cpu"), []
+        for step in (train_step, lambda m, opt, x, t: m.forward_preactivations(x)[-1].cross_entropy(t)):
+            fg.reset_init_seed(5)
+            model = Mlp((3, 4), cpu)
+            params = model.parameters()
+            opt = fg.Sgd(params, 0.1)
+            loss = step(model, opt, x, t)
+            if step is not train_step:
+                loss.backward()
+                opt.step()
+            got.append([loss.numpy()] + [p.numpy() for p in params])
+        assert all(np.array_equal(a, b) for a, b in zip(*got))
+    with pytest.raises(fg.FerrogradError, match=r"target shape \[2, 3\] must match logits shape \[2, 4\]"):
+        train_step(model, opt, x, fg.Tensor.new(np.zeros((2, 3), np.int32), [2, 3], "cpu"))
+    with pytest.raises(fg.FerrogradError, match="token_cross_entropy: the labels must be i32"):
+        train_step(model, opt, x, fg.Tensor.new(np.zeros(2, np.float32), [2], "cpu"))
+
+
 def while_it_runs(call, meanwhile):
     """Seconds that call() took, and how often another thread ran meanwhile, once a millisecond."""
     ticks, go, stop = [], threading.Event(), threading.Event()
