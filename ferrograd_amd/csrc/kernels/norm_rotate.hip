@@ -31,55 +31,11 @@
 // atomics.
 #include <hip/hip_runtime.h>
 
+#include "vectors.hpp"
+
 namespace {
 
 constexpr int kThreads = 256;
-
-template <int VEC>
-struct Vec {
-  float v[VEC];
-};
-
-// A vector of a row, which starts on any float.
-template <int VEC>
-struct Unaligned {
-  typedef float type __attribute__((ext_vector_type(VEC), aligned(4)));
-};
-template <>
-struct Unaligned<1> {
-  typedef float type;
-};
-template <int VEC>
-__device__ inline float element(const typename Unaligned<VEC>::type& v, int e) {
-  if constexpr (VEC == 1) return v;
-  else return v[e];
-}
-
-// `Stream`: past the caches, for what is read once and outputs that would not
-// stay in the Infinity Cache.
-template <int VEC, bool Stream = false>
-__device__ inline Vec<VEC> load(const float* p) {
-  typedef typename Unaligned<VEC>::type vec;
-  const vec v = Stream ? __builtin_nontemporal_load(reinterpret_cast<const vec*>(p)) : *reinterpret_cast<const vec*>(p);
-  Vec<VEC> r;
-#pragma unroll
-  for (int e = 0; e < VEC; e++) r.v[e] = element<VEC>(v, e);
-  return r;
-}
-
-template <int VEC, bool Stream>
-__device__ inline void store(float* p, const Vec<VEC>& r) {
-  typedef typename Unaligned<VEC>::type vec;
-  vec v;
-  if constexpr (VEC == 1) {
-    v = r.v[0];
-  } else {
-#pragma unroll
-    for (int e = 0; e < VEC; e++) v[e] = r.v[e];
-  }
-  if (Stream) __builtin_nontemporal_store(v, reinterpret_cast<vec*>(p));
-  else *reinterpret_cast<vec*>(p) = v;
-}
 
 template <int G>
 __device__ inline float group_sum(float x) {
