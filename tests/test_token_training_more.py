@@ -7,7 +7,7 @@ import time
 import numpy as np
 import pytest
 
-from conftest import seeded
+from conftest import graphs_on, seeded
 from test_token_training import U, check, layer_norm64, loss64, new, normal, some_ids, weighted
 
 
@@ -317,3 +317,73 @@ def test_clip_norm_of_more_than_the_caches_hold(fg, hip, count):
         for value in range(-2, 3):  # a number's products are all the same
             got = np.unique(y.numpy()[x == value])
             assert len(got) == 1 and abs(float(got[0]) - value / total) <= 2.01 * U * abs(value / total)
+
+
+# ── calls together (GPU) ────────────────────────────────────────────────────
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("graphs", [False, True])
+def test_replayed_steps_read_the_batches_that_they_narrow_to(fg, hip, graphs):
+    # The batch's start changes from step to step, under one plan: ids, labels and rows added to them.
+    rows, batch, vocab, dim = 96, 16, 19, 12
+    r = seeded(370)
+    ids, labels = (r.integers(-1, vocab, rows).astype(np.int32) for _ in range(2))
+    more, w, n = normal(371, rows, dim), normal(372, vocab, dim), normal(373, dim)
+    tids, tlabels, tmore, tw, tn = new(fg, ids), new(fg, labels), new(fg, more), new(fg, w, True), new(fg, n, True)
+
+    def step(ids, labels, more):
+        x = tw.embedding(ids, 2.0).add(more).layer_norm(tn)
+        loss = x.matmul(tw.permute([1, 0])).token_cross_entropy(labels)
+        norm, clipped = fg.clip_norm(loss.gradient([tw, tn]), 0.01)
+        outs = [loss, norm] + clipped
+        fg.Tensor.realize_many(outs)
+        new(fg, normal(60, 1000)).exp().numpy()  # other work in between
+        return [t.numpy() for t in outs]
+
+    starts = [0, 5, 16, 80, 5, 33, 79, 0]
+    fresh = [step(*(new(fg, a[s:s + batch]) for a in (ids, labels, more))) for s in starts]
+    with graphs_on(fg, 2 if graphs else 0):
+        fg.clear_caches()
+        for s, want in list(zip(starts, fresh)) * 2:
+            got = step(*(t.narrow(0, s, batch) for t in (tids, tlabels, tmore)))
+            assert all(np.array_equal(a, b) for a, b in zip(got, want)), s
+
+
+@pytest.mark.gpu
+def test_losses_of_the_same_logits_add_up(fg, hip):
+    # Two labels a row, and the same ones twice: each loss is made beside its gradient.
+    x, l0, l1 = 3 * normal(380, 33, 50), *(seeded(381 + i).integers(-1, 50, 33).astype(np.int32) for i in range(2))
+    tx = new(fg, x, True)
+    losses = [tx.token_cross_entropy(new(fg, l)) for l in (l0, l1, l0)]
+    total = losses[0].add(losses[1]).add(losses[2])
+    dx = total.gradient([tx])[0]
+    fg.Tensor.realize_many([total, dx])
+    ((a, ea), (da, eda)), ((b, eb), (db, edb)) = loss64(x, l0), loss64(x, l1)
+    check("total", total.numpy(), 2 * a + b, 2 * ea + eb + 3 * U * (2 * a + b))
+    check("dx", dx.numpy(), 2 * da + db, 2 * eda + edb + 3 * U * (2 * np.abs(da) + np.abs(db)))
+    check("loss", losses[1].numpy(), b, eb)
+
+
+@pytest.mark.gpu
+def test_micro_batches_add_up_before_they_are_clipped(fg, hip):
+    w, g = normal(390, 11, 8), normal(391, 2, 20, 8)
+    ids = seeded(392).integers(0, 11, (2, 20)).astype(np.int32)
+    tw = new(fg, w, True)
+    opt = fg.Sgd([tw], 0.25)
+    for i in range(2):
+        tw.embedding(new(fg, ids[i])).mul(new(fg, g[i])).sum([0, 1]).backward()
+    norm = opt.clip_grad_norm(0.5)
+    opt.step()
+    dw, size = np.zeros(w.shape), np.zeros(w.shape)
+    for i in range(2):
+        np.add.at(dw, ids[i], g[i])
+        np.add.at(size, ids[i], np.abs(g[i]))
+    total = np.sqrt((dw ** 2).sum())
+    # Sums of at most 20 rows in each half, and their sum; the norm and the products by roundings of these.
+    off = 21 * U * size
+    part = np.sqrt((off ** 2).sum())
+    check("norm", norm.numpy(), np.array([total]), part + U * total)
+    want = w - 0.25 * dw * (0.5 / total)
+    check("step", tw.numpy(), want, 0.25 * (0.5 / total) * (off + np.abs(dw) * (part / total + 4 * U)) + U * np.abs(want))
+    assert total > 0.5
