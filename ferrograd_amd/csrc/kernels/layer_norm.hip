@@ -12,11 +12,18 @@
 // second read. L is a part of a wave for short rows, a workgroup for long ones.
 // dw and db are summed in registers over all rows that a lane sees, then over the
 // workgroup, then over the workgroups by a second launch: a fixed order, no
-// atomics. Registers do not hold these sums of more than 16384 columns: x and g
-// are then read again for them. Rows of more than 32768 columns are read again for
-// each of their sums.
+// atomics, and in float32: a lane's rows are all rows over those that the
+// workgroups have at a time (from 32768 of 32 columns to 256 of 16384). Registers
+// do not hold these sums of more than 16384 columns: x and g are then read again
+// for them, in up to 32 parts of the rows. Rows of more than 32768 columns are read
+// again for each of their sums.
 //
-// 16384 rows of 4096: forward 98 us (5.4 TB/s), backward 126 (6.4); of 4095, whose
+// Rows on 1024 lanes leave a little in scratch memory: 24 bytes a lane backward in
+// 4 vectors, 8 in 8, and 36 to 72 forward in 8, where row, weight and bias are 96
+// registers of 128.
+//
+// TB/s of what each must read and write. 16384 rows of 4096: forward 98 us (5.5),
+// backward 126 (6.4; 6.6 of all that goes past the L2 caches); of 4095, whose
 // vectors are unaligned, 102 and 136. 65536 of 1024: 92 and 120 (5.8 and 6.7); of
 // 1023, 101 and 132. 3000 of 20000: 138 (199 with weight and bias read for each
 // row), and backward 133 + 90, where reading each row for each sum took 186, and
@@ -33,8 +40,9 @@ namespace {
 // lane does not own, and what it does not own it writes as the same value again.
 // So each vector is one load and one store (with the last one's elements one by
 // one, for which the wave waits, 16384 rows of 4095 took 150 us backward, not 136,
-// 131072 of 33 18.4, not 16.1, and 4096 of 16383, which lacks the registers for
-// what is moved, 189, not 195). Rows of less than a vector have no other way.
+// 131072 of 33 18.4, not 16.1, but 4096 of 16383, which lacks the registers for
+// what is moved, 189, not 195: 3% that a second form of the two widest splits
+// would save). Rows of less than a vector have no other way.
 template <int L, int K, bool Whole>
 struct Moved {
   int lane, dim;

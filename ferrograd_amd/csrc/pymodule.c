@@ -312,8 +312,8 @@ PyDoc_STRVAR(embedding_doc,
 "embedding(ids, scale=1.0)\n--\n\n"
 "Rows of this weight [vocab, dim] (f32) by id, times scale: [tokens, dim] of ids\n"
 "(an int32 tensor [tokens]). An id outside of [0, vocab) is no token: a row of\n"
-"zeros, and no gradient. The weight's gradient sums its tokens' rows in their\n"
-"order, the same in every run.");
+"zeros, and no gradient. The weight's gradient sums its tokens' rows in an order\n"
+"fixed by the ids and the sizes: the same in every run.");
 
 static PyObject* t_embedding(TensorObject* self, PyObject* args, PyObject* kw) {
   static char* names[] = {"ids", "scale", NULL};

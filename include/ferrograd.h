@@ -89,9 +89,9 @@ int fg_tensor_dropout(fg_tensor* t, double p, uint64_t seed, uint64_t offset, fg
 
 /* Rows of weight [vocab, dim] (f32) by id, times scale: [tokens, dim] of ids
  * (i32 [tokens]). An id outside of [0, vocab) is no token: it gives a row of
- * zeros and has no gradient. The weight's gradient sums its tokens' rows in
- * their order, without atomics: the same in every run. HIP device only. No
- * reference counterpart. */
+ * zeros and has no gradient. The weight's gradient sums its tokens' rows in an
+ * order fixed by the ids and the sizes, without atomics: the same in every run.
+ * HIP device only. No reference counterpart. */
 int fg_tensor_embedding(fg_tensor* weight, fg_tensor* ids, double scale, fg_tensor** out);
 
 /* Layer norm of each row of x [rows, dim] (f32): (x - mean(x)) *
@@ -117,7 +117,8 @@ int fg_tensor_token_cross_entropy(fg_tensor* logits, fg_tensor* labels, fg_tenso
 int fg_global_norm(fg_tensor* const* ts, int n, fg_tensor** out);
 /* That norm, and every tensor times max_norm / max(norm, max_norm) (max_norm
  * finite and above 0) into outs[0, n). A norm of NaN makes them NaN, one of
- * infinity 0 (NaN where a tensor is infinite). */
+ * infinite elements 0 (NaN where a tensor is infinite); one of finite elements that
+ * is past float32's range is infinity in *norm, and clips as the f64 that it is. */
 int fg_clip_norm(fg_tensor* const* ts, int n, double max_norm, fg_tensor** norm, fg_tensor** outs);
 
 /* In-place graph updates (tensor.rs:399-440). */

@@ -55,6 +55,15 @@ def test_a_train_step_tells_labels_by_their_shape(fg, cpu):
         train_step(model, opt, x, fg.Tensor.new(np.zeros(2, np.float32), [2], "cpu"))
 
 
+def test_layer_norm_gradients_of_too_many_columns_are_refused(fg):
+    # Forward it is planned; the launch that adds up the weight's gradient would have 2^32 threads.
+    x, w = fg.Tensor.zeros([1, 1 << 26], "hip"), fg.Tensor.zeros([1 << 26], "hip").with_requires_grad(True)
+    y = x.layer_norm(w)
+    fg.debug_plan([y], fuse=True, render_hip=True)
+    with pytest.raises(fg.FerrogradError, match=r"layer_norm: .* in one launch, which takes 2\^32 - 1 threads"):
+        fg.debug_plan(y.sum([0, 1]).gradient([w]), fuse=True, render_hip=True)
+
+
 def while_it_runs(call, meanwhile):
     """Seconds that call() took, and how often another thread ran meanwhile, once a millisecond."""
     ticks, go, stop = [], threading.Event(), threading.Event()
@@ -300,6 +309,18 @@ def test_token_cross_entropy_of_all_widths_over_many_rows(fg, hip, classes, many
     assert np.array_equal(tx.token_cross_entropy(tl).numpy(), loss.numpy())
     scaled = tx.token_cross_entropy(tl).mul(new(fg, np.array([-2.5], np.float32))).gradient([tx])[0].numpy()
     check_kinds("scaled", scaled, which, *loss64(x, labels, -2.5 * valid / total)[1], alike)
+
+
+@pytest.mark.gpu
+def test_a_norm_past_the_range_clips_as_itself(fg, hip):
+    x = np.where(normal(305, 5001) > 0, 3e38, -2e38).astype(np.float32)
+    total = np.sqrt((x.astype(np.float64) ** 2).sum())  # 2e40
+    for max_norm in (1.0, 1e39):
+        norm, (y,) = fg.clip_norm([new(fg, x)], max_norm)
+        fg.Tensor.realize_many([norm, y])
+        assert norm.numpy()[0] == np.inf
+        want = x.astype(np.float64) * (max_norm / total)
+        check("clipped", y.numpy(), want, 2.01 * U * np.abs(want))
 
 
 @pytest.mark.gpu
