@@ -3,6 +3,7 @@
 
 #include <cstdlib>
 #include <cstring>
+#include <mutex>
 #include <sstream>
 #include <string>
 
@@ -26,8 +27,18 @@ namespace {
 
 thread_local std::string g_err;
 
+// One call at a time: graph nodes, the table of live tensors and the plans are
+// shared, and a thread that lets go of Python's interpreter lock for a call may
+// meet another one that frees a tensor, as collecting garbage does in any thread.
+// Never destroyed: calls may come while the process ends.
+std::recursive_mutex& one_call() {
+  static auto* m = new std::recursive_mutex;
+  return *m;
+}
+
 template <class F>
 int guard(F&& f) {
+  const std::lock_guard<std::recursive_mutex> lock(one_call());
   try {
     f();
     return 0;
@@ -133,8 +144,7 @@ int fg_idx_labels(const char* path, uint8_t* out, size_t capacity, size_t* count
 }
 
 int fg_tensor_free(fg_tensor* t) {
-  delete t;
-  return 0;
+  return guard([&] { delete t; });
 }
 
 int fg_tensor_unary(fg_tensor* t, int op, fg_tensor** out) {
@@ -352,8 +362,7 @@ int fg_tensor_gradient(fg_tensor* loss, fg_tensor** targets, int n, fg_tensor** 
 }
 
 int fg_reset_init_seed(uint64_t seed) {
-  fg::reset_init_seed(seed);
-  return 0;
+  return guard([&] { fg::reset_init_seed(seed); });
 }
 
 int fg_linear_new(int device, int64_t in, int64_t outf, int bias, fg_linear** out) {
@@ -411,8 +420,7 @@ int fg_linear_param(fg_linear* l, int i, fg_tensor** out) {
 }
 
 int fg_linear_free(fg_linear* l) {
-  delete l;
-  return 0;
+  return guard([&] { delete l; });
 }
 
 int fg_sgd_new(fg_tensor** params, int n, float lr, fg_sgd** out) {
@@ -436,8 +444,7 @@ int fg_sgd_step(fg_sgd* s) {
 }
 
 int fg_sgd_free(fg_sgd* s) {
-  delete s;
-  return 0;
+  return guard([&] { delete s; });
 }
 
 int fg_synchronize(int device) {

@@ -13,7 +13,8 @@
  *
  * realize_many and gradient let other Python threads run meanwhile, as the
  * calls through ctypes do: they compile kernels, wait for devices and walk
- * whole graphs. The library itself is used by one thread at a time. */
+ * whole graphs. Tensors that another thread drops then, by collecting garbage for
+ * one, wait for the call's end: the library takes one call at a time. */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <limits.h>

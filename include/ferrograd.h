@@ -9,7 +9,9 @@
  * Every function returns 0 on success, nonzero on error; the message is in
  * fg_last_error(). Handles are owned by the caller and released with the
  * matching *_free. A tensor handle aliases shared tensor state, like a cloned
- * reference Tensor (tensor.rs:30-38).
+ * reference Tensor (tensor.rs:30-38). Calls from several threads follow one
+ * another, so that one may free tensors while another realises; a device's work is
+ * for one thread (ferrograd_hip.h).
  */
 #ifndef FERROGRAD_H
 #define FERROGRAD_H

@@ -1,6 +1,9 @@
 """Embedding, layer norm, the loss of token labels and clipping, further: how
 Python reaches them, and each of their kernels against float64."""
 import inspect
+import os
+import subprocess
+import sys
 import threading
 import time
 
@@ -109,6 +112,48 @@ def test_other_threads_run_while_the_library_works(fg, cpu, kind):
         if seconds > 0.08:
             break
     assert seconds > 0.08 and ticks >= 3, (seconds, ticks)
+
+
+BESIDE = """
+import sys, threading
+sys.path.insert(0, sys.argv[1])
+import numpy as np
+import ferrograd_amd as fg, oracle
+oracle.load()
+stop = threading.Event()
+
+def beside():
+    while not stop.is_set():
+        ts = [fg.Tensor.new(np.ones(64, np.float32), [64], "cpu") for _ in range(20)]
+        y = ts[0]
+        for t in ts:
+            y = y.add(t)
+        del ts, y, t
+
+thread = threading.Thread(target=beside)
+thread.start()
+try:
+    a = fg.Tensor.new(np.arange(64, dtype=np.float32) / 64, [64], "cpu").with_requires_grad(True)
+    for i in range(200):
+        y = a
+        for _ in range(30):
+            y = y.mul(a).add(a)
+        z = a.mul(a).add(a)
+        g = y.sum([0]).gradient([a])[0]
+        fg.Tensor.realize_many([z])
+        assert np.array_equal(z.numpy(), a.numpy() * a.numpy() + a.numpy())
+finally:
+    stop.set()
+    thread.join()
+print("done")
+"""
+
+
+def test_tensors_are_made_and_dropped_while_the_library_works(fg, cpu):
+    # What collecting garbage does in any thread: a program of its own, which a race would end.
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    p = subprocess.run([sys.executable, "-c", BESIDE, root], capture_output=True, text=True, timeout=120)
+    assert p.returncode == 0 and p.stdout.strip() == "done", (p.returncode, p.stderr[-2000:])
 
 
 # ── embedding (GPU) ─────────────────────────────────────────────────────────
